@@ -23,7 +23,7 @@ from . import _abi
 __all__ = [
     "PcuExecutionFaultKind", "TensorArithmeticStep", "PcuFloatUnderflowPolicy",
     "PcuExecutionFault", "CompoundFault", "PcuExecutionError", "Context", "DeviceArray",
-    "lib", "library_path",
+    "lib", "library_path", "bfloat16", "to_bfloat16", "from_bfloat16",
 ]
 
 
@@ -108,6 +108,39 @@ def dtype_code(dtype) -> int:
         return _NP_DTYPE[np.dtype(dtype)]
     except KeyError:
         raise PcuExecutionError(_abi.PCU_ERR_UNSUPPORTED, f"unsupported scalar type {dtype}")
+
+
+# numpy has no bfloat16: arrays of this type hold the upper halves of binary32 bit patterns.
+bfloat16 = np.dtype([("bfloat16", np.uint16)])
+
+
+def to_bfloat16(x) -> np.ndarray:
+    """binary32 values rounded to nearest even (a NaN stays a NaN)."""
+    x = np.ascontiguousarray(x, dtype=np.float32)
+    b = x.view(np.uint32)
+    r = ((b.astype(np.uint64) + 0x7FFF + ((b >> 16) & 1)) >> 16).astype(np.uint16)
+    r = np.where(np.isnan(x), ((b >> 16) | 0x40).astype(np.uint16), r)
+    return np.ascontiguousarray(r).view(bfloat16).reshape(x.shape)
+
+
+def from_bfloat16(x: np.ndarray) -> np.ndarray:
+    return (np.ascontiguousarray(x).view(np.uint16).astype(np.uint32) << 16).view(np.float32).reshape(x.shape)
+
+
+_LOGIT_DTYPE = {np.dtype(np.float32): _abi.PCU_F32, np.dtype(np.float64): _abi.PCU_F64,
+                bfloat16: _abi.PCU_BF16, np.dtype(np.float16): _abi.PCU_F16}
+
+
+def _logit_code(what: str, dtype) -> int:
+    try:
+        return _LOGIT_DTYPE[dtype]
+    except KeyError:
+        raise PcuExecutionError(_abi.PCU_ERR_UNSUPPORTED, f"{what}: unsupported scalar type {dtype}")
+
+
+def _stat_dtype(dtype) -> np.dtype:
+    """The type of a row's statistics: binary32, binary64 for binary64 rows."""
+    return np.dtype(np.float64 if dtype == np.float64 else np.float32)
 
 
 def _require(what: str, x: "DeviceArray", shape, dtype) -> None:
@@ -433,3 +466,142 @@ class Context:
                                             float(np.float32(learning_rate)), int(contracted),
                                             out.ptr))
         return out
+
+    # ------------------------------------------------------ operators on logits
+    # Logits are a [rows, columns] array of float32, float64, float16 or ``bfloat16``; ``vocab``
+    # (default: all columns) names how many leading columns are real where the rest is
+    # padding. Results that are not passed in are allocated.
+    def _logits(self, what: str, x: DeviceArray, vocab: Optional[int]) -> _abi.Logits:
+        code = _logit_code(what, x.dtype)
+        if len(x.shape) != 2 or (vocab is not None and not 0 <= vocab <= x.shape[1]):
+            raise PcuExecutionError(_abi.PCU_ERR_SHAPE, f"{what}: {x.shape} with vocab {vocab}")
+        return _abi.Logits(x.ptr, code, 0, x.shape[0], x.shape[1] if vocab is None else vocab, x.shape[1])
+
+    def _out(self, what: str, x: Optional[DeviceArray], shape, dtype) -> DeviceArray:
+        if x is None:
+            return self.empty(shape, dtype)
+        _require(what, x, shape, dtype)
+        return x
+
+    def native_top_logits(self, logits: DeviceArray, k: int, temperature: float = 1.0,
+                          vocab: Optional[int] = None, values: Optional[DeviceArray] = None,
+                          indices: Optional[DeviceArray] = None,
+                          log_sum: Optional[DeviceArray] = None):
+        """The k largest logits of each row by (value descending, index ascending), their int32
+        indices, and the row's log(sum exp(l / temperature)): ``(values, indices, log_sum)``,
+        a teacher's side of the distillation below (pcu_native_top_logits)."""
+        lg = self._logits("top_logits", logits, vocab)
+        k = int(k)
+        if not 0 <= k <= _abi.LOGITS_MAX_K:
+            raise PcuExecutionError(_abi.PCU_ERR_SHAPE, f"top_logits: k {k} is not in [0, {_abi.LOGITS_MAX_K}]")
+        rows = logits.shape[0]
+        values = self._out("values", values, (rows, k), logits.dtype)
+        indices = self._out("indices", indices, (rows, k), np.int32)
+        log_sum = self._out("log_sum", log_sum, (rows,), _stat_dtype(logits.dtype))
+        self.check(self._lib.pcu_native_top_logits(self.handle, ctypes.byref(lg), k, temperature, values.ptr,
+                                                   indices.ptr, log_sum.ptr))
+        return values, indices, log_sum
+
+    def _distill(self, student: DeviceArray, teacher_values: DeviceArray, teacher_indices: DeviceArray,
+                 teacher_log_sum, labels, temperature: float, distill_weight: float, label_weight: float,
+                 vocab: Optional[int]):
+        lg = self._logits("distill", student, vocab)
+        rows = student.shape[0]
+        if len(teacher_values.shape) != 2:
+            raise PcuExecutionError(_abi.PCU_ERR_SHAPE, f"distill: teacher values are {teacher_values.shape}")
+        k = teacher_values.shape[1]
+        if k > _abi.LOGITS_MAX_K:
+            raise PcuExecutionError(_abi.PCU_ERR_SHAPE, f"distill: {k} entries a row are beyond {_abi.LOGITS_MAX_K}")
+        code = _logit_code("teacher values", teacher_values.dtype)
+        _require("teacher values", teacher_values, (rows, k), teacher_values.dtype)
+        _require("teacher indices", teacher_indices, (rows, k), np.int32)
+        if teacher_log_sum is not None:
+            _require("teacher log-sum", teacher_log_sum, (rows,), _stat_dtype(teacher_values.dtype))
+        if labels is not None:
+            _require("labels", labels, (rows,), np.int32)
+        return lg, _abi.Distill(teacher_values.ptr, teacher_indices.ptr,
+                                teacher_log_sum.ptr if teacher_log_sum is not None else None,
+                                labels.ptr if labels is not None else None, code, k, temperature,
+                                distill_weight, label_weight)
+
+    def native_distill_loss(self, student: DeviceArray, teacher_values: DeviceArray,
+                            teacher_indices: DeviceArray, teacher_log_sum: Optional[DeviceArray] = None,
+                            labels: Optional[DeviceArray] = None, temperature: float = 1.0,
+                            distill_weight: float = 1.0, label_weight: float = 0.0,
+                            vocab: Optional[int] = None, loss: Optional[DeviceArray] = None,
+                            log_sums: Optional[DeviceArray] = None):
+        """Each row's distillation loss against a teacher's top logits (entries with a negative
+        index are absent), plus ``label_weight`` times the cross entropy of its label (negative:
+        none); without ``teacher_log_sum`` the teacher's probabilities are normalised over the
+        row's entries. Returns ``(loss [rows], log_sums [rows, 2])``; see pcu_distill for the
+        formulas."""
+        lg, d = self._distill(student, teacher_values, teacher_indices, teacher_log_sum, labels, temperature,
+                              distill_weight, label_weight, vocab)
+        rows, stat = student.shape[0], _stat_dtype(student.dtype)
+        loss = self._out("loss", loss, (rows,), stat)
+        log_sums = self._out("log_sums", log_sums, (rows, 2), stat)
+        self._call(self._lib.pcu_native_distill_loss, ctypes.byref(lg), ctypes.byref(d), loss.ptr, log_sums.ptr)
+        return loss, log_sums
+
+    def native_distill_backward(self, student: DeviceArray, teacher_values: DeviceArray,
+                                teacher_indices: DeviceArray, log_sums: DeviceArray,
+                                teacher_log_sum: Optional[DeviceArray] = None,
+                                labels: Optional[DeviceArray] = None, temperature: float = 1.0,
+                                distill_weight: float = 1.0, label_weight: float = 0.0,
+                                vocab: Optional[int] = None, row_scale: Optional[DeviceArray] = None,
+                                gradient: Optional[DeviceArray] = None) -> DeviceArray:
+        """The loss's gradient by the student's logits, each row times its ``row_scale``, from
+        native_distill_loss's ``log_sums``: an array like ``student`` (padding columns are 0),
+        which may be ``student`` itself."""
+        lg, d = self._distill(student, teacher_values, teacher_indices, teacher_log_sum, labels, temperature,
+                              distill_weight, label_weight, vocab)
+        (rows, cols), stat = student.shape, _stat_dtype(student.dtype)
+        _require("log_sums", log_sums, (rows, 2), stat)
+        if row_scale is not None:
+            _require("row_scale", row_scale, (rows,), stat)
+        gradient = self._out("gradient", gradient, student.shape, student.dtype)
+        self._call(self._lib.pcu_native_distill_backward, ctypes.byref(lg), ctypes.byref(d), log_sums.ptr,
+                   row_scale.ptr if row_scale is not None else None, gradient.ptr, cols, cols)
+        return gradient
+
+    def native_distill_step(self, student: DeviceArray, teacher_values: DeviceArray,
+                            teacher_indices: DeviceArray, teacher_log_sum: Optional[DeviceArray] = None,
+                            labels: Optional[DeviceArray] = None, temperature: float = 1.0,
+                            distill_weight: float = 1.0, label_weight: float = 0.0,
+                            vocab: Optional[int] = None, row_scale: Optional[DeviceArray] = None,
+                            loss: Optional[DeviceArray] = None, gradient: Optional[DeviceArray] = None):
+        """native_distill_loss and native_distill_backward in one call, which reads the logits once
+        where it can: ``(loss [rows], gradient)``."""
+        lg, d = self._distill(student, teacher_values, teacher_indices, teacher_log_sum, labels, temperature,
+                              distill_weight, label_weight, vocab)
+        (rows, cols), stat = student.shape, _stat_dtype(student.dtype)
+        if row_scale is not None:
+            _require("row_scale", row_scale, (rows,), stat)
+        loss = self._out("loss", loss, (rows,), stat)
+        gradient = self._out("gradient", gradient, student.shape, student.dtype)
+        self._call(self._lib.pcu_native_distill_step, ctypes.byref(lg), ctypes.byref(d),
+                   row_scale.ptr if row_scale is not None else None, loss.ptr, gradient.ptr, cols, cols)
+        return loss, gradient
+
+    def native_sample(self, logits: DeviceArray, uniform: DeviceArray, temperature=1.0, top_k=0, top_p=1.0,
+                      min_p=0.0, vocab: Optional[int] = None, tokens: Optional[DeviceArray] = None,
+                      log_prob: Optional[DeviceArray] = None):
+        """One token a row from the row's uniform random number in [0, 1): ``(tokens int32,
+        log_prob float32)``. A setting is a number for all rows or an array [rows] (float32,
+        ``top_k`` int32); ``temperature`` 0 takes the largest logit, ``top_k`` <= 0 sets no
+        limit. The token depends on nothing but the row, its settings and its random number
+        (see pcu_native_sample)."""
+        lg = self._logits("sample", logits, vocab)
+        rows = logits.shape[0]
+        _require("uniform", uniform, (rows,), np.float32)
+        p = _abi.Sampling(uniform=uniform.ptr)
+        for name, x in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
+            if isinstance(x, DeviceArray):
+                _require(name, x, (rows,), np.int32 if name == "top_k" else np.float32)
+                setattr(p, name, x.ptr)
+            else:
+                setattr(p, name + "_value", x)
+        tokens = self._out("tokens", tokens, (rows,), np.int32)
+        log_prob = self._out("log_prob", log_prob, (rows,), np.float32)
+        self._call(self._lib.pcu_native_sample, ctypes.byref(lg), ctypes.byref(p), tokens.ptr, log_prob.ptr)
+        return tokens, log_prob

@@ -28,7 +28,8 @@ STATUS_NAMES = {
     7: "PCU_ERR_STATE", 8: "PCU_ERR_PROTOCOL",
 }
 
-PCU_F32, PCU_F64 = 0, 1
+PCU_F32, PCU_F64, PCU_BF16, PCU_F16 = 0, 1, 2, 3
+LOGITS_MAX_VOCAB, LOGITS_MAX_K = 1 << 22, 1024
 UNDERFLOW_IEEE, UNDERFLOW_REJECT_SUBNORMAL, UNDERFLOW_ALLOW_GRADUAL = 0, 1, 2
 OP_ADD, OP_SUB, OP_MUL, OP_DIV = 0, 1, 2, 3
 
@@ -117,6 +118,58 @@ class NodeDesc(ctypes.Structure):
     ]
 
 
+class Logits(ctypes.Structure):
+    """pcu_logits."""
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("dtype", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+        ("rows", ctypes.c_uint64),
+        ("vocab", ctypes.c_uint64),
+        ("stride", ctypes.c_uint64),
+    ]
+
+
+class Distill(ctypes.Structure):
+    """pcu_distill."""
+    _fields_ = [
+        ("teacher_values", ctypes.c_void_p),
+        ("teacher_indices", ctypes.c_void_p),
+        ("teacher_log_sum", ctypes.c_void_p),
+        ("labels", ctypes.c_void_p),
+        ("teacher_dtype", ctypes.c_uint32),
+        ("k", ctypes.c_uint32),
+        ("temperature", ctypes.c_double),
+        ("distill_weight", ctypes.c_double),
+        ("label_weight", ctypes.c_double),
+    ]
+
+
+class Sampling(ctypes.Structure):
+    """pcu_sampling."""
+    _fields_ = [
+        ("uniform", ctypes.c_void_p),
+        ("temperature", ctypes.c_void_p),
+        ("top_k", ctypes.c_void_p),
+        ("top_p", ctypes.c_void_p),
+        ("min_p", ctypes.c_void_p),
+        ("temperature_value", ctypes.c_float),
+        ("top_k_value", ctypes.c_int32),
+        ("top_p_value", ctypes.c_float),
+        ("min_p_value", ctypes.c_float),
+    ]
+
+
+_LP = ctypes.POINTER(Logits)
+_DP = ctypes.POINTER(Distill)
+SIGNATURES.update({
+    "pcu_native_top_logits": (_i32, [_vp, _LP, _u32, ctypes.c_double, _vp, _vp, _vp]),
+    "pcu_native_distill_loss": (_i32, [_vp, _LP, _DP, _vp, _vp, _FP]),
+    "pcu_native_distill_backward": (_i32, [_vp, _LP, _DP, _vp, _vp, _vp, _u64, _u64, _FP]),
+    "pcu_native_distill_step": (_i32, [_vp, _LP, _DP, _vp, _vp, _vp, _u64, _u64, _FP]),
+    "pcu_native_sample": (_i32, [_vp, _LP, ctypes.POINTER(Sampling), _vp, _vp, _FP]),
+})
+
 _U32P = ctypes.POINTER(ctypes.c_uint32)
 _U64P = ctypes.POINTER(ctypes.c_uint64)
 SIGNATURES.update({
@@ -157,6 +210,7 @@ KERNEL_IDS = {
     "strict_gemm": 0, "gemm_prefilter": 1, "gemm_replay": 2, "sgd": 3, "binary": 4,
     "relu": 5, "relu_backward": 6, "add_relu": 7, "mse": 8,
     "native_gemm": 9, "native_sgd": 10, "native_mse": 11, "elementwise_chain": 12,
+    "top_logits": 13, "distill": 14, "sample": 15,
 }
 
 _lib = None

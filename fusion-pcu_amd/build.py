@@ -38,7 +38,8 @@ COMMON = [
 ]
 
 SOURCES = ["elementwise.hip", "matmul.hip", "matmul_mfma.hip", "matmul_mid.hip", "matmul_small.hip",
-           "matmul_native.hip", "matmul_valu.hip", "matmul_f64.hip", "runtime.cpp", "graph.cpp"]
+           "matmul_native.hip", "matmul_valu.hip", "matmul_f64.hip", "logits_top.hip", "logits_distill.hip",
+           "logits_sample.hip", "logits.cpp", "runtime.cpp", "graph.cpp"]
 
 
 def _compile(src: str) -> str:

@@ -1,0 +1,568 @@
+// Distillation from a teacher's top logits, forward and backward.
+//
+// Row of V student logits s, k teacher entries (v_j, i_j), temperature T, weights a and b:
+//   q_j  = exp(v_j / T - L), L the teacher's log-sum-exp of the whole row if it is given, else
+//          that of the row's own entries;   Q = sum q_j
+//   p    = softmax(s / T), p1 = softmax(s)
+//   loss = a T^2 sum_j q_j (log q_j - log p[i_j])  +  b (-log p1[y])
+//   ds_v = scale (a T (Q p_v - sum over i_j = v of q_j)  +  b (p1_v - [v = y]))
+// The b terms are there only for rows with a label y >= 0; entries with a negative index are
+// absent. A row without entries and label has loss 0 and gradient 0 whatever it holds.
+//
+// The gradient is dense (Q p_v everywhere) with at most k + 1 places that differ: each
+// workgroup writes its dense part, and after a barrier overwrites those places with the full
+// value, computed anew by the lane that owns the place's first entry, so that no atomics and no
+// order are involved and duplicate indices add up.
+#include "pcu_kernels.hpp"
+#include "pcu_logits.hpp"
+
+#pragma clang fp contract(off)
+
+namespace pcu {
+
+namespace {
+
+// exp(s / T - L) from a given log-sum-exp.
+__device__ __forceinline__ float share(float s, float inv_t, float l) { return exp2_fast(__fmaf_rn(s, inv_t, -l) * kLog2e); }
+__device__ __forceinline__ double share(double s, double inv_t, double l) { return exp(s * inv_t - l); }
+
+template <typename T> __device__ __forceinline__ T widen_teacher(const void *values, int dtype, uint64_t i)
+{
+    switch (dtype) {
+    case kLogitF32: return (T) static_cast<const float *>(values)[i];
+    case kLogitF64: return (T) static_cast<const double *>(values)[i];
+    case kLogitBf16: return (T)(float)static_cast<const __bf16 *>(values)[i];
+    default: return (T)(float)static_cast<const _Float16 *>(values)[i];
+    }
+}
+
+// A row's teacher entries in LDS (k places, then one for the label): the index (-1 when
+// absent), q, log q and the student's logit there (kept, since the gradient may overwrite it).
+template <typename T> struct Entries {
+    T *q, *log_q, *s;
+    int *at;
+    T sum;     // Q
+    int label; // -1: none
+    static size_t bytes(uint32_t k) { return (k + 1) * (3 * sizeof(T) + 4); }
+    __device__ __forceinline__ Entries(void *lds, uint32_t k)
+        : q(static_cast<T *>(lds)), log_q(q + (k + 1)), s(log_q + (k + 1)),
+          at(reinterpret_cast<int *>(s + (k + 1))), sum(0), label(-1)
+    {
+    }
+};
+
+// Loads and normalises the row's entries. `red`: 2 x 16 places.
+template <int NT, typename T>
+__device__ __forceinline__ void load_entries(const DistillArgs &g, uint64_t row, Entries<T> &e, T *red)
+{
+    const int tid = threadIdx.x;
+    uint64_t bad = kNoFault;
+    const T t = (T)g.temperature;
+    T top = -INFINITY;
+    for (uint32_t j = tid; j < g.k; j += NT) {
+        int at = g.teacher_indices[row * g.k + j];
+        T z = widen_teacher<T>(g.teacher_values, g.teacher_dtype, row * g.k + j) / t;
+        if (at >= (int64_t)g.vocab) {
+            bad = pack_fault(row * (g.k + 1) + j, kInvalid) < bad ? pack_fault(row * (g.k + 1) + j, kInvalid) : bad;
+            at = -1;
+        }
+        if (at < 0) {
+            at = -1;
+            z = -INFINITY;
+        }
+        e.at[j] = at;
+        e.log_q[j] = z;
+        top = OpMax()(top, z);
+    }
+    int y = g.labels ? g.labels[row] : -1;
+    if (y >= (int64_t)g.vocab) {
+        if (tid == 0) {
+            const uint64_t f = pack_fault(row * (g.k + 1) + g.k, kInvalid);
+            bad = f < bad ? f : bad;
+        }
+        y = -1;
+    }
+    e.label = y < 0 ? -1 : y;
+    wave_record_fault(bad, g.fault, g.gate);
+    T log_sum;
+    if (g.teacher_log_sum) {
+        log_sum = g.teacher_log_sum_f64 ? (T) static_cast<const double *>(g.teacher_log_sum)[row]
+                                        : (T) static_cast<const float *>(g.teacher_log_sum)[row];
+    } else {
+        top = block_reduce<NT>(top, OpMax(), red);
+        T sum = 0;
+        for (uint32_t j = tid; j < g.k; j += NT) {
+            const T z = e.log_q[j];
+            sum += z == -INFINITY ? (T)0 : exp(z - top);
+        }
+        sum = block_reduce<NT>(sum, OpSum(), red + 16);
+        log_sum = top + log(sum);
+        if constexpr (NT > 64)
+            __syncthreads(); // red is used again below
+    }
+    T sum = 0;
+    for (uint32_t j = tid; j < g.k; j += NT) {
+        const T z = e.log_q[j];
+        const T lq = z - log_sum;
+        const T q = z == -INFINITY ? (T)0 : exp(lq);
+        e.q[j] = q;
+        e.log_q[j] = lq;
+        sum += q;
+    }
+    if (tid == 0) {
+        e.q[g.k] = 0;
+        e.at[g.k] = e.label;
+    }
+    e.sum = block_reduce<NT>(sum, OpSum(), red);
+    if constexpr (NT == 64)
+        __syncthreads();
+}
+
+// Reads the student's logits at the entries' places of [c0, c1), for the two functions below;
+// each lane reads and later uses its own places only.
+template <int NT, typename S, typename T>
+__device__ __forceinline__ void gather_entries(const DistillArgs &g, const S *s, Entries<T> &e, uint32_t c0, uint32_t c1)
+{
+    for (uint32_t j = threadIdx.x; j <= g.k; j += NT) {
+        const int at = e.at[j];
+        if (at >= (int)c0 && at < (int)c1)
+            e.s[j] = (T)s[at];
+    }
+}
+
+// The row's loss from the two log-sum-exps, on every thread. `red`: 2 x 16 places.
+template <int NT, typename T>
+__device__ __forceinline__ T row_loss(const DistillArgs &g, const Entries<T> &e, T lse, T lse1, T *red)
+{
+    T part = 0, hard = 0;
+    const T t = (T)g.temperature;
+    for (uint32_t j = threadIdx.x; j <= g.k; j += NT) {
+        if (e.at[j] < 0)
+            continue;
+        const T v = e.s[j];
+        if (j == g.k) {
+            hard = v == -INFINITY ? (T)INFINITY : lse1 - v;
+        } else if (!(e.q[j] == 0)) {
+            const T log_p = v == -INFINITY ? v : v / t - lse;
+            part += e.q[j] * (e.log_q[j] - log_p);
+        }
+    }
+    part = block_reduce<NT>(part, OpSum(), red);
+    hard = block_reduce<NT>(hard, OpSum(), red + 16);
+    T loss = 0;
+    if (g.distill_weight != 0 && !(e.sum == 0))
+        loss += (T)g.distill_weight * (t * t) * part;
+    if (g.label_weight != 0 && e.label >= 0)
+        loss += (T)g.label_weight * hard;
+    return loss;
+}
+
+// The places of [c0, c1) whose gradient differs from the dense part: `dense(v)` gives the dense
+// gradient of a logit.
+template <int NT, typename S, typename T, typename Dense>
+__device__ __forceinline__ void fix_entries(const DistillArgs &g, S *grad, const Entries<T> &e, uint32_t c0,
+                                            uint32_t c1, T scale, Dense dense)
+{
+    const T per_q = scale * (T)g.distill_weight * (T)g.temperature;
+    const T per_label = scale * (T)g.label_weight;
+    for (uint32_t j = threadIdx.x; j <= g.k; j += NT) {
+        const int at = e.at[j];
+        if (at < (int)c0 || at >= (int)c1)
+            continue;
+        bool first = true;
+        T less = 0;
+        for (uint32_t i = 0; i < g.k; i++)
+            if (e.at[i] == at) {
+                first = first && i >= j;
+                less += e.q[i];
+            }
+        if (!first)
+            continue;
+        T value = dense(e.s[j]);
+        if (per_q != 0)
+            value -= less * per_q;
+        if (at == e.label)
+            value -= per_label;
+        grad[at] = (S)value;
+    }
+}
+
+// ---------------------------------------------------- one workgroup a row, the row in registers
+//
+// Forward, or forward and backward, for rows of at most NT * R vectors: each thread keeps R
+// vectors of the row, so that the row is read once and its gradient written once.
+template <typename S, int NT, int R, bool GRAD>
+__global__ __launch_bounds__(NT) void k_distill_row(DistillArgs g)
+{
+    using T = typename StatOf<S>::T;
+    constexpr int N = kVec<S>;
+    if (block_gate_closed(g.gate))
+        return;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ T red[7][16];
+    const int tid = threadIdx.x;
+    const uint64_t row = blockIdx.x;
+    const S *s = static_cast<const S *>(g.logits) + row * g.stride;
+
+    u32x4 raw[R];
+#pragma unroll
+    for (int r = 0; r < R; r++)
+        raw[r] = load_vec(s, tid + r * NT, g.vocab);
+
+    Entries<T> e(lds, g.k);
+    load_entries<NT>(g, row, e, red[0]);
+
+    T m = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        T v[N];
+        unpack<S>(raw[r], v);
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            m = OpMax()(m, v[i]);
+    }
+    m = block_reduce<NT>(m, OpMax(), red[2]);
+
+    const T inv_t = (T)1 / (T)g.temperature;
+    const bool two = g.temperature != 1.0 && (g.log_sums_out != nullptr || e.label >= 0);
+    const Expo<T> ex(m, inv_t), ex1(m, (T)1);
+    T sum = 0, sum1 = 0;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        T v[N];
+        unpack<S>(raw[r], v);
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            sum += ex(v[i]);
+        if (two) {
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                sum1 += ex1(v[i]);
+        }
+    }
+    sum = block_reduce<NT>(sum, OpSum(), red[3]);
+    sum1 = two ? block_reduce<NT>(sum1, OpSum(), red[4]) : sum;
+    const T lse = ex.log_sum(sum), lse1 = two ? ex1.log_sum(sum1) : lse;
+    if (tid == 0 && g.log_sums_out) {
+        static_cast<T *>(g.log_sums_out)[2 * row] = lse;
+        static_cast<T *>(g.log_sums_out)[2 * row + 1] = lse1;
+    }
+    gather_entries<NT>(g, s, e, 0u, g.vocab);
+    if (g.loss) {
+        const T loss = row_loss<NT>(g, e, lse, lse1, red[5]);
+        if (tid == 0)
+            static_cast<T *>(g.loss)[row] = loss;
+    }
+    if constexpr (GRAD) {
+        const T scale = g.row_scale ? static_cast<const T *>(g.row_scale)[row] : (T)1;
+        T cq = scale * (T)g.distill_weight * (T)g.temperature * e.sum;
+        T cl = e.label >= 0 ? scale * (T)g.label_weight : (T)0;
+        if (!two) {
+            cq += cl;
+            cl = 0;
+        }
+        // Rows whose logits are all minus infinity have no probabilities.
+        const T pq = cq == 0 || sum == 0 ? (T)0 : cq / sum, pl = cl == 0 || sum1 == 0 ? (T)0 : cl / sum1;
+        auto dense = [&](T v) {
+            T out = pq == 0 ? (T)0 : ex(v) * pq;
+            if (pl != 0)
+                out += ex1(v) * pl;
+            return out;
+        };
+        S *grad = static_cast<S *>(g.grad) + row * g.grad_stride;
+        __syncthreads(); // the entries' logits are read: the gradient may lie in the row's place
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            T v[N];
+            unpack<S>(raw[r], v);
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                v[i] = dense(v[i]);
+            store_vec(grad, tid + r * NT, g.vocab, v);
+        }
+        for (uint32_t i = g.vocab + tid; i < g.grad_cols; i += NT)
+            grad[i] = (S)0;
+        __syncthreads();
+        fix_entries<NT>(g, grad, e, 0u, g.vocab, scale, dense);
+    }
+}
+
+// ----------------------------------------------------------- a row split over workgroups
+//
+// Rows that no workgroup holds, and few rows of a long vocabulary: the statistics of chunks of
+// a row, then per row the two log-sum-exps and the loss, then the gradient by chunks.
+template <typename T> struct Partial {
+    T m, sum, sum1;
+};
+
+template <typename S, int NT>
+__global__ __launch_bounds__(NT) void k_distill_stats(DistillArgs g, uint32_t chunks, uint32_t chunk_vecs,
+                                                      Partial<typename StatOf<S>::T> *parts)
+{
+    using T = typename StatOf<S>::T;
+    constexpr int N = kVec<S>;
+    constexpr int U = 4; // vectors in flight a thread
+    if (block_gate_closed(g.gate))
+        return;
+    __shared__ T red[3][16];
+    const uint64_t row = blockIdx.x / chunks;
+    const uint32_t chunk = blockIdx.x % chunks;
+    const S *s = static_cast<const S *>(g.logits) + row * g.stride;
+    const uint32_t first = chunk * chunk_vecs, last = first + chunk_vecs;
+    const T inv_t = (T)1 / (T)g.temperature;
+    const bool two = g.temperature != 1.0;
+
+    // Each thread's running maximum and sums, rescaled when a piece raises the maximum.
+    T m = -INFINITY, sum = 0, sum1 = 0;
+    for (uint32_t i = first + threadIdx.x; i < last; i += NT * U) {
+        u32x4 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            raw[u] = i + u * NT < last ? load_vec(s, i + u * NT, g.vocab) : minus_infinities<S>();
+        T v[U * N], top = m;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            unpack<S>(raw[u], v + u * N);
+#pragma unroll
+        for (int k = 0; k < U * N; k++)
+            top = OpMax()(top, v[k]);
+        const Expo<T> ex(top, inv_t), ex1(top, (T)1);
+        if (top != m) {
+            sum = m == -INFINITY ? sum : sum * ex(m);
+            sum1 = m == -INFINITY ? sum1 : sum1 * ex1(m);
+            m = top;
+        }
+#pragma unroll
+        for (int k = 0; k < U * N; k++)
+            sum += ex(v[k]);
+        if (two) {
+#pragma unroll
+            for (int k = 0; k < U * N; k++)
+                sum1 += ex1(v[k]);
+        }
+    }
+    const T top = block_reduce<NT>(m, OpMax(), red[0]);
+    if (m != top && m != -INFINITY) {
+        sum *= Expo<T>(top, inv_t)(m);
+        sum1 *= Expo<T>(top, (T)1)(m);
+    }
+    sum = block_reduce<NT>(sum, OpSum(), red[1]);
+    sum1 = block_reduce<NT>(sum1, OpSum(), red[2]);
+    if (threadIdx.x == 0)
+        parts[blockIdx.x] = Partial<T>{top, sum, two ? sum1 : sum};
+}
+
+constexpr int kFinishThreads = 256;
+
+template <typename S>
+__global__ __launch_bounds__(kFinishThreads) void k_distill_finish(DistillArgs g, uint32_t chunks,
+                                                                   const Partial<typename StatOf<S>::T> *parts)
+{
+    using T = typename StatOf<S>::T;
+    constexpr int NT = kFinishThreads;
+    if (block_gate_closed(g.gate))
+        return;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ T red[7][16];
+    const uint64_t row = blockIdx.x;
+    const S *s = static_cast<const S *>(g.logits) + row * g.stride;
+    T m = -INFINITY;
+    for (uint32_t c = threadIdx.x; c < chunks; c += NT)
+        m = OpMax()(m, parts[row * chunks + c].m);
+    m = block_reduce<NT>(m, OpMax(), red[0]);
+    const Expo<T> ex(m, (T)1 / (T)g.temperature), ex1(m, (T)1);
+    T sum = 0, sum1 = 0;
+    for (uint32_t c = threadIdx.x; c < chunks; c += NT) {
+        const Partial<T> p = parts[row * chunks + c];
+        // A chunk of minus infinities adds nothing; one with a NaN among them hands it on.
+        sum += p.m == -INFINITY ? p.sum : p.sum * ex(p.m);
+        sum1 += p.m == -INFINITY ? p.sum1 : p.sum1 * ex1(p.m);
+    }
+    sum = block_reduce<NT>(sum, OpSum(), red[1]);
+    sum1 = block_reduce<NT>(sum1, OpSum(), red[2]);
+    const T lse = ex.log_sum(sum), lse1 = g.temperature != 1.0 ? ex1.log_sum(sum1) : lse;
+    if (threadIdx.x == 0) {
+        static_cast<T *>(g.log_sums_out)[2 * row] = lse;
+        static_cast<T *>(g.log_sums_out)[2 * row + 1] = lse1;
+    }
+    if (g.loss) {
+        Entries<T> e(lds, g.k);
+        load_entries<NT>(g, row, e, red[3]);
+        gather_entries<NT>(g, s, e, 0u, g.vocab);
+        const T loss = row_loss<NT>(g, e, lse, lse1, red[5]);
+        if (threadIdx.x == 0)
+            static_cast<T *>(g.loss)[row] = loss;
+    }
+}
+
+// The gradient of one chunk of a row from the row's log-sum-exps.
+template <typename S, int NT>
+__global__ __launch_bounds__(NT) void k_distill_grad(DistillArgs g, uint32_t chunks, uint32_t chunk_vecs)
+{
+    using T = typename StatOf<S>::T;
+    constexpr int N = kVec<S>;
+    constexpr int U = 4;
+    if (block_gate_closed(g.gate))
+        return;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ T red[2][16];
+    const uint64_t row = blockIdx.x / chunks;
+    const uint32_t chunk = blockIdx.x % chunks;
+    const S *s = static_cast<const S *>(g.logits) + row * g.stride;
+    S *grad = static_cast<S *>(g.grad) + row * g.grad_stride;
+    const uint32_t first = chunk * chunk_vecs, last = first + chunk_vecs;
+    const uint32_t c0 = first * N, c1 = last * N < g.vocab ? last * N : g.vocab;
+
+    Entries<T> e(lds, g.k);
+    load_entries<NT>(g, row, e, red[0]);
+    gather_entries<NT>(g, s, e, c0, c1);
+    const T lse = static_cast<const T *>(g.log_sums_in)[2 * row], lse1 = static_cast<const T *>(g.log_sums_in)[2 * row + 1];
+    const T scale = g.row_scale ? static_cast<const T *>(g.row_scale)[row] : (T)1;
+    T pq = scale * (T)g.distill_weight * (T)g.temperature * e.sum;
+    T pl = e.label >= 0 ? scale * (T)g.label_weight : (T)0;
+    if (g.temperature == 1.0) {
+        pq += pl;
+        pl = 0;
+    }
+    if (lse == -INFINITY) // a row of minus infinities has no probabilities
+        pq = 0;
+    if (lse1 == -INFINITY)
+        pl = 0;
+    const T inv_t = (T)1 / (T)g.temperature;
+    auto dense = [&](T v) {
+        T out = pq == 0 ? (T)0 : share(v, inv_t, lse) * pq;
+        if (pl != 0)
+            out += share(v, (T)1, lse1) * pl;
+        return out;
+    };
+    __syncthreads(); // the entries' logits are read: the gradient may lie in the row's place
+    for (uint32_t i = first + threadIdx.x; i < last; i += NT * U) {
+        u32x4 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            raw[u] = i + u * NT < last ? load_vec(s, i + u * NT, g.vocab) : minus_infinities<S>();
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            T v[N];
+            unpack<S>(raw[u], v);
+#pragma unroll
+            for (int k = 0; k < N; k++)
+                v[k] = dense(v[k]);
+            if (i + u * NT < last)
+                store_vec(grad, i + u * NT, g.vocab, v);
+        }
+    }
+    if (chunk == chunks - 1)
+        for (uint32_t i = g.vocab + threadIdx.x; i < g.grad_cols; i += NT)
+            grad[i] = (S)0;
+    __syncthreads();
+    fix_entries<NT>(g, grad, e, c0, c1, scale, dense);
+}
+
+// ------------------------------------------------------------------------- launches
+
+struct Split {
+    uint32_t chunks, vecs;
+};
+constexpr int kSplitThreads = 256;
+
+Split split_of(uint64_t rows, uint32_t vecs)
+{
+    // Enough workgroups for the chip, each with at least 4 vectors a thread.
+    const uint64_t want = (2048 + rows - 1) / rows;
+    const uint64_t most = (vecs + 4 * kSplitThreads - 1) / (4 * kSplitThreads);
+    const uint64_t chunks = want < most ? want : most;
+    const uint32_t each = (uint32_t)((vecs + chunks - 1) / chunks);
+    return Split{(vecs + each - 1) / each, each};
+}
+
+template <typename S, int NT, int R> hipError_t launch_row(hipStream_t s, const DistillArgs &g)
+{
+    const size_t lds = Entries<typename StatOf<S>::T>::bytes(g.k);
+    if (g.grad)
+        hipLaunchKernelGGL((k_distill_row<S, NT, R, true>), dim3((unsigned)g.rows), dim3(NT), lds, s, g);
+    else
+        hipLaunchKernelGGL((k_distill_row<S, NT, R, false>), dim3((unsigned)g.rows), dim3(NT), lds, s, g);
+    return hipGetLastError();
+}
+
+template <typename S> hipError_t launch_grad(hipStream_t s, const DistillArgs &g, Split sp)
+{
+    const size_t lds = Entries<typename StatOf<S>::T>::bytes(g.k);
+    hipLaunchKernelGGL((k_distill_grad<S, kSplitThreads>), dim3((unsigned)(g.rows * sp.chunks)), dim3(kSplitThreads),
+                       lds, s, g, sp.chunks, sp.vecs);
+    return hipGetLastError();
+}
+
+constexpr uint32_t kHeldVecs = 16 * 1024; // vectors of a row that one workgroup holds
+
+bool held(uint64_t rows, uint32_t vecs) { return vecs <= kHeldVecs && (rows >= 64 || vecs <= 1024); }
+
+template <typename S> hipError_t launch_t(hipStream_t s, DistillArgs g, void *scratch)
+{
+    using T = typename StatOf<S>::T;
+    const uint32_t vecs = (g.vocab + kVec<S> - 1) / kVec<S>;
+    if (g.log_sums_in)
+        return launch_grad<S>(s, g, split_of(g.rows, vecs));
+    if (held(g.rows, vecs)) {
+        if (vecs <= 64 * 4)
+            return launch_row<S, 64, 4>(s, g);
+        if (vecs <= 256 * 4)
+            return launch_row<S, 256, 4>(s, g);
+        if (vecs <= 256 * 16)
+            return launch_row<S, 256, 16>(s, g);
+        if (vecs <= 512 * 16)
+            return launch_row<S, 512, 16>(s, g);
+        return launch_row<S, 1024, 16>(s, g);
+    }
+    const Split sp = split_of(g.rows, vecs);
+    Partial<T> *parts = static_cast<Partial<T> *>(scratch);
+    if (!g.log_sums_out)
+        g.log_sums_out = parts + g.rows * sp.chunks;
+    hipLaunchKernelGGL((k_distill_stats<S, kSplitThreads>), dim3((unsigned)(g.rows * sp.chunks)), dim3(kSplitThreads), 0,
+                       s, g, sp.chunks, sp.vecs, parts);
+    hipError_t err = hipGetLastError();
+    if (err != hipSuccess)
+        return err;
+    hipLaunchKernelGGL((k_distill_finish<S>), dim3((unsigned)g.rows), dim3(kFinishThreads), Entries<T>::bytes(g.k), s, g,
+                       sp.chunks, parts);
+    if ((err = hipGetLastError()) != hipSuccess || !g.grad)
+        return err;
+    g.log_sums_in = g.log_sums_out;
+    return launch_grad<S>(s, g, sp);
+}
+
+template <typename S> size_t scratch_t(const DistillArgs &g)
+{
+    using T = typename StatOf<S>::T;
+    const uint32_t vecs = (g.vocab + kVec<S> - 1) / kVec<S>;
+    if (g.rows == 0 || g.log_sums_in || held(g.rows, vecs))
+        return 0;
+    return g.rows * (split_of(g.rows, vecs).chunks * sizeof(Partial<T>) + 2 * sizeof(T));
+}
+
+} // namespace
+
+size_t distill_scratch_bytes(const DistillArgs &g)
+{
+    switch (g.dtype) {
+    case kLogitF32: return scratch_t<float>(g);
+    case kLogitF64: return scratch_t<double>(g);
+    case kLogitBf16: return scratch_t<__bf16>(g);
+    default: return scratch_t<_Float16>(g);
+    }
+}
+
+hipError_t launch_distill(hipStream_t s, const DistillArgs &g, void *scratch)
+{
+    if (g.rows == 0)
+        return hipSuccess;
+    switch (g.dtype) {
+    case kLogitF32: return launch_t<float>(s, g, scratch);
+    case kLogitF64: return launch_t<double>(s, g, scratch);
+    case kLogitBf16: return launch_t<__bf16>(s, g, scratch);
+    default: return launch_t<_Float16>(s, g, scratch);
+    }
+}
+
+} // namespace pcu

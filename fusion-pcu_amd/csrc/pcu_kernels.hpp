@@ -284,6 +284,74 @@ size_t native_mse_scratch_bytes(int dtype, uint64_t n);
 hipError_t launch_native_mse(hipStream_t s, int dtype, uint64_t n, const void *p, const void *t,
                              void *scratch, double scale, void *out, NodeGate gate);
 
+// ------------------------------------------------------------ operators on logits
+// `rows` rows of `vocab` logits, row r at element r * stride. Every limit below is checked by
+// the caller; indices that the inputs hold are checked by the kernels.
+enum : int { kLogitF32 = 0, kLogitF64 = 1, kLogitBf16 = 2, kLogitF16 = 3 };
+constexpr uint32_t kLogitMaxVocab = 1u << 22; // weights of 2^40 each add up below 2^62
+constexpr uint32_t kLogitMaxK = 1024;
+
+// Distillation from a teacher's top logits. Statistics (loss, log_sums, row_scale) are binary32,
+// binary64 for binary64 logits; the teacher's log-sum-exps binary64 where _f64 says so.
+struct DistillArgs {
+    const void *logits = nullptr;
+    int dtype = 0;
+    uint64_t rows = 0, stride = 0;
+    uint32_t vocab = 0, k = 0;
+    const void *teacher_values = nullptr;  // rows x k
+    int teacher_dtype = 0;
+    const int32_t *teacher_indices = nullptr; // rows x k, negative: absent
+    const void *teacher_log_sum = nullptr; // rows, or null: over the row's entries
+    int teacher_log_sum_f64 = 0;
+    const int32_t *labels = nullptr; // rows, negative: none; or null
+    double temperature = 1.0, distill_weight = 1.0, label_weight = 0.0;
+    const void *row_scale = nullptr;    // rows, or null: 1
+    const void *log_sums_in = nullptr;  // rows x 2: the gradient alone, from these
+    void *log_sums_out = nullptr;       // rows x 2, or null
+    void *loss = nullptr;               // rows, or null
+    void *grad = nullptr;               // rows x grad_cols (zeros past the vocabulary), or null
+    uint64_t grad_stride = 0;
+    uint32_t grad_cols = 0;
+    unsigned long long *fault = nullptr; // ordinal row * (k + 1) + entry (k: the label)
+    NodeGate gate{nullptr, 0};
+};
+size_t distill_scratch_bytes(const DistillArgs &g);
+hipError_t launch_distill(hipStream_t s, const DistillArgs &g, void *scratch);
+
+// The k largest logits of each row (value descending, index ascending) and, unless null, the
+// row's log-sum-exp of l / temperature. Places past the vocabulary: minus infinity and -1.
+struct TopArgs {
+    const void *logits = nullptr;
+    int dtype = 0;
+    uint64_t rows = 0, stride = 0;
+    uint32_t vocab = 0, k = 0;
+    double temperature = 1.0;
+    void *values = nullptr;      // rows x k, of the logits' type
+    int32_t *indices = nullptr;  // rows x k
+    void *log_sum = nullptr;     // rows, binary32 (binary64 for binary64 logits), or null
+    NodeGate gate{nullptr, 0};
+};
+hipError_t launch_top(hipStream_t s, const TopArgs &g);
+
+// One token a row. A setting's array holds one value a row; where it is null, `_all` holds for
+// every row. A row with an invalid setting or random number records a fault (ordinal: the row).
+struct SampleArgs {
+    const void *logits = nullptr;
+    int dtype = 0;
+    uint64_t rows = 0, stride = 0;
+    uint32_t vocab = 0;
+    const float *uniform = nullptr;
+    const float *temperature = nullptr, *top_p = nullptr, *min_p = nullptr;
+    const int32_t *top_k = nullptr;
+    float temperature_all = 1.0f, top_p_all = 1.0f, min_p_all = 0.0f;
+    int32_t top_k_all = 0;
+    int32_t *tokens = nullptr;
+    float *log_prob = nullptr; // or null
+    unsigned long long *fault = nullptr;
+    NodeGate gate{nullptr, 0};
+};
+hipError_t launch_sample(hipStream_t s, const SampleArgs &g);
+
 // Small device utilities (fill kernels rather than memsets, so a captured graph replays
 // them as kernels).
 hipError_t launch_fill_u64(hipStream_t s, unsigned long long *p, uint64_t n, uint64_t value);

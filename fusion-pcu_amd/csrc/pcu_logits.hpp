@@ -1,0 +1,196 @@
+// Device helpers of the operators on logits (top logits, distillation, sampling): 16-byte
+// vectors of a row in any of the four types, reductions over a workgroup and the order of a
+// row's values.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "pcu_device.hpp"
+
+#pragma clang fp contract(off)
+
+namespace pcu {
+
+// The type that a row's statistics are held in: 32 bits, 64 for binary64 rows.
+template <typename S> struct StatOf { using T = float; };
+template <> struct StatOf<double> { using T = double; };
+
+// One 16-byte piece of a row. Rows start at any multiple of their type's size (odd
+// vocabularies, padded strides), and the hardware loads and stores 16 bytes at any address:
+// a misaligned piece costs at most one more cache line for each wave's kilobyte.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+
+template <typename S> constexpr int kVec = 16 / (int)sizeof(S);
+
+template <typename S> __device__ __forceinline__ void unpack(const u32x4 &raw, typename StatOf<S>::T *out)
+{
+    if constexpr (sizeof(S) == 8) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            out[i] = __longlong_as_double((long long)(((uint64_t)raw[2 * i + 1] << 32) | raw[2 * i]));
+    } else if constexpr (sizeof(S) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            out[i] = __uint_as_float(raw[i]);
+    } else if constexpr (__is_same(S, __bf16)) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            out[2 * i] = __uint_as_float(raw[i] << 16);
+            out[2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            out[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)raw[i]);
+            out[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(raw[i] >> 16));
+        }
+    }
+}
+
+// Values rounded once (to nearest even) to the row's type.
+template <typename S> __device__ __forceinline__ u32x4 pack(const typename StatOf<S>::T *v)
+{
+    u32x4 raw;
+    if constexpr (sizeof(S) == 8) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint64_t b = (uint64_t)__double_as_longlong(v[i]);
+            raw[2 * i] = (uint32_t)b;
+            raw[2 * i + 1] = (uint32_t)(b >> 32);
+        }
+    } else if constexpr (sizeof(S) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            raw[i] = __float_as_uint(v[i]);
+    } else {
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        typedef S s16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const f32x2 two = {v[2 * i], v[2 * i + 1]};
+            raw[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(two, s16x2));
+        }
+    }
+    return raw;
+}
+
+template <typename S> __device__ __forceinline__ u32x4 minus_infinities()
+{
+    if constexpr (sizeof(S) == 8)
+        return u32x4{0u, 0xfff00000u, 0u, 0xfff00000u};
+    else if constexpr (sizeof(S) == 4)
+        return u32x4{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u};
+    else if constexpr (__is_same(S, __bf16))
+        return u32x4{0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};
+    else
+        return u32x4{0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u};
+}
+
+// Vector i of a row of n values; places past the row's end read as minus infinity, whole
+// vectors past it too.
+template <typename S> __device__ __forceinline__ u32x4 load_vec(const S *row, uint32_t i, uint32_t n)
+{
+    const uint32_t at = i * kVec<S>;
+    if (at + kVec<S> <= n)
+        return *reinterpret_cast<const u32x4_any *>(row + at);
+    u32x4 raw = minus_infinities<S>();
+    if (at < n) {
+        if constexpr (sizeof(S) == 2) {
+            for (uint32_t e = 0; at + e < n; e++) {
+                const uint32_t b = __builtin_bit_cast(uint16_t, row[at + e]);
+                const uint32_t keep = e & 1 ? 0x0000ffffu : 0xffff0000u;
+#pragma unroll
+                for (uint32_t w = 0; w < 4; w++)
+                    if (w == e / 2)
+                        raw[w] = (raw[w] & keep) | (e & 1 ? b << 16 : b);
+            }
+        } else {
+            constexpr uint32_t W = sizeof(S) / 4;
+            const uint32_t *words = reinterpret_cast<const uint32_t *>(row + at);
+#pragma unroll
+            for (uint32_t w = 0; w < 4; w++)
+                if (at + w / W < n)
+                    raw[w] = words[w];
+        }
+    }
+    return raw;
+}
+
+template <typename S>
+__device__ __forceinline__ void store_vec(S *row, uint32_t i, uint32_t n, const typename StatOf<S>::T *v)
+{
+    const uint32_t at = i * kVec<S>;
+    if (at + kVec<S> <= n) {
+        *reinterpret_cast<u32x4_any *>(row + at) = pack<S>(v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < kVec<S>; e++)
+            if (at + e < n)
+                row[at + e] = (S)v[e];
+    }
+}
+
+// --------------------------------------------------------- reductions of a workgroup
+struct OpMax {
+    __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+    __device__ __forceinline__ double operator()(double a, double b) const { return fmax(a, b); }
+};
+struct OpSum {
+    template <typename T> __device__ __forceinline__ T operator()(T a, T b) const { return a + b; }
+};
+
+template <typename T, typename Op> __device__ __forceinline__ T wave_reduce(T v, Op op)
+{
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1)
+        v = op(v, __shfl_xor(v, off, 64));
+    return v;
+}
+
+// Every thread gets the result, folded in one fixed order. `lds`: NT / 64 entries that no
+// other reduction between the same two barriers uses.
+template <int NT, typename T, typename Op> __device__ __forceinline__ T block_reduce(T v, Op op, T *lds)
+{
+    v = wave_reduce(v, op);
+    if constexpr (NT == 64)
+        return v;
+    if ((threadIdx.x & 63) == 0)
+        lds[threadIdx.x / 64] = v;
+    __syncthreads();
+    v = lds[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; w++)
+        v = op(v, lds[w]);
+    return v;
+}
+
+// ------------------------------------------------------------------ exponentials
+// Binary32: the hardware's 2^x (1 ulp) on a product that already holds log2(e).
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr double kLn2 = 0.69314718055994530942;
+
+// exp((s - m) / T) of the row's values against a fixed m. Binary32: the difference first (it
+// is exact near m, and m / T itself may overflow where T is small), then 2^x of the product.
+template <typename T> struct Expo;
+template <> struct Expo<float> {
+    float m, inv_t, c;
+    __device__ __forceinline__ Expo(float mx, float it) : m(mx == -INFINITY ? 0.0f : mx), inv_t(it), c(it * kLog2e) {}
+    __device__ __forceinline__ float operator()(float s) const { return exp2_fast((s - m) * c); }
+    // log(sum of exp(s / T)) from the sum of the above.
+    __device__ __forceinline__ float log_sum(float sum) const
+    {
+        return (float)((double)m * inv_t + (double)__builtin_amdgcn_logf(sum) * kLn2);
+    }
+};
+template <> struct Expo<double> {
+    double inv_t, m;
+    __device__ __forceinline__ Expo(double mx, double it) : inv_t(it), m(mx == -INFINITY ? 0.0 : mx) {}
+    __device__ __forceinline__ double operator()(double s) const { return exp((s - m) * inv_t); }
+    __device__ __forceinline__ double log_sum(double sum) const { return m * inv_t + log(sum); }
+};
+
+} // namespace pcu

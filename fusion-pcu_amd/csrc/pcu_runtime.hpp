@@ -16,7 +16,8 @@ extern thread_local std::string g_thread_error;
 
 // Ordered fault domain of one node (core/dialect/tensor/fault_domain/fault_domain.rs:30-34).
 // Native: an explicitly permitted native compound, which records no arithmetic fault.
-enum class Prim { Elementwise, MatMul, Sgd, Mse, Native };
+// Checked: a native op whose word names the first input that is out of its range.
+enum class Prim { Elementwise, MatMul, Sgd, Mse, Native, Checked };
 
 struct NodeInfo {
     Prim prim;
@@ -25,6 +26,13 @@ struct NodeInfo {
 };
 
 double count_as(int dtype, uint64_t n);
+
+// [p, p + pb) and [q, q + qb) share a byte.
+inline bool ranges_overlap(const void *p, uint64_t pb, const void *q, uint64_t qb)
+{
+    const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
+    return p && q && pb && qb && a < b + qb && b < a + pb;
+}
 
 struct Prepared;
 // A prepared graph gives its device buffers back and forgets its context (defined with the
@@ -104,7 +112,7 @@ struct Ctx {
         void *p = nullptr;
         size_t cap = 0;
     };
-    Scratch matmul_scratch, mse_scratch, bt_scratch, table_scratch;
+    Scratch matmul_scratch, mse_scratch, bt_scratch, table_scratch, logits_scratch;
     uint32_t screen_gen = 0; // generation of the latest MatMul exponent screen
     // Buffers released by the caller are kept for reuse by an allocation of the same size
     // (a training step frees its previous weights and takes as many new ones of the same
@@ -204,6 +212,15 @@ struct Ctx {
     pcu_status op_native_mse(int dtype, uint64_t n, const void *p, const void *t, void *out);
     pcu_status op_native_sgd(int dtype, uint64_t n, const void *w, const void *g, float rate,
                              bool contracted, void *out);
+    // The operators on logits (logits.cpp). `mode` of op_distill: what the call asks for.
+    enum class Distill { Loss, Backward, Step };
+    pcu_status op_top_logits(const pcu_logits *logits, uint32_t k, double temperature, void *values,
+                             int32_t *indices, void *log_sum);
+    pcu_status op_distill(Distill mode, const pcu_logits *student, const pcu_distill *d,
+                          const void *log_sums_in, const void *row_scale, void *loss,
+                          void *log_sums_out, void *grad, uint64_t grad_cols, uint64_t grad_stride);
+    pcu_status op_sample(const pcu_logits *logits, const pcu_sampling *p, int32_t *tokens,
+                         float *log_prob);
 };
 
 } // namespace pcu

@@ -151,7 +151,7 @@ Ctx::~Ctx()
         (void)hipStreamSynchronize(stream);
     if (side)
         (void)hipStreamSynchronize(side);
-    for (Scratch *b : {&matmul_scratch, &mse_scratch, &bt_scratch, &table_scratch})
+    for (Scratch *b : {&matmul_scratch, &mse_scratch, &bt_scratch, &table_scratch, &logits_scratch})
         if (b->p)
             (void)hipFreeAsync(b->p, stream);
     for (const Released &r : reuse)
@@ -426,6 +426,9 @@ static bool decode_word(const NodeInfo &n, uint64_t word, pcu_fault *f)
         return kind != PCU_FAULT_DIVIDE_BY_ZERO;
     case Prim::Native:
         return false; // native kernels never write their word
+    case Prim::Checked:
+        f->element_index = ordinal;
+        return ordinal < n.extent && kind == PCU_FAULT_INVALID;
     }
     return false;
 }
@@ -686,13 +689,6 @@ pcu_status Ctx::resolve_timings()
 static bool valid_dtype(int d) { return d == PCU_F32 || d == PCU_F64; }
 static bool valid_policy(int p) { return p >= 0 && p <= 2; }
 static size_t dsize(int d) { return d == PCU_F32 ? 4 : 8; }
-
-// [p, p + pb) and [q, q + qb) share a byte.
-static bool ranges_overlap(const void *p, uint64_t pb, const void *q, uint64_t qb)
-{
-    const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
-    return p && q && pb && qb && a < b + qb && b < a + pb;
-}
 
 // Elementwise kernels read element i of each operand and then write element i of out, so
 // an out that is exactly an operand (an in-place update) is safe; any other overlap lets a

@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define PCU_ROCM_ABI_VERSION 3
+#define PCU_ROCM_ABI_VERSION 4
 
 typedef struct pcu_ctx pcu_ctx;
 
@@ -54,7 +54,8 @@ typedef enum pcu_status {
                                 * HipError::InvalidExecutionFaultWord(word) */
 } pcu_status;
 
-typedef enum pcu_dtype { PCU_F32 = 0, PCU_F64 = 1 } pcu_dtype;
+/* The operators on logits admit all four types, every other call PCU_F32 and PCU_F64. */
+typedef enum pcu_dtype { PCU_F32 = 0, PCU_F64 = 1, PCU_BF16 = 2, PCU_F16 = 3 } pcu_dtype;
 
 /* PcuFloatUnderflowPolicy (core/scalar_float_underflow.rs:47-58). */
 typedef enum pcu_underflow {
@@ -234,6 +235,107 @@ pcu_status pcu_native_mse(pcu_ctx *ctx, pcu_dtype dtype, uint64_t n, const void 
 pcu_status pcu_native_sgd(pcu_ctx *ctx, pcu_dtype dtype, uint64_t n, const void *weights,
                           const void *gradient, float learning_rate, int contracted, void *out);
 
+/* ----------------------------------------------------------- operators on logits
+ * No counterpart in the reference: what a language model does with its output layer's
+ * logits. Native arithmetic (non-finite results are ordinary values), each call one program
+ * node, rows independent of each other. `fault` reports what only the device can see, an index or
+ * a setting out of its range, as PCU_FAULT_INVALID with the lowest such element (named at
+ * each call); the outputs of the other rows are then unspecified. */
+
+/* `rows` rows of `vocab` values of any dtype; row r starts at element r * stride
+ * (stride >= vocab: the columns between belong to the caller). Any alignment of the type. */
+typedef struct pcu_logits {
+    const void *data;
+    uint32_t dtype; /* pcu_dtype */
+    uint32_t reserved;
+    uint64_t rows, vocab, stride;
+} pcu_logits;
+#define PCU_LOGITS_MAX_VOCAB (1u << 22) /* longest row (and, at 256 times that, stride) */
+#define PCU_LOGITS_MAX_ROWS (1u << 30)
+#define PCU_LOGITS_MAX_K 1024u          /* most entries a row of top logits or of a teacher */
+
+/* The k largest logits of each row by (value descending, index ascending), -0 equal to +0
+ * and NaN after minus infinity. values: rows x k of the logits' type; indices: rows x k;
+ * places past the vocabulary hold minus infinity and -1. log_sum (or NULL): the row's
+ * log(sum exp(l / temperature)), F32 (F64 for F64 logits); minus infinity for a row of minus
+ * infinities, NaN for a row that holds a NaN or plus infinity. temperature > 0. */
+pcu_status pcu_native_top_logits(pcu_ctx *ctx, const pcu_logits *logits, uint32_t k,
+                                 double temperature, void *values, int32_t *indices,
+                                 void *log_sum);
+
+/* Distillation from a teacher's top logits. Row r has k entries (v_j, i_j), a negative index
+ * marking an absent one, and maybe a label y:
+ *   q_j = exp(v_j / T - L), L = teacher_log_sum[r] (the teacher's log-sum-exp of l / T over the
+ *         whole row), or without it the log-sum-exp over the row's entries; Q = sum q_j
+ *   p = softmax(s / T), p1 = softmax(s) over the student's row s
+ *   loss[r] = distill_weight T^2 sum_j q_j (log q_j - log p[i_j]) - label_weight log p1[y]
+ *   gradient[r][v] = row_scale[r] (distill_weight T (Q p_v - sum of q_j with i_j = v)
+ *                                  + label_weight (p1_v - [v = y]))
+ * The label terms belong to rows with y >= 0 only. Terms with weight 0 are left out, whatever
+ * they hold: a row with neither entries nor label has loss 0 and gradient 0. In a row of minus
+ * infinities p is 0. The same index twice adds up. An index or label of vocab or more is a
+ * fault (element_index r * (k + 1) + j, j = k for the label). */
+typedef struct pcu_distill {
+    const void *teacher_values;     /* rows x k of teacher_dtype */
+    const int32_t *teacher_indices; /* rows x k */
+    const void *teacher_log_sum;    /* rows, F64 when teacher_dtype is F64, else F32; or NULL */
+    const int32_t *labels;          /* rows; or NULL */
+    uint32_t teacher_dtype;         /* pcu_dtype */
+    uint32_t k;                     /* 0 .. PCU_LOGITS_MAX_K */
+    double temperature;             /* > 0 */
+    double distill_weight, label_weight;
+} pcu_distill;
+
+/* loss: rows; log_sums (or NULL): rows x 2, the student's log-sum-exp of s / T and of s. Both
+ * F32, F64 for F64 logits (as row_scale below). */
+pcu_status pcu_native_distill_loss(pcu_ctx *ctx, const pcu_logits *student,
+                                   const pcu_distill *distill, void *loss, void *log_sums,
+                                   pcu_fault *fault);
+/* The gradient from the log_sums of pcu_native_distill_loss. gradient: rows x
+ * gradient_cols of the student's type, row r at element r * gradient_stride; columns from vocab
+ * to gradient_cols are set to 0. It may lie exactly on the student's logits (same pointer and
+ * stride); it may overlap no other input. row_scale (or NULL for 1): rows. */
+pcu_status pcu_native_distill_backward(pcu_ctx *ctx, const pcu_logits *student,
+                                       const pcu_distill *distill, const void *log_sums,
+                                       const void *row_scale, void *gradient,
+                                       uint64_t gradient_cols, uint64_t gradient_stride,
+                                       pcu_fault *fault);
+/* Loss and gradient at once: the row is read once where a workgroup can hold it. */
+pcu_status pcu_native_distill_step(pcu_ctx *ctx, const pcu_logits *student,
+                                   const pcu_distill *distill, const void *row_scale, void *loss,
+                                   void *gradient, uint64_t gradient_cols,
+                                   uint64_t gradient_stride, pcu_fault *fault);
+
+/* One token a row, drawn with the given uniform random numbers u (F32, 0 <= u < 1):
+ *   m = the row's maximum (NaN apart); z = (l - m) * (1 / temperature), each operation rounded
+ *       to F32; weight w = floor(2^40 exp(z)), 2^40 at the maximum; NaN and what lies below
+ *       2^-40 of the largest weight have weight 0
+ *   the first top_k of (value descending, index ascending); of these the shortest prefix, at least
+ *   one token, that holds floor(2^31 top_p) / 2^31 of their weight; of these the tokens
+ *   with w >= 2^40 min_p
+ *   the token: the first kept one by index at which the running weight exceeds
+ *   floor(floor(2^31 u) * (kept weight) / 2^31).
+ * Weights are integers: the token depends on nothing but the row, its settings and u.
+ * log_prob (or NULL): F32, log(w / kept weight) of the token. A row without a logit above
+ * minus infinity gets token -1 and log_prob minus infinity.
+ * Settings: an array with one value a row, or, where it is NULL, the value beside it for every
+ * row. temperature in [0, inf), 0 (or a value whose reciprocal overflows) taking the maximum
+ * of lowest index; top_k <= 0 or >= vocab for no limit; top_p in [0, 1]; min_p in [0, 1]. A row
+ * with a setting or u outside its range is a fault (element_index: the row). */
+typedef struct pcu_sampling {
+    const float *uniform;
+    const float *temperature;
+    const int32_t *top_k;
+    const float *top_p;
+    const float *min_p;
+    float temperature_value;
+    int32_t top_k_value;
+    float top_p_value;
+    float min_p_value;
+} pcu_sampling;
+pcu_status pcu_native_sample(pcu_ctx *ctx, const pcu_logits *logits, const pcu_sampling *sampling,
+                             int32_t *tokens, float *log_prob, pcu_fault *fault);
+
 /* ------------------------------------------------------------------ program
  * Between begin and end every op call is only enqueued and numbered as a node (0, 1, ...;
  * pcu_checked_add_relu takes two numbers). pcu_program_end synchronizes once and reports
@@ -276,7 +378,10 @@ typedef enum pcu_kernel_id {
     PCU_KERNEL_NATIVE_SGD = 10,
     PCU_KERNEL_NATIVE_MSE = 11,
     PCU_KERNEL_ELEMENTWISE_CHAIN = 12, /* a prepared program's fused elementwise nodes */
-    PCU_KERNEL_COUNT = 13
+    PCU_KERNEL_TOP_LOGITS = 13,
+    PCU_KERNEL_DISTILL = 14,           /* all launches of one distillation call */
+    PCU_KERNEL_SAMPLE = 15,
+    PCU_KERNEL_COUNT = 16
 } pcu_kernel_id;
 pcu_status pcu_profile_enable(pcu_ctx *ctx, int on);
 pcu_status pcu_profile_read(pcu_ctx *ctx, int kernel, double *total_ms, uint64_t *launches);
