@@ -189,8 +189,9 @@ __device__ __forceinline__ void fix_entries(const DistillArgs &g, S *grad, const
 
 // ---------------------------------------------------- one workgroup a row, the row in registers
 //
-// Forward, or forward and backward, for rows of at most NT * R vectors: each thread keeps R
-// vectors of the row, so that the row is read once and its gradient written once.
+// Forward, or forward and backward, for rows of at most NT * R whole vectors (the values after
+// the last whole one lie one a lane in the first wave): each thread keeps R vectors of the row,
+// so that the row is read once and its gradient written once.
 template <typename S, int NT, int R, bool GRAD>
 __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs g)
 {
@@ -200,19 +201,22 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs g)
         return;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ T red[7][16];
-    const int tid = threadIdx.x;
+    const uint32_t tid = threadIdx.x;
     const uint64_t row = blockIdx.x;
     const S *s = static_cast<const S *>(g.logits) + row * g.stride;
+    const uint32_t whole = g.vocab / N, rest = whole * N + tid;
+    const bool has_rest = rest < g.vocab; // at most N - 1 lanes
 
     u32x4 raw[R];
 #pragma unroll
     for (int r = 0; r < R; r++)
-        raw[r] = load_vec(s, tid + r * NT, g.vocab);
+        raw[r] = tid + r * NT < whole ? load_held(s, r * NT, tid) : minus_infinities<S>();
+    const T extra = has_rest ? (T)s[rest] : (T)-INFINITY;
 
     Entries<T> e(lds, g.k);
     load_entries<NT>(g, row, e, red[0]);
 
-    T m = -INFINITY;
+    T m = extra;
 #pragma unroll
     for (int r = 0; r < R; r++) {
         T v[N];
@@ -220,24 +224,35 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs g)
 #pragma unroll
         for (int i = 0; i < N; i++)
             m = OpMax()(m, v[i]);
+        one_at_a_time();
     }
     m = block_reduce<NT>(m, OpMax(), red[2]);
 
     const T inv_t = (T)1 / (T)g.temperature;
     const bool two = g.temperature != 1.0 && (g.log_sums_out != nullptr || e.label >= 0);
     const Expo<T> ex(m, inv_t), ex1(m, (T)1);
-    T sum = 0, sum1 = 0;
+    T sum = ex(extra), sum1 = two ? ex1(extra) : (T)0;
+    Pass pass = Pass::fresh();
 #pragma unroll
     for (int r = 0; r < R; r++) {
         T v[N];
-        unpack<S>(raw[r], v);
+        unpack<S>(raw[r], v, pass);
 #pragma unroll
         for (int i = 0; i < N; i++)
             sum += ex(v[i]);
-        if (two) {
+        one_at_a_time();
+    }
+    if (two) {
+        pass = Pass::fresh();
+        const Expo<T> f1 = ex1.fresh();
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            T v[N];
+            unpack<S>(raw[r], v, pass);
 #pragma unroll
             for (int i = 0; i < N; i++)
-                sum1 += ex1(v[i]);
+                sum1 += f1(v[i]);
+            one_at_a_time();
         }
     }
     sum = block_reduce<NT>(sum, OpSum(), red[3]);
@@ -263,27 +278,37 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs g)
         }
         // Rows whose logits are all minus infinity have no probabilities.
         const T pq = cq == 0 || sum == 0 ? (T)0 : cq / sum, pl = cl == 0 || sum1 == 0 ? (T)0 : cl / sum1;
-        auto dense = [&](T v) {
-            T out = pq == 0 ? (T)0 : ex(v) * pq;
-            if (pl != 0)
-                out += ex1(v) * pl;
-            return out;
-        };
         S *grad = static_cast<S *>(g.grad) + row * g.grad_stride;
         __syncthreads(); // the entries' logits are read: the gradient may lie in the row's place
+        // The dense part; `value` gives it for one logit.
+        auto write = [&](auto value) {
 #pragma unroll
-        for (int r = 0; r < R; r++) {
-            T v[N];
-            unpack<S>(raw[r], v);
+            for (int r = 0; r < R; r++) {
+                T v[N];
+                unpack<S>(raw[r], v, pass);
 #pragma unroll
-            for (int i = 0; i < N; i++)
-                v[i] = dense(v[i]);
-            store_vec(grad, tid + r * NT, g.vocab, v);
-        }
+                for (int i = 0; i < N; i++)
+                    v[i] = value(v[i]);
+                if (tid + r * NT < whole)
+                    store_held(grad, r * NT, tid, pack<S>(v));
+                one_at_a_time();
+            }
+            if (has_rest)
+                grad[rest] = (S)value(extra);
+            __syncthreads();
+            fix_entries<NT>(g, grad, e, 0u, g.vocab, scale, value);
+        };
         for (uint32_t i = g.vocab + tid; i < g.grad_cols; i += NT)
             grad[i] = (S)0;
-        __syncthreads();
-        fix_entries<NT>(g, grad, e, 0u, g.vocab, scale, dense);
+        pass = Pass::fresh();
+        const Expo<T> fq = ex.fresh(), fl = ex1.fresh(), one = pq != 0 ? fq : fl;
+        const T p1 = pq != 0 ? pq : pl;
+        if (p1 == 0) // nothing asks for the row (or it has no probabilities)
+            write([](T) { return (T)0; });
+        else if (pq == 0 || pl == 0)
+            write([&](T v) { return one(v) * p1; });
+        else
+            write([&](T v) { return fq(v) * pq + fl(v) * pl; });
     }
 }
 
@@ -494,9 +519,13 @@ template <typename S> hipError_t launch_grad(hipStream_t s, const DistillArgs &g
     return hipGetLastError();
 }
 
-constexpr uint32_t kHeldVecs = 16 * 1024; // vectors of a row that one workgroup holds
+// Vectors of a row that one workgroup holds. Binary64 with 1024 threads would spill.
+template <typename S> constexpr uint32_t kHeldVecs = (sizeof(S) == 8 ? 512 : 1024) * 16;
 
-bool held(uint64_t rows, uint32_t vecs) { return vecs <= kHeldVecs && (rows >= 64 || vecs <= 1024); }
+template <typename S> bool held(uint64_t rows, uint32_t vecs)
+{
+    return vecs <= kHeldVecs<S> && (rows >= 64 || vecs <= 1024);
+}
 
 template <typename S> hipError_t launch_t(hipStream_t s, DistillArgs g, void *scratch)
 {
@@ -504,7 +533,7 @@ template <typename S> hipError_t launch_t(hipStream_t s, DistillArgs g, void *sc
     const uint32_t vecs = (g.vocab + kVec<S> - 1) / kVec<S>;
     if (g.log_sums_in)
         return launch_grad<S>(s, g, split_of(g.rows, vecs));
-    if (held(g.rows, vecs)) {
+    if (held<S>(g.rows, vecs)) {
         if (vecs <= 64 * 4)
             return launch_row<S, 64, 4>(s, g);
         if (vecs <= 256 * 4)
@@ -513,7 +542,8 @@ template <typename S> hipError_t launch_t(hipStream_t s, DistillArgs g, void *sc
             return launch_row<S, 256, 16>(s, g);
         if (vecs <= 512 * 16)
             return launch_row<S, 512, 16>(s, g);
-        return launch_row<S, 1024, 16>(s, g);
+        if constexpr (sizeof(S) < 8)
+            return launch_row<S, 1024, 16>(s, g);
     }
     const Split sp = split_of(g.rows, vecs);
     Partial<T> *parts = static_cast<Partial<T> *>(scratch);
@@ -536,7 +566,7 @@ template <typename S> size_t scratch_t(const DistillArgs &g)
 {
     using T = typename StatOf<S>::T;
     const uint32_t vecs = (g.vocab + kVec<S> - 1) / kVec<S>;
-    if (g.rows == 0 || g.log_sums_in || held(g.rows, vecs))
+    if (g.rows == 0 || g.log_sums_in || held<S>(g.rows, vecs))
         return 0;
     return g.rows * (split_of(g.rows, vecs).chunks * sizeof(Partial<T>) + 2 * sizeof(T));
 }

@@ -2,8 +2,9 @@
 //
 //   order: value descending, then index ascending (-0 equal to +0, NaN after minus infinity)
 //   log_sum = log sum_v exp(l_v / T)
-// The prefix (t, c) of k values is found digit by digit of the key; its values are then
-// gathered into LDS, the c values equal to t by index, and sorted there.
+// One workgroup a row, the row in registers where it fits: one read, the maximum and the sum of
+// exponentials, a bound from the maxima of groups of the row, the values that reach it gathered
+// and sorted in LDS (see pcu_select.hpp).
 #include "pcu_kernels.hpp"
 #include "pcu_select.hpp"
 
@@ -13,131 +14,153 @@ namespace pcu {
 
 namespace {
 
-// Sorts `size` (a power of two) entries, by key descending and index ascending; whole workgroup.
-template <int NT, typename K> __device__ __forceinline__ void sort_entries(K *key, uint32_t *at, uint32_t size)
+// The list's place for a row whose values beyond the bound do not fit it: the prefix of k values
+// found digit by digit, its entries gathered, those equal to t by index.
+template <typename S, int NT, typename K, int CAP>
+__device__ __forceinline__ void gather_exactly(const S *s, uint32_t n, uint32_t k, List<K, CAP> &list, uint32_t *bins,
+                                               Digit<uint32_t> *digit, uint32_t *wave_ties)
 {
-    for (uint32_t len = 2; len <= size; len <<= 1)
-        for (uint32_t gap = len >> 1; gap > 0; gap >>= 1) {
-            __syncthreads();
-            for (uint32_t p = threadIdx.x; p < size / 2; p += NT) {
-                const uint32_t a = 2 * p - (p & (gap - 1)), b = a + gap;
-                const K ka = key[a], kb = key[b];
-                const uint32_t ia = at[a], ib = at[b];
-                const bool ordered = ka > kb || (ka == kb && ia < ib);
-                if (ordered != ((a & len) == 0)) {
-                    key[a] = kb;
-                    key[b] = ka;
-                    at[a] = ib;
-                    at[b] = ia;
-                }
-            }
+    using T = typename StatOf<S>::T;
+    constexpr uint32_t N = kVec<S>, W = NT / 64;
+    const uint32_t wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+    const Prefix<K> top = select_count<S, NT>(s, n, k, bins, digit);
+    if (threadIdx.x == 0)
+        list.count = 0;
+    // Each wave's run of the row, in order: its values equal to t, then all entries.
+    const uint32_t vecs = (n + N - 1) / N, run = (vecs + W - 1) / W;
+    const uint32_t first = wave * run, last = first + run < vecs ? first + run : vecs;
+    uint32_t ties = 0;
+    wave_run(s, n, first, last, [&](const T *v, uint32_t, uint32_t count) {
+#pragma unroll
+        for (uint32_t i = 0; i < N; i++)
+            ties += i < count && key_of(v[i]) == top.t;
+        return false;
+    });
+    ties = wave_reduce(ties, OpSum());
+    if (lane == 0)
+        wave_ties[wave] = ties;
+    __syncthreads();
+    uint32_t before = 0;
+    for (uint32_t w = 0; w < wave; w++)
+        before += wave_ties[w];
+    wave_run(s, n, first, last, [&](const T *v, uint32_t at, uint32_t count) {
+        uint32_t own = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < N; i++)
+            own += i < count && key_of(v[i]) == top.t;
+        const uint32_t upto = wave_inclusive_sum(own);
+        uint32_t rank = before + upto - own;
+#pragma unroll
+        for (uint32_t i = 0; i < N; i++) {
+            const K x = key_of(v[i]);
+            if (i < count && (x > top.t || (x == top.t && rank < top.c)))
+                list.add(x, at + i);
+            rank += i < count && x == top.t;
         }
+        before += __shfl(upto, 63, 64);
+        return false;
+    });
     __syncthreads();
 }
 
-template <typename S, int NT> __global__ __launch_bounds__(NT) void k_top(TopArgs g)
+// G groups a thread: at least twice as many groups as k keeps the list short.
+template <typename S, int NT, int R, int G, int CAP> __global__ __launch_bounds__(NT) void k_top(TopArgs g)
 {
     using T = typename StatOf<S>::T;
     using K = typename KeyOf<T>::K;
     constexpr uint32_t N = kVec<S>;
-    constexpr uint32_t W = NT / 64;
     if (block_gate_closed(g.gate))
         return;
-    __shared__ uint32_t bins[256];
+    __shared__ BoundScratch bound;
     __shared__ Digit<uint32_t> digit;
-    __shared__ T red_m[16], red_s[16];
-    __shared__ uint32_t wave_ties[16], entries;
-    __shared__ K key[kLogitMaxK];
-    __shared__ uint32_t place[kLogitMaxK];
-    const uint32_t tid = threadIdx.x, wave = tid / 64, lane = tid & 63;
+    __shared__ T red[4][16];
+    __shared__ uint32_t wave_ties[16];
+    __shared__ List<K, CAP> list;
+    const uint32_t tid = threadIdx.x;
     const uint64_t row = blockIdx.x;
     const S *s = static_cast<const S *>(g.logits) + row * g.stride;
     const uint32_t n = g.vocab, k = g.k < n ? g.k : n;
+    const Row<S, NT, R> held(s, n);
 
-    if (g.log_sum) {
-        T m = -INFINITY;
-        each_vec<S, NT>(s, n, [&](const T *v, uint32_t, uint32_t) {
+    T group[G];
 #pragma unroll
-            for (uint32_t i = 0; i < N; i++)
-                m = OpMax()(m, v[i]);
-        });
-        m = block_reduce<NT>(m, OpMax(), red_m);
+    for (int i = 0; i < G; i++)
+        group[i] = -INFINITY;
+    group[0] = held.extra > -INFINITY ? held.extra : (T)-INFINITY;
+    held.walk([&](const T *v, uint32_t, int step) {
+        T top = v[0];
+#pragma unroll
+        for (uint32_t i = 1; i < N; i++)
+            top = OpMax()(top, v[i]);
+        group[step % G] = OpMax()(group[step % G], top);
+    });
+    T m = group[0];
+#pragma unroll
+    for (int i = 1; i < G; i++)
+        m = OpMax()(m, group[i]);
+    m = block_reduce<NT>(m, OpMax(), red[0]);
+    if (g.log_sum) {
         const Expo<T> ex(m, (T)1 / (T)g.temperature);
-        T sum = 0;
-        each_vec<S, NT>(s, n, [&](const T *v, uint32_t, uint32_t) {
+        T sum = ex(held.extra);
+        held.walk([&](const T *v, uint32_t, int) {
 #pragma unroll
             for (uint32_t i = 0; i < N; i++)
                 sum += ex(v[i]);
         });
-        sum = block_reduce<NT>(sum, OpSum(), red_s);
+        sum = block_reduce<NT>(sum, OpSum(), red[1]);
         if (tid == 0)
             static_cast<T *>(g.log_sum)[row] = ex.log_sum(sum);
     }
-    uint32_t size = 1;
-    while (size < k)
-        size <<= 1;
     if (k > 0) {
-        const Prefix<K> top = select_count<S, NT>(s, n, k, bins, &digit);
-        for (uint32_t j = tid; j < size; j += NT) {
-            key[j] = 0;
-            place[j] = 0xffffffffu; // after every entry of the same key
-        }
         if (tid == 0)
-            entries = 0;
-        // Each wave's run of the row, in order: its values equal to t, then all entries.
-        const uint32_t vecs = (n + N - 1) / N, run = (vecs + W - 1) / W;
-        const uint32_t first = wave * run, last = first + run < vecs ? first + run : vecs;
-        uint32_t ties = 0;
-        wave_run(s, n, first, last, [&](const T *v, uint32_t, uint32_t count) {
+            list.count = 0;
+        const T t = bound_of<NT>(group, m, k, bound, red[2]); // its barriers order the count
+        held.walk([&](const T *v, uint32_t at, int) {
 #pragma unroll
             for (uint32_t i = 0; i < N; i++)
-                ties += i < count && key_of(v[i]) == top.t;
-            return false;
+                if (v[i] >= t && at < held.whole * N) // a held vector past the row is all minus infinity
+                    list.add(key_of(v[i]), at + i);
         });
-        ties = wave_reduce(ties, OpSum());
-        if (lane == 0)
-            wave_ties[wave] = ties;
+        if (held.has_extra && held.extra >= t)
+            list.add(key_of(held.extra), held.extra_at());
         __syncthreads();
-        uint32_t before = 0;
-        for (uint32_t w = 0; w < wave; w++)
-            before += wave_ties[w];
-        wave_run(s, n, first, last, [&](const T *v, uint32_t at, uint32_t count) {
-            uint32_t own = 0;
-#pragma unroll
-            for (uint32_t i = 0; i < N; i++)
-                own += i < count && key_of(v[i]) == top.t;
-            const uint32_t upto = wave_inclusive_sum(own);
-            uint32_t rank = before + upto - own;
-#pragma unroll
-            for (uint32_t i = 0; i < N; i++) {
-                const K x = key_of(v[i]);
-                if (i < count && (x > top.t || (x == top.t && rank < top.c))) {
-                    const uint32_t j = atomicAdd(&entries, 1u);
-                    key[j] = x;
-                    place[j] = at + i;
-                }
-                rank += i < count && x == top.t;
-            }
-            before += __shfl(upto, 63, 64);
-            return false;
-        });
-        sort_entries<NT>(key, place, size);
+        // Fewer than k: the rest of the row are NaNs.
+        uint32_t found = list.count;
+        __syncthreads();
+        if (found > CAP || found < k) {
+            gather_exactly<S, NT>(s, n, k, list, bound.bins, &digit, wave_ties);
+            found = k;
+        }
+        sort_list<NT>(list, found);
     }
     S *values = static_cast<S *>(g.values) + row * g.k;
     int32_t *indices = g.indices + row * g.k;
     for (uint32_t j = tid; j < g.k; j += NT) {
-        values[j] = j < k ? s[place[j]] : (S)-INFINITY;
-        indices[j] = j < k ? (int32_t)place[j] : -1;
+        values[j] = j < k ? s[list.at[j]] : (S)-INFINITY;
+        indices[j] = j < k ? (int32_t)list.at[j] : -1;
     }
+}
+
+template <typename S, int NT, int R> hipError_t launch_row(hipStream_t s, const TopArgs &g)
+{
+    const dim3 grid((unsigned)g.rows), block(NT);
+    if (g.k * 4 <= NT)
+        hipLaunchKernelGGL((k_top<S, NT, R, 1, 512>), grid, block, 0, s, g);
+    else
+        hipLaunchKernelGGL((k_top<S, NT, R, 4, 2048>), grid, block, 0, s, g);
+    return hipGetLastError();
 }
 
 template <typename S> hipError_t launch_t(hipStream_t s, const TopArgs &g)
 {
-    if (g.vocab <= 8192)
-        hipLaunchKernelGGL((k_top<S, 256>), dim3((unsigned)g.rows), dim3(256), 0, s, g);
-    else
-        hipLaunchKernelGGL((k_top<S, 1024>), dim3((unsigned)g.rows), dim3(1024), 0, s, g);
-    return hipGetLastError();
+    const uint32_t vecs = g.vocab / kVec<S>;
+    if (vecs <= 256 * 4)
+        return launch_row<S, 256, 4>(s, g);
+    if (vecs <= 256 * 16 && g.k <= 256)
+        return launch_row<S, 256, 16>(s, g);
+    if (vecs <= 1024 * 16)
+        return launch_row<S, 1024, 16>(s, g);
+    return launch_row<S, 1024, 0>(s, g);
 }
 
 } // namespace

@@ -24,7 +24,21 @@ typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
 template <typename S> constexpr int kVec = 16 / (int)sizeof(S);
 
-template <typename S> __device__ __forceinline__ void unpack(const u32x4 &raw, typename StatOf<S>::T *out)
+// One pass over a row that a thread holds in registers. The compiler would keep what one pass
+// unpacks for the next (twice the registers for 16-bit rows, and spills), so each pass unpacks with
+// constants that it does not know to be those of the pass before.
+struct Pass {
+    uint32_t shift = 16, upper = 0xffff0000u, zero = 0;
+    static __device__ __forceinline__ Pass fresh()
+    {
+        Pass p;
+        asm volatile("" : "+s"(p.shift), "+s"(p.upper), "+s"(p.zero));
+        return p;
+    }
+};
+
+template <typename S>
+__device__ __forceinline__ void unpack(const u32x4 &raw, typename StatOf<S>::T *out, const Pass &p = Pass{})
 {
     if constexpr (sizeof(S) == 8) {
 #pragma unroll
@@ -37,17 +51,21 @@ template <typename S> __device__ __forceinline__ void unpack(const u32x4 &raw, t
     } else if constexpr (__is_same(S, __bf16)) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            out[2 * i] = __uint_as_float(raw[i] << 16);
-            out[2 * i + 1] = __uint_as_float(raw[i] & 0xffff0000u);
+            out[2 * i] = __uint_as_float(raw[i] << p.shift);
+            out[2 * i + 1] = __uint_as_float(raw[i] & p.upper);
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            out[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)raw[i]);
-            out[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(raw[i] >> 16));
+            const uint32_t w = raw[i] | p.zero;
+            out[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)w);
+            out[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> 16));
         }
     }
 }
+
+// Between the vectors of a held row: the scheduler otherwise unpacks many of them at once.
+__device__ __forceinline__ void one_at_a_time() { __builtin_amdgcn_sched_barrier(0); }
 
 // Values rounded once (to nearest even) to the row's type.
 template <typename S> __device__ __forceinline__ u32x4 pack(const typename StatOf<S>::T *v)
@@ -88,13 +106,42 @@ template <typename S> __device__ __forceinline__ u32x4 minus_infinities()
         return u32x4{0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u};
 }
 
+// Whole vector i of a row. The 32-bit byte offset (a row has at most 2^22 values) lets the
+// row's address stay in scalar registers.
+template <typename S> __device__ __forceinline__ u32x4 load_whole(const S *row, uint32_t i)
+{
+    return *reinterpret_cast<const u32x4_any *>(reinterpret_cast<const char *>(row) + i * 16u);
+}
+template <typename S> __device__ __forceinline__ void store_whole(S *row, uint32_t i, const u32x4 &raw)
+{
+    *reinterpret_cast<u32x4_any *>(reinterpret_cast<char *>(row) + i * 16u) = raw;
+}
+
+// The same where a thread holds many vectors of the row: vector `step` + i, `step` the same for
+// the workgroup. The address of the step is kept scalar and unknown to the compiler, which
+// otherwise adds every step to a 64-bit address in vector registers and keeps those.
+template <typename S> __device__ __forceinline__ u32x4 load_held(const S *row, uint32_t step, uint32_t i)
+{
+    typedef const __attribute__((address_space(1))) char *P;
+    P base = (P) reinterpret_cast<const char *>(row) + step * 16u;
+    asm volatile("" : "+s"(base));
+    return *(const __attribute__((address_space(1))) u32x4_any *)(base + i * 16u);
+}
+template <typename S> __device__ __forceinline__ void store_held(S *row, uint32_t step, uint32_t i, const u32x4 &raw)
+{
+    typedef __attribute__((address_space(1))) char *P;
+    P base = (P) reinterpret_cast<char *>(row) + step * 16u;
+    asm volatile("" : "+s"(base));
+    *(__attribute__((address_space(1))) u32x4_any *)(base + i * 16u) = raw;
+}
+
 // Vector i of a row of n values; places past the row's end read as minus infinity, whole
 // vectors past it too.
 template <typename S> __device__ __forceinline__ u32x4 load_vec(const S *row, uint32_t i, uint32_t n)
 {
     const uint32_t at = i * kVec<S>;
     if (at + kVec<S> <= n)
-        return *reinterpret_cast<const u32x4_any *>(row + at);
+        return load_whole(row, i);
     u32x4 raw = minus_infinities<S>();
     if (at < n) {
         if constexpr (sizeof(S) == 2) {
@@ -123,7 +170,7 @@ __device__ __forceinline__ void store_vec(S *row, uint32_t i, uint32_t n, const 
 {
     const uint32_t at = i * kVec<S>;
     if (at + kVec<S> <= n) {
-        *reinterpret_cast<u32x4_any *>(row + at) = pack<S>(v);
+        store_whole(row, i, pack<S>(v));
     } else {
 #pragma unroll
         for (int e = 0; e < kVec<S>; e++)
@@ -180,6 +227,13 @@ template <> struct Expo<float> {
     float m, inv_t, c;
     __device__ __forceinline__ Expo(float mx, float it) : m(mx == -INFINITY ? 0.0f : mx), inv_t(it), c(it * kLog2e) {}
     __device__ __forceinline__ float operator()(float s) const { return exp2_fast((s - m) * c); }
+    // The same function for another pass (see Pass): its differences are not kept either.
+    __device__ __forceinline__ Expo fresh() const
+    {
+        Expo e = *this;
+        asm volatile("" : "+v"(e.m));
+        return e;
+    }
     // log(sum of exp(s / T)) from the sum of the above.
     __device__ __forceinline__ float log_sum(float sum) const
     {
@@ -190,6 +244,12 @@ template <> struct Expo<double> {
     double inv_t, m;
     __device__ __forceinline__ Expo(double mx, double it) : inv_t(it), m(mx == -INFINITY ? 0.0 : mx) {}
     __device__ __forceinline__ double operator()(double s) const { return exp((s - m) * inv_t); }
+    __device__ __forceinline__ Expo fresh() const
+    {
+        Expo e = *this;
+        asm volatile("" : "+v"(e.m));
+        return e;
+    }
     __device__ __forceinline__ double log_sum(double sum) const { return m * inv_t + log(sum); }
 };
 
