@@ -205,8 +205,6 @@ pcu_status Ctx::op_sample(const pcu_logits *l, const pcu_sampling *p, int32_t *t
     unsigned long long *word;
     if ((st = add_node(NodeInfo{Prim::Checked, l->rows, 0}, &word)))
         return st;
-    if ((st = open_words()))
-        return st;
     SampleArgs g;
     g.logits = l->data;
     g.dtype = (int)l->dtype;
@@ -226,8 +224,14 @@ pcu_status Ctx::op_sample(const pcu_logits *l, const pcu_sampling *p, int32_t *t
     g.log_prob = log_prob;
     g.fault = word;
     g.gate = gate_for(word);
+    void *sc = nullptr;
+    const size_t need = sample_scratch_bytes(g);
+    if (need && (st = scratch(logits_scratch, need, false, &sc)))
+        return st;
+    if ((st = open_words()))
+        return st;
     hipEvent_t ev = timer_start(stream);
-    st = hip(launch_sample(stream, g), "sample launch");
+    st = hip(launch_sample(stream, g, sc), "sample launch");
     timer_stop(PCU_KERNEL_SAMPLE, ev, stream);
     return st;
 }

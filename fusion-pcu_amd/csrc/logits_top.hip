@@ -57,7 +57,7 @@ __device__ __forceinline__ void gather_exactly(const S *s, uint32_t n, uint32_t 
                 list.add(x, at + i);
             rank += i < count && x == top.t;
         }
-        before += __shfl(upto, 63, 64);
+        before += from_lane(upto, 63);
         return false;
     });
     __syncthreads();

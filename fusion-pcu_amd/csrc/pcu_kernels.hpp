@@ -347,10 +347,12 @@ struct SampleArgs {
     int32_t top_k_all = 0;
     int32_t *tokens = nullptr;
     float *log_prob = nullptr; // or null
+    uint64_t first_row = 0; // of the call's rows, for the fault's ordinal
     unsigned long long *fault = nullptr;
     NodeGate gate{nullptr, 0};
 };
-hipError_t launch_sample(hipStream_t s, const SampleArgs &g);
+size_t sample_scratch_bytes(const SampleArgs &g);
+hipError_t launch_sample(hipStream_t s, const SampleArgs &g, void *scratch);
 
 // Small device utilities (fill kernels rather than memsets, so a captured graph replays
 // them as kernels).

@@ -181,19 +181,58 @@ __device__ __forceinline__ void store_vec(S *row, uint32_t i, uint32_t n, const 
 
 // --------------------------------------------------------- reductions of a workgroup
 struct OpMax {
+    template <typename T> __device__ __forceinline__ T none() const { return (T)-INFINITY; }
     __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
     __device__ __forceinline__ double operator()(double a, double b) const { return fmax(a, b); }
 };
 struct OpSum {
+    template <typename T> __device__ __forceinline__ T none() const { return (T)0; }
     template <typename T> __device__ __forceinline__ T operator()(T a, T b) const { return a + b; }
 };
+struct OpOr {
+    template <typename T> __device__ __forceinline__ T none() const { return (T)0; }
+    template <typename T> __device__ __forceinline__ T operator()(T a, T b) const { return a | b; }
+};
 
+// v of the lane that DPP control C names, `none` where there is none or row mask M leaves the
+// lane's row of 16 out.
+template <int C, int M, typename T> __device__ __forceinline__ T dpp(T none, T v)
+{
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v), C, M, 0xf, false));
+    } else {
+        const uint64_t n = __builtin_bit_cast(uint64_t, none), x = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp((int)(uint32_t)n, (int)(uint32_t)x, C, M, 0xf, false);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp((int)(n >> 32), (int)(x >> 32), C, M, 0xf, false);
+        return __builtin_bit_cast(T, (uint64_t)hi << 32 | lo);
+    }
+}
+// v folded over lanes 0 .. own, in one fixed order (`none` is op's neutral value). Shifts within
+// rows of 16 lanes, then the rows' totals handed on: no LDS.
+template <typename T, typename Op> __device__ __forceinline__ T wave_upto(T v, Op op, T none)
+{
+    v = op(dpp<0x111, 0xf>(none, v), v); // row_shr:1
+    v = op(dpp<0x112, 0xf>(none, v), v);
+    v = op(dpp<0x114, 0xf>(none, v), v);
+    v = op(dpp<0x118, 0xf>(none, v), v);
+    v = op(dpp<0x142, 0xa>(none, v), v); // row_bcast:15 to rows 1 and 3
+    v = op(dpp<0x143, 0xc>(none, v), v); // row_bcast:31 to rows 2 and 3
+    return v;
+}
+template <typename T> __device__ __forceinline__ T from_lane(T v, int lane)
+{
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+    } else {
+        const uint64_t x = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, lane);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane);
+        return __builtin_bit_cast(T, (uint64_t)hi << 32 | lo);
+    }
+}
 template <typename T, typename Op> __device__ __forceinline__ T wave_reduce(T v, Op op)
 {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1)
-        v = op(v, __shfl_xor(v, off, 64));
-    return v;
+    return from_lane(wave_upto(v, op, op.template none<T>()), 63);
 }
 
 // Every thread gets the result, folded in one fixed order. `lds`: NT / 64 entries that no

@@ -58,17 +58,7 @@ template <typename K> struct Prefix {
 
 // ------------------------------------------------------------------- scans of a wave
 
-template <typename T> __device__ __forceinline__ T wave_inclusive_sum(T v)
-{
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const T o = __shfl_up(v, off, 64);
-        if (lane >= off)
-            v += o;
-    }
-    return v;
-}
+template <typename T> __device__ __forceinline__ T wave_inclusive_sum(T v) { return wave_upto(v, OpSum(), (T)0); }
 
 // --------------------------------------------------------------------- the row
 
@@ -175,8 +165,8 @@ template <typename S, int NT, int R> struct Row {
 // ------------------------------------------------------------------- a short list
 
 template <typename K, int CAP> struct List {
-    K key[CAP];
-    uint32_t at[CAP];
+    __attribute__((aligned(16))) K key[CAP];
+    __attribute__((aligned(16))) uint32_t at[CAP];
     uint32_t count; // may pass CAP: then the list is not whole
 
     __device__ __forceinline__ void add(K k, uint32_t i)
@@ -195,14 +185,28 @@ template <int NT, typename K, int CAP> __device__ __forceinline__ void sort_list
 {
     // Few entries: each finds its place by counting those before it.
     if (n <= 256 && n <= NT) {
+        constexpr uint32_t kAtOnce = 8; // reads in flight
+        if (threadIdx.x < kAtOnce) {
+            l.key[n + threadIdx.x] = 0;
+            l.at[n + threadIdx.x] = 0xffffffffu;
+        }
+        __syncthreads();
         K k = 0;
         uint32_t i = 0, place = 0;
         if (threadIdx.x < n) {
             k = l.key[threadIdx.x];
             i = l.at[threadIdx.x];
-            for (uint32_t j = 0; j < n; j++) {
-                const K o = l.key[j];
-                place += o > k || (o == k && l.at[j] < i);
+            for (uint32_t j = 0; j < n; j += kAtOnce) {
+                K o[kAtOnce];
+                uint32_t a[kAtOnce];
+#pragma unroll
+                for (uint32_t u = 0; u < kAtOnce; u++) {
+                    o[u] = l.key[j + u];
+                    a[u] = l.at[j + u];
+                }
+#pragma unroll
+                for (uint32_t u = 0; u < kAtOnce; u++)
+                    place += o[u] > k || (o[u] == k && a[u] < i);
             }
         }
         __syncthreads();
@@ -237,6 +241,125 @@ template <int NT, typename K, int CAP> __device__ __forceinline__ void sort_list
             }
         }
     __syncthreads();
+}
+
+// ------------------------------------------------------------- one entry of many
+
+// Among 256 bins, from the highest down: the bin in which the running sum reaches `need`
+// (1 <= need <= the sum of all), and what of `need` is left before it. Whole workgroup.
+template <typename H> struct Digit {
+    uint32_t digit;
+    H left;
+};
+template <typename H> __device__ __forceinline__ Digit<H> find_digit(const H *bins, H need, Digit<H> *out)
+{
+    __syncthreads(); // the bins are counted
+    if (threadIdx.x < 64) {
+        const int top = 255 - 4 * (int)threadIdx.x;
+        H b[4], own = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            b[i] = bins[top - i];
+            own += b[i];
+        }
+        const H upto = wave_inclusive_sum(own);
+        H before = upto - own;
+        if (before < need && need <= upto) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (before < need && need <= before + b[i])
+                    *out = Digit<H>{(uint32_t)(top - i), need - before};
+                before += b[i];
+            }
+        }
+    }
+    __syncthreads();
+    return *out;
+}
+
+
+// Entries (key, index) that a workgroup holds, PER a thread.
+template <typename K, int PER> struct Held {
+    K key[PER];
+    uint32_t at[PER];
+};
+template <typename K> struct SelectShared {
+    Digit<unsigned long long> digit;
+    unsigned long long bins[256];
+    K varying[2][16];
+    uint32_t left[16];
+    K key;
+    uint32_t at;
+};
+
+// In the order (key descending, index ascending), or by index alone (BY_INDEX), the entry at which
+// the running sum of the measures reaches `need` (1 <= need <= their sum; entries of measure 0 do
+// not count): its key and index in sh, after a barrier. 8 bits a step, from the highest bit in
+// which the keys differ, until one entry is left.
+template <int NT, bool BY_INDEX, typename K, int PER>
+__device__ __forceinline__ void select_entry(const Held<K, PER> &e, const unsigned long long (&measure)[PER],
+                                             unsigned long long need, int index_bits, SelectShared<K> &sh)
+{
+    bool in[PER];
+#pragma unroll
+    for (int b = 0; b < PER; b++)
+        in[b] = measure[b] != 0;
+    int shift = index_bits > 8 ? index_bits - 8 : 0;
+    bool by_key = !BY_INDEX;
+    if (by_key) {
+        K some = 0, all = 0; // bits set in some key, bits clear in some key
+#pragma unroll
+        for (int b = 0; b < PER; b++)
+            if (in[b]) {
+                some |= e.key[b];
+                all |= ~e.key[b];
+            }
+        some = block_reduce<NT>(some, OpOr(), sh.varying[0]);
+        all = block_reduce<NT>(all, OpOr(), sh.varying[1]);
+        const K varying = some & all;
+        const int top = varying == 0 ? -1 : (sizeof(K) == 8 ? 63 - __builtin_clzll(varying) : 31 - __builtin_clz((uint32_t)varying));
+        if (top < 0)
+            by_key = false;
+        else
+            shift = top > 7 ? top - 7 : 0;
+    }
+    for (int step = 0; step < (int)sizeof(K) + 4; step++) { // at most every byte of a key and an index
+        for (uint32_t b = threadIdx.x; b < 256; b += NT)
+            sh.bins[b] = 0;
+        __syncthreads();
+        uint32_t digit[PER];
+#pragma unroll
+        for (int b = 0; b < PER; b++) {
+            digit[b] = (by_key ? (uint32_t)(e.key[b] >> shift) : ~e.at[b] >> shift) & 255u;
+            if (in[b])
+                atomicAdd(&sh.bins[digit[b]], measure[b]);
+        }
+        const Digit<unsigned long long> d = find_digit(sh.bins, need, &sh.digit);
+        need = d.left;
+        uint32_t left = 0;
+#pragma unroll
+        for (int b = 0; b < PER; b++) {
+            in[b] = in[b] && digit[b] == d.digit;
+            left += in[b];
+        }
+        left = block_reduce<NT>(left, OpSum(), sh.left);
+        if (left == 1) {
+#pragma unroll
+            for (int b = 0; b < PER; b++)
+                if (in[b]) {
+                    sh.key = e.key[b];
+                    sh.at = e.at[b];
+                }
+            __syncthreads();
+            return;
+        }
+        if (shift > 0) {
+            shift = shift > 8 ? shift - 8 : 0;
+        } else { // equal keys: by index
+            by_key = false;
+            shift = index_bits > 8 ? index_bits - 8 : 0;
+        }
+    }
 }
 
 // What a bound's search keeps in LDS.
@@ -305,38 +428,6 @@ __device__ __forceinline__ T bound_of(const T (&group)[G], T m, uint32_t k, Boun
 }
 
 // ---------------------------------------------------------------- digit by digit
-
-// Among 256 bins, from the highest down: the bin in which the running sum reaches `need`
-// (1 <= need <= the sum of all), and what of `need` is left before it. Whole workgroup.
-template <typename H> struct Digit {
-    uint32_t digit;
-    H left;
-};
-template <typename H> __device__ __forceinline__ Digit<H> find_digit(const H *bins, H need, Digit<H> *out)
-{
-    __syncthreads(); // the bins are counted
-    if (threadIdx.x < 64) {
-        const int top = 255 - 4 * (int)threadIdx.x;
-        H b[4], own = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            b[i] = bins[top - i];
-            own += b[i];
-        }
-        const H upto = wave_inclusive_sum(own);
-        H before = upto - own;
-        if (before < need && need <= upto) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (before < need && need <= before + b[i])
-                    *out = Digit<H>{(uint32_t)(top - i), need - before};
-                before += b[i];
-            }
-        }
-    }
-    __syncthreads();
-    return *out;
-}
 
 // The prefix of `k` values (1 <= k <= n).
 template <typename S, int NT>
