@@ -224,14 +224,24 @@ pcu_status Ctx::op_sample(const pcu_logits *l, const pcu_sampling *p, int32_t *t
     g.log_prob = log_prob;
     g.fault = word;
     g.gate = gate_for(word);
-    void *sc = nullptr;
+    void *sc = nullptr, *state = nullptr;
     const size_t need = sample_scratch_bytes(g);
     if (need && (st = scratch(logits_scratch, need, false, &sc)))
+        return st;
+    if (need && (st = scratch(sample_state, sample_state_bytes(), false, &state)))
         return st;
     if ((st = open_words()))
         return st;
     hipEvent_t ev = timer_start(stream);
-    st = hip(launch_sample(stream, g, sc), "sample launch");
+    if (need && !sample_state_zero) {
+        if ((st = hip(launch_fill_u64(stream, static_cast<unsigned long long *>(state), sample_state_bytes() / 8, 0),
+                      "sample state")))
+            return st;
+        sample_state_zero = true;
+    }
+    st = hip(launch_sample(stream, g, sc, state), "sample launch");
+    if (st)
+        sample_state_zero = false;
     timer_stop(PCU_KERNEL_SAMPLE, ev, stream);
     return st;
 }

@@ -118,7 +118,6 @@ __device__ __forceinline__ Prefix<K> select_mass(const S *row, uint32_t n, Prefi
     return {prefix, (uint32_t)((need + w - 1) / w)};
 }
 
-constexpr int kPerThread = 8; // entries of a list that a thread holds
 constexpr uint32_t kSteps = 1024; // of a row's weights in the nucleus search
 
 // The last token of a prefix of the order: kept are the values above `value`, and those equal to it
@@ -177,7 +176,7 @@ __device__ __forceinline__ Last<typename StatOf<S>::T> last_of(const S *s, uint3
 template <typename T, int NT> struct DrawShared {
     Digit<uint32_t> count_digit;
     Digit<mass_t> mass_digit;
-    mass_t red[4][16];
+    mass_t red[4][16], tiles[64];
     uint32_t wave_ties[16], found_at, end;
     SelectShared<typename KeyOf<T>::K> select;
     mass_t steps[kSteps]; // masses of the steps of z, then bins of other searches
@@ -242,37 +241,24 @@ __device__ __forceinline__ End find_end(DrawShared<T, NT> &sh, uint32_t part)
     return {need, sh.mass_digit.left, sh.end};
 }
 
-// A list in registers, with the weights of its entries.
-template <typename T> struct Entries {
-    Held<typename KeyOf<T>::K, kPerThread> e;
-    mass_t w[kPerThread];
-    template <int NT, typename W>
-    __device__ __forceinline__ Entries(const typename KeyOf<T>::K *key, const uint32_t *at, uint32_t count, const W &weight,
-                                       std::integral_constant<int, NT>)
+// One entry of a list, and a list in LDS or in global memory (written by other workgroups of the
+// launch, so read past the caches that they do not share).
+template <typename K> struct Entry {
+    K key;
+    uint32_t at;
+};
+template <typename K> struct LocalList {
+    const K *key;
+    const uint32_t *at;
+    __device__ __forceinline__ Entry<K> operator()(uint32_t j) const { return {key[j], at[j]}; }
+};
+template <typename K> struct SharedList {
+    const K *key;
+    const uint32_t *at;
+    __device__ __forceinline__ Entry<K> operator()(uint32_t j) const
     {
-#pragma unroll
-        for (int b = 0; b < kPerThread; b++) {
-            const uint32_t j = threadIdx.x + b * NT;
-            e.key[b] = j < count ? key[j] : 0;
-            e.at[b] = j < count ? at[j] : 0xffffffffu;
-            w[b] = j < count ? weight(value_of(e.key[b])) : 0;
-        }
-    }
-    template <int NT> __device__ __forceinline__ mass_t mass(mass_t *lds) const
-    {
-        mass_t sum = 0;
-#pragma unroll
-        for (int b = 0; b < kPerThread; b++)
-            sum += w[b];
-        return block_reduce<NT>(sum, OpSum(), lds);
-    }
-    // Leaves the entries up to `last` of the order.
-    template <typename K> __device__ __forceinline__ void cut(K key, uint32_t at)
-    {
-#pragma unroll
-        for (int b = 0; b < kPerThread; b++)
-            if (!(e.key[b] > key || (e.key[b] == key && e.at[b] <= at)))
-                w[b] = 0;
+        return {__hip_atomic_load(key + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
+                __hip_atomic_load(at + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)};
     }
 };
 __device__ __forceinline__ int index_bits(uint32_t n) { return n > 1 ? 32 - __builtin_clz(n - 1) : 1; }
@@ -286,107 +272,221 @@ __device__ __forceinline__ Last<T> nucleus_exactly(const S *s, uint32_t n, Prefi
     return last_of<S, NT>(s, n, pp, sh.wave_ties, &sh.found_at);
 }
 
+// The mass of the list's entries.
+template <int NT, typename L, typename M> __device__ __forceinline__ mass_t mass_of_list(uint32_t count, L list, M measure, mass_t *lds)
+{
+    mass_t sum = 0;
+    for (uint32_t j = threadIdx.x; j < count; j += NT) {
+        const auto e = list(j);
+        sum += measure(e.key, e.at);
+    }
+    return block_reduce<NT>(sum, OpSum(), lds);
+}
+
+constexpr uint32_t kFew = 128; // entries that are drawn from one a thread
+
+// Draws from a list of at most kFew entries in LDS, one a thread, which holds the first top_k of the order
+// (or all of it that is finite): each entry counts the entries before it in the order with
+// their mass, and then, among the kept ones, the mass before it by index. `w`: NT + 4 places.
+// need: what the nucleus has to hold, 0 for `part` of the mass of the first top_k.
+template <int NT, typename K, typename W>
+__device__ __forceinline__ void draw_from_few(const SampleArgs &g, uint64_t row, const Settings &set, K *key, uint32_t *at,
+                                              uint32_t count, mass_t need, const W &weight, mass_t *w, mass_t *red)
+{
+    constexpr uint32_t kAtOnce = 4; // reads in flight
+    const uint32_t tid = threadIdx.x;
+    const bool in = tid < count;
+    const K k = in ? key[tid] : 0;
+    const uint32_t i = in ? at[tid] : 0xffffffffu;
+    mass_t own = in ? weight(value_of(k)) : 0;
+    w[tid] = own;
+    if (tid < kAtOnce) {
+        key[count + tid] = 0; // after every entry
+        at[count + tid] = 0xffffffffu;
+        if (count + tid >= NT)
+            w[count + tid] = 0;
+    }
+    __syncthreads();
+    uint32_t rank = 0;
+    mass_t before = 0;
+    for (uint32_t j = 0; j < count; j += kAtOnce) {
+        K o[kAtOnce];
+        uint32_t a[kAtOnce];
+        mass_t x[kAtOnce];
+#pragma unroll
+        for (uint32_t u = 0; u < kAtOnce; u++) {
+            o[u] = key[j + u];
+            a[u] = at[j + u];
+            x[u] = w[j + u];
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kAtOnce; u++) {
+            const bool earlier = (o[u] > k) | ((o[u] == k) & (a[u] < i));
+            rank += earlier;
+            before += earlier ? x[u] : 0;
+        }
+    }
+    if (rank >= set.k)
+        own = 0;
+    if (set.nucleus()) {
+        if (need == 0) {
+            need = share_of(block_reduce<NT>(own, OpSum(), red), set.part);
+            need = need ? need : 1;
+        }
+        if (before >= need)
+            own = 0;
+    }
+    if (own < set.least)
+        own = 0;
+    const mass_t total = block_reduce<NT>(own, OpSum(), red + 16); // its barrier: the weights are read
+    w[tid] = own;
+    __syncthreads();
+    mass_t running = 0;
+    for (uint32_t j = 0; j < count; j += kAtOnce) {
+        uint32_t a[kAtOnce];
+        mass_t x[kAtOnce];
+#pragma unroll
+        for (uint32_t u = 0; u < kAtOnce; u++) {
+            a[u] = at[j + u];
+            x[u] = w[j + u];
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kAtOnce; u++)
+            running += a[u] < i ? x[u] : 0;
+    }
+    const mass_t target = share_of(total, set.draw);
+    if (running <= target && target < running + own) {
+        g.tokens[row] = (int32_t)i;
+        if (g.log_prob)
+            g.log_prob[row] = logf((float)own / (float)total);
+    }
+}
+
 // Draws from a list of `count` entries, which holds the first top_k of the order (or all of it that is
 // finite). need: what the nucleus has to hold, 0 for `part` of their mass.
-template <typename T, int NT, typename W>
-__device__ __forceinline__ void draw_from_list(const SampleArgs &g, uint64_t row, const Settings &set,
-                                               const typename KeyOf<T>::K *key, const uint32_t *at, uint32_t count,
+template <typename T, int NT, typename L, typename W>
+__device__ __forceinline__ void draw_from_list(const SampleArgs &g, uint64_t row, const Settings &set, L list, uint32_t count,
                                                mass_t need, const W &weight, DrawShared<T, NT> &sh)
 {
+    using K = typename KeyOf<T>::K;
     const int bits = index_bits(g.vocab);
-    Entries<T> list(key, at, count, weight, std::integral_constant<int, NT>());
+    // Kept are the entries up to this one of the order.
+    K last_key = 0;
+    uint32_t last_at = 0xffffffffu;
+    auto kept = [&](K key, uint32_t at) -> mass_t {
+        return key > last_key || (key == last_key && at <= last_at) ? weight(value_of(key)) : 0;
+    };
     if (count > set.k) {
-        mass_t one[kPerThread];
-#pragma unroll
-        for (int b = 0; b < kPerThread; b++)
-            one[b] = threadIdx.x + b * NT < count;
-        select_entry<NT, false>(list.e, one, set.k, bits, sh.select);
-        list.cut(sh.select.key, sh.select.at);
+        select_entry<NT, false>(count, list, [](K, uint32_t) -> mass_t { return 1; }, set.k, bits, sh.select);
+        last_key = sh.select.key;
+        last_at = sh.select.at;
     }
     if (set.nucleus()) {
         if (need == 0) {
-            need = share_of(list.template mass<NT>(sh.red[0]), set.part);
+            need = share_of(mass_of_list<NT>(count, list, kept, sh.red[0]), set.part);
             need = need ? need : 1;
         }
-        select_entry<NT, false>(list.e, list.w, need, bits, sh.select);
-        list.cut(sh.select.key, sh.select.at);
+        select_entry<NT, false>(count, list, kept, need, bits, sh.select);
+        last_key = sh.select.key;
+        last_at = sh.select.at;
     }
-#pragma unroll
-    for (int b = 0; b < kPerThread; b++)
-        list.w[b] = list.w[b] >= set.least ? list.w[b] : 0;
+    auto drawn = [&](K key, uint32_t at) -> mass_t {
+        const mass_t w = kept(key, at);
+        return w >= set.least ? w : 0;
+    };
     // The first by index at which the running mass passes the target.
-    const mass_t total = list.template mass<NT>(sh.red[1]);
-    select_entry<NT, true>(list.e, list.w, share_of(total, set.draw) + 1, bits, sh.select);
-#pragma unroll
-    for (int b = 0; b < kPerThread; b++)
-        if (list.w[b] && list.e.at[b] == sh.select.at) {
-            g.tokens[row] = (int32_t)list.e.at[b];
-            if (g.log_prob)
-                g.log_prob[row] = logf((float)list.w[b] / (float)total);
-        }
+    const mass_t total = mass_of_list<NT>(count, list, drawn, sh.red[1]);
+    select_entry<NT, true>(count, list, drawn, share_of(total, set.draw) + 1, bits, sh.select);
+    if (threadIdx.x == 0) {
+        g.tokens[row] = (int32_t)sh.select.at;
+        if (g.log_prob)
+            g.log_prob[row] = logf((float)weight(value_of(sh.select.key)) / (float)total);
+    }
 }
 
 // Draws along vectors [from, to) of the row (`mass_of` a value and its index). total 0: the vectors
 // are the whole row, and its mass is counted first; else `target` of it lies in the vectors.
-template <typename S, int NT, typename F>
+// `lds`: 64 places.
+template <typename S, typename F>
 __device__ __forceinline__ void draw_along(const SampleArgs &g, uint64_t row, const S *s, uint32_t from, uint32_t to,
                                            uint32_t draw, mass_t total, mass_t target, F mass_of, mass_t *lds)
 {
     using T = typename StatOf<S>::T;
-    constexpr uint32_t N = kVec<S>, W = NT / 64;
+    constexpr uint32_t N = kVec<S>, NT = 256, kTiles = 16, U = 4;
     const uint32_t wave = threadIdx.x / 64, lane = threadIdx.x & 63, n = g.vocab;
-    // The mass of each wave's run, in index order; then along the run that holds the target.
-    const uint32_t run = (to - from + W - 1) / W;
-    const uint32_t first = from + wave * run < to ? from + wave * run : to, past = first + run < to ? first + run : to;
-    mass_t own = 0;
-    wave_run(s, n, first, past, [&](const T *v, uint32_t at, uint32_t count) {
+    auto mass_in = [&](const u32x4 &raw, uint32_t i, mass_t *w) {
+        T v[N];
+        unpack<S>(raw, v);
+        mass_t sum = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < N; i++)
-            if (i < count)
-                own += mass_of(v[i], at + i);
-        return false;
-    });
-    own = wave_reduce(own, OpSum());
-    if (lane == 0)
-        lds[wave] = own;
-    __syncthreads();
+        for (uint32_t e = 0; e < N; e++) {
+            const mass_t x = i < to && i * N + e < n ? mass_of(v[e], i * N + e) : 0;
+            if (w)
+                w[e] = x;
+            sum += x;
+        }
+        return sum;
+    };
+    auto load = [&](uint32_t i) { return i < to ? load_vec(s, i, n) : minus_infinities<S>(); };
     if (total == 0) {
-        for (uint32_t w = 0; w < W; w++)
-            total += lds[w];
+        mass_t own = 0;
+        for (uint32_t i = from + threadIdx.x; i < to; i += NT * U) {
+            u32x4 raw[U];
+#pragma unroll
+            for (uint32_t u = 0; u < U; u++)
+                raw[u] = load(i + u * NT);
+#pragma unroll
+            for (uint32_t u = 0; u < U; u++)
+                own += mass_in(raw[u], i + u * NT, nullptr);
+        }
+        total = block_reduce<NT>(own, OpSum(), lds);
         target = share_of(total, draw);
+        __syncthreads();
     }
-    uint32_t holder = 0;
-    while (holder < W - 1 && target >= lds[holder])
-        target -= lds[holder++];
-    if (wave != holder)
-        return;
-    wave_run(s, n, first, past, [&](const T *v, uint32_t at, uint32_t count) {
-        mass_t w[N], sum = 0;
+    // Tiles of one vector a thread, 16 at a time: the masses of each tile's four waves, in index
+    // order, then within the wave that holds the target.
+    for (uint32_t at = from; at < to; at += NT * kTiles) {
+#pragma unroll 1
+        for (uint32_t t = 0; t < kTiles; t += U) {
+            u32x4 raw[U];
 #pragma unroll
-        for (uint32_t i = 0; i < N; i++) {
-            w[i] = i < count ? mass_of(v[i], at + i) : 0;
-            sum += w[i];
-        }
-        const mass_t upto = wave_inclusive_sum(sum);
-        const uint64_t there = __ballot(upto > target);
-        if (there) {
-            if (lane == (uint32_t)__builtin_ctzll(there)) {
-                mass_t running = upto - sum;
+            for (uint32_t u = 0; u < U; u++)
+                raw[u] = load(at + (t + u) * NT + threadIdx.x);
 #pragma unroll
-                for (uint32_t i = 0; i < N; i++) {
-                    if (running <= target && target < running + w[i]) {
-                        g.tokens[row] = (int32_t)(at + i);
-                        if (g.log_prob)
-                            g.log_prob[row] = logf((float)w[i] / (float)total);
-                    }
-                    running += w[i];
-                }
+            for (uint32_t u = 0; u < U; u++) {
+                const mass_t sum = wave_reduce(mass_in(raw[u], at + (t + u) * NT + threadIdx.x, nullptr), OpSum());
+                if (lane == 0)
+                    lds[(t + u) * 4 + wave] = sum;
             }
-            return true;
         }
-        target -= from_lane(upto, 63);
-        return false;
-    });
+        __syncthreads();
+        const mass_t here = lds[lane], upto = wave_inclusive_sum(here), all = from_lane(upto, 63);
+        if (target >= all) {
+            target -= all;
+            __syncthreads(); // the masses are read
+            continue;
+        }
+        const int cell = __builtin_ctzll(__ballot(upto > target));
+        target -= from_lane(upto - here, cell);
+        if (wave != (uint32_t)cell % 4)
+            return;
+        const uint32_t i = at + (uint32_t)cell / 4 * NT + threadIdx.x;
+        mass_t w[N];
+        const mass_t own = mass_in(load(i), i, w), before = wave_inclusive_sum(own) - own;
+        if (before <= target && target < before + own) {
+            mass_t running = before;
+#pragma unroll
+            for (uint32_t e = 0; e < N; e++) {
+                if (running <= target && target < running + w[e]) {
+                    g.tokens[row] = (int32_t)(i * N + e);
+                    if (g.log_prob)
+                        g.log_prob[row] = logf((float)w[e] / (float)total);
+                }
+                running += w[e];
+            }
+        }
+        return;
+    }
 }
 
 // ------------------------------------------------------- short rows: one workgroup a row
@@ -400,12 +500,10 @@ template <typename S, int NT, int R> __global__ __launch_bounds__(NT) void k_sam
     using T = typename StatOf<S>::T;
     using K = typename KeyOf<T>::K;
     constexpr uint32_t N = kVec<S>;
-    if (block_gate_closed(g.gate))
-        return;
     __shared__ BoundScratch bound;
     __shared__ T red_t[3][16];
     __shared__ DrawShared<T, NT> sh;
-    constexpr uint32_t kCap = kPerThread * NT;
+    constexpr uint32_t kCap = 2048;
     __shared__ List<K, kCap> list;
     const uint32_t tid = threadIdx.x;
     const uint64_t row = blockIdx.x;
@@ -413,6 +511,8 @@ template <typename S, int NT, int R> __global__ __launch_bounds__(NT) void k_sam
     const uint32_t n = g.vocab;
     const Settings set = settings_of(g, row);
     const Row<S, NT, R> held(s, n);
+    if (block_gate_closed(g.gate)) // after the loads: they need not wait for it
+        return;
 
     constexpr int G = 4;
     T group[G];
@@ -435,30 +535,34 @@ template <typename S, int NT, int R> __global__ __launch_bounds__(NT) void k_sam
         return;
     }
     const Weight<T> weight{m, set.inv};
+    const LocalList<K> entries{list.key, list.at};
     if (tid == 0)
         list.count = 0;
     __syncthreads();
     // Adds the row's wanted values to the list; its length.
     auto gather = [&](auto wanted) {
         held.walk([&](const T *v, uint32_t at, int) {
-#pragma unroll
-            for (uint32_t i = 0; i < N; i++)
-                if (v[i] > -INFINITY && wanted(v[i], at + i))
-                    list.add(key_of(v[i]), at + i);
+            list.template add_of<N>(v, [&](T x, int i) { return x > -INFINITY && wanted(x, at + i); },
+                                    [&](int i) { return at + i; });
         });
         if (held.has_extra && held.extra > -INFINITY && wanted(held.extra, held.extra_at()))
             list.add(key_of(held.extra), held.extra_at());
         __syncthreads();
         const uint32_t count = list.count;
-        __syncthreads();
+        list.template fill_keys<NT>(s);
         return count;
     };
 
     if (set.k < n && set.k <= kLogitMaxK) {
-        const T t = bound_of<NT>(group, m, set.k, bound, red_t[1]);
+        const uint32_t top_k[1] = {set.k};
+        const T t = bounds_of<NT>(group, m, top_k, bound, red_t[1]).t[0];
         const uint32_t count = gather([&](T v, uint32_t) { return v >= t; });
+        if (count <= kFew) {
+            draw_from_few<NT>(g, row, set, list.key, list.at, count, 0, weight, sh.steps, sh.red[0]);
+            return;
+        }
         if (count <= kCap) {
-            draw_from_list(g, row, set, list.key, list.at, count, 0, weight, sh);
+            draw_from_list(g, row, set, entries, count, 0, weight, sh);
             return;
         }
         if (tid == 0)
@@ -492,8 +596,12 @@ template <typename S, int NT, int R> __global__ __launch_bounds__(NT) void k_sam
         __syncthreads();
         const End end = find_end(sh, set.part);
         uint32_t count = gather([&](T v, uint32_t i) { return step_of(v) <= end.step && last.keeps(v, i); });
+        if (count <= kFew) {
+            draw_from_few<NT>(g, row, set, list.key, list.at, count, end.need, weight, sh.steps, sh.red[0]);
+            return;
+        }
         if (count <= kCap) {
-            draw_from_list(g, row, set, list.key, list.at, count, end.need, weight, sh);
+            draw_from_list(g, row, set, entries, count, end.need, weight, sh);
             return;
         }
         if (tid == 0)
@@ -501,8 +609,8 @@ template <typename S, int NT, int R> __global__ __launch_bounds__(NT) void k_sam
         __syncthreads();
         count = gather([&](T v, uint32_t i) { return step_of(v) == end.step && last.keeps(v, i); });
         if (count <= kCap) {
-            const Entries<T> in(list.key, list.at, count, weight, std::integral_constant<int, NT>());
-            select_entry<NT, false>(in.e, in.w, end.need - end.above, index_bits(n), sh.select);
+            select_entry<NT, false>(count, entries, [&](K key, uint32_t) { return weight(value_of(key)); },
+                                    end.need - end.above, index_bits(n), sh.select);
             last = Last<T>{value_of(sh.select.key), sh.select.at};
         } else {
             last = nucleus_exactly<S, NT>(s, n, pk, end.need, weight, sh);
@@ -514,34 +622,86 @@ template <typename S, int NT, int R> __global__ __launch_bounds__(NT) void k_sam
         const mass_t w = weight(v);
         return w >= set.least ? w : 0;
     };
-    draw_along<S, NT>(g, row, s, 0u, (n + N - 1) / N, set.draw, 0, 0, mass_of, sh.red[3]);
+    draw_along<S>(g, row, s, 0u, (n + N - 1) / N, set.draw, 0, 0, mass_of, sh.tiles);
+}
+
+// The drawing of a row whose lists did not suffice, or whose top_k no list holds: everything digit
+// by digit over the whole row.
+template <typename S, int NT, typename T>
+__device__ __forceinline__ void draw_by_search(const SampleArgs &g, uint64_t row, const S *s, const Settings &set, T m, DrawShared<T, NT> &sh)
+{
+    using K = typename KeyOf<T>::K;
+    constexpr uint32_t N = kVec<S>;
+    const uint32_t n = g.vocab;
+    const Weight<T> weight{m, set.inv};
+    Last<T> last{-INFINITY, 0xffffffffu};
+    Prefix<K> pk{0, 0};
+    if (set.k < n) {
+        pk = select_count<S, NT>(s, n, set.k, reinterpret_cast<uint32_t *>(sh.steps), &sh.count_digit);
+        if (pk.t)
+            last = last_of<S, NT>(s, n, pk, sh.wave_ties, &sh.found_at);
+    }
+    if (set.nucleus()) {
+        mass_t mass = 0;
+        each_vec<S, NT>(s, n, [&](const T *v, uint32_t at, uint32_t values) {
+#pragma unroll
+            for (uint32_t i = 0; i < N; i++)
+                if (i < values && last.keeps(v[i], at + i))
+                    mass += weight(v[i]);
+        });
+        mass = share_of(block_reduce<NT>(mass, OpSum(), sh.red[0]), set.part);
+        last = nucleus_exactly<S, NT>(s, n, pk, mass ? mass : 1, weight, sh);
+    }
+    draw_along<S>(g, row, s, 0u, (n + N - 1) / N, set.draw, 0, 0,
+                      [&](T v, uint32_t i) -> mass_t {
+                          const mass_t w = last.keeps(v, i) ? weight(v) : 0;
+                          return w >= set.least ? w : 0;
+                      },
+                      sh.tiles);
 }
 
 // ------------------------------------------------- long rows: a row split over workgroups
 //
-// Each row is cut into chunks of consecutive vectors, and the steps above become launches:
-//   1. each chunk's maximum; for a row whose top_k a list can hold, a bound that the chunk's share
-//      of top_k values reaches (such a row's chunks take every chunks-th block of vectors, so
-//      that they hold alike values wherever the row's large ones lie)
-//   2. with the row's maximum: the values beyond the lowest of the bounds into the row's list; or
-//      a nucleus row's masses by steps of z; or the mass of the chunk
-//   3. for a nucleus: the step in which it ends, and the chunks' masses before it
-//   4. for a nucleus: the values of that step into the row's list
-//   5. the drawing: from the list; or in the chunk that holds the target
+// Each row is cut into chunks of consecutive vectors, one workgroup each, and the steps above
+// become up to three launches, the last chunk of a row to finish doing what needs the whole row:
+//   first: the chunk's maximum. A row whose top_k a list can hold: the chunk's values beyond a bound
+//          that top_k of them reach go to the row's list, and the last chunk draws from it.
+//          (Such a row's chunks take every chunks-th block of vectors, so that they hold alike values
+//          wherever the row's large ones lie. Where top_k times the chunks would overflow the list,
+//          the bound is one that the chunk's share of top_k reaches, and the list is made in the
+//          second launch from the lowest of the bounds.)
+//   weigh: with the row's maximum, the chunk's mass, and the last chunk draws in the chunk that
+//          holds the target; or a nucleus row's masses by steps of z, and the last chunk finds
+//          the step in which the nucleus ends
+//   edge:  for a nucleus, the values of that step into the row's list; the last chunk finds the
+//          nucleus' last token among them and draws in the chunk that holds the target
 // One workgroup would take an exponential of every logit of its row at the rate of one CU: a
 // nucleus of a row of 152000 took 280 us.
-enum : uint32_t { kRowNone, kRowList, kRowNucleus, kRowPlain, kRowSearch };
+enum : uint32_t {
+    kRowNone,    // an invalid setting
+    kRowList,    // done in the first launch
+    kRowBound,   // a list made in the second
+    kRowNucleus,
+    kRowPlain,
+    kRowSearch,  // top_k beyond any list
+};
 
 struct RowState {
     mass_t need, above; // of the nucleus
     uint32_t count;     // of the row's list; past its capacity: not whole
     uint32_t step;      // in which the nucleus ends
+    uint32_t done[3];   // chunks that have finished each launch
 };
 
 template <typename T> struct ChunkPart {
     T m;
-    T t; // the bound; for a nucleus row the smallest value above minus infinity
+    T t; // a bound that the chunk's share of top_k reaches; for a nucleus row the smallest value above
+         // minus infinity
 };
+
+constexpr uint32_t kRowCap = 8192; // of a row's list
+constexpr int kChunkThreads = 256;
+constexpr int kChunkListCap = 1024;
 
 template <typename T> struct SplitArgs {
     SampleArgs g;
@@ -549,22 +709,46 @@ template <typename T> struct SplitArgs {
     ChunkPart<T> *part;  // rows x chunks
     mass_t *chunk_mass;  // rows x chunks: kept before the nucleus' last step, or kept
     mass_t *steps;       // rows x chunks x kSteps
-    RowState *state;     // rows
+    RowState *state;     // rows, zero between calls
     typename KeyOf<T>::K *key; // rows x kRowCap
     uint32_t *at;              // rows x kRowCap
 };
 
-__device__ __forceinline__ uint32_t kind_of(const Settings &s, uint32_t n)
+// Whether the chunks' own lists of the top `k` fit the row's (a list holds up to half as many
+// again as its bound was made for).
+__host__ __device__ inline bool list_at_once(uint64_t k, uint32_t chunks)
+{
+    return k * chunks <= kRowCap / 2 && k <= kChunkListCap / 2;
+}
+__device__ __forceinline__ uint32_t kind_of(const Settings &s, uint32_t n, uint32_t chunks)
 {
     if (!s.ok)
         return kRowNone;
     if (s.k < n)
-        return s.k <= kLogitMaxK ? kRowList : kRowSearch;
+        return s.k > kLogitMaxK ? kRowSearch : (list_at_once(s.k, chunks) ? kRowList : kRowBound);
     return s.nucleus() ? kRowNucleus : kRowPlain;
 }
 
-constexpr int kChunkThreads = 256, kRowThreads = 1024;
-constexpr uint32_t kRowCap = kPerThread * kRowThreads; // of a row's list
+// What a chunk hands to the others of its row within a launch is written through the caches that
+// they do not share, and is complete (a wait for the wave's own stores, then the barrier) before the
+// workgroup counts itself as done.
+template <typename V> __device__ __forceinline__ void put(V *p, V v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename V> __device__ __forceinline__ V get(const V *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// Whether this workgroup is the last of the row's chunks; whole workgroup, once a launch.
+__device__ __forceinline__ bool last_chunk(uint32_t *done, uint32_t chunks)
+{
+    __shared__ bool last;
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        last = atomicAdd(done, 1u) + 1u == chunks;
+        if (last)
+            put(done, 0u); // as the next call expects it
+    }
+    __syncthreads();
+    return last;
+}
 
 // The vectors of one chunk of the row, then (last chunk) the values after the last whole vector.
 template <typename S> struct Chunk {
@@ -587,59 +771,203 @@ template <typename S> struct Chunk {
         }
         rest = chunk == chunks - 1 ? whole * N + threadIdx.x : n;
     }
-    // f(value, index, group of 4)
-    template <typename F> __device__ __forceinline__ void each(F f) const
+    static constexpr int U = 4; // vectors in flight
+    // f(values, their number, index of value i by index_of(i)), for four vectors at a time; places
+    // past the chunk hold minus infinity.
+    template <typename F> __device__ __forceinline__ void groups(F f) const
     {
-        constexpr int U = 4;
         for (uint32_t i = first + threadIdx.x; i < past; i += step * U) {
             u32x4 in[U];
+            T v[U * N];
 #pragma unroll
             for (int u = 0; u < U; u++)
                 in[u] = i + u * step < past ? load_whole(s, i + u * step) : minus_infinities<S>();
 #pragma unroll
-            for (int u = 0; u < U; u++) {
+            for (int u = 0; u < U; u++)
+                unpack<S>(in[u], v + u * N);
+            f(v, std::integral_constant<int, U * (int)N>(),
+              [&](int k) { return (i + (uint32_t)k / N * step) * N + (uint32_t)k % N; });
+        }
+        if (rest < n) {
+            const T v[1] = {(T)s[rest]};
+            f(v, std::integral_constant<int, 1>(), [&](int) { return rest; });
+        }
+    }
+    // f(value, index, vector of the four)
+    template <typename F> __device__ __forceinline__ void each(F f) const
+    {
+        groups([&](const T *v, auto count, auto index_of) {
+#pragma unroll
+            for (int k = 0; k < count; k++)
+                f(v[k], index_of(k), k / (int)N);
+        });
+    }
+    // The largest values of this thread's vectors, every eighth of them in one group.
+    static constexpr int kGroups = 8;
+    __device__ __forceinline__ void largest(T (&group)[kGroups]) const
+    {
+#pragma unroll
+        for (int g = 0; g < kGroups; g++)
+            group[g] = -INFINITY;
+        for (uint32_t i = first + threadIdx.x; i < past; i += step * kGroups) {
+            u32x4 in[kGroups];
+#pragma unroll
+            for (int g = 0; g < kGroups; g++)
+                in[g] = i + g * step < past ? load_whole(s, i + g * step) : minus_infinities<S>();
+#pragma unroll
+            for (int g = 0; g < kGroups; g++) {
                 T v[N];
-                unpack<S>(in[u], v);
+                unpack<S>(in[g], v);
 #pragma unroll
                 for (uint32_t e = 0; e < N; e++)
-                    f(v[e], (i + u * step) * N + e, u);
+                    group[g] = OpMax()(group[g], v[e]);
             }
         }
-        if (rest < n)
-            f((T)s[rest], rest, 0);
+    }
+    // The values that reach t (above minus infinity) into the list, from the vectors of the groups
+    // that do; whole workgroup, ends with a barrier.
+    template <typename L> __device__ __forceinline__ void gather(L &list, const T (&group)[kGroups], T t) const
+    {
+        if (threadIdx.x == 0)
+            list.count = 0;
+        __syncthreads();
+        list.add_from(s, group, t, [&](int g, auto f) {
+            for (uint32_t i = first + threadIdx.x + (uint32_t)g * step; i < past; i += step * kGroups)
+                f(i);
+        });
+        if (rest < n && (T)s[rest] >= t)
+            list.add(0, rest);
+        __syncthreads();
+        list.template fill_keys<kChunkThreads>(s);
+    }
+    // The wanted values into the list; whole workgroup, ends with a barrier.
+    template <typename L, typename W> __device__ __forceinline__ void gather(L &list, W wanted) const
+    {
+        if (threadIdx.x == 0)
+            list.count = 0;
+        __syncthreads();
+        groups([&](const T *v, auto count, auto index_of) {
+            list.template add_of<decltype(count)::value>(v, [&](T x, int) { return wanted(x); }, index_of);
+        });
+        __syncthreads();
+        list.template fill_keys<kChunkThreads>(s);
     }
 };
 
-template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_max(SplitArgs<typename StatOf<S>::T> a)
+// A workgroup's list handed to its row's: one place reserved for all of it. A list that does not
+// fit sets the row's count beyond the capacity.
+template <typename K, int CAP, typename T>
+__device__ __forceinline__ void hand_over(const SplitArgs<T> &a, uint64_t row, const List<K, CAP> &list)
 {
-    using T = typename StatOf<S>::T;
-    constexpr int NT = kChunkThreads;
-    if (block_gate_closed(a.g.gate))
+    __shared__ uint32_t base;
+    const uint32_t count = list.count;
+    if (count == 0)
         return;
-    __shared__ BoundScratch bound;
-    __shared__ T red[3][16];
-    const uint64_t row = blockIdx.x / a.chunks;
-    const uint32_t chunk = blockIdx.x % a.chunks, n = a.g.vocab;
-    const Settings set = settings_of(a.g, row);
-    const uint32_t kind = kind_of(set, n);
-    if (chunk == 0 && threadIdx.x == 0)
-        a.state[row].count = 0;
-    const Chunk<S> part(static_cast<const S *>(a.g.logits) + row * a.g.stride, n, chunk, a.chunks, a.chunk_vecs,
-                        kind == kRowList);
-    T group[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    part.each([&](T v, uint32_t, int u) { group[u] = OpMax()(group[u], v); });
-    T m = OpMax()(OpMax()(group[0], group[1]), OpMax()(group[2], group[3]));
-    m = block_reduce<NT>(m, OpMax(), red[0]);
-    T t = -INFINITY;
-    if (kind == kRowList) {
-        t = bound_of<NT>(group, m, (set.k + a.chunks - 1) / a.chunks, bound, red[1]);
-    } else if (kind == kRowNucleus) {
-        t = INFINITY;
-        part.each([&](T v, uint32_t, int) { t = v > -INFINITY && v < t ? v : t; });
-        t = -block_reduce<NT>(-t, OpMax(), red[1]);
-    }
     if (threadIdx.x == 0)
-        a.part[blockIdx.x] = ChunkPart<T>{m, t};
+        base = atomicAdd(&a.state[row].count, count > CAP ? kRowCap + 1u : count);
+    __syncthreads();
+    const uint32_t to = base;
+    if (count > CAP || to + count > kRowCap)
+        return;
+    for (uint32_t j = threadIdx.x; j < count; j += kChunkThreads) {
+        put(&a.key[row * kRowCap + to + j], list.key[j]);
+        put(&a.at[row * kRowCap + to + j], list.at[j]);
+    }
+}
+
+// The row's list for its last chunk: its length (past kRowCap: not whole), and in LDS what of it may
+// belong to the first `k` of the order (not whole past CAP): all of it, or, of up to 8 entries a
+// thread, what reaches a bound from the threads' largest.
+template <typename K, int CAP, typename T>
+__device__ __forceinline__ uint32_t take_list(const SplitArgs<T> &a, uint64_t row, uint32_t k, T m, List<K, CAP> &local,
+                                              BoundScratch &bound, T *red)
+{
+    __shared__ uint32_t count;
+    if (threadIdx.x == 0) {
+        count = get(&a.state[row].count);
+        put(&a.state[row].count, 0u);
+        local.count = 0;
+    }
+    __syncthreads();
+    const uint32_t n = count;
+    constexpr int U = 8, NT = kChunkThreads;
+    if (n > U * NT)
+        local.count = n;
+    if (n > U * NT) {
+        __syncthreads();
+        return n;
+    }
+    const SharedList<K> list{a.key + row * kRowCap, a.at + row * kRowCap};
+    Entry<K> e[U];
+    K top = 0;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const uint32_t j = threadIdx.x + u * NT;
+        e[u] = j < n ? list(j) : Entry<K>{0, 0};
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        top = e[u].key > top ? e[u].key : top;
+    K least = 1; // no entry has key 0
+    if (n > 128 && k < n) {
+        const T group[1] = {top ? value_of(top) : (T)-INFINITY};
+        const uint32_t wanted[1] = {k};
+        const T t = bounds_of<NT>(group, m, wanted, bound, red).t[0];
+        least = t > -INFINITY ? key_of(t) : least;
+    }
+    uint32_t own = 0;
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        own += e[u].key >= least;
+    if (own) {
+        uint32_t to = atomicAdd(&local.count, own);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (e[u].key >= least) {
+                if (to < CAP) {
+                    local.key[to] = e[u].key;
+                    local.at[to] = e[u].at;
+                }
+                to++;
+            }
+    }
+    __syncthreads();
+    return n;
+}
+
+// Draws from the row's list.
+template <typename S, typename T, typename K, int CAP>
+__device__ __forceinline__ void draw_from_row(const SplitArgs<T> &a, uint64_t row, const Settings &set, T m,
+                                              List<K, CAP> &local, BoundScratch &bound, T *red, DrawShared<T, kChunkThreads> &sh)
+{
+    const uint32_t count = take_list(a, row, set.k, m, local, bound, red), here = local.count;
+    const Weight<T> weight{m, set.inv};
+    if (count > kRowCap)
+        draw_by_search<S, kChunkThreads>(a.g, row, static_cast<const S *>(a.g.logits) + row * a.g.stride, set, m, sh);
+    else if (here <= kFew)
+        draw_from_few<kChunkThreads>(a.g, row, set, local.key, local.at, here, 0, weight, sh.steps, sh.red[0]);
+    else if (here <= CAP)
+        draw_from_list(a.g, row, set, LocalList<K>{local.key, local.at}, here, 0, weight, sh);
+    else
+        draw_from_list(a.g, row, set, SharedList<K>{a.key + row * kRowCap, a.at + row * kRowCap}, count, 0, weight, sh);
+}
+
+// Draws in the chunk that holds the target; `in_chunk` the chunks' kept masses, in LDS.
+template <typename S, typename T, typename F>
+__device__ __forceinline__ void draw_in_chunk(const SplitArgs<T> &a, uint64_t row, const Settings &set, const mass_t *in_chunk,
+                                              F mass_of, mass_t *lds)
+{
+    constexpr uint32_t N = kVec<S>;
+    mass_t total = 0;
+    for (uint32_t c = 0; c < a.chunks; c++)
+        total += in_chunk[c];
+    mass_t target = share_of(total, set.draw);
+    uint32_t c = 0;
+    while (c < a.chunks - 1 && target >= in_chunk[c])
+        target -= in_chunk[c++];
+    const uint32_t from = c * a.chunk_vecs, to = c == a.chunks - 1 ? (a.g.vocab + N - 1) / N : from + a.chunk_vecs;
+    draw_along<S>(a.g, row, static_cast<const S *>(a.g.logits) + row * a.g.stride, from, to, set.draw, total,
+                                 target, mass_of, lds);
 }
 
 // The row's maximum, and the lowest of the chunks' bounds or smallest values; one chunk a lane.
@@ -648,31 +976,75 @@ template <typename T> __device__ __forceinline__ ChunkPart<T> row_part(const Spl
     const uint32_t lane = threadIdx.x & 63;
     ChunkPart<T> p{-INFINITY, INFINITY};
     if (lane < a.chunks)
-        p = a.part[row * a.chunks + lane];
+        p = {get(&a.part[row * a.chunks + lane].m), get(&a.part[row * a.chunks + lane].t)};
     return {wave_reduce(p.m, OpMax()), -wave_reduce(-p.t, OpMax())};
 }
 
-// A workgroup's list handed to its row's: one place reserved for all of it. A list that does not
-// fit sets the row's count beyond the capacity.
-template <typename K, int CAP, typename T>
-__device__ __forceinline__ void hand_over(const SplitArgs<T> &a, uint64_t row, const List<K, CAP> &list, uint32_t *base)
-{
-    const uint32_t count = list.count;
-    if (count == 0)
-        return;
-    if (threadIdx.x == 0)
-        *base = atomicAdd(&a.state[row].count, count > CAP ? (uint32_t)kRowCap + 1u : count);
-    __syncthreads();
-    const uint32_t to = *base;
-    if (count > CAP || to + count > kRowCap)
-        return;
-    for (uint32_t j = threadIdx.x; j < count; j += kChunkThreads) {
-        a.key[row * kRowCap + to + j] = list.key[j];
-        a.at[row * kRowCap + to + j] = list.at[j];
-    }
-}
+// The lowest finite value.
+template <typename T> __device__ __forceinline__ T lowest() { return sizeof(T) == 8 ? (T)-1.7976931348623157e308 : (T)-3.402823466e38f; }
 
-constexpr int kChunkListCap = 1024;
+template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_first(SplitArgs<typename StatOf<S>::T> a)
+{
+    using T = typename StatOf<S>::T;
+    using K = typename KeyOf<T>::K;
+    constexpr int NT = kChunkThreads;
+    if (block_gate_closed(a.g.gate))
+        return;
+    __shared__ BoundScratch bound;
+    __shared__ T red[4][16];
+    __shared__ List<K, kChunkListCap> list;
+    __shared__ DrawShared<T, NT> sh;
+    const uint64_t row = blockIdx.x / a.chunks;
+    const uint32_t chunk = blockIdx.x % a.chunks, n = a.g.vocab;
+    const Settings set = settings_of(a.g, row);
+    const uint32_t kind = kind_of(set, n, a.chunks);
+    if (kind == kRowNone) {
+        if (chunk == 0 && threadIdx.x == 0)
+            no_token(a.g, row, false);
+        return;
+    }
+    const Chunk<S> part(static_cast<const S *>(a.g.logits) + row * a.g.stride, n, chunk, a.chunks, a.chunk_vecs,
+                        kind == kRowList || kind == kRowBound);
+    T largest[Chunk<S>::kGroups];
+    part.largest(largest);
+    const T rest = part.rest < n ? (T)part.s[part.rest] : (T)-INFINITY;
+    T group[4]; // half as many for the bounds
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        group[i] = OpMax()(largest[i], largest[i + 4]);
+    group[0] = OpMax()(group[0], rest);
+    T m = OpMax()(OpMax()(group[0], group[1]), OpMax()(group[2], group[3]));
+    m = block_reduce<NT>(m, OpMax(), red[0]);
+    T t = -INFINITY, own = -INFINITY;
+    if (kind == kRowList || kind == kRowBound) {
+        const uint32_t top_k[2] = {(set.k + a.chunks - 1) / a.chunks, set.k};
+        const Bounds<T> b = bounds_of<NT>(group, m, top_k, bound, red[1]);
+        t = b.t[0];
+        own = b.t[1];
+    } else if (kind == kRowNucleus) {
+        t = INFINITY;
+        part.each([&](T v, uint32_t, int) { t = v > -INFINITY && v < t ? v : t; });
+        t = -block_reduce<NT>(-t, OpMax(), red[1]);
+    }
+    if (threadIdx.x == 0) {
+        put(&a.part[blockIdx.x].m, m);
+        put(&a.part[blockIdx.x].t, t);
+    }
+    if (kind != kRowList)
+        return;
+    own = own > lowest<T>() ? own : lowest<T>(); // minus infinity is never drawn
+    part.gather(list, largest, own);
+    hand_over(a, row, list);
+    if (!last_chunk(&a.state[row].done[0], a.chunks))
+        return;
+    const T top = row_part(a, row).m;
+    if (top == -INFINITY) {
+        if (threadIdx.x == 0)
+            no_token(a.g, row, true);
+        return;
+    }
+    draw_from_row<S>(a, row, set, top, list, bound, red[0], sh);
+}
 
 template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_weigh(SplitArgs<typename StatOf<S>::T> a)
 {
@@ -681,44 +1053,54 @@ template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_
     constexpr int NT = kChunkThreads;
     if (block_gate_closed(a.g.gate))
         return;
-    __shared__ union {
-        mass_t steps[kSteps];
-        List<K, kChunkListCap> list;
-    } sh;
-    __shared__ mass_t red[16];
-    __shared__ uint32_t base;
+    __shared__ BoundScratch bound;
+    __shared__ T red[4][16];
+    __shared__ List<K, kChunkListCap> list;
+    __shared__ DrawShared<T, NT> sh;
+    __shared__ mass_t in_chunk[64];
     const uint64_t row = blockIdx.x / a.chunks;
     const uint32_t chunk = blockIdx.x % a.chunks, n = a.g.vocab;
     const Settings set = settings_of(a.g, row);
-    const uint32_t kind = kind_of(set, n);
-    const auto [m, low] = row_part(a, row);
-    if (kind == kRowNone || kind == kRowSearch || m == -INFINITY)
+    const uint32_t kind = kind_of(set, n, a.chunks);
+    if (kind == kRowNone || kind == kRowList)
         return;
-    const Chunk<S> part(static_cast<const S *>(a.g.logits) + row * a.g.stride, n, chunk, a.chunks, a.chunk_vecs,
-                        kind == kRowList);
-    if (kind == kRowList) {
-        const T t = low;
-        if (threadIdx.x == 0)
-            sh.list.count = 0;
-        __syncthreads();
-        part.each([&](T v, uint32_t at, int) {
-            if (v >= t && v > -INFINITY)
-                sh.list.add(key_of(v), at);
-        });
-        __syncthreads();
-        hand_over(a, row, sh.list, &base);
+    const auto [m, low] = row_part(a, row);
+    const S *s = static_cast<const S *>(a.g.logits) + row * a.g.stride;
+    if (m == -INFINITY || kind == kRowSearch) {
+        if (chunk != 0)
+            return;
+        if (m > -INFINITY)
+            draw_by_search<S, NT>(a.g, row, s, set, m, sh);
+        else if (threadIdx.x == 0)
+            no_token(a.g, row, true);
         return;
     }
+    const Chunk<S> part(s, n, chunk, a.chunks, a.chunk_vecs, kind == kRowBound);
     const Weight<T> weight{m, set.inv};
+    if (kind == kRowBound) {
+        const T t = low > lowest<T>() ? low : lowest<T>();
+        part.gather(list, [&](T v) { return v >= t; });
+        hand_over(a, row, list);
+        if (last_chunk(&a.state[row].done[1], a.chunks))
+            draw_from_row<S>(a, row, set, m, list, bound, red[0], sh);
+        return;
+    }
     if (kind == kRowPlain) {
-        mass_t own = 0;
-        part.each([&](T v, uint32_t, int) {
+        auto mass_of = [&](T v, uint32_t) -> mass_t {
             const mass_t w = weight(v);
-            own += w >= set.least ? w : 0;
-        });
-        own = block_reduce<NT>(own, OpSum(), red);
+            return w >= set.least ? w : 0;
+        };
+        mass_t own = 0;
+        part.each([&](T v, uint32_t at, int) { own += mass_of(v, at); });
+        own = block_reduce<NT>(own, OpSum(), sh.red[0]);
         if (threadIdx.x == 0)
-            a.chunk_mass[blockIdx.x] = own;
+            put(&a.chunk_mass[blockIdx.x], own);
+        if (!last_chunk(&a.state[row].done[1], a.chunks))
+            return;
+        if (threadIdx.x < a.chunks)
+            in_chunk[threadIdx.x] = get(&a.chunk_mass[row * a.chunks + threadIdx.x]);
+        __syncthreads();
+        draw_in_chunk<S>(a, row, set, in_chunk, mass_of, sh.tiles);
         return;
     }
     for (uint32_t b = threadIdx.x; b < kSteps; b += NT)
@@ -731,27 +1113,18 @@ template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_
     });
     __syncthreads();
     for (uint32_t b = threadIdx.x; b < kSteps; b += NT)
-        a.steps[(uint64_t)blockIdx.x * kSteps + b] = sh.steps[b];
-}
-
-// The step in which each nucleus ends, and the chunks' masses before it.
-template <typename T> __global__ __launch_bounds__(kRowThreads) void k_sample_end(SplitArgs<T> a)
-{
-    constexpr int NT = kRowThreads;
-    if (block_gate_closed(a.g.gate))
+        put(&a.steps[(uint64_t)blockIdx.x * kSteps + b], sh.steps[b]);
+    if (!last_chunk(&a.state[row].done[1], a.chunks))
         return;
-    __shared__ DrawShared<T, NT> sh;
-    const uint64_t row = blockIdx.x;
-    const Settings set = settings_of(a.g, row);
-    if (kind_of(set, a.g.vocab) != kRowNucleus || row_part(a, row).m == -INFINITY)
-        return;
-    static_assert(kSteps == NT, "one step a thread");
+    // The step in which the nucleus ends, and the chunks' masses before it.
     const mass_t *steps = a.steps + row * a.chunks * kSteps;
-    mass_t sum = 0;
+    for (uint32_t b = threadIdx.x; b < kSteps; b += NT) {
+        mass_t sum = 0;
 #pragma unroll 8
-    for (uint32_t c = 0; c < a.chunks; c++)
-        sum += steps[c * kSteps + threadIdx.x];
-    sh.steps[threadIdx.x] = sum;
+        for (uint32_t c = 0; c < a.chunks; c++)
+            sum += get(&steps[c * kSteps + b]);
+        sh.steps[b] = sum;
+    }
     __syncthreads();
     const End end = find_end(sh, set.part);
     if (threadIdx.x == 0) {
@@ -761,44 +1134,43 @@ template <typename T> __global__ __launch_bounds__(kRowThreads) void k_sample_en
     }
     for (uint32_t c = threadIdx.x / 64; c < a.chunks; c += NT / 64) {
         mass_t before = 0;
-#pragma unroll 8
+#pragma unroll 4
         for (uint32_t b = threadIdx.x & 63; b < end.step; b += 64)
-            before += steps[c * kSteps + b];
+            before += get(&steps[c * kSteps + b]);
         before = wave_reduce(before, OpSum());
         if ((threadIdx.x & 63) == 0)
             a.chunk_mass[row * a.chunks + c] = before;
     }
 }
 
-// The values of the step in which the nucleus ends; where min_p cuts, the chunk's kept mass before it.
 template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_edge(SplitArgs<typename StatOf<S>::T> a)
 {
     using T = typename StatOf<S>::T;
     using K = typename KeyOf<T>::K;
     constexpr int NT = kChunkThreads;
+    constexpr uint32_t N = kVec<S>;
     if (block_gate_closed(a.g.gate))
         return;
+    __shared__ BoundScratch bound;
+    __shared__ T red[4][16];
     __shared__ List<K, kChunkListCap> list;
-    __shared__ mass_t red[16];
-    __shared__ uint32_t base;
+    __shared__ DrawShared<T, NT> sh;
+    __shared__ mass_t in_chunk[64];
     const uint64_t row = blockIdx.x / a.chunks;
     const uint32_t chunk = blockIdx.x % a.chunks, n = a.g.vocab;
     const Settings set = settings_of(a.g, row);
-    const auto [m, low] = row_part(a, row);
-    if (kind_of(set, n) != kRowNucleus || m == -INFINITY)
+    if (kind_of(set, n, a.chunks) != kRowNucleus)
         return;
-    const Chunk<S> part(static_cast<const S *>(a.g.logits) + row * a.g.stride, n, chunk, a.chunks, a.chunk_vecs, false);
+    const auto [m, low] = row_part(a, row);
+    if (m == -INFINITY)
+        return;
+    const S *s = static_cast<const S *>(a.g.logits) + row * a.g.stride;
+    const Chunk<S> part(s, n, chunk, a.chunks, a.chunk_vecs, false);
     const StepOf<T> step_of(m, set.inv, low);
+    const Weight<T> weight{m, set.inv};
     const uint32_t end = a.state[row].step;
-    if (threadIdx.x == 0)
-        list.count = 0;
-    __syncthreads();
-    part.each([&](T v, uint32_t at, int) {
-        if (v > -INFINITY && step_of(v) == end)
-            list.add(key_of(v), at);
-    });
-    if (set.least > 0) {
-        const Weight<T> weight{m, set.inv};
+    part.gather(list, [&](T v) { return v > -INFINITY && step_of(v) == end; });
+    if (set.least > 0) { // of the chunk's mass before the step, what min_p leaves
         mass_t own = 0;
         part.each([&](T v, uint32_t, int) {
             if (v > -INFINITY && step_of(v) < end) {
@@ -806,101 +1178,46 @@ template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_
                 own += w >= set.least ? w : 0;
             }
         });
-        own = block_reduce<NT>(own, OpSum(), red);
+        own = block_reduce<NT>(own, OpSum(), sh.red[0]);
         if (threadIdx.x == 0)
-            a.chunk_mass[blockIdx.x] = own;
+            put(&a.chunk_mass[blockIdx.x], own);
     }
     __syncthreads();
-    hand_over(a, row, list, &base);
-}
-
-template <typename S> __global__ __launch_bounds__(kRowThreads) void k_sample_draw(SplitArgs<typename StatOf<S>::T> a)
-{
-    using T = typename StatOf<S>::T;
-    using K = typename KeyOf<T>::K;
-    constexpr int NT = kRowThreads;
-    constexpr uint32_t N = kVec<S>;
-    if (block_gate_closed(a.g.gate))
+    hand_over(a, row, list);
+    if (!last_chunk(&a.state[row].done[2], a.chunks))
         return;
-    __shared__ DrawShared<T, NT> sh;
-    __shared__ mass_t in_chunk[64];
-    const SampleArgs &g = a.g;
-    const uint64_t row = blockIdx.x;
-    const uint32_t n = g.vocab, tid = threadIdx.x;
-    const S *s = static_cast<const S *>(g.logits) + row * g.stride;
-    const Settings set = settings_of(g, row);
-    const T m = row_part(a, row).m;
-    if (!set.ok || m == -INFINITY) {
-        if (tid == 0)
-            no_token(g, row, set.ok);
+    const uint32_t count = take_list(a, row, kRowCap, m, list, bound, red[0]);
+    if (count > kRowCap) {
+        draw_by_search<S, NT>(a.g, row, s, set, m, sh);
         return;
     }
-    uint32_t kind = kind_of(set, n);
-    const Weight<T> weight{m, set.inv};
-    const uint32_t count = kind == kRowList || kind == kRowNucleus ? a.state[row].count : 0;
-    Last<T> last{-INFINITY, 0xffffffffu};
-    if (count > kRowCap)
-        kind = kRowSearch;
-    const K *key = a.key + row * kRowCap;
-    const uint32_t *at = a.at + row * kRowCap;
-    if (kind == kRowList) {
-        draw_from_list(g, row, set, key, at, count, 0, weight, sh);
-        return;
-    }
-    auto mass_of = [&](T v, uint32_t i) -> mass_t {
-        if (!last.keeps(v, i))
-            return 0;
-        const mass_t w = weight(v);
-        return w >= set.least ? w : 0;
-    };
-    const uint32_t vecs = (n + N - 1) / N;
-    if (kind == kRowSearch) {
-        Prefix<K> pk{0, 0};
-        if (set.k < n) {
-            pk = select_count<S, NT>(s, n, set.k, reinterpret_cast<uint32_t *>(sh.steps), &sh.count_digit);
-            if (pk.t)
-                last = last_of<S, NT>(s, n, pk, sh.wave_ties, &sh.found_at);
-        }
-        if (set.nucleus()) {
-            mass_t mass = 0;
-            each_vec<S, NT>(s, n, [&](const T *v, uint32_t at, uint32_t values) {
-#pragma unroll
-                for (uint32_t i = 0; i < N; i++)
-                    if (i < values && last.keeps(v[i], at + i))
-                        mass += weight(v[i]);
-            });
-            mass = share_of(block_reduce<NT>(mass, OpSum(), sh.red[0]), set.part);
-            last = nucleus_exactly<S, NT>(s, n, pk, mass ? mass : 1, weight, sh);
-        }
-        draw_along<S, NT>(g, row, s, 0u, vecs, set.draw, 0, 0, mass_of, sh.red[3]);
-        return;
-    }
-    if (tid < a.chunks)
-        in_chunk[tid] = a.chunk_mass[row * a.chunks + tid];
-    __syncthreads();
-    if (kind == kRowNucleus) {
-        Entries<T> in(key, at, count, weight, std::integral_constant<int, NT>());
-        select_entry<NT, false>(in.e, in.w, a.state[row].need - a.state[row].above, index_bits(n), sh.select);
+    if (threadIdx.x < a.chunks)
+        in_chunk[threadIdx.x] = get(&a.chunk_mass[row * a.chunks + threadIdx.x]);
+    Last<T> last;
+    auto finish = [&](auto entries) {
+        select_entry<NT, false>(count, entries, [&](K key, uint32_t) { return weight(value_of(key)); },
+                                a.state[row].need - a.state[row].above, index_bits(n), sh.select);
         last = Last<T>{value_of(sh.select.key), sh.select.at};
-        in.cut(sh.select.key, sh.select.at);
-#pragma unroll
-        for (int b = 0; b < kPerThread; b++) {
+        for (uint32_t j = threadIdx.x; j < count; j += NT) {
+            const auto e = entries(j);
+            const mass_t w = weight(value_of(e.key));
             // The values after the last whole vector belong to the last chunk.
-            const uint32_t c = in.e.at[b] / (a.chunk_vecs * N);
-            if (in.w[b] && in.w[b] >= set.least)
-                atomicAdd(&in_chunk[c < a.chunks ? c : a.chunks - 1], in.w[b]);
+            const uint32_t c = e.at / (a.chunk_vecs * N);
+            if (last.keeps(value_of(e.key), e.at) && w >= set.least)
+                atomicAdd(&in_chunk[c < a.chunks ? c : a.chunks - 1], w);
         }
-        __syncthreads();
-    }
-    mass_t total = 0;
-    for (uint32_t c = 0; c < a.chunks; c++)
-        total += in_chunk[c];
-    mass_t target = share_of(total, set.draw);
-    uint32_t c = 0;
-    while (c < a.chunks - 1 && target >= in_chunk[c])
-        target -= in_chunk[c++];
-    const uint32_t from = c * a.chunk_vecs, to = c == a.chunks - 1 ? vecs : from + a.chunk_vecs;
-    draw_along<S, NT>(g, row, s, from, to, set.draw, total, target, mass_of, sh.red[3]);
+    };
+    if (list.count <= kChunkListCap)
+        finish(LocalList<K>{list.key, list.at});
+    else
+        finish(SharedList<K>{a.key + row * kRowCap, a.at + row * kRowCap});
+    __syncthreads();
+    draw_in_chunk<S>(a, row, set, in_chunk,
+                     [&](T v, uint32_t i) -> mass_t {
+                         const mass_t w = last.keeps(v, i) ? weight(v) : 0;
+                         return w >= set.least ? w : 0;
+                     },
+                     sh.tiles);
 }
 
 // ------------------------------------------------------------------------- launches
@@ -909,12 +1226,14 @@ struct Split {
     uint32_t chunks, vecs;
 };
 
-// Chunks of long rows: of about 4096 logits where rows are few, of 16384 where they are many, at
-// most 32 a row (the nucleus adds up 8 KB for each); two at least, so that 1024 values are sought
-// among 2048 groups.
+// Chunks of long rows: 1536 workgroups for the chip, as far as each has four vectors a thread, at most
+// 16384 logits each; at most 32 a row (the nucleus adds up 8 KB for each), and two at least, so that
+// 1024 values are sought among 2048 groups.
 Split split_of(uint64_t rows, uint32_t vocab, uint32_t per_vec)
 {
-    uint64_t chunks = vocab / (rows < 64 ? 4096 : 16384);
+    const uint64_t want = (1536 + rows - 1) / rows, most = vocab / (4 * kChunkThreads * per_vec), least = vocab / 16384;
+    uint64_t chunks = want < most ? want : most;
+    chunks = chunks < least ? least : chunks;
     chunks = chunks < 2 ? 2 : (chunks > 32 ? 32 : chunks);
     const uint32_t whole = vocab / per_vec;
     const uint32_t vecs = (uint32_t)((whole + chunks - 1) / chunks);
@@ -943,11 +1262,11 @@ template <typename S> size_t scratch_t(const SampleArgs &g, SplitArgs<typename S
         at += (bytes + 255) / 256 * 256;
         return base + here;
     };
-    char *part = take(parts * sizeof(ChunkPart<T>)), *mass = take(parts * sizeof(mass_t)), *state = take(rows * sizeof(RowState));
+    char *part = take(parts * sizeof(ChunkPart<T>)), *mass = take(parts * sizeof(mass_t));
     char *steps = take(has_nucleus(g) ? parts * kSteps * sizeof(mass_t) : 0);
     char *key = take(rows * kRowCap * sizeof(K)), *places = take(rows * kRowCap * 4);
     if (a)
-        *a = SplitArgs<T>{g, sp.chunks, sp.vecs, (ChunkPart<T> *)part, (mass_t *)mass, (mass_t *)steps, (RowState *)state,
+        *a = SplitArgs<T>{g, sp.chunks, sp.vecs, (ChunkPart<T> *)part, (mass_t *)mass, (mass_t *)steps, nullptr,
                           (K *)key, (uint32_t *)places};
     return at;
 }
@@ -971,7 +1290,7 @@ SampleArgs rows_from(const SampleArgs &all, uint64_t from, uint64_t most)
     return g;
 }
 
-template <typename S> hipError_t launch_t(hipStream_t s, const SampleArgs &all, void *scratch)
+template <typename S> hipError_t launch_t(hipStream_t s, const SampleArgs &all, void *scratch, void *state)
 {
     using T = typename StatOf<S>::T;
     if (short_row(all, kVec<S>)) {
@@ -981,15 +1300,17 @@ template <typename S> hipError_t launch_t(hipStream_t s, const SampleArgs &all, 
     for (uint64_t from = 0; from < all.rows; from += kSlabRows) {
         SplitArgs<T> a;
         scratch_t<S>(all, &a, static_cast<char *>(scratch));
+        a.state = static_cast<RowState *>(state);
         a.g = rows_from(all, from, kSlabRows);
-        const dim3 parts((unsigned)(a.g.rows * a.chunks)), rows((unsigned)a.g.rows);
-        hipLaunchKernelGGL((k_sample_max<S>), parts, dim3(kChunkThreads), 0, s, a);
-        hipLaunchKernelGGL((k_sample_weigh<S>), parts, dim3(kChunkThreads), 0, s, a);
-        if (has_nucleus(all)) {
-            hipLaunchKernelGGL((k_sample_end<T>), rows, dim3(kRowThreads), 0, s, a);
-            hipLaunchKernelGGL((k_sample_edge<S>), parts, dim3(kChunkThreads), 0, s, a);
-        }
-        hipLaunchKernelGGL((k_sample_draw<S>), rows, dim3(kRowThreads), 0, s, a);
+        const dim3 parts((unsigned)(a.g.rows * a.chunks)), block(kChunkThreads);
+        // Every row's list is made and drawn from in the first launch where top_k says so for all.
+        const bool lists = !all.top_k && all.top_k_all > 0 && (uint32_t)all.top_k_all < all.vocab &&
+                           list_at_once((uint64_t)all.top_k_all, a.chunks);
+        hipLaunchKernelGGL((k_sample_first<S>), parts, block, 0, s, a);
+        if (!lists)
+            hipLaunchKernelGGL((k_sample_weigh<S>), parts, block, 0, s, a);
+        if (!lists && has_nucleus(all))
+            hipLaunchKernelGGL((k_sample_edge<S>), parts, block, 0, s, a);
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess)
             return err;
@@ -1011,15 +1332,17 @@ size_t sample_scratch_bytes(const SampleArgs &g)
     }
 }
 
-hipError_t launch_sample(hipStream_t s, const SampleArgs &g, void *scratch)
+size_t sample_state_bytes() { return kSlabRows * sizeof(RowState); }
+
+hipError_t launch_sample(hipStream_t s, const SampleArgs &g, void *scratch, void *state)
 {
     if (g.rows == 0)
         return hipSuccess;
     switch (g.dtype) {
-    case kLogitF32: return launch_t<float>(s, g, scratch);
-    case kLogitF64: return launch_t<double>(s, g, scratch);
-    case kLogitBf16: return launch_t<__bf16>(s, g, scratch);
-    default: return launch_t<_Float16>(s, g, scratch);
+    case kLogitF32: return launch_t<float>(s, g, scratch, state);
+    case kLogitF64: return launch_t<double>(s, g, scratch, state);
+    case kLogitBf16: return launch_t<__bf16>(s, g, scratch, state);
+    default: return launch_t<_Float16>(s, g, scratch, state);
     }
 }
 

@@ -82,7 +82,7 @@ template <typename S, int NT, int R, int G, int CAP> __global__ __launch_bounds_
     const uint32_t n = g.vocab, k = g.k < n ? g.k : n;
     const Row<S, NT, R> held(s, n);
 
-    T group[G];
+    T group[G], largest[R ? R : 1]; // of the groups, and of each held vector
 #pragma unroll
     for (int i = 0; i < G; i++)
         group[i] = -INFINITY;
@@ -92,6 +92,8 @@ template <typename S, int NT, int R, int G, int CAP> __global__ __launch_bounds_
 #pragma unroll
         for (uint32_t i = 1; i < N; i++)
             top = OpMax()(top, v[i]);
+        if constexpr (R > 0)
+            largest[step] = top;
         group[step % G] = OpMax()(group[step % G], top);
     });
     T m = group[0];
@@ -114,16 +116,19 @@ template <typename S, int NT, int R, int G, int CAP> __global__ __launch_bounds_
     if (k > 0) {
         if (tid == 0)
             list.count = 0;
-        const T t = bound_of<NT>(group, m, k, bound, red[2]); // its barriers order the count
-        held.walk([&](const T *v, uint32_t at, int) {
-#pragma unroll
-            for (uint32_t i = 0; i < N; i++)
-                if (v[i] >= t && at < held.whole * N) // a held vector past the row is all minus infinity
-                    list.add(key_of(v[i]), at + i);
-        });
+        const uint32_t wanted[1] = {k};
+        const T t = bounds_of<NT>(group, m, wanted, bound, red[2]).t[0]; // its barriers order the count
+        if (R > 0 && t > -INFINITY)
+            list.add_from(s, largest, t, [&](int r, auto f) { f(tid + (uint32_t)r * NT); });
+        else
+            held.walk([&](const T *v, uint32_t at, int) {
+                if (at < held.whole * N) // a held vector past the row is all minus infinity
+                    list.template add_of<N>(v, [&](T x, int) { return x >= t; }, [&](int i) { return at + i; });
+            });
         if (held.has_extra && held.extra >= t)
             list.add(key_of(held.extra), held.extra_at());
         __syncthreads();
+        list.template fill_keys<NT>(s);
         // Fewer than k: the rest of the row are NaNs.
         uint32_t found = list.count;
         __syncthreads();

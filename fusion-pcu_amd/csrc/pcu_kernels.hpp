@@ -351,8 +351,12 @@ struct SampleArgs {
     unsigned long long *fault = nullptr;
     NodeGate gate{nullptr, 0};
 };
+// Scratch of sample_scratch_bytes (0: none, and no state either), and a state of
+// sample_state_bytes that is zero at the first call and that every call leaves zero unless the stage
+// gate closes while it runs.
 size_t sample_scratch_bytes(const SampleArgs &g);
-hipError_t launch_sample(hipStream_t s, const SampleArgs &g, void *scratch);
+size_t sample_state_bytes();
+hipError_t launch_sample(hipStream_t s, const SampleArgs &g, void *scratch, void *state);
 
 // Small device utilities (fill kernels rather than memsets, so a captured graph replays
 // them as kernels).

@@ -112,7 +112,10 @@ struct Ctx {
         void *p = nullptr;
         size_t cap = 0;
     };
-    Scratch matmul_scratch, mse_scratch, bt_scratch, table_scratch, logits_scratch;
+    Scratch matmul_scratch, mse_scratch, bt_scratch, table_scratch, logits_scratch, sample_state;
+    // The counters of the sampler's rows (sample_state) are zero. Not so before their first use
+    // and after a fault: a stage gate that closes during a launch leaves some of them counted.
+    bool sample_state_zero = false;
     uint32_t screen_gen = 0; // generation of the latest MatMul exponent screen
     // Buffers released by the caller are kept for reuse by an allocation of the same size
     // (a training step frees its previous weights and takes as many new ones of the same

@@ -177,6 +177,49 @@ template <typename K, int CAP> struct List {
             at[j] = i;
         }
     }
+    // Of M values the indices of those that `wanted` says, value i at index index_of(i); their keys
+    // are put in by fill_keys, all at once.
+    template <int M, typename T, typename W, typename I>
+    __device__ __forceinline__ void add_of(const T *v, W wanted, I index_of)
+    {
+        static_assert(M <= 32, "one bit a value");
+        uint32_t mask = 0;
+#pragma unroll
+        for (int i = 0; i < M; i++)
+            mask |= wanted(v[i], i) ? 1u << i : 0u;
+        if (mask) {
+            uint32_t j = atomicAdd(&count, (uint32_t)__builtin_popcount(mask));
+            for (; mask; mask &= mask - 1, j++)
+                if (j < CAP)
+                    at[j] = index_of(__builtin_ctz(mask));
+        }
+    }
+    // The indices of the values that reach t (t > minus infinity) in those of a thread's M vectors whose
+    // largest values do; vector_of(i, f) calls f(index) for the vectors of group i, and they are read again
+    // (they are in the caches): few lanes have any, and hardly one has two.
+    template <int M, typename S, typename T, typename V>
+    __device__ __forceinline__ void add_from(const S *row, const T (&largest)[M], T t, V vectors_of)
+    {
+        constexpr int N = kVec<S>;
+        uint32_t mask = 0;
+#pragma unroll
+        for (int i = 0; i < M; i++)
+            mask |= largest[i] >= t ? 1u << i : 0u;
+        for (; mask; mask &= mask - 1)
+            vectors_of(__builtin_ctz(mask), [&](uint32_t vec) {
+                T v[N];
+                unpack<S>(load_whole(row, vec), v);
+                add_of<N>(v, [&](T x, int) { return x >= t; }, [&](int e) { return vec * N + (uint32_t)e; });
+            });
+    }
+    // Whole workgroup, after a barrier; ends with one.
+    template <int NT, typename S> __device__ __forceinline__ void fill_keys(const S *row)
+    {
+        const uint32_t n = count < CAP ? count : CAP;
+        for (uint32_t j = threadIdx.x; j < n; j += NT)
+            key[j] = key_of((typename StatOf<S>::T)row[at[j]]);
+        __syncthreads();
+    }
 };
 
 // Sorts the list's first n entries by key descending, index ascending (n <= CAP, a power of two);
@@ -206,7 +249,7 @@ template <int NT, typename K, int CAP> __device__ __forceinline__ void sort_list
                 }
 #pragma unroll
                 for (uint32_t u = 0; u < kAtOnce; u++)
-                    place += o[u] > k || (o[u] == k && a[u] < i);
+                    place += (o[u] > k) | ((o[u] == k) & (a[u] < i));
             }
         }
         __syncthreads();
@@ -278,78 +321,81 @@ template <typename H> __device__ __forceinline__ Digit<H> find_digit(const H *bi
 }
 
 
-// Entries (key, index) that a workgroup holds, PER a thread.
-template <typename K, int PER> struct Held {
-    K key[PER];
-    uint32_t at[PER];
-};
 template <typename K> struct SelectShared {
     Digit<unsigned long long> digit;
     unsigned long long bins[256];
+    uint32_t counts[256];
     K varying[2][16];
-    uint32_t left[16];
     K key;
     uint32_t at;
 };
 
-// In the order (key descending, index ascending), or by index alone (BY_INDEX), the entry at which
-// the running sum of the measures reaches `need` (1 <= need <= their sum; entries of measure 0 do
-// not count): its key and index in sh, after a barrier. 8 bits a step, from the highest bit in
-// which the keys differ, until one entry is left.
-template <int NT, bool BY_INDEX, typename K, int PER>
-__device__ __forceinline__ void select_entry(const Held<K, PER> &e, const unsigned long long (&measure)[PER],
-                                             unsigned long long need, int index_bits, SelectShared<K> &sh)
+// Among `count` entries, entry(j) giving (key, index), in the order (key descending, index
+// ascending) or by index alone (BY_INDEX): the entry at which the running sum of
+// measure(key, index) reaches `need` (1 <= need <= their sum; entries of measure 0 do not count).
+// Its key and index are in sh after a barrier. 8 bits a step, from the highest bit in which the
+// keys differ, until one entry is left; indices are below 2^index_bits and differ.
+template <int NT, bool BY_INDEX, typename K, typename E, typename M>
+__device__ __forceinline__ void select_entry(uint32_t count, E entry, M measure, unsigned long long need, int index_bits,
+                                             SelectShared<K> &sh)
 {
-    bool in[PER];
-#pragma unroll
-    for (int b = 0; b < PER; b++)
-        in[b] = measure[b] != 0;
+    K key_bits = 0, key_mask = 0;          // of the key, found so far
+    uint32_t at_bits = 0, at_mask = 0;     // of the index' complement
     int shift = index_bits > 8 ? index_bits - 8 : 0;
     bool by_key = !BY_INDEX;
     if (by_key) {
-        K some = 0, all = 0; // bits set in some key, bits clear in some key
-#pragma unroll
-        for (int b = 0; b < PER; b++)
-            if (in[b]) {
-                some |= e.key[b];
-                all |= ~e.key[b];
-            }
+        K some = 0, none = 0; // bits set in some key, bits clear in some key
+        for (uint32_t j = threadIdx.x; j < count; j += NT) {
+            const K key = entry(j).key;
+            some |= key;
+            none |= ~key;
+        }
         some = block_reduce<NT>(some, OpOr(), sh.varying[0]);
-        all = block_reduce<NT>(all, OpOr(), sh.varying[1]);
-        const K varying = some & all;
+        none = block_reduce<NT>(none, OpOr(), sh.varying[1]);
+        const K varying = some & none;
+        key_bits = some & ~none; // the bits that all share
+        key_mask = ~varying;
         const int top = varying == 0 ? -1 : (sizeof(K) == 8 ? 63 - __builtin_clzll(varying) : 31 - __builtin_clz((uint32_t)varying));
         if (top < 0)
             by_key = false;
         else
             shift = top > 7 ? top - 7 : 0;
     }
-    for (int step = 0; step < (int)sizeof(K) + 4; step++) { // at most every byte of a key and an index
-        for (uint32_t b = threadIdx.x; b < 256; b += NT)
+    for (int step = 0; step < (int)sizeof(K) + 5; step++) { // at most every byte of a key and an index
+        for (uint32_t b = threadIdx.x; b < 256; b += NT) {
             sh.bins[b] = 0;
+            sh.counts[b] = 0;
+        }
         __syncthreads();
-        uint32_t digit[PER];
-#pragma unroll
-        for (int b = 0; b < PER; b++) {
-            digit[b] = (by_key ? (uint32_t)(e.key[b] >> shift) : ~e.at[b] >> shift) & 255u;
-            if (in[b])
-                atomicAdd(&sh.bins[digit[b]], measure[b]);
+        auto digit_of = [&](const auto &e) { return (by_key ? (uint32_t)(e.key >> shift) : ~e.at >> shift) & 255u; };
+        auto in = [&](const auto &e) { return (BY_INDEX || (e.key & key_mask) == key_bits) && (~e.at & at_mask) == at_bits; };
+        for (uint32_t j = threadIdx.x; j < count; j += NT) {
+            const auto e = entry(j);
+            if (in(e)) {
+                const unsigned long long w = measure(e.key, e.at);
+                if (w) {
+                    atomicAdd(&sh.bins[digit_of(e)], w);
+                    atomicAdd(&sh.counts[digit_of(e)], 1u);
+                }
+            }
         }
         const Digit<unsigned long long> d = find_digit(sh.bins, need, &sh.digit);
         need = d.left;
-        uint32_t left = 0;
-#pragma unroll
-        for (int b = 0; b < PER; b++) {
-            in[b] = in[b] && digit[b] == d.digit;
-            left += in[b];
+        if (by_key) {
+            key_bits |= (K)d.digit << shift;
+            key_mask |= (K)255 << shift;
+        } else {
+            at_bits |= d.digit << shift;
+            at_mask |= 255u << shift;
         }
-        left = block_reduce<NT>(left, OpSum(), sh.left);
-        if (left == 1) {
-#pragma unroll
-            for (int b = 0; b < PER; b++)
-                if (in[b]) {
-                    sh.key = e.key[b];
-                    sh.at = e.at[b];
+        if (sh.counts[d.digit] == 1) {
+            for (uint32_t j = threadIdx.x; j < count; j += NT) {
+                const auto e = entry(j);
+                if (in(e) && measure(e.key, e.at)) {
+                    sh.key = e.key;
+                    sh.at = e.at;
                 }
+            }
             __syncthreads();
             return;
         }
@@ -359,21 +405,26 @@ __device__ __forceinline__ void select_entry(const Held<K, PER> &e, const unsign
             by_key = false;
             shift = index_bits > 8 ? index_bits - 8 : 0;
         }
+        __syncthreads(); // the counts are read
     }
 }
 
 // What a bound's search keeps in LDS.
 struct BoundScratch {
     uint32_t bins[256];
-    uint32_t bin, wave_min_at;
+    uint32_t bin[2];
+};
+template <typename T> struct Bounds {
+    T t[2];
 };
 
-// A bound that at least k of the row's values reach, from the largest value of each of this
+// Bounds that at least k[0], and k[1], of the values reach, from the largest value of each of this
 // thread's G groups: a histogram of the group maxima in 256 even steps from the row's maximum
 // m down to their smallest finite one, and the smallest group maximum in the bins that
 // together hold k groups. Minus infinity where fewer than k groups have a finite maximum.
-template <int NT, int G, typename T>
-__device__ __forceinline__ T bound_of(const T (&group)[G], T m, uint32_t k, BoundScratch &sc, T *red)
+// `red`: 3 x 16 places.
+template <int NT, int G, int COUNT, typename T>
+__device__ __forceinline__ Bounds<T> bounds_of(const T (&group)[G], T m, const uint32_t (&k)[COUNT], BoundScratch &sc, T *red)
 {
     T low = INFINITY;
 #pragma unroll
@@ -382,6 +433,8 @@ __device__ __forceinline__ T bound_of(const T (&group)[G], T m, uint32_t k, Boun
             low = group[g] < low ? group[g] : low;
     for (uint32_t b = threadIdx.x; b < 256; b += NT)
         sc.bins[b] = 0;
+    if (threadIdx.x < COUNT)
+        sc.bin[threadIdx.x] = 256;
     low = -block_reduce<NT>(-low, OpMax(), red);
     if constexpr (NT == 64)
         __syncthreads();
@@ -390,12 +443,13 @@ __device__ __forceinline__ T bound_of(const T (&group)[G], T m, uint32_t k, Boun
         const float x = (float)((m - v) * scale);
         return x < 255.0f ? (uint32_t)x : (x >= 255.0f ? 255u : 0u);
     };
+    uint32_t bin[G];
 #pragma unroll
-    for (int g = 0; g < G; g++)
-        if (group[g] > -INFINITY)
-            atomicAdd(&sc.bins[bin_of(group[g])], 1u);
-    if (threadIdx.x == 0)
-        sc.bin = 256;
+    for (int g = 0; g < G; g++) {
+        bin[g] = group[g] > -INFINITY ? bin_of(group[g]) : 256;
+        if (bin[g] < 256)
+            atomicAdd(&sc.bins[bin[g]], 1u);
+    }
     __syncthreads();
     if (threadIdx.x < 64) {
         const uint32_t first = 4 * threadIdx.x;
@@ -405,26 +459,34 @@ __device__ __forceinline__ T bound_of(const T (&group)[G], T m, uint32_t k, Boun
             b[i] = sc.bins[first + i];
             own += b[i];
         }
-        uint32_t before = wave_inclusive_sum(own) - own;
-        if (before < k && k <= before + own) {
+        const uint32_t upto = wave_inclusive_sum(own);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (before < k && k <= before + b[i])
-                    sc.bin = first + i;
-                before += b[i];
+        for (int c = 0; c < COUNT; c++) {
+            uint32_t before = upto - own;
+            if (before < k[c] && k[c] <= upto) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (before < k[c] && k[c] <= before + b[i])
+                        sc.bin[c] = first + i;
+                    before += b[i];
+                }
             }
         }
     }
     __syncthreads();
-    const uint32_t last = sc.bin;
-    if (last == 256)
-        return -INFINITY;
-    T least = INFINITY;
+    Bounds<T> out;
 #pragma unroll
-    for (int g = 0; g < G; g++)
-        if (group[g] > -INFINITY && bin_of(group[g]) <= last)
-            least = group[g] < least ? group[g] : least;
-    return -block_reduce<NT>(-least, OpMax(), red + 16);
+    for (int c = 0; c < COUNT; c++) {
+        const uint32_t last = sc.bin[c];
+        T least = INFINITY;
+#pragma unroll
+        for (int g = 0; g < G; g++)
+            if (bin[g] <= last && bin[g] < 256)
+                least = group[g] < least ? group[g] : least;
+        least = -block_reduce<NT>(-least, OpMax(), red + 16 * (c + 1));
+        out.t[c] = last == 256 ? (T)-INFINITY : least;
+    }
+    return out;
 }
 
 // ---------------------------------------------------------------- digit by digit

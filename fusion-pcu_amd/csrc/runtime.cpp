@@ -151,7 +151,8 @@ Ctx::~Ctx()
         (void)hipStreamSynchronize(stream);
     if (side)
         (void)hipStreamSynchronize(side);
-    for (Scratch *b : {&matmul_scratch, &mse_scratch, &bt_scratch, &table_scratch, &logits_scratch})
+    for (Scratch *b : {&matmul_scratch, &mse_scratch, &bt_scratch, &table_scratch, &logits_scratch,
+                       &sample_state})
         if (b->p)
             (void)hipFreeAsync(b->p, stream);
     for (const Released &r : reuse)
@@ -521,13 +522,17 @@ pcu_status Ctx::end_program_all(std::vector<pcu_fault> *faults)
         if (host_words[i] == kNoFaultWord)
             continue;
         pcu_fault f;
-        if ((st = decode_node(i, &f)))
+        if ((st = decode_node(i, &f))) {
+            sample_state_zero = false;
             return st;
+        }
         faults->push_back(f);
     }
     has_held_fault = !faults->empty();
-    if (has_held_fault)
+    if (has_held_fault) {
         held_fault = faults->front();
+        sample_state_zero = false;
+    }
     return PCU_OK;
 }
 
@@ -545,6 +550,7 @@ pcu_status Ctx::end_program(pcu_fault *first)
             continue;
         pcu_fault f;
         if ((st = decode_node(i, &f))) {
+            sample_state_zero = false;
             if (first)
                 *first = protocol_fault;
             return st;
@@ -558,6 +564,7 @@ pcu_status Ctx::end_program(pcu_fault *first)
     if (!found)
         return PCU_OK;
     held_fault = earliest;
+    sample_state_zero = false;
     if (first)
         *first = earliest;
     return PCU_ARITHMETIC_FAULT;
