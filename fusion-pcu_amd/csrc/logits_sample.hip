@@ -176,7 +176,7 @@ __device__ __forceinline__ Last<typename StatOf<S>::T> last_of(const S *s, uint3
 template <typename T, int NT> struct DrawShared {
     Digit<uint32_t> count_digit;
     Digit<mass_t> mass_digit;
-    mass_t red[4][16], tiles[64];
+    mass_t red[4][16], tiles[16];
     uint32_t wave_ties[16], found_at, end;
     SelectShared<typename KeyOf<T>::K> select;
     mass_t steps[kSteps]; // masses of the steps of z, then bins of other searches
@@ -406,13 +406,13 @@ __device__ __forceinline__ void draw_from_list(const SampleArgs &g, uint64_t row
 
 // Draws along vectors [from, to) of the row (`mass_of` a value and its index). total 0: the vectors
 // are the whole row, and its mass is counted first; else `target` of it lies in the vectors.
-// `lds`: 64 places.
+// `lds`: 16 places.
 template <typename S, typename F>
 __device__ __forceinline__ void draw_along(const SampleArgs &g, uint64_t row, const S *s, uint32_t from, uint32_t to,
                                            uint32_t draw, mass_t total, mass_t target, F mass_of, mass_t *lds)
 {
     using T = typename StatOf<S>::T;
-    constexpr uint32_t N = kVec<S>, NT = 256, kTiles = 16, U = 4;
+    constexpr uint32_t N = kVec<S>, NT = 256, U = 4;
     const uint32_t wave = threadIdx.x / 64, lane = threadIdx.x & 63, n = g.vocab;
     auto mass_in = [&](const u32x4 &raw, uint32_t i, mass_t *w) {
         T v[N];
@@ -424,6 +424,8 @@ __device__ __forceinline__ void draw_along(const SampleArgs &g, uint64_t row, co
             if (w)
                 w[e] = x;
             sum += x;
+            if (e % 4 == 3) // eight exponentials at once would take the registers of two waves
+                one_at_a_time();
         }
         return sum;
     };
@@ -443,24 +445,21 @@ __device__ __forceinline__ void draw_along(const SampleArgs &g, uint64_t row, co
         target = share_of(total, draw);
         __syncthreads();
     }
-    // Tiles of one vector a thread, 16 at a time: the masses of each tile's four waves, in index
+    // Tiles of one vector a thread, four at a time: the masses of each tile's four waves, in index
     // order, then within the wave that holds the target.
-    for (uint32_t at = from; at < to; at += NT * kTiles) {
-#pragma unroll 1
-        for (uint32_t t = 0; t < kTiles; t += U) {
-            u32x4 raw[U];
+    for (uint32_t at = from; at < to; at += NT * U) {
+        u32x4 raw[U];
 #pragma unroll
-            for (uint32_t u = 0; u < U; u++)
-                raw[u] = load(at + (t + u) * NT + threadIdx.x);
+        for (uint32_t t = 0; t < U; t++)
+            raw[t] = load(at + t * NT + threadIdx.x);
 #pragma unroll
-            for (uint32_t u = 0; u < U; u++) {
-                const mass_t sum = wave_reduce(mass_in(raw[u], at + (t + u) * NT + threadIdx.x, nullptr), OpSum());
-                if (lane == 0)
-                    lds[(t + u) * 4 + wave] = sum;
-            }
+        for (uint32_t t = 0; t < U; t++) {
+            const mass_t sum = wave_reduce(mass_in(raw[t], at + t * NT + threadIdx.x, nullptr), OpSum());
+            if (lane == 0)
+                lds[t * 4 + wave] = sum;
         }
         __syncthreads();
-        const mass_t here = lds[lane], upto = wave_inclusive_sum(here), all = from_lane(upto, 63);
+        const mass_t here = lane < 4 * U ? lds[lane] : 0, upto = wave_inclusive_sum(here), all = from_lane(upto, 63);
         if (target >= all) {
             target -= all;
             __syncthreads(); // the masses are read
@@ -701,7 +700,7 @@ template <typename T> struct ChunkPart {
 
 constexpr uint32_t kRowCap = 8192; // of a row's list
 constexpr int kChunkThreads = 256;
-constexpr int kChunkListCap = 1024;
+constexpr int kChunkListCap = 1024, kEdgeListCap = 2048; // in LDS
 
 template <typename T> struct SplitArgs {
     SampleArgs g;
@@ -771,35 +770,36 @@ template <typename S> struct Chunk {
         }
         rest = chunk == chunks - 1 ? whole * N + threadIdx.x : n;
     }
-    static constexpr int U = 4; // vectors in flight
-    // f(values, their number, index of value i by index_of(i)), for four vectors at a time; places
+    // f(values, their number, index of the first) for each vector, four loads in flight; places
     // past the chunk hold minus infinity.
-    template <typename F> __device__ __forceinline__ void groups(F f) const
+    template <typename F> __device__ __forceinline__ void vectors(F f) const
     {
+        constexpr int U = 4;
         for (uint32_t i = first + threadIdx.x; i < past; i += step * U) {
             u32x4 in[U];
-            T v[U * N];
 #pragma unroll
             for (int u = 0; u < U; u++)
                 in[u] = i + u * step < past ? load_whole(s, i + u * step) : minus_infinities<S>();
 #pragma unroll
-            for (int u = 0; u < U; u++)
-                unpack<S>(in[u], v + u * N);
-            f(v, std::integral_constant<int, U * (int)N>(),
-              [&](int k) { return (i + (uint32_t)k / N * step) * N + (uint32_t)k % N; });
+            for (int u = 0; u < U; u++) {
+                T v[N];
+                unpack<S>(in[u], v);
+                f(v, std::integral_constant<int, (int)N>(), (i + u * step) * N);
+                one_at_a_time();
+            }
         }
         if (rest < n) {
             const T v[1] = {(T)s[rest]};
-            f(v, std::integral_constant<int, 1>(), [&](int) { return rest; });
+            f(v, std::integral_constant<int, 1>(), rest);
         }
     }
-    // f(value, index, vector of the four)
+    // f(value, index)
     template <typename F> __device__ __forceinline__ void each(F f) const
     {
-        groups([&](const T *v, auto count, auto index_of) {
+        vectors([&](const T *v, auto count, uint32_t at) {
 #pragma unroll
             for (int k = 0; k < count; k++)
-                f(v[k], index_of(k), k / (int)N);
+                f(v[k], at + k);
         });
     }
     // The largest values of this thread's vectors, every eighth of them in one group.
@@ -846,8 +846,8 @@ template <typename S> struct Chunk {
         if (threadIdx.x == 0)
             list.count = 0;
         __syncthreads();
-        groups([&](const T *v, auto count, auto index_of) {
-            list.template add_of<decltype(count)::value>(v, [&](T x, int) { return wanted(x); }, index_of);
+        vectors([&](const T *v, auto count, uint32_t at) {
+            list.template add_of<decltype(count)::value>(v, [&](T x, int) { return wanted(x); }, [&](int k) { return at + k; });
         });
         __syncthreads();
         list.template fill_keys<kChunkThreads>(s);
@@ -1023,7 +1023,7 @@ template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_
         own = b.t[1];
     } else if (kind == kRowNucleus) {
         t = INFINITY;
-        part.each([&](T v, uint32_t, int) { t = v > -INFINITY && v < t ? v : t; });
+        part.each([&](T v, uint32_t) { t = v > -INFINITY && v < t ? v : t; });
         t = -block_reduce<NT>(-t, OpMax(), red[1]);
     }
     if (threadIdx.x == 0) {
@@ -1091,7 +1091,7 @@ template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_
             return w >= set.least ? w : 0;
         };
         mass_t own = 0;
-        part.each([&](T v, uint32_t at, int) { own += mass_of(v, at); });
+        part.each([&](T v, uint32_t at) { own += mass_of(v, at); });
         own = block_reduce<NT>(own, OpSum(), sh.red[0]);
         if (threadIdx.x == 0)
             put(&a.chunk_mass[blockIdx.x], own);
@@ -1107,7 +1107,7 @@ template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_
         sh.steps[b] = 0;
     __syncthreads();
     const StepOf<T> step_of(m, set.inv, low);
-    part.each([&](T v, uint32_t, int) {
+    part.each([&](T v, uint32_t) {
         if (const mass_t w = weight(v))
             atomicAdd(&sh.steps[step_of(v)], w);
     });
@@ -1153,7 +1153,7 @@ template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_
         return;
     __shared__ BoundScratch bound;
     __shared__ T red[4][16];
-    __shared__ List<K, kChunkListCap> list;
+    __shared__ List<K, kEdgeListCap> list;
     __shared__ DrawShared<T, NT> sh;
     __shared__ mass_t in_chunk[64];
     const uint64_t row = blockIdx.x / a.chunks;
@@ -1172,7 +1172,7 @@ template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_
     part.gather(list, [&](T v) { return v > -INFINITY && step_of(v) == end; });
     if (set.least > 0) { // of the chunk's mass before the step, what min_p leaves
         mass_t own = 0;
-        part.each([&](T v, uint32_t, int) {
+        part.each([&](T v, uint32_t) {
             if (v > -INFINITY && step_of(v) < end) {
                 const mass_t w = weight(v);
                 own += w >= set.least ? w : 0;
@@ -1207,7 +1207,7 @@ template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_
                 atomicAdd(&in_chunk[c < a.chunks ? c : a.chunks - 1], w);
         }
     };
-    if (list.count <= kChunkListCap)
+    if (list.count <= kEdgeListCap)
         finish(LocalList<K>{list.key, list.at});
     else
         finish(SharedList<K>{a.key + row * kRowCap, a.at + row * kRowCap});

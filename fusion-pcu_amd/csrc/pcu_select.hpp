@@ -63,28 +63,18 @@ template <typename T> __device__ __forceinline__ T wave_inclusive_sum(T v) { ret
 // --------------------------------------------------------------------- the row
 
 // Calls f(values, first index, count of real ones) for every vector of the row, each thread its
-// own ones, four loads in flight.
+// own ones. One at a time: it serves rare rows, in kernels whose registers it must not raise.
 template <typename S, int NT, typename F>
 __device__ __forceinline__ void each_vec(const S *row, uint32_t n, F f)
 {
     using T = typename StatOf<S>::T;
     constexpr uint32_t N = kVec<S>;
-    constexpr int U = 4;
     const uint32_t vecs = (n + N - 1) / N;
-    for (uint32_t i = threadIdx.x; i < vecs; i += NT * U) {
-        u32x4 raw[U];
-#pragma unroll
-        for (int u = 0; u < U; u++)
-            raw[u] = load_vec(row, i + u * NT, n);
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const uint32_t at = (i + u * NT) * N;
-            if (at < n) {
-                T v[N];
-                unpack<S>(raw[u], v);
-                f(v, at, n - at < N ? n - at : N);
-            }
-        }
+#pragma unroll 1
+    for (uint32_t i = threadIdx.x; i < vecs; i += NT) {
+        T v[N];
+        unpack<S>(load_vec(row, i, n), v);
+        f(v, i * N, n - i * N < N ? n - i * N : N);
     }
 }
 
