@@ -138,9 +138,18 @@ def _logit_code(what: str, dtype) -> int:
         raise PcuExecutionError(_abi.PCU_ERR_UNSUPPORTED, f"{what}: unsupported scalar type {dtype}")
 
 
+_FLOAT32, _FLOAT64, _INT32 = np.dtype(np.float32), np.dtype(np.float64), np.dtype(np.int32)
+
+
 def _stat_dtype(dtype) -> np.dtype:
     """The type of a row's statistics: binary32, binary64 for binary64 rows."""
-    return np.dtype(np.float64 if dtype == np.float64 else np.float32)
+    return _FLOAT64 if dtype is _FLOAT64 or dtype == _FLOAT64 else _FLOAT32
+
+
+def _need(what: str, x: "DeviceArray", shape: Tuple[int, ...], dtype: np.dtype) -> None:
+    """_require on a path that a token takes: shape a tuple, dtype a numpy dtype."""
+    if x.shape != shape or (x.dtype is not dtype and x.dtype != dtype):
+        _require(what, x, shape, dtype)
 
 
 def _require(what: str, x: "DeviceArray", shape, dtype) -> None:
@@ -480,7 +489,7 @@ class Context:
     def _out(self, what: str, x: Optional[DeviceArray], shape, dtype) -> DeviceArray:
         if x is None:
             return self.empty(shape, dtype)
-        _require(what, x, shape, dtype)
+        _need(what, x, shape, dtype)
         return x
 
     def native_top_logits(self, logits: DeviceArray, k: int, temperature: float = 1.0,
@@ -496,7 +505,7 @@ class Context:
             raise PcuExecutionError(_abi.PCU_ERR_SHAPE, f"top_logits: k {k} is not in [0, {_abi.LOGITS_MAX_K}]")
         rows = logits.shape[0]
         values = self._out("values", values, (rows, k), logits.dtype)
-        indices = self._out("indices", indices, (rows, k), np.int32)
+        indices = self._out("indices", indices, (rows, k), _INT32)
         log_sum = self._out("log_sum", log_sum, (rows,), _stat_dtype(logits.dtype))
         self.check(self._lib.pcu_native_top_logits(self.handle, ctypes.byref(lg), k, temperature, values.ptr,
                                                    indices.ptr, log_sum.ptr))
@@ -513,12 +522,12 @@ class Context:
         if k > _abi.LOGITS_MAX_K:
             raise PcuExecutionError(_abi.PCU_ERR_SHAPE, f"distill: {k} entries a row are beyond {_abi.LOGITS_MAX_K}")
         code = _logit_code("teacher values", teacher_values.dtype)
-        _require("teacher values", teacher_values, (rows, k), teacher_values.dtype)
-        _require("teacher indices", teacher_indices, (rows, k), np.int32)
+        _need("teacher values", teacher_values, (rows, k), teacher_values.dtype)
+        _need("teacher indices", teacher_indices, (rows, k), _INT32)
         if teacher_log_sum is not None:
-            _require("teacher log-sum", teacher_log_sum, (rows,), _stat_dtype(teacher_values.dtype))
+            _need("teacher log-sum", teacher_log_sum, (rows,), _stat_dtype(teacher_values.dtype))
         if labels is not None:
-            _require("labels", labels, (rows,), np.int32)
+            _need("labels", labels, (rows,), _INT32)
         return lg, _abi.Distill(teacher_values.ptr, teacher_indices.ptr,
                                 teacher_log_sum.ptr if teacher_log_sum is not None else None,
                                 labels.ptr if labels is not None else None, code, k, temperature,
@@ -556,9 +565,9 @@ class Context:
         lg, d = self._distill(student, teacher_values, teacher_indices, teacher_log_sum, labels, temperature,
                               distill_weight, label_weight, vocab)
         (rows, cols), stat = student.shape, _stat_dtype(student.dtype)
-        _require("log_sums", log_sums, (rows, 2), stat)
+        _need("log_sums", log_sums, (rows, 2), stat)
         if row_scale is not None:
-            _require("row_scale", row_scale, (rows,), stat)
+            _need("row_scale", row_scale, (rows,), stat)
         gradient = self._out("gradient", gradient, student.shape, student.dtype)
         self._call(self._lib.pcu_native_distill_backward, ctypes.byref(lg), ctypes.byref(d), log_sums.ptr,
                    row_scale.ptr if row_scale is not None else None, gradient.ptr, cols, cols)
@@ -576,7 +585,7 @@ class Context:
                               distill_weight, label_weight, vocab)
         (rows, cols), stat = student.shape, _stat_dtype(student.dtype)
         if row_scale is not None:
-            _require("row_scale", row_scale, (rows,), stat)
+            _need("row_scale", row_scale, (rows,), stat)
         loss = self._out("loss", loss, (rows,), stat)
         gradient = self._out("gradient", gradient, student.shape, student.dtype)
         self._call(self._lib.pcu_native_distill_step, ctypes.byref(lg), ctypes.byref(d),
@@ -593,15 +602,15 @@ class Context:
         (see pcu_native_sample)."""
         lg = self._logits("sample", logits, vocab)
         rows = logits.shape[0]
-        _require("uniform", uniform, (rows,), np.float32)
+        _need("uniform", uniform, (rows,), _FLOAT32)
         p = _abi.Sampling(uniform=uniform.ptr)
         for name, x in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
             if isinstance(x, DeviceArray):
-                _require(name, x, (rows,), np.int32 if name == "top_k" else np.float32)
+                _need(name, x, (rows,), _INT32 if name == "top_k" else _FLOAT32)
                 setattr(p, name, x.ptr)
             else:
                 setattr(p, name + "_value", x)
-        tokens = self._out("tokens", tokens, (rows,), np.int32)
-        log_prob = self._out("log_prob", log_prob, (rows,), np.float32)
+        tokens = self._out("tokens", tokens, (rows,), _INT32)
+        log_prob = self._out("log_prob", log_prob, (rows,), _FLOAT32)
         self._call(self._lib.pcu_native_sample, ctypes.byref(lg), ctypes.byref(p), tokens.ptr, log_prob.ptr)
         return tokens, log_prob

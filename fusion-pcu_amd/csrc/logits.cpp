@@ -91,9 +91,17 @@ pcu_status Ctx::op_top_logits(const pcu_logits *l, uint32_t k, double temperatur
     g.indices = indices;
     g.log_sum = log_sum;
     g.gate = gate_for(word);
+    ProgramClose close;
+    if (implicit_program && nodes.size() == 1)
+        close_next = true; // a call of its own: its kernel ends the program
+    if ((st = take_close(&close)))
+        return st;
+    bool closed = false;
     hipEvent_t t = timer_start(stream);
-    st = hip(launch_top(stream, g), "top_logits launch");
+    st = hip(launch_top(stream, g, close, &closed), "top_logits launch");
     timer_stop(PCU_KERNEL_TOP_LOGITS, t, stream);
+    if (!st && closed)
+        closed_seq = ++pub_seq;
     return st;
 }
 
@@ -232,6 +240,12 @@ pcu_status Ctx::op_sample(const pcu_logits *l, const pcu_sampling *p, int32_t *t
         return st;
     if ((st = open_words()))
         return st;
+    ProgramClose close;
+    if (implicit_program && nodes.size() == 1)
+        close_next = true; // a call of its own: its last kernel ends the program
+    if ((st = take_close(&close)))
+        return st;
+    bool closed = false;
     hipEvent_t ev = timer_start(stream);
     if (need && !sample_state_zero) {
         if ((st = hip(launch_fill_u64(stream, static_cast<unsigned long long *>(state), sample_state_bytes() / 8, 0),
@@ -239,10 +253,12 @@ pcu_status Ctx::op_sample(const pcu_logits *l, const pcu_sampling *p, int32_t *t
             return st;
         sample_state_zero = true;
     }
-    st = hip(launch_sample(stream, g, sc, state), "sample launch");
+    st = hip(launch_sample(stream, g, sc, state, close, &closed), "sample launch");
     if (st)
         sample_state_zero = false;
     timer_stop(PCU_KERNEL_SAMPLE, ev, stream);
+    if (!st && closed)
+        closed_seq = ++pub_seq;
     return st;
 }
 

@@ -75,6 +75,13 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs &g, uint64_t ro
     return s;
 }
 
+__device__ __forceinline__ void put_token(const SampleArgs &g, uint64_t row, int32_t token, float log_prob)
+{
+    put(g.tokens + row, token);
+    if (g.log_prob)
+        put(g.log_prob + row, log_prob);
+}
+
 // A row from which nothing can be drawn; an invalid setting is a fault. One thread.
 __device__ __forceinline__ void no_token(const SampleArgs &g, uint64_t row, bool ok)
 {
@@ -82,9 +89,7 @@ __device__ __forceinline__ void no_token(const SampleArgs &g, uint64_t row, bool
         atomicMin(g.fault, (unsigned long long)pack_fault(g.first_row + row, kInvalid));
         gate_record(g.gate);
     }
-    g.tokens[row] = -1;
-    if (g.log_prob)
-        g.log_prob[row] = -INFINITY;
+    put_token(g, row, -1, -INFINITY);
 }
 
 // The prefix of S_k = (tk, ck) that holds `need` (1 <= need <= mass of S_k).
@@ -356,9 +361,7 @@ __device__ __forceinline__ void draw_from_few(const SampleArgs &g, uint64_t row,
     }
     const mass_t target = share_of(total, set.draw);
     if (running <= target && target < running + own) {
-        g.tokens[row] = (int32_t)i;
-        if (g.log_prob)
-            g.log_prob[row] = logf((float)own / (float)total);
+        put_token(g, row, (int32_t)i, logf((float)own / (float)total));
     }
 }
 
@@ -397,11 +400,8 @@ __device__ __forceinline__ void draw_from_list(const SampleArgs &g, uint64_t row
     // The first by index at which the running mass passes the target.
     const mass_t total = mass_of_list<NT>(count, list, drawn, sh.red[1]);
     select_entry<NT, true>(count, list, drawn, share_of(total, set.draw) + 1, bits, sh.select);
-    if (threadIdx.x == 0) {
-        g.tokens[row] = (int32_t)sh.select.at;
-        if (g.log_prob)
-            g.log_prob[row] = logf((float)weight(value_of(sh.select.key)) / (float)total);
-    }
+    if (threadIdx.x == 0)
+        put_token(g, row, (int32_t)sh.select.at, logf((float)weight(value_of(sh.select.key)) / (float)total));
 }
 
 // Draws along vectors [from, to) of the row (`mass_of` a value and its index). total 0: the vectors
@@ -476,11 +476,8 @@ __device__ __forceinline__ void draw_along(const SampleArgs &g, uint64_t row, co
             mass_t running = before;
 #pragma unroll
             for (uint32_t e = 0; e < N; e++) {
-                if (running <= target && target < running + w[e]) {
-                    g.tokens[row] = (int32_t)(i * N + e);
-                    if (g.log_prob)
-                        g.log_prob[row] = logf((float)w[e] / (float)total);
-                }
+                if (running <= target && target < running + w[e])
+                    put_token(g, row, (int32_t)(i * N + e), logf((float)w[e] / (float)total));
                 running += w[e];
             }
         }
@@ -494,7 +491,7 @@ __device__ __forceinline__ void draw_along(const SampleArgs &g, uint64_t row, co
 // everything else in LDS. Rows with a nucleus: the masses of even steps of z, then the list of the
 // values down to the step in which the nucleus ends, or, when that is long, of that step alone.
 // Then the drawing: over the list, or over the row.
-template <typename S, int NT, int R> __global__ __launch_bounds__(NT) void k_sample(SampleArgs g)
+template <typename S, int NT, int R> __device__ __forceinline__ void sample_row(const SampleArgs &g)
 {
     using T = typename StatOf<S>::T;
     using K = typename KeyOf<T>::K;
@@ -624,6 +621,13 @@ template <typename S, int NT, int R> __global__ __launch_bounds__(NT) void k_sam
     draw_along<S>(g, row, s, 0u, (n + N - 1) / N, set.draw, 0, 0, mass_of, sh.tiles);
 }
 
+// A call of its own ends its program in this kernel (close).
+template <typename S, int NT, int R> __global__ __launch_bounds__(NT) void k_sample(SampleArgs g, ProgramClose close)
+{
+    sample_row<S, NT, R>(g);
+    program_close_block(close);
+}
+
 // The drawing of a row whose lists did not suffice, or whose top_k no list holds: everything digit
 // by digit over the whole row.
 template <typename S, int NT, typename T>
@@ -729,11 +733,8 @@ __device__ __forceinline__ uint32_t kind_of(const Settings &s, uint32_t n, uint3
 }
 
 // What a chunk hands to the others of its row within a launch is written through the caches that
-// they do not share, and is complete (a wait for the wave's own stores, then the barrier) before the
-// workgroup counts itself as done.
-template <typename V> __device__ __forceinline__ void put(V *p, V v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-template <typename V> __device__ __forceinline__ V get(const V *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-
+// they do not share (put), and is complete (a wait for the wave's own stores, then the barrier)
+// before the workgroup counts itself as done.
 // Whether this workgroup is the last of the row's chunks; whole workgroup, once a launch.
 __device__ __forceinline__ bool last_chunk(uint32_t *done, uint32_t chunks)
 {
@@ -983,13 +984,13 @@ template <typename T> __device__ __forceinline__ ChunkPart<T> row_part(const Spl
 // The lowest finite value.
 template <typename T> __device__ __forceinline__ T lowest() { return sizeof(T) == 8 ? (T)-1.7976931348623157e308 : (T)-3.402823466e38f; }
 
-template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_first(SplitArgs<typename StatOf<S>::T> a)
+template <typename S> __device__ __forceinline__ bool sample_first(const SplitArgs<typename StatOf<S>::T> &a)
 {
     using T = typename StatOf<S>::T;
     using K = typename KeyOf<T>::K;
     constexpr int NT = kChunkThreads;
     if (block_gate_closed(a.g.gate))
-        return;
+        return blockIdx.x % a.chunks == 0;
     __shared__ BoundScratch bound;
     __shared__ T red[4][16];
     __shared__ List<K, kChunkListCap> list;
@@ -1001,7 +1002,7 @@ template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_
     if (kind == kRowNone) {
         if (chunk == 0 && threadIdx.x == 0)
             no_token(a.g, row, false);
-        return;
+        return chunk == 0;
     }
     const Chunk<S> part(static_cast<const S *>(a.g.logits) + row * a.g.stride, n, chunk, a.chunks, a.chunk_vecs,
                         kind == kRowList || kind == kRowBound);
@@ -1031,28 +1032,29 @@ template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_
         put(&a.part[blockIdx.x].t, t);
     }
     if (kind != kRowList)
-        return;
+        return false;
     own = own > lowest<T>() ? own : lowest<T>(); // minus infinity is never drawn
     part.gather(list, largest, own);
     hand_over(a, row, list);
     if (!last_chunk(&a.state[row].done[0], a.chunks))
-        return;
+        return false;
     const T top = row_part(a, row).m;
     if (top == -INFINITY) {
         if (threadIdx.x == 0)
             no_token(a.g, row, true);
-        return;
+        return true;
     }
     draw_from_row<S>(a, row, set, top, list, bound, red[0], sh);
+    return true;
 }
 
-template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_weigh(SplitArgs<typename StatOf<S>::T> a)
+template <typename S> __device__ __forceinline__ bool sample_weigh(const SplitArgs<typename StatOf<S>::T> &a)
 {
     using T = typename StatOf<S>::T;
     using K = typename KeyOf<T>::K;
     constexpr int NT = kChunkThreads;
     if (block_gate_closed(a.g.gate))
-        return;
+        return blockIdx.x % a.chunks == 0;
     __shared__ BoundScratch bound;
     __shared__ T red[4][16];
     __shared__ List<K, kChunkListCap> list;
@@ -1063,17 +1065,17 @@ template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_
     const Settings set = settings_of(a.g, row);
     const uint32_t kind = kind_of(set, n, a.chunks);
     if (kind == kRowNone || kind == kRowList)
-        return;
+        return chunk == 0;
     const auto [m, low] = row_part(a, row);
     const S *s = static_cast<const S *>(a.g.logits) + row * a.g.stride;
     if (m == -INFINITY || kind == kRowSearch) {
         if (chunk != 0)
-            return;
+            return false;
         if (m > -INFINITY)
             draw_by_search<S, NT>(a.g, row, s, set, m, sh);
         else if (threadIdx.x == 0)
             no_token(a.g, row, true);
-        return;
+        return true;
     }
     const Chunk<S> part(s, n, chunk, a.chunks, a.chunk_vecs, kind == kRowBound);
     const Weight<T> weight{m, set.inv};
@@ -1081,9 +1083,10 @@ template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_
         const T t = low > lowest<T>() ? low : lowest<T>();
         part.gather(list, [&](T v) { return v >= t; });
         hand_over(a, row, list);
-        if (last_chunk(&a.state[row].done[1], a.chunks))
-            draw_from_row<S>(a, row, set, m, list, bound, red[0], sh);
-        return;
+        if (!last_chunk(&a.state[row].done[1], a.chunks))
+            return false;
+        draw_from_row<S>(a, row, set, m, list, bound, red[0], sh);
+        return true;
     }
     if (kind == kRowPlain) {
         auto mass_of = [&](T v, uint32_t) -> mass_t {
@@ -1096,12 +1099,12 @@ template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_
         if (threadIdx.x == 0)
             put(&a.chunk_mass[blockIdx.x], own);
         if (!last_chunk(&a.state[row].done[1], a.chunks))
-            return;
+            return false;
         if (threadIdx.x < a.chunks)
             in_chunk[threadIdx.x] = get(&a.chunk_mass[row * a.chunks + threadIdx.x]);
         __syncthreads();
         draw_in_chunk<S>(a, row, set, in_chunk, mass_of, sh.tiles);
-        return;
+        return true;
     }
     for (uint32_t b = threadIdx.x; b < kSteps; b += NT)
         sh.steps[b] = 0;
@@ -1115,7 +1118,7 @@ template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_
     for (uint32_t b = threadIdx.x; b < kSteps; b += NT)
         put(&a.steps[(uint64_t)blockIdx.x * kSteps + b], sh.steps[b]);
     if (!last_chunk(&a.state[row].done[1], a.chunks))
-        return;
+        return false;
     // The step in which the nucleus ends, and the chunks' masses before it.
     const mass_t *steps = a.steps + row * a.chunks * kSteps;
     for (uint32_t b = threadIdx.x; b < kSteps; b += NT) {
@@ -1141,16 +1144,17 @@ template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_
         if ((threadIdx.x & 63) == 0)
             a.chunk_mass[row * a.chunks + c] = before;
     }
+    return false;
 }
 
-template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_edge(SplitArgs<typename StatOf<S>::T> a)
+template <typename S> __device__ __forceinline__ bool sample_edge(const SplitArgs<typename StatOf<S>::T> &a)
 {
     using T = typename StatOf<S>::T;
     using K = typename KeyOf<T>::K;
     constexpr int NT = kChunkThreads;
     constexpr uint32_t N = kVec<S>;
     if (block_gate_closed(a.g.gate))
-        return;
+        return blockIdx.x % a.chunks == 0;
     __shared__ BoundScratch bound;
     __shared__ T red[4][16];
     __shared__ List<K, kEdgeListCap> list;
@@ -1160,10 +1164,10 @@ template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_
     const uint32_t chunk = blockIdx.x % a.chunks, n = a.g.vocab;
     const Settings set = settings_of(a.g, row);
     if (kind_of(set, n, a.chunks) != kRowNucleus)
-        return;
+        return chunk == 0;
     const auto [m, low] = row_part(a, row);
     if (m == -INFINITY)
-        return;
+        return chunk == 0;
     const S *s = static_cast<const S *>(a.g.logits) + row * a.g.stride;
     const Chunk<S> part(s, n, chunk, a.chunks, a.chunk_vecs, false);
     const StepOf<T> step_of(m, set.inv, low);
@@ -1185,11 +1189,11 @@ template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_
     __syncthreads();
     hand_over(a, row, list);
     if (!last_chunk(&a.state[row].done[2], a.chunks))
-        return;
+        return false;
     const uint32_t count = take_list(a, row, kRowCap, m, list, bound, red[0]);
     if (count > kRowCap) {
         draw_by_search<S, NT>(a.g, row, s, set, m, sh);
-        return;
+        return true;
     }
     if (threadIdx.x < a.chunks)
         in_chunk[threadIdx.x] = get(&a.chunk_mass[row * a.chunks + threadIdx.x]);
@@ -1218,6 +1222,41 @@ template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_
                          return w >= set.least ? w : 0;
                      },
                      sh.tiles);
+    return true;
+}
+
+// The end of the program by a call's last launch (close): of each row one workgroup, the one that
+// finished it or, of rows finished by earlier launches, its first, takes a ticket; the last of
+// them ends the program. All of the rows' other workgroups have finished before it.
+template <typename T> __device__ __forceinline__ void close_rows(const SplitArgs<T> &a, const ProgramClose &c, bool finisher)
+{
+    if (c.words == nullptr || !finisher)
+        return;
+    __shared__ int last;
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0)
+        last = atomicAdd(c.ticket, 1u) + 1u == a.g.rows;
+    __syncthreads();
+    if (last && threadIdx.x < 64) {
+        __atomic_thread_fence(__ATOMIC_ACQUIRE);
+        if (threadIdx.x == 0)
+            *c.ticket = 0u; // every row has its ticket
+        program_close_wave(c);
+    }
+}
+
+template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_first(SplitArgs<typename StatOf<S>::T> a, ProgramClose close)
+{
+    close_rows(a, close, sample_first<S>(a));
+}
+template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_weigh(SplitArgs<typename StatOf<S>::T> a, ProgramClose close)
+{
+    close_rows(a, close, sample_weigh<S>(a));
+}
+template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_edge(SplitArgs<typename StatOf<S>::T> a, ProgramClose close)
+{
+    close_rows(a, close, sample_edge<S>(a));
 }
 
 // ------------------------------------------------------------------------- launches
@@ -1290,11 +1329,11 @@ SampleArgs rows_from(const SampleArgs &all, uint64_t from, uint64_t most)
     return g;
 }
 
-template <typename S> hipError_t launch_t(hipStream_t s, const SampleArgs &all, void *scratch, void *state)
+template <typename S> hipError_t launch_t(hipStream_t s, const SampleArgs &all, void *scratch, void *state, const ProgramClose &close)
 {
     using T = typename StatOf<S>::T;
     if (short_row(all, kVec<S>)) {
-        hipLaunchKernelGGL((k_sample<S, 256, 4>), dim3((unsigned)all.rows), dim3(256), 0, s, all);
+        hipLaunchKernelGGL((k_sample<S, 256, 4>), dim3((unsigned)all.rows), dim3(256), 0, s, all, close);
         return hipGetLastError();
     }
     for (uint64_t from = 0; from < all.rows; from += kSlabRows) {
@@ -1306,11 +1345,13 @@ template <typename S> hipError_t launch_t(hipStream_t s, const SampleArgs &all, 
         // Every row's list is made and drawn from in the first launch where top_k says so for all.
         const bool lists = !all.top_k && all.top_k_all > 0 && (uint32_t)all.top_k_all < all.vocab &&
                            list_at_once((uint64_t)all.top_k_all, a.chunks);
-        hipLaunchKernelGGL((k_sample_first<S>), parts, block, 0, s, a);
+        const bool edges = !lists && has_nucleus(all);
+        const ProgramClose none;
+        hipLaunchKernelGGL((k_sample_first<S>), parts, block, 0, s, a, lists ? close : none);
         if (!lists)
-            hipLaunchKernelGGL((k_sample_weigh<S>), parts, block, 0, s, a);
-        if (!lists && has_nucleus(all))
-            hipLaunchKernelGGL((k_sample_edge<S>), parts, block, 0, s, a);
+            hipLaunchKernelGGL((k_sample_weigh<S>), parts, block, 0, s, a, edges ? none : close);
+        if (edges)
+            hipLaunchKernelGGL((k_sample_edge<S>), parts, block, 0, s, a, close);
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess)
             return err;
@@ -1334,15 +1375,19 @@ size_t sample_scratch_bytes(const SampleArgs &g)
 
 size_t sample_state_bytes() { return kSlabRows * sizeof(RowState); }
 
-hipError_t launch_sample(hipStream_t s, const SampleArgs &g, void *scratch, void *state)
+hipError_t launch_sample(hipStream_t s, const SampleArgs &g, void *scratch, void *state, ProgramClose close, bool *closed)
 {
+    *closed = false;
     if (g.rows == 0)
         return hipSuccess;
+    if (g.rows > kCloseMaxBlocks)
+        close = ProgramClose{};
+    *closed = close.words != nullptr;
     switch (g.dtype) {
-    case kLogitF32: return launch_t<float>(s, g, scratch, state);
-    case kLogitF64: return launch_t<double>(s, g, scratch, state);
-    case kLogitBf16: return launch_t<__bf16>(s, g, scratch, state);
-    default: return launch_t<_Float16>(s, g, scratch, state);
+    case kLogitF32: return launch_t<float>(s, g, scratch, state, close);
+    case kLogitF64: return launch_t<double>(s, g, scratch, state, close);
+    case kLogitBf16: return launch_t<__bf16>(s, g, scratch, state, close);
+    default: return launch_t<_Float16>(s, g, scratch, state, close);
     }
 }
 

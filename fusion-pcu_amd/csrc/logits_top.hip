@@ -64,13 +64,11 @@ __device__ __forceinline__ void gather_exactly(const S *s, uint32_t n, uint32_t 
 }
 
 // G groups a thread: at least twice as many groups as k keeps the list short.
-template <typename S, int NT, int R, int G, int CAP> __global__ __launch_bounds__(NT) void k_top(TopArgs g)
+template <typename S, int NT, int R, int G, int CAP> __device__ __forceinline__ void top_row(const TopArgs &g)
 {
     using T = typename StatOf<S>::T;
     using K = typename KeyOf<T>::K;
     constexpr uint32_t N = kVec<S>;
-    if (block_gate_closed(g.gate))
-        return;
     __shared__ BoundScratch bound;
     __shared__ Digit<uint32_t> digit;
     __shared__ T red[4][16];
@@ -81,6 +79,8 @@ template <typename S, int NT, int R, int G, int CAP> __global__ __launch_bounds_
     const S *s = static_cast<const S *>(g.logits) + row * g.stride;
     const uint32_t n = g.vocab, k = g.k < n ? g.k : n;
     const Row<S, NT, R> held(s, n);
+    if (block_gate_closed(g.gate)) // after the loads: they need not wait for it
+        return;
 
     T group[G], largest[R ? R : 1]; // of the groups, and of each held vector
 #pragma unroll
@@ -111,7 +111,7 @@ template <typename S, int NT, int R, int G, int CAP> __global__ __launch_bounds_
         });
         sum = block_reduce<NT>(sum, OpSum(), red[1]);
         if (tid == 0)
-            static_cast<T *>(g.log_sum)[row] = ex.log_sum(sum);
+            put(static_cast<T *>(g.log_sum) + row, ex.log_sum(sum));
     }
     if (k > 0) {
         if (tid == 0)
@@ -141,44 +141,56 @@ template <typename S, int NT, int R, int G, int CAP> __global__ __launch_bounds_
     S *values = static_cast<S *>(g.values) + row * g.k;
     int32_t *indices = g.indices + row * g.k;
     for (uint32_t j = tid; j < g.k; j += NT) {
-        values[j] = j < k ? s[list.at[j]] : (S)-INFINITY;
-        indices[j] = j < k ? (int32_t)list.at[j] : -1;
+        put(values + j, j < k ? s[list.at[j]] : (S)-INFINITY);
+        put(indices + j, j < k ? (int32_t)list.at[j] : -1);
     }
 }
 
-template <typename S, int NT, int R> hipError_t launch_row(hipStream_t s, const TopArgs &g)
+// A call of its own ends its program in this kernel (close).
+template <typename S, int NT, int R, int G, int CAP>
+__global__ __launch_bounds__(NT) void k_top(TopArgs g, ProgramClose close)
+{
+    top_row<S, NT, R, G, CAP>(g);
+    program_close_block(close);
+}
+
+template <typename S, int NT, int R> hipError_t launch_row(hipStream_t s, const TopArgs &g, const ProgramClose &close)
 {
     const dim3 grid((unsigned)g.rows), block(NT);
     if (g.k * 4 <= NT)
-        hipLaunchKernelGGL((k_top<S, NT, R, 1, 512>), grid, block, 0, s, g);
+        hipLaunchKernelGGL((k_top<S, NT, R, 1, 512>), grid, block, 0, s, g, close);
     else
-        hipLaunchKernelGGL((k_top<S, NT, R, 4, 2048>), grid, block, 0, s, g);
+        hipLaunchKernelGGL((k_top<S, NT, R, 4, 2048>), grid, block, 0, s, g, close);
     return hipGetLastError();
 }
 
-template <typename S> hipError_t launch_t(hipStream_t s, const TopArgs &g)
+template <typename S> hipError_t launch_t(hipStream_t s, const TopArgs &g, const ProgramClose &close)
 {
     const uint32_t vecs = g.vocab / kVec<S>;
     if (vecs <= 256 * 4)
-        return launch_row<S, 256, 4>(s, g);
+        return launch_row<S, 256, 4>(s, g, close);
     if (vecs <= 256 * 16 && g.k <= 256)
-        return launch_row<S, 256, 16>(s, g);
+        return launch_row<S, 256, 16>(s, g, close);
     if (vecs <= 1024 * 16)
-        return launch_row<S, 1024, 16>(s, g);
-    return launch_row<S, 1024, 0>(s, g);
+        return launch_row<S, 1024, 16>(s, g, close);
+    return launch_row<S, 1024, 0>(s, g, close);
 }
 
 } // namespace
 
-hipError_t launch_top(hipStream_t s, const TopArgs &g)
+hipError_t launch_top(hipStream_t s, const TopArgs &g, ProgramClose close, bool *closed)
 {
+    *closed = false;
     if (g.rows == 0)
         return hipSuccess;
+    if (g.rows > kCloseMaxBlocks)
+        close = ProgramClose{};
+    *closed = close.words != nullptr;
     switch (g.dtype) {
-    case kLogitF32: return launch_t<float>(s, g);
-    case kLogitF64: return launch_t<double>(s, g);
-    case kLogitBf16: return launch_t<__bf16>(s, g);
-    default: return launch_t<_Float16>(s, g);
+    case kLogitF32: return launch_t<float>(s, g, close);
+    case kLogitF64: return launch_t<double>(s, g, close);
+    case kLogitBf16: return launch_t<__bf16>(s, g, close);
+    default: return launch_t<_Float16>(s, g, close);
     }
 }
 

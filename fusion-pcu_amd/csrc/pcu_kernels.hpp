@@ -331,7 +331,9 @@ struct TopArgs {
     void *log_sum = nullptr;     // rows, binary32 (binary64 for binary64 logits), or null
     NodeGate gate{nullptr, 0};
 };
-hipError_t launch_top(hipStream_t s, const TopArgs &g);
+// `close` (when set, and there are few enough rows for one ticket each): the launch also ends the
+// program; *closed tells whether it does (so do the samples' launches).
+hipError_t launch_top(hipStream_t s, const TopArgs &g, ProgramClose close, bool *closed);
 
 // One token a row. A setting's array holds one value a row; where it is null, `_all` holds for
 // every row. A row with an invalid setting or random number records a fault (ordinal: the row).
@@ -356,7 +358,8 @@ struct SampleArgs {
 // gate closes while it runs.
 size_t sample_scratch_bytes(const SampleArgs &g);
 size_t sample_state_bytes();
-hipError_t launch_sample(hipStream_t s, const SampleArgs &g, void *scratch, void *state);
+hipError_t launch_sample(hipStream_t s, const SampleArgs &g, void *scratch, void *state, ProgramClose close,
+                         bool *closed);
 
 // Small device utilities (fill kernels rather than memsets, so a captured graph replays
 // them as kernels).

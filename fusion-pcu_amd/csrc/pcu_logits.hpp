@@ -179,6 +179,18 @@ __device__ __forceinline__ void store_vec(S *row, uint32_t i, uint32_t n, const 
     }
 }
 
+// Stores and loads past the caches that the chip's parts do not share: what a workgroup hands to
+// others of its launch, and results of a launch that ends its program itself (the caller may read
+// them from another stream before the kernel's own end has written the caches back).
+template <typename V> __device__ __forceinline__ void put(V *p, V v)
+{
+    if constexpr (sizeof(V) == 2)
+        __hip_atomic_store(reinterpret_cast<uint16_t *>(p), __builtin_bit_cast(uint16_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    else
+        __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename V> __device__ __forceinline__ V get(const V *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
 // --------------------------------------------------------- reductions of a workgroup
 struct OpMax {
     template <typename T> __device__ __forceinline__ T none() const { return (T)-INFINITY; }
