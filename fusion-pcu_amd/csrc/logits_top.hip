@@ -74,6 +74,7 @@ template <typename S, int NT, int R, int G, int CAP> __device__ __forceinline__ 
     __shared__ T red[4][16];
     __shared__ uint32_t wave_ties[16];
     __shared__ List<K, CAP> list;
+    __shared__ SortShared<T> sort;
     const uint32_t tid = threadIdx.x;
     const uint64_t row = blockIdx.x;
     const S *s = static_cast<const S *>(g.logits) + row * g.stride;
@@ -136,7 +137,7 @@ template <typename S, int NT, int R, int G, int CAP> __device__ __forceinline__ 
             gather_exactly<S, NT>(s, n, k, list, bound.bins, &digit, wave_ties);
             found = k;
         }
-        sort_list<NT>(list, found);
+        sort_list<NT>(list, found, m, sort);
     }
     S *values = static_cast<S *>(g.values) + row * g.k;
     int32_t *indices = g.indices + row * g.k;
@@ -171,7 +172,7 @@ template <typename S> hipError_t launch_t(hipStream_t s, const TopArgs &g, const
         return launch_row<S, 256, 4>(s, g, close);
     if (vecs <= 256 * 16 && g.k <= 256)
         return launch_row<S, 256, 16>(s, g, close);
-    if (vecs <= 1024 * 16)
+    if (sizeof(S) < 8 && vecs <= 1024 * 16) // binary64 would spill
         return launch_row<S, 1024, 16>(s, g, close);
     return launch_row<S, 1024, 0>(s, g, close);
 }
