@@ -181,9 +181,17 @@ pcu_status Ctx::op_distill(Distill mode, const pcu_logits *l, const pcu_distill 
         return st;
     if ((st = open_words()))
         return st;
+    ProgramClose close;
+    if (implicit_program && nodes.size() == 1)
+        close_next = true; // a call of its own: its kernel ends the program
+    if ((st = take_close(&close)))
+        return st;
+    bool closed = false;
     hipEvent_t t = timer_start(stream);
-    st = hip(launch_distill(stream, g, sc), "distill launch");
+    st = hip(launch_distill(stream, g, sc, close, &closed), "distill launch");
     timer_stop(PCU_KERNEL_DISTILL, t, stream);
+    if (!st && closed)
+        closed_seq = ++pub_seq;
     return st;
 }
 

@@ -16,6 +16,8 @@
 #include "pcu_kernels.hpp"
 #include "pcu_logits.hpp"
 
+#include <type_traits>
+
 #pragma clang fp contract(off)
 
 namespace pcu {
@@ -51,17 +53,36 @@ template <typename T> struct Entries {
     }
 };
 
-// Loads and normalises the row's entries. `red`: 2 x 16 places.
+// What load_entries takes from global memory first: this thread's first entry and the label. Loaded
+// ahead of the row's vectors, since loads come back in order.
+template <typename T> struct FirstEntry {
+    int at = -1, label = -1;
+    T v = 0, log_sum = 0;
+    __device__ __forceinline__ FirstEntry(const DistillArgs &g, uint64_t row)
+    {
+        if (threadIdx.x < g.k) {
+            at = g.teacher_indices[row * g.k + threadIdx.x];
+            v = widen_teacher<T>(g.teacher_values, g.teacher_dtype, row * g.k + threadIdx.x);
+        }
+        if (g.labels)
+            label = g.labels[row];
+        if (g.teacher_log_sum)
+            log_sum = g.teacher_log_sum_f64 ? (T) static_cast<const double *>(g.teacher_log_sum)[row]
+                                            : (T) static_cast<const float *>(g.teacher_log_sum)[row];
+    }
+};
+
+// Normalises the row's entries. `red`: 2 x 16 places.
 template <int NT, typename T>
-__device__ __forceinline__ void load_entries(const DistillArgs &g, uint64_t row, Entries<T> &e, T *red)
+__device__ __forceinline__ void load_entries(const DistillArgs &g, uint64_t row, const FirstEntry<T> &ahead, Entries<T> &e, T *red)
 {
-    const int tid = threadIdx.x;
+    const uint32_t tid = threadIdx.x;
     uint64_t bad = kNoFault;
     const T t = (T)g.temperature;
     T top = -INFINITY;
     for (uint32_t j = tid; j < g.k; j += NT) {
-        int at = g.teacher_indices[row * g.k + j];
-        T z = widen_teacher<T>(g.teacher_values, g.teacher_dtype, row * g.k + j) / t;
+        int at = j == tid ? ahead.at : g.teacher_indices[row * g.k + j];
+        T z = (j == tid ? ahead.v : widen_teacher<T>(g.teacher_values, g.teacher_dtype, row * g.k + j)) / t;
         if (at >= (int64_t)g.vocab) {
             bad = pack_fault(row * (g.k + 1) + j, kInvalid) < bad ? pack_fault(row * (g.k + 1) + j, kInvalid) : bad;
             at = -1;
@@ -74,7 +95,7 @@ __device__ __forceinline__ void load_entries(const DistillArgs &g, uint64_t row,
         e.log_q[j] = z;
         top = OpMax()(top, z);
     }
-    int y = g.labels ? g.labels[row] : -1;
+    int y = ahead.label;
     if (y >= (int64_t)g.vocab) {
         if (tid == 0) {
             const uint64_t f = pack_fault(row * (g.k + 1) + g.k, kInvalid);
@@ -86,8 +107,7 @@ __device__ __forceinline__ void load_entries(const DistillArgs &g, uint64_t row,
     wave_record_fault(bad, g.fault, g.gate);
     T log_sum;
     if (g.teacher_log_sum) {
-        log_sum = g.teacher_log_sum_f64 ? (T) static_cast<const double *>(g.teacher_log_sum)[row]
-                                        : (T) static_cast<const float *>(g.teacher_log_sum)[row];
+        log_sum = ahead.log_sum;
     } else {
         top = block_reduce<NT>(top, OpMax(), red);
         T sum = 0;
@@ -183,7 +203,7 @@ __device__ __forceinline__ void fix_entries(const DistillArgs &g, S *grad, const
             value -= less * per_q;
         if (at == e.label)
             value -= per_label;
-        grad[at] = (S)value;
+        put(grad + at, (S)value);
     }
 }
 
@@ -192,13 +212,13 @@ __device__ __forceinline__ void fix_entries(const DistillArgs &g, S *grad, const
 // Forward, or forward and backward, for rows of at most NT * R whole vectors (the values after
 // the last whole one lie one a lane in the first wave): each thread keeps R vectors of the row,
 // so that the row is read once and its gradient written once.
-template <typename S, int NT, int R, bool GRAD>
-__global__ __launch_bounds__(NT) void k_distill_row(DistillArgs g)
+// Rows up to here end the program of a call of their own in its kernel.
+constexpr uint32_t kCloseVecs = 1024;
+
+template <typename S, int NT, int R, bool GRAD> __device__ __forceinline__ void distill_row(const DistillArgs &g)
 {
     using T = typename StatOf<S>::T;
     constexpr int N = kVec<S>;
-    if (block_gate_closed(g.gate))
-        return;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ T red[7][16];
     const uint32_t tid = threadIdx.x;
@@ -207,66 +227,74 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs g)
     const uint32_t whole = g.vocab / N, rest = whole * N + tid;
     const bool has_rest = rest < g.vocab; // at most N - 1 lanes
 
+    const FirstEntry<T> ahead(g, row);
     u32x4 raw[R];
 #pragma unroll
     for (int r = 0; r < R; r++)
         raw[r] = tid + r * NT < whole ? load_held(s, r * NT, tid) : minus_infinities<S>();
     const T extra = has_rest ? (T)s[rest] : (T)-INFINITY;
 
+    if (block_gate_closed(g.gate)) // after the loads: they need not wait for it
+        return;
+
     Entries<T> e(lds, g.k);
-    load_entries<NT>(g, row, e, red[0]);
+    load_entries<NT>(g, row, ahead, e, red[0]);
 
-    T m = extra;
-#pragma unroll
-    for (int r = 0; r < R; r++) {
-        T v[N];
-        unpack<S>(raw[r], v);
-#pragma unroll
-        for (int i = 0; i < N; i++)
-            m = OpMax()(m, v[i]);
-        one_at_a_time();
-    }
-    m = block_reduce<NT>(m, OpMax(), red[2]);
-
+    // Each thread's maximum and sums over the vectors as they arrive, two at a time, the sums
+    // rescaled when the maximum rises.
     const T inv_t = (T)1 / (T)g.temperature;
     const bool two = g.temperature != 1.0 && (g.log_sums_out != nullptr || e.label >= 0);
-    const Expo<T> ex(m, inv_t), ex1(m, (T)1);
-    T sum = ex(extra), sum1 = two ? ex1(extra) : (T)0;
-    Pass pass = Pass::fresh();
+    T m = extra, sum = Expo<T>(m, inv_t)(extra), sum1 = two ? Expo<T>(m, (T)1)(extra) : (T)0;
+    auto add_up = [&](auto both) {
+        const Pass pass = Pass::fresh();
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-        T v[N];
-        unpack<S>(raw[r], v, pass);
-#pragma unroll
-        for (int i = 0; i < N; i++)
-            sum += ex(v[i]);
-        one_at_a_time();
-    }
-    if (two) {
-        pass = Pass::fresh();
-        const Expo<T> f1 = ex1.fresh();
-#pragma unroll
-        for (int r = 0; r < R; r++) {
-            T v[N];
+        for (int r = 0; r < R; r += 2) {
+            T v[2 * N];
             unpack<S>(raw[r], v, pass);
+            unpack<S>(raw[r + 1], v + N, pass);
+            T top = m;
 #pragma unroll
-            for (int i = 0; i < N; i++)
-                sum1 += f1(v[i]);
+            for (int i = 0; i < 2 * N; i++)
+                top = OpMax()(top, v[i]);
+            const Expo<T> ex(top, inv_t), ex1(top, (T)1);
+            sum *= m == -INFINITY ? (T)1 : ex(m); // 0, or NaN, while there is no maximum
+            if (both)
+                sum1 *= m == -INFINITY ? (T)1 : ex1(m);
+#pragma unroll
+            for (int i = 0; i < 2 * N; i++) {
+                sum += ex(v[i]);
+                if (both)
+                    sum1 += ex1(v[i]);
+            }
+            m = top;
             one_at_a_time();
         }
-    }
+    };
+    if (two)
+        add_up(std::true_type());
+    else
+        add_up(std::false_type());
+    const T own = m;
+    m = block_reduce<NT>(m, OpMax(), red[2]);
+    const Expo<T> ex(m, inv_t), ex1(m, (T)1);
+    sum *= own == -INFINITY ? (T)1 : ex(own); // without a maximum the sum is 0, or NaN
     sum = block_reduce<NT>(sum, OpSum(), red[3]);
-    sum1 = two ? block_reduce<NT>(sum1, OpSum(), red[4]) : sum;
+    if (two) {
+        sum1 *= own == -INFINITY ? (T)1 : ex1(own);
+        sum1 = block_reduce<NT>(sum1, OpSum(), red[4]);
+    } else {
+        sum1 = sum;
+    }
     const T lse = ex.log_sum(sum), lse1 = two ? ex1.log_sum(sum1) : lse;
     if (tid == 0 && g.log_sums_out) {
-        static_cast<T *>(g.log_sums_out)[2 * row] = lse;
-        static_cast<T *>(g.log_sums_out)[2 * row + 1] = lse1;
+        put(static_cast<T *>(g.log_sums_out) + 2 * row, lse);
+        put(static_cast<T *>(g.log_sums_out) + 2 * row + 1, lse1);
     }
     gather_entries<NT>(g, s, e, 0u, g.vocab);
     if (g.loss) {
         const T loss = row_loss<NT>(g, e, lse, lse1, red[5]);
         if (tid == 0)
-            static_cast<T *>(g.loss)[row] = loss;
+            put(static_cast<T *>(g.loss) + row, loss);
     }
     if constexpr (GRAD) {
         const T scale = g.row_scale ? static_cast<const T *>(g.row_scale)[row] : (T)1;
@@ -280,6 +308,7 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs g)
         const T pq = cq == 0 || sum == 0 ? (T)0 : cq / sum, pl = cl == 0 || sum1 == 0 ? (T)0 : cl / sum1;
         S *grad = static_cast<S *>(g.grad) + row * g.grad_stride;
         __syncthreads(); // the entries' logits are read: the gradient may lie in the row's place
+        const Pass pass = Pass::fresh();
         // The dense part; `value` gives it for one logit.
         auto write = [&](auto value) {
 #pragma unroll
@@ -290,17 +319,16 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs g)
                 for (int i = 0; i < N; i++)
                     v[i] = value(v[i]);
                 if (tid + r * NT < whole)
-                    store_held(grad, r * NT, tid, pack<S>(v));
+                    store_held<NT * R <= kCloseVecs>(grad, r * NT, tid, pack<S>(v), g.store);
                 one_at_a_time();
             }
             if (has_rest)
-                grad[rest] = (S)value(extra);
+                put(grad + rest, (S)value(extra));
             __syncthreads();
             fix_entries<NT>(g, grad, e, 0u, g.vocab, scale, value);
         };
         for (uint32_t i = g.vocab + tid; i < g.grad_cols; i += NT)
-            grad[i] = (S)0;
-        pass = Pass::fresh();
+            put(grad + i, (S)0);
         const Expo<T> fq = ex.fresh(), fl = ex1.fresh(), one = pq != 0 ? fq : fl;
         const T p1 = pq != 0 ? pq : pl;
         if (p1 == 0) // nothing asks for the row (or it has no probabilities)
@@ -312,17 +340,26 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs g)
     }
 }
 
+// A call of its own ends its program in this kernel (close).
+template <typename S, int NT, int R, bool GRAD>
+__global__ __launch_bounds__(NT) void k_distill_row(DistillArgs g, ProgramClose close)
+{
+    distill_row<S, NT, R, GRAD>(g);
+    program_close_block(close);
+}
+
 // ----------------------------------------------------------- a row split over workgroups
 //
 // Rows that no workgroup holds, and few rows of a long vocabulary: the statistics of chunks of
-// a row, then per row the two log-sum-exps and the loss, then the gradient by chunks.
+// a row, with the logits at the entries; then per chunk the row's two log-sum-exps from all its
+// chunks and the gradient, the loss with the first (or, for the loss alone, one workgroup a row).
 template <typename T> struct Partial {
     T m, sum, sum1;
 };
 
 template <typename S, int NT>
 __global__ __launch_bounds__(NT) void k_distill_stats(DistillArgs g, uint32_t chunks, uint32_t chunk_vecs,
-                                                      Partial<typename StatOf<S>::T> *parts)
+                                                      Partial<typename StatOf<S>::T> *parts, typename StatOf<S>::T *picked)
 {
     using T = typename StatOf<S>::T;
     constexpr int N = kVec<S>;
@@ -337,6 +374,14 @@ __global__ __launch_bounds__(NT) void k_distill_stats(DistillArgs g, uint32_t ch
     const T inv_t = (T)1 / (T)g.temperature;
     const bool two = g.temperature != 1.0;
 
+    if (picked) { // what the loss needs, before a gradient in place overwrites it
+        const uint32_t c0 = first * N, c1 = last * N < g.vocab ? last * N : g.vocab;
+        for (uint32_t j = threadIdx.x; j <= g.k; j += NT) {
+            const int at = j < g.k ? g.teacher_indices[row * g.k + j] : (g.labels ? g.labels[row] : -1);
+            if (at >= (int)c0 && at < (int)c1)
+                picked[row * (g.k + 1) + j] = (T)s[at];
+        }
+    }
     // Each thread's running maximum and sums, rescaled when a piece raises the maximum.
     T m = -INFINITY, sum = 0, sum1 = 0;
     for (uint32_t i = first + threadIdx.x; i < last; i += NT * U) {
@@ -377,24 +422,17 @@ __global__ __launch_bounds__(NT) void k_distill_stats(DistillArgs g, uint32_t ch
         parts[blockIdx.x] = Partial<T>{top, sum, two ? sum1 : sum};
 }
 
-constexpr int kFinishThreads = 256;
-
-template <typename S>
-__global__ __launch_bounds__(kFinishThreads) void k_distill_finish(DistillArgs g, uint32_t chunks,
-                                                                   const Partial<typename StatOf<S>::T> *parts)
+// The row's two log-sum-exps from its chunks'. `red`: 3 x 16 places.
+template <typename T> struct LogSums {
+    T lse, lse1;
+};
+template <int NT, typename T>
+__device__ __forceinline__ LogSums<T> log_sums_of(const DistillArgs &g, uint64_t row, uint32_t chunks, const Partial<T> *parts, T *red)
 {
-    using T = typename StatOf<S>::T;
-    constexpr int NT = kFinishThreads;
-    if (block_gate_closed(g.gate))
-        return;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-    __shared__ T red[7][16];
-    const uint64_t row = blockIdx.x;
-    const S *s = static_cast<const S *>(g.logits) + row * g.stride;
     T m = -INFINITY;
     for (uint32_t c = threadIdx.x; c < chunks; c += NT)
         m = OpMax()(m, parts[row * chunks + c].m);
-    m = block_reduce<NT>(m, OpMax(), red[0]);
+    m = block_reduce<NT>(m, OpMax(), red);
     const Expo<T> ex(m, (T)1 / (T)g.temperature), ex1(m, (T)1);
     T sum = 0, sum1 = 0;
     for (uint32_t c = threadIdx.x; c < chunks; c += NT) {
@@ -403,34 +441,51 @@ __global__ __launch_bounds__(kFinishThreads) void k_distill_finish(DistillArgs g
         sum += p.m == -INFINITY ? p.sum : p.sum * ex(p.m);
         sum1 += p.m == -INFINITY ? p.sum1 : p.sum1 * ex1(p.m);
     }
-    sum = block_reduce<NT>(sum, OpSum(), red[1]);
-    sum1 = block_reduce<NT>(sum1, OpSum(), red[2]);
-    const T lse = ex.log_sum(sum), lse1 = g.temperature != 1.0 ? ex1.log_sum(sum1) : lse;
-    if (threadIdx.x == 0) {
-        static_cast<T *>(g.log_sums_out)[2 * row] = lse;
-        static_cast<T *>(g.log_sums_out)[2 * row + 1] = lse1;
-    }
-    if (g.loss) {
-        Entries<T> e(lds, g.k);
-        load_entries<NT>(g, row, e, red[3]);
-        gather_entries<NT>(g, s, e, 0u, g.vocab);
-        const T loss = row_loss<NT>(g, e, lse, lse1, red[5]);
-        if (threadIdx.x == 0)
-            static_cast<T *>(g.loss)[row] = loss;
-    }
+    sum = block_reduce<NT>(sum, OpSum(), red + 16);
+    sum1 = block_reduce<NT>(sum1, OpSum(), red + 32);
+    const T lse = ex.log_sum(sum);
+    return {lse, g.temperature != 1.0 ? ex1.log_sum(sum1) : lse};
 }
 
-// The gradient of one chunk of a row from the row's log-sum-exps.
+constexpr int kFinishThreads = 256;
+
+template <typename S>
+__global__ __launch_bounds__(kFinishThreads) void k_distill_finish(DistillArgs g, uint32_t chunks,
+                                                                   const Partial<typename StatOf<S>::T> *parts)
+{
+    using T = typename StatOf<S>::T;
+    constexpr int NT = kFinishThreads;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ T red[7][16];
+    const uint64_t row = blockIdx.x;
+    const FirstEntry<T> ahead(g, row);
+    if (block_gate_closed(g.gate))
+        return;
+    const LogSums<T> sums = log_sums_of<NT>(g, row, chunks, parts, red[0]);
+    if (threadIdx.x == 0 && g.log_sums_out) {
+        static_cast<T *>(g.log_sums_out)[2 * row] = sums.lse;
+        static_cast<T *>(g.log_sums_out)[2 * row + 1] = sums.lse1;
+    }
+    Entries<T> e(lds, g.k);
+    load_entries<NT>(g, row, ahead, e, red[3]);
+    gather_entries<NT>(g, static_cast<const S *>(g.logits) + row * g.stride, e, 0u, g.vocab);
+    const T loss = row_loss<NT>(g, e, sums.lse, sums.lse1, red[5]);
+    if (threadIdx.x == 0)
+        static_cast<T *>(g.loss)[row] = loss;
+}
+
+// The gradient of one chunk of a row, from the row's given log-sum-exps or (parts) from its chunks',
+// and then the loss with the first chunk.
 template <typename S, int NT>
-__global__ __launch_bounds__(NT) void k_distill_grad(DistillArgs g, uint32_t chunks, uint32_t chunk_vecs)
+__global__ __launch_bounds__(NT) void k_distill_grad(DistillArgs g, uint32_t chunks, uint32_t chunk_vecs,
+                                                     const Partial<typename StatOf<S>::T> *parts,
+                                                     const typename StatOf<S>::T *picked)
 {
     using T = typename StatOf<S>::T;
     constexpr int N = kVec<S>;
     constexpr int U = 4;
-    if (block_gate_closed(g.gate))
-        return;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    __shared__ T red[2][16];
+    __shared__ T red[7][16];
     const uint64_t row = blockIdx.x / chunks;
     const uint32_t chunk = blockIdx.x % chunks;
     const S *s = static_cast<const S *>(g.logits) + row * g.stride;
@@ -438,10 +493,34 @@ __global__ __launch_bounds__(NT) void k_distill_grad(DistillArgs g, uint32_t chu
     const uint32_t first = chunk * chunk_vecs, last = first + chunk_vecs;
     const uint32_t c0 = first * N, c1 = last * N < g.vocab ? last * N : g.vocab;
 
+    const FirstEntry<T> ahead(g, row);
+    u32x4 raw[U]; // the first vectors come while the entries are made ready
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const uint32_t i = first + threadIdx.x + u * NT;
+        raw[u] = i < last ? load_vec(s, i, g.vocab) : minus_infinities<S>();
+    }
+    if (block_gate_closed(g.gate))
+        return;
     Entries<T> e(lds, g.k);
-    load_entries<NT>(g, row, e, red[0]);
+    load_entries<NT>(g, row, ahead, e, red[0]);
+    T lse, lse1;
+    if (parts) {
+        const LogSums<T> sums = log_sums_of<NT>(g, row, chunks, parts, red[2]);
+        lse = sums.lse;
+        lse1 = sums.lse1;
+        if (chunk == 0) {
+            for (uint32_t j = threadIdx.x; j <= g.k; j += NT)
+                e.s[j] = e.at[j] >= 0 ? picked[row * (g.k + 1) + j] : (T)0;
+            const T loss = row_loss<NT>(g, e, lse, lse1, red[5]);
+            if (threadIdx.x == 0)
+                static_cast<T *>(g.loss)[row] = loss;
+        }
+    } else {
+        lse = static_cast<const T *>(g.log_sums_in)[2 * row];
+        lse1 = static_cast<const T *>(g.log_sums_in)[2 * row + 1];
+    }
     gather_entries<NT>(g, s, e, c0, c1);
-    const T lse = static_cast<const T *>(g.log_sums_in)[2 * row], lse1 = static_cast<const T *>(g.log_sums_in)[2 * row + 1];
     const T scale = g.row_scale ? static_cast<const T *>(g.row_scale)[row] : (T)1;
     T pq = scale * (T)g.distill_weight * (T)g.temperature * e.sum;
     T pl = e.label >= 0 ? scale * (T)g.label_weight : (T)0;
@@ -462,19 +541,22 @@ __global__ __launch_bounds__(NT) void k_distill_grad(DistillArgs g, uint32_t chu
     };
     __syncthreads(); // the entries' logits are read: the gradient may lie in the row's place
     for (uint32_t i = first + threadIdx.x; i < last; i += NT * U) {
-        u32x4 raw[U];
+        u32x4 now[U];
 #pragma unroll
-        for (int u = 0; u < U; u++)
-            raw[u] = i + u * NT < last ? load_vec(s, i + u * NT, g.vocab) : minus_infinities<S>();
+        for (int u = 0; u < U; u++) {
+            now[u] = raw[u];
+            const uint32_t next = i + (U + u) * NT;
+            raw[u] = next < last ? load_vec(s, next, g.vocab) : minus_infinities<S>();
+        }
 #pragma unroll
         for (int u = 0; u < U; u++) {
             T v[N];
-            unpack<S>(raw[u], v);
+            unpack<S>(now[u], v);
 #pragma unroll
             for (int k = 0; k < N; k++)
                 v[k] = dense(v[k]);
             if (i + u * NT < last)
-                store_vec(grad, i + u * NT, g.vocab, v);
+                store_vec(grad, i + u * NT, g.vocab, v, g.store == kStorePast);
         }
     }
     if (chunk == chunks - 1)
@@ -485,6 +567,12 @@ __global__ __launch_bounds__(NT) void k_distill_grad(DistillArgs g, uint32_t chu
 }
 
 // ------------------------------------------------------------------------- launches
+
+// A large gradient is stored past the caches: with the logits, and the output layer that both come from
+// and go to, it would not stay in the chip's 256 MiB, and the logits' own reads come faster
+// (4096 x 128000 bf16 533 -> 492 us a call, 1025 x 50257 f16, 103 MB, 69 -> 59 us). A smaller one
+// is left where its reader finds it.
+constexpr uint64_t kPastCaches = 64ull << 20;
 
 struct Split {
     uint32_t chunks, vecs;
@@ -501,21 +589,23 @@ Split split_of(uint64_t rows, uint32_t vecs)
     return Split{(vecs + each - 1) / each, each};
 }
 
-template <typename S, int NT, int R> hipError_t launch_row(hipStream_t s, const DistillArgs &g)
+template <typename S, int NT, int R> hipError_t launch_row(hipStream_t s, const DistillArgs &g, const ProgramClose &close)
 {
     const size_t lds = Entries<typename StatOf<S>::T>::bytes(g.k);
     if (g.grad)
-        hipLaunchKernelGGL((k_distill_row<S, NT, R, true>), dim3((unsigned)g.rows), dim3(NT), lds, s, g);
+        hipLaunchKernelGGL((k_distill_row<S, NT, R, true>), dim3((unsigned)g.rows), dim3(NT), lds, s, g, close);
     else
-        hipLaunchKernelGGL((k_distill_row<S, NT, R, false>), dim3((unsigned)g.rows), dim3(NT), lds, s, g);
+        hipLaunchKernelGGL((k_distill_row<S, NT, R, false>), dim3((unsigned)g.rows), dim3(NT), lds, s, g, close);
     return hipGetLastError();
 }
 
-template <typename S> hipError_t launch_grad(hipStream_t s, const DistillArgs &g, Split sp)
+template <typename S>
+hipError_t launch_grad(hipStream_t s, const DistillArgs &g, Split sp, const Partial<typename StatOf<S>::T> *parts,
+                       const typename StatOf<S>::T *picked)
 {
     const size_t lds = Entries<typename StatOf<S>::T>::bytes(g.k);
     hipLaunchKernelGGL((k_distill_grad<S, kSplitThreads>), dim3((unsigned)(g.rows * sp.chunks)), dim3(kSplitThreads),
-                       lds, s, g, sp.chunks, sp.vecs);
+                       lds, s, g, sp.chunks, sp.vecs, parts, picked);
     return hipGetLastError();
 }
 
@@ -527,39 +617,37 @@ template <typename S> bool held(uint64_t rows, uint32_t vecs)
     return vecs <= kHeldVecs<S> && (rows >= 64 || vecs <= 1024);
 }
 
-template <typename S> hipError_t launch_t(hipStream_t s, DistillArgs g, void *scratch)
+template <typename S> hipError_t launch_t(hipStream_t s, const DistillArgs &g, void *scratch, const ProgramClose &close)
 {
     using T = typename StatOf<S>::T;
     const uint32_t vecs = (g.vocab + kVec<S> - 1) / kVec<S>;
     if (g.log_sums_in)
-        return launch_grad<S>(s, g, split_of(g.rows, vecs));
+        return launch_grad<S>(s, g, split_of(g.rows, vecs), nullptr, nullptr);
     if (held<S>(g.rows, vecs)) {
         if (vecs <= 64 * 4)
-            return launch_row<S, 64, 4>(s, g);
+            return launch_row<S, 64, 4>(s, g, close);
         if (vecs <= 256 * 4)
-            return launch_row<S, 256, 4>(s, g);
+            return launch_row<S, 256, 4>(s, g, close);
         if (vecs <= 256 * 16)
-            return launch_row<S, 256, 16>(s, g);
+            return launch_row<S, 256, 16>(s, g, close);
         if (vecs <= 512 * 16)
-            return launch_row<S, 512, 16>(s, g);
+            return launch_row<S, 512, 16>(s, g, close);
         if constexpr (sizeof(S) < 8)
-            return launch_row<S, 1024, 16>(s, g);
+            return launch_row<S, 1024, 16>(s, g, close);
     }
     const Split sp = split_of(g.rows, vecs);
     Partial<T> *parts = static_cast<Partial<T> *>(scratch);
-    if (!g.log_sums_out)
-        g.log_sums_out = parts + g.rows * sp.chunks;
+    T *picked = reinterpret_cast<T *>(parts + g.rows * sp.chunks);
     hipLaunchKernelGGL((k_distill_stats<S, kSplitThreads>), dim3((unsigned)(g.rows * sp.chunks)), dim3(kSplitThreads), 0,
-                       s, g, sp.chunks, sp.vecs, parts);
-    hipError_t err = hipGetLastError();
+                       s, g, sp.chunks, sp.vecs, parts, g.grad ? picked : nullptr);
+    const hipError_t err = hipGetLastError();
     if (err != hipSuccess)
         return err;
+    if (g.grad)
+        return launch_grad<S>(s, g, sp, parts, picked);
     hipLaunchKernelGGL((k_distill_finish<S>), dim3((unsigned)g.rows), dim3(kFinishThreads), Entries<T>::bytes(g.k), s, g,
                        sp.chunks, parts);
-    if ((err = hipGetLastError()) != hipSuccess || !g.grad)
-        return err;
-    g.log_sums_in = g.log_sums_out;
-    return launch_grad<S>(s, g, sp);
+    return hipGetLastError();
 }
 
 template <typename S> size_t scratch_t(const DistillArgs &g)
@@ -568,7 +656,7 @@ template <typename S> size_t scratch_t(const DistillArgs &g)
     const uint32_t vecs = (g.vocab + kVec<S> - 1) / kVec<S>;
     if (g.rows == 0 || g.log_sums_in || held<S>(g.rows, vecs))
         return 0;
-    return g.rows * (split_of(g.rows, vecs).chunks * sizeof(Partial<T>) + 2 * sizeof(T));
+    return g.rows * (split_of(g.rows, vecs).chunks * sizeof(Partial<T>) + (g.grad ? g.k + 1 : 0) * sizeof(T));
 }
 
 } // namespace
@@ -583,15 +671,24 @@ size_t distill_scratch_bytes(const DistillArgs &g)
     }
 }
 
-hipError_t launch_distill(hipStream_t s, const DistillArgs &g, void *scratch)
+hipError_t launch_distill(hipStream_t s, DistillArgs g, void *scratch, ProgramClose close, bool *closed)
 {
+    *closed = false;
     if (g.rows == 0)
         return hipSuccess;
+    const uint64_t size = g.dtype == kLogitF64 ? 8 : g.dtype == kLogitF32 ? 4 : 2;
+    if (g.log_sums_in || g.rows > kCloseMaxBlocks || g.vocab > kCloseVecs * 16 / size)
+        close = ProgramClose{};
+    *closed = close.words != nullptr;
+    if (*closed)
+        g.store = kStoreThrough;
+    else if (g.grad && g.rows * g.grad_cols * size > kPastCaches)
+        g.store = kStorePast;
     switch (g.dtype) {
-    case kLogitF32: return launch_t<float>(s, g, scratch);
-    case kLogitF64: return launch_t<double>(s, g, scratch);
-    case kLogitBf16: return launch_t<__bf16>(s, g, scratch);
-    default: return launch_t<_Float16>(s, g, scratch);
+    case kLogitF32: return launch_t<float>(s, g, scratch, close);
+    case kLogitF64: return launch_t<double>(s, g, scratch, close);
+    case kLogitBf16: return launch_t<__bf16>(s, g, scratch, close);
+    default: return launch_t<_Float16>(s, g, scratch, close);
     }
 }
 

@@ -290,6 +290,8 @@ hipError_t launch_native_mse(hipStream_t s, int dtype, uint64_t n, const void *p
 enum : int { kLogitF32 = 0, kLogitF64 = 1, kLogitBf16 = 2, kLogitF16 = 3 };
 constexpr uint32_t kLogitMaxVocab = 1u << 22; // weights of 2^40 each add up below 2^62
 constexpr uint32_t kLogitMaxK = 1024;
+// How a gradient is stored: plainly; past the caches; through them, in a kernel that ends its program.
+enum : int { kStorePlain = 0, kStorePast = 1, kStoreThrough = 2 };
 
 // Distillation from a teacher's top logits. Statistics (loss, log_sums, row_scale) are binary32,
 // binary64 for binary64 logits; the teacher's log-sum-exps binary64 where _f64 says so.
@@ -312,11 +314,12 @@ struct DistillArgs {
     void *grad = nullptr;               // rows x grad_cols (zeros past the vocabulary), or null
     uint64_t grad_stride = 0;
     uint32_t grad_cols = 0;
+    int store = kStorePlain;            // set by the launch: how the gradient is stored
     unsigned long long *fault = nullptr; // ordinal row * (k + 1) + entry (k: the label)
     NodeGate gate{nullptr, 0};
 };
 size_t distill_scratch_bytes(const DistillArgs &g);
-hipError_t launch_distill(hipStream_t s, const DistillArgs &g, void *scratch);
+hipError_t launch_distill(hipStream_t s, DistillArgs g, void *scratch, ProgramClose close, bool *closed);
 
 // The k largest logits of each row (value descending, index ascending) and, unless null, the
 // row's log-sum-exp of l / temperature. Places past the vocabulary: minus infinity and -1.

@@ -112,10 +112,6 @@ template <typename S> __device__ __forceinline__ u32x4 load_whole(const S *row, 
 {
     return *reinterpret_cast<const u32x4_any *>(reinterpret_cast<const char *>(row) + i * 16u);
 }
-template <typename S> __device__ __forceinline__ void store_whole(S *row, uint32_t i, const u32x4 &raw)
-{
-    *reinterpret_cast<u32x4_any *>(reinterpret_cast<char *>(row) + i * 16u) = raw;
-}
 
 // The same where a thread holds many vectors of the row: vector `step` + i, `step` the same for
 // the workgroup. The address of the step is kept scalar and unknown to the compiler, which
@@ -127,12 +123,49 @@ template <typename S> __device__ __forceinline__ u32x4 load_held(const S *row, u
     asm volatile("" : "+s"(base));
     return *(const __attribute__((address_space(1))) u32x4_any *)(base + i * 16u);
 }
-template <typename S> __device__ __forceinline__ void store_held(S *row, uint32_t step, uint32_t i, const u32x4 &raw)
+// Stores and loads past the caches that the chip's parts do not share: what a workgroup hands to
+// others of its launch, and results of a launch that ends its program itself (the caller may read
+// them from another stream before the kernel's own end has written the caches back).
+template <typename V> __device__ __forceinline__ void put(V *p, V v)
+{
+    if constexpr (sizeof(V) == 2)
+        __hip_atomic_store(reinterpret_cast<uint16_t *>(p), __builtin_bit_cast(uint16_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    else
+        __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename V> __device__ __forceinline__ V get(const V *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+// A vector, as words, or as values where 2-byte values are not aligned to words.
+template <typename S> __device__ __forceinline__ void put_vec(S *p, const u32x4 &raw)
+{
+    if (sizeof(S) == 2 && (reinterpret_cast<uintptr_t>(p) & 2)) {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            put(reinterpret_cast<uint16_t *>(p) + e, (uint16_t)(raw[e / 2] >> (e & 1 ? 16 : 0)));
+    } else {
+#pragma unroll
+        for (int w = 0; w < 4; w++)
+            put(reinterpret_cast<uint32_t *>(p) + w, raw[w]);
+    }
+}
+
+__device__ __forceinline__ void apart() { asm volatile(""); }
+// THROUGH: the kernel may be one that ends its program.
+template <bool THROUGH, typename S>
+__device__ __forceinline__ void store_held(S *row, uint32_t step, uint32_t i, const u32x4 &raw, int how)
 {
     typedef __attribute__((address_space(1))) char *P;
+    typedef __attribute__((address_space(1))) u32x4_any *V;
     P base = (P) reinterpret_cast<char *>(row) + step * 16u;
     asm volatile("" : "+s"(base));
-    *(__attribute__((address_space(1))) u32x4_any *)(base + i * 16u) = raw;
+    if (how == kStorePast) {
+        apart(); // or the two stores would become one, and an ordinary one
+        __builtin_nontemporal_store(raw, (V)(base + i * 16u));
+        apart();
+    } else if (THROUGH && how == kStoreThrough) {
+        put_vec(row + (step + i) * kVec<S>, raw);
+    } else {
+        *(V)(base + i * 16u) = raw;
+    }
 }
 
 // Vector i of a row of n values; places past the row's end read as minus infinity, whole
@@ -166,11 +199,16 @@ template <typename S> __device__ __forceinline__ u32x4 load_vec(const S *row, ui
 }
 
 template <typename S>
-__device__ __forceinline__ void store_vec(S *row, uint32_t i, uint32_t n, const typename StatOf<S>::T *v)
+__device__ __forceinline__ void store_vec(S *row, uint32_t i, uint32_t n, const typename StatOf<S>::T *v, bool past)
 {
     const uint32_t at = i * kVec<S>;
     if (at + kVec<S> <= n) {
-        store_whole(row, i, pack<S>(v));
+        if (past) {
+            apart();
+            __builtin_nontemporal_store(pack<S>(v), reinterpret_cast<u32x4_any *>(reinterpret_cast<char *>(row) + i * 16u));
+            apart();
+        } else
+            *reinterpret_cast<u32x4_any *>(reinterpret_cast<char *>(row) + i * 16u) = pack<S>(v);
     } else {
 #pragma unroll
         for (int e = 0; e < kVec<S>; e++)
@@ -178,18 +216,6 @@ __device__ __forceinline__ void store_vec(S *row, uint32_t i, uint32_t n, const 
                 row[at + e] = (S)v[e];
     }
 }
-
-// Stores and loads past the caches that the chip's parts do not share: what a workgroup hands to
-// others of its launch, and results of a launch that ends its program itself (the caller may read
-// them from another stream before the kernel's own end has written the caches back).
-template <typename V> __device__ __forceinline__ void put(V *p, V v)
-{
-    if constexpr (sizeof(V) == 2)
-        __hip_atomic_store(reinterpret_cast<uint16_t *>(p), __builtin_bit_cast(uint16_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    else
-        __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-template <typename V> __device__ __forceinline__ V get(const V *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 // --------------------------------------------------------- reductions of a workgroup
 struct OpMax {
