@@ -25,6 +25,10 @@ namespace {
 typedef unsigned long long mass_t;
 constexpr mass_t kOne = 1ull << 40;
 
+// A sum complete here: the compiler may not put off its additions and hold the masses instead (the
+// kernels on long rows took 94 registers for that, 5 workgroups a CU for 7).
+__device__ __forceinline__ void added(mass_t &sum) { asm volatile("" : "+v"(sum)); }
+
 // floor(mass * part / 2^31), mass < 2^62, part <= 2^31.
 __device__ __forceinline__ mass_t share_of(mass_t mass, uint32_t part)
 {
@@ -113,6 +117,7 @@ __device__ __forceinline__ Prefix<K> select_mass(const S *row, uint32_t n, Prefi
                 const K key = key_of(v[i]);
                 if (i < count && key > pk.t && ((key ^ prefix) >> shift) < 256)
                     atomicAdd(&bins[(uint32_t)(key >> shift) & 255u], weight(v[i]));
+                one_at_a_time();
             }
         });
         const Digit<mass_t> d = find_digit(bins, need, found);
@@ -424,8 +429,10 @@ __device__ __forceinline__ void draw_along(const SampleArgs &g, uint64_t row, co
             if (w)
                 w[e] = x;
             sum += x;
-            if (e % 4 == 3) // eight exponentials at once would take the registers of two waves
+            if (e % 4 == 3) { // eight exponentials at once would take the registers of two waves
+                added(sum);
                 one_at_a_time();
+            }
         }
         return sum;
     };
@@ -648,9 +655,11 @@ __device__ __forceinline__ void draw_by_search(const SampleArgs &g, uint64_t row
         mass_t mass = 0;
         each_vec<S, NT>(s, n, [&](const T *v, uint32_t at, uint32_t values) {
 #pragma unroll
-            for (uint32_t i = 0; i < N; i++)
+            for (uint32_t i = 0; i < N; i++) {
                 if (i < values && last.keeps(v[i], at + i))
                     mass += weight(v[i]);
+                added(mass);
+            }
         });
         mass = share_of(block_reduce<NT>(mass, OpSum(), sh.red[0]), set.part);
         last = nucleus_exactly<S, NT>(s, n, pk, mass ? mass : 1, weight, sh);
@@ -799,8 +808,11 @@ template <typename S> struct Chunk {
     {
         vectors([&](const T *v, auto count, uint32_t at) {
 #pragma unroll
-            for (int k = 0; k < count; k++)
+            for (int k = 0; k < count; k++) {
                 f(v[k], at + k);
+                if (k % 4 == 3)
+                    one_at_a_time();
+            }
         });
     }
     // The largest values of this thread's vectors, every eighth of them in one group.
@@ -1094,7 +1106,10 @@ template <typename S> __device__ __forceinline__ bool sample_weigh(const SplitAr
             return w >= set.least ? w : 0;
         };
         mass_t own = 0;
-        part.each([&](T v, uint32_t at) { own += mass_of(v, at); });
+        part.each([&](T v, uint32_t at) {
+            own += mass_of(v, at);
+            added(own);
+        });
         own = block_reduce<NT>(own, OpSum(), sh.red[0]);
         if (threadIdx.x == 0)
             put(&a.chunk_mass[blockIdx.x], own);
@@ -1119,30 +1134,32 @@ template <typename S> __device__ __forceinline__ bool sample_weigh(const SplitAr
         put(&a.steps[(uint64_t)blockIdx.x * kSteps + b], sh.steps[b]);
     if (!last_chunk(&a.state[row].done[1], a.chunks))
         return false;
-    // The step in which the nucleus ends, and the chunks' masses before it.
+    // The step in which the nucleus ends, from the sums of the chunks' steps; 16 loads in flight.
     const mass_t *steps = a.steps + row * a.chunks * kSteps;
-    for (uint32_t b = threadIdx.x; b < kSteps; b += NT) {
-        mass_t sum = 0;
-#pragma unroll 8
-        for (uint32_t c = 0; c < a.chunks; c++)
-            sum += get(&steps[c * kSteps + b]);
-        sh.steps[b] = sum;
+    constexpr uint32_t E = kSteps / NT, U = 4;
+    mass_t sum[E] = {};
+    for (uint32_t c = 0; c < a.chunks; c += U) {
+        mass_t x[U][E];
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++)
+#pragma unroll
+            for (uint32_t e = 0; e < E; e++)
+                x[u][e] = c + u < a.chunks ? get(&steps[(c + u) * kSteps + e * NT + threadIdx.x]) : 0;
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++)
+#pragma unroll
+            for (uint32_t e = 0; e < E; e++)
+                sum[e] += x[u][e];
     }
+#pragma unroll
+    for (uint32_t e = 0; e < E; e++)
+        sh.steps[e * NT + threadIdx.x] = sum[e];
     __syncthreads();
     const End end = find_end(sh, set.part);
     if (threadIdx.x == 0) {
         a.state[row].need = end.need;
         a.state[row].above = end.above;
         a.state[row].step = end.step;
-    }
-    for (uint32_t c = threadIdx.x / 64; c < a.chunks; c += NT / 64) {
-        mass_t before = 0;
-#pragma unroll 4
-        for (uint32_t b = threadIdx.x & 63; b < end.step; b += 64)
-            before += get(&steps[c * kSteps + b]);
-        before = wave_reduce(before, OpSum());
-        if ((threadIdx.x & 63) == 0)
-            a.chunk_mass[row * a.chunks + c] = before;
     }
     return false;
 }
@@ -1174,18 +1191,26 @@ template <typename S> __device__ __forceinline__ bool sample_edge(const SplitArg
     const Weight<T> weight{m, set.inv};
     const uint32_t end = a.state[row].step;
     part.gather(list, [&](T v) { return v > -INFINITY && step_of(v) == end; });
-    if (set.least > 0) { // of the chunk's mass before the step, what min_p leaves
-        mass_t own = 0;
+    // The chunk's mass before the step, or what min_p leaves of it.
+    mass_t own = 0;
+    if (set.least > 0) {
         part.each([&](T v, uint32_t) {
             if (v > -INFINITY && step_of(v) < end) {
                 const mass_t w = weight(v);
                 own += w >= set.least ? w : 0;
+                added(own);
             }
         });
-        own = block_reduce<NT>(own, OpSum(), sh.red[0]);
-        if (threadIdx.x == 0)
-            put(&a.chunk_mass[blockIdx.x], own);
+    } else {
+#pragma unroll
+        for (uint32_t e = 0; e < kSteps / NT; e++) {
+            const mass_t here = a.steps[(uint64_t)blockIdx.x * kSteps + e * NT + threadIdx.x];
+            own += e * NT + threadIdx.x < end ? here : 0;
+        }
     }
+    own = block_reduce<NT>(own, OpSum(), sh.red[0]);
+    if (threadIdx.x == 0)
+        put(&a.chunk_mass[blockIdx.x], own);
     __syncthreads();
     hand_over(a, row, list);
     if (!last_chunk(&a.state[row].done[2], a.chunks))
