@@ -1,0 +1,180 @@
+"""The operators on logits as they are used together, and where the way a call is carried out
+changes with its sizes: every way gives a row the same results, bit for bit."""
+import importlib.util
+import os
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.fixture(scope="module")
+def ctx(pcu_pkg):
+    c = pcu_pkg.Context(0)
+    yield c
+    c.close()
+
+
+def test_the_example_learns_and_writes(ctx, pcu_pkg):
+    spec = importlib.util.spec_from_file_location("distill_and_sample", os.path.join(ROOT, "examples", "distill_and_sample.py"))
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    losses, text = example.run(ctx)
+    # Plain 64-bit training on inputs drawn alike ends at 0.23 of its first loss.
+    assert np.all(np.isfinite(losses)) and losses[-1] < 0.5 * losses[0]
+    assert text.shape == (4, 13) and np.all((text >= 0) & (text < 1000))
+    again, same = example.run(ctx)
+    assert losses == again and np.array_equal(text, same)
+
+
+def _distill_args(ctx, rng, rows, vocab, k, dtype=np.float32):
+    s = rng.normal(0, 2, (rows, vocab)).astype(dtype)
+    ti = rng.integers(0, vocab, (rows, k)).astype(np.int32)
+    ti[0, : k // 2] = ti[0, 0]  # duplicates
+    ti[rows // 2, 1] = -1
+    tv = rng.normal(0, 2, (rows, k)).astype(np.float32)
+    labels = rng.integers(-1, vocab, rows).astype(np.int32)
+    return s, tv, ti, labels
+
+
+def _some(a, rows):
+    return np.ascontiguousarray(a[rows])
+
+
+# 64 rows end their program in the kernel, 65 do not.
+@pytest.mark.parametrize("vocab", [250, 1000])
+@pytest.mark.parametrize("dtype", [np.float32, np.float64, np.float16])
+@pytest.mark.parametrize("pad", [0, 3])
+def test_small_calls_give_a_row_what_larger_ones_do(ctx, vocab, dtype, pad):
+    rng = np.random.default_rng(vocab + pad)
+    rows = 130
+    s, tv, ti, labels = _distill_args(ctx, rng, rows, vocab + pad, 9, dtype)
+    ti, labels = np.minimum(ti, vocab - 1), np.minimum(labels, vocab - 1)
+
+    def call(part):
+        x = ctx.upload(_some(s, part))
+        loss, grad = ctx.native_distill_step(x, ctx.upload(_some(tv, part)), ctx.upload(_some(ti, part)), vocab=vocab,
+                                             labels=ctx.upload(_some(labels, part)), temperature=1.7, label_weight=0.4)
+        loss2, sums = ctx.native_distill_loss(x, ctx.upload(_some(tv, part)), ctx.upload(_some(ti, part)), vocab=vocab,
+                                              labels=ctx.upload(_some(labels, part)), temperature=1.7, label_weight=0.4)
+        values, indices, log_sum = ctx.native_top_logits(x, 9, vocab=vocab)
+        tokens, log_prob = ctx.native_sample(x, ctx.upload(np.linspace(0, 0.99, rows, dtype=np.float32)[part]), top_p=0.9,
+                                             vocab=vocab)
+        return [a.numpy() for a in (loss, grad, loss2, sums, values, indices, log_sum, tokens, log_prob)]
+
+    whole = call(np.arange(rows))
+    for part in (np.arange(64), np.arange(64, 65), np.arange(65, 130)):
+        for a, b in zip(call(part), whole):
+            np.testing.assert_array_equal(a, b[part])
+
+
+# Rows split over workgroups (few of them) and rows that one workgroup holds; the sums' order differs,
+# so the bound is that of two sums of n positive terms and the exponentials of each.
+def test_few_long_rows_agree_with_many(ctx):
+    rng = np.random.default_rng(3)
+    rows, vocab, k = 64, 40007, 20
+    s, tv, ti, labels = _distill_args(ctx, rng, rows, vocab, k)
+    kw = dict(temperature=1.3, label_weight=0.6)
+    many = ctx.native_distill_step(ctx.upload(s), ctx.upload(tv), ctx.upload(ti), labels=ctx.upload(labels), **kw)
+    few = ctx.native_distill_step(ctx.upload(s[:5]), ctx.upload(tv[:5]), ctx.upload(ti[:5]), labels=ctx.upload(labels[:5]), **kw)
+    rel = 2 * 2.0 ** -24 * (8 * np.abs(s).max() + vocab / 64 + 64)
+    scale = 1.3 * 1.3 + 0.6
+    for a, b in zip(few, many):
+        a, b = a.numpy().astype(np.float64), b.numpy()[:5].astype(np.float64)
+        assert np.max(np.abs(a - b)) <= rel * scale * 16
+
+
+@pytest.mark.parametrize("rows,vocab", [(3, 70001), (5, 150000), (70, 9001)])
+@pytest.mark.parametrize("temperature", [1.0, 2.0])
+def test_a_gradient_in_the_logits_place(ctx, rows, vocab, temperature):
+    rng = np.random.default_rng(rows)
+    s, tv, ti, labels = _distill_args(ctx, rng, rows, vocab, 30)
+    args = [ctx.upload(a) for a in (tv, ti)]
+    kw = dict(labels=ctx.upload(labels), temperature=temperature, label_weight=0.5)
+    x = ctx.upload(s)
+    loss, grad = ctx.native_distill_step(x, *args, **kw)
+    loss2, grad2 = ctx.native_distill_step(x, *args, gradient=x, **kw)
+    assert grad2 is x
+    np.testing.assert_array_equal(loss.numpy(), loss2.numpy())
+    np.testing.assert_array_equal(grad.numpy(), x.numpy())
+    x = ctx.upload(s)
+    _, sums = ctx.native_distill_loss(x, *args, **kw)
+    apart = ctx.native_distill_backward(x, *args, sums, **kw).numpy()
+    ctx.native_distill_backward(x, *args, sums, gradient=x, **kw)
+    np.testing.assert_array_equal(apart, x.numpy())
+
+
+def test_a_large_gradient_is_a_small_ones(ctx):
+    """Gradients above the size that is stored past the caches against those of the rows' halves."""
+    rng = np.random.default_rng(4)
+    rows, vocab = 300, 60001  # 72 MB
+    s, tv, ti, labels = _distill_args(ctx, rng, rows, vocab, 40)
+
+    def call(part):
+        x = ctx.upload(_some(s, part))
+        args = [ctx.upload(_some(a, part)) for a in (tv, ti)]
+        kw = dict(labels=ctx.upload(_some(labels, part)), temperature=2.0, label_weight=0.2)
+        loss, grad = ctx.native_distill_step(x, *args, **kw)
+        _, sums = ctx.native_distill_loss(x, *args, **kw)
+        back = ctx.native_distill_backward(x, *args, sums, **kw)
+        return [a.numpy() for a in (loss, grad, sums, back)]
+
+    whole = call(np.arange(rows))
+    for part in (np.arange(150), np.arange(150, 300)):
+        for a, b in zip(call(part), whole):
+            np.testing.assert_array_equal(a, b[part])
+
+
+def _mixed(ctx, rng, rows):
+    return {"temperature": ctx.upload((0.5 + rng.random(rows)).astype(np.float32)),
+            "top_k": ctx.upload(np.where(rng.random(rows) < 0.5, rng.integers(1, 1500, rows), 0).astype(np.int32)),
+            "top_p": ctx.upload(np.where(rng.random(rows) < 0.5, rng.random(rows), 1.0).astype(np.float32)),
+            "min_p": ctx.upload(np.where(rng.random(rows) < 0.3, 0.1, 0.0).astype(np.float32))}
+
+
+@pytest.mark.parametrize("dtype,vocab", [(np.float64, 2101), (np.float32, 4111)])
+def test_samples_of_more_rows_than_share_a_scratch(ctx, dtype, vocab):
+    rng = np.random.default_rng(vocab)
+    rows = 2100
+    x = rng.normal(0, 2, (rows, vocab)).astype(dtype)
+    u = rng.random(rows).astype(np.float32)
+    settings = _mixed(ctx, rng, rows)
+    tokens, log_prob = ctx.native_sample(ctx.upload(x), ctx.upload(u), **settings)
+    tokens, log_prob = tokens.numpy(), log_prob.numpy()
+    assert np.all((tokens >= 0) & (tokens < vocab))
+    host = {n: a.numpy() for n, a in settings.items()}
+    for part in (np.arange(7), np.arange(1000, 1070), np.arange(2040, 2100)):
+        t, lp = ctx.native_sample(ctx.upload(_some(x, part)), ctx.upload(u[part]),
+                                  **{n: ctx.upload(_some(a, part)) for n, a in host.items()})
+        np.testing.assert_array_equal(t.numpy(), tokens[part])
+        np.testing.assert_array_equal(lp.numpy(), log_prob[part])
+
+
+def test_samples_after_a_fault_are_what_they_were(ctx, pcu_pkg):
+    """What the launches of long rows leave for the next call is in order again after a fault, in a
+    call of its own and in a program whose later nodes are skipped."""
+    rng = np.random.default_rng(12)
+    rows, vocab = 40, 30001
+    x = ctx.upload(rng.normal(0, 2, (rows, vocab)).astype(np.float32))
+    u = rng.random(rows).astype(np.float32)
+    good, settings = ctx.upload(u), _mixed(ctx, rng, rows)
+    bad = u.copy()
+    bad[17] = 1.5
+    bad = ctx.upload(bad)
+    want = ctx.native_sample(x, good, **settings)[0].numpy()
+    with pytest.raises(pcu_pkg.PcuExecutionError) as e:
+        ctx.native_sample(x, bad, **settings)
+    assert e.value.tensor_fault.element_index == 17
+    np.testing.assert_array_equal(ctx.native_sample(x, good, **settings)[0].numpy(), want)
+    with pytest.raises(pcu_pkg.PcuExecutionError):
+        with ctx.program():
+            ctx.native_sample(x, bad, **settings)
+            ctx.native_sample(x, good, **settings)
+    for _ in range(2):
+        np.testing.assert_array_equal(ctx.native_sample(x, good, **settings)[0].numpy(), want)
+    with ctx.program():
+        tokens = [ctx.native_sample(x, good, **settings)[0] for _ in range(3)]
+    for t in tokens:
+        np.testing.assert_array_equal(t.numpy(), want)
