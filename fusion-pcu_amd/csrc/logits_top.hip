@@ -5,6 +5,11 @@
 // One workgroup a row, the row in registers where it fits: one read, the maximum and the sum of
 // exponentials, a bound from the maxima of groups of the row, the values that reach it gathered
 // and sorted in LDS (see pcu_select.hpp).
+//
+// Many rows are bound by their one read: 2048 x 32000 bf16 with k = 64 takes 33.8 us of kernel, 3.9
+// TB/s, where a copy reaches 4.9; 511 x 50257 f32 with k = 500 takes 41 us, 2.5 TB/s, since one row a
+// CU at a time lays its list and sort (14 us) open behind its read. A few short rows are a chain of
+// barriers: 64 x 1000 f32 with k = 8 takes 8.8 us, the end of the program among them.
 #include "pcu_kernels.hpp"
 #include "pcu_select.hpp"
 
@@ -147,7 +152,9 @@ template <typename S, int NT, int R, int G, int CAP> __device__ __forceinline__ 
     }
 }
 
-// A call of its own ends its program in this kernel (close).
+// A call of its own of at most kCloseMaxBlocks rows ends its program in this kernel (close): 64 x 1000
+// f32 17.5 us a call with a launch for it, 14.9 so; with every row's ticket on the one counter 2048
+// rows take 106 us for 48.
 template <typename S, int NT, int R, int G, int CAP>
 __global__ __launch_bounds__(NT) void k_top(TopArgs g, ProgramClose close)
 {
@@ -165,6 +172,15 @@ template <typename S, int NT, int R> hipError_t launch_row(hipStream_t s, const 
     return hipGetLastError();
 }
 
+// As few threads as hold the row, with at most 16 vectors each, since the reductions' and the list's
+// barriers cost by the wave, and 4 groups for each of the k wanted (2 above k = 256). Microseconds
+// a call, against the next form:
+//   256 x 4 to 256 x 16: 2048 x 4096 f32, k 16, 24.9 and 34
+//   256 x 16 to 1024 x 4: 2048 x 32000 bf16, k 64, 57 and 62; k above 256 overflows the list too
+//     often (512 x 16000 f32: k 300 30 with 1024 x 4 and 41, k 1000 47 and 149)
+//   512 x 16 to 1024 x 16: 512 x 32000 f32, k 64, 29 and 50
+//   1024 x 16 to a row read again for each walk: 511 x 50257 f32, k 500, 51 and 63. (Binary64 with
+//     that many would spill.)
 template <typename S> hipError_t launch_t(hipStream_t s, const TopArgs &g, const ProgramClose &close)
 {
     const uint32_t vecs = g.vocab / kVec<S>;
@@ -172,8 +188,13 @@ template <typename S> hipError_t launch_t(hipStream_t s, const TopArgs &g, const
         return launch_row<S, 256, 4>(s, g, close);
     if (vecs <= 256 * 16 && g.k <= 256)
         return launch_row<S, 256, 16>(s, g, close);
-    if (sizeof(S) < 8 && vecs <= 1024 * 16) // binary64 would spill
-        return launch_row<S, 1024, 16>(s, g, close);
+    if (vecs <= 1024 * 4)
+        return launch_row<S, 1024, 4>(s, g, close);
+    if (vecs <= 512 * 16)
+        return launch_row<S, 512, 16>(s, g, close);
+    if constexpr (sizeof(S) < 8)
+        if (vecs <= 1024 * 16)
+            return launch_row<S, 1024, 16>(s, g, close);
     return launch_row<S, 1024, 0>(s, g, close);
 }
 
