@@ -11,6 +11,12 @@
 // Weights are integers, so every mass is exact whatever the order of its additions: a row's
 // token does not depend on how the row is split over lanes, and a tie never does. A token below
 // 2^-40 of the largest weight is never drawn. The exponential is the library's binary32 one.
+//
+// What bounds it: not the one read of the logits but the steps that wait for the whole row (maximum,
+// bound or masses, list, place in the order, drawing), each a few barriers and trips to memory, over
+// up to three launches. One row of 128000 bf16 with top-k and top-p takes 17 us of kernel in one launch,
+// 64 x 50257 f32 with top-p 6 + 14 + 23 us, 512 x 152000 bf16 of mixed settings 63 + 47 + 58 us
+// (156 MB: 32 us at the rate of a copy).
 #include "pcu_kernels.hpp"
 #include "pcu_select.hpp"
 
@@ -293,7 +299,10 @@ template <int NT, typename L, typename M> __device__ __forceinline__ mass_t mass
     return block_reduce<NT>(sum, OpSum(), lds);
 }
 
-constexpr uint32_t kFew = 128; // entries that are drawn from one a thread
+// Entries that are drawn from one a thread, which reads the whole list twice: 1 x 128000 bf16 with top-k
+// 50 and top-p 27 us a call, 40 from the list digit by digit; 32 x 50257 f32 with top-k 100, lists of 96
+// to 128, 43 and 37.
+constexpr uint32_t kFew = 96;
 
 // Draws from a list of at most kFew entries in LDS, one a thread, which holds the first top_k of the order
 // (or all of it that is finite): each entry counts the entries before it in the order with
@@ -679,7 +688,7 @@ __device__ __forceinline__ void draw_by_search(const SampleArgs &g, uint64_t row
 //   first: the chunk's maximum. A row whose top_k a list can hold: the chunk's values beyond a bound
 //          that top_k of them reach go to the row's list, and the last chunk draws from it.
 //          (Such a row's chunks take every chunks-th block of vectors, so that they hold alike values
-//          wherever the row's large ones lie. Where top_k times the chunks would overflow the list,
+//          wherever the row's large ones lie. Where top_k times the chunks would make the list long,
 //          the bound is one that the chunk's share of top_k reaches, and the list is made in the
 //          second launch from the lowest of the bounds.)
 //   weigh: with the row's maximum, the chunk's mass, and the last chunk draws in the chunk that
@@ -726,12 +735,13 @@ template <typename T> struct SplitArgs {
     uint32_t *at;              // rows x kRowCap
 };
 
-// Whether the chunks' own lists of the top `k` fit the row's (a list holds up to half as many
-// again as its bound was made for).
-__host__ __device__ inline bool list_at_once(uint64_t k, uint32_t chunks)
-{
-    return k * chunks <= kRowCap / 2 && k <= kChunkListCap / 2;
-}
+// Whether the chunks' own lists of the top `k` make the row's: then the first launch ends the row, but
+// its last chunk takes a list of all of them, up to half as many again as the bounds were made for.
+// (32 x 50257 f32 in 12 chunks, microseconds a call: top-k 50 28, 35 with a second launch; top-k 100 43 and
+// 41; top-k 300 68 and 42.)
+constexpr uint64_t kListAtOnce = 1024;
+__host__ __device__ inline bool list_at_once(uint64_t k, uint32_t chunks) { return k * chunks <= kListAtOnce; }
+static_assert(kListAtOnce / 2 * 3 / 2 <= kChunkListCap, "a chunk's list of k <= kListAtOnce / 2 values fits");
 __device__ __forceinline__ uint32_t kind_of(const Settings &s, uint32_t n, uint32_t chunks)
 {
     if (!s.ok)
@@ -1291,8 +1301,9 @@ struct Split {
 };
 
 // Chunks of long rows: 1536 workgroups for the chip, as far as each has four vectors a thread, at most
-// 16384 logits each; at most 32 a row (the nucleus adds up 8 KB for each), and two at least, so that
-// 1024 values are sought among 2048 groups.
+// about 16384 logits each (512 x 152000 bf16 of mixed settings: 181 us a call; 217 with twice as many
+// to a chunk, 307 with half); at most 32 a row (the nucleus adds up 8 KB for each), and two at least, so
+// that 1024 values are sought among 2048 groups.
 Split split_of(uint64_t rows, uint32_t vocab, uint32_t per_vec)
 {
     const uint64_t want = (1536 + rows - 1) / rows, most = vocab / (4 * kChunkThreads * per_vec), least = vocab / 16384;
@@ -1306,7 +1317,9 @@ Split split_of(uint64_t rows, uint32_t vocab, uint32_t per_vec)
 
 constexpr uint64_t kSlabRows = 1024; // rows that share one scratch
 
-// Rows of up to 1024 whole vectors are one workgroup's.
+// Rows of up to 1024 whole vectors are one workgroup's: one launch, the row in registers (microseconds a
+// call, and split: 1024 x 8000 bf16 of mixed settings 64 and 91, 64 x 4000 f32 with top-k 21 and 28, 1024
+// rows with top-p 59 and 67, 64 rows 53 and 49).
 bool short_row(const SampleArgs &g, uint32_t per_vec) { return g.vocab / per_vec <= 256 * 4; }
 
 // Whether a row may have a nucleus.

@@ -7,9 +7,9 @@
 // and sorted in LDS (see pcu_select.hpp).
 //
 // Many rows are bound by their one read: 2048 x 32000 bf16 with k = 64 takes 33.8 us of kernel, 3.9
-// TB/s, where a copy reaches 4.9; 511 x 50257 f32 with k = 500 takes 41 us, 2.5 TB/s, since one row a
-// CU at a time lays its list and sort (14 us) open behind its read. A few short rows are a chain of
-// barriers: 64 x 1000 f32 with k = 8 takes 8.8 us, the end of the program among them.
+// TB/s, where a copy reaches 4.9; 511 x 50257 f32 with k = 500 takes 41 us, 2.5 TB/s: a row
+// takes a CU's registers whole, and its list and sort lie open behind its read. A few short rows are a
+// chain of barriers: 64 x 1000 f32 with k = 8 takes 8.8 us, the end of the program among them.
 #include "pcu_kernels.hpp"
 #include "pcu_select.hpp"
 
@@ -152,9 +152,9 @@ template <typename S, int NT, int R, int G, int CAP> __device__ __forceinline__ 
     }
 }
 
-// A call of its own of at most kCloseMaxBlocks rows ends its program in this kernel (close): 64 x 1000
-// f32 17.5 us a call with a launch for it, 14.9 so; with every row's ticket on the one counter 2048
-// rows take 106 us for 48.
+// A call of its own of at most kCloseMaxBlocks rows ends its program in this kernel (close) instead of
+// a launch of 4 us; with every row's ticket on the one counter 2048 x 32000 bf16 took 106 us a call for
+// 48.
 template <typename S, int NT, int R, int G, int CAP>
 __global__ __launch_bounds__(NT) void k_top(TopArgs g, ProgramClose close)
 {
@@ -173,8 +173,7 @@ template <typename S, int NT, int R> hipError_t launch_row(hipStream_t s, const 
 }
 
 // As few threads as hold the row, with at most 16 vectors each, since the reductions' and the list's
-// barriers cost by the wave, and 4 groups for each of the k wanted (2 above k = 256). Microseconds
-// a call, against the next form:
+// barriers cost by the wave. Microseconds a call, against the next form:
 //   256 x 4 to 256 x 16: 2048 x 4096 f32, k 16, 24.9 and 34
 //   256 x 16 to 1024 x 4: 2048 x 32000 bf16, k 64, 57 and 62; k above 256 overflows the list too
 //     often (512 x 16000 f32: k 300 30 with 1024 x 4 and 41, k 1000 47 and 149)
