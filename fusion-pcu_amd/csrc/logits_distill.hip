@@ -229,7 +229,9 @@ template <typename S, int NT, int R, bool GRAD> __device__ __forceinline__ void 
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ T red[7][16];
     const uint32_t tid = threadIdx.x;
-    const uint64_t row = blockIdx.x;
+    const uint64_t row = row_of_block();
+    if (row >= g.rows)
+        return;
     const S *s = static_cast<const S *>(g.logits) + row * g.stride;
     const uint32_t whole = g.vocab / N, rest = whole * N + tid;
     const bool has_rest = rest < g.vocab; // at most N - 1 lanes
@@ -495,8 +497,11 @@ __global__ __launch_bounds__(NT) void k_distill_grad(DistillArgs g, uint32_t chu
     constexpr int U = 4;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ T red[7][16];
-    const uint64_t row = blockIdx.x / chunks;
-    const uint32_t chunk = blockIdx.x % chunks;
+    const uint32_t block = row_of_block(); // rows x chunks of them, below 2^31
+    const uint64_t row = block / chunks;
+    const uint32_t chunk = block % chunks;
+    if (row >= g.rows)
+        return;
     const S *s = static_cast<const S *>(g.logits) + row * g.stride;
     S *grad = static_cast<S *>(g.grad) + row * g.grad_stride;
     const uint32_t first = chunk * chunk_vecs, last = first + chunk_vecs;
@@ -592,6 +597,7 @@ Split split_of(uint64_t rows, uint32_t vecs)
 {
     // Enough workgroups for the chip, each with at least 4 vectors a thread.
     const uint64_t want = (2048 + rows - 1) / rows;
+    vecs = vecs ? vecs : 1; // a row without logits is one chunk
     const uint64_t most = (vecs + 4 * kSplitThreads - 1) / (4 * kSplitThreads);
     const uint64_t chunks = want < most ? want : most;
     const uint32_t each = (uint32_t)((vecs + chunks - 1) / chunks);
@@ -602,9 +608,9 @@ template <typename S, int NT, int R> hipError_t launch_row(hipStream_t s, const 
 {
     const size_t lds = Entries<typename StatOf<S>::T>::bytes(g.k);
     if (g.grad)
-        hipLaunchKernelGGL((k_distill_row<S, NT, R, true>), dim3((unsigned)g.rows), dim3(NT), lds, s, g, close);
+        hipLaunchKernelGGL((k_distill_row<S, NT, R, true>), row_grid(g.rows), dim3(NT), lds, s, g, close);
     else
-        hipLaunchKernelGGL((k_distill_row<S, NT, R, false>), dim3((unsigned)g.rows), dim3(NT), lds, s, g, close);
+        hipLaunchKernelGGL((k_distill_row<S, NT, R, false>), row_grid(g.rows), dim3(NT), lds, s, g, close);
     return hipGetLastError();
 }
 
@@ -613,7 +619,7 @@ hipError_t launch_grad(hipStream_t s, const DistillArgs &g, Split sp, const Part
                        const typename StatOf<S>::T *picked)
 {
     const size_t lds = Entries<typename StatOf<S>::T>::bytes(g.k);
-    hipLaunchKernelGGL((k_distill_grad<S, kSplitThreads>), dim3((unsigned)(g.rows * sp.chunks)), dim3(kSplitThreads),
+    hipLaunchKernelGGL((k_distill_grad<S, kSplitThreads>), row_grid(g.rows * sp.chunks), dim3(kSplitThreads),
                        lds, s, g, sp.chunks, sp.vecs, parts, picked);
     return hipGetLastError();
 }

@@ -518,7 +518,9 @@ template <typename S, int NT, int R> __device__ __forceinline__ void sample_row(
     constexpr uint32_t kCap = 2048;
     __shared__ List<K, kCap> list;
     const uint32_t tid = threadIdx.x;
-    const uint64_t row = blockIdx.x;
+    const uint64_t row = row_of_block();
+    if (row >= g.rows)
+        return;
     const S *s = static_cast<const S *>(g.logits) + row * g.stride;
     const uint32_t n = g.vocab;
     const Settings set = settings_of(g, row);
@@ -1371,7 +1373,7 @@ template <typename S> hipError_t launch_t(hipStream_t s, const SampleArgs &all, 
 {
     using T = typename StatOf<S>::T;
     if (short_row(all, kVec<S>)) {
-        hipLaunchKernelGGL((k_sample<S, 256, 4>), dim3((unsigned)all.rows), dim3(256), 0, s, all, close);
+        hipLaunchKernelGGL((k_sample<S, 256, 4>), row_grid(all.rows), dim3(256), 0, s, all, close);
         return hipGetLastError();
     }
     for (uint64_t from = 0; from < all.rows; from += kSlabRows) {

@@ -81,7 +81,9 @@ template <typename S, int NT, int R, int G, int CAP> __device__ __forceinline__ 
     __shared__ List<K, CAP> list;
     __shared__ SortShared<T> sort;
     const uint32_t tid = threadIdx.x;
-    const uint64_t row = blockIdx.x;
+    const uint64_t row = row_of_block();
+    if (row >= g.rows)
+        return;
     const S *s = static_cast<const S *>(g.logits) + row * g.stride;
     const uint32_t n = g.vocab, k = g.k < n ? g.k : n;
     const Row<S, NT, R> held(s, n);
@@ -164,7 +166,7 @@ __global__ __launch_bounds__(NT) void k_top(TopArgs g, ProgramClose close)
 
 template <typename S, int NT, int R> hipError_t launch_row(hipStream_t s, const TopArgs &g, const ProgramClose &close)
 {
-    const dim3 grid((unsigned)g.rows), block(NT);
+    const dim3 grid = row_grid(g.rows), block(NT);
     if (g.k * 4 <= NT)
         hipLaunchKernelGGL((k_top<S, NT, R, 1, 512>), grid, block, 0, s, g, close);
     else

@@ -217,6 +217,15 @@ __device__ __forceinline__ void store_vec(S *row, uint32_t i, uint32_t n, const 
     }
 }
 
+// One workgroup a row: a launch's threads have to stay below 2^32 along each axis of its grid, so many
+// rows take its second axis too. Rows past the last one (~0 below) have workgroups without work.
+constexpr uint32_t kRowsAlong = 1u << 20;
+inline dim3 row_grid(uint64_t rows)
+{
+    return rows <= kRowsAlong ? dim3((unsigned)rows) : dim3(kRowsAlong, (unsigned)((rows + kRowsAlong - 1) / kRowsAlong));
+}
+__device__ __forceinline__ uint32_t row_of_block() { return blockIdx.y * kRowsAlong + blockIdx.x; }
+
 // --------------------------------------------------------- reductions of a workgroup
 struct OpMax {
     template <typename T> __device__ __forceinline__ T none() const { return (T)-INFINITY; }

@@ -178,3 +178,50 @@ def test_samples_after_a_fault_are_what_they_were(ctx, pcu_pkg):
         tokens = [ctx.native_sample(x, good, **settings)[0] for _ in range(3)]
     for t in tokens:
         np.testing.assert_array_equal(t.numpy(), want)
+
+
+def test_more_rows_than_one_axis_of_a_grid(ctx, pcu_pkg):
+    """17 million rows of three logits: more threads than a launch takes along one axis."""
+    rows, vocab = (1 << 24) + 259, 3
+    rng = np.random.default_rng(9)
+    x = rng.integers(-8, 9, (rows, vocab), dtype=np.int8).astype(np.float16)
+    xd = ctx.upload(x)
+    values, indices, _ = ctx.native_top_logits(xd, 1)
+    first = np.argmax(x, axis=1)  # the lowest index of the largest
+    assert np.array_equal(indices.numpy()[:, 0], first)
+    assert np.array_equal(values.numpy()[:, 0], x[np.arange(rows), first])
+    tokens, _ = ctx.native_sample(xd, ctx.upload(np.zeros(rows, np.float32)), top_k=1)
+    assert np.array_equal(tokens.numpy(), first)
+    # One entry a row, the largest logit: q = 1 and T = 1, so the gradient is p less one there.
+    loss, grad = ctx.native_distill_step(xd, values, indices)
+    back = ctx.native_distill_backward(xd, values, indices, ctx.native_distill_loss(xd, values, indices)[1])
+    e = np.exp(x.astype(np.float32) - x.max(axis=1, keepdims=True))
+    total = e.sum(axis=1)
+    # Exponents of at most 16: each side within 200 units of binary32; the gradient's own rounding 2^-11.
+    tol = 400 * 2.0 ** -24
+    want = e / total[:, None]
+    want[np.arange(rows), first] -= 1
+    assert np.max(np.abs(loss.numpy() - np.log(total))) <= tol
+    for g in (grad, back):
+        assert np.max(np.abs(g.numpy() - want)) <= tol + 2.0 ** -11
+    labels = np.full(rows, -1, np.int32)
+    labels[-1] = vocab
+    with pytest.raises(pcu_pkg.PcuExecutionError) as e:
+        ctx.native_distill_loss(xd, values, indices, labels=ctx.upload(labels), label_weight=1.0)
+    assert e.value.tensor_fault.element_index == (rows - 1) * 2 + 1
+
+
+def test_rows_without_logits(ctx):
+    """Rows of padding alone: every output as a row without probabilities has it."""
+    x = ctx.upload(np.ones((5, 3), np.float32))
+    tv, ti = ctx.upload(np.zeros((5, 2), np.float32)), ctx.upload(np.full((5, 2), -1, np.int32))
+    loss, grad = ctx.native_distill_step(x, tv, ti, vocab=0)
+    assert np.all(loss.numpy() == 0) and np.all(grad.numpy() == 0)
+    loss, sums = ctx.native_distill_loss(x, tv, ti, vocab=0)
+    assert np.all(loss.numpy() == 0) and np.all(np.isneginf(sums.numpy()))
+    grad = ctx.native_distill_backward(x, tv, ti, sums, vocab=0)
+    assert np.all(grad.numpy() == 0)
+    values, indices, log_sum = ctx.native_top_logits(x, 2, vocab=0)
+    assert np.all(np.isneginf(values.numpy())) and np.all(indices.numpy() == -1) and np.all(np.isneginf(log_sum.numpy()))
+    tokens, log_prob = ctx.native_sample(x, ctx.upload(np.zeros(5, np.float32)), vocab=0)
+    assert np.all(tokens.numpy() == -1) and np.all(np.isneginf(log_prob.numpy()))
