@@ -15,7 +15,7 @@
 // What bounds it: not the one read of the logits but the steps that wait for the whole row (maximum,
 // bound or masses, list, place in the order, drawing), each a few barriers and trips to memory, over
 // up to three launches. One row of 128000 bf16 with top-k and top-p takes 17 us of kernel in one launch,
-// 64 x 50257 f32 with top-p 6 + 14 + 23 us, 512 x 152000 bf16 of mixed settings 63 + 47 + 58 us
+// 64 x 50257 f32 with top-p 6 + 14 + 24 us, 512 x 152000 bf16 of mixed settings 52 + 53 + 59 us
 // (156 MB: 32 us at the rate of a copy).
 #include "pcu_kernels.hpp"
 #include "pcu_select.hpp"
