@@ -2,7 +2,7 @@
 implementations in 64 bits, at the sizes, ties, masks and settings where they can go wrong.
 
 Tolerances. u is half the statistics' unit roundoff spacing (2^-24 binary32, 2^-53 binary64).
-A row's exponentials are taken of s * c - m * c with c = log2(e) / T, which carries 3 roundings,
+A row's exponentials are taken of (s - m) * c with c = log2(e) / T, which carries 3 roundings,
 so an exponent x in natural units is off by at most 4 u |x| and the exponential by 2 u more (the
 hardware's 2^x and the product); a sum of n positive terms over at least 64 lanes adds at most
 (n / 64 + 16) u. With B the largest |s / T| (and |v / T|) of finite values this bounds the relative
