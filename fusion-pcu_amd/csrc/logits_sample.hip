@@ -756,7 +756,8 @@ __device__ __forceinline__ uint32_t kind_of(const Settings &s, uint32_t n, uint3
 // What a chunk hands to the others of its row within a launch is written through the caches that
 // they do not share (put), and is complete (a wait for the wave's own stores, then the barrier)
 // before the workgroup counts itself as done.
-// Whether this workgroup is the last of the row's chunks; whole workgroup, once a launch.
+// Whether this workgroup is the last of the row's chunks; whole workgroup, at most once a launch, and
+// by all of the row's chunks or by none.
 __device__ __forceinline__ bool last_chunk(uint32_t *done, uint32_t chunks)
 {
     __shared__ bool last;
@@ -770,6 +771,9 @@ __device__ __forceinline__ bool last_chunk(uint32_t *done, uint32_t chunks)
     __syncthreads();
     return last;
 }
+
+// How a chunk left a launch: without having counted itself for its row, or counted, as the last or not.
+enum Left : int { kUncounted, kCounted, kCountedLast };
 
 // The vectors of one chunk of the row, then (last chunk) the values after the last whole vector.
 template <typename S> struct Chunk {
@@ -1008,13 +1012,13 @@ template <typename T> __device__ __forceinline__ ChunkPart<T> row_part(const Spl
 // The lowest finite value.
 template <typename T> __device__ __forceinline__ T lowest() { return sizeof(T) == 8 ? (T)-1.7976931348623157e308 : (T)-3.402823466e38f; }
 
-template <typename S> __device__ __forceinline__ bool sample_first(const SplitArgs<typename StatOf<S>::T> &a)
+template <typename S> __device__ __forceinline__ Left sample_first(const SplitArgs<typename StatOf<S>::T> &a)
 {
     using T = typename StatOf<S>::T;
     using K = typename KeyOf<T>::K;
     constexpr int NT = kChunkThreads;
     if (block_gate_closed(a.g.gate))
-        return blockIdx.x % a.chunks == 0;
+        return kUncounted;
     __shared__ BoundScratch bound;
     __shared__ T red[4][16];
     __shared__ List<K, kChunkListCap> list;
@@ -1026,7 +1030,7 @@ template <typename S> __device__ __forceinline__ bool sample_first(const SplitAr
     if (kind == kRowNone) {
         if (chunk == 0 && threadIdx.x == 0)
             no_token(a.g, row, false);
-        return chunk == 0;
+        return kUncounted;
     }
     const Chunk<S> part(static_cast<const S *>(a.g.logits) + row * a.g.stride, n, chunk, a.chunks, a.chunk_vecs,
                         kind == kRowList || kind == kRowBound);
@@ -1056,29 +1060,29 @@ template <typename S> __device__ __forceinline__ bool sample_first(const SplitAr
         put(&a.part[blockIdx.x].t, t);
     }
     if (kind != kRowList)
-        return false;
+        return kUncounted;
     own = own > lowest<T>() ? own : lowest<T>(); // minus infinity is never drawn
     part.gather(list, largest, own);
     hand_over(a, row, list);
     if (!last_chunk(&a.state[row].done[0], a.chunks))
-        return false;
+        return kCounted;
     const T top = row_part(a, row).m;
     if (top == -INFINITY) {
         if (threadIdx.x == 0)
             no_token(a.g, row, true);
-        return true;
+        return kCountedLast;
     }
     draw_from_row<S>(a, row, set, top, list, bound, red[0], sh);
-    return true;
+    return kCountedLast;
 }
 
-template <typename S> __device__ __forceinline__ bool sample_weigh(const SplitArgs<typename StatOf<S>::T> &a)
+template <typename S> __device__ __forceinline__ Left sample_weigh(const SplitArgs<typename StatOf<S>::T> &a)
 {
     using T = typename StatOf<S>::T;
     using K = typename KeyOf<T>::K;
     constexpr int NT = kChunkThreads;
     if (block_gate_closed(a.g.gate))
-        return blockIdx.x % a.chunks == 0;
+        return kUncounted;
     __shared__ BoundScratch bound;
     __shared__ T red[4][16];
     __shared__ List<K, kChunkListCap> list;
@@ -1089,17 +1093,17 @@ template <typename S> __device__ __forceinline__ bool sample_weigh(const SplitAr
     const Settings set = settings_of(a.g, row);
     const uint32_t kind = kind_of(set, n, a.chunks);
     if (kind == kRowNone || kind == kRowList)
-        return chunk == 0;
+        return kUncounted;
     const auto [m, low] = row_part(a, row);
     const S *s = static_cast<const S *>(a.g.logits) + row * a.g.stride;
     if (m == -INFINITY || kind == kRowSearch) {
         if (chunk != 0)
-            return false;
+            return kUncounted;
         if (m > -INFINITY)
             draw_by_search<S, NT>(a.g, row, s, set, m, sh);
         else if (threadIdx.x == 0)
             no_token(a.g, row, true);
-        return true;
+        return kUncounted;
     }
     const Chunk<S> part(s, n, chunk, a.chunks, a.chunk_vecs, kind == kRowBound);
     const Weight<T> weight{m, set.inv};
@@ -1108,9 +1112,9 @@ template <typename S> __device__ __forceinline__ bool sample_weigh(const SplitAr
         part.gather(list, [&](T v) { return v >= t; });
         hand_over(a, row, list);
         if (!last_chunk(&a.state[row].done[1], a.chunks))
-            return false;
+            return kCounted;
         draw_from_row<S>(a, row, set, m, list, bound, red[0], sh);
-        return true;
+        return kCountedLast;
     }
     if (kind == kRowPlain) {
         auto mass_of = [&](T v, uint32_t) -> mass_t {
@@ -1126,12 +1130,12 @@ template <typename S> __device__ __forceinline__ bool sample_weigh(const SplitAr
         if (threadIdx.x == 0)
             put(&a.chunk_mass[blockIdx.x], own);
         if (!last_chunk(&a.state[row].done[1], a.chunks))
-            return false;
+            return kCounted;
         if (threadIdx.x < a.chunks)
             in_chunk[threadIdx.x] = get(&a.chunk_mass[row * a.chunks + threadIdx.x]);
         __syncthreads();
         draw_in_chunk<S>(a, row, set, in_chunk, mass_of, sh.tiles);
-        return true;
+        return kCountedLast;
     }
     for (uint32_t b = threadIdx.x; b < kSteps; b += NT)
         sh.steps[b] = 0;
@@ -1145,7 +1149,7 @@ template <typename S> __device__ __forceinline__ bool sample_weigh(const SplitAr
     for (uint32_t b = threadIdx.x; b < kSteps; b += NT)
         put(&a.steps[(uint64_t)blockIdx.x * kSteps + b], sh.steps[b]);
     if (!last_chunk(&a.state[row].done[1], a.chunks))
-        return false;
+        return kCounted;
     // The step in which the nucleus ends, from the sums of the chunks' steps; 16 loads in flight.
     const mass_t *steps = a.steps + row * a.chunks * kSteps;
     constexpr uint32_t E = kSteps / NT, U = 4;
@@ -1173,17 +1177,17 @@ template <typename S> __device__ __forceinline__ bool sample_weigh(const SplitAr
         a.state[row].above = end.above;
         a.state[row].step = end.step;
     }
-    return false;
+    return kCountedLast;
 }
 
-template <typename S> __device__ __forceinline__ bool sample_edge(const SplitArgs<typename StatOf<S>::T> &a)
+template <typename S> __device__ __forceinline__ Left sample_edge(const SplitArgs<typename StatOf<S>::T> &a)
 {
     using T = typename StatOf<S>::T;
     using K = typename KeyOf<T>::K;
     constexpr int NT = kChunkThreads;
     constexpr uint32_t N = kVec<S>;
     if (block_gate_closed(a.g.gate))
-        return blockIdx.x % a.chunks == 0;
+        return kUncounted;
     __shared__ BoundScratch bound;
     __shared__ T red[4][16];
     __shared__ List<K, kEdgeListCap> list;
@@ -1193,10 +1197,10 @@ template <typename S> __device__ __forceinline__ bool sample_edge(const SplitArg
     const uint32_t chunk = blockIdx.x % a.chunks, n = a.g.vocab;
     const Settings set = settings_of(a.g, row);
     if (kind_of(set, n, a.chunks) != kRowNucleus)
-        return chunk == 0;
+        return kUncounted;
     const auto [m, low] = row_part(a, row);
     if (m == -INFINITY)
-        return chunk == 0;
+        return kUncounted;
     const S *s = static_cast<const S *>(a.g.logits) + row * a.g.stride;
     const Chunk<S> part(s, n, chunk, a.chunks, a.chunk_vecs, false);
     const StepOf<T> step_of(m, set.inv, low);
@@ -1226,11 +1230,11 @@ template <typename S> __device__ __forceinline__ bool sample_edge(const SplitArg
     __syncthreads();
     hand_over(a, row, list);
     if (!last_chunk(&a.state[row].done[2], a.chunks))
-        return false;
+        return kCounted;
     const uint32_t count = take_list(a, row, kRowCap, m, list, bound, red[0]);
     if (count > kRowCap) {
         draw_by_search<S, NT>(a.g, row, s, set, m, sh);
-        return true;
+        return kCountedLast;
     }
     if (threadIdx.x < a.chunks)
         in_chunk[threadIdx.x] = get(&a.chunk_mass[row * a.chunks + threadIdx.x]);
@@ -1259,15 +1263,20 @@ template <typename S> __device__ __forceinline__ bool sample_edge(const SplitArg
                          return w >= set.least ? w : 0;
                      },
                      sh.tiles);
-    return true;
+    return kCountedLast;
 }
 
-// The end of the program by a call's last launch (close): of each row one workgroup, the one that
-// finished it or, of rows finished by earlier launches, its first, takes a ticket; the last of
-// them ends the program. All of the rows' other workgroups have finished before it.
-template <typename T> __device__ __forceinline__ void close_rows(const SplitArgs<T> &a, const ProgramClose &c, bool finisher)
+// The end of the program by a call's last launch (close), number `launch` of it: every workgroup counts
+// itself once for its row, here where its way through the launch did not; the last of a row takes
+// the row's ticket, and the last ticket ends the program. So no workgroup is left that reads the call's
+// arrays once the caller may write them again: a chunk of a row that an earlier launch finished, or
+// that another chunk draws from alone, still reads the row's settings, however late it starts.
+template <typename T>
+__device__ __forceinline__ void close_rows(const SplitArgs<T> &a, const ProgramClose &c, int launch, Left left)
 {
-    if (c.words == nullptr || !finisher)
+    if (c.words == nullptr || left == kCounted)
+        return;
+    if (left == kUncounted && !last_chunk(&a.state[blockIdx.x / a.chunks].done[launch], a.chunks))
         return;
     __shared__ int last;
     __builtin_amdgcn_s_waitcnt(0);
@@ -1285,15 +1294,15 @@ template <typename T> __device__ __forceinline__ void close_rows(const SplitArgs
 
 template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_first(SplitArgs<typename StatOf<S>::T> a, ProgramClose close)
 {
-    close_rows(a, close, sample_first<S>(a));
+    close_rows(a, close, 0, sample_first<S>(a));
 }
 template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_weigh(SplitArgs<typename StatOf<S>::T> a, ProgramClose close)
 {
-    close_rows(a, close, sample_weigh<S>(a));
+    close_rows(a, close, 1, sample_weigh<S>(a));
 }
 template <typename S> __global__ __launch_bounds__(kChunkThreads) void k_sample_edge(SplitArgs<typename StatOf<S>::T> a, ProgramClose close)
 {
-    close_rows(a, close, sample_edge<S>(a));
+    close_rows(a, close, 2, sample_edge<S>(a));
 }
 
 // ------------------------------------------------------------------------- launches

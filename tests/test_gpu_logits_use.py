@@ -225,3 +225,41 @@ def test_rows_without_logits(ctx):
     assert np.all(np.isneginf(values.numpy())) and np.all(indices.numpy() == -1) and np.all(np.isneginf(log_sum.numpy()))
     tokens, log_prob = ctx.native_sample(x, ctx.upload(np.zeros(5, np.float32)), vocab=0)
     assert np.all(tokens.numpy() == -1) and np.all(np.isneginf(log_prob.numpy()))
+
+
+def test_settings_may_change_as_soon_as_a_call_is_back(ctx, pcu_pkg):
+    """Small calls end their program in their last launch. The caller then writes the next settings
+    from another stream, while a third keeps the chip's units busy, so that workgroups start late: the
+    calls' tokens are those of calls that nothing disturbs. Settings change every row's way through the
+    launches: the largest logit alone, top-k in one launch and in two, beyond any list, no truncation, a
+    nucleus, rows without a logit."""
+    rng = np.random.default_rng(21)
+    rows, vocab = 64, 20001
+    x = rng.normal(0, 2, (rows, vocab)).astype(np.float32)
+    x[5] = -np.inf
+    x, u = ctx.upload(x), ctx.upload(rng.random(rows).astype(np.float32))
+    ones, none = np.ones(rows, np.float32), np.zeros(rows, np.int32)
+    mixed = {n: a.numpy() for n, a in _mixed(ctx, rng, rows).items()}
+    nucleus = dict(temperature=ones, top_k=none, top_p=0.9 * ones, min_p=0 * ones)
+    ways = [dict(nucleus, top_p=ones), nucleus, mixed, dict(nucleus, temperature=0 * ones), nucleus,
+            dict(nucleus, top_k=none + 20, top_p=ones), nucleus, dict(nucleus, top_k=none + 900), mixed,
+            dict(nucleus, top_k=none + 3000, top_p=ones), nucleus]
+    want = [[a.numpy() for a in ctx.native_sample(x, u, **{n: ctx.upload(a) for n, a in w.items()})] for w in ways]
+    with pcu_pkg.Context(0) as writer, pcu_pkg.Context(0) as busy:
+        settings = {n: ctx.upload(a) for n, a in ways[0].items()}
+        theirs = {n: pcu_pkg.DeviceArray(writer, a.ptr, a.shape, a.dtype) for n, a in settings.items()}
+        tokens, log_prob = ctx.empty((rows,), np.int32), ctx.empty((rows,), np.float32)
+        a = busy.upload(rng.normal(0, 1, (2048, 2048)).astype(np.float32))
+        out = busy.empty((2048, 2048), np.float32)
+        for _ in range(4):
+            with busy.program():
+                for _ in range(40):
+                    busy.native_matmul(a, a, out=out)
+                for w, way in enumerate(ways):
+                    for n in theirs:
+                        writer.upload_into(theirs[n], way[n])
+                    ctx.native_sample(x, u, **settings, tokens=tokens, log_prob=log_prob)
+                    for n in theirs:
+                        writer.upload_into(theirs[n], ways[(w + 1) % len(ways)][n])
+                    np.testing.assert_array_equal(tokens.numpy(), want[w][0])
+                    np.testing.assert_array_equal(log_prob.numpy(), want[w][1])
