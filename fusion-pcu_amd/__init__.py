@@ -13,6 +13,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import enum
+import operator
 from dataclasses import dataclass
 from typing import Optional, Sequence, Tuple
 
@@ -608,6 +609,9 @@ class Context:
             if isinstance(x, DeviceArray):
                 _need(name, x, (rows,), _INT32 if name == "top_k" else _FLOAT32)
                 setattr(p, name, x.ptr)
+            elif name == "top_k":  # past 31 bits every number sets no limit, as 0 does
+                x = operator.index(x)
+                p.top_k_value = x if 0 < x < 1 << 31 else 0
             else:
                 setattr(p, name + "_value", x)
         tokens = self._out("tokens", tokens, (rows,), _INT32)

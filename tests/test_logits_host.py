@@ -59,3 +59,26 @@ def test_a_null_context_is_refused(pcu_pkg):
     assert lib.pcu_native_distill_backward(None, lg_p, d_p, None, None, None, 0, 0, None) == _abi.PCU_ERR_ARGUMENT
     assert lib.pcu_native_distill_step(None, lg_p, d_p, None, None, None, 0, 0, None) == _abi.PCU_ERR_ARGUMENT
     assert lib.pcu_native_sample(None, lg_p, p_p, None, None, None) == _abi.PCU_ERR_ARGUMENT
+
+
+@pytest.mark.parametrize("top_k,passed", [(5, 5), (0, 0), (-3, -1), (2 ** 31 - 1, 2 ** 31 - 1), (2 ** 31, 0),
+                                          (2 ** 32 + 5, 0), (-2 ** 32 + 7, 0), (np.int64(2 ** 40), 0), (np.int32(7), 7)])
+def test_a_top_k_beyond_32_bits_sets_no_limit(pcu_pkg, top_k, passed):
+    """The C ABI takes 32 bits; a larger number is no limit (0), not what its low bits say."""
+    from fusion_pcu_amd import _abi
+    seen = []
+
+    class Lib:
+        def pcu_native_sample(self, handle, logits, sampling, tokens, log_prob, fault):
+            seen.append(sampling._obj.top_k_value)
+            return _abi.PCU_OK
+
+    ctx = pcu_pkg.Context.__new__(pcu_pkg.Context)
+    ctx.handle, ctx._lib = None, Lib()
+    array = lambda shape, dtype: pcu_pkg.DeviceArray(ctx, 4096, shape, dtype)
+    ctx.native_sample(array((2, 9), np.float32), array((2,), np.float32), top_k=top_k,
+                      tokens=array((2,), np.int32), log_prob=array((2,), np.float32))
+    assert seen[0] == passed or (seen[0] <= 0 and passed <= 0)
+    with pytest.raises(TypeError):
+        ctx.native_sample(array((2, 9), np.float32), array((2,), np.float32), top_k=2.5,
+                          tokens=array((2,), np.int32), log_prob=array((2,), np.float32))
