@@ -40,6 +40,25 @@ static pcu_status check_logits(Ctx *c, const char *what, const pcu_logits *l)
     return PCU_OK;
 }
 
+// Whether the kernels can work with a temperature: it and what they make of it have to be numbers in
+// the statistics' type (the exponent's factor is log2(e) / T; a loss takes the square, in binary64).
+static bool valid_temperature(uint32_t dtype, double temperature, bool squared)
+{
+    if (!(temperature > 0) || !std::isfinite(temperature))
+        return false;
+    if (dtype == PCU_F64)
+        return std::isfinite(1.0 / temperature) &&
+               (!squared || (temperature * temperature > 0 && std::isfinite(temperature * temperature)));
+    const float t = (float)temperature;
+    return t > 0 && std::isfinite(t) && std::isfinite(1.0f / t * (float)M_LOG2E);
+}
+
+// A weight that is a number in the statistics' type.
+static bool valid_weight(uint32_t dtype, double weight)
+{
+    return dtype == PCU_F64 ? std::isfinite(weight) : std::isfinite((float)weight);
+}
+
 // An output against one input.
 struct Range {
     const void *p;
@@ -63,7 +82,7 @@ pcu_status Ctx::op_top_logits(const pcu_logits *l, uint32_t k, double temperatur
         fail("top_logits: k %u is beyond %u", k, PCU_LOGITS_MAX_K);
         return PCU_ERR_SHAPE;
     }
-    if ((l->rows && k && (!values || !indices)) || !(temperature > 0) || !std::isfinite(temperature)) {
+    if ((l->rows && k && (!values || !indices)) || !valid_temperature(l->dtype, temperature, false)) {
         fail("top_logits: invalid argument");
         return PCU_ERR_ARGUMENT;
     }
@@ -113,8 +132,9 @@ pcu_status Ctx::op_distill(Distill mode, const pcu_logits *l, const pcu_distill 
     if (st)
         return st;
     if (!d || d->teacher_dtype > PCU_F16 ||
-        (l->rows && d->k && (!d->teacher_values || !d->teacher_indices)) || !(d->temperature > 0) ||
-        !std::isfinite(d->temperature) || !std::isfinite(d->distill_weight) || !std::isfinite(d->label_weight) ||
+        (l->rows && d->k && (!d->teacher_values || !d->teacher_indices)) ||
+        !valid_temperature(l->dtype, d->temperature, mode != Distill::Backward) ||
+        !valid_weight(l->dtype, d->distill_weight) || !valid_weight(l->dtype, d->label_weight) ||
         (l->rows && mode != Distill::Backward && !loss) || (l->rows && mode == Distill::Backward && !log_sums_in) ||
         (l->rows && grad_cols && mode != Distill::Loss && !grad)) {
         fail("distill: invalid argument");

@@ -175,8 +175,9 @@ __device__ __forceinline__ T row_loss(const DistillArgs &g, const Entries<T> &e,
     part = block_reduce<NT>(part, OpSum(), red);
     hard = block_reduce<NT>(hard, OpSum(), red + 16);
     T loss = 0;
+    // In binary64: the square of a temperature leaves binary32's range before the loss does.
     if (g.distill_weight != 0 && !(e.sum == 0))
-        loss += (T)g.distill_weight * (t * t) * part;
+        loss += (T)(g.distill_weight * ((double)t * t) * part);
     if (g.label_weight != 0 && e.label >= 0)
         loss += (T)g.label_weight * hard;
     return loss;

@@ -258,7 +258,9 @@ typedef struct pcu_logits {
  * and NaN after minus infinity. values: rows x k of the logits' type; indices: rows x k;
  * places past the vocabulary hold minus infinity and -1. log_sum (or NULL): the row's
  * log(sum exp(l / temperature)), F32 (F64 for F64 logits); minus infinity for a row of minus
- * infinities, NaN for a row that holds a NaN or plus infinity. temperature > 0. */
+ * infinities, NaN for a row that holds a NaN or plus infinity. temperature: a positive number that, as
+ * its reciprocal times log2(e), is finite in F32 (F64 for F64 logits); 2^-127 to 2^127 are. Where
+ * l / temperature of the largest logit leaves that type, log_sum is infinite. */
 pcu_status pcu_native_top_logits(pcu_ctx *ctx, const pcu_logits *logits, uint32_t k,
                                  double temperature, void *values, int32_t *indices,
                                  void *log_sum);
@@ -282,8 +284,9 @@ typedef struct pcu_distill {
     const int32_t *labels;          /* rows; or NULL */
     uint32_t teacher_dtype;         /* pcu_dtype */
     uint32_t k;                     /* 0 .. PCU_LOGITS_MAX_K */
-    double temperature;             /* > 0 */
-    double distill_weight, label_weight;
+    double temperature;             /* as above; for a loss of F64 logits its square is finite too, and not 0.
+                                     * Values divided by it have to stay in the type, or be minus infinity */
+    double distill_weight, label_weight; /* finite in F32 (F64 for F64 logits) */
 } pcu_distill;
 
 /* loss: rows; log_sums (or NULL): rows x 2, the student's log-sum-exp of s / T and of s. Both

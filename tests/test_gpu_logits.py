@@ -695,3 +695,98 @@ def test_rows_past_two_to_the_thirty_one_elements(ctx, pcu_pkg):
     assert np.all(err <= 16 * rel + OUT_U["f16"] * np.abs(want[2]) * 1.01 + LEAST["f16"])
     np.testing.assert_array_equal(got[:, vocab:], a[:, vocab:])  # the columns between are the caller's
     buf.free()
+
+
+# ----------------------------------------------------------- the range of a temperature
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_temperatures_without_a_number_for_them_are_refused(ctx, pcu_pkg, dtype):
+    """Beyond the range in which the temperature, log2(e) / T and a loss's T^2 are numbers of the
+    statistics' type."""
+    a, _ = _stored(pcu_pkg, np.array([[0.0, -1.0, -np.inf, -2.0]]), dtype)
+    s = ctx.upload(a)
+    tv, ti = ctx.upload(np.zeros((1, 2), np.float32)), ctx.upload(np.array([[0, 1]], np.int32))
+    sums = ctx.upload(np.zeros((1, 2), np.float64 if dtype == "f64" else np.float32))
+    step = lambda **kw: ctx.native_distill_step(s, tv, ti, **kw)
+    loss = lambda **kw: ctx.native_distill_loss(s, tv, ti, **kw)
+    backward = lambda **kw: ctx.native_distill_backward(s, tv, ti, sums, **kw)
+    top = lambda **kw: ctx.native_top_logits(s, 2, **kw)
+
+    def refused(call, **kw):
+        with pytest.raises(pcu_pkg.PcuExecutionError) as e:
+            call(**kw)
+        assert e.value.status == 2
+
+    for t in ((1e-310, 5e-324) if dtype == "f64" else (4e-39, 1e-40, 1e-60, 3.5e38, 1e200)):
+        for call in (step, loss, backward, top):
+            refused(call, temperature=t)
+    if dtype == "f64":
+        for t in (1e-200, 1e200):  # the square
+            refused(step, temperature=t)
+            refused(loss, temperature=t)
+            backward(temperature=t)
+            top(temperature=t)
+    else:
+        for name in ("distill_weight", "label_weight"):
+            for call in (step, loss, backward):
+                refused(call, **{name: 1e39})
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab", [(3, 700), (70, 9001), (3, 140001)])
+def test_temperatures_at_the_ends_of_the_range(ctx, pcu_pkg, rows, vocab, dtype):
+    """Logits of 0, -1 and masked ones, and powers of two as temperatures: everything below is exact but
+    for the large temperature's log-sum-exps and probabilities, which carry the tolerance of any other."""
+    rng = np.random.default_rng(vocab)
+    stat = np.float64 if dtype == "f64" else np.float32
+    x = np.where(rng.random((rows, vocab)) < 0.3, -np.inf, -1.0)
+    best = rng.integers(0, vocab - 2, rows)
+    x[np.arange(rows), best] = 0.0
+    x[:, vocab - 2:] = -1.0
+    a, x = _stored(pcu_pkg, x, dtype)
+    s = ctx.upload(a)
+    # The teacher's choice is the last logit, 1 below the student's.
+    ti = np.tile(np.array([[vocab - 2, vocab - 1]], np.int32), (rows, 1))
+    tv = np.tile(np.array([[-1.0, 0.0]], stat), (rows, 1))
+    tv_d, ti_d = ctx.upload(tv), ctx.upload(ti)
+    for t in ((2.0 ** -500, 2.0 ** -40) if dtype == "f64" else (2.0 ** -127, 2.0 ** -100, 2.0 ** -40)):
+        # All mass lies on the largest: q and p are 0 or 1, loss T^2 / T, gradient -T and T.
+        values, indices, log_sum = ctx.native_top_logits(s, 1, temperature=t)
+        assert np.array_equal(indices.numpy()[:, 0], best) and np.all(log_sum.numpy() == 0)
+        loss, grad = ctx.native_distill_step(s, tv_d, ti_d, temperature=t)
+        loss2, sums = ctx.native_distill_loss(s, tv_d, ti_d, temperature=t)
+        back = ctx.native_distill_backward(s, tv_d, ti_d, sums, temperature=t)
+        want = np.zeros((rows, vocab))
+        want[np.arange(rows), best] = t
+        want[:, vocab - 1] = -t
+        want = _stored(pcu_pkg, want, dtype)[1]
+        assert np.all(sums.numpy()[:, 0] == 0)
+        assert np.all(loss.numpy() == t) and np.all(loss2.numpy() == t)
+        for g in (grad, back):
+            np.testing.assert_array_equal(_values(pcu_pkg, g.numpy(), dtype), want)
+    t = 2.0 ** 127
+    n = np.sum(~np.isneginf(x), axis=1)
+    rel = _relative(dtype, vocab, np.array([1.0]))
+    assert np.max(np.abs(ctx.native_top_logits(s, 1, temperature=t)[2].numpy() - np.log(n))) <= rel
+    loss, sums = ctx.native_distill_loss(s, tv_d, ti_d, temperature=t)
+    assert np.max(np.abs(sums.numpy()[:, 0] - np.log(n))) <= rel
+    # T^2 (log(n / 2)) is past binary32, and a number in binary64.
+    want = t * t * np.log(n / 2)
+    if dtype == "f64":
+        assert np.all(np.abs(loss.numpy() - want) <= 4 * rel * t * t * (2 + np.log(n)))
+    else:
+        assert np.all(np.isposinf(loss.numpy()))
+    # Small enough a weight brings the loss, and 2^-127 the gradient's factor, back.
+    weight = 2.0 ** -140 if dtype != "f64" else 2.0 ** -127
+    loss, grad = ctx.native_distill_step(s, tv_d, ti_d, temperature=t, distill_weight=weight)
+    assert np.all(np.abs(loss.numpy() - weight * want) <= (4 * rel + _u(dtype)) * weight * t * t * (2 + np.log(n)))
+    loss, sums = ctx.native_distill_loss(s, tv_d, ti_d, temperature=t)
+    back = ctx.native_distill_backward(s, tv_d, ti_d, sums, temperature=t, distill_weight=2.0 ** -126)
+    _, grad = ctx.native_distill_step(s, tv_d, ti_d, temperature=t, distill_weight=2.0 ** -126)
+    want = np.where(np.isneginf(x), 0.0, 1.0 / n[:, None])
+    want[:, vocab - 2:] -= 0.5
+    for g in (grad, back):
+        got = _values(pcu_pkg, g.numpy(), dtype) / 2
+        assert np.all(np.abs(got - want) <= 4 * rel * (np.abs(want) + 1.0 / n[:, None]) + OUT_U[dtype] * np.abs(want) * 1.01
+                      + LEAST[dtype])
