@@ -12,6 +12,9 @@ static_assert(kLogitF32 == PCU_F32 && kLogitF64 == PCU_F64 && kLogitBf16 == PCU_
 static uint64_t logit_size(uint32_t dtype) { return dtype == PCU_F64 ? 8 : dtype == PCU_F32 ? 4 : 2; }
 static uint64_t stat_size(uint32_t dtype) { return dtype == PCU_F64 ? 8 : 4; }
 
+// A pointer to values of `size` bytes: the kernels load and store them whole (null passes).
+static bool aligned(const void *p, uint64_t size) { return ((uintptr_t)p & (size - 1)) == 0; }
+
 // Bytes from the first element of `rows` strided rows of `cols` to past the last one.
 static uint64_t strided_bytes(uint64_t rows, uint64_t cols, uint64_t stride, uint64_t size)
 {
@@ -27,7 +30,7 @@ static pcu_status check_logits(Ctx *c, const char *what, const pcu_logits *l)
 {
     constexpr uint64_t kMaxStride = (uint64_t)PCU_LOGITS_MAX_VOCAB << 8;
     if (!l || l->dtype > PCU_F16 || (l->rows && l->vocab && !l->data) ||
-        ((uintptr_t)l->data & (logit_size(l->dtype) - 1))) {
+        !aligned(l->data, logit_size(l->dtype))) {
         c->fail("%s: invalid logits", what);
         return PCU_ERR_ARGUMENT;
     }
@@ -84,6 +87,10 @@ pcu_status Ctx::op_top_logits(const pcu_logits *l, uint32_t k, double temperatur
     }
     if ((l->rows && k && (!values || !indices)) || !valid_temperature(l->dtype, temperature, false)) {
         fail("top_logits: invalid argument");
+        return PCU_ERR_ARGUMENT;
+    }
+    if (!aligned(values, logit_size(l->dtype)) || !aligned(indices, 4) || !aligned(log_sum, stat_size(l->dtype))) {
+        fail("top_logits: an output is not aligned to its type");
         return PCU_ERR_ARGUMENT;
     }
     const Range in{l->data, logits_bytes(*l)};
@@ -147,10 +154,16 @@ pcu_status Ctx::op_distill(Distill mode, const pcu_logits *l, const pcu_distill 
     const uint64_t size = logit_size(l->dtype), stat = stat_size(l->dtype);
     if (mode != Distill::Loss &&
         (grad_cols < l->vocab || grad_stride < grad_cols || grad_stride > ((uint64_t)PCU_LOGITS_MAX_VOCAB << 8) ||
-         grad_cols - l->vocab > PCU_LOGITS_MAX_VOCAB || ((uintptr_t)grad & (size - 1)))) {
+         grad_cols - l->vocab > PCU_LOGITS_MAX_VOCAB || !aligned(grad, size))) {
         fail("distill: a gradient of %llu columns, stride %llu, for %llu logits", (unsigned long long)grad_cols,
              (unsigned long long)grad_stride, (unsigned long long)l->vocab);
         return PCU_ERR_SHAPE;
+    }
+    if (!aligned(d->teacher_values, logit_size(d->teacher_dtype)) || !aligned(d->teacher_indices, 4) ||
+        !aligned(d->teacher_log_sum, stat_size(d->teacher_dtype)) || !aligned(d->labels, 4) || !aligned(row_scale, stat) ||
+        !aligned(log_sums_in, stat) || !aligned(loss, stat) || !aligned(log_sums_out, stat)) {
+        fail("distill: a tensor is not aligned to its type");
+        return PCU_ERR_ARGUMENT;
     }
     const Range student{l->data, logits_bytes(*l)};
     const Range values{d->teacher_values, l->rows * d->k * logit_size(d->teacher_dtype)},
@@ -224,6 +237,12 @@ pcu_status Ctx::op_sample(const pcu_logits *l, const pcu_sampling *p, int32_t *t
         fail("sample: invalid argument");
         return PCU_ERR_ARGUMENT;
     }
+    for (const void *x : {(const void *)p->uniform, (const void *)p->temperature, (const void *)p->top_k,
+                          (const void *)p->top_p, (const void *)p->min_p, (const void *)tokens, (const void *)log_prob})
+        if (!aligned(x, 4)) {
+            fail("sample: a tensor is not aligned to its type");
+            return PCU_ERR_ARGUMENT;
+        }
     const uint64_t b = l->rows * 4;
     const Range logits{l->data, logits_bytes(*l)}, u{p->uniform, b}, t{p->temperature, b}, tk{p->top_k, b},
         tp{p->top_p, b}, mp{p->min_p, b}, out{tokens, b}, lp{log_prob, b};

@@ -238,9 +238,10 @@ pcu_status pcu_native_sgd(pcu_ctx *ctx, pcu_dtype dtype, uint64_t n, const void 
 /* ----------------------------------------------------------- operators on logits
  * No counterpart in the reference: what a language model does with its output layer's
  * logits. Native arithmetic (non-finite results are ordinary values), each call one program
- * node, rows independent of each other. `fault` reports what only the device can see, an index or
- * a setting out of its range, as PCU_FAULT_INVALID with the lowest such element (named at
- * each call); the outputs of the other rows are then unspecified. */
+ * node, rows independent of each other. A pointer that is not aligned to its type is
+ * refused. `fault` reports what only the device can see, an index or a setting out of its
+ * range, as PCU_FAULT_INVALID with the lowest such element (named at each call); the outputs
+ * of the other rows are then unspecified. */
 
 /* `rows` rows of `vocab` values of any dtype; row r starts at element r * stride
  * (stride >= vocab: the columns between belong to the caller). Any alignment of the type. */

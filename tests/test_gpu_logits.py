@@ -790,3 +790,50 @@ def test_temperatures_at_the_ends_of_the_range(ctx, pcu_pkg, rows, vocab, dtype)
         got = _values(pcu_pkg, g.numpy(), dtype) / 2
         assert np.all(np.abs(got - want) <= 4 * rel * (np.abs(want) + 1.0 / n[:, None]) + OUT_U[dtype] * np.abs(want) * 1.01
                       + LEAST[dtype])
+
+
+def test_pointers_that_are_not_aligned_to_their_type_are_refused(ctx, pcu_pkg):
+    """Before any launch; each pointer of the C ABI in turn, off by half a value. Aligned ones pass."""
+    from fusion_pcu_amd import _abi
+    lib = pcu_pkg.lib()
+    f = lambda *shape: ctx.upload(np.zeros(shape, np.float64)).ptr
+    lg = lambda dtype: _abi.Logits(f(4, 50), dtype, 0, 2, 20, 20)
+
+    def each(call, pointers, off):
+        assert call(*pointers) == 0
+        for i in range(len(pointers)):
+            moved = list(pointers)
+            moved[i] += off[i]
+            assert call(*moved) == 2, i
+
+    for dtype, size, stat in ((_abi.PCU_F32, 4, 4), (_abi.PCU_F64, 8, 8), (_abi.PCU_BF16, 2, 4), (_abi.PCU_F16, 2, 4)):
+        x = lg(dtype)
+        each(lambda v, i, s: lib.pcu_native_top_logits(ctx.handle, ctypes.byref(x), 3, 1.0, v, i, s),
+             [f(8), f(8), f(8)], [size // 2, 2, stat // 2])
+
+        def distill(mode):
+            def call(tv, ti, tl, labels, scale, sums, loss, out):
+                d = _abi.Distill(tv, ti, tl, labels, dtype, 3, 1.0, 0.5, 0.5)
+                args = (ctx.handle, ctypes.byref(x), ctypes.byref(d))
+                if mode == "loss":
+                    return lib.pcu_native_distill_loss(*args, loss, out, None)
+                if mode == "backward":
+                    return lib.pcu_native_distill_backward(*args, sums, scale, f(8, 8), 20, 20, None)
+                return lib.pcu_native_distill_step(*args, scale, loss, f(8, 8), 20, 20, None)
+            return call
+
+        teacher, steps = [f(8), f(8), f(8), f(8)], [size // 2, 2, stat // 2, 2]
+        a, b, c = f(8), f(8), f(8)
+        one = stat // 2
+        each(lambda tv, ti, tl, y, loss, out: distill("loss")(tv, ti, tl, y, None, None, loss, out), teacher + [a, b],
+             steps + [one, one])
+        each(lambda tv, ti, tl, y, scale, sums: distill("backward")(tv, ti, tl, y, scale, sums, None, None), teacher + [a, b],
+             steps + [one, one])
+        each(lambda tv, ti, tl, y, scale, loss: distill("step")(tv, ti, tl, y, scale, None, loss, None), teacher + [a, c],
+             steps + [one, one])
+
+        def sample(u, t, tk, tp, mp, tokens, log_prob):
+            p = _abi.Sampling(u, t, tk, tp, mp, 1.0, 0, 1.0, 0.0)
+            return lib.pcu_native_sample(ctx.handle, ctypes.byref(x), ctypes.byref(p), tokens, log_prob, None)
+
+        each(sample, [f(8) for _ in range(7)], [2] * 7)
