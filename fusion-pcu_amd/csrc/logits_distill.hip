@@ -165,10 +165,12 @@ __device__ __forceinline__ T row_loss(const DistillArgs &g, const Entries<T> &e,
         if (e.at[j] < 0)
             continue;
         const T v = e.s[j];
+        // log p of a masked logit is minus infinity also where all are masked (not the difference of
+        // two infinities), but NaN in a row that has no log-sum-exp.
         if (j == g.k) {
-            hard = v == -INFINITY ? (T)INFINITY : lse1 - v;
+            hard = v == -INFINITY && lse1 == lse1 ? (T)INFINITY : lse1 - v;
         } else if (!(e.q[j] == 0)) {
-            const T log_p = v == -INFINITY ? v : v / t - lse;
+            const T log_p = v == -INFINITY && lse == lse ? v : v / t - lse;
             part += e.q[j] * (e.log_q[j] - log_p);
         }
     }

@@ -837,3 +837,28 @@ def test_pointers_that_are_not_aligned_to_their_type_are_refused(ctx, pcu_pkg):
             return lib.pcu_native_sample(ctx.handle, ctypes.byref(x), ctypes.byref(p), tokens, log_prob, None)
 
         each(sample, [f(8) for _ in range(7)], [2] * 7)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [50, 9000, 150000])
+def test_a_masked_entry_of_a_row_with_nan_has_no_probability_either(ctx, pcu_pkg, vocab, dtype):
+    """log p of a row that holds a NaN or plus infinity is NaN everywhere, at a masked entry or label as
+    at any other; in a row of masked logits alone it is minus infinity."""
+    s = np.zeros((6, vocab))
+    s[:, [3, 4]] = -np.inf
+    s[[0, 3], 7] = np.nan
+    s[[1, 4], 9] = np.inf
+    s[[2, 5]] = -np.inf
+    s = ctx.upload(_stored(pcu_pkg, s, dtype)[0])
+    tv = ctx.upload(np.zeros((6, 1), np.float32))
+    ti = np.full((6, 1), -1, np.int32)
+    labels = np.full(6, -1, np.int32)
+    ti[:3], labels[3:] = 3, 4  # rows of an entry alone, rows of a label alone
+    args = (s, tv, ctx.upload(ti))
+    kw = dict(labels=ctx.upload(labels), distill_weight=0.5, label_weight=0.5, temperature=2.0)
+    loss, grad = ctx.native_distill_step(*args, **kw)
+    for x in (loss, ctx.native_distill_loss(*args, **kw)[0]):
+        x = x.numpy()
+        assert np.all(np.isnan(x[[0, 1, 3, 4]])) and np.all(np.isposinf(x[[2, 5]]))
+    got = _values(pcu_pkg, grad.numpy(), dtype)
+    assert np.all(np.isnan(got[[0, 1, 3, 4]])) and not np.any(np.isnan(got[[2, 5]]))
