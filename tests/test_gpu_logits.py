@@ -862,3 +862,73 @@ def test_a_masked_entry_of_a_row_with_nan_has_no_probability_either(ctx, pcu_pkg
         assert np.all(np.isnan(x[[0, 1, 3, 4]])) and np.all(np.isposinf(x[[2, 5]]))
     got = _values(pcu_pkg, grad.numpy(), dtype)
     assert np.all(np.isnan(got[[0, 1, 3, 4]])) and not np.any(np.isnan(got[[2, 5]]))
+
+
+# --------------------------------------------- settings that hold for every row of a call
+
+
+def _check_sample_of_all(ctx, pkg, x64, dtype, setting, u, names=None):
+    """Rows of x64 with one setting, given as numbers, against the definition."""
+    a, x = _stored(pkg, x64, dtype)
+    temperature, top_k, top_p, min_p = setting
+    u = np.asarray(u, np.float32)
+    tokens, log_prob = ctx.native_sample(ctx.upload(a), ctx.upload(u), temperature=temperature, top_k=top_k, top_p=top_p,
+                                         min_p=min_p)
+    tokens, log_prob = tokens.numpy(), log_prob.numpy()
+    for r in range(x.shape[0]):
+        want = _plain_sample(x[r], u[r], float(np.float32(temperature)), top_k, top_p, min_p, dtype)
+        where = (names[r] if names else r, setting, float(u[r]))
+        drawn = [t for t, _ in want]
+        assert min(drawn) <= tokens[r] <= max(drawn), where
+        near = [lp for t, lp in want if t == tokens[r]]
+        if near:
+            tol = 2.0 ** -20 * (1 + abs(near[0])) + 2.0 ** -40 * np.exp(-near[0])
+            assert np.isneginf(near[0]) and np.isneginf(log_prob[r]) or \
+                min(near) - tol <= log_prob[r] <= max(near) + tol, where
+
+
+# temperature, top_k, top_p, min_p. Long rows are done by the first launch where the chunks' lists of
+# top_k make the row's, by the second without a nucleus or with a longer list, by the third with one.
+ALL_ROWS = [(0.8, 50, 0.9, 0.0), (1.0, 5, 1.0, 0.0), (1.0, 1, 1.0, 0.0), (1.0, 0, 1.0, 0.05), (1.2, 0, 1.0, 0.0), (0.9, 0, 0.95, 0.0),
+            (1.0, 0, 0.9, 0.02), (1.0, 400, 1.0, 0.0), (0.7, 400, 0.8, 0.1), (1.0, 3000, 1.0, 0.0), (1.0, 3000, 0.9, 0.0),
+            (0.0, 0, 1.0, 0.0), (0.0, 0, 0.9, 0.0), (0.0, 50, 0.9, 0.1)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [9001, 70000])
+@pytest.mark.parametrize("copies", [1, 5])  # 16 rows end their program in the last launch, 80 do not
+def test_samples_with_one_setting_are_the_definitions(ctx, pcu_pkg, vocab, copies, dtype):
+    if copies > 1 and (vocab > 10000 or dtype in ("f64", "f16")):
+        pytest.skip("covered by the shorter rows of the other types")
+    rng = np.random.default_rng(vocab + copies)
+    rows = _hard_rows(vocab, rng)
+    names = list(rows) * copies
+    x = np.tile(np.stack(list(rows.values())), (copies, 1))
+    for setting in ALL_ROWS:
+        _check_sample_of_all(ctx, pcu_pkg, x, dtype, setting, rng.random(len(names)), names)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab", [(1, 50257), (3, 128000), (64, 9001)])
+def test_samples_of_ordinary_rows_with_one_setting(ctx, pcu_pkg, rows, vocab, dtype):
+    rng = np.random.default_rng(rows + vocab)
+    x = rng.normal(0, 2, (rows, vocab)) - 2 * np.log1p(rng.random((rows, vocab)) * vocab)
+    for setting in ALL_ROWS:
+        _check_sample_of_all(ctx, pcu_pkg, x, dtype, setting, rng.random(rows))
+
+
+@pytest.mark.parametrize("rows,vocab", [(4, 9001), (64, 9001), (4, 40001), (70, 9001)])
+def test_one_invalid_random_number_of_a_call(ctx, pcu_pkg, rows, vocab):
+    """The row is reported, however the call ends its program, and the next call is a clean one."""
+    rng = np.random.default_rng(rows)
+    x = ctx.upload(rng.normal(0, 2, (rows, vocab)).astype(np.float32))
+    u = rng.random(rows).astype(np.float32)
+    good = ctx.upload(u)
+    u[rows - 2] = 1.0
+    bad = ctx.upload(u)
+    for temperature, top_k, top_p, min_p in ALL_ROWS:
+        kw = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        want = [a.numpy() for a in ctx.native_sample(x, good, **kw)]
+        assert _fault(pcu_pkg, lambda: ctx.native_sample(x, bad, **kw)).element_index == rows - 2
+        for a, b in zip(ctx.native_sample(x, good, **kw), want):
+            np.testing.assert_array_equal(a.numpy(), b)
