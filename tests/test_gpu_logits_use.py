@@ -263,3 +263,76 @@ def test_settings_may_change_as_soon_as_a_call_is_back(ctx, pcu_pkg):
                         writer.upload_into(theirs[n], ways[(w + 1) % len(ways)][n])
                     np.testing.assert_array_equal(tokens.numpy(), want[w][0])
                     np.testing.assert_array_equal(log_prob.numpy(), want[w][1])
+
+
+def test_small_calls_results_are_there_for_any_stream(ctx, pcu_pkg):
+    """What a call that ends its own program returns is complete for a copy on another stream that
+    starts as soon as the call is back: each call's inputs and results differ from the last one's."""
+    rng = np.random.default_rng(31)
+    rows, vocab, k, calls = 48, 1000, 9, 30
+    inputs, want = [], []
+    for c in range(calls):
+        s, tv, ti, labels = _distill_args(ctx, rng, rows, vocab, k)
+        long = rng.normal(0, 2, (rows, 12 * vocab)).astype(np.float32)
+        inputs.append([ctx.upload(a) for a in (s, tv, ti, labels, rng.random(rows).astype(np.float32), long)])
+    out = {"loss": ctx.empty((rows,), np.float32), "gradient": ctx.empty((rows, vocab), np.float32),
+           "values": ctx.empty((rows, k), np.float32), "indices": ctx.empty((rows, k), np.int32),
+           "log_sum": ctx.empty((rows,), np.float32), "tokens": ctx.empty((rows,), np.int32),
+           "log_prob": ctx.empty((rows,), np.float32)}
+
+    def call(i, read):
+        s, tv, ti, labels, u, long = inputs[i]
+        got = []
+        ctx.native_distill_step(s, tv, ti, labels=labels, temperature=1.7, label_weight=0.4, loss=out["loss"],
+                                gradient=out["gradient"])
+        got += [read("gradient"), read("loss")]
+        ctx.native_top_logits(s, k, values=out["values"], indices=out["indices"], log_sum=out["log_sum"])
+        got += [read("values"), read("indices"), read("log_sum")]
+        for x in (s, long):
+            for kw in (dict(top_k=20), dict(top_p=0.9), dict(min_p=0.1), dict(temperature=0.0)):
+                ctx.native_sample(x, u, tokens=out["tokens"], log_prob=out["log_prob"], **kw)
+                got += [read("tokens"), read("log_prob")]
+        return got
+
+    for i in range(calls):
+        want.append(call(i, lambda name: out[name].numpy()))
+    with pcu_pkg.Context(0) as reader:
+        theirs = {n: pcu_pkg.DeviceArray(reader, a.ptr, a.shape, a.dtype) for n, a in out.items()}
+        for i in range(calls):
+            for a, b in zip(call(i, lambda name: theirs[name].numpy()), want[i]):
+                np.testing.assert_array_equal(a, b)
+
+
+def test_two_contexts_sample_at_the_same_time(ctx, pcu_pkg):
+    """Each context has its own counters and lists: programs of both, open at once, and calls from two
+    threads."""
+    import threading
+    rng = np.random.default_rng(33)
+    rows, vocab = 40, 30001
+    with pcu_pkg.Context(0) as other:
+        both = []
+        for c in (ctx, other):
+            x = c.upload(rng.normal(0, 2, (rows, vocab)).astype(np.float32))
+            u = c.upload(rng.random(rows).astype(np.float32))
+            settings = _mixed(c, rng, rows)
+            both.append((c, x, u, settings, c.native_sample(x, u, **settings)[0].numpy(),
+                         c.native_sample(x, u, top_k=30, top_p=0.9)[0].numpy()))
+        with ctx.program(), other.program():
+            drawn = [[c.native_sample(x, u, **settings)[0] for c, x, u, settings, _, _ in both] for _ in range(10)]
+        for pair in drawn:
+            for tokens, (_, _, _, _, want, _) in zip(pair, both):
+                np.testing.assert_array_equal(tokens.numpy(), want)
+        wrong = []
+
+        def work(c, x, u, settings, want, want_k):
+            for _ in range(50):
+                if not np.array_equal(c.native_sample(x, u, **settings)[0].numpy(), want) or \
+                   not np.array_equal(c.native_sample(x, u, top_k=30, top_p=0.9)[0].numpy(), want_k):
+                    wrong.append(c)
+
+        threads = [threading.Thread(target=work, args=a) for a in both]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not wrong
