@@ -15,9 +15,9 @@
 // order are involved and duplicate indices add up.
 //
 // What bounds it: one read of the logits and one write of the gradient. 4096 x 128000 bf16, loss and
-// gradient, takes 477 us of kernel (4.4 TB/s; a copy reaches 4.9), 1025 x 50257 f16, the gradient
-// alone, 45 us (4.6 TB/s), the loss alone of 512 x 32000 f32 18 us (3.7 TB/s); a few short rows
-// are a chain of loads, reductions and the program's end (64 x 1000 f64: 12.6 us).
+// gradient, takes 499 us of kernel (4.2 TB/s; a copy reaches 4.9), 1025 x 50257 f16, the gradient
+// alone, 47 us (4.4 TB/s), the loss alone of 512 x 32000 f32 19 us (3.4 TB/s); a few short rows
+// are a chain of loads, reductions and the program's end (64 x 1000 f64: 13 us). Medians of 32 calls.
 #include "pcu_kernels.hpp"
 #include "pcu_logits.hpp"
 
@@ -365,7 +365,7 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistillArgs g, ProgramClose 
 // Rows that no workgroup holds, and few rows of a long vocabulary: the statistics of chunks of
 // a row, with the logits at the entries; then per chunk the row's two log-sum-exps from all its
 // chunks and the gradient, the loss with the first (or, for the loss alone, one workgroup a row).
-// 16 x 200001 f32: 6 + 12 us of kernels, the second's reads out of the caches, 29.1 us a call; with a
+// 16 x 200001 f32: 6 + 13 us of kernels, the second's reads out of the caches, 29.3 us a call; with a
 // launch of its own between them for the loss and the log-sum-exps 32.6.
 template <typename T> struct Partial {
     T m, sum, sum1;

@@ -16,14 +16,15 @@ struct NodeGate {
 
 enum : int { kOpAdd = 0, kOpSub = 1, kOpMul = 2, kOpDiv = 3 };
 
-// The end of a program done by the launch of its last op (a MatMul or MSE that is the program's
-// only node, or a final SGD update) instead of a publication launch of its own: the n fault
-// words go to the coherent pinned mirror host_words and are reset to `value`, the stage gate is opened, and then the
-// sequence number `seq` is stored to host_seq (the host waits on it). `ticket` (zero between
-// launches) counts the workgroups or waves that have finished when the last of them must do
-// it. words == nullptr: no.
+// The end of a program done by the launch of its last op (a MatMul, MSE or operator on logits that is
+// the program's only node, or a final SGD update) instead of a publication launch of its own: the n
+// fault words go to the coherent pinned mirror host_words and are reset to `value`, the stage gate is
+// opened, and then the sequence number `seq` is stored to host_seq (the host waits on it). `ticket`
+// (zero between launches) counts the workgroups or waves that have finished when the last of
+// them must do it. words == nullptr: no.
 // A launch that ends the program takes one ticket per workgroup on a single counter; it
-// does so only with at most this many workgroups (else the tickets queue too long).
+// does so only with at most this many workgroups (else the tickets queue too long). A sample of rows
+// in chunks counts the workgroups of each row on a counter of the row first and takes one ticket a row.
 constexpr unsigned kCloseMaxBlocks = 64;
 struct ProgramClose {
     unsigned long long *words = nullptr;
@@ -288,7 +289,7 @@ hipError_t launch_native_mse(hipStream_t s, int dtype, uint64_t n, const void *p
 // `rows` rows of `vocab` logits, row r at element r * stride. Every limit below is checked by
 // the caller; indices that the inputs hold are checked by the kernels.
 enum : int { kLogitF32 = 0, kLogitF64 = 1, kLogitBf16 = 2, kLogitF16 = 3 };
-constexpr uint32_t kLogitMaxVocab = 1u << 22; // weights of 2^40 each add up below 2^62
+constexpr uint32_t kLogitMaxVocab = 1u << 22; // weights of 2^40 each add up to 2^62 at most
 constexpr uint32_t kLogitMaxK = 1024;
 // How a gradient is stored: plainly; past the caches; through them, in a kernel that ends its program.
 enum : int { kStorePlain = 0, kStorePast = 1, kStoreThrough = 2 };

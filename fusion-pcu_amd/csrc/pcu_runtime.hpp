@@ -59,8 +59,8 @@ struct Ctx {
     unsigned long long *host_words = nullptr;
     unsigned long long *host_seq = nullptr;
     uint64_t pub_seq = 0;
-    // The open program's end is done by its only node's last kernel (a MatMul: see
-    // ProgramClose) under this sequence number; 0: read_words launches the publication.
+    // The open program's end is done by its last op's last kernel (see ProgramClose) under this
+    // sequence number; 0: read_words launches the publication.
     uint64_t closed_seq = 0;
     bool in_program = false;
     bool implicit_program = false;
@@ -165,8 +165,8 @@ struct Ctx {
         c.ticket = ticket_word();
         return c;
     }
-    // The program's next op is its last: an SGD update (or pair) then ends the program in
-    // its own kernel when its grid is small (see op_sgd).
+    // The program's next op is its last: an SGD update (or pair) or an operator on logits then
+    // ends the program in its own kernel when its grid, or its rows, are few (see op_sgd).
     bool close_next = false;
     void close_with_next_op() { close_next = in_program; }
     pcu_status take_close(ProgramClose *c);
