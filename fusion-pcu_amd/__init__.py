@@ -618,3 +618,93 @@ class Context:
         log_prob = self._out("log_prob", log_prob, (rows,), _FLOAT32)
         self._call(self._lib.pcu_native_sample, ctypes.byref(lg), ctypes.byref(p), tokens.ptr, log_prob.ptr)
         return tokens, log_prob
+
+    # ----------------------------------- operators around a model's products
+    # Rows are [rows, columns] arrays of float32, float64, float16 or ``bfloat16``, tokens and labels
+    # int32 arrays. Results that are not passed in are allocated.
+    def _rows(self, what: str, x: DeviceArray) -> _abi.Rows:
+        code = _logit_code(what, x.dtype)
+        if len(x.shape) != 2:
+            raise PcuExecutionError(_abi.PCU_ERR_SHAPE, f"{what}: {x.shape} is no array of rows")
+        return _abi.Rows(x.ptr, code, 0, x.shape[0], x.shape[1], x.shape[1])
+
+    def native_embedding(self, table: DeviceArray, tokens: DeviceArray, scale: float = 1.0,
+                         out: Optional[DeviceArray] = None) -> DeviceArray:
+        """``scale`` times the table's row of each token, [tokens, width]; a negative token's row is
+        zeros (pcu_native_embedding)."""
+        rows = self._rows("embedding", table)
+        if len(tokens.shape) != 1:
+            raise PcuExecutionError(_abi.PCU_ERR_SHAPE, f"embedding: tokens are {tokens.shape}")
+        _need("tokens", tokens, tokens.shape, _INT32)
+        count, width = tokens.shape[0], table.shape[1]
+        out = self._out("out", out, (count, width), table.dtype)
+        self._call(self._lib.pcu_native_embedding, ctypes.byref(rows), tokens.ptr, count, scale, out.ptr, width)
+        return out
+
+    def native_embedding_backward(self, gradient: DeviceArray, tokens: DeviceArray, table_rows: int,
+                                  scale: float = 1.0, base: Optional[DeviceArray] = None,
+                                  out: Optional[DeviceArray] = None) -> DeviceArray:
+        """The gradient by a table of ``table_rows`` rows: ``base`` (default: zeros; it may be ``out``)
+        plus ``scale`` times the sum of each token's rows of ``gradient``, in their order
+        (pcu_native_embedding_backward)."""
+        rows = self._rows("embedding gradient", gradient)
+        count, width = gradient.shape
+        table_rows = operator.index(table_rows)
+        if not 0 <= table_rows <= _abi.TABLE_MAX_ROWS:
+            raise PcuExecutionError(_abi.PCU_ERR_SHAPE, f"embedding gradient: a table of {table_rows} rows")
+        _need("tokens", tokens, (count,), _INT32)
+        if base is not None:
+            _need("base", base, (table_rows, width), gradient.dtype)
+        out = self._out("out", out, (table_rows, width), gradient.dtype)
+        self._call(self._lib.pcu_native_embedding_backward, ctypes.byref(rows), tokens.ptr, table_rows, scale,
+                   base.ptr if base is not None else None, width, out.ptr, width)
+        return out
+
+    def _norm_weights(self, x: DeviceArray, weights) -> int:
+        """The type's code of the weights among `weights` that there are."""
+        dtype = next((w.dtype for w in weights if w is not None), x.dtype)
+        if dtype != x.dtype and not (dtype == _FLOAT32 and x.dtype.itemsize == 2):
+            raise PcuExecutionError(_abi.PCU_ERR_SHAPE, f"layer_norm: weights of {dtype} for rows of {x.dtype}")
+        for w in weights:
+            if w is not None:
+                _need("weight", w, (x.shape[1],), dtype)
+        return _logit_code("layer_norm", dtype)
+
+    def native_layer_norm(self, x: DeviceArray, weight: Optional[DeviceArray] = None,
+                          bias: Optional[DeviceArray] = None, eps: float = 1e-5,
+                          out: Optional[DeviceArray] = None, stats: Optional[DeviceArray] = None):
+        """Layer norm of each row: ``(out, stats)``, ``stats`` [rows, 2] the mean and the reciprocal
+        of the standard deviation, as the backward pass takes them. ``weight`` and ``bias`` are of
+        the rows' type, or float32 for 16-bit rows; ``out`` may be ``x`` (pcu_native_layer_norm)."""
+        rows = self._rows("layer_norm", x)
+        code = self._norm_weights(x, (weight, bias))
+        out = self._out("out", out, x.shape, x.dtype)
+        stats = self._out("stats", stats, (x.shape[0], 2), _stat_dtype(x.dtype))
+        self.check(self._lib.pcu_native_layer_norm(
+            self.handle, ctypes.byref(rows), weight.ptr if weight is not None else None,
+            bias.ptr if bias is not None else None, code, eps, out.ptr, x.shape[1], stats.ptr))
+        return out, stats
+
+    def native_layer_norm_backward(self, x: DeviceArray, stats: DeviceArray, gradient: DeviceArray,
+                                   weight: Optional[DeviceArray] = None, x_gradient: Optional[DeviceArray] = None,
+                                   weight_gradient: Optional[DeviceArray] = None,
+                                   bias_gradient: Optional[DeviceArray] = None):
+        """The gradients of native_layer_norm from its ``x`` and ``stats``: ``(x_gradient,
+        weight_gradient, bias_gradient)``. With a ``weight``, or an array for one of them, the weight's
+        and the bias's are computed, else None. ``x_gradient`` may be ``gradient`` or ``x``
+        (pcu_native_layer_norm_backward)."""
+        rows = self._rows("layer_norm", x)
+        width = x.shape[1]
+        _need("stats", stats, (x.shape[0], 2), _stat_dtype(x.dtype))
+        _need("gradient", gradient, x.shape, x.dtype)
+        code = self._norm_weights(x, (weight, weight_gradient, bias_gradient))
+        x_gradient = self._out("x_gradient", x_gradient, x.shape, x.dtype)
+        if weight is not None:
+            weight_gradient = weight_gradient if weight_gradient is not None else self.empty((width,), weight.dtype)
+            bias_gradient = bias_gradient if bias_gradient is not None else self.empty((width,), weight.dtype)
+        self.check(self._lib.pcu_native_layer_norm_backward(
+            self.handle, ctypes.byref(rows), stats.ptr, gradient.ptr, width,
+            weight.ptr if weight is not None else None, code, x_gradient.ptr, width,
+            weight_gradient.ptr if weight_gradient is not None else None,
+            bias_gradient.ptr if bias_gradient is not None else None))
+        return x_gradient, weight_gradient, bias_gradient

@@ -30,6 +30,7 @@ STATUS_NAMES = {
 
 PCU_F32, PCU_F64, PCU_BF16, PCU_F16 = 0, 1, 2, 3
 LOGITS_MAX_VOCAB, LOGITS_MAX_K = 1 << 22, 1024
+ROWS_MAX_COLS, TABLE_MAX_ROWS = 1 << 22, 1 << 22
 UNDERFLOW_IEEE, UNDERFLOW_REJECT_SUBNORMAL, UNDERFLOW_ALLOW_GRADUAL = 0, 1, 2
 OP_ADD, OP_SUB, OP_MUL, OP_DIV = 0, 1, 2, 3
 
@@ -170,6 +171,27 @@ SIGNATURES.update({
     "pcu_native_sample": (_i32, [_vp, _LP, ctypes.POINTER(Sampling), _vp, _vp, _FP]),
 })
 
+
+class Rows(ctypes.Structure):
+    """pcu_rows."""
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("dtype", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+        ("rows", ctypes.c_uint64),
+        ("cols", ctypes.c_uint64),
+        ("stride", ctypes.c_uint64),
+    ]
+
+
+_RP = ctypes.POINTER(Rows)
+SIGNATURES.update({
+    "pcu_native_embedding": (_i32, [_vp, _RP, _vp, _u64, ctypes.c_double, _vp, _u64, _FP]),
+    "pcu_native_embedding_backward": (_i32, [_vp, _RP, _vp, _u64, ctypes.c_double, _vp, _u64, _vp, _u64, _FP]),
+    "pcu_native_layer_norm": (_i32, [_vp, _RP, _vp, _vp, _i32, ctypes.c_double, _vp, _u64, _vp]),
+    "pcu_native_layer_norm_backward": (_i32, [_vp, _RP, _vp, _vp, _u64, _vp, _i32, _vp, _u64, _vp, _vp]),
+})
+
 _U32P = ctypes.POINTER(ctypes.c_uint32)
 _U64P = ctypes.POINTER(ctypes.c_uint64)
 SIGNATURES.update({
@@ -210,7 +232,8 @@ KERNEL_IDS = {
     "strict_gemm": 0, "gemm_prefilter": 1, "gemm_replay": 2, "sgd": 3, "binary": 4,
     "relu": 5, "relu_backward": 6, "add_relu": 7, "mse": 8,
     "native_gemm": 9, "native_sgd": 10, "native_mse": 11, "elementwise_chain": 12,
-    "top_logits": 13, "distill": 14, "sample": 15,
+    "top_logits": 13, "distill": 14, "sample": 15, "embedding": 16, "layer_norm": 17,
+    "cross_entropy": 18,
 }
 
 _lib = None

@@ -1,0 +1,611 @@
+// Embedding lookup with scaling, and the table's gradient.
+//
+//   out[i] = scale * table[t_i]                 (a negative token: zeros)
+//   grad[v] = base[v] + scale * (sum of g[i] over the i with t_i = v, i ascending)
+//
+// The gradient sorts the tokens (stable, so a row's terms are added in one order whatever the
+// launch did), then every row of the table is written once by the lanes that own it: no atomics on
+// values, no second pass over the table to clear it. Both directions are bound by HBM.
+#include "pcu_logits.hpp"
+
+#pragma clang fp contract(off)
+
+namespace pcu {
+namespace {
+
+// Lanes a row takes: a row's 16-byte vectors, as a power of two of at most 64.
+inline int row_lanes(uint32_t vecs)
+{
+    int t = 1;
+    while (t < 64 && (uint32_t)t < vecs)
+        t *= 2;
+    return t;
+}
+
+// A vector of a row, stored past the caches by a launch that ends its program.
+template <typename S> __device__ __forceinline__ void store_row(S *row, uint32_t i, uint32_t n, const typename StatOf<S>::T *v, bool through)
+{
+    if (!through) {
+        store_vec(row, i, n, v, false);
+        return;
+    }
+    const uint32_t at = i * kVec<S>;
+    if (at + kVec<S> <= n) {
+        put_vec(row + at, pack<S>(v));
+    } else {
+#pragma unroll
+        for (int e = 0; e < kVec<S>; e++)
+            if (at + e < n)
+                put(row + at + e, (S)v[e]);
+    }
+}
+
+// `lanes` lanes a row (a power of two of at most 64), 256 threads a workgroup.
+template <typename S> __global__ __launch_bounds__(256) void k_embed(EmbedArgs g, int lanes, ProgramClose close)
+{
+    using T = typename StatOf<S>::T;
+    if (block_gate_closed(g.gate))
+        return;
+    const uint32_t lane = threadIdx.x & (lanes - 1), per_block = 256 / lanes;
+    const uint64_t i = (uint64_t)row_of_block() * per_block + threadIdx.x / lanes;
+    const uint32_t vecs = (g.width + kVec<S> - 1) / kVec<S>;
+    const T scale = (T)g.scale;
+    uint64_t key = kNoFault;
+    if (i < g.rows) {
+        const int32_t t = g.tokens[i];
+        S *out = static_cast<S *>(g.out) + i * g.out_stride;
+        if (t >= 0 && (uint64_t)t < g.vocab) {
+            const S *row = static_cast<const S *>(g.table) + (uint64_t)t * g.table_stride;
+            for (uint32_t v0 = lane; v0 < vecs; v0 += 4 * lanes) {
+                u32x4 raw[4];
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                    if (v0 + q * lanes < vecs)
+                        raw[q] = load_vec(row, v0 + q * lanes, g.width);
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                    if (v0 + q * lanes < vecs) {
+                        T x[kVec<S>];
+                        unpack<S>(raw[q], x);
+#pragma unroll
+                        for (int e = 0; e < kVec<S>; e++)
+                            x[e] *= scale;
+                        store_row(out, v0 + q * lanes, g.width, x, close.words != nullptr);
+                    }
+            }
+        } else {
+            if (t >= 0)
+                key = pack_fault(i, kInvalid);
+            const T zero[kVec<S>] = {};
+            for (uint32_t v = lane; v < vecs; v += lanes)
+                store_row(out, v, g.width, zero, close.words != nullptr);
+        }
+    }
+    wave_record_fault(key, g.fault, g.gate);
+    program_close_block(close);
+}
+
+template <typename S> hipError_t launch_embed_t(hipStream_t s, const EmbedArgs &g, ProgramClose close, bool *closed)
+{
+    const int lanes = row_lanes((g.width + kVec<S> - 1) / kVec<S>);
+    const uint64_t blocks = (g.rows + 256 / lanes - 1) / (256 / lanes);
+    if (blocks > kCloseMaxBlocks)
+        close = ProgramClose{};
+    *closed = close.words != nullptr;
+    hipLaunchKernelGGL((k_embed<S>), row_grid(blocks), dim3(256), 0, s, g, lanes, close);
+    return hipGetLastError();
+}
+
+// ------------------------------------------------------------------ sorting tokens
+// Keys are the tokens, absent and invalid ones as `vocab` (they come last and are not summed).
+// Two stable counting passes over half of the key's bits each (at most 12). A tile of keys is
+// ranked by one workgroup: its waves take consecutive runs of it, 64 keys at a time, and lanes with
+// equal digits find each other by one ballot for each bit.
+constexpr int kSortTile = 4096, kSortThreads = 512, kSortRounds = kSortTile / kSortThreads;
+constexpr int kSortWaves = kSortThreads / 64;
+
+__device__ __forceinline__ uint32_t token_key(const int32_t *tokens, uint64_t i, uint32_t vocab)
+{
+    const int32_t t = tokens[i];
+    return t >= 0 && (uint32_t)t < vocab ? (uint32_t)t : vocab;
+}
+
+// Of the lanes with the same digit (and `on`): those before this one, and all of them.
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool on)
+{
+    uint64_t same = __ballot(on);
+    for (int b = 0; b < bits; b++) {
+        const uint64_t set = __ballot((digit >> b) & 1);
+        same &= (digit >> b) & 1 ? set : ~set;
+    }
+    return same;
+}
+
+// How often each digit occurs in a tile: counts[tile][digit].
+__global__ __launch_bounds__(kSortThreads) void k_sort_count(EmbedBackArgs g, const uint32_t *keys, int shift, int bits,
+                                                             uint32_t *counts)
+{
+    extern __shared__ uint32_t hist[];
+    if (block_gate_closed(g.gate))
+        return;
+    const uint32_t bins = 1u << bits;
+    for (uint32_t b = threadIdx.x; b < bins; b += kSortThreads)
+        hist[b] = 0;
+    __syncthreads();
+    uint64_t key = kNoFault;
+    for (int r = 0; r < kSortRounds; r++) {
+        const uint64_t i = (uint64_t)blockIdx.x * kSortTile + r * kSortThreads + threadIdx.x;
+        if (i < g.rows) {
+            uint32_t k;
+            if (keys) {
+                k = keys[i];
+            } else {
+                const int32_t t = g.tokens[i];
+                if (t >= 0 && (uint32_t)t >= g.vocab && key == kNoFault)
+                    key = pack_fault(i, kInvalid);
+                k = token_key(g.tokens, i, g.vocab);
+            }
+            atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
+        }
+    }
+    wave_record_fault(key, g.fault, g.gate);
+    __syncthreads();
+    for (uint32_t b = threadIdx.x; b < bins; b += kSortThreads)
+        counts[(uint64_t)blockIdx.x * bins + b] = hist[b];
+}
+
+// Ranks of a tile's keys among the tile's equal digits, wave by wave: rank[r] within the wave, and
+// wave_count[wave][digit], the wave's number of each digit.
+template <typename Key>
+__device__ __forceinline__ void rank_tile(Key key_at, uint64_t n, uint64_t tile0, int shift, int bits,
+                                          uint32_t (&k)[kSortRounds], uint32_t (&rank)[kSortRounds], uint32_t *wave_count)
+{
+    const uint32_t bins = 1u << bits, wave = threadIdx.x / 64, lane = threadIdx.x & 63;
+    uint32_t *mine = wave_count + wave * bins;
+    for (uint32_t b = threadIdx.x; b < bins * kSortWaves; b += kSortThreads)
+        wave_count[b] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kSortRounds; r++) {
+        const uint64_t i = tile0 + wave * (kSortTile / kSortWaves) + r * 64 + lane;
+        const bool on = i < n;
+        k[r] = on ? key_at(i) : ~0u;
+        const uint32_t d = (k[r] >> shift) & (bins - 1);
+        const uint64_t same = same_digit(d, bits, on);
+        const uint64_t before = same & ((1ull << lane) - 1);
+        const uint32_t base = on ? mine[d] : 0;
+        rank[r] = base + (uint32_t)__popcll(before);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (on && before == 0)
+            mine[d] = base + (uint32_t)__popcll(same);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    __syncthreads();
+}
+
+// Exclusive prefix over a tile's or launch's bins, in place: v[b] becomes the sum before bin b.
+__device__ __forceinline__ void scan_bins(uint32_t *v, uint32_t bins, uint32_t *part)
+{
+    const uint32_t each = (bins + kSortThreads - 1) / kSortThreads, b0 = threadIdx.x * each;
+    uint32_t sum = 0;
+    for (uint32_t b = b0; b < b0 + each && b < bins; b++)
+        sum += v[b];
+    const uint32_t upto = wave_upto(sum, OpSum{}, 0u);
+    if ((threadIdx.x & 63) == 63)
+        part[threadIdx.x / 64] = upto;
+    __syncthreads();
+    uint32_t at = upto - sum;
+    for (uint32_t w = 0; w < threadIdx.x / 64; w++)
+        at += part[w];
+    for (uint32_t b = b0; b < b0 + each && b < bins; b++) {
+        const uint32_t n = v[b];
+        v[b] = at;
+        at += n;
+    }
+    __syncthreads();
+}
+
+// One workgroup a digit: its count in each tile becomes its count in the tiles before, and its
+// count in all of them goes to totals.
+__global__ __launch_bounds__(kSortThreads) void k_sort_scan(EmbedBackArgs g, int bits, uint32_t tiles, uint32_t *counts,
+                                                            uint32_t *totals)
+{
+    __shared__ uint32_t part[kSortWaves];
+    if (block_gate_closed(g.gate))
+        return;
+    uint32_t before = 0;
+    for (uint32_t t0 = 0; t0 < tiles; t0 += kSortThreads) {
+        const uint32_t t = t0 + threadIdx.x;
+        uint32_t *c = counts + ((uint64_t)t << bits) + blockIdx.x;
+        const uint32_t n = t < tiles ? *c : 0, upto = wave_upto(n, OpSum{}, 0u);
+        if ((threadIdx.x & 63) == 63)
+            part[threadIdx.x / 64] = upto;
+        __syncthreads();
+        uint32_t at = before + upto - n;
+#pragma unroll
+        for (uint32_t w = 0; w < kSortWaves; w++) {
+            at += w < threadIdx.x / 64 ? part[w] : 0;
+            before += part[w];
+        }
+        if (t < tiles)
+            *c = at;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0)
+        totals[blockIdx.x] = before;
+}
+
+// Moves a tile's keys and places to where the digit's order puts them: after all smaller digits,
+// and after the digit in the tiles before.
+__global__ __launch_bounds__(kSortThreads) void k_sort_move(EmbedBackArgs g, const uint32_t *keys, const uint32_t *places,
+                                                            int shift, int bits, const uint32_t *counts, const uint32_t *totals,
+                                                            uint32_t *keys_out, uint32_t *places_out)
+{
+    extern __shared__ uint32_t lds[];
+    if (block_gate_closed(g.gate))
+        return;
+    const uint32_t bins = 1u << bits, wave = threadIdx.x / 64;
+    uint32_t *first = lds, *wave_count = lds + bins, *part = wave_count + bins * kSortWaves;
+    uint32_t k[kSortRounds], rank[kSortRounds];
+    rank_tile([&](uint64_t i) { return keys ? keys[i] : token_key(g.tokens, i, g.vocab); }, g.rows,
+              (uint64_t)blockIdx.x * kSortTile, shift, bits, k, rank, wave_count);
+    for (uint32_t b = threadIdx.x; b < bins; b += kSortThreads)
+        first[b] = totals[b];
+    __syncthreads();
+    scan_bins(first, bins, part);
+    for (uint32_t b = threadIdx.x; b < bins; b += kSortThreads) {
+        uint32_t at = first[b] + counts[(uint64_t)blockIdx.x * bins + b];
+        for (int w = 0; w < kSortWaves; w++) {
+            const uint32_t n = wave_count[w * bins + b];
+            wave_count[w * bins + b] = at;
+            at += n;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kSortRounds; r++) {
+        const uint64_t i = (uint64_t)blockIdx.x * kSortTile + wave * (kSortTile / kSortWaves) + r * 64 + (threadIdx.x & 63);
+        if (i < g.rows) {
+            const uint32_t to = wave_count[wave * bins + ((k[r] >> shift) & (bins - 1))] + rank[r];
+            keys_out[to] = k[r];
+            places_out[to] = places ? places[i] : (uint32_t)i;
+        }
+    }
+}
+
+// One tile at most: both passes in one workgroup, through LDS.
+__global__ __launch_bounds__(kSortThreads) void k_sort_one(EmbedBackArgs g, int bits, uint32_t *keys_out, uint32_t *places_out)
+{
+    extern __shared__ uint32_t lds[];
+    if (block_gate_closed(g.gate))
+        return;
+    const uint32_t bins = 1u << bits, wave = threadIdx.x / 64, lane = threadIdx.x & 63, n = (uint32_t)g.rows;
+    uint32_t *first = lds, *wave_count = lds + bins, *part = wave_count + bins * kSortWaves;
+    uint32_t *mid_key = part + kSortWaves, *mid_place = mid_key + kSortTile;
+    uint64_t key = kNoFault;
+    for (uint32_t i = threadIdx.x; i < n; i += kSortThreads) {
+        const int32_t t = g.tokens[i];
+        if (t >= 0 && (uint32_t)t >= g.vocab && key == kNoFault)
+            key = pack_fault(i, kInvalid);
+    }
+    wave_record_fault(key, g.fault, g.gate);
+    for (int pass = 0; pass < 2; pass++) {
+        uint32_t k[kSortRounds], rank[kSortRounds];
+        rank_tile([&](uint64_t i) { return pass ? mid_key[i] : token_key(g.tokens, i, g.vocab); }, n, 0, pass * bits, bits,
+                  k, rank, wave_count);
+        for (uint32_t b = threadIdx.x; b < bins; b += kSortThreads) {
+            uint32_t all = 0;
+            for (int w = 0; w < kSortWaves; w++)
+                all += wave_count[w * bins + b];
+            first[b] = all;
+        }
+        __syncthreads();
+        scan_bins(first, bins, part);
+        for (uint32_t b = threadIdx.x; b < bins; b += kSortThreads) {
+            uint32_t at = first[b];
+            for (int w = 0; w < kSortWaves; w++) {
+                const uint32_t c = wave_count[w * bins + b];
+                wave_count[w * bins + b] = at;
+                at += c;
+            }
+        }
+        uint32_t place[kSortRounds];
+#pragma unroll
+        for (int r = 0; r < kSortRounds; r++) {
+            const uint32_t i = wave * (kSortTile / kSortWaves) + r * 64 + lane;
+            place[r] = pass && i < n ? mid_place[i] : i;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kSortRounds; r++) {
+            const uint32_t i = wave * (kSortTile / kSortWaves) + r * 64 + lane;
+            if (i < n) {
+                const uint32_t to = wave_count[wave * bins + ((k[r] >> (pass * bits)) & (bins - 1))] + rank[r];
+                (pass ? keys_out : mid_key)[to] = k[r];
+                (pass ? places_out : mid_place)[to] = place[r];
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// --------------------------------------------------------------------- summing
+// First of the n sorted keys that is at least v.
+__device__ __forceinline__ uint32_t lower_bound(const uint32_t *keys, uint32_t n, uint32_t v)
+{
+    uint32_t lo = 0, len = n;
+    while (len > 0) {
+        const uint32_t half = len / 2;
+        if (keys[lo + half] < v) {
+            lo += half + 1;
+            len -= half + 1;
+        } else {
+            len = half;
+        }
+    }
+    return lo;
+}
+
+// Rows of more terms than this are added up by several waves, kLong terms each (aligned in the
+// sorted order), whose sums are added in order afterwards.
+constexpr uint32_t kLong = 64;
+
+// Where the terms of a key lie.
+struct Run {
+    uint32_t lo, hi;
+};
+__device__ __forceinline__ Run run_of(const uint32_t *keys, uint32_t n, uint32_t key)
+{
+    return Run{lower_bound(keys, n, key), lower_bound(keys, n, key + 1)};
+}
+
+// sum += terms [lo, hi) of the sorted order, vector v of each, one after another.
+template <typename S, typename T>
+__device__ __forceinline__ void add_terms(const EmbedBackArgs &g, const uint32_t *places, uint32_t lo, uint32_t hi, uint32_t v,
+                                          T (&sum)[kVec<S>])
+{
+    constexpr int U = 8;
+    for (uint32_t j = lo; j < hi; j += U) {
+        u32x4 raw[U];
+#pragma unroll
+        for (int q = 0; q < U; q++)
+            if (j + q < hi)
+                raw[q] = load_vec(static_cast<const S *>(g.gradient) + (uint64_t)places[j + q] * g.gradient_stride, v, g.width);
+#pragma unroll
+        for (int q = 0; q < U; q++)
+            if (j + q < hi) {
+                T x[kVec<S>];
+                unpack<S>(raw[q], x);
+#pragma unroll
+                for (int e = 0; e < kVec<S>; e++)
+                    sum[e] += x[e];
+            }
+    }
+}
+
+template <typename S, typename T>
+__device__ __forceinline__ void write_sum(const EmbedBackArgs &g, uint32_t row, uint32_t v, bool any, const T (&sum)[kVec<S>])
+{
+    const T scale = (T)g.scale;
+    T y[kVec<S>];
+    S *out = static_cast<S *>(g.out) + (uint64_t)row * g.out_stride;
+    if (g.base) {
+        if (!any && g.base == g.out)
+            return; // the row keeps what it holds
+        unpack<S>(load_vec(static_cast<const S *>(g.base) + (uint64_t)row * g.base_stride, v, g.width), y);
+#pragma unroll
+        for (int e = 0; e < kVec<S>; e++)
+            y[e] = any ? y[e] + scale * sum[e] : y[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < kVec<S>; e++)
+            y[e] = any ? scale * sum[e] : (T)0;
+    }
+    store_vec(out, v, g.width, y, false);
+}
+
+template <typename S, typename T>
+__device__ __forceinline__ void leave_part(const EmbedBackArgs &g, const uint32_t *places, uint32_t lo, uint32_t hi, uint32_t v, T *out)
+{
+    T sum[kVec<S>] = {};
+    add_terms<S>(g, places, lo, hi, v, sum);
+#pragma unroll
+    for (int e = 0; e < kVec<S>; e++)
+        out[e] = sum[e];
+}
+
+constexpr uint32_t kRowsAWave = 16;
+
+// Workgroups [0, row_blocks) write the table's rows; the others leave the sums of long rows' parts,
+// part c (terms c kLong ..) with its first row's sum at 2 c and its last row's at 2 c + 1.
+template <typename S>
+__global__ __launch_bounds__(256) void k_embed_sum(EmbedBackArgs g, const uint32_t *keys, const uint32_t *places, int lanes,
+                                                   uint32_t row_blocks, void *parts)
+{
+    using T = typename StatOf<S>::T;
+    if (block_gate_closed(g.gate))
+        return;
+    const uint32_t n = (uint32_t)g.rows, lane = threadIdx.x & (lanes - 1), sub = threadIdx.x / lanes, subs = 256 / lanes;
+    const uint32_t vecs = (g.width + kVec<S> - 1) / kVec<S>, v = blockIdx.y * lanes + lane;
+    if (blockIdx.x < row_blocks) {
+        // kRowsAWave rows a wave: its lanes look them all up at once.
+        __shared__ uint32_t from[4][kRowsAWave + 1];
+        const uint32_t wave = threadIdx.x / 64, row0 = (blockIdx.x * 4 + wave) * kRowsAWave;
+        if ((threadIdx.x & 63) <= kRowsAWave)
+            from[wave][threadIdx.x & 63] = lower_bound(keys, n, min(row0 + (threadIdx.x & 63), g.vocab));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const uint32_t subs_wave = 64 / lanes;
+        for (uint32_t r = sub % subs_wave; r < kRowsAWave; r += subs_wave) {
+            if (row0 + r >= g.vocab || v >= vecs)
+                continue;
+            const uint32_t lo = from[wave][r], hi = from[wave][r + 1];
+            if (hi - lo > kLong)
+                continue;
+            T sum[kVec<S>] = {};
+            add_terms<S>(g, places, lo, hi, v, sum);
+            write_sum<S>(g, row0 + r, v, hi > lo, sum);
+        }
+        return;
+    }
+    const uint32_t c = (blockIdx.x - row_blocks) * subs + sub, lo = c * kLong;
+    if (lo >= n || v >= vecs)
+        return;
+    const uint32_t hi = min(lo + kLong, n), first = keys[lo], last = keys[hi - 1];
+    T *out = static_cast<T *>(parts) + ((uint64_t)2 * c * vecs + v) * kVec<S>;
+    const Run head = run_of(keys, n, first);
+    if (first < g.vocab && head.hi - head.lo > kLong)
+        leave_part<S>(g, places, lo, min(hi, head.hi), v, out);
+    if (last == first || last >= g.vocab)
+        return;
+    const Run tail = run_of(keys, n, last);
+    if (tail.hi - tail.lo > kLong)
+        leave_part<S>(g, places, tail.lo, hi, v, out + (uint64_t)vecs * kVec<S>);
+}
+
+// The long rows, each by the part in which it begins.
+template <typename S>
+__global__ __launch_bounds__(256) void k_embed_join(EmbedBackArgs g, const uint32_t *keys, int lanes, const void *parts)
+{
+    using T = typename StatOf<S>::T;
+    if (block_gate_closed(g.gate))
+        return;
+    const uint32_t n = (uint32_t)g.rows, lane = threadIdx.x & (lanes - 1), subs = 256 / lanes;
+    const uint32_t vecs = (g.width + kVec<S> - 1) / kVec<S>, v = blockIdx.y * lanes + lane;
+    const uint32_t c = blockIdx.x * subs + threadIdx.x / lanes, lo = c * kLong;
+    if (lo >= n || v >= vecs)
+        return;
+    const uint32_t first = keys[lo], last = keys[min(lo + kLong, n) - 1];
+    const Run run = run_of(keys, n, last);
+    if (last >= g.vocab || run.hi - run.lo <= kLong || run.lo < lo)
+        return;
+    const T *from = static_cast<const T *>(parts) + (uint64_t)v * kVec<S>;
+    const uint64_t part = (uint64_t)vecs * kVec<S>;
+    const uint32_t more = (run.hi - 1) / kLong - c; // parts after this one
+    T sum[kVec<S>];
+#pragma unroll
+    for (int e = 0; e < kVec<S>; e++)
+        sum[e] = from[(2 * (uint64_t)c + (first == last ? 0 : 1)) * part + e];
+    constexpr uint32_t U = 4;
+    for (uint32_t j = 1; j <= more; j += U) {
+        T x[U][kVec<S>];
+#pragma unroll
+        for (uint32_t q = 0; q < U; q++)
+            if (j + q <= more)
+#pragma unroll
+                for (int e = 0; e < kVec<S>; e++)
+                    x[q][e] = from[2 * (uint64_t)(c + j + q) * part + e];
+#pragma unroll
+        for (uint32_t q = 0; q < U; q++)
+            if (j + q <= more)
+#pragma unroll
+                for (int e = 0; e < kVec<S>; e++)
+                    sum[e] += x[q][e];
+    }
+    write_sum<S>(g, last, v, true, sum);
+}
+
+// What the gradient's scratch holds: sorted keys and places, those of the first pass, the tiles'
+// digit counts and the launch's, and the long rows' parts.
+struct EmbedPlan {
+    int bits;             // of each of the two digits
+    uint32_t tiles, lds;  // of the sort
+    bool one;             // a single workgroup sorts
+    uint64_t keys, counts, totals, parts, bytes;
+    explicit EmbedPlan(const EmbedBackArgs &g)
+    {
+        bits = 1;
+        while ((1ull << (2 * bits)) <= g.vocab) // the largest key is vocab
+            bits++;
+        const uint64_t bins = 1ull << bits;
+        tiles = (uint32_t)((g.rows + kSortTile - 1) / kSortTile);
+        lds = (uint32_t)((bins * (1 + kSortWaves) + kSortWaves) * 4);
+        one = tiles <= 1 && bits <= 11; // its keys and places fit beside the counts in 160 KiB
+        const int size = logit_size_of(g.dtype);
+        const uint64_t vecs = ((uint64_t)g.width * size + 15) / 16, stat = size == 8 ? 8 : 4;
+        auto take = [&](uint64_t n) {
+            const uint64_t at = bytes;
+            bytes += (n + 255) / 256 * 256;
+            return at;
+        };
+        bytes = 0;
+        keys = take(4 * 4 * g.rows);
+        counts = take(one ? 0 : bins * tiles * 4);
+        totals = take(one ? 0 : bins * 4);
+        parts = take(g.rows > kLong ? (g.rows + kLong - 1) / kLong * 2 * vecs * (16 / size) * stat : 0);
+    }
+};
+
+// A kernel whose LDS is beyond what a launch may have unasked.
+template <typename K> hipError_t allow_lds(K *kernel, uint32_t bytes)
+{
+    return bytes > 65536 ? hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes)
+                         : hipSuccess;
+}
+
+template <typename S> hipError_t launch_embed_back_t(hipStream_t s, const EmbedBackArgs &g, void *scratch)
+{
+    const EmbedPlan p(g);
+    char *sc = static_cast<char *>(scratch);
+    uint32_t *keys = reinterpret_cast<uint32_t *>(sc + p.keys), *places = keys + g.rows;
+    uint32_t *mid_keys = places + g.rows, *mid_places = mid_keys + g.rows;
+    uint32_t *counts = reinterpret_cast<uint32_t *>(sc + p.counts), *totals = reinterpret_cast<uint32_t *>(sc + p.totals);
+    hipError_t e;
+    if (p.one) {
+        const uint32_t lds = p.lds + 2 * kSortTile * 4;
+        if ((e = allow_lds(k_sort_one, lds)))
+            return e;
+        hipLaunchKernelGGL(k_sort_one, dim3(1), dim3(kSortThreads), lds, s, g, p.bits, keys, places);
+    } else {
+        if ((e = allow_lds(k_sort_move, p.lds)))
+            return e;
+        const uint32_t bins = 1u << p.bits;
+        for (int pass = 0; pass < 2; pass++) {
+            const uint32_t *in = pass ? mid_keys : nullptr;
+            hipLaunchKernelGGL(k_sort_count, dim3(p.tiles), dim3(kSortThreads), bins * 4, s, g, in, pass * p.bits, p.bits, counts);
+            hipLaunchKernelGGL(k_sort_scan, dim3(bins), dim3(kSortThreads), 0, s, g, p.bits, p.tiles, counts, totals);
+            hipLaunchKernelGGL(k_sort_move, dim3(p.tiles), dim3(kSortThreads), p.lds, s, g, in, pass ? mid_places : nullptr,
+                               pass * p.bits, p.bits, counts, totals, pass ? keys : mid_keys, pass ? places : mid_places);
+        }
+    }
+    const uint32_t vecs = (g.width + kVec<S> - 1) / kVec<S>;
+    const int lanes = row_lanes(vecs);
+    const uint32_t subs = 256 / lanes, across = (vecs + lanes - 1) / lanes;
+    const uint32_t row_blocks = (uint32_t)((g.vocab + 4 * kRowsAWave - 1) / (4 * kRowsAWave));
+    const uint32_t part_blocks = g.rows > kLong ? (uint32_t)(((g.rows + kLong - 1) / kLong + subs - 1) / subs) : 0;
+    hipLaunchKernelGGL((k_embed_sum<S>), dim3(row_blocks + part_blocks, across), dim3(256), 0, s, g, keys, places, lanes,
+                       row_blocks, sc + p.parts);
+    if (part_blocks)
+        hipLaunchKernelGGL((k_embed_join<S>), dim3(part_blocks, across), dim3(256), 0, s, g, keys, lanes, sc + p.parts);
+    return hipGetLastError();
+}
+
+} // namespace
+
+hipError_t launch_embed(hipStream_t s, const EmbedArgs &g, ProgramClose close, bool *closed)
+{
+    *closed = false;
+    if (g.rows == 0 || g.width == 0)
+        return hipSuccess;
+    switch (g.dtype) {
+    case kLogitF32: return launch_embed_t<float>(s, g, close, closed);
+    case kLogitF64: return launch_embed_t<double>(s, g, close, closed);
+    case kLogitBf16: return launch_embed_t<__bf16>(s, g, close, closed);
+    default: return launch_embed_t<_Float16>(s, g, close, closed);
+    }
+}
+
+size_t embed_back_scratch_bytes(const EmbedBackArgs &g) { return g.width && g.vocab ? EmbedPlan(g).bytes : 0; }
+
+hipError_t launch_embed_back(hipStream_t s, const EmbedBackArgs &g, void *scratch)
+{
+    if (g.width == 0 || g.vocab == 0)
+        return hipSuccess;
+    switch (g.dtype) {
+    case kLogitF32: return launch_embed_back_t<float>(s, g, scratch);
+    case kLogitF64: return launch_embed_back_t<double>(s, g, scratch);
+    case kLogitBf16: return launch_embed_back_t<__bf16>(s, g, scratch);
+    default: return launch_embed_back_t<_Float16>(s, g, scratch);
+    }
+}
+
+} // namespace pcu

@@ -1,25 +1,11 @@
 // The operators on logits behind the C ABI: argument checks, scratch and launches.
-#include "pcu_runtime.hpp"
-
-#include <cmath>
+#include "pcu_checks.hpp"
 
 namespace pcu {
 
 static_assert(kLogitMaxVocab == PCU_LOGITS_MAX_VOCAB && kLogitMaxK == PCU_LOGITS_MAX_K, "one limit");
 static_assert(kLogitF32 == PCU_F32 && kLogitF64 == PCU_F64 && kLogitBf16 == PCU_BF16 && kLogitF16 == PCU_F16,
               "one numbering");
-
-static uint64_t logit_size(uint32_t dtype) { return dtype == PCU_F64 ? 8 : dtype == PCU_F32 ? 4 : 2; }
-static uint64_t stat_size(uint32_t dtype) { return dtype == PCU_F64 ? 8 : 4; }
-
-// A pointer to values of `size` bytes: the kernels load and store them whole (null passes).
-static bool aligned(const void *p, uint64_t size) { return ((uintptr_t)p & (size - 1)) == 0; }
-
-// Bytes from the first element of `rows` strided rows of `cols` to past the last one.
-static uint64_t strided_bytes(uint64_t rows, uint64_t cols, uint64_t stride, uint64_t size)
-{
-    return rows && cols ? ((rows - 1) * stride + cols) * size : 0;
-}
 
 static uint64_t logits_bytes(const pcu_logits &l)
 {
@@ -54,25 +40,6 @@ static bool valid_temperature(uint32_t dtype, double temperature, bool squared)
                (!squared || (temperature * temperature > 0 && std::isfinite(temperature * temperature)));
     const float t = (float)temperature;
     return t > 0 && std::isfinite(t) && std::isfinite(1.0f / t * (float)M_LOG2E);
-}
-
-// A weight that is a number in the statistics' type.
-static bool valid_weight(uint32_t dtype, double weight)
-{
-    return dtype == PCU_F64 ? std::isfinite(weight) : std::isfinite((float)weight);
-}
-
-// An output against one input.
-struct Range {
-    const void *p;
-    uint64_t bytes;
-};
-template <size_t N> static bool overlaps_any(Range out, const Range (&in)[N])
-{
-    for (const Range &r : in)
-        if (ranges_overlap(out.p, out.bytes, r.p, r.bytes))
-            return true;
-    return false;
 }
 
 pcu_status Ctx::op_top_logits(const pcu_logits *l, uint32_t k, double temperature, void *values,
@@ -307,19 +274,6 @@ pcu_status Ctx::op_sample(const pcu_logits *l, const pcu_sampling *p, int32_t *t
     if (!st && closed)
         closed_seq = ++pub_seq;
     return st;
-}
-
-// Opens a call on `ctx` as the other op entry points do.
-static Ctx *enter(pcu_ctx *ctx, pcu_status *st)
-{
-    Ctx *c = reinterpret_cast<Ctx *>(ctx);
-    if (!c) {
-        g_thread_error = "null context";
-        *st = PCU_ERR_ARGUMENT;
-        return nullptr;
-    }
-    *st = c->start_op();
-    return *st ? nullptr : c;
 }
 
 } // namespace pcu

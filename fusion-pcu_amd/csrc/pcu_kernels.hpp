@@ -365,6 +365,102 @@ size_t sample_state_bytes();
 hipError_t launch_sample(hipStream_t s, const SampleArgs &g, void *scratch, void *state, ProgramClose close,
                          bool *closed);
 
+// ------------------------------------------- operators around a model's products
+inline int logit_size_of(int dtype) { return dtype == kLogitF64 ? 8 : dtype == kLogitF32 ? 4 : 2; }
+
+// Rows of a table by token, times `scale`; a negative token's row is zeros. A token of `vocab` or
+// more records a fault (ordinal: its place).
+struct EmbedArgs {
+    const void *table = nullptr;
+    int dtype = 0;
+    uint32_t vocab = 0, width = 0;
+    uint64_t table_stride = 0;
+    const int32_t *tokens = nullptr;
+    uint64_t rows = 0;
+    double scale = 1.0;
+    void *out = nullptr;
+    uint64_t out_stride = 0;
+    unsigned long long *fault = nullptr;
+    NodeGate gate{nullptr, 0};
+};
+hipError_t launch_embed(hipStream_t s, const EmbedArgs &g, ProgramClose close, bool *closed);
+
+// The table's gradient: base (or zeros) plus scale times the sum of each token's rows of `gradient`,
+// in their order. `base` may be `out`.
+struct EmbedBackArgs {
+    const void *gradient = nullptr;
+    int dtype = 0;
+    uint32_t vocab = 0, width = 0;
+    uint64_t rows = 0, gradient_stride = 0;
+    const int32_t *tokens = nullptr;
+    double scale = 1.0;
+    const void *base = nullptr;
+    uint64_t base_stride = 0;
+    void *out = nullptr;
+    uint64_t out_stride = 0;
+    unsigned long long *fault = nullptr;
+    NodeGate gate{nullptr, 0};
+};
+size_t embed_back_scratch_bytes(const EmbedBackArgs &g);
+hipError_t launch_embed_back(hipStream_t s, const EmbedBackArgs &g, void *scratch);
+
+// Layer norm of rows, and its gradients. Statistics (mean, 1 / standard deviation) are binary32,
+// binary64 for binary64 rows. weight and bias (or null) are of weight_dtype: the rows' type, or
+// binary32 for 16-bit rows.
+struct NormArgs {
+    const void *x = nullptr;
+    int dtype = 0, weight_dtype = 0;
+    uint64_t rows = 0, stride = 0;
+    uint32_t width = 0;
+    const void *weight = nullptr, *bias = nullptr;
+    double eps = 0.0;
+    void *out = nullptr;
+    uint64_t out_stride = 0;
+    void *stats = nullptr; // rows x 2, or null
+    NodeGate gate{nullptr, 0};
+};
+hipError_t launch_norm(hipStream_t s, const NormArgs &g, ProgramClose close, bool *closed);
+
+struct NormBackArgs {
+    const void *x = nullptr;
+    int dtype = 0, weight_dtype = 0;
+    uint64_t rows = 0, stride = 0;
+    uint32_t width = 0;
+    const void *stats = nullptr; // rows x 2
+    const void *gradient = nullptr;
+    uint64_t gradient_stride = 0;
+    const void *weight = nullptr;
+    void *x_gradient = nullptr; // or null
+    uint64_t x_gradient_stride = 0;
+    void *weight_gradient = nullptr, *bias_gradient = nullptr; // width of weight_dtype, or null
+    NodeGate gate{nullptr, 0};
+};
+size_t norm_back_scratch_bytes(const NormBackArgs &g);
+hipError_t launch_norm_back(hipStream_t s, const NormBackArgs &g, void *scratch);
+
+// The cross entropy of softmax(features * weights^T) against labels, and its gradients, with the
+// logits never in memory. Binary32, bfloat16 or binary16; loss, log_sum and row_scale are binary32.
+struct EntropyArgs {
+    const void *features = nullptr;
+    int dtype = 0;
+    uint64_t rows = 0, feature_stride = 0;
+    uint32_t width = 0, vocab = 0;
+    const void *weights = nullptr; // vocab x width
+    uint64_t weight_stride = 0;
+    const int32_t *labels = nullptr; // rows, negative: none
+    const float *log_sum_in = nullptr; // rows: the gradients alone, from these
+    const float *row_scale = nullptr;  // rows, or null: 1
+    float *loss = nullptr, *log_sum_out = nullptr; // rows, or null
+    void *feature_gradient = nullptr; // rows x width, or null
+    uint64_t feature_gradient_stride = 0;
+    void *weight_gradient = nullptr; // weight_gradient_rows x width (zeros past the vocabulary), or null
+    uint64_t weight_gradient_rows = 0, weight_gradient_stride = 0;
+    unsigned long long *fault = nullptr; // ordinal: the row whose label is out of range
+    NodeGate gate{nullptr, 0};
+};
+size_t entropy_scratch_bytes(const EntropyArgs &g);
+hipError_t launch_entropy(hipStream_t s, const EntropyArgs &g, void *scratch);
+
 // Small device utilities (fill kernels rather than memsets, so a captured graph replays
 // them as kernels).
 hipError_t launch_fill_u64(hipStream_t s, unsigned long long *p, uint64_t n, uint64_t value);

@@ -112,7 +112,8 @@ struct Ctx {
         void *p = nullptr;
         size_t cap = 0;
     };
-    Scratch matmul_scratch, mse_scratch, bt_scratch, table_scratch, logits_scratch, sample_state;
+    Scratch matmul_scratch, mse_scratch, bt_scratch, table_scratch, logits_scratch, sample_state,
+        layer_scratch;
     // The counters of the sampler's rows (sample_state) are zero. Not so before their first use
     // and after a fault: a stage gate that closes during a launch leaves some of them counted.
     bool sample_state_zero = false;
@@ -224,6 +225,18 @@ struct Ctx {
                           void *log_sums_out, void *grad, uint64_t grad_cols, uint64_t grad_stride);
     pcu_status op_sample(const pcu_logits *logits, const pcu_sampling *p, int32_t *tokens,
                          float *log_prob);
+    // The operators around a model's products (layers.cpp).
+    pcu_status op_embedding(const pcu_rows *table, const int32_t *tokens, uint64_t count, double scale,
+                            void *out, uint64_t out_stride);
+    pcu_status op_embedding_backward(const pcu_rows *gradient, const int32_t *tokens, uint64_t table_rows,
+                                     double scale, const void *base, uint64_t base_stride, void *out,
+                                     uint64_t out_stride);
+    pcu_status op_layer_norm(const pcu_rows *x, const void *weight, const void *bias, int weight_dtype,
+                             double eps, void *out, uint64_t out_stride, void *stats);
+    pcu_status op_layer_norm_backward(const pcu_rows *x, const void *stats, const void *gradient,
+                                      uint64_t gradient_stride, const void *weight, int weight_dtype,
+                                      void *x_gradient, uint64_t x_gradient_stride, void *weight_gradient,
+                                      void *bias_gradient);
 };
 
 } // namespace pcu

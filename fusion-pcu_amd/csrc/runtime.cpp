@@ -152,7 +152,7 @@ Ctx::~Ctx()
     if (side)
         (void)hipStreamSynchronize(side);
     for (Scratch *b : {&matmul_scratch, &mse_scratch, &bt_scratch, &table_scratch, &logits_scratch,
-                       &sample_state})
+                       &sample_state, &layer_scratch})
         if (b->p)
             (void)hipFreeAsync(b->p, stream);
     for (const Released &r : reuse)

@@ -33,7 +33,7 @@
 extern "C" {
 #endif
 
-#define PCU_ROCM_ABI_VERSION 4
+#define PCU_ROCM_ABI_VERSION 5
 
 typedef struct pcu_ctx pcu_ctx;
 
@@ -54,7 +54,8 @@ typedef enum pcu_status {
                                 * HipError::InvalidExecutionFaultWord(word) */
 } pcu_status;
 
-/* The operators on logits admit all four types, every other call PCU_F32 and PCU_F64. */
+/* The operators on logits and those around a model's products admit the 16-bit types too, every
+ * other call PCU_F32 and PCU_F64. */
 typedef enum pcu_dtype { PCU_F32 = 0, PCU_F64 = 1, PCU_BF16 = 2, PCU_F16 = 3 } pcu_dtype;
 
 /* PcuFloatUnderflowPolicy (core/scalar_float_underflow.rs:47-58). */
@@ -340,6 +341,59 @@ typedef struct pcu_sampling {
 pcu_status pcu_native_sample(pcu_ctx *ctx, const pcu_logits *logits, const pcu_sampling *sampling,
                              int32_t *tokens, float *log_prob, pcu_fault *fault);
 
+/* ------------------------------------------------ operators around a model's products
+ * No counterpart in the reference: what a language model does before and behind its products.
+ * Native arithmetic (non-finite results are ordinary values), each call one program node. A
+ * pointer that is not aligned to its type is refused. Sums and statistics are F32, F64 for F64
+ * rows, and are added in an order that the sizes alone determine; results are rounded once to
+ * their type. `fault` reports a token or label that is out of its range as PCU_FAULT_INVALID with the
+ * lowest such element; what the call's outputs then hold is unspecified. */
+
+/* `rows` rows of `cols` values of any dtype; row r starts at element r * stride
+ * (stride >= cols: the columns between belong to the caller). Any alignment of the type. */
+typedef struct pcu_rows {
+    const void *data;
+    uint32_t dtype; /* pcu_dtype */
+    uint32_t reserved;
+    uint64_t rows, cols, stride;
+} pcu_rows;
+#define PCU_ROWS_MAX_COLS (1u << 22)
+#define PCU_ROWS_MAX_ROWS (1u << 30) /* and strides */
+#define PCU_TABLE_MAX_ROWS (1u << 22) /* of a table of embeddings or an output layer's weights */
+
+/* out[i] = scale * table[tokens[i]] for i < count, rows of table.cols values of the table's type;
+ * a negative token's row is zeros. A token of table.rows or more is a fault (element_index i). */
+pcu_status pcu_native_embedding(pcu_ctx *ctx, const pcu_rows *table, const int32_t *tokens,
+                                uint64_t count, double scale, void *out, uint64_t out_stride,
+                                pcu_fault *fault);
+/* The gradient by the table: out[v] = base[v] + scale * (the sum of gradient[i] over the i with
+ * tokens[i] = v, in their order) for each of table_rows rows; base may be NULL (zeros) or out itself
+ * (same stride: rows whose token does not occur keep their bits and are not touched), else it overlaps nothing that is written.
+ * Negative tokens are left out; one of table_rows or more is a fault. */
+pcu_status pcu_native_embedding_backward(pcu_ctx *ctx, const pcu_rows *gradient,
+                                         const int32_t *tokens, uint64_t table_rows, double scale,
+                                         const void *base, uint64_t base_stride, void *out,
+                                         uint64_t out_stride, pcu_fault *fault);
+
+/* Each row on its own: m = mean of x, r = 1 / sqrt(mean of (x - m)^2 + eps),
+ * out = (x - m) r weight + bias. weight and bias (either may be NULL): x.cols values of
+ * weight_dtype, which is x's type, or F32 for 16-bit rows. eps: a finite number >= 0. stats (or
+ * NULL): rows x 2, m and r. out may lie exactly on x (same pointer and stride). */
+pcu_status pcu_native_layer_norm(pcu_ctx *ctx, const pcu_rows *x, const void *weight,
+                                 const void *bias, pcu_dtype weight_dtype, double eps, void *out,
+                                 uint64_t out_stride, void *stats);
+/* With n = (x - m) r from the forward pass's stats and g = gradient * weight (weight NULL: 1):
+ *   x_gradient      = r (g - mean of g - n * (mean of g n)), rows of x's type
+ *   weight_gradient = the sum over the rows of gradient * n, bias_gradient of gradient, x.cols
+ *                     values of weight_dtype
+ * gradient: rows of x's type at gradient_stride. Any of the outputs may be NULL. x_gradient may lie
+ * exactly on gradient or on x (same pointer and stride). */
+pcu_status pcu_native_layer_norm_backward(pcu_ctx *ctx, const pcu_rows *x, const void *stats,
+                                          const void *gradient, uint64_t gradient_stride,
+                                          const void *weight, pcu_dtype weight_dtype,
+                                          void *x_gradient, uint64_t x_gradient_stride,
+                                          void *weight_gradient, void *bias_gradient);
+
 /* ------------------------------------------------------------------ program
  * Between begin and end every op call is only enqueued and numbered as a node (0, 1, ...;
  * pcu_checked_add_relu takes two numbers). pcu_program_end synchronizes once and reports
@@ -385,7 +439,10 @@ typedef enum pcu_kernel_id {
     PCU_KERNEL_TOP_LOGITS = 13,
     PCU_KERNEL_DISTILL = 14,           /* all launches of one distillation call */
     PCU_KERNEL_SAMPLE = 15,
-    PCU_KERNEL_COUNT = 16
+    PCU_KERNEL_EMBEDDING = 16,         /* lookup, or all launches of one gradient */
+    PCU_KERNEL_LAYER_NORM = 17,        /* all launches of one call, either direction */
+    PCU_KERNEL_CROSS_ENTROPY = 18,     /* all launches of one call */
+    PCU_KERNEL_COUNT = 19
 } pcu_kernel_id;
 pcu_status pcu_profile_enable(pcu_ctx *ctx, int on);
 pcu_status pcu_profile_read(pcu_ctx *ctx, int kernel, double *total_ms, uint64_t *launches);
