@@ -708,3 +708,66 @@ class Context:
             weight_gradient.ptr if weight_gradient is not None else None,
             bias_gradient.ptr if bias_gradient is not None else None))
         return x_gradient, weight_gradient, bias_gradient
+
+    def _entropy(self, features: DeviceArray, weights: DeviceArray, labels: DeviceArray, vocab: Optional[int]):
+        x, w = self._rows("cross_entropy", features), self._rows("cross_entropy", weights)
+        if features.dtype != weights.dtype or features.shape[1] != weights.shape[1] or \
+                (vocab is not None and not 0 <= vocab <= weights.shape[0]):
+            raise PcuExecutionError(
+                _abi.PCU_ERR_SHAPE, f"cross_entropy: features {features.shape} {features.dtype}, weights "
+                f"{weights.shape} {weights.dtype}, vocab {vocab}")
+        if vocab is not None:
+            w.rows = vocab
+        _need("labels", labels, (features.shape[0],), _INT32)
+        return x, w
+
+    def native_cross_entropy_loss(self, features: DeviceArray, weights: DeviceArray, labels: DeviceArray,
+                                  vocab: Optional[int] = None, loss: Optional[DeviceArray] = None,
+                                  log_sum: Optional[DeviceArray] = None):
+        """Each row's cross entropy of softmax(features * weights^T) against its label (negative:
+        none, loss 0), without the logits in memory: ``(loss [rows], log_sum [rows])``, float32.
+        ``weights`` holds one row a token; ``vocab`` (default: all) names how many leading rows are
+        real. float32, float16 and ``bfloat16`` (pcu_native_cross_entropy_loss)."""
+        x, w = self._entropy(features, weights, labels, vocab)
+        rows = features.shape[0]
+        loss = self._out("loss", loss, (rows,), _FLOAT32)
+        log_sum = self._out("log_sum", log_sum, (rows,), _FLOAT32)
+        self._call(self._lib.pcu_native_cross_entropy_loss, ctypes.byref(x), ctypes.byref(w), labels.ptr, loss.ptr, log_sum.ptr)
+        return loss, log_sum
+
+    def native_cross_entropy_backward(self, features: DeviceArray, weights: DeviceArray, labels: DeviceArray,
+                                      log_sum: DeviceArray, row_scale: Optional[DeviceArray] = None,
+                                      vocab: Optional[int] = None, feature_gradient: Optional[DeviceArray] = None,
+                                      weight_gradient: Optional[DeviceArray] = None):
+        """The gradients of the loss, each row times its ``row_scale``, from
+        native_cross_entropy_loss's ``log_sum``: ``(feature_gradient, weight_gradient)``, like
+        ``features`` and ``weights`` (rows past the vocabulary are 0)."""
+        x, w = self._entropy(features, weights, labels, vocab)
+        rows, width = features.shape
+        _need("log_sum", log_sum, (rows,), _FLOAT32)
+        if row_scale is not None:
+            _need("row_scale", row_scale, (rows,), _FLOAT32)
+        feature_gradient = self._out("feature_gradient", feature_gradient, features.shape, features.dtype)
+        weight_gradient = self._out("weight_gradient", weight_gradient, weights.shape, weights.dtype)
+        self._call(self._lib.pcu_native_cross_entropy_backward, ctypes.byref(x), ctypes.byref(w), labels.ptr, log_sum.ptr,
+                   row_scale.ptr if row_scale is not None else None, feature_gradient.ptr, width, weight_gradient.ptr,
+                   weights.shape[0], width)
+        return feature_gradient, weight_gradient
+
+    def native_cross_entropy_step(self, features: DeviceArray, weights: DeviceArray, labels: DeviceArray,
+                                  row_scale: Optional[DeviceArray] = None, vocab: Optional[int] = None,
+                                  loss: Optional[DeviceArray] = None, feature_gradient: Optional[DeviceArray] = None,
+                                  weight_gradient: Optional[DeviceArray] = None):
+        """native_cross_entropy_loss and native_cross_entropy_backward in one call:
+        ``(loss [rows], feature_gradient, weight_gradient)``."""
+        x, w = self._entropy(features, weights, labels, vocab)
+        rows, width = features.shape
+        if row_scale is not None:
+            _need("row_scale", row_scale, (rows,), _FLOAT32)
+        loss = self._out("loss", loss, (rows,), _FLOAT32)
+        feature_gradient = self._out("feature_gradient", feature_gradient, features.shape, features.dtype)
+        weight_gradient = self._out("weight_gradient", weight_gradient, weights.shape, weights.dtype)
+        self._call(self._lib.pcu_native_cross_entropy_step, ctypes.byref(x), ctypes.byref(w), labels.ptr,
+                   row_scale.ptr if row_scale is not None else None, loss.ptr, feature_gradient.ptr, width,
+                   weight_gradient.ptr, weights.shape[0], width)
+        return loss, feature_gradient, weight_gradient

@@ -190,6 +190,9 @@ SIGNATURES.update({
     "pcu_native_embedding_backward": (_i32, [_vp, _RP, _vp, _u64, ctypes.c_double, _vp, _u64, _vp, _u64, _FP]),
     "pcu_native_layer_norm": (_i32, [_vp, _RP, _vp, _vp, _i32, ctypes.c_double, _vp, _u64, _vp]),
     "pcu_native_layer_norm_backward": (_i32, [_vp, _RP, _vp, _vp, _u64, _vp, _i32, _vp, _u64, _vp, _vp]),
+    "pcu_native_cross_entropy_loss": (_i32, [_vp, _RP, _RP, _vp, _vp, _vp, _FP]),
+    "pcu_native_cross_entropy_backward": (_i32, [_vp, _RP, _RP, _vp, _vp, _vp, _vp, _u64, _vp, _u64, _u64, _FP]),
+    "pcu_native_cross_entropy_step": (_i32, [_vp, _RP, _RP, _vp, _vp, _vp, _vp, _u64, _vp, _u64, _u64, _FP]),
 })
 
 _U32P = ctypes.POINTER(ctypes.c_uint32)

@@ -1,0 +1,821 @@
+// The cross entropy of an output layer, l = x W^T, loss = log(sum exp l) - l[label], and its gradients
+// G = s (softmax(l) - [v = label]), dx = G W, dW = G^T x, with the logits never in memory.
+//
+// The loss is one product whose tiles leave a (maximum, sum of exponentials) for each row and the
+// label's logit; a reduction joins them. The gradients go over the vocabulary in pieces: a piece's
+// logits are made again and turned into G where they lie in registers, G goes to a buffer that the
+// caches hold, and two products read it. That is 2 products of rows x vocab x width for a loss, 8 / 2 for
+// a step against 6 / 2 if the logits were kept.
+//
+// 16-bit features and weights go to the matrix cores as they are. Binary32 ones are split into three
+// bfloat16 parts of 8 bits (exact), of whose products six are summed, smallest first: binary32's precision
+// at a sixth of the 16-bit rate, against the binary32 matrix instructions' sixteenth. G is rounded
+// to the operands' precision (8, 11 or 3 x 8 bits) before its products, as every training in 16 bits rounds
+// the logits' gradient. It is kept relative to the largest row scale, so that rows with that
+// scale, usually all, have the exact factor 1, and in binary16 2^14 times as large: the smallest
+// probability it holds is then 2^-38.
+#include "pcu_entropy_tile.hpp"
+
+#pragma clang fp contract(off)
+
+namespace pcu {
+namespace {
+
+// The first 8 bits of a value, as a bfloat16; v becomes the rest. Three of them are the whole value;
+// what is not finite is its first part alone.
+__device__ __forceinline__ uint32_t first_part(float &v)
+{
+    const uint32_t b = __float_as_uint(v);
+    if ((b & 0x7f800000u) == 0x7f800000u) {
+        v = 0.0f;
+        return (b >> 16) | ((b & 0x7fffffu) ? 0x40u : 0u);
+    }
+    v -= __uint_as_float(b & 0xffff0000u); // exact
+    return b >> 16;
+}
+
+template <typename S> struct ElemOf { using T = S; };
+template <> struct ElemOf<float> { using T = __bf16; };
+template <typename S> constexpr int kParts = sizeof(S) == 4 ? 3 : 1;
+template <typename S> constexpr float kBoost = __is_same(S, _Float16) ? 16384.0f : 1.0f;
+
+// Rows as the tiles take them: parts, zeros past `cols` up to out_ld and past `rows` up to
+// out_rows, and zeros in rows whose label is absent (labels given), whatever those hold.
+struct PackArgs {
+    const void *in = nullptr;
+    uint64_t ld = 0;
+    uint32_t rows = 0, cols = 0;
+    const int32_t *labels = nullptr;
+    uint32_t vocab = 0;
+    uint16_t *out = nullptr;
+    uint64_t plane = 0;
+    uint32_t out_rows = 0, out_ld = 0;
+    NodeGate gate{nullptr, 0};
+};
+
+template <typename S> __device__ __forceinline__ void pack_rows(const PackArgs &g, uint64_t block, uint64_t blocks)
+{
+    const uint32_t pieces = g.out_ld / 8; // of 8 values
+    const uint64_t all = (uint64_t)g.out_rows * pieces;
+    for (uint64_t i = block * 256 + threadIdx.x; i < all; i += blocks * 256) {
+        const uint32_t r = (uint32_t)(i / pieces), c = (uint32_t)(i % pieces) * 8;
+        bool on = r < g.rows && c < g.cols;
+        if (on && g.labels) {
+            const int32_t y = g.labels[r];
+            on = y >= 0 && (uint32_t)y < g.vocab;
+        }
+        uint16_t *out = g.out + (uint64_t)r * g.out_ld + c;
+        if constexpr (sizeof(S) == 2) {
+            u32x4 raw = {0, 0, 0, 0};
+            if (on) {
+                raw = load_vec(static_cast<const S *>(g.in) + r * g.ld, c / 8, g.cols);
+#pragma unroll
+                for (uint32_t e = 0; e < 8; e++)
+                    if (c + e >= g.cols)
+                        raw[e / 2] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
+            }
+            *reinterpret_cast<u32x4 *>(out) = raw;
+        } else {
+            float v[8] = {};
+            if (on) {
+                const float *row = static_cast<const float *>(g.in) + r * g.ld;
+                unpack<float>(load_vec(row, c / 4, g.cols), v);
+                unpack<float>(load_vec(row, c / 4 + 1, g.cols), v + 4);
+            }
+            u32x4 raw[3] = {};
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) {
+                float x = c + e < g.cols ? v[e] : 0.0f;
+#pragma unroll
+                for (int k = 0; k < 3; k++)
+                    raw[k][e / 2] |= first_part(x) << (16 * (e & 1));
+            }
+#pragma unroll
+            for (int k = 0; k < 3; k++)
+                *reinterpret_cast<u32x4 *>(out + k * g.plane) = raw[k];
+        }
+    }
+}
+
+template <typename S> __global__ __launch_bounds__(256) void k_pack(PackArgs g)
+{
+    if (block_gate_closed(g.gate))
+        return;
+    pack_rows<S>(g, blockIdx.x, gridDim.x);
+}
+
+// What the tiles and reductions know of a row.
+struct RowData {
+    int32_t *label;   // -1: none (or out of range: a fault)
+    float *scale;     // relative to *factor; 0 where there is no label
+    float *log_sum;
+    float *own;       // the label's logit
+    float *factor;    // what a gradient's sums are multiplied by
+};
+
+struct PrepArgs {
+    const int32_t *labels = nullptr;
+    const float *row_scale = nullptr;
+    uint32_t rows = 0, vocab = 0;
+    float boost = 1.0f;
+    RowData row{};
+    unsigned long long *fault = nullptr;
+};
+
+// One workgroup: labels, their faults, the largest finite |scale| and the scales relative to it.
+__device__ __forceinline__ void prepare_rows(const PrepArgs &p, const NodeGate &gate)
+{
+    __shared__ float lds[4];
+    uint64_t key = kNoFault;
+    float most = 0.0f;
+    for (uint32_t r = threadIdx.x; r < p.rows; r += 256) {
+        int32_t y = p.labels[r];
+        if (y >= 0 && (uint32_t)y >= p.vocab) {
+            if (key == kNoFault)
+                key = pack_fault(r, kInvalid);
+            y = -1;
+        }
+        p.row.label[r] = y < 0 ? -1 : y;
+        if (y >= 0) {
+            const float s = p.row_scale ? fabsf(p.row_scale[r]) : 1.0f;
+            if (s < INFINITY)
+                most = fmaxf(most, s);
+        }
+    }
+    wave_record_fault(key, p.fault, gate);
+    most = block_reduce<256>(most, OpMax{}, lds);
+    if (most == 0.0f)
+        most = 1.0f;
+    for (uint32_t r = threadIdx.x; r < p.rows; r += 256) {
+        const float s = p.row_scale ? p.row_scale[r] : 1.0f;
+        p.row.scale[r] = p.row.label[r] >= 0 ? s / most : 0.0f;
+    }
+    if (threadIdx.x == 0)
+        *p.row.factor = most / p.boost;
+}
+
+// The features packed and the rows prepared, by one launch.
+template <typename S> __global__ __launch_bounds__(256) void k_entropy_open(PackArgs g, PrepArgs p)
+{
+    if (block_gate_closed(g.gate))
+        return;
+    if (blockIdx.x == 0)
+        prepare_rows(p, g.gate);
+    else
+        pack_rows<S>(g, blockIdx.x - 1, gridDim.x - 1);
+}
+
+// ----------------------------------------------------------------------- tiles
+struct LogitArgs {
+    EntropyOperand w, x;       // rows: vocabulary, features
+    uint32_t pairs = 1, slabs = 0;
+    uint32_t tiles_m = 0, tiles_n = 0;
+    uint32_t first = 0;        // vocabulary of w's first row
+    uint32_t vocab = 0, rows = 0;
+    RowData row{};
+    float2 *partial = nullptr; // [tile of the vocabulary][partial_ld], the loss
+    uint32_t partial_ld = 0, partial_first = 0;
+    uint16_t *grad = nullptr;  // [row][grad_ld], the gradient, and its parts
+    uint64_t grad_plane = 0;
+    uint32_t grad_ld = 0;
+    float boost = 1.0f;
+    NodeGate gate{nullptr, 0};
+};
+
+// Vocabulary down, rows across: a lane holds 16 SM logits of each of its SN rows.
+template <typename S, class Cfg, bool GRAD> __global__ __launch_bounds__(Cfg::kThreads) void k_logits(LogitArgs g)
+{
+    using E = typename ElemOf<S>::T;
+    constexpr int SM = Cfg::SM, SN = Cfg::SN, BM = Cfg::BM, BN = Cfg::BN;
+    extern __shared__ __align__(16) char lds[];
+    if (block_gate_closed(g.gate))
+        return;
+    const EntropyTile t = entropy_tile(blockIdx.x, g.tiles_m, g.tiles_n, 1);
+    const uint32_t m0 = t.tm * BM, n0 = t.tn * BN;
+    f32x16 acc[SM][SN];
+    entropy_product<E, Cfg, false, false>(g.w, g.x, g.pairs, m0, n0, 0, g.slabs, lds, acc);
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64, half = lane / 32;
+    const uint32_t wm = wave / Cfg::WN * SM * 32, wn = wave % Cfg::WN * SN * 32;
+    const uint32_t v0 = g.first + m0 + wm + 4 * half; // of acc[i][j][r]: v0 + 32 i + 8 (r / 4) + r % 4
+    if constexpr (!GRAD) {
+        float2 *red = reinterpret_cast<float2 *>(lds + Cfg::kTile);
+        const bool ragged = g.first + m0 + BM > g.vocab;
+#pragma unroll
+        for (int j = 0; j < SN; j++) {
+            const uint32_t n = n0 + wn + 32 * j + (lane & 31);
+            const int32_t label = n < g.rows ? g.row.label[n] : -1;
+            if (label >= 0 && (uint32_t)label - (g.first + m0 + wm) < SM * 32u) {
+#pragma unroll
+                for (int i = 0; i < SM; i++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        if (v0 + 32 * i + 8 * (r / 4) + r % 4 == (uint32_t)label)
+                            g.row.own[n] = acc[i][j][r];
+            }
+            if (ragged) {
+#pragma unroll
+                for (int i = 0; i < SM; i++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        if (v0 + 32 * i + 8 * (r / 4) + r % 4 >= g.vocab)
+                            acc[i][j][r] = -INFINITY;
+            }
+            float m = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < SM; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    m = fmaxf(m, acc[i][j][r]);
+            m = fmaxf(m, __shfl_xor(m, 32));
+            const float from = m == -INFINITY ? 0.0f : m;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < SM; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    sum += exp2_fast((acc[i][j][r] - from) * kLog2e);
+            sum += __shfl_xor(sum, 32);
+            if (half == 0)
+                red[wave / Cfg::WN * BN + wn + 32 * j + (lane & 31)] = make_float2(m, sum);
+        }
+        __syncthreads();
+        for (uint32_t c = threadIdx.x; c < (uint32_t)BN; c += Cfg::kThreads) {
+            float2 a = red[c];
+#pragma unroll
+            for (int k = 1; k < Cfg::WM; k++) {
+                const float2 b = red[k * BN + c];
+                const float m = fmaxf(a.x, b.x), from = m == -INFINITY ? 0.0f : m;
+                a = make_float2(m, a.y * exp2_fast((a.x - from) * kLog2e) + b.y * exp2_fast((b.x - from) * kLog2e));
+            }
+            g.partial[(uint64_t)(g.partial_first + t.tm) * g.partial_ld + n0 + c] = a;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < SN; j++) {
+            const uint32_t n = n0 + wn + 32 * j + (lane & 31);
+            const bool in = n < g.rows;
+            const int32_t label = in ? g.row.label[n] : -1;
+            const float scale = in ? g.row.scale[n] * g.boost : 0.0f, log_sum = in ? g.row.log_sum[n] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < SM; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const uint32_t v = v0 + 32 * i + 8 * (r / 4) + r % 4;
+                    const float p = exp2_fast((acc[i][j][r] - log_sum) * kLog2e);
+                    const float d = ((int32_t)v == label ? p - 1.0f : p) * scale;
+                    acc[i][j][r] = label >= 0 && v < g.vocab ? d : 0.0f;
+                }
+        }
+        // Through LDS, so that a row's values are stored side by side.
+        uint16_t *tile = reinterpret_cast<uint16_t *>(lds);
+#pragma unroll
+        for (int part = 0; part < kParts<S>; part++) {
+            if (part)
+                __syncthreads();
+#pragma unroll
+            for (int j = 0; j < SN; j++)
+#pragma unroll
+                for (int i = 0; i < SM; i++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        uint32_t two[2];
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int e = 4 * q + 2 * h;
+                            if constexpr (kParts<S> == 1) {
+                                typedef float f32x2 __attribute__((ext_vector_type(2)));
+                                typedef S s16x2 __attribute__((ext_vector_type(2)));
+                                const f32x2 x = {acc[i][j][e], acc[i][j][e + 1]};
+                                two[h] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, s16x2));
+                            } else {
+                                // A part, and what is left for the next ones.
+                                float lo = acc[i][j][e], hi = acc[i][j][e + 1];
+                                two[h] = first_part(lo) | first_part(hi) << 16;
+                                acc[i][j][e] = lo;
+                                acc[i][j][e + 1] = hi;
+                            }
+                        }
+                        *reinterpret_cast<uint2 *>(tile + (wn + 32 * j + (lane & 31)) * Cfg::kOutPitch + wm + 32 * i + 8 * q + 4 * half) =
+                            make_uint2(two[0], two[1]);
+                    }
+            __syncthreads();
+            for (uint32_t i = threadIdx.x; i < BN * BM / 8; i += Cfg::kThreads) {
+                const uint32_t n = i / (BM / 8), c = i % (BM / 8) * 8;
+                *reinterpret_cast<u32x4 *>(g.grad + part * g.grad_plane + (uint64_t)(n0 + n) * g.grad_ld + m0 + c) =
+                    *reinterpret_cast<const u32x4 *>(tile + n * Cfg::kOutPitch + c);
+            }
+        }
+    }
+}
+
+// Each row's log-sum-exp from its tiles', and its loss: 16 rows a workgroup, 16 threads each.
+__global__ __launch_bounds__(256) void k_entropy_loss(const float2 *partial, uint32_t ld, uint32_t tiles, uint32_t rows, RowData row,
+                                                      float *loss, float *log_sum, NodeGate gate)
+{
+    __shared__ float2 red[16][16];
+    if (block_gate_closed(gate))
+        return;
+    const uint32_t c = threadIdx.x & 15, k = threadIdx.x / 16, n = blockIdx.x * 16 + c;
+    auto join = [](float2 a, float2 b) {
+        const float m = fmaxf(a.x, b.x), from = m == -INFINITY ? 0.0f : m;
+        return make_float2(m, a.y * exp2_fast((a.x - from) * kLog2e) + b.y * exp2_fast((b.x - from) * kLog2e));
+    };
+    float2 a = make_float2(-INFINITY, 0.0f);
+    if (n < rows) {
+        constexpr uint32_t U = 4;
+        for (uint32_t t = k; t < tiles; t += 16 * U) {
+            float2 b[U];
+#pragma unroll
+            for (uint32_t q = 0; q < U; q++)
+                b[q] = t + 16 * q < tiles ? partial[(uint64_t)(t + 16 * q) * ld + n] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+            for (uint32_t q = 0; q < U; q++)
+                a = join(a, b[q]);
+        }
+    }
+    red[k][c] = a;
+    __syncthreads();
+    if (k || n >= rows)
+        return;
+    for (int q = 1; q < 16; q++)
+        a = join(a, red[q][c]);
+    const float from = a.x == -INFINITY ? 0.0f : a.x;
+    // A NaN among the logits is not in the maximum, but in the sum.
+    const float l = (float)((double)from + (double)__builtin_amdgcn_logf(a.y) * kLn2);
+    row.log_sum[n] = l;
+    if (log_sum)
+        log_sum[n] = l;
+    if (loss)
+        loss[n] = row.label[n] >= 0 ? l - row.own[n] : 0.0f;
+}
+
+struct ProductArgs {
+    EntropyOperand a, b;
+    uint32_t pairs = 1, slabs = 0, splits = 1;
+    uint32_t tiles_m = 0, tiles_n = 0;
+    float *sums = nullptr; // [split][row][sums_ld], the features' gradient
+    uint64_t sums_split = 0;
+    uint32_t sums_ld = 0;
+    int add = 0;           // to what `sums` holds
+    const float *factor = nullptr;
+    void *out = nullptr;   // [vocabulary][out_ld], the weights' gradient
+    uint64_t out_ld = 0;
+    uint32_t out_rows = 0, out_cols = 0;
+    int out_whole = 0;     // 16-byte stores are aligned and inside the rows
+    NodeGate gate{nullptr, 0};
+};
+
+// dx: width down (from the weights, k-major), rows across (G); sums in binary32, k split.
+template <typename S, class Cfg> __global__ __launch_bounds__(Cfg::kThreads) void k_feature_gradient(ProductArgs g)
+{
+    using E = typename ElemOf<S>::T;
+    constexpr int SM = Cfg::SM, SN = Cfg::SN;
+    extern __shared__ __align__(16) char lds[];
+    if (block_gate_closed(g.gate))
+        return;
+    const EntropyTile t = entropy_tile(blockIdx.x, g.tiles_m, g.tiles_n, g.splits);
+    const uint32_t m0 = t.tm * Cfg::BM, n0 = t.tn * Cfg::BN;
+    const uint32_t k_lo = (uint32_t)((uint64_t)g.slabs * t.split / g.splits), k_hi = (uint32_t)((uint64_t)g.slabs * (t.split + 1) / g.splits);
+    f32x16 acc[SM][SN];
+    entropy_product<E, Cfg, true, false>(g.a, g.b, g.pairs, m0, n0, k_lo, k_hi, lds, acc);
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    const uint32_t m = m0 + wave / Cfg::WN * SM * 32 + 4 * (lane / 32), n = n0 + wave % Cfg::WN * SN * 32 + (lane & 31);
+#pragma unroll
+    for (int j = 0; j < SN; j++)
+#pragma unroll
+        for (int i = 0; i < SM; i++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                float4 *to = reinterpret_cast<float4 *>(g.sums + t.split * g.sums_split + (uint64_t)(n + 32 * j) * g.sums_ld + m + 32 * i + 8 * q);
+                float4 v = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+                if (g.add) {
+                    const float4 o = *to;
+                    v = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+                }
+                *to = v;
+            }
+}
+
+// dx from the splits' sums, in their order.
+template <typename S>
+__global__ __launch_bounds__(256) void k_feature_join(const float *sums, uint64_t split, uint32_t splits, uint32_t ld, uint32_t rows,
+                                                      uint32_t cols, const float *factor, S *out, uint64_t out_ld, NodeGate gate)
+{
+    if (block_gate_closed(gate))
+        return;
+    constexpr int V = kVec<S>;
+    const uint32_t pieces = (cols + V - 1) / V;
+    const float f = *factor;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < (uint64_t)rows * pieces; i += (uint64_t)gridDim.x * 256) {
+        const uint32_t r = (uint32_t)(i / pieces), c = (uint32_t)(i % pieces);
+        float v[V] = {};
+        for (uint32_t s = 0; s < splits; s++) {
+            const float *from = sums + s * split + (uint64_t)r * ld + c * V;
+#pragma unroll
+            for (int q = 0; q < V; q += 4) {
+                const float4 x = *reinterpret_cast<const float4 *>(from + q);
+                v[q] += x.x;
+                v[q + 1] += x.y;
+                v[q + 2] += x.z;
+                v[q + 3] += x.w;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < V; e++)
+            v[e] *= f;
+        store_vec(out + r * out_ld, c, cols, v, false);
+    }
+}
+
+// dW: width down (from the features, k-major), vocabulary across (G, k-major).
+template <typename S, class Cfg> __global__ __launch_bounds__(Cfg::kThreads) void k_weight_gradient(ProductArgs g)
+{
+    using E = typename ElemOf<S>::T;
+    constexpr int SM = Cfg::SM, SN = Cfg::SN, BM = Cfg::BM, BN = Cfg::BN;
+    extern __shared__ __align__(16) char lds[];
+    if (block_gate_closed(g.gate))
+        return;
+    const EntropyTile t = entropy_tile(blockIdx.x, g.tiles_m, g.tiles_n, 1);
+    const uint32_t m0 = t.tm * BM, n0 = t.tn * BN;
+    f32x16 acc[SM][SN];
+    entropy_product<E, Cfg, true, true>(g.a, g.b, g.pairs, m0, n0, 0, g.slabs, lds, acc);
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    const uint32_t wm = wave / Cfg::WN * SM * 32 + 4 * (lane / 32), wn = wave % Cfg::WN * SN * 32 + (lane & 31);
+    const float f = *g.factor;
+    S *out = static_cast<S *>(g.out);
+    if constexpr (sizeof(S) == 4) {
+#pragma unroll
+        for (int j = 0; j < SN; j++) {
+            const uint32_t n = n0 + wn + 32 * j;
+            if (n >= g.out_rows)
+                continue;
+#pragma unroll
+            for (int i = 0; i < SM; i++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const uint32_t m = m0 + wm + 32 * i + 8 * q;
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        v[e] = acc[i][j][4 * q + e] * f;
+                    float *to = out + (uint64_t)n * g.out_ld + m;
+                    if (g.out_whole && m + 4 <= g.out_cols)
+                        *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
+                    else
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (m + e < g.out_cols)
+                                to[e] = v[e];
+                }
+        }
+    } else {
+        S *tile = reinterpret_cast<S *>(lds);
+#pragma unroll
+        for (int j = 0; j < SN; j++)
+#pragma unroll
+            for (int i = 0; i < SM; i++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    typedef float f32x4 __attribute__((ext_vector_type(4)));
+                    typedef S s16x4_t __attribute__((ext_vector_type(4)));
+                    f32x4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        v[e] = acc[i][j][4 * q + e] * f;
+                    *reinterpret_cast<s16x4_t *>(tile + (wn + 32 * j) * Cfg::kOutPitch + wm + 32 * i + 8 * q) =
+                        __builtin_convertvector(v, s16x4_t);
+                }
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < BN * BM / 8; i += Cfg::kThreads) {
+            const uint32_t n = i / (BM / 8), c = i % (BM / 8) * 8;
+            if (n0 + n >= g.out_rows || m0 + c >= g.out_cols)
+                continue;
+            const S *from = tile + n * Cfg::kOutPitch + c;
+            S *to = out + (uint64_t)(n0 + n) * g.out_ld + m0 + c;
+            if (g.out_whole && m0 + c + 8 <= g.out_cols)
+                *reinterpret_cast<u32x4 *>(to) = *reinterpret_cast<const u32x4 *>(from);
+            else
+                for (uint32_t e = 0; e < 8 && m0 + c + e < g.out_cols; e++)
+                    to[e] = from[e];
+        }
+    }
+}
+
+// Rows of zeros: of the weights' gradient past the vocabulary, or where there are no rows.
+template <typename S> __global__ __launch_bounds__(256) void k_zero_rows(S *out, uint64_t ld, uint64_t rows, uint32_t cols, NodeGate gate)
+{
+    if (block_gate_closed(gate))
+        return;
+    const uint32_t pieces = (cols + kVec<S> - 1) / kVec<S>;
+    const typename StatOf<S>::T zero[kVec<S>] = {};
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < rows * pieces; i += (uint64_t)gridDim.x * 256)
+        store_vec(out + i / pieces * ld, (uint32_t)(i % pieces), cols, zero, false);
+}
+
+// ---------------------------------------------------------------------- launches
+using Large = EntropyCfg<2, 4, 4, 2>;  // 256 x 256
+using Middle = EntropyCfg<2, 2, 2, 2>; // 128 x 128
+using Thin = EntropyCfg<4, 1, 2, 1>;   // 256 x 32, few rows
+
+constexpr uint64_t round_up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
+
+enum class Side { Large, Middle, Thin };
+inline uint32_t side_m(Side s) { return s == Side::Middle ? 128 : 256; }
+inline uint32_t side_n(Side s) { return s == Side::Large ? 256 : s == Side::Middle ? 128 : 32; }
+
+// 256 x 256 tiles where they fill three quarters of the CUs.
+inline Side choose(uint64_t m, uint64_t n)
+{
+    return (m + 255) / 256 * ((n + 255) / 256) * 4 >= 3 * kGfx950Cus ? Side::Large : Side::Middle;
+}
+
+// How a call goes over its vocabulary and what its scratch holds.
+struct EntropyPlan {
+    bool grads, pack_weights, keep_weights;
+    uint32_t parts, ld;    // of packed rows
+    uint64_t rows_up;      // rows with padding
+    uint64_t piece;        // vocabulary of a piece, a multiple of 256
+    Side logits, features, weights;
+    uint32_t splits, sums_ld;
+    uint64_t x, w, partial, grad, sums, label, scale, log_sum, own, factor, bytes;
+
+    explicit EntropyPlan(const EntropyArgs &g)
+    {
+        grads = g.feature_gradient || g.weight_gradient;
+        parts = g.dtype == kLogitF32 ? 3 : 1;
+        ld = (uint32_t)round_up(g.width, kSlabK);
+        rows_up = round_up(g.rows, 256);
+        // 16-bit weights are read in place where direct loads can: whole slabs, 16-byte pieces, and a
+        // tile's rows within 32-bit offsets.
+        pack_weights = parts == 3 || g.width % kSlabK || g.weight_stride % 8 || ((uintptr_t)g.weights & 15) ||
+                       g.weight_stride * 2 * 256 > UINT32_MAX;
+        const uint64_t vocab_up = round_up(g.vocab, 256);
+        const uint64_t row_bytes = 2ull * parts * ld;
+        // G's piece is what the 256 MiB cache behind the L2s can hold; packed weights are kept
+        // for the second pass where they are no more than 512 MiB.
+        constexpr uint64_t kGradBytes = 192ull << 20, kWeightBytes = 512ull << 20;
+        piece = kGradBytes / (rows_up ? rows_up * 2 * parts : 1) / 256 * 256;
+        piece = piece < 256 ? 256 : piece > vocab_up ? vocab_up : piece;
+        keep_weights = pack_weights && vocab_up * row_bytes <= kWeightBytes;
+        if (!grads)
+            piece = vocab_up;
+        if (pack_weights && !keep_weights) {
+            const uint64_t fit = kWeightBytes / row_bytes / 256 * 256;
+            piece = piece < fit ? piece : fit < 256 ? 256 : fit;
+        }
+        logits = g.rows <= 32 ? Side::Thin : choose(g.vocab, g.rows);
+        features = g.rows <= 32 ? Side::Thin : choose(g.width, g.rows);
+        weights = choose(g.width, piece < g.vocab ? piece : g.vocab);
+        const uint64_t tiles = ((g.width + side_m(features) - 1) / side_m(features)) * ((g.rows + side_n(features) - 1) / side_n(features));
+        const uint64_t per = features == Side::Large ? 1 : 2; // workgroups a CU
+        const uint64_t want = tiles ? (per * kGfx950Cus + tiles / 2) / tiles : 1, most = (piece + 4 * kSlabK - 1) / (4 * kSlabK);
+        splits = (uint32_t)(want < 1 ? 1 : want > most ? (most ? most : 1) : want);
+        sums_ld = (uint32_t)round_up(g.width, 256);
+        bytes = 0;
+        auto take = [&](uint64_t n) {
+            const uint64_t at = bytes;
+            bytes += round_up(n, 256);
+            return at;
+        };
+        x = take(rows_up * row_bytes);
+        w = take(pack_weights ? (keep_weights ? vocab_up : piece) * row_bytes : 0);
+        partial = take(g.log_sum_in ? 0 : (vocab_up / 128) * rows_up * 8);
+        grad = take(grads ? piece * rows_up * 2 * parts : 0);
+        sums = take(g.feature_gradient ? splits * rows_up * sums_ld * 4ull : 0);
+        label = take(g.rows * 4);
+        scale = take(g.rows * 4);
+        log_sum = take(g.rows * 4);
+        own = take(g.rows * 4);
+        factor = take(4);
+    }
+};
+
+template <typename K> hipError_t with_lds(K *kernel, uint32_t bytes)
+{
+    return bytes > 65536 ? hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes)
+                         : hipSuccess;
+}
+
+template <typename S, class Cfg, bool GRAD> hipError_t run_logits(hipStream_t s, LogitArgs a, uint64_t vocab_rows, uint64_t rows)
+{
+    a.tiles_m = (uint32_t)((vocab_rows + Cfg::BM - 1) / Cfg::BM);
+    a.tiles_n = (uint32_t)((rows + Cfg::BN - 1) / Cfg::BN);
+    hipError_t e = with_lds(k_logits<S, Cfg, GRAD>, Cfg::kLds);
+    if (e)
+        return e;
+    hipLaunchKernelGGL((k_logits<S, Cfg, GRAD>), dim3(a.tiles_m * a.tiles_n), dim3(Cfg::kThreads), Cfg::kLds, s, a);
+    return hipGetLastError();
+}
+template <typename S, bool GRAD> hipError_t logits_by(Side side, hipStream_t s, const LogitArgs &a, uint64_t vocab_rows, uint64_t rows)
+{
+    switch (side) {
+    case Side::Large: return run_logits<S, Large, GRAD>(s, a, vocab_rows, rows);
+    case Side::Middle: return run_logits<S, Middle, GRAD>(s, a, vocab_rows, rows);
+    default: return run_logits<S, Thin, GRAD>(s, a, vocab_rows, rows);
+    }
+}
+
+template <typename S, class Cfg> hipError_t run_features(hipStream_t s, ProductArgs a, uint64_t width, uint64_t rows)
+{
+    a.tiles_m = (uint32_t)((width + Cfg::BM - 1) / Cfg::BM);
+    a.tiles_n = (uint32_t)((rows + Cfg::BN - 1) / Cfg::BN);
+    hipError_t e = with_lds(k_feature_gradient<S, Cfg>, Cfg::kLds);
+    if (e)
+        return e;
+    hipLaunchKernelGGL((k_feature_gradient<S, Cfg>), dim3(a.tiles_m * a.tiles_n * a.splits), dim3(Cfg::kThreads), Cfg::kLds, s, a);
+    return hipGetLastError();
+}
+template <typename S, class Cfg> hipError_t run_weights(hipStream_t s, ProductArgs a, uint64_t width, uint64_t vocab_rows)
+{
+    a.tiles_m = (uint32_t)((width + Cfg::BM - 1) / Cfg::BM);
+    a.tiles_n = (uint32_t)((vocab_rows + Cfg::BN - 1) / Cfg::BN);
+    hipError_t e = with_lds(k_weight_gradient<S, Cfg>, Cfg::kLds);
+    if (e)
+        return e;
+    hipLaunchKernelGGL((k_weight_gradient<S, Cfg>), dim3(a.tiles_m * a.tiles_n), dim3(Cfg::kThreads), Cfg::kLds, s, a);
+    return hipGetLastError();
+}
+
+inline unsigned pack_blocks(uint64_t rows, uint64_t ld)
+{
+    const uint64_t n = (rows * (ld / 8) + 255) / 256;
+    return (unsigned)(n < 1 ? 1 : n > 8192 ? 8192 : n);
+}
+
+template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyArgs &g, void *scratch)
+{
+    const EntropyPlan p(g);
+    char *sc = static_cast<char *>(scratch);
+    const RowData row{reinterpret_cast<int32_t *>(sc + p.label), reinterpret_cast<float *>(sc + p.scale),
+                      g.log_sum_in ? const_cast<float *>(g.log_sum_in) : reinterpret_cast<float *>(sc + p.log_sum),
+                      reinterpret_cast<float *>(sc + p.own), reinterpret_cast<float *>(sc + p.factor)};
+    hipError_t e;
+    const bool whole_pass = !g.log_sum_in;
+    const uint32_t pairs = p.parts == 3 ? kPartPairs : 1, slabs = p.ld / kSlabK;
+
+    PackArgs px;
+    px.in = g.features;
+    px.ld = g.feature_stride;
+    px.rows = (uint32_t)g.rows;
+    px.cols = g.width;
+    px.labels = p.grads ? g.labels : nullptr; // rows without a label reach no gradient
+    px.vocab = g.vocab;
+    px.out = reinterpret_cast<uint16_t *>(sc + p.x);
+    px.plane = p.rows_up * p.ld;
+    px.out_rows = (uint32_t)p.rows_up;
+    px.out_ld = p.ld;
+    px.gate = g.gate;
+    PrepArgs pp;
+    pp.labels = g.labels;
+    pp.row_scale = g.row_scale;
+    pp.rows = (uint32_t)g.rows;
+    pp.vocab = g.vocab;
+    pp.boost = kBoost<S>;
+    pp.row = row;
+    pp.fault = g.fault;
+    if (g.rows) {
+        hipLaunchKernelGGL((k_entropy_open<S>), dim3(1 + pack_blocks(p.rows_up, p.ld)), dim3(256), 0, s, px, pp);
+        if ((e = hipGetLastError()))
+            return e;
+    }
+
+    const EntropyOperand x{px.out, px.plane, p.ld, (uint32_t)p.rows_up, p.ld};
+    // The weights of vocabulary [v, v + n), packed by this call where they have to be.
+    auto weights = [&](uint64_t v, uint64_t n, bool packed, EntropyOperand *o) {
+        const S *from = static_cast<const S *>(g.weights) + v * g.weight_stride;
+        if (!p.pack_weights) {
+            *o = EntropyOperand{reinterpret_cast<const uint16_t *>(from), 0, (uint32_t)g.weight_stride, (uint32_t)n, g.width};
+            return hipSuccess;
+        }
+        uint16_t *to = reinterpret_cast<uint16_t *>(sc + p.w) + (p.keep_weights ? v * p.ld : 0);
+        const uint64_t plane = (p.keep_weights ? round_up(g.vocab, 256) : p.piece) * p.ld;
+        *o = EntropyOperand{to, plane, p.ld, (uint32_t)n, p.ld};
+        if (packed)
+            return hipSuccess;
+        PackArgs pw;
+        pw.in = from;
+        pw.ld = g.weight_stride;
+        pw.rows = pw.out_rows = (uint32_t)n;
+        pw.cols = g.width;
+        pw.out = to;
+        pw.plane = plane;
+        pw.out_ld = p.ld;
+        pw.gate = g.gate;
+        hipLaunchKernelGGL((k_pack<S>), dim3(pack_blocks(n, p.ld)), dim3(256), 0, s, pw);
+        return hipGetLastError();
+    };
+
+    LogitArgs l;
+    l.x = x;
+    l.pairs = pairs;
+    l.slabs = slabs;
+    l.vocab = g.vocab;
+    l.rows = (uint32_t)g.rows;
+    l.row = row;
+    l.partial = reinterpret_cast<float2 *>(sc + p.partial);
+    l.partial_ld = (uint32_t)p.rows_up;
+    l.grad = reinterpret_cast<uint16_t *>(sc + p.grad);
+    l.grad_plane = p.rows_up * p.piece;
+    l.grad_ld = (uint32_t)p.piece;
+    l.boost = kBoost<S>;
+    l.gate = g.gate;
+    if (whole_pass && g.rows) {
+        // Weights that need not be packed, or all fit when they are, take one launch.
+        const uint64_t step = !p.pack_weights || p.keep_weights ? round_up(g.vocab, 256) : p.piece;
+        uint32_t tiles = 0;
+        for (uint64_t v = 0; v < g.vocab; v += step) {
+            const uint64_t n = g.vocab - v < step ? g.vocab - v : step;
+            if ((e = weights(v, n, false, &l.w)))
+                return e;
+            l.first = (uint32_t)v;
+            l.partial_first = tiles;
+            if ((e = logits_by<S, false>(p.logits, s, l, n, g.rows)))
+                return e;
+            tiles += (uint32_t)((n + side_m(p.logits) - 1) / side_m(p.logits));
+        }
+        hipLaunchKernelGGL(k_entropy_loss, dim3((unsigned)((g.rows + 15) / 16)), dim3(256), 0, s, l.partial, l.partial_ld, tiles,
+                           (uint32_t)g.rows, row, g.loss, g.log_sum_out, g.gate);
+        if ((e = hipGetLastError()))
+            return e;
+    }
+    if (!p.grads)
+        return hipSuccess;
+
+    ProductArgs f;
+    f.pairs = pairs;
+    f.sums = reinterpret_cast<float *>(sc + p.sums);
+    f.sums_split = p.rows_up * p.sums_ld;
+    f.sums_ld = p.sums_ld;
+    f.splits = p.splits;
+    f.gate = g.gate;
+    ProductArgs d;
+    d.pairs = pairs;
+    d.a = EntropyOperand{x.p, x.plane, x.ld, (uint32_t)round_up(g.rows, kSlabK), x.ld};
+    d.slabs = (uint32_t)((g.rows + kSlabK - 1) / kSlabK);
+    d.factor = row.factor;
+    d.out_ld = g.weight_gradient_stride;
+    d.out_cols = g.width;
+    constexpr uint32_t kStoreVec = 16 / sizeof(S);
+    d.out_whole = !((uintptr_t)g.weight_gradient & 15) && g.weight_gradient_stride % kStoreVec == 0;
+    d.gate = g.gate;
+    const uint64_t vocab = g.rows ? g.vocab : 0;
+    for (uint64_t v = 0; v < vocab; v += p.piece) {
+        const uint64_t n = vocab - v < p.piece ? vocab - v : p.piece;
+        if ((e = weights(v, n, p.keep_weights && whole_pass, &l.w)))
+            return e;
+        l.first = (uint32_t)v;
+        // Rows up to a whole slab: the weights' gradient reads those.
+        if ((e = logits_by<S, true>(p.logits, s, l, n, round_up(g.rows, kSlabK))))
+            return e;
+        if (g.feature_gradient) {
+            f.a = l.w;
+            f.b = EntropyOperand{l.grad, l.grad_plane, l.grad_ld, (uint32_t)p.rows_up, l.grad_ld};
+            f.slabs = (uint32_t)((n + kSlabK - 1) / kSlabK);
+            f.add = v > 0;
+            e = p.features == Side::Large    ? run_features<S, Large>(s, f, g.width, g.rows)
+                : p.features == Side::Middle ? run_features<S, Middle>(s, f, g.width, g.rows)
+                                             : run_features<S, Thin>(s, f, g.width, g.rows);
+            if (e)
+                return e;
+        }
+        if (g.weight_gradient) {
+            d.b = EntropyOperand{l.grad, l.grad_plane, l.grad_ld, d.a.rows, l.grad_ld};
+            d.out = static_cast<S *>(g.weight_gradient) + v * g.weight_gradient_stride;
+            d.out_rows = (uint32_t)n;
+            e = p.weights == Side::Large ? run_weights<S, Large>(s, d, g.width, n) : run_weights<S, Middle>(s, d, g.width, n);
+            if (e)
+                return e;
+        }
+    }
+    if (g.feature_gradient && g.rows) {
+        const uint64_t n = (g.rows * ((g.width + kVec<S> - 1) / kVec<S>) + 255) / 256;
+        hipLaunchKernelGGL((k_feature_join<S>), dim3((unsigned)(n > 8192 ? 8192 : n)), dim3(256), 0, s, f.sums, f.sums_split,
+                           vocab ? p.splits : 0, f.sums_ld, (uint32_t)g.rows, g.width, row.factor, static_cast<S *>(g.feature_gradient),
+                           g.feature_gradient_stride, g.gate);
+        if ((e = hipGetLastError()))
+            return e;
+    }
+    if (g.weight_gradient && g.weight_gradient_rows > vocab) {
+        const uint64_t rows = g.weight_gradient_rows - vocab, n = (rows * ((g.width + kVec<S> - 1) / kVec<S>) + 255) / 256;
+        hipLaunchKernelGGL((k_zero_rows<S>), dim3((unsigned)(n > 8192 ? 8192 : n)), dim3(256), 0, s,
+                           static_cast<S *>(g.weight_gradient) + vocab * g.weight_gradient_stride, g.weight_gradient_stride, rows,
+                           g.width, g.gate);
+        return hipGetLastError();
+    }
+    return hipSuccess;
+}
+
+} // namespace
+
+size_t entropy_scratch_bytes(const EntropyArgs &g) { return EntropyPlan(g).bytes; }
+
+hipError_t launch_entropy(hipStream_t s, const EntropyArgs &g, void *scratch)
+{
+    switch (g.dtype) {
+    case kLogitF32: return launch_entropy_t<float>(s, g, scratch);
+    case kLogitBf16: return launch_entropy_t<__bf16>(s, g, scratch);
+    default: return launch_entropy_t<_Float16>(s, g, scratch);
+    }
+}
+
+} // namespace pcu

@@ -275,6 +275,75 @@ pcu_status Ctx::op_layer_norm_backward(const pcu_rows *x, const void *stats, con
     return st;
 }
 
+pcu_status Ctx::op_cross_entropy(const pcu_rows *features, const pcu_rows *weights, bool loss, EntropyArgs g)
+{
+    pcu_status st = check_rows(this, "cross_entropy: features", features);
+    if (st || (st = check_rows(this, "cross_entropy: weights", weights)))
+        return st;
+    if (features->dtype != weights->dtype) {
+        fail("cross_entropy: features and weights of different types");
+        return PCU_ERR_ARGUMENT;
+    }
+    if (features->dtype == PCU_F64) {
+        fail("cross_entropy: F64 features are not admitted");
+        return PCU_ERR_UNSUPPORTED;
+    }
+    const uint64_t rows = features->rows, width = features->cols, size = logit_size(features->dtype);
+    if (width != weights->cols || width < 1 || width > PCU_ENTROPY_MAX_WIDTH || rows > PCU_ENTROPY_MAX_ROWS ||
+        weights->rows > PCU_TABLE_MAX_ROWS) {
+        fail("cross_entropy: %llu x %llu features, %llu x %llu weights", (unsigned long long)rows, (unsigned long long)width,
+             (unsigned long long)weights->rows, (unsigned long long)weights->cols);
+        return PCU_ERR_SHAPE;
+    }
+    if (g.weight_gradient && (g.weight_gradient_rows < weights->rows || g.weight_gradient_rows > PCU_TABLE_MAX_ROWS)) {
+        fail("cross_entropy: a gradient of %llu rows for %llu", (unsigned long long)g.weight_gradient_rows,
+             (unsigned long long)weights->rows);
+        return PCU_ERR_SHAPE;
+    }
+    if ((g.feature_gradient && (st = check_like(this, "cross_entropy: feature gradient", g.feature_gradient, rows, width,
+                                                g.feature_gradient_stride, size))) ||
+        (g.weight_gradient && (st = check_like(this, "cross_entropy: weight gradient", g.weight_gradient, g.weight_gradient_rows,
+                                               width, g.weight_gradient_stride, size))))
+        return st;
+    if ((rows && (!g.labels || (loss ? !g.loss : !g.log_sum_in))) || !aligned(g.labels, 4) || !aligned(g.log_sum_in, 4) ||
+        !aligned(g.row_scale, 4) || !aligned(g.loss, 4) || !aligned(g.log_sum_out, 4)) {
+        fail("cross_entropy: invalid argument");
+        return PCU_ERR_ARGUMENT;
+    }
+    const Range x = rows_range(*features), w = rows_range(*weights), labels{g.labels, rows * 4}, sums{g.log_sum_in, rows * 4},
+        scale{g.row_scale, rows * 4};
+    const Range l{g.loss, rows * 4}, ls{g.log_sum_out, rows * 4},
+        dx{g.feature_gradient, strided_bytes(rows, width, g.feature_gradient_stride, size)},
+        dw{g.weight_gradient, strided_bytes(g.weight_gradient_rows, width, g.weight_gradient_stride, size)};
+    if (overlaps_any(l, {x, w, labels, sums, scale, ls, dx, dw}) || overlaps_any(ls, {x, w, labels, sums, scale, dx, dw}) ||
+        overlaps_any(dx, {x, w, labels, sums, scale, dw}) || overlaps_any(dw, {x, w, labels, sums, scale})) {
+        fail("cross_entropy: an output overlaps another tensor");
+        return PCU_ERR_ARGUMENT;
+    }
+    unsigned long long *word;
+    if ((st = add_node(NodeInfo{Prim::Checked, rows, 0}, &word)))
+        return st;
+    g.features = features->data;
+    g.dtype = (int)features->dtype;
+    g.rows = rows;
+    g.feature_stride = features->stride;
+    g.width = (uint32_t)width;
+    g.vocab = (uint32_t)weights->rows;
+    g.weights = weights->data;
+    g.weight_stride = weights->stride;
+    g.fault = word;
+    g.gate = gate_for(word);
+    void *sc = nullptr;
+    if ((st = scratch(layer_scratch, entropy_scratch_bytes(g), false, &sc)))
+        return st;
+    if ((st = open_words()))
+        return st;
+    hipEvent_t t = timer_start(stream);
+    st = hip(launch_entropy(stream, g, sc), "cross_entropy launch");
+    timer_stop(PCU_KERNEL_CROSS_ENTROPY, t, stream);
+    return st;
+}
+
 } // namespace pcu
 
 using pcu::Ctx;
@@ -324,6 +393,62 @@ pcu_status pcu_native_layer_norm_backward(pcu_ctx *ctx, const pcu_rows *x, const
         return st;
     return c->finish_op(c->op_layer_norm_backward(x, stats, gradient, gradient_stride, weight, (int)weight_dtype, x_gradient,
                                                   x_gradient_stride, weight_gradient, bias_gradient), nullptr);
+}
+
+pcu_status pcu_native_cross_entropy_loss(pcu_ctx *ctx, const pcu_rows *features, const pcu_rows *weights,
+                                         const int32_t *labels, float *loss, float *log_sum, pcu_fault *fault)
+{
+    pcu_status st;
+    Ctx *c = pcu::enter(ctx, &st);
+    if (!c)
+        return st;
+    pcu::EntropyArgs g;
+    g.labels = labels;
+    g.loss = loss;
+    g.log_sum_out = log_sum;
+    return c->finish_op(c->op_cross_entropy(features, weights, true, g), fault);
+}
+
+pcu_status pcu_native_cross_entropy_backward(pcu_ctx *ctx, const pcu_rows *features, const pcu_rows *weights,
+                                             const int32_t *labels, const float *log_sum, const float *row_scale,
+                                             void *feature_gradient, uint64_t feature_gradient_stride, void *weight_gradient,
+                                             uint64_t weight_gradient_rows, uint64_t weight_gradient_stride, pcu_fault *fault)
+{
+    pcu_status st;
+    Ctx *c = pcu::enter(ctx, &st);
+    if (!c)
+        return st;
+    pcu::EntropyArgs g;
+    g.labels = labels;
+    g.log_sum_in = log_sum;
+    g.row_scale = row_scale;
+    g.feature_gradient = feature_gradient;
+    g.feature_gradient_stride = feature_gradient_stride;
+    g.weight_gradient = weight_gradient;
+    g.weight_gradient_rows = weight_gradient_rows;
+    g.weight_gradient_stride = weight_gradient_stride;
+    return c->finish_op(c->op_cross_entropy(features, weights, false, g), fault);
+}
+
+pcu_status pcu_native_cross_entropy_step(pcu_ctx *ctx, const pcu_rows *features, const pcu_rows *weights,
+                                         const int32_t *labels, const float *row_scale, float *loss, void *feature_gradient,
+                                         uint64_t feature_gradient_stride, void *weight_gradient, uint64_t weight_gradient_rows,
+                                         uint64_t weight_gradient_stride, pcu_fault *fault)
+{
+    pcu_status st;
+    Ctx *c = pcu::enter(ctx, &st);
+    if (!c)
+        return st;
+    pcu::EntropyArgs g;
+    g.labels = labels;
+    g.row_scale = row_scale;
+    g.loss = loss;
+    g.feature_gradient = feature_gradient;
+    g.feature_gradient_stride = feature_gradient_stride;
+    g.weight_gradient = weight_gradient;
+    g.weight_gradient_rows = weight_gradient_rows;
+    g.weight_gradient_stride = weight_gradient_stride;
+    return c->finish_op(c->op_cross_entropy(features, weights, true, g), fault);
 }
 
 } // extern "C"

@@ -237,6 +237,8 @@ struct Ctx {
                                       uint64_t gradient_stride, const void *weight, int weight_dtype,
                                       void *x_gradient, uint64_t x_gradient_stride, void *weight_gradient,
                                       void *bias_gradient);
+    // `g` carries the call's pointers, sizes and strides; the rest is filled in.
+    pcu_status op_cross_entropy(const pcu_rows *features, const pcu_rows *weights, bool loss, EntropyArgs g);
 };
 
 } // namespace pcu

@@ -394,6 +394,40 @@ pcu_status pcu_native_layer_norm_backward(pcu_ctx *ctx, const pcu_rows *x, const
                                           void *x_gradient, uint64_t x_gradient_stride,
                                           void *weight_gradient, void *bias_gradient);
 
+/* The cross entropy of an output layer whose logits l = features * weights^T (one row of weights a
+ * token, as a table of embeddings) are in no array. Features and weights are of one type, F32, BF16
+ * or F16 (F64: PCU_ERR_UNSUPPORTED; a product and pcu_native_distill_step with k = 0 do that).
+ *   log_sum[r] = log(sum exp l_r), loss[r] = log_sum[r] - l[r][labels[r]]
+ *   G[r][v] = row_scale[r] (exp(l[r][v] - log_sum[r]) - [v = labels[r]])
+ *   feature_gradient = G * weights, weight_gradient = G^T * features
+ * A row with a negative label has loss 0 and reaches no gradient, whatever its features hold; one of
+ * weights.rows or more is a fault (element_index: the row). loss, log_sum and row_scale (NULL: 1)
+ * are F32. Sums are F32; F32 operands enter with 24 bits; G is rounded to the operands' precision, which
+ * for F16 holds what is above 2^-38 of the largest row_scale. */
+#define PCU_ENTROPY_MAX_ROWS (1u << 22)
+#define PCU_ENTROPY_MAX_WIDTH (1u << 16) /* and at least 1 */
+/* log_sum may be NULL. */
+pcu_status pcu_native_cross_entropy_loss(pcu_ctx *ctx, const pcu_rows *features,
+                                         const pcu_rows *weights, const int32_t *labels,
+                                         float *loss, float *log_sum, pcu_fault *fault);
+/* The gradients from the log_sum of the loss. Either may be NULL. feature_gradient: rows of the
+ * features' type. weight_gradient: weight_gradient_rows >= weights.rows rows of that type, zeros past
+ * the vocabulary. */
+pcu_status pcu_native_cross_entropy_backward(pcu_ctx *ctx, const pcu_rows *features,
+                                             const pcu_rows *weights, const int32_t *labels,
+                                             const float *log_sum, const float *row_scale,
+                                             void *feature_gradient,
+                                             uint64_t feature_gradient_stride,
+                                             void *weight_gradient, uint64_t weight_gradient_rows,
+                                             uint64_t weight_gradient_stride, pcu_fault *fault);
+/* Loss and gradients at once. */
+pcu_status pcu_native_cross_entropy_step(pcu_ctx *ctx, const pcu_rows *features,
+                                         const pcu_rows *weights, const int32_t *labels,
+                                         const float *row_scale, float *loss,
+                                         void *feature_gradient, uint64_t feature_gradient_stride,
+                                         void *weight_gradient, uint64_t weight_gradient_rows,
+                                         uint64_t weight_gradient_stride, pcu_fault *fault);
+
 /* ------------------------------------------------------------------ program
  * Between begin and end every op call is only enqueued and numbered as a node (0, 1, ...;
  * pcu_checked_add_relu takes two numbers). pcu_program_end synchronizes once and reports
