@@ -101,7 +101,7 @@ template <typename S> hipError_t launch_embed_t(hipStream_t s, const EmbedArgs &
 // Two stable counting passes over half of the key's bits each (at most 12). A tile of keys is
 // ranked by one workgroup: its waves take consecutive runs of it, 64 keys at a time, and lanes with
 // equal digits find each other by one ballot for each bit.
-constexpr int kSortTile = 4096, kSortThreads = 512, kSortRounds = kSortTile / kSortThreads;
+constexpr int kSortTile = 2048, kSortThreads = 512, kSortRounds = kSortTile / kSortThreads;
 constexpr int kSortWaves = kSortThreads / 64;
 
 __device__ __forceinline__ uint32_t token_key(const int32_t *tokens, uint64_t i, uint32_t vocab)
@@ -360,8 +360,8 @@ __device__ __forceinline__ Run run_of(const uint32_t *keys, uint32_t n, uint32_t
 }
 
 // sum += terms [lo, hi) of the sorted order, vector v of each, one after another.
-template <typename S, typename T>
-__device__ __forceinline__ void add_terms(const EmbedBackArgs &g, const uint32_t *places, uint32_t lo, uint32_t hi, uint32_t v,
+template <typename S, typename P, typename T>
+__device__ __forceinline__ void add_terms(const EmbedBackArgs &g, const P *places, uint32_t lo, uint32_t hi, uint32_t v,
                                           T (&sum)[kVec<S>])
 {
     constexpr int U = 8;
@@ -383,25 +383,234 @@ __device__ __forceinline__ void add_terms(const EmbedBackArgs &g, const uint32_t
     }
 }
 
+// Row `row`, vector v: base (raw; zeros without one) plus scale times `sum`.
 template <typename S, typename T>
-__device__ __forceinline__ void write_sum(const EmbedBackArgs &g, uint32_t row, uint32_t v, bool any, const T (&sum)[kVec<S>])
+__device__ __forceinline__ void write_sum(const EmbedBackArgs &g, uint32_t row, uint32_t v, const u32x4 &base, const T (&sum)[kVec<S>],
+                                          bool through = false)
 {
     const T scale = (T)g.scale;
     T y[kVec<S>];
-    S *out = static_cast<S *>(g.out) + (uint64_t)row * g.out_stride;
     if (g.base) {
-        if (!any && g.base == g.out)
-            return; // the row keeps what it holds
-        unpack<S>(load_vec(static_cast<const S *>(g.base) + (uint64_t)row * g.base_stride, v, g.width), y);
+        unpack<S>(base, y);
 #pragma unroll
         for (int e = 0; e < kVec<S>; e++)
-            y[e] = any ? y[e] + scale * sum[e] : y[e];
+            y[e] += scale * sum[e];
     } else {
 #pragma unroll
         for (int e = 0; e < kVec<S>; e++)
-            y[e] = any ? scale * sum[e] : (T)0;
+            y[e] = scale * sum[e];
     }
-    store_vec(out, v, g.width, y, false);
+    S *out = static_cast<S *>(g.out) + (uint64_t)row * g.out_stride;
+    if (through)
+        store_row(out, v, g.width, y, true);
+    else
+        store_vec(out, v, g.width, y, g.past);
+}
+template <typename S> __device__ __forceinline__ u32x4 load_base(const EmbedBackArgs &g, uint32_t row, uint32_t v)
+{
+    return g.base ? load_vec(static_cast<const S *>(g.base) + (uint64_t)row * g.base_stride, v, g.width) : u32x4{0, 0, 0, 0};
+}
+
+// Rows row0 + [0, rows) of the table by a wave, rows <= 16, but those of more than kLong terms; lane r
+// holds from, row r's first term (and lane `rows` the end), and term(j) gives a term's place. All
+// control is scalar: rows without terms keep their base; the others' terms are walked across the rows'
+// ends, so that their loads, and the bases' with them, are under way together. vec: the lane's vector.
+template <typename S, bool BASE, typename Term>
+__device__ __forceinline__ void wave_rows(const EmbedBackArgs &g, uint32_t row0, uint32_t rows, uint32_t from, uint32_t vec, bool on,
+                                          Term term)
+{
+    using T = typename StatOf<S>::T;
+    constexpr int U = BASE ? 4 : 8, V = kVec<S>;
+    const uint32_t lane = threadIdx.x & 63, next = __shfl(from, lane + 1);
+    const uint32_t all = (1u << rows) - 1;
+    uint32_t empty = (uint32_t)__ballot(lane < rows && from == next) & all;
+    const uint32_t many = (uint32_t)__ballot(lane < rows && next - from > kLong) & all;
+    if (!BASE) {
+        const T zero[V] = {};
+        for (; empty; empty &= empty - 1)
+            if (on)
+                store_vec(static_cast<S *>(g.out) + (uint64_t)(row0 + __builtin_ctz(empty)) * g.out_stride, vec, g.width, zero, g.past);
+    } else if (g.base != g.out) {
+        while (empty) {
+            u32x4 raw[U];
+            uint32_t e = empty;
+#pragma unroll
+            for (int q = 0; q < U; q++, e &= e - 1)
+                if (e && on)
+                    raw[q] = load_base<S>(g, row0 + __builtin_ctz(e), vec);
+#pragma unroll
+            for (int q = 0; q < U; q++, empty &= empty - 1)
+                if (empty && on) {
+                    T y[V];
+                    unpack<S>(raw[q], y);
+                    store_vec(static_cast<S *>(g.out) + (uint64_t)(row0 + __builtin_ctz(empty)) * g.out_stride, vec, g.width, y, g.past);
+                }
+        }
+    }
+    T sum[V] = {};
+    for (uint32_t r = 0; r < rows;) {
+        // Rows [r, r_end) are not long.
+        const uint32_t rest = many >> r, r_end = rest ? r + __builtin_ctz(rest) : rows;
+        const uint32_t hi = from_lane(from, r_end);
+        for (uint32_t j0 = from_lane(from, r); j0 < hi; j0 += 64) {
+            const uint32_t n = min(hi - j0, 64u), place = lane < n ? term(j0 + lane) : 0;
+            for (uint32_t j = 0; j < n; j += U) {
+                u32x4 raw[U], base[U];
+                uint32_t row[U];
+#pragma unroll
+                for (int q = 0; q < U; q++) {
+                    row[q] = ~0u;
+                    if (j + q < n) {
+                        while (from_lane(next, r) <= j0 + j + q)
+                            r++;
+                        if (on)
+                            raw[q] = load_vec(static_cast<const S *>(g.gradient) + (uint64_t)from_lane(place, j + q) * g.gradient_stride, vec, g.width);
+                        if (from_lane(next, r) == j0 + j + q + 1) { // the row's last one
+                            row[q] = row0 + r;
+                            if (BASE && on)
+                                base[q] = load_base<S>(g, row[q], vec);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < U; q++)
+                    if (j + q < n) {
+                        T x[V];
+                        unpack<S>(raw[q], x);
+#pragma unroll
+                        for (int e = 0; e < V; e++)
+                            sum[e] += x[e];
+                        if (row[q] != ~0u) {
+                            if (on)
+                                write_sum<S>(g, row[q], vec, base[q], sum);
+#pragma unroll
+                            for (int e = 0; e < V; e++)
+                                sum[e] = 0;
+                        }
+                    }
+            }
+        }
+        r = r_end + 1;
+    }
+}
+
+// The same for rows of fewer than 64 vectors: `lanes` lanes a row, one row after another for each
+// group of lanes. from: in LDS.
+template <typename S, typename P>
+__device__ __forceinline__ void narrow_rows(const EmbedBackArgs &g, const P *places, const uint32_t *from, uint32_t row0, uint32_t rows,
+                                            int lanes, uint32_t vecs)
+{
+    using T = typename StatOf<S>::T;
+    const uint32_t lane = threadIdx.x & 63, v = lane & (lanes - 1);
+    for (uint32_t r = lane / lanes; r < rows; r += 64 / lanes) {
+        const uint32_t lo = from[r], hi = from[r + 1];
+        if (v >= vecs || hi - lo > kLong || (lo == hi && g.base && g.base == g.out))
+            continue;
+        const u32x4 base = load_base<S>(g, row0 + r, v);
+        T sum[kVec<S>] = {};
+        add_terms<S>(g, places, lo, hi, v, sum);
+        if (lo == hi) {
+            unpack<S>(base, sum);
+            store_vec(static_cast<S *>(g.out) + (uint64_t)(row0 + r) * g.out_stride, v, g.width, sum, g.past);
+        } else {
+            write_sum<S>(g, row0 + r, v, base, sum);
+        }
+    }
+}
+
+// A few tokens: no sort, one launch. Its first workgroups (`sums` of them) add up the rows of every
+// token that occurs for the first time: a wave takes a token and 64 vectors of the row, and finds the
+// token's other places by looking all of them over. The others fill the rest of the table's gradient with
+// zeros or its base, `each` vectors side by side; they leave out the rows that occur. 511 tokens,
+// 50257 x 768 F32: as two launches, all rows filled and then some written again, 22 and 10 us (a plain
+// fill of the 154 MB takes 22.6, past the caches 27); waves that looked for the tokens of 16 rows each
+// took 41 to 46, and sorting first 55 in three launches.
+constexpr uint32_t kDirect = 1024, kRowsAWave = 16, kFillBlocks = 8 * kGfx950Cus;
+constexpr uint32_t kFillRows = (1u << 22) / kFillBlocks + 2; // rows that a workgroup's vectors can lie in
+
+template <typename S> __device__ __forceinline__ void fill_rows(const EmbedBackArgs &g, uint32_t block, uint64_t each, bool through)
+{
+    __shared__ uint32_t occurs[(kFillRows + 31) / 32];
+    const uint32_t n = (uint32_t)g.rows, vecs = (g.width + kVec<S> - 1) / kVec<S>;
+    const uint64_t lo = block * each, hi = min(lo + each, (uint64_t)g.vocab * vecs);
+    const uint32_t row0 = (uint32_t)(lo / vecs);
+    for (uint32_t w = threadIdx.x; w < (kFillRows + 31) / 32; w += 256)
+        occurs[w] = 0;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n; i += 256) {
+        const int32_t t = g.tokens[i];
+        if (t >= 0 && (uint32_t)t - row0 < kFillRows)
+            atomicOr(&occurs[((uint32_t)t - row0) / 32], 1u << (((uint32_t)t - row0) & 31));
+    }
+    __syncthreads();
+    for (uint64_t i = lo + threadIdx.x; i < hi; i += 256) {
+        const uint32_t row = (uint32_t)(i / vecs), v = (uint32_t)(i % vecs);
+        if (occurs[(row - row0) / 32] >> ((row - row0) & 31) & 1)
+            continue;
+        typename StatOf<S>::T y[kVec<S>];
+        unpack<S>(load_base<S>(g, row, v), y);
+        store_row(static_cast<S *>(g.out) + (uint64_t)row * g.out_stride, v, g.width, y, through);
+    }
+}
+
+template <typename S>
+__global__ __launch_bounds__(256) void k_embed_first(EmbedBackArgs g, uint32_t across, uint32_t sums, uint64_t each, ProgramClose close)
+{
+    using T = typename StatOf<S>::T;
+    constexpr int V = kVec<S>, N = kDirect / 64, U = 8;
+    if (block_gate_closed(g.gate))
+        return;
+    if (blockIdx.x >= sums) {
+        fill_rows<S>(g, blockIdx.x - sums, each, close.words != nullptr);
+        program_close_block(close);
+        return;
+    }
+    const uint32_t n = (uint32_t)g.rows, lane = threadIdx.x & 63, vecs = (g.width + V - 1) / V;
+    const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64), i = unit / across;
+    const uint32_t v = unit % across * 64 + lane;
+    const int32_t t = i < n ? g.tokens[i] : -1;
+    const bool valid = t >= 0 && (uint32_t)t < g.vocab;
+    wave_record_fault(t >= 0 && !valid && lane == 0 ? pack_fault(i, kInvalid) : kNoFault, g.fault, g.gate);
+    uint64_t same[N]; // bit l of same[q]: place 64 q + l
+    bool first = valid;
+    if (valid) {
+        int32_t other[N];
+#pragma unroll
+        for (int q = 0; q < N; q++)
+            other[q] = (uint32_t)q * 64 + lane < n ? g.tokens[q * 64 + lane] : -1;
+#pragma unroll
+        for (int q = 0; q < N; q++) {
+            same[q] = __ballot(other[q] == t);
+            if ((uint32_t)q < i / 64 ? same[q] != 0 : (uint32_t)q == i / 64 && (same[q] & ((1ull << (i & 63)) - 1)))
+                first = false;
+        }
+    }
+    if (first) {
+        const u32x4 base = v < vecs ? load_base<S>(g, t, v) : u32x4{};
+        T sum[V] = {};
+#pragma unroll
+        for (int q = 0; q < N; q++)
+            for (uint64_t left = same[q]; left;) {
+                u32x4 raw[U];
+                uint64_t l = left;
+#pragma unroll
+                for (int k = 0; k < U; k++, l &= l - 1)
+                    if (l && v < vecs)
+                        raw[k] = load_vec(static_cast<const S *>(g.gradient) + (uint64_t)(q * 64 + __builtin_ctzll(l)) * g.gradient_stride, v, g.width);
+#pragma unroll
+                for (int k = 0; k < U; k++, left &= left - 1)
+                    if (left) {
+                        T x[V];
+                        unpack<S>(raw[k], x);
+#pragma unroll
+                        for (int e = 0; e < V; e++)
+                            sum[e] += x[e];
+                    }
+            }
+        if (v < vecs)
+            write_sum<S>(g, t, v, base, sum, close.words != nullptr);
+    }
+    program_close_block(close);
 }
 
 template <typename S, typename T>
@@ -414,11 +623,9 @@ __device__ __forceinline__ void leave_part(const EmbedBackArgs &g, const uint32_
         out[e] = sum[e];
 }
 
-constexpr uint32_t kRowsAWave = 16;
-
 // Workgroups [0, row_blocks) write the table's rows; the others leave the sums of long rows' parts,
 // part c (terms c kLong ..) with its first row's sum at 2 c and its last row's at 2 c + 1.
-template <typename S>
+template <typename S, bool BASE>
 __global__ __launch_bounds__(256) void k_embed_sum(EmbedBackArgs g, const uint32_t *keys, const uint32_t *places, int lanes,
                                                    uint32_t row_blocks, void *parts)
 {
@@ -429,36 +636,33 @@ __global__ __launch_bounds__(256) void k_embed_sum(EmbedBackArgs g, const uint32
     const uint32_t vecs = (g.width + kVec<S> - 1) / kVec<S>, v = blockIdx.y * lanes + lane;
     if (blockIdx.x < row_blocks) {
         // kRowsAWave rows a wave: its lanes look them all up at once.
-        __shared__ uint32_t from[4][kRowsAWave + 1];
-        const uint32_t wave = threadIdx.x / 64, row0 = (blockIdx.x * 4 + wave) * kRowsAWave;
-        if ((threadIdx.x & 63) <= kRowsAWave)
-            from[wave][threadIdx.x & 63] = lower_bound(keys, n, min(row0 + (threadIdx.x & 63), g.vocab));
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        const uint32_t subs_wave = 64 / lanes;
-        for (uint32_t r = sub % subs_wave; r < kRowsAWave; r += subs_wave) {
-            if (row0 + r >= g.vocab || v >= vecs)
-                continue;
-            const uint32_t lo = from[wave][r], hi = from[wave][r + 1];
-            if (hi - lo > kLong)
-                continue;
-            T sum[kVec<S>] = {};
-            add_terms<S>(g, places, lo, hi, v, sum);
-            write_sum<S>(g, row0 + r, v, hi > lo, sum);
+        __shared__ uint32_t lds_from[4][kRowsAWave + 1];
+        const uint32_t wave = threadIdx.x / 64, lane64 = threadIdx.x & 63, row0 = (blockIdx.x * 4 + wave) * kRowsAWave;
+        const uint32_t rows = row0 < g.vocab ? min(kRowsAWave, g.vocab - row0) : 0;
+        const uint32_t from = lower_bound(keys, n, min(row0 + min(lane64, kRowsAWave), g.vocab));
+        if (lanes < 64) {
+            if (lane64 <= kRowsAWave)
+                lds_from[wave][lane64] = from;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            narrow_rows<S>(g, places, lds_from[wave], row0, rows, lanes, vecs);
+        } else if (rows) {
+            wave_rows<S, BASE>(g, row0, rows, from, v, v < vecs, [&](uint32_t j) { return places[j]; });
         }
         return;
     }
     const uint32_t c = (blockIdx.x - row_blocks) * subs + sub, lo = c * kLong;
-    if (lo >= n || v >= vecs)
+    if (lo >= n)
         return;
     const uint32_t hi = min(lo + kLong, n), first = keys[lo], last = keys[hi - 1];
-    T *out = static_cast<T *>(parts) + ((uint64_t)2 * c * vecs + v) * kVec<S>;
-    const Run head = run_of(keys, n, first);
-    if (first < g.vocab && head.hi - head.lo > kLong)
-        leave_part<S>(g, places, lo, min(hi, head.hi), v, out);
-    if (last == first || last >= g.vocab)
+    const Run head = run_of(keys, n, first), tail = run_of(keys, n, last);
+    const bool leave_head = first < g.vocab && head.hi - head.lo > kLong;
+    const bool leave_tail = last != first && last < g.vocab && tail.hi - tail.lo > kLong;
+    if (v >= vecs)
         return;
-    const Run tail = run_of(keys, n, last);
-    if (tail.hi - tail.lo > kLong)
+    T *out = static_cast<T *>(parts) + ((uint64_t)2 * c * vecs + v) * kVec<S>;
+    if (leave_head)
+        leave_part<S>(g, places, lo, min(hi, head.hi), v, out);
+    if (leave_tail)
         leave_part<S>(g, places, tail.lo, hi, v, out + (uint64_t)vecs * kVec<S>);
 }
 
@@ -501,7 +705,7 @@ __global__ __launch_bounds__(256) void k_embed_join(EmbedBackArgs g, const uint3
                 for (int e = 0; e < kVec<S>; e++)
                     sum[e] += x[q][e];
     }
-    write_sum<S>(g, last, v, true, sum);
+    write_sum<S>(g, last, v, load_base<S>(g, last, v), sum);
 }
 
 // What the gradient's scratch holds: sorted keys and places, those of the first pass, the tiles'
@@ -513,6 +717,9 @@ struct EmbedPlan {
     uint64_t keys, counts, totals, parts, bytes;
     explicit EmbedPlan(const EmbedBackArgs &g)
     {
+        bytes = 0;
+        if (g.rows <= kDirect) // no sort
+            return;
         bits = 1;
         while ((1ull << (2 * bits)) <= g.vocab) // the largest key is vocab
             bits++;
@@ -527,11 +734,10 @@ struct EmbedPlan {
             bytes += (n + 255) / 256 * 256;
             return at;
         };
-        bytes = 0;
         keys = take(4 * 4 * g.rows);
         counts = take(one ? 0 : bins * tiles * 4);
         totals = take(one ? 0 : bins * 4);
-        parts = take(g.rows > kLong ? (g.rows + kLong - 1) / kLong * 2 * vecs * (16 / size) * stat : 0);
+        parts = take((g.rows + kLong - 1) / kLong * 2 * vecs * (16 / size) * stat);
     }
 };
 
@@ -542,9 +748,28 @@ template <typename K> hipError_t allow_lds(K *kernel, uint32_t bytes)
                          : hipSuccess;
 }
 
-template <typename S> hipError_t launch_embed_back_t(hipStream_t s, const EmbedBackArgs &g, void *scratch)
+template <typename S> hipError_t launch_embed_back_t(hipStream_t s, EmbedBackArgs g, void *scratch, ProgramClose close, bool *closed)
 {
     const EmbedPlan p(g);
+    const uint32_t vecs = (g.width + kVec<S> - 1) / kVec<S>;
+    const int lanes = row_lanes(vecs);
+    const uint32_t across = (vecs + lanes - 1) / lanes;
+    const uint32_t row_blocks = (uint32_t)((g.vocab + 4 * kRowsAWave - 1) / (4 * kRowsAWave));
+    if (g.rows <= kDirect) {
+        const uint64_t all = g.base && g.base == g.out ? 0 : (uint64_t)g.vocab * vecs, wanted = (all + 1023) / 1024;
+        const uint64_t fill = wanted < kFillBlocks ? wanted : kFillBlocks, each = fill ? ((all + fill - 1) / fill + 255) / 256 * 256 : 0;
+        const uint32_t sums = (uint32_t)((g.rows * across + 3) / 4), blocks = sums + (uint32_t)fill;
+        if (blocks == 0)
+            return hipSuccess;
+        if (blocks > kCloseMaxBlocks)
+            close = ProgramClose{};
+        *closed = close.words != nullptr;
+        hipLaunchKernelGGL((k_embed_first<S>), dim3(blocks), dim3(256), 0, s, g, across, sums, each, close);
+        return hipGetLastError();
+    }
+    // Where every row is read and written, storing past the caches is the faster way (32768 tokens,
+    // 32000 x 2048 bf16 with a base: 129 and 162 us).
+    g.past = g.base && (uint64_t)g.vocab * g.width * sizeof(S) > 64u << 20;
     char *sc = static_cast<char *>(scratch);
     uint32_t *keys = reinterpret_cast<uint32_t *>(sc + p.keys), *places = keys + g.rows;
     uint32_t *mid_keys = places + g.rows, *mid_places = mid_keys + g.rows;
@@ -567,15 +792,13 @@ template <typename S> hipError_t launch_embed_back_t(hipStream_t s, const EmbedB
                                pass * p.bits, p.bits, counts, totals, pass ? keys : mid_keys, pass ? places : mid_places);
         }
     }
-    const uint32_t vecs = (g.width + kVec<S> - 1) / kVec<S>;
-    const int lanes = row_lanes(vecs);
-    const uint32_t subs = 256 / lanes, across = (vecs + lanes - 1) / lanes;
-    const uint32_t row_blocks = (uint32_t)((g.vocab + 4 * kRowsAWave - 1) / (4 * kRowsAWave));
-    const uint32_t part_blocks = g.rows > kLong ? (uint32_t)(((g.rows + kLong - 1) / kLong + subs - 1) / subs) : 0;
-    hipLaunchKernelGGL((k_embed_sum<S>), dim3(row_blocks + part_blocks, across), dim3(256), 0, s, g, keys, places, lanes,
-                       row_blocks, sc + p.parts);
-    if (part_blocks)
-        hipLaunchKernelGGL((k_embed_join<S>), dim3(part_blocks, across), dim3(256), 0, s, g, keys, lanes, sc + p.parts);
+    const uint32_t subs = 256 / lanes, part_blocks = (uint32_t)(((g.rows + kLong - 1) / kLong + subs - 1) / subs);
+    const dim3 grid(row_blocks + part_blocks, across);
+    if (g.base)
+        hipLaunchKernelGGL((k_embed_sum<S, true>), grid, dim3(256), 0, s, g, keys, places, lanes, row_blocks, sc + p.parts);
+    else
+        hipLaunchKernelGGL((k_embed_sum<S, false>), grid, dim3(256), 0, s, g, keys, places, lanes, row_blocks, sc + p.parts);
+    hipLaunchKernelGGL((k_embed_join<S>), dim3(part_blocks, across), dim3(256), 0, s, g, keys, lanes, sc + p.parts);
     return hipGetLastError();
 }
 
@@ -596,15 +819,16 @@ hipError_t launch_embed(hipStream_t s, const EmbedArgs &g, ProgramClose close, b
 
 size_t embed_back_scratch_bytes(const EmbedBackArgs &g) { return g.width && g.vocab ? EmbedPlan(g).bytes : 0; }
 
-hipError_t launch_embed_back(hipStream_t s, const EmbedBackArgs &g, void *scratch)
+hipError_t launch_embed_back(hipStream_t s, const EmbedBackArgs &g, void *scratch, ProgramClose close, bool *closed)
 {
+    *closed = false;
     if (g.width == 0 || g.vocab == 0)
         return hipSuccess;
     switch (g.dtype) {
-    case kLogitF32: return launch_embed_back_t<float>(s, g, scratch);
-    case kLogitF64: return launch_embed_back_t<double>(s, g, scratch);
-    case kLogitBf16: return launch_embed_back_t<__bf16>(s, g, scratch);
-    default: return launch_embed_back_t<_Float16>(s, g, scratch);
+    case kLogitF32: return launch_embed_back_t<float>(s, g, scratch, close, closed);
+    case kLogitF64: return launch_embed_back_t<double>(s, g, scratch, close, closed);
+    case kLogitBf16: return launch_embed_back_t<__bf16>(s, g, scratch, close, closed);
+    default: return launch_embed_back_t<_Float16>(s, g, scratch, close, closed);
     }
 }
 

@@ -207,16 +207,16 @@ template <typename S, typename W> hipError_t launch_norm_t(hipStream_t s, const 
 }
 
 // ------------------------------------------------------------------- backward
-// Workgroups of 1024 threads, LANES a row, R vectors a lane: each takes the rows from its own on by
+// Workgroups of NT threads, LANES a row, R vectors a lane: each takes the rows from its own on by
 // the grid's step, the next one's loads under way while this one is worked on, and leaves its sums
 // down the columns at part[workgroup][2][vecs * kVec].
-template <typename S, typename W, int LANES, int R, bool SUMS>
-__global__ __launch_bounds__(1024) void k_norm_back(NormBackArgs g, void *parts)
+template <typename S, typename W, int NT, int LANES, int R, bool SUMS>
+__global__ __launch_bounds__(NT) void k_norm_back(NormBackArgs g, void *parts)
 {
     using T = typename StatOf<S>::T;
-    constexpr int G = 1024 / LANES, V = kVec<S>;
+    constexpr int G = NT / LANES, V = kVec<S>;
     extern __shared__ __align__(16) char dyn[]; // the groups' sums at the end
-    __shared__ T lds[2][2 * 16];
+    __shared__ T lds[2 * NT / 64];
     if (block_gate_closed(g.gate))
         return;
     const uint32_t lane = threadIdx.x % LANES, group = threadIdx.x / LANES, n = g.width, vecs = (n + V - 1) / V;
@@ -280,7 +280,7 @@ __global__ __launch_bounds__(1024) void k_norm_back(NormBackArgs g, void *parts)
         if (r + step < g.rows)
             fetch(r + step);
         if (g.x_gradient) {
-            row_sums<1024, LANES, 2>(sum, lds[0]);
+            row_sums<NT, LANES, 2>(sum, lds);
             const T c0 = sum[0] * inv_n, c1 = sum[1] * inv_n;
             if (on) {
                 S *out = static_cast<S *>(g.x_gradient) + r * g.x_gradient_stride;
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(1024) void k_norm_back(NormBackArgs g, void *parts)
                 __syncthreads();
         }
         if (G > 1)
-            for (uint32_t i = threadIdx.x; i < 2 * vecs * V; i += 1024)
+            for (uint32_t i = threadIdx.x; i < 2 * vecs * V; i += NT)
                 part[i] = all[i];
     }
 }
@@ -409,38 +409,56 @@ __global__ __launch_bounds__(1024) void k_norm_back_wide(NormBackArgs g, const v
     }
 }
 
-// The workgroups' sums, in their order: 16 columns a workgroup of 256 threads (a thread takes every
-// 16th workgroup's, then the 16 sums are added in order).
+// The workgroups' sums of both gradients, in their order: 64 columns a workgroup, 16 waves that each take
+// every 16th workgroup's, then the waves' sums.
 template <typename S, typename W>
-__global__ __launch_bounds__(256) void k_norm_back_join(NormBackArgs g, const void *parts, uint32_t count)
+__global__ __launch_bounds__(1024) void k_norm_back_join(NormBackArgs g, const void *parts, uint32_t count, ProgramClose close)
 {
     using T = typename StatOf<S>::T;
     constexpr int V = kVec<S>;
-    __shared__ T lds[16][17];
+    __shared__ T lds[2][16][64];
     if (block_gate_closed(g.gate))
         return;
-    const uint32_t cols = (g.width + V - 1) / V * V, c = threadIdx.x & 15, k = threadIdx.x / 16;
-    const uint32_t at = blockIdx.x * 16 + c;
-    W *out = static_cast<W *>(blockIdx.y ? g.bias_gradient : g.weight_gradient);
-    if (!out)
-        return;
-    const T *from = static_cast<const T *>(parts) + (uint64_t)blockIdx.y * cols + at;
-    T sum = 0;
-    if (at < cols)
-        for (uint32_t p = k; p < count; p += 16)
-            sum += from[(uint64_t)p * 2 * cols];
-    lds[k][c] = sum;
-    __syncthreads();
-    if (k == 0 && at < g.width) {
-        for (int q = 1; q < 16; q++)
-            sum += lds[q][c];
-        out[at] = (W)sum;
+    const uint32_t cols = (g.width + V - 1) / V * V, c = threadIdx.x & 63, k = threadIdx.x / 64;
+    const uint32_t at = blockIdx.x * 64 + c;
+    const T *from = static_cast<const T *>(parts) + at;
+    T sum[2] = {0, 0};
+    if (at < cols) {
+        constexpr uint32_t U = 4;
+        for (uint32_t p = k; p < count; p += 16 * U) {
+            T x[U][2];
+#pragma unroll
+            for (uint32_t q = 0; q < U; q++)
+#pragma unroll
+                for (int o = 0; o < 2; o++)
+                    x[q][o] = p + 16 * q < count ? from[((uint64_t)(p + 16 * q) * 2 + o) * cols] : (T)0;
+#pragma unroll
+            for (uint32_t q = 0; q < U; q++) {
+                sum[0] += x[q][0];
+                sum[1] += x[q][1];
+            }
+        }
     }
+    lds[0][k][c] = sum[0];
+    lds[1][k][c] = sum[1];
+    __syncthreads();
+    W *out = static_cast<W *>(k ? g.bias_gradient : g.weight_gradient);
+    if (k < 2 && out && at < g.width) {
+        T all = lds[k][0][c];
+        for (int q = 1; q < 16; q++)
+            all += lds[k][q][c];
+        if (close.words)
+            put(out + at, (W)all);
+        else
+            out[at] = (W)all;
+    }
+    program_close_block(close);
 }
 
-// How the backward pass is launched.
+// How the backward pass is launched. Few rows take workgroups of 256 threads where those of 1024
+// would leave CUs without one.
 struct NormBackPlan {
-    uint32_t lanes = 0, r = 0, grid = 0; // lanes == 0: rows too long to hold
+    uint32_t threads = 1024, lanes = 0, r = 0, grid = 0; // lanes == 0: rows too long to hold
     uint64_t sums = 0, parts = 0, bytes = 0;
     NormBackPlan(const NormBackArgs &g)
     {
@@ -453,7 +471,9 @@ struct NormBackPlan {
         else if (vecs <= 512) lanes = 256, r = 2;
         else if (vecs <= 1024) lanes = 1024, r = 1;
         else if (vecs <= 2048) lanes = 1024, r = 2;
-        const uint64_t groups = lanes ? 1024 / lanes : 1, most = 256;
+        if (lanes && lanes <= 256 && g.rows * lanes < 2ull * 1024 * kGfx950Cus)
+            threads = 256;
+        const uint64_t groups = lanes ? threads / lanes : 1, most = threads == 256 ? 512 : kGfx950Cus;
         const uint64_t need = (g.rows + groups - 1) / groups;
         grid = (uint32_t)(need < most ? need : most);
         parts = lanes ? 0 : (g.rows * 2 * stat + 255) / 256 * 256;
@@ -461,48 +481,61 @@ struct NormBackPlan {
     }
 };
 
-template <typename S, typename W, int LANES, int R>
-hipError_t launch_norm_held(hipStream_t s, const NormBackArgs &g, const NormBackPlan &p, char *sc, bool want)
+template <typename S, typename W, int NT, int LANES, int R>
+void launch_norm_held(hipStream_t s, const NormBackArgs &g, const NormBackPlan &p, char *sc, bool want)
 {
     using T = typename StatOf<S>::T;
     const uint32_t vecs = (g.width + kVec<S> - 1) / kVec<S>;
-    const uint32_t lds = want && LANES < 1024 ? 2 * vecs * kVec<S> * (uint32_t)sizeof(T) : 0;
+    const uint32_t lds = want && LANES < NT ? 2 * vecs * kVec<S> * (uint32_t)sizeof(T) : 0;
     if (want)
-        hipLaunchKernelGGL((k_norm_back<S, W, LANES, R, true>), dim3(p.grid), dim3(1024), lds, s, g, sc + p.parts);
+        hipLaunchKernelGGL((k_norm_back<S, W, NT, LANES, R, true>), dim3(p.grid), dim3(NT), lds, s, g, sc + p.parts);
     else
-        hipLaunchKernelGGL((k_norm_back<S, W, LANES, R, false>), dim3(p.grid), dim3(1024), 0, s, g, nullptr);
-    return hipGetLastError();
+        hipLaunchKernelGGL((k_norm_back<S, W, NT, LANES, R, false>), dim3(p.grid), dim3(NT), 0, s, g, nullptr);
 }
 
-template <typename S, typename W> hipError_t launch_norm_back_t(hipStream_t s, const NormBackArgs &g, void *scratch)
+template <typename S, typename W, int NT> void launch_norm_narrow(hipStream_t s, const NormBackArgs &g, const NormBackPlan &p, char *sc, bool want)
+{
+    if (p.lanes == 16)
+        launch_norm_held<S, W, NT, 16, 1>(s, g, p, sc, want);
+    else if (p.lanes == 64 && p.r == 1)
+        launch_norm_held<S, W, NT, 64, 1>(s, g, p, sc, want);
+    else if (p.lanes == 64)
+        launch_norm_held<S, W, NT, 64, 2>(s, g, p, sc, want);
+    else
+        launch_norm_held<S, W, NT, 256, 2>(s, g, p, sc, want);
+}
+
+template <typename S, typename W>
+hipError_t launch_norm_back_t(hipStream_t s, const NormBackArgs &g, void *scratch, ProgramClose close, bool *closed)
 {
     const NormBackPlan p(g);
     char *sc = static_cast<char *>(scratch);
     const bool want = g.weight_gradient || g.bias_gradient;
     const uint32_t vecs = (g.width + kVec<S> - 1) / kVec<S>;
-    hipError_t e = hipSuccess;
     if (p.grid) {
         if (p.lanes == 0) {
             hipLaunchKernelGGL((k_norm_back_sums<S, W>), row_grid(g.rows), dim3(1024), 0, s, g, sc + p.sums);
             hipLaunchKernelGGL((k_norm_back_wide<S, W>), dim3(p.grid, (vecs + 1023) / 1024), dim3(1024), 0, s, g, sc + p.sums, sc + p.parts);
-            e = hipGetLastError();
-        } else if (p.lanes == 16) {
-            e = launch_norm_held<S, W, 16, 1>(s, g, p, sc, want);
-        } else if (p.lanes == 64 && p.r == 1) {
-            e = launch_norm_held<S, W, 64, 1>(s, g, p, sc, want);
-        } else if (p.lanes == 64) {
-            e = launch_norm_held<S, W, 64, 2>(s, g, p, sc, want);
-        } else if (p.lanes == 256) {
-            e = launch_norm_held<S, W, 256, 2>(s, g, p, sc, want);
+        } else if (p.threads == 256) {
+            launch_norm_narrow<S, W, 256>(s, g, p, sc, want);
+        } else if (p.lanes <= 256) {
+            launch_norm_narrow<S, W, 1024>(s, g, p, sc, want);
         } else if (p.r == 1) {
-            e = launch_norm_held<S, W, 1024, 1>(s, g, p, sc, want);
+            launch_norm_held<S, W, 1024, 1024, 1>(s, g, p, sc, want);
         } else {
-            e = launch_norm_held<S, W, 1024, 2>(s, g, p, sc, want);
+            launch_norm_held<S, W, 1024, 1024, 2>(s, g, p, sc, want);
         }
+        const hipError_t e = hipGetLastError();
+        if (e)
+            return e;
     }
-    if (e || !want)
-        return e;
-    hipLaunchKernelGGL((k_norm_back_join<S, W>), dim3((g.width + 15) / 16, 2), dim3(256), 0, s, g, sc + p.parts, p.grid);
+    if (!want)
+        return hipSuccess;
+    const uint32_t blocks = (g.width + 63) / 64;
+    if (blocks > kCloseMaxBlocks)
+        close = ProgramClose{};
+    *closed = close.words != nullptr;
+    hipLaunchKernelGGL((k_norm_back_join<S, W>), dim3(blocks), dim3(1024), 0, s, g, sc + p.parts, p.grid, close);
     return hipGetLastError();
 }
 
@@ -527,19 +560,20 @@ hipError_t launch_norm(hipStream_t s, const NormArgs &g, ProgramClose close, boo
 
 size_t norm_back_scratch_bytes(const NormBackArgs &g) { return g.width ? NormBackPlan(g).bytes : 0; }
 
-hipError_t launch_norm_back(hipStream_t s, const NormBackArgs &g, void *scratch)
+hipError_t launch_norm_back(hipStream_t s, const NormBackArgs &g, void *scratch, ProgramClose close, bool *closed)
 {
+    *closed = false;
     if (g.width == 0)
         return hipSuccess;
     switch (g.dtype) {
-    case kLogitF32: return launch_norm_back_t<float, float>(s, g, scratch);
-    case kLogitF64: return launch_norm_back_t<double, double>(s, g, scratch);
+    case kLogitF32: return launch_norm_back_t<float, float>(s, g, scratch, close, closed);
+    case kLogitF64: return launch_norm_back_t<double, double>(s, g, scratch, close, closed);
     case kLogitBf16:
-        return g.weight_dtype == kLogitF32 ? launch_norm_back_t<__bf16, float>(s, g, scratch)
-                                           : launch_norm_back_t<__bf16, __bf16>(s, g, scratch);
+        return g.weight_dtype == kLogitF32 ? launch_norm_back_t<__bf16, float>(s, g, scratch, close, closed)
+                                           : launch_norm_back_t<__bf16, __bf16>(s, g, scratch, close, closed);
     default:
-        return g.weight_dtype == kLogitF32 ? launch_norm_back_t<_Float16, float>(s, g, scratch)
-                                           : launch_norm_back_t<_Float16, _Float16>(s, g, scratch);
+        return g.weight_dtype == kLogitF32 ? launch_norm_back_t<_Float16, float>(s, g, scratch, close, closed)
+                                           : launch_norm_back_t<_Float16, _Float16>(s, g, scratch, close, closed);
     }
 }
 

@@ -143,9 +143,17 @@ pcu_status Ctx::op_embedding_backward(const pcu_rows *gradient, const int32_t *t
         return st;
     if ((st = open_words()))
         return st;
+    ProgramClose close;
+    if (implicit_program && nodes.size() == 1)
+        close_next = true; // a call of its own: its last kernel ends the program
+    if ((st = take_close(&close)))
+        return st;
+    bool closed = false;
     hipEvent_t t = timer_start(stream);
-    st = hip(launch_embed_back(stream, g, sc), "embedding gradient launch");
+    st = hip(launch_embed_back(stream, g, sc, close, &closed), "embedding gradient launch");
     timer_stop(PCU_KERNEL_EMBEDDING, t, stream);
+    if (!st && closed)
+        closed_seq = ++pub_seq;
     return st;
 }
 
@@ -269,9 +277,17 @@ pcu_status Ctx::op_layer_norm_backward(const pcu_rows *x, const void *stats, con
         return st;
     if ((st = open_words()))
         return st;
+    ProgramClose close;
+    if (implicit_program && nodes.size() == 1)
+        close_next = true; // a call of its own: its last kernel ends the program
+    if ((st = take_close(&close)))
+        return st;
+    bool closed = false;
     hipEvent_t t = timer_start(stream);
-    st = hip(launch_norm_back(stream, g, sc), "layer_norm gradient launch");
+    st = hip(launch_norm_back(stream, g, sc, close, &closed), "layer_norm gradient launch");
     timer_stop(PCU_KERNEL_LAYER_NORM, t, stream);
+    if (!st && closed)
+        closed_seq = ++pub_seq;
     return st;
 }
 

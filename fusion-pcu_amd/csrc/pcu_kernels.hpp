@@ -398,11 +398,12 @@ struct EmbedBackArgs {
     uint64_t base_stride = 0;
     void *out = nullptr;
     uint64_t out_stride = 0;
+    bool past = false; // set by the launch: a large result is stored past the caches
     unsigned long long *fault = nullptr;
     NodeGate gate{nullptr, 0};
 };
 size_t embed_back_scratch_bytes(const EmbedBackArgs &g);
-hipError_t launch_embed_back(hipStream_t s, const EmbedBackArgs &g, void *scratch);
+hipError_t launch_embed_back(hipStream_t s, const EmbedBackArgs &g, void *scratch, ProgramClose close, bool *closed);
 
 // Layer norm of rows, and its gradients. Statistics (mean, 1 / standard deviation) are binary32,
 // binary64 for binary64 rows. weight and bias (or null) are of weight_dtype: the rows' type, or
@@ -436,7 +437,7 @@ struct NormBackArgs {
     NodeGate gate{nullptr, 0};
 };
 size_t norm_back_scratch_bytes(const NormBackArgs &g);
-hipError_t launch_norm_back(hipStream_t s, const NormBackArgs &g, void *scratch);
+hipError_t launch_norm_back(hipStream_t s, const NormBackArgs &g, void *scratch, ProgramClose close, bool *closed);
 
 // The cross entropy of softmax(features * weights^T) against labels, and its gradients, with the
 // logits never in memory. Binary32, bfloat16 or binary16; loss, log_sum and row_scale are binary32.

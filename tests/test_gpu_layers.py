@@ -151,7 +151,8 @@ def test_embedding_of_strided_rows(ctx, pcu_pkg, dtype, code, lead, width, strid
 
 BACK_SHAPES = [(1, 1, 1), (0, 9, 5), (5, 1, 8), (64, 1000, 64), (65, 1000, 63), (700, 3, 40), (511, 50257, 20),
                (4096, 100, 33), (4097, 100, 33), (5000, 40000, 17), (20000, 300000, 4), (9000, 65536, 9), (300, 70, 2500),
-               (200, 4194304, 1)]
+               (200, 4194304, 1), (1024, 17, 9), (1025, 17, 9), (1500, 100, 33), (2048, 50000, 12), (2049, 50000, 12),
+               (1200, 4194304, 1)]
 
 
 def _tokens(rng, count, vocab, how):
