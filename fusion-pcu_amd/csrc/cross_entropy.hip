@@ -16,6 +16,8 @@
 // probability it holds is then 2^-38.
 #include "pcu_entropy_tile.hpp"
 
+#include <cmath>
+
 #pragma clang fp contract(off)
 
 namespace pcu {
@@ -182,7 +184,14 @@ struct LogitArgs {
     NodeGate gate{nullptr, 0};
 };
 
-// Vocabulary down, rows across: a lane holds 16 SM logits of each of its SN rows.
+// (maximum, sum of exponentials against it) of two sets of logits together.
+__device__ __forceinline__ float2 join_sums(float2 a, float2 b)
+{
+    const float m = fmaxf(a.x, b.x), from = m == -INFINITY ? 0.0f : m;
+    return make_float2(m, a.y * exp2_fast((a.x - from) * kLog2e) + b.y * exp2_fast((b.x - from) * kLog2e));
+}
+
+// Vocabulary down, rows across: a lane holds 4 SM logits of each of its SN rows.
 template <typename S, class Cfg, bool GRAD> __global__ __launch_bounds__(Cfg::kThreads) void k_logits(LogitArgs g)
 {
     using E = typename ElemOf<S>::T;
@@ -192,78 +201,78 @@ template <typename S, class Cfg, bool GRAD> __global__ __launch_bounds__(Cfg::kT
         return;
     const EntropyTile t = entropy_tile(blockIdx.x, g.tiles_m, g.tiles_n, 1);
     const uint32_t m0 = t.tm * BM, n0 = t.tn * BN;
-    f32x16 acc[SM][SN];
+    f32x4 acc[SM][SN];
     entropy_product<E, Cfg, false, false>(g.w, g.x, g.pairs, m0, n0, 0, g.slabs, lds, acc);
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64, half = lane / 32;
-    const uint32_t wm = wave / Cfg::WN * SM * 32, wn = wave % Cfg::WN * SN * 32;
-    const uint32_t v0 = g.first + m0 + wm + 4 * half; // of acc[i][j][r]: v0 + 32 i + 8 (r / 4) + r % 4
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    const uint32_t wm = wave / Cfg::WN * SM * 16, wn = wave % Cfg::WN * SN * 16;
+    const uint32_t v0 = g.first + m0 + wm; // of acc[i][j][r]: v0 + acc_row(i, r)
+    const bool ragged = g.first + m0 + BM > g.vocab;
     if constexpr (!GRAD) {
         float2 *red = reinterpret_cast<float2 *>(lds + Cfg::kTile);
-        const bool ragged = g.first + m0 + BM > g.vocab;
 #pragma unroll
         for (int j = 0; j < SN; j++) {
-            const uint32_t n = n0 + wn + 32 * j + (lane & 31);
+            const uint32_t n = n0 + wn + acc_col(j);
             const int32_t label = n < g.rows ? g.row.label[n] : -1;
-            if (label >= 0 && (uint32_t)label - (g.first + m0 + wm) < SM * 32u) {
+            if (label >= 0 && (uint32_t)label - v0 < SM * 16u) {
 #pragma unroll
                 for (int i = 0; i < SM; i++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++)
-                        if (v0 + 32 * i + 8 * (r / 4) + r % 4 == (uint32_t)label)
+                    for (int r = 0; r < 4; r++)
+                        if (v0 + acc_row(i, r) == (uint32_t)label)
                             g.row.own[n] = acc[i][j][r];
             }
             if (ragged) {
 #pragma unroll
                 for (int i = 0; i < SM; i++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++)
-                        if (v0 + 32 * i + 8 * (r / 4) + r % 4 >= g.vocab)
+                    for (int r = 0; r < 4; r++)
+                        if (v0 + acc_row(i, r) >= g.vocab)
                             acc[i][j][r] = -INFINITY;
             }
             float m = -INFINITY;
 #pragma unroll
             for (int i = 0; i < SM; i++)
 #pragma unroll
-                for (int r = 0; r < 16; r++)
+                for (int r = 0; r < 4; r++)
                     m = fmaxf(m, acc[i][j][r]);
+            m = fmaxf(m, __shfl_xor(m, 16));
             m = fmaxf(m, __shfl_xor(m, 32));
             const float from = m == -INFINITY ? 0.0f : m;
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < SM; i++)
 #pragma unroll
-                for (int r = 0; r < 16; r++)
+                for (int r = 0; r < 4; r++)
                     sum += exp2_fast((acc[i][j][r] - from) * kLog2e);
+            sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);
-            if (half == 0)
-                red[wave / Cfg::WN * BN + wn + 32 * j + (lane & 31)] = make_float2(m, sum);
+            if (lane < 16)
+                red[wave / Cfg::WN * BN + wn + acc_col(j)] = make_float2(m, sum);
         }
         __syncthreads();
         for (uint32_t c = threadIdx.x; c < (uint32_t)BN; c += Cfg::kThreads) {
             float2 a = red[c];
 #pragma unroll
-            for (int k = 1; k < Cfg::WM; k++) {
-                const float2 b = red[k * BN + c];
-                const float m = fmaxf(a.x, b.x), from = m == -INFINITY ? 0.0f : m;
-                a = make_float2(m, a.y * exp2_fast((a.x - from) * kLog2e) + b.y * exp2_fast((b.x - from) * kLog2e));
-            }
+            for (int k = 1; k < Cfg::WM; k++)
+                a = join_sums(a, red[k * BN + c]);
             g.partial[(uint64_t)(g.partial_first + t.tm) * g.partial_ld + n0 + c] = a;
         }
     } else {
 #pragma unroll
         for (int j = 0; j < SN; j++) {
-            const uint32_t n = n0 + wn + 32 * j + (lane & 31);
+            const uint32_t n = n0 + wn + acc_col(j);
             const bool in = n < g.rows;
             const int32_t label = in ? g.row.label[n] : -1;
             const float scale = in ? g.row.scale[n] * g.boost : 0.0f, log_sum = in ? g.row.log_sum[n] : 0.0f;
+            const bool mine = label >= 0 && (uint32_t)label - v0 < SM * 16u;
 #pragma unroll
             for (int i = 0; i < SM; i++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const uint32_t v = v0 + 32 * i + 8 * (r / 4) + r % 4;
-                    const float p = exp2_fast((acc[i][j][r] - log_sum) * kLog2e);
-                    const float d = ((int32_t)v == label ? p - 1.0f : p) * scale;
-                    acc[i][j][r] = label >= 0 && v < g.vocab ? d : 0.0f;
+                for (int r = 0; r < 4; r++) {
+                    float p = exp2_fast((acc[i][j][r] - log_sum) * kLog2e);
+                    if (mine && v0 + acc_row(i, r) == (uint32_t)label)
+                        p -= 1.0f;
+                    acc[i][j][r] = label >= 0 && !(ragged && v0 + acc_row(i, r) >= g.vocab) ? p * scale : 0.0f;
                 }
         }
         // Through LDS, so that a row's values are stored side by side.
@@ -275,29 +284,25 @@ template <typename S, class Cfg, bool GRAD> __global__ __launch_bounds__(Cfg::kT
 #pragma unroll
             for (int j = 0; j < SN; j++)
 #pragma unroll
-                for (int i = 0; i < SM; i++)
+                for (int i = 0; i < SM; i++) {
+                    uint32_t two[2];
 #pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        uint32_t two[2];
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const int e = 4 * q + 2 * h;
-                            if constexpr (kParts<S> == 1) {
-                                typedef float f32x2 __attribute__((ext_vector_type(2)));
-                                typedef S s16x2 __attribute__((ext_vector_type(2)));
-                                const f32x2 x = {acc[i][j][e], acc[i][j][e + 1]};
-                                two[h] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, s16x2));
-                            } else {
-                                // A part, and what is left for the next ones.
-                                float lo = acc[i][j][e], hi = acc[i][j][e + 1];
-                                two[h] = first_part(lo) | first_part(hi) << 16;
-                                acc[i][j][e] = lo;
-                                acc[i][j][e + 1] = hi;
-                            }
+                    for (int h = 0; h < 2; h++) {
+                        if constexpr (kParts<S> == 1) {
+                            typedef float f32x2 __attribute__((ext_vector_type(2)));
+                            typedef S s16x2 __attribute__((ext_vector_type(2)));
+                            const f32x2 x = {acc[i][j][2 * h], acc[i][j][2 * h + 1]};
+                            two[h] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, s16x2));
+                        } else {
+                            // A part, and what is left for the next ones.
+                            float lo = acc[i][j][2 * h], hi = acc[i][j][2 * h + 1];
+                            two[h] = first_part(lo) | first_part(hi) << 16;
+                            acc[i][j][2 * h] = lo;
+                            acc[i][j][2 * h + 1] = hi;
                         }
-                        *reinterpret_cast<uint2 *>(tile + (wn + 32 * j + (lane & 31)) * Cfg::kOutPitch + wm + 32 * i + 8 * q + 4 * half) =
-                            make_uint2(two[0], two[1]);
                     }
+                    *reinterpret_cast<uint2 *>(tile + (wn + acc_col(j)) * Cfg::kOutPitch + wm + acc_row(i, 0)) = make_uint2(two[0], two[1]);
+                }
             __syncthreads();
             for (uint32_t i = threadIdx.x; i < BN * BM / 8; i += Cfg::kThreads) {
                 const uint32_t n = i / (BM / 8), c = i % (BM / 8) * 8;
@@ -316,10 +321,6 @@ __global__ __launch_bounds__(256) void k_entropy_loss(const float2 *partial, uin
     if (block_gate_closed(gate))
         return;
     const uint32_t c = threadIdx.x & 15, k = threadIdx.x / 16, n = blockIdx.x * 16 + c;
-    auto join = [](float2 a, float2 b) {
-        const float m = fmaxf(a.x, b.x), from = m == -INFINITY ? 0.0f : m;
-        return make_float2(m, a.y * exp2_fast((a.x - from) * kLog2e) + b.y * exp2_fast((b.x - from) * kLog2e));
-    };
     float2 a = make_float2(-INFINITY, 0.0f);
     if (n < rows) {
         constexpr uint32_t U = 4;
@@ -330,7 +331,7 @@ __global__ __launch_bounds__(256) void k_entropy_loss(const float2 *partial, uin
                 b[q] = t + 16 * q < tiles ? partial[(uint64_t)(t + 16 * q) * ld + n] : make_float2(-INFINITY, 0.0f);
 #pragma unroll
             for (uint32_t q = 0; q < U; q++)
-                a = join(a, b[q]);
+                a = join_sums(a, b[q]);
         }
     }
     red[k][c] = a;
@@ -338,7 +339,7 @@ __global__ __launch_bounds__(256) void k_entropy_loss(const float2 *partial, uin
     if (k || n >= rows)
         return;
     for (int q = 1; q < 16; q++)
-        a = join(a, red[q][c]);
+        a = join_sums(a, red[q][c]);
     const float from = a.x == -INFINITY ? 0.0f : a.x;
     // A NaN among the logits is not in the maximum, but in the sum.
     const float l = (float)((double)from + (double)__builtin_amdgcn_logf(a.y) * kLn2);
@@ -376,24 +377,16 @@ template <typename S, class Cfg> __global__ __launch_bounds__(Cfg::kThreads) voi
     const EntropyTile t = entropy_tile(blockIdx.x, g.tiles_m, g.tiles_n, g.splits);
     const uint32_t m0 = t.tm * Cfg::BM, n0 = t.tn * Cfg::BN;
     const uint32_t k_lo = (uint32_t)((uint64_t)g.slabs * t.split / g.splits), k_hi = (uint32_t)((uint64_t)g.slabs * (t.split + 1) / g.splits);
-    f32x16 acc[SM][SN];
+    f32x4 acc[SM][SN];
     entropy_product<E, Cfg, true, false>(g.a, g.b, g.pairs, m0, n0, k_lo, k_hi, lds, acc);
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-    const uint32_t m = m0 + wave / Cfg::WN * SM * 32 + 4 * (lane / 32), n = n0 + wave % Cfg::WN * SN * 32 + (lane & 31);
+    const uint32_t wave = threadIdx.x / 64, m = m0 + wave / Cfg::WN * SM * 16, n = n0 + wave % Cfg::WN * SN * 16;
 #pragma unroll
     for (int j = 0; j < SN; j++)
 #pragma unroll
-        for (int i = 0; i < SM; i++)
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                float4 *to = reinterpret_cast<float4 *>(g.sums + t.split * g.sums_split + (uint64_t)(n + 32 * j) * g.sums_ld + m + 32 * i + 8 * q);
-                float4 v = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
-                if (g.add) {
-                    const float4 o = *to;
-                    v = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
-                }
-                *to = v;
-            }
+        for (int i = 0; i < SM; i++) {
+            f32x4 *to = reinterpret_cast<f32x4 *>(g.sums + t.split * g.sums_split + (uint64_t)(n + acc_col(j)) * g.sums_ld + m + acc_row(i, 0));
+            *to = g.add ? *to + acc[i][j] : acc[i][j];
+        }
 }
 
 // dx from the splits' sums, in their order.
@@ -437,54 +430,40 @@ template <typename S, class Cfg> __global__ __launch_bounds__(Cfg::kThreads) voi
         return;
     const EntropyTile t = entropy_tile(blockIdx.x, g.tiles_m, g.tiles_n, 1);
     const uint32_t m0 = t.tm * BM, n0 = t.tn * BN;
-    f32x16 acc[SM][SN];
+    f32x4 acc[SM][SN];
     entropy_product<E, Cfg, true, true>(g.a, g.b, g.pairs, m0, n0, 0, g.slabs, lds, acc);
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-    const uint32_t wm = wave / Cfg::WN * SM * 32 + 4 * (lane / 32), wn = wave % Cfg::WN * SN * 32 + (lane & 31);
+    const uint32_t wave = threadIdx.x / 64, wm = wave / Cfg::WN * SM * 16, wn = wave % Cfg::WN * SN * 16;
     const float f = *g.factor;
     S *out = static_cast<S *>(g.out);
     if constexpr (sizeof(S) == 4) {
 #pragma unroll
         for (int j = 0; j < SN; j++) {
-            const uint32_t n = n0 + wn + 32 * j;
+            const uint32_t n = n0 + wn + acc_col(j);
             if (n >= g.out_rows)
                 continue;
 #pragma unroll
-            for (int i = 0; i < SM; i++)
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const uint32_t m = m0 + wm + 32 * i + 8 * q;
-                    float v[4];
+            for (int i = 0; i < SM; i++) {
+                const uint32_t m = m0 + wm + acc_row(i, 0);
+                const f32x4 v = acc[i][j] * f;
+                float *to = out + (uint64_t)n * g.out_ld + m;
+                if (g.out_whole && m + 4 <= g.out_cols)
+                    *reinterpret_cast<f32x4 *>(to) = v;
+                else
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        v[e] = acc[i][j][4 * q + e] * f;
-                    float *to = out + (uint64_t)n * g.out_ld + m;
-                    if (g.out_whole && m + 4 <= g.out_cols)
-                        *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
-                    else
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (m + e < g.out_cols)
-                                to[e] = v[e];
-                }
+                        if (m + e < g.out_cols)
+                            to[e] = v[e];
+            }
         }
     } else {
         S *tile = reinterpret_cast<S *>(lds);
+        typedef S s16x4_t __attribute__((ext_vector_type(4)));
 #pragma unroll
         for (int j = 0; j < SN; j++)
 #pragma unroll
             for (int i = 0; i < SM; i++)
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    typedef float f32x4 __attribute__((ext_vector_type(4)));
-                    typedef S s16x4_t __attribute__((ext_vector_type(4)));
-                    f32x4 v;
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        v[e] = acc[i][j][4 * q + e] * f;
-                    *reinterpret_cast<s16x4_t *>(tile + (wn + 32 * j) * Cfg::kOutPitch + wm + 32 * i + 8 * q) =
-                        __builtin_convertvector(v, s16x4_t);
-                }
+                *reinterpret_cast<s16x4_t *>(tile + (wn + acc_col(j)) * Cfg::kOutPitch + wm + acc_row(i, 0)) =
+                    __builtin_convertvector(acc[i][j] * f, s16x4_t);
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < BN * BM / 8; i += Cfg::kThreads) {
             const uint32_t n = i / (BM / 8), c = i % (BM / 8) * 8;
@@ -513,20 +492,35 @@ template <typename S> __global__ __launch_bounds__(256) void k_zero_rows(S *out,
 }
 
 // ---------------------------------------------------------------------- launches
-using Large = EntropyCfg<2, 4, 4, 2>;  // 256 x 256
-using Middle = EntropyCfg<2, 2, 2, 2>; // 128 x 128
-using Thin = EntropyCfg<4, 1, 2, 1>;   // 256 x 32, few rows
+using Large = EntropyCfg<4, 2, 4, 8>;  // 256 x 256
+using Middle = EntropyCfg<2, 2, 4, 4>; // 128 x 128
+using Half = EntropyCfg<2, 2, 4, 2>;   // 128 x 64
+using Thin = EntropyCfg<4, 1, 4, 2>;   // 256 x 32
 
 constexpr uint64_t round_up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
 
-enum class Side { Large, Middle, Thin };
-inline uint32_t side_m(Side s) { return s == Side::Middle ? 128 : 256; }
-inline uint32_t side_n(Side s) { return s == Side::Large ? 256 : s == Side::Middle ? 128 : 32; }
-
-// 256 x 256 tiles where they fill three quarters of the CUs.
-inline Side choose(uint64_t m, uint64_t n)
+enum class Side { Large, Middle, Half, Thin };
+inline uint32_t side_m(Side s) { return s == Side::Large || s == Side::Thin ? 256 : 128; }
+inline uint32_t side_n(Side s) { return s == Side::Large ? 256 : s == Side::Middle ? 128 : s == Side::Half ? 64 : 32; }
+inline uint64_t tiles_of(Side s, uint64_t m, uint64_t n)
 {
-    return (m + 255) / 256 * ((n + 255) / 256) * 4 >= 3 * kGfx950Cus ? Side::Large : Side::Middle;
+    return (m + side_m(s) - 1) / side_m(s) * ((n + side_n(s) - 1) / side_n(s));
+}
+
+// The tile of an m x n product, by the rounds that its tiles take on the CUs, in the time of a 128 x 128
+// tile at the larger one's rate: a round of 256 x 256 tiles (one a CU, 1450 TFLOP/s) takes 4, one of two
+// 128 x 128 tiles a CU (1050 TFLOP/s) 2.8, of one a CU 1.8. A product split along k fills its last round.
+inline Side choose(uint64_t m, uint64_t n, bool split)
+{
+    const double large = (double)tiles_of(Side::Large, m, n) / kGfx950Cus, middle = (double)tiles_of(Side::Middle, m, n) / kGfx950Cus;
+    if (split)
+        return 4 * large <= 1.4 * middle ? Side::Large : Side::Middle;
+    return 4 * std::ceil(large) <= (middle <= 1 ? 1.8 : 2.8 * std::ceil(middle / 2)) ? Side::Large : Side::Middle;
+}
+// The same where n are the call's rows: few of them take narrower tiles, which read the weights at HBM's rate.
+inline Side choose_rows(uint64_t m, uint64_t rows, bool split)
+{
+    return rows <= 32 ? Side::Thin : rows <= 64 ? Side::Half : choose(m, rows, split);
 }
 
 // How a call goes over its vocabulary and what its scratch holds.
@@ -563,11 +557,11 @@ struct EntropyPlan {
             const uint64_t fit = kWeightBytes / row_bytes / 256 * 256;
             piece = piece < fit ? piece : fit < 256 ? 256 : fit;
         }
-        logits = g.rows <= 32 ? Side::Thin : choose(g.vocab, g.rows);
-        features = g.rows <= 32 ? Side::Thin : choose(g.width, g.rows);
-        weights = choose(g.width, piece < g.vocab ? piece : g.vocab);
-        const uint64_t tiles = ((g.width + side_m(features) - 1) / side_m(features)) * ((g.rows + side_n(features) - 1) / side_n(features));
-        const uint64_t per = features == Side::Large ? 1 : 2; // workgroups a CU
+        logits = choose_rows(g.vocab, g.rows, false);
+        features = choose_rows(g.width, g.rows, true);
+        weights = choose(g.width, piece < g.vocab ? piece : g.vocab, false);
+        const uint64_t tiles = tiles_of(features, g.width, g.rows);
+        const uint64_t per = features == Side::Large ? 1 : features == Side::Half ? 3 : 2; // workgroups a CU
         const uint64_t want = tiles ? (per * kGfx950Cus + tiles / 2) / tiles : 1, most = (piece + 4 * kSlabK - 1) / (4 * kSlabK);
         splits = (uint32_t)(want < 1 ? 1 : want > most ? (most ? most : 1) : want);
         sums_ld = (uint32_t)round_up(g.width, 256);
@@ -611,6 +605,7 @@ template <typename S, bool GRAD> hipError_t logits_by(Side side, hipStream_t s, 
     switch (side) {
     case Side::Large: return run_logits<S, Large, GRAD>(s, a, vocab_rows, rows);
     case Side::Middle: return run_logits<S, Middle, GRAD>(s, a, vocab_rows, rows);
+    case Side::Half: return run_logits<S, Half, GRAD>(s, a, vocab_rows, rows);
     default: return run_logits<S, Thin, GRAD>(s, a, vocab_rows, rows);
     }
 }
@@ -774,6 +769,7 @@ template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyAr
             f.add = v > 0;
             e = p.features == Side::Large    ? run_features<S, Large>(s, f, g.width, g.rows)
                 : p.features == Side::Middle ? run_features<S, Middle>(s, f, g.width, g.rows)
+                : p.features == Side::Half   ? run_features<S, Half>(s, f, g.width, g.rows)
                                              : run_features<S, Thin>(s, f, g.width, g.rows);
             if (e)
                 return e;

@@ -1,13 +1,16 @@
 // Matrix-core tiles of the output layer's cross entropy (gfx950): 16-bit operands, F32 sums.
 //
 // A workgroup makes a BM x BN tile of C = A B, k in slabs of 64. An operand's slab lies in LDS as
-// it lies in memory, either k-contiguous (one row of A or column of B: 128 bytes) or k-major (`T`:
-// 64 rows of BM or BN values), and comes there by direct loads, two slabs in LDS at a time. A lane
-// of the 32 x 32 x 16 instruction takes 8 consecutive k of one row or column: one 16-byte read of a
+// it lies in memory, either k-contiguous (64 values of a row of A or column of B side by side) or k-major
+// (`T`: 64 rows of BM or BN values), and comes there by direct loads, one slab ahead. A lane of the
+// 16 x 16 x 32 instruction takes 8 consecutive k of one row or column: one 16-byte read of a
 // k-contiguous slab, two transposing 8-byte reads of a k-major one. The 16-byte pieces of a slab's
-// row are permuted by the row (in the loads' addresses, so that LDS stays dense): by its low 3 bits
-// where k is contiguous, so that 8 lanes read 128 different bytes; by twice its low 2 bits where it
-// is k-major, so that the 4 rows of a transposing read do.
+// row are permuted by the row (in the loads' addresses, so that LDS stays dense): by half of it
+// where k is contiguous, and by twice its bits 0, 1 and 3 where it is k-major, so that the 16 lanes (32 of
+// a transposing read) that are served at once touch all 256 bytes of LDS's banks.
+//
+// What bounds the tiles is power: the clock falls to 1.7 GHz under them. On random values the
+// 16 x 16 x 32 instruction alone reaches 2290 TFLOP/s, the 32 x 32 x 16 one 1940 (both 2400 on zeros).
 #pragma once
 
 #include "pcu_gemm_stage.hpp"
@@ -17,32 +20,35 @@
 
 namespace pcu {
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-template <typename E> __device__ __forceinline__ f32x16 mfma16(s16x8 a, s16x8 b, f32x16 c)
+template <typename E> __device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, f32x4 c)
 {
     if constexpr (__is_same(E, __bf16))
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     else
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
 constexpr int kSlabK = 64;
 
-// WM x WN waves, each with SM x SN subtiles of 32 x 32.
+// WM x WN waves, each with SM x SN subtiles of 16 x 16.
 template <int WM_, int WN_, int SM_, int SN_> struct EntropyCfg {
     static constexpr int WM = WM_, WN = WN_, SM = SM_, SN = SN_;
-    static constexpr int BM = WM * SM * 32, BN = WN * SN * 32, kWaves = WM * WN, kThreads = 64 * kWaves;
+    static constexpr int BM = WM * SM * 16, BN = WN * SN * 16, kWaves = WM * WN, kThreads = 64 * kWaves;
     static constexpr int kSlabA = BM * kSlabK * 2, kSlabB = BN * kSlabK * 2, kStage = kSlabA + kSlabB; // bytes
     static constexpr int kOutPitch = BM + 8; // of a 16-bit output tile in LDS, in values
     static constexpr int kTile = 2 * kStage > BN * kOutPitch * 2 ? 2 * kStage : BN * kOutPitch * 2;
     static constexpr int kReduce = WM * BN * 8; // bytes for a reduction over the tile's rows
     static constexpr int kLds = kTile + kReduce;
 };
+// Where acc[i][j][r] of a lane lies in its wave's tile.
+__device__ __forceinline__ uint32_t acc_row(int i, int r) { return 16 * i + 4 * ((threadIdx.x & 63) / 16) + r; }
+__device__ __forceinline__ uint32_t acc_col(int j) { return 16 * j + (threadIdx.x & 15); }
 
 // One operand: `ld` values from row to row (k-contiguous: rows of C; k-major: k), `plane` from one
 // 16-bit part of a binary32 operand to the next. Past `rows` rows and (k-major) `cols` columns the last
@@ -60,75 +66,73 @@ constexpr int kPartPairs = 6;
 __device__ __forceinline__ uint32_t part_a(uint32_t s) { return (0x201100u >> (20 - 4 * s)) & 15; }
 __device__ __forceinline__ uint32_t part_b(uint32_t s) { return (0x021010u >> (20 - 4 * s)) & 15; }
 
+// How the pieces of a k-major slab's row are permuted.
+__device__ __forceinline__ uint32_t k_major_swap(uint32_t k) { return 2 * ((k & 3) | (k >> 1 & 4)); }
+
 template <class Cfg, int ROWS, bool T> struct SlabLoader {
     static constexpr int IPW = ROWS / 8 / Cfg::kWaves; // 1 KiB loads a wave
-    static_assert(IPW * 8 * Cfg::kWaves == ROWS, "every wave loads whole rows");
-    static constexpr int kChunks = ROWS / 8; // 16-byte pieces of a k-major row
+    static_assert(IPW * 8 * Cfg::kWaves == ROWS, "every wave loads as much");
+    static constexpr int kPieces = (T ? ROWS : kSlabK) / 8; // 16-byte pieces of a row
     uint32_t off[IPW];
-    __device__ __forceinline__ int k_of(int wave, int q) const { return ((wave * IPW + q) * 64 + (threadIdx.x & 63)) / kChunks; }
+    __device__ __forceinline__ int row_of(int wave, int q) const { return ((wave * IPW + q) * 64 + (threadIdx.x & 63)) / kPieces; }
     // at: the tile's first row (k-contiguous) or column (k-major).
     __device__ __forceinline__ void init(const EntropyOperand &o, uint32_t at, int wave)
     {
-        const uint32_t lane = threadIdx.x & 63;
+        const uint32_t piece = (threadIdx.x & 63) % kPieces;
 #pragma unroll
         for (int q = 0; q < IPW; q++) {
-            if constexpr (!T) {
-                const uint32_t r = (wave * IPW + q) * 8 + lane / 8;
-                off[q] = min(r, o.rows - 1 - at) * o.ld * 2 + ((lane & 7) ^ (lane / 8)) * 16;
-            } else {
-                const uint32_t k = k_of(wave, q), c = (lane % kChunks) ^ (2 * (k & 3));
-                off[q] = k * o.ld * 2 + min(c * 8, o.cols - 8 - at) * 2;
-            }
+            const uint32_t r = row_of(wave, q);
+            if constexpr (!T)
+                off[q] = min(r, o.rows - 1 - at) * o.ld * 2 + (piece ^ (r / 2 & 7)) * 16;
+            else
+                off[q] = r * o.ld * 2 + min((piece ^ k_major_swap(r)) * 8, o.cols - 8 - at) * 2;
         }
     }
     // The slab of k0, part `part`, into `lds`.
     __device__ __forceinline__ void load(const EntropyOperand &o, uint32_t at, uint32_t part, uint32_t k0, uint32_t lds, int wave) const
     {
         const uint16_t *base = o.p + part * o.plane + (T ? (uint64_t)k0 * o.ld + at : (uint64_t)at * o.ld + k0);
-        if (T && k0 + kSlabK > o.rows) { // the last rows are read again
+        const bool over = T && k0 + kSlabK > o.rows;
 #pragma unroll
-            for (int q = 0; q < IPW; q++) {
-                const uint32_t k = k_of(wave, q), over = k0 + k >= o.rows ? k0 + k - (o.rows - 1) : 0;
-                load_lds<4>(base, off[q] - over * o.ld * 2, lds + (wave * IPW + q) * 1024);
+        for (int q = 0; q < IPW; q++) {
+            uint32_t from = off[q];
+            if (T && over) { // the last row is read again
+                const uint32_t k = row_of(wave, q);
+                from -= k0 + k >= o.rows ? (k0 + k - (o.rows - 1)) * o.ld * 2 : 0;
             }
-            return;
+            load_lds<4>(base, from, __builtin_amdgcn_readfirstlane(lds + (wave * IPW + q) * 1024));
         }
-#pragma unroll
-        for (int q = 0; q < IPW; q++)
-            load_lds<4>(base, off[q], lds + (wave * IPW + q) * 1024);
     }
 };
 
-// Fragments of an operand's slab: subtile i, 16 values of k from 16 kk on.
-template <int ROWS, bool T> struct SlabReader {
-    uint32_t at[T ? 2 : 4];
+// Fragments of an operand's slab: subtile i of S, 32 values of k from 32 kk on.
+template <int ROWS, int S, bool T> struct SlabReader {
+    uint32_t at[T ? S : 2];
     // first: the wave's first row or column of the slab.
     __device__ __forceinline__ void init(uint32_t first)
     {
         const uint32_t lane = threadIdx.x & 63;
         if constexpr (!T) {
-            // Row first + lane % 32, piece 2 kk + lane / 32.
+            // Row first + lane % 16, piece 4 kk + lane / 16.
 #pragma unroll
-            for (int kk = 0; kk < 4; kk++)
-                at[kk] = (first + (lane & 31)) * 128 + (((2 * kk + lane / 32) ^ (lane & 7)) * 16);
+            for (int kk = 0; kk < 2; kk++)
+                at[kk] = (first + (lane & 15)) * 128 + (((4 * kk + lane / 16) ^ (lane / 2 & 7)) * 16);
         } else {
-            // Lanes 16 g ..: columns 16 (g & 1) .., k 8 (g >> 1) ..; a lane reads 4 columns of row j / 4.
-            const uint32_t j = lane & 15, g = lane / 16, row = 8 * (g >> 1) + j / 4;
+            // Lanes 16 g ..: k 8 g .. of 16 columns; a lane reads 4 columns of row j / 4.
+            const uint32_t j = lane & 15, g = lane / 16, row = 8 * g + j / 4;
 #pragma unroll
-            for (int odd = 0; odd < 2; odd++) {
-                const uint32_t c = (first + 32 * odd + 16 * (g & 1)) / 8 + (j & 3) / 2;
-                at[odd] = row * ROWS * 2 + ((c ^ (2 * (j / 4))) * 16) + (j & 1) * 8;
+            for (int i = 0; i < S; i++) {
+                const uint32_t c = (first + 16 * i) / 8 + (j & 3) / 2;
+                at[i] = row * ROWS * 2 + ((c ^ k_major_swap(row)) * 16) + (j & 1) * 8;
             }
         }
     }
     __device__ __forceinline__ s16x8 read(const char *slab, int i, int kk) const
     {
         if constexpr (!T) {
-            return *reinterpret_cast<const s16x8 *>(slab + at[kk] + i * 32 * 128);
+            return *reinterpret_cast<const s16x8 *>(slab + at[kk] + i * 16 * 128);
         } else {
-            // Subtiles i and i + 2 lie 128 bytes apart whatever the permutation (it moves pieces
-            // within 128 bytes).
-            const char *p = slab + at[i & 1] + (i >> 1) * 128 + kk * 16 * ROWS * 2;
+            const char *p = slab + at[i] + kk * 32 * ROWS * 2;
             typedef __attribute__((address_space(3))) s16x4 *P;
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(p));
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(p + 4 * ROWS * 2));
@@ -160,25 +164,23 @@ __device__ __forceinline__ EntropyTile entropy_tile(uint32_t bid, uint32_t tiles
 template <typename E, class Cfg, bool TA, bool TB>
 __device__ __forceinline__ void entropy_product(const EntropyOperand &a, const EntropyOperand &b, uint32_t pairs, uint32_t m0,
                                                 uint32_t n0, uint32_t k_lo, uint32_t k_hi, char *lds,
-                                                f32x16 (&acc)[Cfg::SM][Cfg::SN])
+                                                f32x4 (&acc)[Cfg::SM][Cfg::SN])
 {
     constexpr int SM = Cfg::SM, SN = Cfg::SN;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     SlabLoader<Cfg, Cfg::BM, TA> la;
     SlabLoader<Cfg, Cfg::BN, TB> lb;
-    SlabReader<Cfg::BM, TA> ra;
-    SlabReader<Cfg::BN, TB> rb;
+    SlabReader<Cfg::BM, SM, TA> ra;
+    SlabReader<Cfg::BN, SN, TB> rb;
     la.init(a, m0, wave);
     lb.init(b, n0, wave);
-    ra.init(wave / Cfg::WN * SM * 32);
-    rb.init(wave % Cfg::WN * SN * 32);
+    ra.init(wave / Cfg::WN * SM * 16);
+    rb.init(wave % Cfg::WN * SN * 16);
 #pragma unroll
     for (int i = 0; i < SM; i++)
 #pragma unroll
         for (int j = 0; j < SN; j++)
-#pragma unroll
-            for (int r = 0; r < 16; r++)
-                acc[i][j][r] = 0.0f;
+            acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     if (k_lo >= k_hi)
         return;
     const uint32_t lds0 = lds_address(lds);
@@ -196,14 +198,14 @@ __device__ __forceinline__ void entropy_product(const EntropyOperand &a, const E
     auto compute = [&](int stage) __attribute__((always_inline)) {
         const char *sa = lds + stage * Cfg::kStage, *sb = sa + Cfg::kSlabA;
 #pragma unroll
-        for (int kk = 0; kk < 4; kk++) {
+        for (int kk = 0; kk < kSlabK / 32; kk++) {
             s16x8 fa[SM], fb[SN];
-#pragma unroll
-            for (int i = 0; i < SM; i++)
-                fa[i] = ra.read(sa, i, kk);
 #pragma unroll
             for (int j = 0; j < SN; j++)
                 fb[j] = rb.read(sb, j, kk);
+#pragma unroll
+            for (int i = 0; i < SM; i++)
+                fa[i] = ra.read(sa, i, kk);
 #pragma unroll
             for (int i = 0; i < SM; i++)
 #pragma unroll
