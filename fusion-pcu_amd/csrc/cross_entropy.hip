@@ -156,15 +156,18 @@ __device__ __forceinline__ void prepare_rows(const PrepArgs &p, const NodeGate &
         *p.row.factor = most / p.boost;
 }
 
-// The features packed and the rows prepared, by one launch.
-template <typename S> __global__ __launch_bounds__(256) void k_entropy_open(PackArgs g, PrepArgs p)
+// The features packed (by `blocks` workgroups), the weights packed if they are to be kept, and the
+// rows prepared, by one launch.
+template <typename S> __global__ __launch_bounds__(256) void k_entropy_open(PackArgs g, uint32_t blocks, PackArgs w, PrepArgs p)
 {
     if (block_gate_closed(g.gate))
         return;
     if (blockIdx.x == 0)
         prepare_rows(p, g.gate);
+    else if (blockIdx.x <= blocks)
+        pack_rows<S>(g, blockIdx.x - 1, blocks);
     else
-        pack_rows<S>(g, blockIdx.x - 1, gridDim.x - 1);
+        pack_rows<S>(w, blockIdx.x - 1 - blocks, gridDim.x - 1 - blocks);
 }
 
 // ----------------------------------------------------------------------- tiles
@@ -177,6 +180,8 @@ struct LogitArgs {
     RowData row{};
     float2 *partial = nullptr; // [tile of the vocabulary][partial_ld], the loss
     uint32_t partial_ld = 0, partial_first = 0;
+    uint32_t join = 0;         // the gradient: so many tiles' sums of a row to join first (0: they are joined)
+    float *loss = nullptr;
     uint16_t *grad = nullptr;  // [row][grad_ld], the gradient, and its parts
     uint64_t grad_plane = 0;
     uint32_t grad_ld = 0;
@@ -191,6 +196,30 @@ __device__ __forceinline__ float2 join_sums(float2 a, float2 b)
     return make_float2(m, a.y * exp2_fast((a.x - from) * kLog2e) + b.y * exp2_fast((b.x - from) * kLog2e));
 }
 
+// A row's share k of 16 of its tiles' sums, in order; share 0 joined with the others, in order, is the
+// row's. Both ways that a row's sums are joined go by this.
+__device__ __forceinline__ float2 join_share(const float2 *partial, uint32_t ld, uint32_t tiles, uint32_t n, uint32_t k)
+{
+    constexpr uint32_t U = 4;
+    float2 a = make_float2(-INFINITY, 0.0f);
+    for (uint32_t t = k; t < tiles; t += 16 * U) {
+        float2 b[U];
+#pragma unroll
+        for (uint32_t q = 0; q < U; q++)
+            b[q] = t + 16 * q < tiles ? partial[(uint64_t)(t + 16 * q) * ld + n] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+        for (uint32_t q = 0; q < U; q++)
+            a = join_sums(a, b[q]);
+    }
+    return a;
+}
+__device__ __forceinline__ float log_of(float2 a)
+{
+    const float from = a.x == -INFINITY ? 0.0f : a.x;
+    // A NaN among the logits is not in the maximum, but in the sum.
+    return (float)((double)from + (double)__builtin_amdgcn_logf(a.y) * kLn2);
+}
+
 // Vocabulary down, rows across: a lane holds 4 SM logits of each of its SN rows.
 template <typename S, class Cfg, bool GRAD> __global__ __launch_bounds__(Cfg::kThreads) void k_logits(LogitArgs g)
 {
@@ -201,6 +230,22 @@ template <typename S, class Cfg, bool GRAD> __global__ __launch_bounds__(Cfg::kT
         return;
     const EntropyTile t = entropy_tile(blockIdx.x, g.tiles_m, g.tiles_n, 1);
     const uint32_t m0 = t.tm * BM, n0 = t.tn * BN;
+    float *own_sum = reinterpret_cast<float *>(lds + Cfg::kTile);
+    if (GRAD && g.join) {
+        float2 *share = reinterpret_cast<float2 *>(lds);
+        for (uint32_t i = threadIdx.x; i < 16u * BN; i += Cfg::kThreads)
+            share[i] = join_share(g.partial, g.partial_ld, g.join, n0 + i % BN, i / BN);
+        __syncthreads();
+        for (uint32_t c = threadIdx.x; c < (uint32_t)BN; c += Cfg::kThreads) {
+            float2 a = share[c];
+            for (int q = 1; q < 16; q++)
+                a = join_sums(a, share[q * BN + c]);
+            const float l = own_sum[c] = log_of(a);
+            if (t.tm == 0 && g.first == 0 && g.loss && n0 + c < g.rows)
+                g.loss[n0 + c] = g.row.label[n0 + c] >= 0 ? l - g.row.own[n0 + c] : 0.0f;
+        }
+        __syncthreads();
+    }
     f32x4 acc[SM][SN];
     entropy_product<E, Cfg, false, false>(g.w, g.x, g.pairs, m0, n0, 0, g.slabs, lds, acc);
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
@@ -263,7 +308,8 @@ template <typename S, class Cfg, bool GRAD> __global__ __launch_bounds__(Cfg::kT
             const uint32_t n = n0 + wn + acc_col(j);
             const bool in = n < g.rows;
             const int32_t label = in ? g.row.label[n] : -1;
-            const float scale = in ? g.row.scale[n] * g.boost : 0.0f, log_sum = in ? g.row.log_sum[n] : 0.0f;
+            const float scale = in ? g.row.scale[n] * g.boost : 0.0f;
+            const float log_sum = g.join ? own_sum[n - n0] : in ? g.row.log_sum[n] : 0.0f;
             const bool mine = label >= 0 && (uint32_t)label - v0 < SM * 16u;
 #pragma unroll
             for (int i = 0; i < SM; i++)
@@ -315,39 +361,27 @@ template <typename S, class Cfg, bool GRAD> __global__ __launch_bounds__(Cfg::kT
 
 // Each row's log-sum-exp from its tiles', and its loss: 16 rows a workgroup, 16 threads each.
 __global__ __launch_bounds__(256) void k_entropy_loss(const float2 *partial, uint32_t ld, uint32_t tiles, uint32_t rows, RowData row,
-                                                      float *loss, float *log_sum, NodeGate gate)
+                                                      float *loss, float *log_sum, NodeGate gate, ProgramClose close)
 {
     __shared__ float2 red[16][16];
     if (block_gate_closed(gate))
         return;
     const uint32_t c = threadIdx.x & 15, k = threadIdx.x / 16, n = blockIdx.x * 16 + c;
-    float2 a = make_float2(-INFINITY, 0.0f);
-    if (n < rows) {
-        constexpr uint32_t U = 4;
-        for (uint32_t t = k; t < tiles; t += 16 * U) {
-            float2 b[U];
-#pragma unroll
-            for (uint32_t q = 0; q < U; q++)
-                b[q] = t + 16 * q < tiles ? partial[(uint64_t)(t + 16 * q) * ld + n] : make_float2(-INFINITY, 0.0f);
-#pragma unroll
-            for (uint32_t q = 0; q < U; q++)
-                a = join_sums(a, b[q]);
-        }
-    }
-    red[k][c] = a;
+    red[k][c] = n < rows ? join_share(partial, ld, tiles, n, k) : make_float2(0.0f, 0.0f);
     __syncthreads();
-    if (k || n >= rows)
-        return;
-    for (int q = 1; q < 16; q++)
-        a = join_sums(a, red[q][c]);
-    const float from = a.x == -INFINITY ? 0.0f : a.x;
-    // A NaN among the logits is not in the maximum, but in the sum.
-    const float l = (float)((double)from + (double)__builtin_amdgcn_logf(a.y) * kLn2);
-    row.log_sum[n] = l;
-    if (log_sum)
-        log_sum[n] = l;
-    if (loss)
-        loss[n] = row.label[n] >= 0 ? l - row.own[n] : 0.0f;
+    if (k == 0 && n < rows) {
+        float2 a = red[0][c];
+        for (int q = 1; q < 16; q++)
+            a = join_sums(a, red[q][c]);
+        const float l = log_of(a);
+        row.log_sum[n] = l;
+        // Stored past the caches, in case the launch ends its program.
+        if (log_sum)
+            put(log_sum + n, l);
+        if (loss)
+            put(loss + n, row.label[n] >= 0 ? l - row.own[n] : 0.0f);
+    }
+    program_close_block(close);
 }
 
 struct ProductArgs {
@@ -367,14 +401,11 @@ struct ProductArgs {
 };
 
 // dx: width down (from the weights, k-major), rows across (G); sums in binary32, k split.
-template <typename S, class Cfg> __global__ __launch_bounds__(Cfg::kThreads) void k_feature_gradient(ProductArgs g)
+template <typename S, class Cfg> __device__ __forceinline__ void feature_tile(const ProductArgs &g, uint32_t block, char *lds)
 {
     using E = typename ElemOf<S>::T;
     constexpr int SM = Cfg::SM, SN = Cfg::SN;
-    extern __shared__ __align__(16) char lds[];
-    if (block_gate_closed(g.gate))
-        return;
-    const EntropyTile t = entropy_tile(blockIdx.x, g.tiles_m, g.tiles_n, g.splits);
+    const EntropyTile t = entropy_tile(block, g.tiles_m, g.tiles_n, g.splits);
     const uint32_t m0 = t.tm * Cfg::BM, n0 = t.tn * Cfg::BN;
     const uint32_t k_lo = (uint32_t)((uint64_t)g.slabs * t.split / g.splits), k_hi = (uint32_t)((uint64_t)g.slabs * (t.split + 1) / g.splits);
     f32x4 acc[SM][SN];
@@ -388,11 +419,18 @@ template <typename S, class Cfg> __global__ __launch_bounds__(Cfg::kThreads) voi
             *to = g.add ? *to + acc[i][j] : acc[i][j];
         }
 }
+template <typename S, class Cfg> __global__ __launch_bounds__(Cfg::kThreads) void k_feature_gradient(ProductArgs g)
+{
+    extern __shared__ __align__(16) char lds[];
+    if (!block_gate_closed(g.gate))
+        feature_tile<S, Cfg>(g, blockIdx.x, lds);
+}
 
 // dx from the splits' sums, in their order.
 template <typename S>
 __global__ __launch_bounds__(256) void k_feature_join(const float *sums, uint64_t split, uint32_t splits, uint32_t ld, uint32_t rows,
-                                                      uint32_t cols, const float *factor, S *out, uint64_t out_ld, NodeGate gate)
+                                                      uint32_t cols, const float *factor, S *out, uint64_t out_ld, NodeGate gate,
+                                                      ProgramClose close)
 {
     if (block_gate_closed(gate))
         return;
@@ -416,19 +454,27 @@ __global__ __launch_bounds__(256) void k_feature_join(const float *sums, uint64_
 #pragma unroll
         for (int e = 0; e < V; e++)
             v[e] *= f;
-        store_vec(out + r * out_ld, c, cols, v, false);
+        S *row = out + r * out_ld;
+        if (close.words && (c + 1) * V <= cols) {
+            put_vec(row + c * V, pack<S>(v));
+        } else if (close.words) {
+#pragma unroll
+            for (int e = 0; e < V; e++)
+                if (c * V + e < cols)
+                    put(row + c * V + e, (S)v[e]);
+        } else {
+            store_vec(row, c, cols, v, false);
+        }
     }
+    program_close_block(close);
 }
 
 // dW: width down (from the features, k-major), vocabulary across (G, k-major).
-template <typename S, class Cfg> __global__ __launch_bounds__(Cfg::kThreads) void k_weight_gradient(ProductArgs g)
+template <typename S, class Cfg> __device__ __forceinline__ void weight_tile(const ProductArgs &g, uint32_t block, char *lds)
 {
     using E = typename ElemOf<S>::T;
     constexpr int SM = Cfg::SM, SN = Cfg::SN, BM = Cfg::BM, BN = Cfg::BN;
-    extern __shared__ __align__(16) char lds[];
-    if (block_gate_closed(g.gate))
-        return;
-    const EntropyTile t = entropy_tile(blockIdx.x, g.tiles_m, g.tiles_n, 1);
+    const EntropyTile t = entropy_tile(block, g.tiles_m, g.tiles_n, 1);
     const uint32_t m0 = t.tm * BM, n0 = t.tn * BN;
     f32x4 acc[SM][SN];
     entropy_product<E, Cfg, true, true>(g.a, g.b, g.pairs, m0, n0, 0, g.slabs, lds, acc);
@@ -478,6 +524,25 @@ template <typename S, class Cfg> __global__ __launch_bounds__(Cfg::kThreads) voi
                     to[e] = from[e];
         }
     }
+}
+
+template <typename S, class Cfg> __global__ __launch_bounds__(Cfg::kThreads) void k_weight_gradient(ProductArgs g)
+{
+    extern __shared__ __align__(16) char lds[];
+    if (!block_gate_closed(g.gate))
+        weight_tile<S, Cfg>(g, blockIdx.x, lds);
+}
+// Both in one launch, `features` workgroups for the first: neither fills the CUs alone.
+template <typename S, class CfgF, class CfgW> __global__ __launch_bounds__(CfgF::kThreads) void k_both_gradients(ProductArgs f, uint32_t features, ProductArgs w)
+{
+    static_assert(CfgF::kThreads == CfgW::kThreads, "one kind of workgroup");
+    extern __shared__ __align__(16) char lds[];
+    if (block_gate_closed(f.gate))
+        return;
+    if (blockIdx.x < features)
+        feature_tile<S, CfgF>(f, blockIdx.x, lds);
+    else
+        weight_tile<S, CfgW>(w, blockIdx.x - features, lds);
 }
 
 // Rows of zeros: of the weights' gradient past the vocabulary, or where there are no rows.
@@ -531,6 +596,7 @@ struct EntropyPlan {
     uint64_t piece;        // vocabulary of a piece, a multiple of 256
     Side logits, features, weights;
     uint32_t splits, sums_ld;
+    uint64_t sums_rows;
     uint64_t x, w, partial, grad, sums, label, scale, log_sum, own, factor, bytes;
 
     explicit EntropyPlan(const EntropyArgs &g)
@@ -562,9 +628,10 @@ struct EntropyPlan {
         weights = choose(g.width, piece < g.vocab ? piece : g.vocab, false);
         const uint64_t tiles = tiles_of(features, g.width, g.rows);
         const uint64_t per = features == Side::Large ? 1 : features == Side::Half ? 3 : 2; // workgroups a CU
-        const uint64_t want = tiles ? (per * kGfx950Cus + tiles / 2) / tiles : 1, most = (piece + 4 * kSlabK - 1) / (4 * kSlabK);
+        const uint64_t want = tiles ? (per * kGfx950Cus + tiles / 2) / tiles : 1, most = (piece + kSlabK - 1) / kSlabK;
         splits = (uint32_t)(want < 1 ? 1 : want > most ? (most ? most : 1) : want);
         sums_ld = (uint32_t)round_up(g.width, 256);
+        sums_rows = round_up(g.rows, side_n(features));
         bytes = 0;
         auto take = [&](uint64_t n) {
             const uint64_t at = bytes;
@@ -575,7 +642,7 @@ struct EntropyPlan {
         w = take(pack_weights ? (keep_weights ? vocab_up : piece) * row_bytes : 0);
         partial = take(g.log_sum_in ? 0 : (vocab_up / 128) * rows_up * 8);
         grad = take(grads ? piece * rows_up * 2 * parts : 0);
-        sums = take(g.feature_gradient ? splits * rows_up * sums_ld * 4ull : 0);
+        sums = take(g.feature_gradient ? splits * sums_rows * sums_ld * 4ull : 0);
         label = take(g.rows * 4);
         scale = take(g.rows * 4);
         log_sum = take(g.rows * 4);
@@ -631,13 +698,34 @@ template <typename S, class Cfg> hipError_t run_weights(hipStream_t s, ProductAr
     return hipGetLastError();
 }
 
+// Tiles of a row whose sums the gradient's workgroups join themselves, instead of a launch before.
+constexpr uint32_t kJoinTiles = 32;
+
 inline unsigned pack_blocks(uint64_t rows, uint64_t ld)
 {
     const uint64_t n = (rows * (ld / 8) + 255) / 256;
     return (unsigned)(n < 1 ? 1 : n > 8192 ? 8192 : n);
 }
 
-template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyArgs &g, void *scratch)
+// Features' and weights' gradients of a piece in one launch, the weights' by 128 x 128 tiles.
+template <typename S, class Cfg>
+hipError_t run_both(hipStream_t s, ProductArgs f, ProductArgs w, uint64_t width, uint64_t rows, uint64_t vocab_rows)
+{
+    f.tiles_m = (uint32_t)((width + Cfg::BM - 1) / Cfg::BM);
+    f.tiles_n = (uint32_t)((rows + Cfg::BN - 1) / Cfg::BN);
+    w.tiles_m = (uint32_t)((width + Middle::BM - 1) / Middle::BM);
+    w.tiles_n = (uint32_t)((vocab_rows + Middle::BN - 1) / Middle::BN);
+    constexpr uint32_t lds = Cfg::kLds > Middle::kLds ? Cfg::kLds : Middle::kLds;
+    hipError_t e = with_lds(k_both_gradients<S, Cfg, Middle>, lds);
+    if (e)
+        return e;
+    const uint32_t features = f.tiles_m * f.tiles_n * f.splits;
+    hipLaunchKernelGGL((k_both_gradients<S, Cfg, Middle>), dim3(features + w.tiles_m * w.tiles_n), dim3(Cfg::kThreads), lds, s, f,
+                       features, w);
+    return hipGetLastError();
+}
+
+template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyArgs &g, void *scratch, ProgramClose close, bool *closed)
 {
     const EntropyPlan p(g);
     char *sc = static_cast<char *>(scratch);
@@ -668,35 +756,40 @@ template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyAr
     pp.boost = kBoost<S>;
     pp.row = row;
     pp.fault = g.fault;
+    // Parts of kept weights: one plane after another over the whole vocabulary; of others, of a piece.
+    const uint64_t weight_plane = (p.keep_weights ? round_up(g.vocab, 256) : p.piece) * p.ld;
+    auto pack_weights = [&](uint64_t v, uint64_t n, uint16_t *to) {
+        PackArgs pw;
+        pw.in = static_cast<const S *>(g.weights) + v * g.weight_stride;
+        pw.ld = g.weight_stride;
+        pw.rows = pw.out_rows = (uint32_t)n;
+        pw.cols = g.width;
+        pw.out = to;
+        pw.plane = weight_plane;
+        pw.out_ld = p.ld;
+        pw.gate = g.gate;
+        return pw;
+    };
+    uint16_t *const packed = reinterpret_cast<uint16_t *>(sc + p.w);
     if (g.rows) {
-        hipLaunchKernelGGL((k_entropy_open<S>), dim3(1 + pack_blocks(p.rows_up, p.ld)), dim3(256), 0, s, px, pp);
+        const unsigned bx = pack_blocks(p.rows_up, p.ld), bw = p.keep_weights && g.vocab ? pack_blocks(g.vocab, p.ld) : 0;
+        hipLaunchKernelGGL((k_entropy_open<S>), dim3(1 + bx + bw), dim3(256), 0, s, px, bx, pack_weights(0, g.vocab, packed), pp);
         if ((e = hipGetLastError()))
             return e;
     }
 
     const EntropyOperand x{px.out, px.plane, p.ld, (uint32_t)p.rows_up, p.ld};
-    // The weights of vocabulary [v, v + n), packed by this call where they have to be.
-    auto weights = [&](uint64_t v, uint64_t n, bool packed, EntropyOperand *o) {
-        const S *from = static_cast<const S *>(g.weights) + v * g.weight_stride;
+    // The weights of vocabulary [v, v + n), packed here where they are not kept.
+    auto weights = [&](uint64_t v, uint64_t n, EntropyOperand *o) {
         if (!p.pack_weights) {
-            *o = EntropyOperand{reinterpret_cast<const uint16_t *>(from), 0, (uint32_t)g.weight_stride, (uint32_t)n, g.width};
+            *o = EntropyOperand{static_cast<const uint16_t *>(g.weights) + v * g.weight_stride, 0, (uint32_t)g.weight_stride,
+                                (uint32_t)n, g.width};
             return hipSuccess;
         }
-        uint16_t *to = reinterpret_cast<uint16_t *>(sc + p.w) + (p.keep_weights ? v * p.ld : 0);
-        const uint64_t plane = (p.keep_weights ? round_up(g.vocab, 256) : p.piece) * p.ld;
-        *o = EntropyOperand{to, plane, p.ld, (uint32_t)n, p.ld};
-        if (packed)
+        *o = EntropyOperand{p.keep_weights ? packed + v * p.ld : packed, weight_plane, p.ld, (uint32_t)n, p.ld};
+        if (p.keep_weights)
             return hipSuccess;
-        PackArgs pw;
-        pw.in = from;
-        pw.ld = g.weight_stride;
-        pw.rows = pw.out_rows = (uint32_t)n;
-        pw.cols = g.width;
-        pw.out = to;
-        pw.plane = plane;
-        pw.out_ld = p.ld;
-        pw.gate = g.gate;
-        hipLaunchKernelGGL((k_pack<S>), dim3(pack_blocks(n, p.ld)), dim3(256), 0, s, pw);
+        hipLaunchKernelGGL((k_pack<S>), dim3(pack_blocks(n, p.ld)), dim3(256), 0, s, pack_weights(v, n, packed));
         return hipGetLastError();
     };
 
@@ -720,7 +813,7 @@ template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyAr
         uint32_t tiles = 0;
         for (uint64_t v = 0; v < g.vocab; v += step) {
             const uint64_t n = g.vocab - v < step ? g.vocab - v : step;
-            if ((e = weights(v, n, false, &l.w)))
+            if ((e = weights(v, n, &l.w)))
                 return e;
             l.first = (uint32_t)v;
             l.partial_first = tiles;
@@ -728,10 +821,19 @@ template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyAr
                 return e;
             tiles += (uint32_t)((n + side_m(p.logits) - 1) / side_m(p.logits));
         }
-        hipLaunchKernelGGL(k_entropy_loss, dim3((unsigned)((g.rows + 15) / 16)), dim3(256), 0, s, l.partial, l.partial_ld, tiles,
-                           (uint32_t)g.rows, row, g.loss, g.log_sum_out, g.gate);
-        if ((e = hipGetLastError()))
-            return e;
+        // A few tiles' sums are joined by the gradient's workgroups, each for its rows.
+        if (p.grads && tiles > 0 && tiles <= kJoinTiles) {
+            l.join = tiles;
+            l.loss = g.loss;
+        } else {
+            const unsigned blocks = (unsigned)((g.rows + 15) / 16);
+            const ProgramClose c = !p.grads && blocks <= kCloseMaxBlocks ? close : ProgramClose{};
+            *closed = c.words != nullptr;
+            hipLaunchKernelGGL(k_entropy_loss, dim3(blocks), dim3(256), 0, s, l.partial, l.partial_ld, tiles, (uint32_t)g.rows, row,
+                               g.loss, g.log_sum_out, g.gate, c);
+            if ((e = hipGetLastError()))
+                return e;
+        }
     }
     if (!p.grads)
         return hipSuccess;
@@ -739,7 +841,7 @@ template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyAr
     ProductArgs f;
     f.pairs = pairs;
     f.sums = reinterpret_cast<float *>(sc + p.sums);
-    f.sums_split = p.rows_up * p.sums_ld;
+    f.sums_split = p.sums_rows * p.sums_ld;
     f.sums_ld = p.sums_ld;
     f.splits = p.splits;
     f.gate = g.gate;
@@ -756,17 +858,28 @@ template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyAr
     const uint64_t vocab = g.rows ? g.vocab : 0;
     for (uint64_t v = 0; v < vocab; v += p.piece) {
         const uint64_t n = vocab - v < p.piece ? vocab - v : p.piece;
-        if ((e = weights(v, n, p.keep_weights && whole_pass, &l.w)))
+        if ((e = weights(v, n, &l.w)))
             return e;
         l.first = (uint32_t)v;
         // Rows up to a whole slab: the weights' gradient reads those.
         if ((e = logits_by<S, true>(p.logits, s, l, n, round_up(g.rows, kSlabK))))
             return e;
+        f.a = l.w;
+        f.b = EntropyOperand{l.grad, l.grad_plane, l.grad_ld, (uint32_t)p.rows_up, l.grad_ld};
+        f.slabs = (uint32_t)((n + kSlabK - 1) / kSlabK);
+        f.add = v > 0;
+        d.b = EntropyOperand{l.grad, l.grad_plane, l.grad_ld, d.a.rows, l.grad_ld};
+        d.out = static_cast<S *>(g.weight_gradient) + v * g.weight_gradient_stride;
+        d.out_rows = (uint32_t)n;
+        if (g.feature_gradient && g.weight_gradient && p.weights == Side::Middle && p.features != Side::Large) {
+            e = p.features == Side::Middle ? run_both<S, Middle>(s, f, d, g.width, g.rows, n)
+                : p.features == Side::Half ? run_both<S, Half>(s, f, d, g.width, g.rows, n)
+                                           : run_both<S, Thin>(s, f, d, g.width, g.rows, n);
+            if (e)
+                return e;
+            continue;
+        }
         if (g.feature_gradient) {
-            f.a = l.w;
-            f.b = EntropyOperand{l.grad, l.grad_plane, l.grad_ld, (uint32_t)p.rows_up, l.grad_ld};
-            f.slabs = (uint32_t)((n + kSlabK - 1) / kSlabK);
-            f.add = v > 0;
             e = p.features == Side::Large    ? run_features<S, Large>(s, f, g.width, g.rows)
                 : p.features == Side::Middle ? run_features<S, Middle>(s, f, g.width, g.rows)
                 : p.features == Side::Half   ? run_features<S, Half>(s, f, g.width, g.rows)
@@ -775,27 +888,28 @@ template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyAr
                 return e;
         }
         if (g.weight_gradient) {
-            d.b = EntropyOperand{l.grad, l.grad_plane, l.grad_ld, d.a.rows, l.grad_ld};
-            d.out = static_cast<S *>(g.weight_gradient) + v * g.weight_gradient_stride;
-            d.out_rows = (uint32_t)n;
             e = p.weights == Side::Large ? run_weights<S, Large>(s, d, g.width, n) : run_weights<S, Middle>(s, d, g.width, n);
             if (e)
                 return e;
         }
     }
-    if (g.feature_gradient && g.rows) {
-        const uint64_t n = (g.rows * ((g.width + kVec<S> - 1) / kVec<S>) + 255) / 256;
-        hipLaunchKernelGGL((k_feature_join<S>), dim3((unsigned)(n > 8192 ? 8192 : n)), dim3(256), 0, s, f.sums, f.sums_split,
-                           vocab ? p.splits : 0, f.sums_ld, (uint32_t)g.rows, g.width, row.factor, static_cast<S *>(g.feature_gradient),
-                           g.feature_gradient_stride, g.gate);
-        if ((e = hipGetLastError()))
-            return e;
-    }
+    // Rows past the vocabulary first: the features' gradient may end the program.
     if (g.weight_gradient && g.weight_gradient_rows > vocab) {
         const uint64_t rows = g.weight_gradient_rows - vocab, n = (rows * ((g.width + kVec<S> - 1) / kVec<S>) + 255) / 256;
         hipLaunchKernelGGL((k_zero_rows<S>), dim3((unsigned)(n > 8192 ? 8192 : n)), dim3(256), 0, s,
                            static_cast<S *>(g.weight_gradient) + vocab * g.weight_gradient_stride, g.weight_gradient_stride, rows,
                            g.width, g.gate);
+        if ((e = hipGetLastError()))
+            return e;
+    }
+    if (g.feature_gradient && g.rows) {
+        const uint64_t n = (g.rows * ((g.width + kVec<S> - 1) / kVec<S>) + 255) / 256;
+        if (n > kCloseMaxBlocks)
+            close = ProgramClose{};
+        *closed = close.words != nullptr;
+        hipLaunchKernelGGL((k_feature_join<S>), dim3((unsigned)(n > 8192 ? 8192 : n)), dim3(256), 0, s, f.sums, f.sums_split,
+                           vocab ? p.splits : 0, f.sums_ld, (uint32_t)g.rows, g.width, row.factor, static_cast<S *>(g.feature_gradient),
+                           g.feature_gradient_stride, g.gate, close);
         return hipGetLastError();
     }
     return hipSuccess;
@@ -805,12 +919,13 @@ template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyAr
 
 size_t entropy_scratch_bytes(const EntropyArgs &g) { return EntropyPlan(g).bytes; }
 
-hipError_t launch_entropy(hipStream_t s, const EntropyArgs &g, void *scratch)
+hipError_t launch_entropy(hipStream_t s, const EntropyArgs &g, void *scratch, ProgramClose close, bool *closed)
 {
+    *closed = false;
     switch (g.dtype) {
-    case kLogitF32: return launch_entropy_t<float>(s, g, scratch);
-    case kLogitBf16: return launch_entropy_t<__bf16>(s, g, scratch);
-    default: return launch_entropy_t<_Float16>(s, g, scratch);
+    case kLogitF32: return launch_entropy_t<float>(s, g, scratch, close, closed);
+    case kLogitBf16: return launch_entropy_t<__bf16>(s, g, scratch, close, closed);
+    default: return launch_entropy_t<_Float16>(s, g, scratch, close, closed);
     }
 }
 

@@ -354,9 +354,17 @@ pcu_status Ctx::op_cross_entropy(const pcu_rows *features, const pcu_rows *weigh
         return st;
     if ((st = open_words()))
         return st;
+    ProgramClose close;
+    if (implicit_program && nodes.size() == 1)
+        close_next = true; // a call of its own: its last kernel ends the program
+    if ((st = take_close(&close)))
+        return st;
+    bool closed = false;
     hipEvent_t t = timer_start(stream);
-    st = hip(launch_entropy(stream, g, sc), "cross_entropy launch");
+    st = hip(launch_entropy(stream, g, sc, close, &closed), "cross_entropy launch");
     timer_stop(PCU_KERNEL_CROSS_ENTROPY, t, stream);
+    if (!st && closed)
+        closed_seq = ++pub_seq;
     return st;
 }
 

@@ -460,7 +460,7 @@ struct EntropyArgs {
     NodeGate gate{nullptr, 0};
 };
 size_t entropy_scratch_bytes(const EntropyArgs &g);
-hipError_t launch_entropy(hipStream_t s, const EntropyArgs &g, void *scratch);
+hipError_t launch_entropy(hipStream_t s, const EntropyArgs &g, void *scratch, ProgramClose close, bool *closed);
 
 // Small device utilities (fill kernels rather than memsets, so a captured graph replays
 // them as kernels).
