@@ -198,9 +198,8 @@ __device__ __forceinline__ float2 join_sums(float2 a, float2 b)
 
 // A row's share k of 16 of its tiles' sums, in order; share 0 joined with the others, in order, is the
 // row's. Both ways that a row's sums are joined go by this.
-__device__ __forceinline__ float2 join_share(const float2 *partial, uint32_t ld, uint32_t tiles, uint32_t n, uint32_t k)
+template <uint32_t U> __device__ __forceinline__ float2 join_share(const float2 *partial, uint32_t ld, uint32_t tiles, uint32_t n, uint32_t k)
 {
-    constexpr uint32_t U = 4;
     float2 a = make_float2(-INFINITY, 0.0f);
     for (uint32_t t = k; t < tiles; t += 16 * U) {
         float2 b[U];
@@ -221,7 +220,7 @@ __device__ __forceinline__ float log_of(float2 a)
 }
 
 // Vocabulary down, rows across: a lane holds 4 SM logits of each of its SN rows.
-template <typename S, class Cfg, bool GRAD> __global__ __launch_bounds__(Cfg::kThreads) void k_logits(LogitArgs g)
+template <typename S, class Cfg, bool GRAD, bool CARRY> __global__ __launch_bounds__(Cfg::kThreads) void k_logits(LogitArgs g)
 {
     using E = typename ElemOf<S>::T;
     constexpr int SM = Cfg::SM, SN = Cfg::SN, BM = Cfg::BM, BN = Cfg::BN;
@@ -234,7 +233,7 @@ template <typename S, class Cfg, bool GRAD> __global__ __launch_bounds__(Cfg::kT
     if (GRAD && g.join) {
         float2 *share = reinterpret_cast<float2 *>(lds);
         for (uint32_t i = threadIdx.x; i < 16u * BN; i += Cfg::kThreads)
-            share[i] = join_share(g.partial, g.partial_ld, g.join, n0 + i % BN, i / BN);
+            share[i] = join_share<2>(g.partial, g.partial_ld, g.join, n0 + i % BN, i / BN);
         __syncthreads();
         for (uint32_t c = threadIdx.x; c < (uint32_t)BN; c += Cfg::kThreads) {
             float2 a = share[c];
@@ -247,7 +246,7 @@ template <typename S, class Cfg, bool GRAD> __global__ __launch_bounds__(Cfg::kT
         __syncthreads();
     }
     f32x4 acc[SM][SN];
-    entropy_product<E, Cfg, false, false>(g.w, g.x, g.pairs, m0, n0, 0, g.slabs, lds, acc);
+    entropy_product<E, Cfg, false, false, CARRY>(g.w, g.x, g.pairs, m0, n0, 0, g.slabs, lds, acc);
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
     const uint32_t wm = wave / Cfg::WN * SM * 16, wn = wave % Cfg::WN * SN * 16;
     const uint32_t v0 = g.first + m0 + wm; // of acc[i][j][r]: v0 + acc_row(i, r)
@@ -367,7 +366,7 @@ __global__ __launch_bounds__(256) void k_entropy_loss(const float2 *partial, uin
     if (block_gate_closed(gate))
         return;
     const uint32_t c = threadIdx.x & 15, k = threadIdx.x / 16, n = blockIdx.x * 16 + c;
-    red[k][c] = n < rows ? join_share(partial, ld, tiles, n, k) : make_float2(0.0f, 0.0f);
+    red[k][c] = n < rows ? join_share<16>(partial, ld, tiles, n, k) : make_float2(0.0f, 0.0f);
     __syncthreads();
     if (k == 0 && n < rows) {
         float2 a = red[0][c];
@@ -396,7 +395,6 @@ struct ProductArgs {
     void *out = nullptr;   // [vocabulary][out_ld], the weights' gradient
     uint64_t out_ld = 0;
     uint32_t out_rows = 0, out_cols = 0;
-    int out_whole = 0;     // 16-byte stores are aligned and inside the rows
     NodeGate gate{nullptr, 0};
 };
 
@@ -409,7 +407,7 @@ template <typename S, class Cfg> __device__ __forceinline__ void feature_tile(co
     const uint32_t m0 = t.tm * Cfg::BM, n0 = t.tn * Cfg::BN;
     const uint32_t k_lo = (uint32_t)((uint64_t)g.slabs * t.split / g.splits), k_hi = (uint32_t)((uint64_t)g.slabs * (t.split + 1) / g.splits);
     f32x4 acc[SM][SN];
-    entropy_product<E, Cfg, true, false>(g.a, g.b, g.pairs, m0, n0, k_lo, k_hi, lds, acc);
+    entropy_product<E, Cfg, true, false, false>(g.a, g.b, g.pairs, m0, n0, k_lo, k_hi, lds, acc);
     const uint32_t wave = threadIdx.x / 64, m = m0 + wave / Cfg::WN * SM * 16, n = n0 + wave % Cfg::WN * SN * 16;
 #pragma unroll
     for (int j = 0; j < SN; j++)
@@ -440,16 +438,22 @@ __global__ __launch_bounds__(256) void k_feature_join(const float *sums, uint64_
     for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < (uint64_t)rows * pieces; i += (uint64_t)gridDim.x * 256) {
         const uint32_t r = (uint32_t)(i / pieces), c = (uint32_t)(i % pieces);
         float v[V] = {};
-        for (uint32_t s = 0; s < splits; s++) {
+        constexpr uint32_t U = 8; // splits under way together
+        for (uint32_t s = 0; s < splits; s += U) {
+            f32x4 x[U][V / 4];
             const float *from = sums + s * split + (uint64_t)r * ld + c * V;
 #pragma unroll
-            for (int q = 0; q < V; q += 4) {
-                const float4 x = *reinterpret_cast<const float4 *>(from + q);
-                v[q] += x.x;
-                v[q + 1] += x.y;
-                v[q + 2] += x.z;
-                v[q + 3] += x.w;
-            }
+            for (uint32_t u = 0; u < U; u++)
+                if (s + u < splits)
+#pragma unroll
+                    for (int q = 0; q < V / 4; q++)
+                        x[u][q] = *reinterpret_cast<const f32x4 *>(from + u * split + 4 * q);
+#pragma unroll
+            for (uint32_t u = 0; u < U; u++)
+                if (s + u < splits)
+#pragma unroll
+                    for (int e = 0; e < V; e++)
+                        v[e] += x[u][e / 4][e % 4];
         }
 #pragma unroll
         for (int e = 0; e < V; e++)
@@ -477,7 +481,7 @@ template <typename S, class Cfg> __device__ __forceinline__ void weight_tile(con
     const EntropyTile t = entropy_tile(block, g.tiles_m, g.tiles_n, 1);
     const uint32_t m0 = t.tm * BM, n0 = t.tn * BN;
     f32x4 acc[SM][SN];
-    entropy_product<E, Cfg, true, true>(g.a, g.b, g.pairs, m0, n0, 0, g.slabs, lds, acc);
+    entropy_product<E, Cfg, true, true, false>(g.a, g.b, g.pairs, m0, n0, 0, g.slabs, lds, acc);
     const uint32_t wave = threadIdx.x / 64, wm = wave / Cfg::WN * SM * 16, wn = wave % Cfg::WN * SN * 16;
     const float f = *g.factor;
     S *out = static_cast<S *>(g.out);
@@ -492,8 +496,9 @@ template <typename S, class Cfg> __device__ __forceinline__ void weight_tile(con
                 const uint32_t m = m0 + wm + acc_row(i, 0);
                 const f32x4 v = acc[i][j] * f;
                 float *to = out + (uint64_t)n * g.out_ld + m;
-                if (g.out_whole && m + 4 <= g.out_cols)
-                    *reinterpret_cast<f32x4 *>(to) = v;
+                typedef f32x4 f32x4_any __attribute__((aligned(4)));
+                if (m + 4 <= g.out_cols)
+                    *reinterpret_cast<f32x4_any *>(to) = v;
                 else
 #pragma unroll
                     for (int e = 0; e < 4; e++)
@@ -517,8 +522,8 @@ template <typename S, class Cfg> __device__ __forceinline__ void weight_tile(con
                 continue;
             const S *from = tile + n * Cfg::kOutPitch + c;
             S *to = out + (uint64_t)(n0 + n) * g.out_ld + m0 + c;
-            if (g.out_whole && m0 + c + 8 <= g.out_cols)
-                *reinterpret_cast<u32x4 *>(to) = *reinterpret_cast<const u32x4 *>(from);
+            if (m0 + c + 8 <= g.out_cols)
+                *reinterpret_cast<u32x4_any *>(to) = *reinterpret_cast<const u32x4 *>(from);
             else
                 for (uint32_t e = 0; e < 8 && m0 + c + e < g.out_cols; e++)
                     to[e] = from[e];
@@ -557,40 +562,46 @@ template <typename S> __global__ __launch_bounds__(256) void k_zero_rows(S *out,
 }
 
 // ---------------------------------------------------------------------- launches
-using Large = EntropyCfg<4, 2, 4, 8>;  // 256 x 256
-using Middle = EntropyCfg<2, 2, 4, 4>; // 128 x 128
-using Half = EntropyCfg<2, 2, 4, 2>;   // 128 x 64
-using Thin = EntropyCfg<4, 1, 4, 2>;   // 256 x 32
+using Large = EntropyCfg<4, 2, 4, 8, 2>;  // 256 x 256
+using Middle = EntropyCfg<2, 2, 4, 4, 2>; // 128 x 128
+using Half = EntropyCfg<2, 2, 4, 2, 3>;   // 128 x 64
+using Thin = EntropyCfg<4, 1, 2, 2, 3>;   // 128 x 32
 
 constexpr uint64_t round_up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
 
 enum class Side { Large, Middle, Half, Thin };
-inline uint32_t side_m(Side s) { return s == Side::Large || s == Side::Thin ? 256 : 128; }
+inline uint32_t side_m(Side s) { return s == Side::Large ? 256 : 128; }
 inline uint32_t side_n(Side s) { return s == Side::Large ? 256 : s == Side::Middle ? 128 : s == Side::Half ? 64 : 32; }
 inline uint64_t tiles_of(Side s, uint64_t m, uint64_t n)
 {
     return (m + side_m(s) - 1) / side_m(s) * ((n + side_n(s) - 1) / side_n(s));
 }
 
-// The tile of an m x n product, by the rounds that its tiles take on the CUs, in the time of a 128 x 128
-// tile at the larger one's rate: a round of 256 x 256 tiles (one a CU, 1450 TFLOP/s) takes 4, one of two
-// 128 x 128 tiles a CU (1050 TFLOP/s) 2.8, of one a CU 1.8. A product split along k fills its last round.
-inline Side choose(uint64_t m, uint64_t n, bool split)
+// What a slab of a pair of parts takes a round of tiles, in us: one 256 x 256 tile a CU (1450 TFLOP/s),
+// two of 128 x 128 (1050 TFLOP/s), and the narrower ones, which wait for their loads.
+inline double slab_us(Side s) { return s == Side::Large ? 1.5 : s == Side::Middle ? 1.0 : 0.6; }
+
+// The tile of an m x n product over so many slabs: by the rounds that the tiles take on the CUs, each
+// with its start and end (777 x 32003 x 1000: 83 us by 504 tiles of 256 x 256, 104 by 128 x 128), or,
+// where k can be split, by the whole work, unless a CU would have next to none of it.
+inline Side choose(uint64_t m, uint64_t n, uint64_t slabs, bool split)
 {
-    const double large = (double)tiles_of(Side::Large, m, n) / kGfx950Cus, middle = (double)tiles_of(Side::Middle, m, n) / kGfx950Cus;
+    const double large = (double)tiles_of(Side::Large, m, n) / kGfx950Cus, middle = (double)tiles_of(Side::Middle, m, n) / (2 * kGfx950Cus);
     if (split)
-        return 4 * large <= 1.4 * middle ? Side::Large : Side::Middle;
-    return 4 * std::ceil(large) <= (middle <= 1 ? 1.8 : 2.8 * std::ceil(middle / 2)) ? Side::Large : Side::Middle;
+        return large * slab_us(Side::Large) <= middle * slab_us(Side::Middle) && large * slabs >= 4 ? Side::Large : Side::Middle;
+    const auto rounds = [](double n) { return n <= 1 ? 1.0 : (n + std::ceil(n)) / 2; }; // a last one that few take runs faster
+    return rounds(large) * (14 + slabs * slab_us(Side::Large)) <= rounds(middle) * (8 + slabs * slab_us(Side::Middle)) ? Side::Large
+                                                                                                                     : Side::Middle;
 }
 // The same where n are the call's rows: few of them take narrower tiles, which read the weights at HBM's rate.
-inline Side choose_rows(uint64_t m, uint64_t rows, bool split)
+inline Side choose_rows(uint64_t m, uint64_t rows, uint64_t slabs, bool split)
 {
-    return rows <= 32 ? Side::Thin : rows <= 64 ? Side::Half : choose(m, rows, split);
+    return rows <= 32 ? Side::Thin : rows <= 64 ? Side::Half : choose(m, rows, slabs, split);
 }
 
 // How a call goes over its vocabulary and what its scratch holds.
 struct EntropyPlan {
-    bool grads, pack_weights, keep_weights;
+    bool grads, pack_weights, keep_weights, carry;
     uint32_t parts, ld;    // of packed rows
     uint64_t rows_up;      // rows with padding
     uint64_t piece;        // vocabulary of a piece, a multiple of 256
@@ -605,15 +616,20 @@ struct EntropyPlan {
         parts = g.dtype == kLogitF32 ? 3 : 1;
         ld = (uint32_t)round_up(g.width, kSlabK);
         rows_up = round_up(g.rows, 256);
-        // 16-bit weights are read in place where direct loads can: whole slabs, 16-byte pieces, and a
-        // tile's rows within 32-bit offsets.
-        pack_weights = parts == 3 || g.width % kSlabK || g.weight_stride % 8 || ((uintptr_t)g.weights & 15) ||
-                       g.weight_stride * 2 * 256 > UINT32_MAX;
+        // 16-bit weights are read in place where direct loads can: whole slabs, 16-byte pieces, a
+        // tile's rows within 32-bit offsets. Others go through registers for a loss, which reads them
+        // once, and are copied for the gradients (24 rows, vocabulary 97088, width 3098: 151 us against
+        // 390; a step of 29 rows, 34688 x 3211: three passes 324 us, the copy and three passes 248).
+        const bool direct = g.width % kSlabK == 0 && g.weight_stride % 8 == 0 && ((uintptr_t)g.weights & 15) == 0 &&
+                            g.weight_stride * 2 * 256 <= UINT32_MAX;
+        pack_weights = parts == 3 || (!direct && grads);
+        carry = !pack_weights && !direct;
         const uint64_t vocab_up = round_up(g.vocab, 256);
         const uint64_t row_bytes = 2ull * parts * ld;
         // G's piece is what the 256 MiB cache behind the L2s can hold; packed weights are kept
-        // for the second pass where they are no more than 512 MiB.
-        constexpr uint64_t kGradBytes = 192ull << 20, kWeightBytes = 512ull << 20;
+        // for the second pass where they are no more than 2 GiB (of 288 GB; splitting 1 GB of weights
+        // takes 450 us).
+        constexpr uint64_t kGradBytes = 192ull << 20, kWeightBytes = 2ull << 30;
         piece = kGradBytes / (rows_up ? rows_up * 2 * parts : 1) / 256 * 256;
         piece = piece < 256 ? 256 : piece > vocab_up ? vocab_up : piece;
         keep_weights = pack_weights && vocab_up * row_bytes <= kWeightBytes;
@@ -623,15 +639,19 @@ struct EntropyPlan {
             const uint64_t fit = kWeightBytes / row_bytes / 256 * 256;
             piece = piece < fit ? piece : fit < 256 ? 256 : fit;
         }
-        logits = choose_rows(g.vocab, g.rows, false);
-        features = choose_rows(g.width, g.rows, true);
-        weights = choose(g.width, piece < g.vocab ? piece : g.vocab, false);
+        const uint64_t pairs = parts == 3 ? kPartPairs : 1, within = piece < g.vocab ? piece : g.vocab, most = (within + kSlabK - 1) / kSlabK;
+        logits = choose_rows(g.vocab, g.rows, ld / kSlabK * pairs, false);
+        features = choose_rows(g.width, g.rows, most * pairs, true);
+        weights = choose(g.width, within, (g.rows + kSlabK - 1) / kSlabK * pairs, false);
         const uint64_t tiles = tiles_of(features, g.width, g.rows);
         const uint64_t per = features == Side::Large ? 1 : features == Side::Half ? 3 : 2; // workgroups a CU
-        const uint64_t want = tiles ? (per * kGfx950Cus + tiles / 2) / tiles : 1, most = (piece + kSlabK - 1) / kSlabK;
-        splits = (uint32_t)(want < 1 ? 1 : want > most ? (most ? most : 1) : want);
+        const uint64_t want = tiles ? (per * kGfx950Cus + tiles / 2) / tiles : 1;
         sums_ld = (uint32_t)round_up(g.width, 256);
         sums_rows = round_up(g.rows, side_n(features));
+        // Splits that fill the CUs, but no more than pay: a split's sums are written and read at 4 TB/s.
+        const double best = std::sqrt(most * pairs * slab_us(features) / (sums_rows * sums_ld * 8 / 4e6 + 1e-3));
+        const uint64_t pay = best < 1 ? 1 : (uint64_t)best, cut = want < pay ? want : pay;
+        splits = (uint32_t)(cut < 1 ? 1 : cut > most ? (most ? most : 1) : cut);
         bytes = 0;
         auto take = [&](uint64_t n) {
             const uint64_t at = bytes;
@@ -657,23 +677,30 @@ template <typename K> hipError_t with_lds(K *kernel, uint32_t bytes)
                          : hipSuccess;
 }
 
-template <typename S, class Cfg, bool GRAD> hipError_t run_logits(hipStream_t s, LogitArgs a, uint64_t vocab_rows, uint64_t rows)
+template <typename S, class Cfg, bool GRAD, bool CARRY> hipError_t run_logits(hipStream_t s, LogitArgs a, uint64_t vocab_rows, uint64_t rows)
 {
     a.tiles_m = (uint32_t)((vocab_rows + Cfg::BM - 1) / Cfg::BM);
     a.tiles_n = (uint32_t)((rows + Cfg::BN - 1) / Cfg::BN);
-    hipError_t e = with_lds(k_logits<S, Cfg, GRAD>, Cfg::kLds);
+    hipError_t e = with_lds(k_logits<S, Cfg, GRAD, CARRY>, Cfg::kLds);
     if (e)
         return e;
-    hipLaunchKernelGGL((k_logits<S, Cfg, GRAD>), dim3(a.tiles_m * a.tiles_n), dim3(Cfg::kThreads), Cfg::kLds, s, a);
+    hipLaunchKernelGGL((k_logits<S, Cfg, GRAD, CARRY>), dim3(a.tiles_m * a.tiles_n), dim3(Cfg::kThreads), Cfg::kLds, s, a);
     return hipGetLastError();
 }
-template <typename S, bool GRAD> hipError_t logits_by(Side side, hipStream_t s, const LogitArgs &a, uint64_t vocab_rows, uint64_t rows)
+template <typename S, class Cfg, bool GRAD> hipError_t logits_of(bool carry, hipStream_t s, const LogitArgs &a, uint64_t vocab_rows, uint64_t rows)
+{
+    if constexpr (sizeof(S) == 2 && !GRAD)
+        if (carry)
+            return run_logits<S, Cfg, GRAD, true>(s, a, vocab_rows, rows);
+    return run_logits<S, Cfg, GRAD, false>(s, a, vocab_rows, rows);
+}
+template <typename S, bool GRAD> hipError_t logits_by(Side side, bool carry, hipStream_t s, const LogitArgs &a, uint64_t vocab_rows, uint64_t rows)
 {
     switch (side) {
-    case Side::Large: return run_logits<S, Large, GRAD>(s, a, vocab_rows, rows);
-    case Side::Middle: return run_logits<S, Middle, GRAD>(s, a, vocab_rows, rows);
-    case Side::Half: return run_logits<S, Half, GRAD>(s, a, vocab_rows, rows);
-    default: return run_logits<S, Thin, GRAD>(s, a, vocab_rows, rows);
+    case Side::Large: return logits_of<S, Large, GRAD>(carry, s, a, vocab_rows, rows);
+    case Side::Middle: return logits_of<S, Middle, GRAD>(carry, s, a, vocab_rows, rows);
+    case Side::Half: return logits_of<S, Half, GRAD>(carry, s, a, vocab_rows, rows);
+    default: return logits_of<S, Thin, GRAD>(carry, s, a, vocab_rows, rows);
     }
 }
 
@@ -817,7 +844,7 @@ template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyAr
                 return e;
             l.first = (uint32_t)v;
             l.partial_first = tiles;
-            if ((e = logits_by<S, false>(p.logits, s, l, n, g.rows)))
+            if ((e = logits_by<S, false>(p.logits, p.carry, s, l, n, g.rows)))
                 return e;
             tiles += (uint32_t)((n + side_m(p.logits) - 1) / side_m(p.logits));
         }
@@ -852,8 +879,6 @@ template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyAr
     d.factor = row.factor;
     d.out_ld = g.weight_gradient_stride;
     d.out_cols = g.width;
-    constexpr uint32_t kStoreVec = 16 / sizeof(S);
-    d.out_whole = !((uintptr_t)g.weight_gradient & 15) && g.weight_gradient_stride % kStoreVec == 0;
     d.gate = g.gate;
     const uint64_t vocab = g.rows ? g.vocab : 0;
     for (uint64_t v = 0; v < vocab; v += p.piece) {
@@ -862,7 +887,7 @@ template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyAr
             return e;
         l.first = (uint32_t)v;
         // Rows up to a whole slab: the weights' gradient reads those.
-        if ((e = logits_by<S, true>(p.logits, s, l, n, round_up(g.rows, kSlabK))))
+        if ((e = logits_by<S, true>(p.logits, p.carry, s, l, n, round_up(g.rows, kSlabK))))
             return e;
         f.a = l.w;
         f.b = EntropyOperand{l.grad, l.grad_plane, l.grad_ld, (uint32_t)p.rows_up, l.grad_ld};

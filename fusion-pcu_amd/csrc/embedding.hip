@@ -543,8 +543,14 @@ template <typename S> __device__ __forceinline__ void fill_rows(const EmbedBackA
             atomicOr(&occurs[((uint32_t)t - row0) / 32], 1u << (((uint32_t)t - row0) & 31));
     }
     __syncthreads();
-    for (uint64_t i = lo + threadIdx.x; i < hi; i += 256) {
-        const uint32_t row = (uint32_t)(i / vecs), v = (uint32_t)(i % vecs);
+    // Row and vector of each step by addition: a division a vector is dearer than its store.
+    const uint32_t down = 256 / vecs, along = 256 % vecs;
+    uint32_t row = (uint32_t)((lo + threadIdx.x) / vecs), v = (uint32_t)((lo + threadIdx.x) % vecs);
+    for (uint64_t i = lo + threadIdx.x; i < hi; i += 256, row += down, v += along) {
+        if (v >= vecs) {
+            v -= vecs;
+            row++;
+        }
         if (occurs[(row - row0) / 32] >> ((row - row0) & 31) & 1)
             continue;
         typename StatOf<S>::T y[kVec<S>];
@@ -627,7 +633,7 @@ __device__ __forceinline__ void leave_part(const EmbedBackArgs &g, const uint32_
 // part c (terms c kLong ..) with its first row's sum at 2 c and its last row's at 2 c + 1.
 template <typename S, bool BASE>
 __global__ __launch_bounds__(256) void k_embed_sum(EmbedBackArgs g, const uint32_t *keys, const uint32_t *places, int lanes,
-                                                   uint32_t row_blocks, void *parts)
+                                                   uint32_t each, uint32_t row_blocks, void *parts)
 {
     using T = typename StatOf<S>::T;
     if (block_gate_closed(g.gate))
@@ -635,13 +641,13 @@ __global__ __launch_bounds__(256) void k_embed_sum(EmbedBackArgs g, const uint32
     const uint32_t n = (uint32_t)g.rows, lane = threadIdx.x & (lanes - 1), sub = threadIdx.x / lanes, subs = 256 / lanes;
     const uint32_t vecs = (g.width + kVec<S> - 1) / kVec<S>, v = blockIdx.y * lanes + lane;
     if (blockIdx.x < row_blocks) {
-        // kRowsAWave rows a wave: its lanes look them all up at once.
+        // `each` rows a wave (kRowsAWave at most): its lanes look them all up at once.
         __shared__ uint32_t lds_from[4][kRowsAWave + 1];
-        const uint32_t wave = threadIdx.x / 64, lane64 = threadIdx.x & 63, row0 = (blockIdx.x * 4 + wave) * kRowsAWave;
-        const uint32_t rows = row0 < g.vocab ? min(kRowsAWave, g.vocab - row0) : 0;
-        const uint32_t from = lower_bound(keys, n, min(row0 + min(lane64, kRowsAWave), g.vocab));
+        const uint32_t wave = threadIdx.x / 64, lane64 = threadIdx.x & 63, row0 = (blockIdx.x * 4 + wave) * each;
+        const uint32_t rows = row0 < g.vocab ? min(each, g.vocab - row0) : 0;
+        const uint32_t from = lower_bound(keys, n, min(row0 + min(lane64, each), g.vocab));
         if (lanes < 64) {
-            if (lane64 <= kRowsAWave)
+            if (lane64 <= each)
                 lds_from[wave][lane64] = from;
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             narrow_rows<S>(g, places, lds_from[wave], row0, rows, lanes, vecs);
@@ -754,7 +760,6 @@ template <typename S> hipError_t launch_embed_back_t(hipStream_t s, EmbedBackArg
     const uint32_t vecs = (g.width + kVec<S> - 1) / kVec<S>;
     const int lanes = row_lanes(vecs);
     const uint32_t across = (vecs + lanes - 1) / lanes;
-    const uint32_t row_blocks = (uint32_t)((g.vocab + 4 * kRowsAWave - 1) / (4 * kRowsAWave));
     if (g.rows <= kDirect) {
         const uint64_t all = g.base && g.base == g.out ? 0 : (uint64_t)g.vocab * vecs, wanted = (all + 1023) / 1024;
         const uint64_t fill = wanted < kFillBlocks ? wanted : kFillBlocks, each = fill ? ((all + fill - 1) / fill + 255) / 256 * 256 : 0;
@@ -793,11 +798,17 @@ template <typename S> hipError_t launch_embed_back_t(hipStream_t s, EmbedBackArg
         }
     }
     const uint32_t subs = 256 / lanes, part_blocks = (uint32_t)(((g.rows + kLong - 1) / kLong + subs - 1) / subs);
+    // Rows a wave, so that there are 8 waves a CU at least: the terms of one wave's rows are added one
+    // after another (46272 tokens, 479 x 768 bf16: 194 us with 16 rows a wave).
+    uint32_t each = kRowsAWave;
+    while (each > 1 && (uint64_t)g.vocab * across < (uint64_t)each * 8 * kGfx950Cus)
+        each /= 2;
+    const uint32_t row_blocks = (uint32_t)((g.vocab + 4 * each - 1) / (4 * each));
     const dim3 grid(row_blocks + part_blocks, across);
     if (g.base)
-        hipLaunchKernelGGL((k_embed_sum<S, true>), grid, dim3(256), 0, s, g, keys, places, lanes, row_blocks, sc + p.parts);
+        hipLaunchKernelGGL((k_embed_sum<S, true>), grid, dim3(256), 0, s, g, keys, places, lanes, each, row_blocks, sc + p.parts);
     else
-        hipLaunchKernelGGL((k_embed_sum<S, false>), grid, dim3(256), 0, s, g, keys, places, lanes, row_blocks, sc + p.parts);
+        hipLaunchKernelGGL((k_embed_sum<S, false>), grid, dim3(256), 0, s, g, keys, places, lanes, each, row_blocks, sc + p.parts);
     hipLaunchKernelGGL((k_embed_join<S>), dim3(part_blocks, across), dim3(256), 0, s, g, keys, lanes, sc + p.parts);
     return hipGetLastError();
 }

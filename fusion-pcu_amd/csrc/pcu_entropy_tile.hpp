@@ -2,7 +2,8 @@
 //
 // A workgroup makes a BM x BN tile of C = A B, k in slabs of 64. An operand's slab lies in LDS as
 // it lies in memory, either k-contiguous (64 values of a row of A or column of B side by side) or k-major
-// (`T`: 64 rows of BM or BN values), and comes there by direct loads, one slab ahead. A lane of the
+// (`T`: 64 rows of BM or BN values), and comes there by direct loads, one or more slabs ahead, or (A
+// alone, where its rows do not start at multiples of 16 bytes or end inside a slab) through registers. A lane of the
 // 16 x 16 x 32 instruction takes 8 consecutive k of one row or column: one 16-byte read of a
 // k-contiguous slab, two transposing 8-byte reads of a k-major one. The 16-byte pieces of a slab's
 // row are permuted by the row (in the loads' addresses, so that LDS stays dense): by half of it
@@ -36,13 +37,13 @@ template <typename E> __device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, 
 
 constexpr int kSlabK = 64;
 
-// WM x WN waves, each with SM x SN subtiles of 16 x 16.
-template <int WM_, int WN_, int SM_, int SN_> struct EntropyCfg {
-    static constexpr int WM = WM_, WN = WN_, SM = SM_, SN = SN_;
+// WM x WN waves, each with SM x SN subtiles of 16 x 16; STAGES slabs in LDS.
+template <int WM_, int WN_, int SM_, int SN_, int STAGES> struct EntropyCfg {
+    static constexpr int WM = WM_, WN = WN_, SM = SM_, SN = SN_, kStages = STAGES;
     static constexpr int BM = WM * SM * 16, BN = WN * SN * 16, kWaves = WM * WN, kThreads = 64 * kWaves;
     static constexpr int kSlabA = BM * kSlabK * 2, kSlabB = BN * kSlabK * 2, kStage = kSlabA + kSlabB; // bytes
     static constexpr int kOutPitch = BM + 8; // of a 16-bit output tile in LDS, in values
-    static constexpr int kTile = 2 * kStage > BN * kOutPitch * 2 ? 2 * kStage : BN * kOutPitch * 2;
+    static constexpr int kTile = kStages * kStage > BN * kOutPitch * 2 ? kStages * kStage : BN * kOutPitch * 2;
     static constexpr int kReduce = WM * BN * 8; // bytes for a reduction over the tile's rows
     static constexpr int kLds = kTile + kReduce;
 };
@@ -53,6 +54,7 @@ __device__ __forceinline__ uint32_t acc_col(int j) { return 16 * j + (threadIdx.
 // One operand: `ld` values from row to row (k-contiguous: rows of C; k-major: k), `plane` from one
 // 16-bit part of a binary32 operand to the next. Past `rows` rows and (k-major) `cols` columns the last
 // ones are read again: what they give is not stored, or meets zeros in the other operand.
+// Through registers, what lies past `cols` (of k, too) is zero and never read.
 struct EntropyOperand {
     const uint16_t *p = nullptr;
     uint64_t plane = 0;
@@ -102,6 +104,40 @@ template <class Cfg, int ROWS, bool T> struct SlabLoader {
             }
             load_lds<4>(base, from, __builtin_amdgcn_readfirstlane(lds + (wave * IPW + q) * 1024));
         }
+    }
+};
+
+// The same through registers, for rows at any alignment of their type and of any length.
+template <class Cfg, int ROWS, bool T> struct SlabCarrier {
+    static constexpr int IPW = ROWS / 8 / Cfg::kWaves, kPieces = (T ? ROWS : kSlabK) / 8;
+    u32x4 held[IPW];
+    __device__ __forceinline__ void fetch(const EntropyOperand &o, uint32_t at, uint32_t k0, int wave)
+    {
+        const uint32_t lane = threadIdx.x & 63;
+        const bool ragged = (T ? at + ROWS : k0 + kSlabK) > o.cols;
+#pragma unroll
+        for (int q = 0; q < IPW; q++) {
+            const uint32_t r = ((wave * IPW + q) * 64 + lane) / kPieces, piece = lane % kPieces;
+            const uint32_t row = min((T ? k0 : at) + r, o.rows - 1);
+            const uint32_t c = (T ? at : k0) + (T ? piece ^ k_major_swap(r) : piece ^ (r / 2 & 7)) * 8;
+            const uint16_t *from = o.p + (uint64_t)row * o.ld + c;
+            if (!ragged || c + 8 <= o.cols) {
+                held[q] = *reinterpret_cast<const u32x4_any *>(from);
+            } else {
+                u32x4 raw = {0, 0, 0, 0};
+#pragma unroll
+                for (uint32_t e = 0; e < 8; e++)
+                    if (c + e < o.cols)
+                        raw[e / 2] |= (uint32_t)from[e] << (16 * (e & 1));
+                held[q] = raw;
+            }
+        }
+    }
+    __device__ __forceinline__ void stash(char *slab, int wave) const
+    {
+#pragma unroll
+        for (int q = 0; q < IPW; q++)
+            *reinterpret_cast<u32x4 *>(slab + (wave * IPW + q) * 1024 + (threadIdx.x & 63) * 16) = held[q];
     }
 };
 
@@ -160,8 +196,9 @@ __device__ __forceinline__ EntropyTile entropy_tile(uint32_t bid, uint32_t tiles
 }
 
 // acc = the tile of A B over slabs [k_lo, k_hi) of each pair of parts. a, b: the operands; m0, n0: the
-// tile's first row and column; lds: Cfg::kTile bytes. No LDS is read after the last barrier.
-template <typename E, class Cfg, bool TA, bool TB>
+// tile's first row and column; lds: Cfg::kTile bytes. CARRY: A goes through registers (one part alone).
+// No LDS is read after the last barrier.
+template <typename E, class Cfg, bool TA, bool TB, bool CARRY>
 __device__ __forceinline__ void entropy_product(const EntropyOperand &a, const EntropyOperand &b, uint32_t pairs, uint32_t m0,
                                                 uint32_t n0, uint32_t k_lo, uint32_t k_hi, char *lds,
                                                 f32x4 (&acc)[Cfg::SM][Cfg::SN])
@@ -169,10 +206,12 @@ __device__ __forceinline__ void entropy_product(const EntropyOperand &a, const E
     constexpr int SM = Cfg::SM, SN = Cfg::SN;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     SlabLoader<Cfg, Cfg::BM, TA> la;
+    SlabCarrier<Cfg, Cfg::BM, TA> ca;
     SlabLoader<Cfg, Cfg::BN, TB> lb;
     SlabReader<Cfg::BM, SM, TA> ra;
     SlabReader<Cfg::BN, SN, TB> rb;
-    la.init(a, m0, wave);
+    if constexpr (!CARRY)
+        la.init(a, m0, wave);
     lb.init(b, n0, wave);
     ra.init(wave / Cfg::WN * SM * 16);
     rb.init(wave % Cfg::WN * SN * 16);
@@ -188,7 +227,10 @@ __device__ __forceinline__ void entropy_product(const EntropyOperand &a, const E
     uint32_t pair = kPartPairs - pairs, slab = k_lo;
     const uint32_t steps = pairs * (k_hi - k_lo);
     auto issue = [&](int stage) __attribute__((always_inline)) {
-        la.load(a, m0, part_a(pair), slab * kSlabK, lds0 + stage * Cfg::kStage, wave);
+        if constexpr (CARRY)
+            ca.fetch(a, m0, slab * kSlabK, wave);
+        else
+            la.load(a, m0, part_a(pair), slab * kSlabK, lds0 + stage * Cfg::kStage, wave);
         lb.load(b, n0, part_b(pair), slab * kSlabK, lds0 + stage * Cfg::kStage + Cfg::kSlabA, wave);
         if (++slab == k_hi) {
             slab = k_lo;
@@ -213,23 +255,54 @@ __device__ __forceinline__ void entropy_product(const EntropyOperand &a, const E
                     acc[i][j] = mfma16<E>(fa[i], fb[j], acc[i][j]);
         }
     };
-    issue(0);
-    wait_lds_loads();
-    __syncthreads();
-    // Two slabs a trip, so that each stage's addresses are constants.
-    for (uint32_t s = 0; s < steps; s += 2) {
-        if (s + 1 < steps)
-            issue(1);
-        compute(0);
-        wait_lds_loads();
-        __syncthreads();
-        if (s + 1 < steps) {
-            if (s + 2 < steps)
-                issue(0);
-            compute(1);
+    if constexpr (Cfg::kStages == 2 || CARRY) {
+        auto arrive = [&](int stage) __attribute__((always_inline)) {
+            if constexpr (CARRY)
+                ca.stash(lds + stage * Cfg::kStage, wave); // (again what was fetched last, past the last slab)
             wait_lds_loads();
             __syncthreads();
+        };
+        issue(0);
+        arrive(0);
+        // Two slabs a trip, so that each stage's addresses are constants. (The conditions stand where
+        // the compiler keeps the sums in registers: leaving the loop amid a trip spilled them.)
+        for (uint32_t s = 0; s < steps; s += 2) {
+            if (s + 1 < steps)
+                issue(1);
+            compute(0);
+            arrive(1);
+            if (s + 1 < steps) {
+                if (s + 2 < steps)
+                    issue(0);
+                compute(1);
+                arrive(0);
+            }
         }
+    } else {
+        // kStages - 1 slabs ahead. A slab is there when no more than the later ones' loads are
+        // outstanding and every wave has come to the barrier; then every wave is done with the slab
+        // before, too, whose stage the next load takes.
+        constexpr int N = Cfg::kStages, kLoads = SlabLoader<Cfg, Cfg::BM, TA>::IPW + SlabLoader<Cfg, Cfg::BN, TB>::IPW;
+#pragma unroll
+        for (int st = 0; st < N - 1; st++)
+            if ((uint32_t)st < steps)
+                issue(st);
+        for (uint32_t s = 0; s < steps; s += N) {
+#pragma unroll
+            for (int st = 0; st < N; st++) {
+                if (s + st >= steps)
+                    break;
+                if (s + st + N - 2 < steps)
+                    wait_loads_but<(N - 2) * kLoads>();
+                else
+                    wait_lds_loads();
+                __syncthreads();
+                if (s + st + N - 1 < steps)
+                    issue((st + N - 1) % N);
+                compute(st);
+            }
+        }
+        __syncthreads();
     }
 }
 
