@@ -4,7 +4,7 @@
 //   grad[v] = base[v] + scale * (sum of g[i] over the i with t_i = v, i ascending)
 //
 // The gradient sorts the tokens (stable, so a row's terms are added in one order whatever the
-// launch did), then every row of the table is written once by the lanes that own it: no atomics on
+// launch did); then every row of the table is written once, by the lanes that own it: no atomics on
 // values, no second pass over the table to clear it. Both directions are bound by HBM.
 #include "pcu_logits.hpp"
 
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_scan(EmbedBackArgs g, int
 // Moves a tile's keys and places to where the digit's order puts them: after all smaller digits,
 // and after the digit in the tiles before.
 __global__ __launch_bounds__(kSortThreads) void k_sort_move(EmbedBackArgs g, const uint32_t *keys, const uint32_t *places,
-                                                            int shift, int bits, const uint32_t *counts, const uint32_t *totals,
+                                                            int shift, int bits, const uint32_t *counts, const uint32_t *totals, uint32_t tiles,
                                                             uint32_t *keys_out, uint32_t *places_out)
 {
     extern __shared__ uint32_t lds[];
@@ -249,12 +249,19 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_move(EmbedBackArgs g, con
     uint32_t k[kSortRounds], rank[kSortRounds];
     rank_tile([&](uint64_t i) { return keys ? keys[i] : token_key(g.tokens, i, g.vocab); }, g.rows,
               (uint64_t)blockIdx.x * kSortTile, shift, bits, k, rank, wave_count);
-    for (uint32_t b = threadIdx.x; b < bins; b += kSortThreads)
-        first[b] = totals[b];
+    // A digit's count in all tiles; without totals (few tiles) the tiles' counts are added up here.
+    for (uint32_t b = threadIdx.x; b < bins; b += kSortThreads) {
+        uint32_t all = totals ? totals[b] : 0;
+        for (uint32_t t = 0; !totals && t < tiles; t++)
+            all += counts[(uint64_t)t * bins + b];
+        first[b] = all;
+    }
     __syncthreads();
     scan_bins(first, bins, part);
     for (uint32_t b = threadIdx.x; b < bins; b += kSortThreads) {
-        uint32_t at = first[b] + counts[(uint64_t)blockIdx.x * bins + b];
+        uint32_t at = first[b] + (totals ? counts[(uint64_t)blockIdx.x * bins + b] : 0);
+        for (uint32_t t = 0; !totals && t < blockIdx.x; t++)
+            at += counts[(uint64_t)t * bins + b];
         for (int w = 0; w < kSortWaves; w++) {
             const uint32_t n = wave_count[w * bins + b];
             wave_count[w * bins + b] = at;
@@ -330,34 +337,27 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_one(EmbedBackArgs g, int 
 }
 
 // --------------------------------------------------------------------- summing
-// First of the n sorted keys that is at least v.
+// First of the n sorted keys that is at least v; a wave looks at 64 of them at a time.
 __device__ __forceinline__ uint32_t lower_bound(const uint32_t *keys, uint32_t n, uint32_t v)
 {
     uint32_t lo = 0, len = n;
     while (len > 0) {
-        const uint32_t half = len / 2;
-        if (keys[lo + half] < v) {
-            lo += half + 1;
-            len -= half + 1;
-        } else {
-            len = half;
-        }
+        const uint32_t step = (len + 63) / 64, at = (threadIdx.x & 63) * step;
+        const uint32_t below = (uint32_t)__popcll(__ballot(at < len && keys[lo + min(at, len - 1)] < v));
+        if (below == 0)
+            break;
+        const uint32_t skip = (below - 1) * step + 1;
+        lo += skip;
+        len = min(step - 1, len - skip);
     }
     return lo;
 }
 
-// Rows of more terms than this are added up by several waves, kLong terms each (aligned in the
-// sorted order), whose sums are added in order afterwards.
-constexpr uint32_t kLong = 64;
-
-// Where the terms of a key lie.
-struct Run {
-    uint32_t lo, hi;
-};
-__device__ __forceinline__ Run run_of(const uint32_t *keys, uint32_t n, uint32_t key)
-{
-    return Run{lower_bound(keys, n, key), lower_bound(keys, n, key + 1)};
-}
+// A wave takes the rows whose first term is one of kStarts sorted ones. Rows of more than kLong terms
+// are added up by several waves, kLong terms each (a part, aligned in the sorted order), whose sums are
+// added in order afterwards. The other rows that begin in a wave's share end within its 64 lanes.
+constexpr uint32_t kStarts = 16, kLong = 48;
+static_assert(kStarts - 1 + kLong < 64, "a short row's end is in sight");
 
 // sum += terms [lo, hi) of the sorted order, vector v of each, one after another.
 template <typename S, typename P, typename T>
@@ -411,109 +411,78 @@ template <typename S> __device__ __forceinline__ u32x4 load_base(const EmbedBack
     return g.base ? load_vec(static_cast<const S *>(g.base) + (uint64_t)row * g.base_stride, v, g.width) : u32x4{0, 0, 0, 0};
 }
 
-// Rows row0 + [0, rows) of the table by a wave, rows <= 16, but those of more than kLong terms; lane r
-// holds from, row r's first term (and lane `rows` the end), and term(j) gives a term's place. All
-// control is scalar: rows without terms keep their base; the others' terms are walked across the rows'
-// ends, so that their loads, and the bases' with them, are under way together. vec: the lane's vector.
-template <typename S, bool BASE, typename Term>
-__device__ __forceinline__ void wave_rows(const EmbedBackArgs &g, uint32_t row0, uint32_t rows, uint32_t from, uint32_t vec, bool on,
-                                          Term term)
+// Row sums of the runs of equal keys that begin at sorted terms [16 chunk, 16 chunk + 16), but long
+// ones. Rows of 64 vectors or more (lanes 64): all control is scalar, and the terms are walked across the
+// rows' ends, so that their loads, and the bases' with them, are under way together. Narrower rows: each
+// group of `lanes` lanes takes every so-manieth run. vec: the lane's vector.
+template <typename S, bool BASE>
+__device__ __forceinline__ void sum_runs(const EmbedBackArgs &g, const uint32_t *keys, const uint32_t *places, uint32_t chunk, int lanes,
+                                         uint32_t vec, bool on)
 {
     using T = typename StatOf<S>::T;
     constexpr int U = BASE ? 4 : 8, V = kVec<S>;
-    const uint32_t lane = threadIdx.x & 63, next = __shfl(from, lane + 1);
-    const uint32_t all = (1u << rows) - 1;
-    uint32_t empty = (uint32_t)__ballot(lane < rows && from == next) & all;
-    const uint32_t many = (uint32_t)__ballot(lane < rows && next - from > kLong) & all;
-    if (!BASE) {
-        const T zero[V] = {};
-        for (; empty; empty &= empty - 1)
-            if (on)
-                store_vec(static_cast<S *>(g.out) + (uint64_t)(row0 + __builtin_ctz(empty)) * g.out_stride, vec, g.width, zero, g.past);
-    } else if (g.base != g.out) {
-        while (empty) {
-            u32x4 raw[U];
-            uint32_t e = empty;
+    const uint32_t n = (uint32_t)g.rows, lane = threadIdx.x & 63, at = chunk * kStarts + lane;
+    const uint32_t key = at < n ? keys[at] : ~0u, place = at < n ? places[at] : 0;
+    uint32_t prev = __shfl_up(key, 1);
+    if (lane == 0)
+        prev = at > 0 ? keys[at - 1] : ~0u;
+    const uint64_t change = __ballot(key != prev), after = change >> 1 >> lane;
+    const uint32_t len = after ? (uint32_t)__builtin_ctzll(after) + 1 : 64 - lane; // beyond sight: long
+    const uint64_t starts = __ballot(lane < kStarts && key != prev && key < g.vocab && len <= kLong);
+    if (lanes == 64) {
+        const uint64_t upto = change & (~0ull >> (63 - lane));
+        uint64_t terms = __ballot(upto && (starts >> (63 - __builtin_clzll(upto | 1)) & 1));
+        const uint64_t lasts = terms & change >> 1;
+        T sum[V] = {};
+        while (terms) {
+            u32x4 raw[U], base[U];
+            uint64_t t = terms;
 #pragma unroll
-            for (int q = 0; q < U; q++, e &= e - 1)
-                if (e && on)
-                    raw[q] = load_base<S>(g, row0 + __builtin_ctz(e), vec);
-#pragma unroll
-            for (int q = 0; q < U; q++, empty &= empty - 1)
-                if (empty && on) {
-                    T y[V];
-                    unpack<S>(raw[q], y);
-                    store_vec(static_cast<S *>(g.out) + (uint64_t)(row0 + __builtin_ctz(empty)) * g.out_stride, vec, g.width, y, g.past);
-                }
-        }
-    }
-    T sum[V] = {};
-    for (uint32_t r = 0; r < rows;) {
-        // Rows [r, r_end) are not long.
-        const uint32_t rest = many >> r, r_end = rest ? r + __builtin_ctz(rest) : rows;
-        const uint32_t hi = from_lane(from, r_end);
-        for (uint32_t j0 = from_lane(from, r); j0 < hi; j0 += 64) {
-            const uint32_t n = min(hi - j0, 64u), place = lane < n ? term(j0 + lane) : 0;
-            for (uint32_t j = 0; j < n; j += U) {
-                u32x4 raw[U], base[U];
-                uint32_t row[U];
-#pragma unroll
-                for (int q = 0; q < U; q++) {
-                    row[q] = ~0u;
-                    if (j + q < n) {
-                        while (from_lane(next, r) <= j0 + j + q)
-                            r++;
-                        if (on)
-                            raw[q] = load_vec(static_cast<const S *>(g.gradient) + (uint64_t)from_lane(place, j + q) * g.gradient_stride, vec, g.width);
-                        if (from_lane(next, r) == j0 + j + q + 1) { // the row's last one
-                            row[q] = row0 + r;
-                            if (BASE && on)
-                                base[q] = load_base<S>(g, row[q], vec);
-                        }
+            for (int q = 0; q < U; q++, t &= t - 1)
+                if (t) {
+                    const int l = __builtin_ctzll(t);
+                    if (on) {
+                        raw[q] = load_vec(static_cast<const S *>(g.gradient) + (uint64_t)from_lane(place, l) * g.gradient_stride, vec, g.width);
+                        if (BASE && lasts >> l & 1)
+                            base[q] = load_base<S>(g, from_lane(key, l), vec);
                     }
                 }
 #pragma unroll
-                for (int q = 0; q < U; q++)
-                    if (j + q < n) {
-                        T x[V];
-                        unpack<S>(raw[q], x);
+            for (int q = 0; q < U; q++, terms &= terms - 1)
+                if (terms) {
+                    const int l = __builtin_ctzll(terms);
+                    T x[V];
+                    unpack<S>(raw[q], x);
+#pragma unroll
+                    for (int e = 0; e < V; e++)
+                        sum[e] += x[e];
+                    if (lasts >> l & 1) {
+                        if (on)
+                            write_sum<S>(g, from_lane(key, l), vec, base[q], sum);
 #pragma unroll
                         for (int e = 0; e < V; e++)
-                            sum[e] += x[e];
-                        if (row[q] != ~0u) {
-                            if (on)
-                                write_sum<S>(g, row[q], vec, base[q], sum);
-#pragma unroll
-                            for (int e = 0; e < V; e++)
-                                sum[e] = 0;
-                        }
+                            sum[e] = 0;
                     }
-            }
+                }
         }
-        r = r_end + 1;
+        return;
     }
-}
-
-// The same for rows of fewer than 64 vectors: `lanes` lanes a row, one row after another for each
-// group of lanes. from: in LDS.
-template <typename S, typename P>
-__device__ __forceinline__ void narrow_rows(const EmbedBackArgs &g, const P *places, const uint32_t *from, uint32_t row0, uint32_t rows,
-                                            int lanes, uint32_t vecs)
-{
-    using T = typename StatOf<S>::T;
-    const uint32_t lane = threadIdx.x & 63, v = lane & (lanes - 1);
-    for (uint32_t r = lane / lanes; r < rows; r += 64 / lanes) {
-        const uint32_t lo = from[r], hi = from[r + 1];
-        if (v >= vecs || hi - lo > kLong || (lo == hi && g.base && g.base == g.out))
-            continue;
-        const u32x4 base = load_base<S>(g, row0 + r, v);
-        T sum[kVec<S>] = {};
-        add_terms<S>(g, places, lo, hi, v, sum);
-        if (lo == hi) {
-            unpack<S>(base, sum);
-            store_vec(static_cast<S *>(g.out) + (uint64_t)(row0 + r) * g.out_stride, v, g.width, sum, g.past);
-        } else {
-            write_sum<S>(g, row0 + r, v, base, sum);
+    const uint32_t runs = (uint32_t)__popcll(starts), subs = 64 / lanes;
+    uint64_t left = starts;
+    for (uint32_t r = 0; r < runs; r += subs) {
+        // This group's run: the (lane / lanes)-th of those left.
+        uint64_t mine = left;
+        for (uint32_t k = 0; k < lane / lanes; k++)
+            mine &= mine - 1;
+        for (uint32_t k = 0; k < subs; k++)
+            left &= left - 1;
+        const int l = mine ? __builtin_ctzll(mine) : 0;
+        const uint32_t row = __shfl(key, l), terms = __shfl(len, l);
+        if (mine && on) {
+            const u32x4 base = load_base<S>(g, row, vec);
+            T sum[V] = {};
+            add_terms<S>(g, places + chunk * kStarts, l, l + terms, vec, sum);
+            write_sum<S>(g, row, vec, base, sum);
         }
     }
 }
@@ -525,22 +494,28 @@ __device__ __forceinline__ void narrow_rows(const EmbedBackArgs &g, const P *pla
 // 50257 x 768 F32: as two launches, all rows filled and then some written again, 22 and 10 us (a plain
 // fill of the 154 MB takes 22.6, past the caches 27); waves that looked for the tokens of 16 rows each
 // took 41 to 46, and sorting first 55 in three launches.
-constexpr uint32_t kDirect = 1024, kRowsAWave = 16, kFillBlocks = 8 * kGfx950Cus;
+constexpr uint32_t kDirect = 1024, kFillBlocks = 8 * kGfx950Cus;
 constexpr uint32_t kFillRows = (1u << 22) / kFillBlocks + 2; // rows that a workgroup's vectors can lie in
 
-template <typename S> __device__ __forceinline__ void fill_rows(const EmbedBackArgs &g, uint32_t block, uint64_t each, bool through)
+template <typename S>
+__device__ __forceinline__ void fill_rows(const EmbedBackArgs &g, const uint32_t *keys, uint32_t block, uint64_t each, bool through)
 {
     __shared__ uint32_t occurs[(kFillRows + 31) / 32];
     const uint32_t n = (uint32_t)g.rows, vecs = (g.width + kVec<S> - 1) / kVec<S>;
     const uint64_t lo = block * each, hi = min(lo + each, (uint64_t)g.vocab * vecs);
+    if (lo >= hi)
+        return;
     const uint32_t row0 = (uint32_t)(lo / vecs);
     for (uint32_t w = threadIdx.x; w < (kFillRows + 31) / 32; w += 256)
         occurs[w] = 0;
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n; i += 256) {
-        const int32_t t = g.tokens[i];
-        if (t >= 0 && (uint32_t)t - row0 < kFillRows)
-            atomicOr(&occurs[((uint32_t)t - row0) / 32], 1u << (((uint32_t)t - row0) & 31));
+    // The rows that occur, from the sorted keys or (few tokens) from all of them.
+    const uint32_t first = keys ? lower_bound(keys, n, row0) : 0;
+    const uint32_t last = keys ? lower_bound(keys, n, min((uint32_t)((hi - 1) / vecs) + 1, g.vocab)) : n;
+    for (uint32_t i = first + threadIdx.x; i < last; i += 256) {
+        const uint32_t t = keys ? keys[i] : (uint32_t)g.tokens[i]; // an absent one is no row's
+        if (t - row0 < kFillRows)
+            atomicOr(&occurs[(t - row0) / 32], 1u << ((t - row0) & 31));
     }
     __syncthreads();
     // Row and vector of each step by addition: a division a vector is dearer than its store.
@@ -555,7 +530,11 @@ template <typename S> __device__ __forceinline__ void fill_rows(const EmbedBackA
             continue;
         typename StatOf<S>::T y[kVec<S>];
         unpack<S>(load_base<S>(g, row, v), y);
-        store_row(static_cast<S *>(g.out) + (uint64_t)row * g.out_stride, v, g.width, y, through);
+        S *out = static_cast<S *>(g.out) + (uint64_t)row * g.out_stride;
+        if (through)
+            store_row(out, v, g.width, y, true);
+        else
+            store_vec(out, v, g.width, y, g.past);
     }
 }
 
@@ -567,7 +546,7 @@ __global__ __launch_bounds__(256) void k_embed_first(EmbedBackArgs g, uint32_t a
     if (block_gate_closed(g.gate))
         return;
     if (blockIdx.x >= sums) {
-        fill_rows<S>(g, blockIdx.x - sums, each, close.words != nullptr);
+        fill_rows<S>(g, nullptr, blockIdx.x - sums, each, close.words != nullptr);
         program_close_block(close);
         return;
     }
@@ -619,99 +598,131 @@ __global__ __launch_bounds__(256) void k_embed_first(EmbedBackArgs g, uint32_t a
     program_close_block(close);
 }
 
-template <typename S, typename T>
-__device__ __forceinline__ void leave_part(const EmbedBackArgs &g, const uint32_t *places, uint32_t lo, uint32_t hi, uint32_t v, T *out)
+// A part's rows at its ends: how many of its terms are its first key's and its last key's, and how many
+// terms more those keys have right before and behind the part (64 for 64 or more).
+struct Part {
+    uint32_t lo, hi, first, last, head, tail, before, behind;
+    __device__ __forceinline__ Part(const uint32_t *keys, uint32_t n, uint32_t c)
+    {
+        const uint32_t lane = threadIdx.x & 63;
+        lo = c * kLong;
+        hi = min(lo + kLong, n);
+        const uint32_t m = hi - lo, key = lane < m ? keys[lo + lane] : ~0u;
+        first = from_lane(key, 0);
+        last = from_lane(key, (int)m - 1);
+        const uint64_t in = (1ull << m) - 1; // m <= 48
+        head = (uint32_t)__builtin_ctzll(~(__ballot(key == first) & in));
+        tail = (uint32_t)__builtin_clzll(~((__ballot(key == last) & in) << (64 - m)));
+        before = run_length(lane < lo ? keys[lo - 1 - lane] : ~0u, first);
+        behind = run_length(hi + lane < n ? keys[hi + lane] : ~0u, last);
+    }
+    static __device__ __forceinline__ uint32_t run_length(uint32_t key, uint32_t of)
+    {
+        const uint64_t other = ~__ballot(key == of);
+        return other ? (uint32_t)__builtin_ctzll(other) : 64;
+    }
+    __device__ __forceinline__ bool head_long() const { return before + head + (head == hi - lo ? behind : 0) > kLong; }
+    __device__ __forceinline__ bool tail_long() const { return tail + behind + (tail == hi - lo ? before : 0) > kLong; }
+};
+
+// The sum of terms [lo, hi), vector vec, of a wave whose groups of `lanes` lanes take a share each.
+template <typename S>
+__device__ __forceinline__ void leave_part(const EmbedBackArgs &g, const uint32_t *places, uint32_t lo, uint32_t hi, int lanes, uint32_t vec,
+                                           bool on, typename StatOf<S>::T *out)
 {
-    T sum[kVec<S>] = {};
-    add_terms<S>(g, places, lo, hi, v, sum);
+    using T = typename StatOf<S>::T;
+    constexpr int V = kVec<S>;
+    const uint32_t lane = threadIdx.x & 63, subs = 64 / lanes, each = (hi - lo + subs - 1) / subs, sub = lane / lanes;
+    const uint32_t a = min(lo + sub * each, hi), b = min(a + each, hi);
+    T sum[V] = {};
+    if (on)
+        add_terms<S>(g, places, a, b, vec, sum);
+    T all[V];
 #pragma unroll
-    for (int e = 0; e < kVec<S>; e++)
-        out[e] = sum[e];
+    for (int e = 0; e < V; e++) {
+        all[e] = __shfl(sum[e], lane & (lanes - 1));
+        for (uint32_t k = 1; k < subs; k++)
+            all[e] += __shfl(sum[e], (lane & (lanes - 1)) + k * lanes);
+        if (on && sub == 0)
+            out[e] = all[e];
+    }
 }
 
-// Workgroups [0, row_blocks) write the table's rows; the others leave the sums of long rows' parts,
-// part c (terms c kLong ..) with its first row's sum at 2 c and its last row's at 2 c + 1.
+// Workgroups [0, runs): waves with the rows that begin in their terms; [runs, parts): waves that leave the
+// sums of long rows' parts, part c with its first row's sum at 2 c and its last row's at 2 c + 1; the
+// others fill the rows that do not occur. A wave takes 64 vectors of the rows, of `across`.
 template <typename S, bool BASE>
 __global__ __launch_bounds__(256) void k_embed_sum(EmbedBackArgs g, const uint32_t *keys, const uint32_t *places, int lanes,
-                                                   uint32_t each, uint32_t row_blocks, void *parts)
+                                                   uint32_t across, uint32_t runs, uint32_t parts, uint64_t each, void *sums)
 {
     using T = typename StatOf<S>::T;
     if (block_gate_closed(g.gate))
         return;
-    const uint32_t n = (uint32_t)g.rows, lane = threadIdx.x & (lanes - 1), sub = threadIdx.x / lanes, subs = 256 / lanes;
-    const uint32_t vecs = (g.width + kVec<S> - 1) / kVec<S>, v = blockIdx.y * lanes + lane;
-    if (blockIdx.x < row_blocks) {
-        // `each` rows a wave (kRowsAWave at most): its lanes look them all up at once.
-        __shared__ uint32_t lds_from[4][kRowsAWave + 1];
-        const uint32_t wave = threadIdx.x / 64, lane64 = threadIdx.x & 63, row0 = (blockIdx.x * 4 + wave) * each;
-        const uint32_t rows = row0 < g.vocab ? min(each, g.vocab - row0) : 0;
-        const uint32_t from = lower_bound(keys, n, min(row0 + min(lane64, each), g.vocab));
-        if (lanes < 64) {
-            if (lane64 <= each)
-                lds_from[wave][lane64] = from;
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            narrow_rows<S>(g, places, lds_from[wave], row0, rows, lanes, vecs);
-        } else if (rows) {
-            wave_rows<S, BASE>(g, row0, rows, from, v, v < vecs, [&](uint32_t j) { return places[j]; });
-        }
+    if (blockIdx.x >= parts) {
+        fill_rows<S>(g, keys, blockIdx.x - parts, each, false);
         return;
     }
-    const uint32_t c = (blockIdx.x - row_blocks) * subs + sub, lo = c * kLong;
-    if (lo >= n)
+    const uint32_t n = (uint32_t)g.rows, vecs = (g.width + kVec<S> - 1) / kVec<S>, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const bool of_runs = blockIdx.x < runs;
+    const uint32_t unit = (blockIdx.x - (of_runs ? 0 : runs)) * 4 + wave, c = unit / across;
+    const uint32_t vec = unit % across * 64 + (threadIdx.x & (lanes - 1));
+    if (of_runs) {
+        if (c * kStarts < n)
+            sum_runs<S, BASE>(g, keys, places, c, lanes, vec, vec < vecs);
         return;
-    const uint32_t hi = min(lo + kLong, n), first = keys[lo], last = keys[hi - 1];
-    const Run head = run_of(keys, n, first), tail = run_of(keys, n, last);
-    const bool leave_head = first < g.vocab && head.hi - head.lo > kLong;
-    const bool leave_tail = last != first && last < g.vocab && tail.hi - tail.lo > kLong;
-    if (v >= vecs)
+    }
+    if (c * kLong >= n)
         return;
-    T *out = static_cast<T *>(parts) + ((uint64_t)2 * c * vecs + v) * kVec<S>;
-    if (leave_head)
-        leave_part<S>(g, places, lo, min(hi, head.hi), v, out);
-    if (leave_tail)
-        leave_part<S>(g, places, tail.lo, hi, v, out + (uint64_t)vecs * kVec<S>);
+    const Part p(keys, n, c);
+    T *out = static_cast<T *>(sums) + ((uint64_t)2 * c * vecs + vec) * kVec<S>;
+    if (p.first < g.vocab && p.head_long())
+        leave_part<S>(g, places, p.lo, p.lo + p.head, lanes, vec, vec < vecs, out);
+    if (p.last != p.first && p.last < g.vocab && p.tail_long())
+        leave_part<S>(g, places, p.hi - p.tail, p.hi, lanes, vec, vec < vecs, out + (uint64_t)vecs * kVec<S>);
 }
 
 // The long rows, each by the part in which it begins.
 template <typename S>
-__global__ __launch_bounds__(256) void k_embed_join(EmbedBackArgs g, const uint32_t *keys, int lanes, const void *parts)
+__global__ __launch_bounds__(256) void k_embed_join(EmbedBackArgs g, const uint32_t *keys, int lanes, uint32_t across, const void *sums)
 {
     using T = typename StatOf<S>::T;
+    constexpr int V = kVec<S>;
     if (block_gate_closed(g.gate))
         return;
-    const uint32_t n = (uint32_t)g.rows, lane = threadIdx.x & (lanes - 1), subs = 256 / lanes;
-    const uint32_t vecs = (g.width + kVec<S> - 1) / kVec<S>, v = blockIdx.y * lanes + lane;
-    const uint32_t c = blockIdx.x * subs + threadIdx.x / lanes, lo = c * kLong;
-    if (lo >= n || v >= vecs)
+    const uint32_t n = (uint32_t)g.rows, vecs = (g.width + V - 1) / V, unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t c = unit / across, vec = unit % across * 64 + (threadIdx.x & 63);
+    if (c * kLong >= n)
         return;
-    const uint32_t first = keys[lo], last = keys[min(lo + kLong, n) - 1];
-    const Run run = run_of(keys, n, last);
-    if (last >= g.vocab || run.hi - run.lo <= kLong || run.lo < lo)
+    const Part p(keys, n, c);
+    if (p.last >= g.vocab || !p.tail_long() || (p.tail == p.hi - p.lo && p.before > 0))
         return;
-    const T *from = static_cast<const T *>(parts) + (uint64_t)v * kVec<S>;
-    const uint64_t part = (uint64_t)vecs * kVec<S>;
-    const uint32_t more = (run.hi - 1) / kLong - c; // parts after this one
-    T sum[kVec<S>];
+    const uint32_t end = p.behind < 64 ? p.hi + p.behind : lower_bound(keys, n, p.last + 1);
+    if (vec >= vecs || (threadIdx.x & 63) >= (uint32_t)lanes)
+        return;
+    const T *from = static_cast<const T *>(sums) + (uint64_t)vec * V;
+    const uint64_t part = (uint64_t)vecs * V;
+    const uint32_t more = (end - 1) / kLong - c; // parts after this one
+    T sum[V];
 #pragma unroll
-    for (int e = 0; e < kVec<S>; e++)
-        sum[e] = from[(2 * (uint64_t)c + (first == last ? 0 : 1)) * part + e];
-    constexpr uint32_t U = 4;
+    for (int e = 0; e < V; e++)
+        sum[e] = from[(2 * (uint64_t)c + (p.first == p.last ? 0 : 1)) * part + e];
+    constexpr uint32_t U = 8;
     for (uint32_t j = 1; j <= more; j += U) {
-        T x[U][kVec<S>];
+        T x[U][V];
 #pragma unroll
         for (uint32_t q = 0; q < U; q++)
             if (j + q <= more)
 #pragma unroll
-                for (int e = 0; e < kVec<S>; e++)
+                for (int e = 0; e < V; e++)
                     x[q][e] = from[2 * (uint64_t)(c + j + q) * part + e];
 #pragma unroll
         for (uint32_t q = 0; q < U; q++)
             if (j + q <= more)
 #pragma unroll
-                for (int e = 0; e < kVec<S>; e++)
+                for (int e = 0; e < V; e++)
                     sum[e] += x[q][e];
     }
-    write_sum<S>(g, last, v, load_base<S>(g, last, v), sum);
+    write_sum<S>(g, p.last, vec, load_base<S>(g, p.last, vec), sum);
 }
 
 // What the gradient's scratch holds: sorted keys and places, those of the first pass, the tiles'
@@ -747,6 +758,9 @@ struct EmbedPlan {
     }
 };
 
+// Tiles whose counts the moving workgroups add up themselves.
+constexpr uint32_t kFewTiles = 32;
+
 // A kernel whose LDS is beyond what a launch may have unasked.
 template <typename K> hipError_t allow_lds(K *kernel, uint32_t bytes)
 {
@@ -760,9 +774,10 @@ template <typename S> hipError_t launch_embed_back_t(hipStream_t s, EmbedBackArg
     const uint32_t vecs = (g.width + kVec<S> - 1) / kVec<S>;
     const int lanes = row_lanes(vecs);
     const uint32_t across = (vecs + lanes - 1) / lanes;
+    // Vectors of the table that are filled, if no row keeps its place, by how many workgroups.
+    const uint64_t all = g.base && g.base == g.out ? 0 : (uint64_t)g.vocab * vecs, wanted = (all + 1023) / 1024;
+    const uint64_t fill = wanted < kFillBlocks ? wanted : kFillBlocks, each = fill ? ((all + fill - 1) / fill + 255) / 256 * 256 : 0;
     if (g.rows <= kDirect) {
-        const uint64_t all = g.base && g.base == g.out ? 0 : (uint64_t)g.vocab * vecs, wanted = (all + 1023) / 1024;
-        const uint64_t fill = wanted < kFillBlocks ? wanted : kFillBlocks, each = fill ? ((all + fill - 1) / fill + 255) / 256 * 256 : 0;
         const uint32_t sums = (uint32_t)((g.rows * across + 3) / 4), blocks = sums + (uint32_t)fill;
         if (blocks == 0)
             return hipSuccess;
@@ -792,24 +807,20 @@ template <typename S> hipError_t launch_embed_back_t(hipStream_t s, EmbedBackArg
         for (int pass = 0; pass < 2; pass++) {
             const uint32_t *in = pass ? mid_keys : nullptr;
             hipLaunchKernelGGL(k_sort_count, dim3(p.tiles), dim3(kSortThreads), bins * 4, s, g, in, pass * p.bits, p.bits, counts);
-            hipLaunchKernelGGL(k_sort_scan, dim3(bins), dim3(kSortThreads), 0, s, g, p.bits, p.tiles, counts, totals);
+            if (p.tiles > kFewTiles)
+                hipLaunchKernelGGL(k_sort_scan, dim3(bins), dim3(kSortThreads), 0, s, g, p.bits, p.tiles, counts, totals);
             hipLaunchKernelGGL(k_sort_move, dim3(p.tiles), dim3(kSortThreads), p.lds, s, g, in, pass ? mid_places : nullptr,
-                               pass * p.bits, p.bits, counts, totals, pass ? keys : mid_keys, pass ? places : mid_places);
+                               pass * p.bits, p.bits, counts, p.tiles > kFewTiles ? totals : nullptr, p.tiles, pass ? keys : mid_keys, pass ? places : mid_places);
         }
     }
-    const uint32_t subs = 256 / lanes, part_blocks = (uint32_t)(((g.rows + kLong - 1) / kLong + subs - 1) / subs);
-    // Rows a wave, so that there are 8 waves a CU at least: the terms of one wave's rows are added one
-    // after another (46272 tokens, 479 x 768 bf16: 194 us with 16 rows a wave).
-    uint32_t each = kRowsAWave;
-    while (each > 1 && (uint64_t)g.vocab * across < (uint64_t)each * 8 * kGfx950Cus)
-        each /= 2;
-    const uint32_t row_blocks = (uint32_t)((g.vocab + 4 * each - 1) / (4 * each));
-    const dim3 grid(row_blocks + part_blocks, across);
+    const uint32_t runs = (uint32_t)(((g.rows + kStarts - 1) / kStarts * across + 3) / 4);
+    const uint32_t parts = (uint32_t)(((g.rows + kLong - 1) / kLong * across + 3) / 4);
+    const dim3 grid(runs + parts + (uint32_t)fill);
     if (g.base)
-        hipLaunchKernelGGL((k_embed_sum<S, true>), grid, dim3(256), 0, s, g, keys, places, lanes, each, row_blocks, sc + p.parts);
+        hipLaunchKernelGGL((k_embed_sum<S, true>), grid, dim3(256), 0, s, g, keys, places, lanes, across, runs, runs + parts, each, sc + p.parts);
     else
-        hipLaunchKernelGGL((k_embed_sum<S, false>), grid, dim3(256), 0, s, g, keys, places, lanes, each, row_blocks, sc + p.parts);
-    hipLaunchKernelGGL((k_embed_join<S>), dim3(part_blocks, across), dim3(256), 0, s, g, keys, lanes, sc + p.parts);
+        hipLaunchKernelGGL((k_embed_sum<S, false>), grid, dim3(256), 0, s, g, keys, places, lanes, across, runs, runs + parts, each, sc + p.parts);
+    hipLaunchKernelGGL((k_embed_join<S>), dim3(parts), dim3(256), 0, s, g, keys, lanes, across, sc + p.parts);
     return hipGetLastError();
 }
 

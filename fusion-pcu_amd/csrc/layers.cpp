@@ -100,11 +100,12 @@ pcu_status Ctx::op_embedding_backward(const pcu_rows *gradient, const int32_t *t
     pcu_status st = check_rows(this, "embedding gradient", gradient);
     if (st)
         return st;
-    if (table_rows > PCU_TABLE_MAX_ROWS) {
-        fail("embedding gradient: a table of %llu rows: beyond the limits", (unsigned long long)table_rows);
+    const uint64_t size = logit_size(gradient->dtype), cols = gradient->cols;
+    if (table_rows > PCU_TABLE_MAX_ROWS || gradient->rows * ((cols * size + 1023) / 1024) > 1ull << 28) {
+        fail("embedding gradient: %llu x %llu for a table of %llu rows: beyond the limits", (unsigned long long)gradient->rows,
+             (unsigned long long)cols, (unsigned long long)table_rows);
         return PCU_ERR_SHAPE;
     }
-    const uint64_t size = logit_size(gradient->dtype), cols = gradient->cols;
     if ((st = check_like(this, "embedding gradient: out", out, table_rows, cols, out_stride, size)) ||
         (base && (st = check_like(this, "embedding gradient: base", base, table_rows, cols, base_stride, size))))
         return st;
@@ -305,8 +306,9 @@ pcu_status Ctx::op_cross_entropy(const pcu_rows *features, const pcu_rows *weigh
         return PCU_ERR_UNSUPPORTED;
     }
     const uint64_t rows = features->rows, width = features->cols, size = logit_size(features->dtype);
+    constexpr uint64_t kMost = 1ull << 37; // of any two of the sizes: the launches' grids
     if (width != weights->cols || width < 1 || width > PCU_ENTROPY_MAX_WIDTH || rows > PCU_ENTROPY_MAX_ROWS ||
-        weights->rows > PCU_TABLE_MAX_ROWS) {
+        weights->rows > PCU_TABLE_MAX_ROWS || rows * weights->rows > kMost || rows * width > kMost || width * weights->rows > kMost) {
         fail("cross_entropy: %llu x %llu features, %llu x %llu weights", (unsigned long long)rows, (unsigned long long)width,
              (unsigned long long)weights->rows, (unsigned long long)weights->cols);
         return PCU_ERR_SHAPE;

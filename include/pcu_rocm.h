@@ -369,7 +369,8 @@ pcu_status pcu_native_embedding(pcu_ctx *ctx, const pcu_rows *table, const int32
 /* The gradient by the table: out[v] = base[v] + scale * (the sum of gradient[i] over the i with
  * tokens[i] = v, in their order) for each of table_rows rows; base may be NULL (zeros) or out itself
  * (same stride: rows whose token does not occur keep their bits and are not touched), else it overlaps nothing that is written.
- * Negative tokens are left out; one of table_rows or more is a fault. */
+ * Negative tokens are left out; one of table_rows or more is a fault. At most 2^28 rows of 1 KiB
+ * (or less) each, or as much in longer ones. */
 pcu_status pcu_native_embedding_backward(pcu_ctx *ctx, const pcu_rows *gradient,
                                          const int32_t *tokens, uint64_t table_rows, double scale,
                                          const void *base, uint64_t base_stride, void *out,
@@ -404,7 +405,7 @@ pcu_status pcu_native_layer_norm_backward(pcu_ctx *ctx, const pcu_rows *x, const
  * weights.rows or more is a fault (element_index: the row). loss, log_sum and row_scale (NULL: 1)
  * are F32. Sums are F32; F32 operands enter with 24 bits; G is rounded to the operands' precision, which
  * for F16 holds what is above 2^-38 of the largest row_scale. */
-#define PCU_ENTROPY_MAX_ROWS (1u << 22)
+#define PCU_ENTROPY_MAX_ROWS (1u << 22) /* and the product of any two of the three sizes at most 2^37 */
 #define PCU_ENTROPY_MAX_WIDTH (1u << 16) /* and at least 1 */
 /* log_sum may be NULL. */
 pcu_status pcu_native_cross_entropy_loss(pcu_ctx *ctx, const pcu_rows *features,

@@ -405,6 +405,8 @@ def test_refusals(ctx, pcu_pkg):
     assert loss(h, R(big.ptr, r=(1 << 22) + 1), R(w.ptr, 30), y.ptr, out.ptr, None, None) == S
     assert loss(h, R(big.ptr), R(w.ptr, (1 << 22) + 1), y.ptr, out.ptr, None, None) == S
     assert loss(h, R(big.ptr, c=(1 << 16) + 1, s=1 << 17), R(w.ptr, 30, (1 << 16) + 1, 1 << 17), y.ptr, out.ptr, None, None) == S
+    assert loss(h, R(big.ptr, r=1 << 22), R(w.ptr, 1 << 16), y.ptr, out.ptr, None, None) == S
+    assert loss(h, R(big.ptr, c=1 << 16, s=1 << 16), R(w.ptr, 1 << 22, 1 << 16, 1 << 16), y.ptr, out.ptr, None, None) == S
     step = lib.pcu_native_cross_entropy_step
     assert step(h, R(x.ptr), R(w.ptr, 30), y.ptr, None, out.ptr, None, 0, out.ptr + 64, 29, 8, None) == S
     assert step(h, R(x.ptr), R(w.ptr, 30), y.ptr, None, out.ptr, out.ptr + 64, 7, None, 0, 0, None) == S

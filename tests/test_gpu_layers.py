@@ -169,7 +169,7 @@ def _tokens(rng, count, vocab, how):
 
 
 def _sum_in_order(pkg, g, tokens, vocab, base, scale, dtype):
-    """The definition, each term added in its place, in the statistics' type (rows of at most 64)."""
+    """The definition, each term added in its place, in the statistics' type."""
     stat = np.float64 if dtype == "f64" else np.float32
     acc = np.zeros((vocab, g.shape[1]), stat)
     with np.errstate(invalid="ignore"):
@@ -184,9 +184,9 @@ def _sum_in_order(pkg, g, tokens, vocab, base, scale, dtype):
 @pytest.mark.parametrize("count,vocab,width", BACK_SHAPES)
 @pytest.mark.parametrize("how", ["text", "one", "absent"])
 def test_embedding_backward_sums_each_tokens_rows(ctx, pcu_pkg, count, vocab, width, how, dtype):
-    """Rows of at most 64 terms are added one after another: the same bits. Longer ones are off by
-    at most one rounding a term (64 a part and the parts after them), one for the scale and one for
-    the base; the bound counts n + 4 of the magnitudes' sum."""
+    """Rows of at most 48 terms, and all rows of at most 1024 tokens, are added one after another: the
+    same bits. Longer ones are off by at most one rounding a term (of a part, then of the parts), one for
+    the scale and one for the base; the bound counts n + 4 of the magnitudes' sum."""
     rng = np.random.default_rng(count + vocab + width)
     tokens = _tokens(rng, count, vocab, how)
     g, gv = _stored(pcu_pkg, rng.normal(0, 1, (count, width)), dtype)
@@ -197,7 +197,7 @@ def test_embedding_backward_sums_each_tokens_rows(ctx, pcu_pkg, count, vocab, wi
         got = ctx.native_embedding_backward(ctx.upload(g), ctx.upload(tokens), vocab, scale=scale, base=dev_b).numpy()
         counts = np.bincount(tokens[tokens >= 0], minlength=vocab)
         want = _sum_in_order(pcu_pkg, g, tokens, vocab, b, scale, dtype)
-        short = counts <= 64
+        short = counts <= (1024 if count <= 1024 else 48)
         rounded, _ = _stored(pcu_pkg, want, dtype)
         np.testing.assert_array_equal(_bits(got)[short], _bits(rounded)[short])
         if not np.all(short):
@@ -216,13 +216,13 @@ def test_embedding_backward_sums_each_tokens_rows(ctx, pcu_pkg, count, vocab, wi
 def test_embedding_backward_adds_in_the_terms_order(ctx):
     """Terms whose sum depends on the order: 2^24 and ones, the large one first, last and amid, in
     one part and in several."""
-    for count in (40, 64, 65, 1000):
+    for count in (40, 64, 65, 1000, 1500, 5000):
         for at in (0, count // 2, count - 1):
             g = np.ones((count, 3), np.float32)
             g[at] = 2.0 ** 24
             g[at - 1, 1] = -2.0 ** 24
             got = ctx.native_embedding_backward(ctx.upload(g), ctx.upload(np.zeros(count, np.int32)), 2).numpy()
-            if count <= 64:
+            if count <= 1024:
                 want = np.zeros(3, np.float32)
                 for row in g:
                     want = want + row
@@ -233,6 +233,30 @@ def test_embedding_backward_adds_in_the_terms_order(ctx):
             again = ctx.native_embedding_backward(ctx.upload(g), ctx.upload(np.zeros(count, np.int32)), 2).numpy()
             np.testing.assert_array_equal(got, again)
             assert not np.any(got[1])
+
+
+@pytest.mark.parametrize("width", [3, 40, 300, 1100])
+def test_embedding_backward_of_rows_at_the_parts_borders(ctx, pcu_pkg, width):
+    """Rows of 46 to 51 terms (the longest of one wave has 48), of 95 to 98 and longer ones, at every
+    offset to the parts of 48 terms that the others' numbers bring about; whole numbers, so any order
+    gives the same sums."""
+    rng = np.random.default_rng(width)
+    lengths = [46, 47, 48, 49, 50, 51, 1, 2, 95, 96, 97, 98, 300, 1, 64, 16, 17, 15, 143, 144, 145, 3, 500, 48, 49, 48]
+    for shift in range(0, 50, 7):
+        order = rng.permutation(len(lengths))
+        counts = np.array([shift] + [lengths[i] for i in order], np.int64)
+        tokens = np.repeat(np.arange(len(counts)) * 2 + 1, counts).astype(np.int32)
+        rng.shuffle(tokens)
+        assert tokens.size > 1024
+        g = rng.integers(-8, 9, (tokens.size, width)).astype(np.float32)
+        vocab = 2 * len(counts) + 3
+        want = np.zeros((vocab, width), np.float32)
+        np.add.at(want, tokens, g)
+        got = ctx.native_embedding_backward(ctx.upload(g), ctx.upload(tokens), vocab).numpy()
+        np.testing.assert_array_equal(got, want)
+        base = rng.integers(-8, 9, (vocab, width)).astype(np.float32)
+        got = ctx.native_embedding_backward(ctx.upload(g), ctx.upload(tokens), vocab, base=ctx.upload(base)).numpy()
+        np.testing.assert_array_equal(got, want + base)
 
 
 def test_embedding_gradient_leaves_absent_rows_out(ctx):
@@ -532,6 +556,8 @@ def test_refusals(ctx, pcu_pkg):
     assert lib.pcu_native_embedding_backward(h, rows(big.ptr), t.ptr, 4, 1.0, x.ptr, 9, x.ptr, 8, f) == A
     assert lib.pcu_native_embedding_backward(h, rows(big.ptr), t.ptr, 4, 1.0, big.ptr + 4096, 8, big.ptr + 4100, 8, f) == A
     assert lib.pcu_native_embedding_backward(h, rows(big.ptr), t.ptr, 4, 1.0, None, 0, None, 8, f) == A
+    assert lib.pcu_native_embedding_backward(h, rows(big.ptr, r=1 << 29), t.ptr, 4, 1.0, None, 0, x.ptr, 8, f) == S
+    assert lib.pcu_native_embedding_backward(h, rows(big.ptr, r=1 << 20, c=1 << 18, s=1 << 18), t.ptr, 4, 1.0, None, 0, x.ptr, 1 << 18, f) == S
     assert lib.pcu_native_layer_norm(h, rows(big.ptr), None, None, 1, 1e-5, x.ptr, 8, None) == A
     assert lib.pcu_native_layer_norm(h, rows(big.ptr), None, None, 0, 1e-5, big.ptr + 4, 8, None) == A
     assert lib.pcu_native_layer_norm(h, rows(big.ptr), x.ptr, None, 0, 1e-5, big.ptr, 8, x.ptr) == A
