@@ -15,6 +15,7 @@
 // scale, usually all, have the exact factor 1, and in binary16 2^14 times as large: the smallest
 // probability it holds is then 2^-38.
 #include "pcu_entropy_tile.hpp"
+#include "pcu_rows.hpp"
 
 #include <cmath>
 
@@ -69,25 +70,20 @@ template <typename S> __device__ __forceinline__ void pack_rows(const PackArgs &
         uint16_t *out = g.out + (uint64_t)r * g.out_ld + c;
         if constexpr (sizeof(S) == 2) {
             u32x4 raw = {0, 0, 0, 0};
-            if (on) {
-                raw = load_vec(static_cast<const S *>(g.in) + r * g.ld, c / 8, g.cols);
-#pragma unroll
-                for (uint32_t e = 0; e < 8; e++)
-                    if (c + e >= g.cols)
-                        raw[e / 2] &= e & 1 ? 0x0000ffffu : 0xffff0000u;
-            }
+            if (on)
+                raw = load_piece(static_cast<const S *>(g.in) + r * g.ld, c / 8, g.cols);
             *reinterpret_cast<u32x4 *>(out) = raw;
         } else {
             float v[8] = {};
             if (on) {
                 const float *row = static_cast<const float *>(g.in) + r * g.ld;
-                unpack<float>(load_vec(row, c / 4, g.cols), v);
-                unpack<float>(load_vec(row, c / 4 + 1, g.cols), v + 4);
+                unpack<float>(load_piece(row, c / 4, g.cols), v);
+                unpack<float>(load_piece(row, c / 4 + 1, g.cols), v + 4);
             }
             u32x4 raw[3] = {};
 #pragma unroll
             for (uint32_t e = 0; e < 8; e++) {
-                float x = c + e < g.cols ? v[e] : 0.0f;
+                float x = v[e];
 #pragma unroll
                 for (int k = 0; k < 3; k++)
                     raw[k][e / 2] |= first_part(x) << (16 * (e & 1));

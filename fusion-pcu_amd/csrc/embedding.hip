@@ -6,7 +6,7 @@
 // The gradient sorts the tokens (stable, so a row's terms are added in one order whatever the
 // launch did); then every row of the table is written once, by the lanes that own it: no atomics on
 // values, no second pass over the table to clear it. Both directions are bound by HBM.
-#include "pcu_logits.hpp"
+#include "pcu_rows.hpp"
 
 #pragma clang fp contract(off)
 
@@ -61,7 +61,7 @@ template <typename S> __global__ __launch_bounds__(256) void k_embed(EmbedArgs g
 #pragma unroll
                 for (int q = 0; q < 4; q++)
                     if (v0 + q * lanes < vecs)
-                        raw[q] = load_vec(row, v0 + q * lanes, g.width);
+                        raw[q] = load_piece(row, v0 + q * lanes, g.width);
 #pragma unroll
                 for (int q = 0; q < 4; q++)
                     if (v0 + q * lanes < vecs) {
@@ -370,7 +370,7 @@ __device__ __forceinline__ void add_terms(const EmbedBackArgs &g, const P *place
 #pragma unroll
         for (int q = 0; q < U; q++)
             if (j + q < hi)
-                raw[q] = load_vec(static_cast<const S *>(g.gradient) + (uint64_t)places[j + q] * g.gradient_stride, v, g.width);
+                raw[q] = load_piece(static_cast<const S *>(g.gradient) + (uint64_t)places[j + q] * g.gradient_stride, v, g.width);
 #pragma unroll
         for (int q = 0; q < U; q++)
             if (j + q < hi) {
@@ -408,7 +408,7 @@ __device__ __forceinline__ void write_sum(const EmbedBackArgs &g, uint32_t row, 
 }
 template <typename S> __device__ __forceinline__ u32x4 load_base(const EmbedBackArgs &g, uint32_t row, uint32_t v)
 {
-    return g.base ? load_vec(static_cast<const S *>(g.base) + (uint64_t)row * g.base_stride, v, g.width) : u32x4{0, 0, 0, 0};
+    return g.base ? load_piece(static_cast<const S *>(g.base) + (uint64_t)row * g.base_stride, v, g.width) : u32x4{0, 0, 0, 0};
 }
 
 // Row sums of the runs of equal keys that begin at sorted terms [16 chunk, 16 chunk + 16), but long
@@ -442,7 +442,7 @@ __device__ __forceinline__ void sum_runs(const EmbedBackArgs &g, const uint32_t 
                 if (t) {
                     const int l = __builtin_ctzll(t);
                     if (on) {
-                        raw[q] = load_vec(static_cast<const S *>(g.gradient) + (uint64_t)from_lane(place, l) * g.gradient_stride, vec, g.width);
+                        raw[q] = load_piece(static_cast<const S *>(g.gradient) + (uint64_t)from_lane(place, l) * g.gradient_stride, vec, g.width);
                         if (BASE && lasts >> l & 1)
                             base[q] = load_base<S>(g, from_lane(key, l), vec);
                     }
@@ -521,20 +521,36 @@ __device__ __forceinline__ void fill_rows(const EmbedBackArgs &g, const uint32_t
     // Row and vector of each step by addition: a division a vector is dearer than its store.
     const uint32_t down = 256 / vecs, along = 256 % vecs;
     uint32_t row = (uint32_t)((lo + threadIdx.x) / vecs), v = (uint32_t)((lo + threadIdx.x) % vecs);
-    for (uint64_t i = lo + threadIdx.x; i < hi; i += 256, row += down, v += along) {
-        if (v >= vecs) {
-            v -= vecs;
-            row++;
+    constexpr int U = 4;
+    for (uint64_t i = lo + threadIdx.x; i < hi; i += 256 * U) {
+        u32x4 raw[U];
+        uint32_t rows[U], at[U];
+#pragma unroll
+        for (int q = 0; q < U; q++) {
+            rows[q] = row;
+            at[q] = v;
+            if (i + 256 * q >= hi || occurs[(row - row0) / 32] >> ((row - row0) & 31) & 1)
+                rows[q] = ~0u;
+            else
+                raw[q] = load_base<S>(g, row, v);
+            row += down;
+            v += along;
+            if (v >= vecs) {
+                v -= vecs;
+                row++;
+            }
         }
-        if (occurs[(row - row0) / 32] >> ((row - row0) & 31) & 1)
-            continue;
-        typename StatOf<S>::T y[kVec<S>];
-        unpack<S>(load_base<S>(g, row, v), y);
-        S *out = static_cast<S *>(g.out) + (uint64_t)row * g.out_stride;
-        if (through)
-            store_row(out, v, g.width, y, true);
-        else
-            store_vec(out, v, g.width, y, g.past);
+#pragma unroll
+        for (int q = 0; q < U; q++)
+            if (rows[q] != ~0u) {
+                typename StatOf<S>::T y[kVec<S>];
+                unpack<S>(raw[q], y);
+                S *out = static_cast<S *>(g.out) + (uint64_t)rows[q] * g.out_stride;
+                if (through)
+                    store_row(out, at[q], g.width, y, true);
+                else
+                    store_vec(out, at[q], g.width, y, g.past);
+            }
     }
 }
 
@@ -581,7 +597,7 @@ __global__ __launch_bounds__(256) void k_embed_first(EmbedBackArgs g, uint32_t a
 #pragma unroll
                 for (int k = 0; k < U; k++, l &= l - 1)
                     if (l && v < vecs)
-                        raw[k] = load_vec(static_cast<const S *>(g.gradient) + (uint64_t)(q * 64 + __builtin_ctzll(l)) * g.gradient_stride, v, g.width);
+                        raw[k] = load_piece(static_cast<const S *>(g.gradient) + (uint64_t)(q * 64 + __builtin_ctzll(l)) * g.gradient_stride, v, g.width);
 #pragma unroll
                 for (int k = 0; k < U; k++, left &= left - 1)
                     if (left) {

@@ -6,7 +6,7 @@
 // Both directions are bound by HBM: a row is read once and held in registers while its sums are
 // taken. The weight's gradients are sums down the columns: every workgroup adds up its rows in
 // registers, and a second launch adds up the workgroups in their order.
-#include "pcu_logits.hpp"
+#include "pcu_rows.hpp"
 
 #pragma clang fp contract(off)
 
@@ -59,10 +59,10 @@ template <typename S, typename W>
 __device__ __forceinline__ void load_weights(const W *w, uint32_t i, uint32_t n, typename StatOf<S>::T (&out)[kVec<S>])
 {
     if constexpr (sizeof(W) == sizeof(S)) {
-        unpack<W>(load_vec(w, i, n), out);
+        unpack<W>(load_piece(w, i, n), out);
     } else {
-        unpack<W>(load_vec(w, 2 * i, n), out);
-        unpack<W>(load_vec(w, 2 * i + 1, n), out + 4);
+        unpack<W>(load_piece(w, 2 * i, n), out);
+        unpack<W>(load_piece(w, 2 * i + 1, n), out + 4);
     }
 }
 
@@ -117,7 +117,7 @@ __global__ __launch_bounds__(NT) void k_norm(NormArgs g, ProgramClose close)
         } else {
             for (uint32_t i = lane; on && i < vecs; i += LANES) {
                 T v[kVec<S>];
-                unpack<S>(load_vec(x, i, n), v);
+                unpack<S>(load_piece(x, i, n), v);
                 f(i, v, min(n - i * kVec<S>, (uint32_t)kVec<S>));
             }
         }
@@ -126,7 +126,7 @@ __global__ __launch_bounds__(NT) void k_norm(NormArgs g, ProgramClose close)
 #pragma unroll
         for (int q = 0; q < R; q++)
             if (on && q * LANES + lane < vecs)
-                held[q] = load_vec(x, q * LANES + lane, n);
+                held[q] = load_piece(x, q * LANES + lane, n);
     }
     T sum[1] = {0};
     walk([&](uint32_t, const T *v, uint32_t m) {
@@ -230,8 +230,8 @@ __global__ __launch_bounds__(NT) void k_norm_back(NormBackArgs g, void *parts)
 #pragma unroll
         for (int q = 0; q < R; q++)
             if (q * LANES + lane < vecs) {
-                x[q] = load_vec(xr, q * LANES + lane, n);
-                dy[q] = load_vec(dr, q * LANES + lane, n);
+                x[q] = load_piece(xr, q * LANES + lane, n);
+                dy[q] = load_piece(dr, q * LANES + lane, n);
             }
         const T *s = static_cast<const T *>(g.stats) + 2 * r;
         st[0] = s[0];
@@ -350,8 +350,8 @@ template <typename S, typename W> __global__ __launch_bounds__(1024) void k_norm
     T sum[2] = {0, 0};
     for (uint32_t i = threadIdx.x; i < vecs; i += 1024) {
         T x[V], d[V], ws[V], s0 = 0, s1 = 0;
-        unpack<S>(load_vec(xr, i, n), x);
-        unpack<S>(load_vec(dr, i, n), d);
+        unpack<S>(load_piece(xr, i, n), x);
+        unpack<S>(load_piece(dr, i, n), d);
         if (w)
             load_weights<S, W>(w, i, n, ws);
 #pragma unroll
@@ -388,8 +388,8 @@ __global__ __launch_bounds__(1024) void k_norm_back_wide(NormBackArgs g, const v
     for (uint64_t r = blockIdx.x; r < g.rows; r += gridDim.x) {
         const T mean = static_cast<const T *>(g.stats)[2 * r], rstd = static_cast<const T *>(g.stats)[2 * r + 1];
         T x[V], d[V];
-        unpack<S>(load_vec(static_cast<const S *>(g.x) + r * g.stride, i, n), x);
-        unpack<S>(load_vec(static_cast<const S *>(g.gradient) + r * g.gradient_stride, i, n), d);
+        unpack<S>(load_piece(static_cast<const S *>(g.x) + r * g.stride, i, n), x);
+        unpack<S>(load_piece(static_cast<const S *>(g.gradient) + r * g.gradient_stride, i, n), d);
         const T c0 = static_cast<const T *>(sums)[2 * r], c1 = static_cast<const T *>(sums)[2 * r + 1];
 #pragma unroll
         for (int e = 0; e < V; e++) {
