@@ -169,7 +169,7 @@ template <typename S> __global__ __launch_bounds__(256) void k_entropy_open(Pack
 // ----------------------------------------------------------------------- tiles
 struct LogitArgs {
     EntropyOperand w, x;       // rows: vocabulary, features
-    uint32_t pairs = 1, slabs = 0;
+    uint32_t slabs = 0;        // of kSlabK
     uint32_t tiles_m = 0, tiles_n = 0;
     uint32_t first = 0;        // vocabulary of w's first row
     uint32_t vocab = 0, rows = 0;
@@ -241,10 +241,19 @@ template <typename S, class Cfg, bool GRAD, bool CARRY> __global__ __launch_boun
         }
         __syncthreads();
     }
+    // What the end needs of the rows is under way before the product.
+    const uint32_t wave = threadIdx.x / 64, wm = wave / Cfg::WN * SM * 16, wn = wave % Cfg::WN * SN * 16;
+    int32_t labels[SN];
+    float scales[SN];
+#pragma unroll
+    for (int j = 0; j < SN; j++) {
+        const uint32_t n = n0 + wn + acc_col(j);
+        labels[j] = n < g.rows ? g.row.label[n] : -1;
+        scales[j] = GRAD && n < g.rows ? g.row.scale[n] * g.boost : 0.0f;
+    }
     f32x4 acc[SM][SN];
-    entropy_product<E, Cfg, false, false, CARRY>(g.w, g.x, g.pairs, m0, n0, 0, g.slabs, lds, acc);
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-    const uint32_t wm = wave / Cfg::WN * SM * 16, wn = wave % Cfg::WN * SN * 16;
+    entropy_product<E, Cfg, false, false, CARRY>(g.w, g.x, m0, n0, 0, g.slabs * (kSlabK / Cfg::K), lds, acc);
+    const uint32_t lane = threadIdx.x & 63;
     const uint32_t v0 = g.first + m0 + wm; // of acc[i][j][r]: v0 + acc_row(i, r)
     const bool ragged = g.first + m0 + BM > g.vocab;
     if constexpr (!GRAD) {
@@ -252,7 +261,7 @@ template <typename S, class Cfg, bool GRAD, bool CARRY> __global__ __launch_boun
 #pragma unroll
         for (int j = 0; j < SN; j++) {
             const uint32_t n = n0 + wn + acc_col(j);
-            const int32_t label = n < g.rows ? g.row.label[n] : -1;
+            const int32_t label = labels[j];
             if (label >= 0 && (uint32_t)label - v0 < SM * 16u) {
 #pragma unroll
                 for (int i = 0; i < SM; i++)
@@ -302,8 +311,8 @@ template <typename S, class Cfg, bool GRAD, bool CARRY> __global__ __launch_boun
         for (int j = 0; j < SN; j++) {
             const uint32_t n = n0 + wn + acc_col(j);
             const bool in = n < g.rows;
-            const int32_t label = in ? g.row.label[n] : -1;
-            const float scale = in ? g.row.scale[n] * g.boost : 0.0f;
+            const int32_t label = labels[j];
+            const float scale = scales[j];
             const float log_sum = g.join ? own_sum[n - n0] : in ? g.row.log_sum[n] : 0.0f;
             const bool mine = label >= 0 && (uint32_t)label - v0 < SM * 16u;
 #pragma unroll
@@ -381,7 +390,7 @@ __global__ __launch_bounds__(256) void k_entropy_loss(const float2 *partial, uin
 
 struct ProductArgs {
     EntropyOperand a, b;
-    uint32_t pairs = 1, slabs = 0, splits = 1;
+    uint32_t slabs = 0, splits = 1; // of kSlabK
     uint32_t tiles_m = 0, tiles_n = 0;
     float *sums = nullptr; // [split][row][sums_ld], the features' gradient
     uint64_t sums_split = 0;
@@ -403,7 +412,7 @@ template <typename S, class Cfg> __device__ __forceinline__ void feature_tile(co
     const uint32_t m0 = t.tm * Cfg::BM, n0 = t.tn * Cfg::BN;
     const uint32_t k_lo = (uint32_t)((uint64_t)g.slabs * t.split / g.splits), k_hi = (uint32_t)((uint64_t)g.slabs * (t.split + 1) / g.splits);
     f32x4 acc[SM][SN];
-    entropy_product<E, Cfg, true, false, false>(g.a, g.b, g.pairs, m0, n0, k_lo, k_hi, lds, acc);
+    entropy_product<E, Cfg, true, false, false>(g.a, g.b, m0, n0, k_lo * (kSlabK / Cfg::K), k_hi * (kSlabK / Cfg::K), lds, acc);
     const uint32_t wave = threadIdx.x / 64, m = m0 + wave / Cfg::WN * SM * 16, n = n0 + wave % Cfg::WN * SN * 16;
 #pragma unroll
     for (int j = 0; j < SN; j++)
@@ -477,7 +486,7 @@ template <typename S, class Cfg> __device__ __forceinline__ void weight_tile(con
     const EntropyTile t = entropy_tile(block, g.tiles_m, g.tiles_n, 1);
     const uint32_t m0 = t.tm * BM, n0 = t.tn * BN;
     f32x4 acc[SM][SN];
-    entropy_product<E, Cfg, true, true, false>(g.a, g.b, g.pairs, m0, n0, 0, g.slabs, lds, acc);
+    entropy_product<E, Cfg, true, true, false>(g.a, g.b, m0, n0, 0, g.slabs * (kSlabK / Cfg::K), lds, acc);
     const uint32_t wave = threadIdx.x / 64, wm = wave / Cfg::WN * SM * 16, wn = wave % Cfg::WN * SN * 16;
     const float f = *g.factor;
     S *out = static_cast<S *>(g.out);
@@ -558,41 +567,73 @@ template <typename S> __global__ __launch_bounds__(256) void k_zero_rows(S *out,
 }
 
 // ---------------------------------------------------------------------- launches
-using Large = EntropyCfg<4, 2, 4, 8, 2>;  // 256 x 256
-using Middle = EntropyCfg<2, 2, 4, 4, 2>; // 128 x 128
-using Half = EntropyCfg<2, 2, 4, 2, 3>;   // 128 x 64
-using Thin = EntropyCfg<4, 1, 2, 2, 3>;   // 128 x 32
+template <typename S> struct Tiles {
+    using Large = EntropyCfg<4, 2, 4, 8, 64, 2, 1>;  // 256 x 256
+    using Middle = EntropyCfg<2, 2, 4, 4, 64, 2, 1>; // 128 x 128
+    using Half = EntropyCfg<2, 2, 4, 2, 64, 3, 1>;   // 128 x 64
+    using Thin = EntropyCfg<4, 1, 2, 2, 64, 3, 1>;   // 128 x 32
+};
+template <> struct Tiles<float> {
+    using Large = EntropyCfg<4, 2, 4, 4, 32, 2, 3>;  // 256 x 128
+    using Middle = EntropyCfg<2, 2, 4, 4, 32, 2, 3>; // 128 x 128
+    using Half = EntropyCfg<2, 2, 4, 2, 32, 4, 3>;   // 128 x 64
+    using Thin = EntropyCfg<4, 1, 2, 2, 64, 2, 3>;   // 128 x 32
+};
 
 constexpr uint64_t round_up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
 
 enum class Side { Large, Middle, Half, Thin };
 inline uint32_t side_m(Side s) { return s == Side::Large ? 256 : 128; }
-inline uint32_t side_n(Side s) { return s == Side::Large ? 256 : s == Side::Middle ? 128 : s == Side::Half ? 64 : 32; }
-inline uint64_t tiles_of(Side s, uint64_t m, uint64_t n)
+inline uint32_t side_n(Side s, uint32_t parts) { return s == Side::Large ? (parts == 1 ? 256 : 128) : s == Side::Middle ? 128 : s == Side::Half ? 64 : 32; }
+
+// What choices go by, measured: workgroups a CU, and what a slab of kSlabK takes them, in us (the
+// 256 x 256 tiles of 16-bit values run at 1450 TFLOP/s, the 128 x 128 ones at 1050), the first where each CU
+// has as many, the second alone on it.
+struct SideTime {
+    uint32_t per_cu;
+    double full, alone;
+};
+inline SideTime side_time(Side s, uint32_t parts)
 {
-    return (m + side_m(s) - 1) / side_m(s) * ((n + side_n(s) - 1) / side_n(s));
+    if (parts == 1)
+        return s == Side::Large ? SideTime{1, 1.5, 1.5} : s == Side::Middle ? SideTime{2, 1.0, 0.65} : s == Side::Half ? SideTime{2, 0.6, 0.45} : SideTime{2, 0.45, 0.4};
+    return s == Side::Large ? SideTime{1, 4.2, 4.2} : s == Side::Middle ? SideTime{1, 2.7, 2.7} : s == Side::Half ? SideTime{1, 1.5, 1.5} : SideTime{1, 1.1, 1.1};
+}
+inline uint64_t tiles_of(Side s, uint32_t parts, uint64_t m, uint64_t n)
+{
+    return (m + side_m(s) - 1) / side_m(s) * ((n + side_n(s, parts) - 1) / side_n(s, parts));
 }
 
-// What a slab of a pair of parts takes a round of tiles, in us: one 256 x 256 tile a CU (1450 TFLOP/s),
-// two of 128 x 128 (1050 TFLOP/s), and the narrower ones, which wait for their loads.
-inline double slab_us(Side s) { return s == Side::Large ? 1.5 : s == Side::Middle ? 1.0 : 0.6; }
-
-// The tile of an m x n product over so many slabs: by the rounds that the tiles take on the CUs, each
-// with its start and end (777 x 32003 x 1000: 83 us by 504 tiles of 256 x 256, 104 by 128 x 128), or,
-// where k can be split, by the whole work, unless a CU would have next to none of it.
-inline Side choose(uint64_t m, uint64_t n, uint64_t slabs, bool split)
+// An m x n product's tiles, each over so many slabs: the rounds that they take on the CUs, each with its
+// start and end (777 x 32003 x 1000: 83 us by 504 tiles of 256 x 256, 104 by 128 x 128).
+inline double product_us(Side s, uint32_t parts, uint64_t m, uint64_t n, uint64_t slabs)
 {
-    const double large = (double)tiles_of(Side::Large, m, n) / kGfx950Cus, middle = (double)tiles_of(Side::Middle, m, n) / (2 * kGfx950Cus);
-    if (split)
-        return large * slab_us(Side::Large) <= middle * slab_us(Side::Middle) && large * slabs >= 4 ? Side::Large : Side::Middle;
-    const auto rounds = [](double n) { return n <= 1 ? 1.0 : (n + std::ceil(n)) / 2; }; // a last one that few take runs faster
-    return rounds(large) * (14 + slabs * slab_us(Side::Large)) <= rounds(middle) * (8 + slabs * slab_us(Side::Middle)) ? Side::Large
-                                                                                                                     : Side::Middle;
+    const SideTime t = side_time(s, parts);
+    const double tiles = (double)tiles_of(s, parts, m, n);
+    if (tiles <= kGfx950Cus)
+        return 8 + slabs * t.alone;
+    const double n_rounds = tiles / (t.per_cu * kGfx950Cus);
+    // A last round that few take runs faster.
+    return (n_rounds <= 1 ? 1.0 : (n_rounds + std::ceil(n_rounds)) / 2) * ((s == Side::Large ? 14 : 8) + slabs * t.full);
 }
-// The same where n are the call's rows: few of them take narrower tiles, which read the weights at HBM's rate.
-inline Side choose_rows(uint64_t m, uint64_t rows, uint64_t slabs, bool split)
+inline Side choose(uint32_t parts, uint64_t m, uint64_t n, uint64_t slabs, bool narrow)
 {
-    return rows <= 32 ? Side::Thin : rows <= 64 ? Side::Half : choose(m, rows, slabs, split);
+    Side best = Side::Middle;
+    for (Side s : {Side::Large, Side::Half, Side::Thin})
+        if ((narrow || s == Side::Large) && product_us(s, parts, m, n, slabs) < product_us(best, parts, m, n, slabs))
+            best = s;
+    return best;
+}
+// Where k can be split: by the whole work, unless a CU would have next to none of it. Few rows take
+// narrower tiles, which read the weights at HBM's rate.
+inline Side choose_split(uint32_t parts, uint64_t m, uint64_t rows, uint64_t slabs)
+{
+    if (rows <= 64)
+        return rows <= 32 ? Side::Thin : Side::Half;
+    const SideTime l = side_time(Side::Large, parts), k = side_time(Side::Middle, parts);
+    const double large = (double)tiles_of(Side::Large, parts, m, rows) / (l.per_cu * kGfx950Cus);
+    const double middle = (double)tiles_of(Side::Middle, parts, m, rows) / (k.per_cu * kGfx950Cus);
+    return large * l.full <= middle * k.full && large * slabs >= 4 ? Side::Large : Side::Middle;
 }
 
 // How a call goes over its vocabulary and what its scratch holds.
@@ -635,17 +676,17 @@ struct EntropyPlan {
             const uint64_t fit = kWeightBytes / row_bytes / 256 * 256;
             piece = piece < fit ? piece : fit < 256 ? 256 : fit;
         }
-        const uint64_t pairs = parts == 3 ? kPartPairs : 1, within = piece < g.vocab ? piece : g.vocab, most = (within + kSlabK - 1) / kSlabK;
-        logits = choose_rows(g.vocab, g.rows, ld / kSlabK * pairs, false);
-        features = choose_rows(g.width, g.rows, most * pairs, true);
-        weights = choose(g.width, within, (g.rows + kSlabK - 1) / kSlabK * pairs, false);
-        const uint64_t tiles = tiles_of(features, g.width, g.rows);
-        const uint64_t per = features == Side::Large ? 1 : features == Side::Half ? 3 : 2; // workgroups a CU
-        const uint64_t want = tiles ? (per * kGfx950Cus + tiles / 2) / tiles : 1;
+        const uint64_t within = piece < g.vocab ? piece : g.vocab, most = (within + kSlabK - 1) / kSlabK;
+        logits = g.rows <= 64 ? choose_split(parts, g.vocab, g.rows, 1) : choose(parts, g.vocab, g.rows, ld / kSlabK, true);
+        features = choose_split(parts, g.width, g.rows, most);
+        weights = choose(parts, g.width, within, (g.rows + kSlabK - 1) / kSlabK, false);
+        const uint64_t tiles = tiles_of(features, parts, g.width, g.rows);
+        const uint64_t per = side_time(features, parts).per_cu, want = tiles ? per * kGfx950Cus / tiles : 1;
         sums_ld = (uint32_t)round_up(g.width, 256);
-        sums_rows = round_up(g.rows, side_n(features));
-        // Splits that fill the CUs, but no more than pay: a split's sums are written and read at 4 TB/s.
-        const double best = std::sqrt(most * pairs * slab_us(features) / (sums_rows * sums_ld * 8 / 4e6 + 1e-3));
+        sums_rows = round_up(g.rows, side_n(features, parts));
+        // Splits that fill the CUs, but no more than pay: a split's sums are written and read at 4 TB/s, 8 of
+        // them in a trip to memory.
+        const double best = std::sqrt(most * side_time(features, parts).full / (sums_rows * sums_ld * 8 / 4e6 + 0.15));
         const uint64_t pay = best < 1 ? 1 : (uint64_t)best, cut = want < pay ? want : pay;
         splits = (uint32_t)(cut < 1 ? 1 : cut > most ? (most ? most : 1) : cut);
         bytes = 0;
@@ -693,10 +734,10 @@ template <typename S, class Cfg, bool GRAD> hipError_t logits_of(bool carry, hip
 template <typename S, bool GRAD> hipError_t logits_by(Side side, bool carry, hipStream_t s, const LogitArgs &a, uint64_t vocab_rows, uint64_t rows)
 {
     switch (side) {
-    case Side::Large: return logits_of<S, Large, GRAD>(carry, s, a, vocab_rows, rows);
-    case Side::Middle: return logits_of<S, Middle, GRAD>(carry, s, a, vocab_rows, rows);
-    case Side::Half: return logits_of<S, Half, GRAD>(carry, s, a, vocab_rows, rows);
-    default: return logits_of<S, Thin, GRAD>(carry, s, a, vocab_rows, rows);
+    case Side::Large: return logits_of<S, typename Tiles<S>::Large, GRAD>(carry, s, a, vocab_rows, rows);
+    case Side::Middle: return logits_of<S, typename Tiles<S>::Middle, GRAD>(carry, s, a, vocab_rows, rows);
+    case Side::Half: return logits_of<S, typename Tiles<S>::Half, GRAD>(carry, s, a, vocab_rows, rows);
+    default: return logits_of<S, typename Tiles<S>::Thin, GRAD>(carry, s, a, vocab_rows, rows);
     }
 }
 
@@ -734,6 +775,7 @@ inline unsigned pack_blocks(uint64_t rows, uint64_t ld)
 template <typename S, class Cfg>
 hipError_t run_both(hipStream_t s, ProductArgs f, ProductArgs w, uint64_t width, uint64_t rows, uint64_t vocab_rows)
 {
+    using Middle = typename Tiles<S>::Middle;
     f.tiles_m = (uint32_t)((width + Cfg::BM - 1) / Cfg::BM);
     f.tiles_n = (uint32_t)((rows + Cfg::BN - 1) / Cfg::BN);
     w.tiles_m = (uint32_t)((width + Middle::BM - 1) / Middle::BM);
@@ -757,7 +799,7 @@ template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyAr
                       reinterpret_cast<float *>(sc + p.own), reinterpret_cast<float *>(sc + p.factor)};
     hipError_t e;
     const bool whole_pass = !g.log_sum_in;
-    const uint32_t pairs = p.parts == 3 ? kPartPairs : 1, slabs = p.ld / kSlabK;
+    const uint32_t slabs = p.ld / kSlabK;
 
     PackArgs px;
     px.in = g.features;
@@ -818,7 +860,6 @@ template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyAr
 
     LogitArgs l;
     l.x = x;
-    l.pairs = pairs;
     l.slabs = slabs;
     l.vocab = g.vocab;
     l.rows = (uint32_t)g.rows;
@@ -862,14 +903,12 @@ template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyAr
         return hipSuccess;
 
     ProductArgs f;
-    f.pairs = pairs;
     f.sums = reinterpret_cast<float *>(sc + p.sums);
     f.sums_split = p.sums_rows * p.sums_ld;
     f.sums_ld = p.sums_ld;
     f.splits = p.splits;
     f.gate = g.gate;
     ProductArgs d;
-    d.pairs = pairs;
     d.a = EntropyOperand{x.p, x.plane, x.ld, (uint32_t)round_up(g.rows, kSlabK), x.ld};
     d.slabs = (uint32_t)((g.rows + kSlabK - 1) / kSlabK);
     d.factor = row.factor;
@@ -893,23 +932,23 @@ template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyAr
         d.out = static_cast<S *>(g.weight_gradient) + v * g.weight_gradient_stride;
         d.out_rows = (uint32_t)n;
         if (g.feature_gradient && g.weight_gradient && p.weights == Side::Middle && p.features != Side::Large) {
-            e = p.features == Side::Middle ? run_both<S, Middle>(s, f, d, g.width, g.rows, n)
-                : p.features == Side::Half ? run_both<S, Half>(s, f, d, g.width, g.rows, n)
-                                           : run_both<S, Thin>(s, f, d, g.width, g.rows, n);
+            e = p.features == Side::Middle ? run_both<S, typename Tiles<S>::Middle>(s, f, d, g.width, g.rows, n)
+                : p.features == Side::Half ? run_both<S, typename Tiles<S>::Half>(s, f, d, g.width, g.rows, n)
+                                           : run_both<S, typename Tiles<S>::Thin>(s, f, d, g.width, g.rows, n);
             if (e)
                 return e;
             continue;
         }
         if (g.feature_gradient) {
-            e = p.features == Side::Large    ? run_features<S, Large>(s, f, g.width, g.rows)
-                : p.features == Side::Middle ? run_features<S, Middle>(s, f, g.width, g.rows)
-                : p.features == Side::Half   ? run_features<S, Half>(s, f, g.width, g.rows)
-                                             : run_features<S, Thin>(s, f, g.width, g.rows);
+            e = p.features == Side::Large    ? run_features<S, typename Tiles<S>::Large>(s, f, g.width, g.rows)
+                : p.features == Side::Middle ? run_features<S, typename Tiles<S>::Middle>(s, f, g.width, g.rows)
+                : p.features == Side::Half   ? run_features<S, typename Tiles<S>::Half>(s, f, g.width, g.rows)
+                                             : run_features<S, typename Tiles<S>::Thin>(s, f, g.width, g.rows);
             if (e)
                 return e;
         }
         if (g.weight_gradient) {
-            e = p.weights == Side::Large ? run_weights<S, Large>(s, d, g.width, n) : run_weights<S, Middle>(s, d, g.width, n);
+            e = p.weights == Side::Large ? run_weights<S, typename Tiles<S>::Large>(s, d, g.width, n) : run_weights<S, typename Tiles<S>::Middle>(s, d, g.width, n);
             if (e)
                 return e;
         }

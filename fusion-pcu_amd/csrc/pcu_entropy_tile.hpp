@@ -1,13 +1,13 @@
 // Matrix-core tiles of the output layer's cross entropy (gfx950): 16-bit operands, F32 sums.
 //
-// A workgroup makes a BM x BN tile of C = A B, k in slabs of 64. An operand's slab lies in LDS as
-// it lies in memory, either k-contiguous (64 values of a row of A or column of B side by side) or k-major
-// (`T`: 64 rows of BM or BN values), and comes there by direct loads, one or more slabs ahead, or (A
+// A workgroup makes a BM x BN tile of C = A B, k in slabs of K. An operand's slab lies in LDS as
+// it lies in memory, either k-contiguous (K values of a row of A or column of B side by side) or k-major
+// (`T`: K rows of BM or BN values), and comes there by direct loads, one or more slabs ahead, or (A
 // alone, where its rows do not start at multiples of 16 bytes or end inside a slab) through registers. A lane of the
 // 16 x 16 x 32 instruction takes 8 consecutive k of one row or column: one 16-byte read of a
 // k-contiguous slab, two transposing 8-byte reads of a k-major one. The 16-byte pieces of a slab's
-// row are permuted by the row (in the loads' addresses, so that LDS stays dense): by half of it
-// where k is contiguous, and by twice its bits 0, 1 and 3 where it is k-major, so that the 16 lanes (32 of
+// row are permuted by the row (in the loads' addresses, so that LDS stays dense): by half of it (a
+// quarter in slabs of 32) where k is contiguous, and by twice its bits 0, 1 and 3 where it is k-major, so that the 16 lanes (32 of
 // a transposing read) that are served at once touch all 256 bytes of LDS's banks.
 //
 // What bounds the tiles is power: the clock falls to 1.7 GHz under them. On random values the
@@ -35,17 +35,26 @@ template <typename E> __device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, 
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-constexpr int kSlabK = 64;
+constexpr int kSlabK = 64; // operands are padded to whole slabs of the longer kind
 
-// WM x WN waves, each with SM x SN subtiles of 16 x 16; STAGES slabs in LDS.
-template <int WM_, int WN_, int SM_, int SN_, int STAGES> struct EntropyCfg {
-    static constexpr int WM = WM_, WN = WN_, SM = SM_, SN = SN_, kStages = STAGES;
+// Binary32 operands come as three parts of 8 bits, exact together. Of the nine products of two operands'
+// parts the three smallest (below 2^-24 of the whole) are left out; small ones are added first. All
+// parts of a slab lie in LDS at once: 6 products for 3 + 3 parts read. (Parts pair by pair through the
+// 16-bit tiles: 1024 x 50257 x 768 1.93 ms a step, 64 x 1000 x 64 55 us.)
+constexpr int kPartPairs = 6;
+__device__ constexpr int kPartA[kPartPairs] = {2, 0, 1, 1, 0, 0}, kPartB[kPartPairs] = {0, 2, 1, 0, 1, 0};
+
+// WM x WN waves, each with SM x SN subtiles of 16 x 16; slabs of K, STAGES of them in LDS, of PARTS parts.
+template <int WM_, int WN_, int SM_, int SN_, int K_, int STAGES, int PARTS> struct EntropyCfg {
+    static constexpr int WM = WM_, WN = WN_, SM = SM_, SN = SN_, K = K_, kStages = STAGES, kParts = PARTS;
+    static_assert((K == 32 || K == 64) && (PARTS == 1 || PARTS == 3), "slabs");
     static constexpr int BM = WM * SM * 16, BN = WN * SN * 16, kWaves = WM * WN, kThreads = 64 * kWaves;
-    static constexpr int kSlabA = BM * kSlabK * 2, kSlabB = BN * kSlabK * 2, kStage = kSlabA + kSlabB; // bytes
+    static constexpr int kSlabA = BM * K * 2, kSlabB = BN * K * 2, kStage = PARTS * (kSlabA + kSlabB); // bytes
     static constexpr int kOutPitch = BM + 8; // of a 16-bit output tile in LDS, in values
     static constexpr int kTile = kStages * kStage > BN * kOutPitch * 2 ? kStages * kStage : BN * kOutPitch * 2;
     static constexpr int kReduce = WM * BN * 8; // bytes for a reduction over the tile's rows
     static constexpr int kLds = kTile + kReduce;
+    static_assert(kLds + 64 <= 160 * 1024, "LDS");
 };
 // Where acc[i][j][r] of a lane lies in its wave's tile.
 __device__ __forceinline__ uint32_t acc_row(int i, int r) { return 16 * i + 4 * ((threadIdx.x & 63) / 16) + r; }
@@ -61,20 +70,15 @@ struct EntropyOperand {
     uint32_t ld = 0, rows = 0, cols = 0;
 };
 
-// Parts of a binary32 operand: 8 bits each, exact together. Of the nine products of two operands'
-// parts the three smallest (below 2^-24 of the whole) are left out, and the small ones come first.
-// A 16-bit operand is its own single part (the last pair).
-constexpr int kPartPairs = 6;
-__device__ __forceinline__ uint32_t part_a(uint32_t s) { return (0x201100u >> (20 - 4 * s)) & 15; }
-__device__ __forceinline__ uint32_t part_b(uint32_t s) { return (0x021010u >> (20 - 4 * s)) & 15; }
-
 // How the pieces of a k-major slab's row are permuted.
 __device__ __forceinline__ uint32_t k_major_swap(uint32_t k) { return 2 * ((k & 3) | (k >> 1 & 4)); }
 
+__device__ __forceinline__ uint32_t k_contiguous_swap(uint32_t row, int k) { return k == 64 ? row / 2 & 7 : row / 4 & 3; }
+
 template <class Cfg, int ROWS, bool T> struct SlabLoader {
-    static constexpr int IPW = ROWS / 8 / Cfg::kWaves; // 1 KiB loads a wave
-    static_assert(IPW * 8 * Cfg::kWaves == ROWS, "every wave loads as much");
-    static constexpr int kPieces = (T ? ROWS : kSlabK) / 8; // 16-byte pieces of a row
+    static constexpr int K = Cfg::K, IPW = ROWS * K / 512 / Cfg::kWaves; // 1 KiB loads a wave and part
+    static_assert(IPW * 512 * Cfg::kWaves == ROWS * K, "every wave loads as much");
+    static constexpr int kPieces = (T ? ROWS : K) / 8; // 16-byte pieces of a row
     uint32_t off[IPW];
     __device__ __forceinline__ int row_of(int wave, int q) const { return ((wave * IPW + q) * 64 + (threadIdx.x & 63)) / kPieces; }
     // at: the tile's first row (k-contiguous) or column (k-major).
@@ -85,41 +89,46 @@ template <class Cfg, int ROWS, bool T> struct SlabLoader {
         for (int q = 0; q < IPW; q++) {
             const uint32_t r = row_of(wave, q);
             if constexpr (!T)
-                off[q] = min(r, o.rows - 1 - at) * o.ld * 2 + (piece ^ (r / 2 & 7)) * 16;
+                off[q] = min(r, o.rows - 1 - at) * o.ld * 2 + (piece ^ k_contiguous_swap(r, K)) * 16;
             else
                 off[q] = r * o.ld * 2 + min((piece ^ k_major_swap(r)) * 8, o.cols - 8 - at) * 2;
         }
     }
-    // The slab of k0, part `part`, into `lds`.
-    __device__ __forceinline__ void load(const EntropyOperand &o, uint32_t at, uint32_t part, uint32_t k0, uint32_t lds, int wave) const
+    // The slab of k0, all its parts, into `lds`.
+    __device__ __forceinline__ void load(const EntropyOperand &o, uint32_t at, uint32_t k0, uint32_t lds, int wave) const
     {
-        const uint16_t *base = o.p + part * o.plane + (T ? (uint64_t)k0 * o.ld + at : (uint64_t)at * o.ld + k0);
-        const bool over = T && k0 + kSlabK > o.rows;
+        // Past the last row (padding to whole slabs) the last one is read again.
+        const bool over = T && k0 + K > o.rows;
+        const uint32_t k1 = T ? min(k0, o.rows - 1) : k0;
 #pragma unroll
-        for (int q = 0; q < IPW; q++) {
-            uint32_t from = off[q];
-            if (T && over) { // the last row is read again
-                const uint32_t k = row_of(wave, q);
-                from -= k0 + k >= o.rows ? (k0 + k - (o.rows - 1)) * o.ld * 2 : 0;
+        for (int part = 0; part < Cfg::kParts; part++) {
+            const uint16_t *base = o.p + part * o.plane + (T ? (uint64_t)k1 * o.ld + at : (uint64_t)at * o.ld + k0);
+#pragma unroll
+            for (int q = 0; q < IPW; q++) {
+                uint32_t from = off[q];
+                if (T && over) {
+                    const uint32_t k = row_of(wave, q), to = min(k0 + k, o.rows - 1) - k1;
+                    from -= (k - to) * o.ld * 2;
+                }
+                load_lds<4>(base, from, __builtin_amdgcn_readfirstlane(lds + part * ROWS * K * 2 + (wave * IPW + q) * 1024));
             }
-            load_lds<4>(base, from, __builtin_amdgcn_readfirstlane(lds + (wave * IPW + q) * 1024));
         }
     }
 };
 
 // The same through registers, for rows at any alignment of their type and of any length.
 template <class Cfg, int ROWS, bool T> struct SlabCarrier {
-    static constexpr int IPW = ROWS / 8 / Cfg::kWaves, kPieces = (T ? ROWS : kSlabK) / 8;
+    static constexpr int K = Cfg::K, IPW = ROWS * K / 512 / Cfg::kWaves, kPieces = (T ? ROWS : K) / 8;
     u32x4 held[IPW];
     __device__ __forceinline__ void fetch(const EntropyOperand &o, uint32_t at, uint32_t k0, int wave)
     {
         const uint32_t lane = threadIdx.x & 63;
-        const bool ragged = (T ? at + ROWS : k0 + kSlabK) > o.cols;
+        const bool ragged = (T ? at + ROWS : k0 + K) > o.cols;
 #pragma unroll
         for (int q = 0; q < IPW; q++) {
             const uint32_t r = ((wave * IPW + q) * 64 + lane) / kPieces, piece = lane % kPieces;
             const uint32_t row = min((T ? k0 : at) + r, o.rows - 1);
-            const uint32_t c = (T ? at : k0) + (T ? piece ^ k_major_swap(r) : piece ^ (r / 2 & 7)) * 8;
+            const uint32_t c = (T ? at : k0) + (T ? piece ^ k_major_swap(r) : piece ^ k_contiguous_swap(r, K)) * 8;
             const uint16_t *from = o.p + (uint64_t)row * o.ld + c;
             if (!ragged || c + 8 <= o.cols) {
                 held[q] = *reinterpret_cast<const u32x4_any *>(from);
@@ -141,9 +150,9 @@ template <class Cfg, int ROWS, bool T> struct SlabCarrier {
     }
 };
 
-// Fragments of an operand's slab: subtile i of S, 32 values of k from 32 kk on.
-template <int ROWS, int S, bool T> struct SlabReader {
-    uint32_t at[T ? S : 2];
+// Fragments of an operand's slab (one part): subtile i of S, 32 values of k from 32 kk on.
+template <int K, int ROWS, int S, bool T> struct SlabReader {
+    uint32_t at[T ? S : K / 32];
     // first: the wave's first row or column of the slab.
     __device__ __forceinline__ void init(uint32_t first)
     {
@@ -151,8 +160,8 @@ template <int ROWS, int S, bool T> struct SlabReader {
         if constexpr (!T) {
             // Row first + lane % 16, piece 4 kk + lane / 16.
 #pragma unroll
-            for (int kk = 0; kk < 2; kk++)
-                at[kk] = (first + (lane & 15)) * 128 + (((4 * kk + lane / 16) ^ (lane / 2 & 7)) * 16);
+            for (int kk = 0; kk < K / 32; kk++)
+                at[kk] = (first + (lane & 15)) * K * 2 + (((4 * kk + lane / 16) ^ k_contiguous_swap(lane & 15, K)) * 16);
         } else {
             // Lanes 16 g ..: k 8 g .. of 16 columns; a lane reads 4 columns of row j / 4.
             const uint32_t j = lane & 15, g = lane / 16, row = 8 * g + j / 4;
@@ -166,7 +175,7 @@ template <int ROWS, int S, bool T> struct SlabReader {
     __device__ __forceinline__ s16x8 read(const char *slab, int i, int kk) const
     {
         if constexpr (!T) {
-            return *reinterpret_cast<const s16x8 *>(slab + at[kk] + i * 16 * 128);
+            return *reinterpret_cast<const s16x8 *>(slab + at[kk] + i * 16 * K * 2);
         } else {
             const char *p = slab + at[i] + kk * 32 * ROWS * 2;
             typedef __attribute__((address_space(3))) s16x4 *P;
@@ -195,21 +204,21 @@ __device__ __forceinline__ EntropyTile entropy_tile(uint32_t bid, uint32_t tiles
     return t;
 }
 
-// acc = the tile of A B over slabs [k_lo, k_hi) of each pair of parts. a, b: the operands; m0, n0: the
-// tile's first row and column; lds: Cfg::kTile bytes. CARRY: A goes through registers (one part alone).
-// No LDS is read after the last barrier.
+// acc = the tile of A B over slabs [k_lo, k_hi). a, b: the operands; m0, n0: the tile's first row and
+// column; lds: Cfg::kTile bytes. CARRY: A goes through registers (one part alone). No LDS is read after
+// the last barrier.
 template <typename E, class Cfg, bool TA, bool TB, bool CARRY>
-__device__ __forceinline__ void entropy_product(const EntropyOperand &a, const EntropyOperand &b, uint32_t pairs, uint32_t m0,
-                                                uint32_t n0, uint32_t k_lo, uint32_t k_hi, char *lds,
-                                                f32x4 (&acc)[Cfg::SM][Cfg::SN])
+__device__ __forceinline__ void entropy_product(const EntropyOperand &a, const EntropyOperand &b, uint32_t m0, uint32_t n0, uint32_t k_lo,
+                                                uint32_t k_hi, char *lds, f32x4 (&acc)[Cfg::SM][Cfg::SN])
 {
-    constexpr int SM = Cfg::SM, SN = Cfg::SN;
+    constexpr int SM = Cfg::SM, SN = Cfg::SN, K = Cfg::K;
+    static_assert(!CARRY || Cfg::kParts == 1, "parts are packed");
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     SlabLoader<Cfg, Cfg::BM, TA> la;
     SlabCarrier<Cfg, Cfg::BM, TA> ca;
     SlabLoader<Cfg, Cfg::BN, TB> lb;
-    SlabReader<Cfg::BM, SM, TA> ra;
-    SlabReader<Cfg::BN, SN, TB> rb;
+    SlabReader<K, Cfg::BM, SM, TA> ra;
+    SlabReader<K, Cfg::BN, SN, TB> rb;
     if constexpr (!CARRY)
         la.init(a, m0, wave);
     lb.init(b, n0, wave);
@@ -223,36 +232,37 @@ __device__ __forceinline__ void entropy_product(const EntropyOperand &a, const E
     if (k_lo >= k_hi)
         return;
     const uint32_t lds0 = lds_address(lds);
-    // The next slab to load.
-    uint32_t pair = kPartPairs - pairs, slab = k_lo;
-    const uint32_t steps = pairs * (k_hi - k_lo);
+    uint32_t slab = k_lo; // the next one to load
+    const uint32_t steps = k_hi - k_lo;
     auto issue = [&](int stage) __attribute__((always_inline)) {
         if constexpr (CARRY)
-            ca.fetch(a, m0, slab * kSlabK, wave);
+            ca.fetch(a, m0, slab * K, wave);
         else
-            la.load(a, m0, part_a(pair), slab * kSlabK, lds0 + stage * Cfg::kStage, wave);
-        lb.load(b, n0, part_b(pair), slab * kSlabK, lds0 + stage * Cfg::kStage + Cfg::kSlabA, wave);
-        if (++slab == k_hi) {
-            slab = k_lo;
-            pair++;
-        }
+            la.load(a, m0, slab * K, lds0 + stage * Cfg::kStage, wave);
+        lb.load(b, n0, slab * K, lds0 + stage * Cfg::kStage + Cfg::kParts * Cfg::kSlabA, wave);
+        slab++;
     };
     auto compute = [&](int stage) __attribute__((always_inline)) {
-        const char *sa = lds + stage * Cfg::kStage, *sb = sa + Cfg::kSlabA;
+        const char *sa = lds + stage * Cfg::kStage, *sb = sa + Cfg::kParts * Cfg::kSlabA;
 #pragma unroll
-        for (int kk = 0; kk < kSlabK / 32; kk++) {
-            s16x8 fa[SM], fb[SN];
+        for (int kk = 0; kk < K / 32; kk++) {
+            s16x8 fa[Cfg::kParts][SM], fb[Cfg::kParts][SN];
 #pragma unroll
-            for (int j = 0; j < SN; j++)
-                fb[j] = rb.read(sb, j, kk);
-#pragma unroll
-            for (int i = 0; i < SM; i++)
-                fa[i] = ra.read(sa, i, kk);
-#pragma unroll
-            for (int i = 0; i < SM; i++)
+            for (int part = 0; part < Cfg::kParts; part++) {
 #pragma unroll
                 for (int j = 0; j < SN; j++)
-                    acc[i][j] = mfma16<E>(fa[i], fb[j], acc[i][j]);
+                    fb[part][j] = rb.read(sb + part * Cfg::kSlabB, j, kk);
+#pragma unroll
+                for (int i = 0; i < SM; i++)
+                    fa[part][i] = ra.read(sa + part * Cfg::kSlabA, i, kk);
+            }
+#pragma unroll
+            for (int pair = Cfg::kParts == 1 ? kPartPairs - 1 : 0; pair < kPartPairs; pair++)
+#pragma unroll
+                for (int i = 0; i < SM; i++)
+#pragma unroll
+                    for (int j = 0; j < SN; j++)
+                        acc[i][j] = mfma16<E>(fa[kPartA[pair]][i], fb[kPartB[pair]][j], acc[i][j]);
         }
     };
     if constexpr (Cfg::kStages == 2 || CARRY) {
@@ -282,7 +292,7 @@ __device__ __forceinline__ void entropy_product(const EntropyOperand &a, const E
         // kStages - 1 slabs ahead. A slab is there when no more than the later ones' loads are
         // outstanding and every wave has come to the barrier; then every wave is done with the slab
         // before, too, whose stage the next load takes.
-        constexpr int N = Cfg::kStages, kLoads = SlabLoader<Cfg, Cfg::BM, TA>::IPW + SlabLoader<Cfg, Cfg::BN, TB>::IPW;
+        constexpr int N = Cfg::kStages, kLoads = Cfg::kParts * (SlabLoader<Cfg, Cfg::BM, TA>::IPW + SlabLoader<Cfg, Cfg::BN, TB>::IPW);
 #pragma unroll
         for (int st = 0; st < N - 1; st++)
             if ((uint32_t)st < steps)
