@@ -573,10 +573,12 @@ template <typename S> struct Tiles {
     using Half = EntropyCfg<2, 2, 4, 2, 64, 3, 1>;   // 128 x 64
     using Thin = EntropyCfg<4, 1, 2, 2, 64, 3, 1>;   // 128 x 32
 };
+// Three parts leave LDS for one workgroup a CU: 8 waves of it, so that one reads while another multiplies
+// (256 x 4247 x 1728 by 128 x 64 tiles: 50 us with 4 waves, 36 with 8).
 template <> struct Tiles<float> {
     using Large = EntropyCfg<4, 2, 4, 4, 32, 2, 3>;  // 256 x 128
-    using Middle = EntropyCfg<2, 2, 4, 4, 32, 2, 3>; // 128 x 128
-    using Half = EntropyCfg<2, 2, 4, 2, 32, 4, 3>;   // 128 x 64
+    using Middle = EntropyCfg<4, 2, 2, 4, 32, 3, 3>; // 128 x 128
+    using Half = EntropyCfg<4, 2, 2, 2, 64, 2, 3>;   // 128 x 64
     using Thin = EntropyCfg<4, 1, 2, 2, 64, 2, 3>;   // 128 x 32
 };
 
@@ -597,7 +599,7 @@ inline SideTime side_time(Side s, uint32_t parts)
 {
     if (parts == 1)
         return s == Side::Large ? SideTime{1, 1.5, 1.5} : s == Side::Middle ? SideTime{2, 1.0, 0.65} : s == Side::Half ? SideTime{2, 0.6, 0.45} : SideTime{2, 0.45, 0.4};
-    return s == Side::Large ? SideTime{1, 4.2, 4.2} : s == Side::Middle ? SideTime{1, 2.7, 2.7} : s == Side::Half ? SideTime{1, 1.5, 1.5} : SideTime{1, 1.1, 1.1};
+    return s == Side::Large ? SideTime{1, 4.2, 4.2} : s == Side::Middle ? SideTime{1, 2.4, 2.4} : s == Side::Half ? SideTime{1, 1.05, 1.05} : SideTime{1, 1.1, 1.1};
 }
 inline uint64_t tiles_of(Side s, uint32_t parts, uint64_t m, uint64_t n)
 {
@@ -931,10 +933,16 @@ template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyAr
         d.b = EntropyOperand{l.grad, l.grad_plane, l.grad_ld, d.a.rows, l.grad_ld};
         d.out = static_cast<S *>(g.weight_gradient) + v * g.weight_gradient_stride;
         d.out_rows = (uint32_t)n;
-        if (g.feature_gradient && g.weight_gradient && p.weights == Side::Middle && p.features != Side::Large) {
-            e = p.features == Side::Middle ? run_both<S, typename Tiles<S>::Middle>(s, f, d, g.width, g.rows, n)
-                : p.features == Side::Half ? run_both<S, typename Tiles<S>::Half>(s, f, d, g.width, g.rows, n)
-                                           : run_both<S, typename Tiles<S>::Thin>(s, f, d, g.width, g.rows, n);
+        // (The narrowest tiles of binary32 have fewer waves.)
+        constexpr bool kThinToo = Tiles<S>::Thin::kThreads == Tiles<S>::Middle::kThreads;
+        if (g.feature_gradient && g.weight_gradient && p.weights == Side::Middle &&
+            (p.features == Side::Middle || p.features == Side::Half || (kThinToo && p.features == Side::Thin))) {
+            if (p.features == Side::Middle)
+                e = run_both<S, typename Tiles<S>::Middle>(s, f, d, g.width, g.rows, n);
+            else if (p.features == Side::Half)
+                e = run_both<S, typename Tiles<S>::Half>(s, f, d, g.width, g.rows, n);
+            else if constexpr (kThinToo)
+                e = run_both<S, typename Tiles<S>::Thin>(s, f, d, g.width, g.rows, n);
             if (e)
                 return e;
             continue;

@@ -79,6 +79,7 @@ template <class Cfg, int ROWS, bool T> struct SlabLoader {
     static constexpr int K = Cfg::K, IPW = ROWS * K / 512 / Cfg::kWaves; // 1 KiB loads a wave and part
     static_assert(IPW * 512 * Cfg::kWaves == ROWS * K, "every wave loads as much");
     static constexpr int kPieces = (T ? ROWS : K) / 8; // 16-byte pieces of a row
+    static_assert(!T || kPieces >= 16, "the permutation stays within a row");
     uint32_t off[IPW];
     __device__ __forceinline__ int row_of(int wave, int q) const { return ((wave * IPW + q) * 64 + (threadIdx.x & 63)) / kPieces; }
     // at: the tile's first row (k-contiguous) or column (k-major).
