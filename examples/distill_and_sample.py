@@ -5,7 +5,7 @@
 The teacher's output layer is run once over every context and only its top logits are kept
 (``native_top_logits``). A training step is one program: the student's logits, the loss with its
 gradient (``native_distill_step``), the weights' gradient and their update. Afterwards the student
-continues a batch of sequences, one token a row and step (``native_sample``).
+continues a batch of sequences, one token a row and step (``native_embedding``, ``native_sample``).
 """
 import importlib.util
 import os
@@ -57,7 +57,7 @@ def write(ctx, table, weights, first, length, rng):
     tokens = [np.asarray(first, np.int32)]
     features, uniform = ctx.empty((len(first), table.shape[1]), np.float32), ctx.empty((len(first),), np.float32)
     for _ in range(length):
-        ctx.upload_into(features, table[tokens[-1]])
+        ctx.native_embedding(table, ctx.upload(tokens[-1]), out=features)
         ctx.upload_into(uniform, rng.random(len(first), np.float32))
         logits = ctx.native_matmul(features, weights)
         tokens.append(ctx.native_sample(logits, uniform, temperature=0.8, top_k=40, top_p=0.95, min_p=0.01)[0].numpy())
@@ -73,8 +73,9 @@ def run(ctx, vocab=1000, steps=60, seed=0):
     labels = ctx.upload(teacher[1].numpy()[:, 0].copy())  # the teacher's first choice
     student_table = np.ascontiguousarray(table[:, :48])   # the student sees less
     weights = ctx.upload(np.zeros((48, vocab), np.float32))
-    losses = train(ctx, ctx.upload(student_table), weights, teacher, labels, steps, learning_rate=20.0, temperature=2.0)
-    return losses, write(ctx, student_table, weights, np.arange(4), 12, rng)
+    student = ctx.upload(student_table)
+    losses = train(ctx, student, weights, teacher, labels, steps, learning_rate=20.0, temperature=2.0)
+    return losses, write(ctx, student, weights, np.arange(4), 12, rng)
 
 
 def main():
