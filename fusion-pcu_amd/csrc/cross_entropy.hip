@@ -4,8 +4,8 @@
 // The loss is one product whose tiles leave a (maximum, sum of exponentials) for each row and the
 // label's logit; a reduction joins them. The gradients go over the vocabulary in pieces: a piece's
 // logits are made again and turned into G where they lie in registers, G goes to a buffer that the
-// caches hold, and two products read it. That is 2 products of rows x vocab x width for a loss, 8 / 2 for
-// a step against 6 / 2 if the logits were kept.
+// caches hold, and two products read it. That is one product of rows x vocab x width for a loss and four for
+// a step, against three if the logits were kept (4096 x 128000: 1 GB in 16 bits, written and read twice).
 //
 // 16-bit features and weights go to the matrix cores as they are. Binary32 ones are split into three
 // bfloat16 parts of 8 bits (exact), of whose products six are summed, smallest first: binary32's precision
