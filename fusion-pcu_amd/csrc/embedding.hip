@@ -8,6 +8,8 @@
 // values, no second pass over the table to clear it. Both directions are bound by HBM.
 #include "pcu_rows.hpp"
 
+#include <type_traits>
+
 #pragma clang fp contract(off)
 
 namespace pcu {
@@ -558,7 +560,7 @@ template <typename S>
 __global__ __launch_bounds__(256) void k_embed_first(EmbedBackArgs g, uint32_t across, uint32_t sums, uint64_t each, ProgramClose close)
 {
     using T = typename StatOf<S>::T;
-    constexpr int V = kVec<S>, N = kDirect / 64, U = 8;
+    constexpr int V = kVec<S>, N = kDirect / 64;
     if (block_gate_closed(g.gate))
         return;
     if (blockIdx.x >= sums) {
@@ -589,25 +591,42 @@ __global__ __launch_bounds__(256) void k_embed_first(EmbedBackArgs g, uint32_t a
     if (first) {
         const u32x4 base = v < vecs ? load_base<S>(g, t, v) : u32x4{};
         T sum[V] = {};
+        // U terms' loads under way together, no branch between them: past the last term it is read again (1024 terms
+        // of one token, 64 wide: 102 us with a branch a load, 65 so; 16 at a time 63).
+        auto add_terms = [&](auto count, auto load, uint64_t &left, int q) {
+            constexpr int U = decltype(count)::value;
+            u32x4 raw[U];
+            uint64_t l = left;
+            uint32_t place = 0;
 #pragma unroll
-        for (int q = 0; q < N; q++)
-            for (uint64_t left = same[q]; left;) {
-                u32x4 raw[U];
-                uint64_t l = left;
-#pragma unroll
-                for (int k = 0; k < U; k++, l &= l - 1)
-                    if (l && v < vecs)
-                        raw[k] = load_piece(static_cast<const S *>(g.gradient) + (uint64_t)(q * 64 + __builtin_ctzll(l)) * g.gradient_stride, v, g.width);
-#pragma unroll
-                for (int k = 0; k < U; k++, left &= left - 1)
-                    if (left) {
-                        T x[V];
-                        unpack<S>(raw[k], x);
-#pragma unroll
-                        for (int e = 0; e < V; e++)
-                            sum[e] += x[e];
-                    }
+            for (int k = 0; k < U; k++) {
+                place = l ? __builtin_ctzll(l) : place;
+                raw[k] = load(static_cast<const S *>(g.gradient) + (uint64_t)(q * 64 + place) * g.gradient_stride);
+                l &= l - 1;
             }
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                T x[V];
+                unpack<S>(raw[k], x);
+#pragma unroll
+                for (int e = 0; e < V; e++)
+                    sum[e] += left ? x[e] : (T)0; // (no sum is -0)
+                left &= left - 1;
+            }
+        };
+        auto add_all = [&](auto load) {
+            for (int q = 0; q < N; q++)
+                for (uint64_t left = same[q]; left;)
+                    if (left & (left - 1))
+                        add_terms(std::integral_constant<int, 8>{}, load, left, q);
+                    else
+                        add_terms(std::integral_constant<int, 1>{}, load, left, q);
+        };
+        const uint32_t mine = min(v, vecs - 1);
+        if (__all((mine + 1) * V <= g.width))
+            add_all([&](const S *row) { return load_whole(row, mine); });
+        else
+            add_all([&](const S *row) { return load_piece(row, mine, g.width); });
         if (v < vecs)
             write_sum<S>(g, t, v, base, sum, close.words != nullptr);
     }
