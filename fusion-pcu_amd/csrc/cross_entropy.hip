@@ -24,19 +24,6 @@
 namespace pcu {
 namespace {
 
-// The first 8 bits of a value, as a bfloat16; v becomes the rest. Three of them are the whole value;
-// what is not finite is its first part alone.
-__device__ __forceinline__ uint32_t first_part(float &v)
-{
-    const uint32_t b = __float_as_uint(v);
-    if ((b & 0x7f800000u) == 0x7f800000u) {
-        v = 0.0f;
-        return (b >> 16) | ((b & 0x7fffffu) ? 0x40u : 0u);
-    }
-    v -= __uint_as_float(b & 0xffff0000u); // exact
-    return b >> 16;
-}
-
 template <typename S> struct ElemOf { using T = S; };
 template <> struct ElemOf<float> { using T = __bf16; };
 template <typename S> constexpr int kParts = sizeof(S) == 4 ? 3 : 1;
@@ -80,14 +67,8 @@ template <typename S> __device__ __forceinline__ void pack_rows(const PackArgs &
                 unpack<float>(load_piece(row, c / 4, g.cols), v);
                 unpack<float>(load_piece(row, c / 4 + 1, g.cols), v + 4);
             }
-            u32x4 raw[3] = {};
-#pragma unroll
-            for (uint32_t e = 0; e < 8; e++) {
-                float x = v[e];
-#pragma unroll
-                for (int k = 0; k < 3; k++)
-                    raw[k][e / 2] |= first_part(x) << (16 * (e & 1));
-            }
+            u32x4 raw[3];
+            split8(v, raw);
 #pragma unroll
             for (int k = 0; k < 3; k++)
                 *reinterpret_cast<u32x4 *>(out + k * g.plane) = raw[k];
@@ -252,7 +233,9 @@ template <typename S, class Cfg, bool GRAD, bool CARRY> __global__ __launch_boun
         scales[j] = GRAD && n < g.rows ? g.row.scale[n] * g.boost : 0.0f;
     }
     f32x4 acc[SM][SN];
-    entropy_product<E, Cfg, false, false, CARRY>(g.w, g.x, m0, n0, 0, g.slabs * (kSlabK / Cfg::K), lds, acc);
+    // (The gradient's tiles go on to a whole slab of rows: those past the last one are zeros.)
+    const uint32_t slabs = GRAD && n0 >= g.rows ? 0 : g.slabs * (kSlabK / Cfg::K);
+    entropy_product<E, Cfg, false, false, CARRY>(g.w, g.x, m0, n0, 0, slabs, lds, acc);
     const uint32_t lane = threadIdx.x & 63;
     const uint32_t v0 = g.first + m0 + wm; // of acc[i][j][r]: v0 + acc_row(i, r)
     const bool ragged = g.first + m0 + BM > g.vocab;
@@ -404,7 +387,7 @@ struct ProductArgs {
 };
 
 // dx: width down (from the weights, k-major), rows across (G); sums in binary32, k split.
-template <typename S, class Cfg> __device__ __forceinline__ void feature_tile(const ProductArgs &g, uint32_t block, char *lds)
+template <typename S, class Cfg, bool CARRY> __device__ __forceinline__ void feature_tile(const ProductArgs &g, uint32_t block, char *lds)
 {
     using E = typename ElemOf<S>::T;
     constexpr int SM = Cfg::SM, SN = Cfg::SN;
@@ -412,7 +395,7 @@ template <typename S, class Cfg> __device__ __forceinline__ void feature_tile(co
     const uint32_t m0 = t.tm * Cfg::BM, n0 = t.tn * Cfg::BN;
     const uint32_t k_lo = (uint32_t)((uint64_t)g.slabs * t.split / g.splits), k_hi = (uint32_t)((uint64_t)g.slabs * (t.split + 1) / g.splits);
     f32x4 acc[SM][SN];
-    entropy_product<E, Cfg, true, false, false>(g.a, g.b, m0, n0, k_lo * (kSlabK / Cfg::K), k_hi * (kSlabK / Cfg::K), lds, acc);
+    entropy_product<E, Cfg, true, false, CARRY>(g.a, g.b, m0, n0, k_lo * (kSlabK / Cfg::K), k_hi * (kSlabK / Cfg::K), lds, acc);
     const uint32_t wave = threadIdx.x / 64, m = m0 + wave / Cfg::WN * SM * 16, n = n0 + wave % Cfg::WN * SN * 16;
 #pragma unroll
     for (int j = 0; j < SN; j++)
@@ -422,11 +405,11 @@ template <typename S, class Cfg> __device__ __forceinline__ void feature_tile(co
             *to = g.add ? *to + acc[i][j] : acc[i][j];
         }
 }
-template <typename S, class Cfg> __global__ __launch_bounds__(Cfg::kThreads) void k_feature_gradient(ProductArgs g)
+template <typename S, class Cfg, bool CARRY> __global__ __launch_bounds__(Cfg::kThreads) void k_feature_gradient(ProductArgs g)
 {
     extern __shared__ __align__(16) char lds[];
     if (!block_gate_closed(g.gate))
-        feature_tile<S, Cfg>(g, blockIdx.x, lds);
+        feature_tile<S, Cfg, CARRY>(g, blockIdx.x, lds);
 }
 
 // dx from the splits' sums, in their order.
@@ -543,14 +526,14 @@ template <typename S, class Cfg> __global__ __launch_bounds__(Cfg::kThreads) voi
         weight_tile<S, Cfg>(g, blockIdx.x, lds);
 }
 // Both in one launch, `features` workgroups for the first: neither fills the CUs alone.
-template <typename S, class CfgF, class CfgW> __global__ __launch_bounds__(CfgF::kThreads) void k_both_gradients(ProductArgs f, uint32_t features, ProductArgs w)
+template <typename S, class CfgF, class CfgW, bool CARRY> __global__ __launch_bounds__(CfgF::kThreads) void k_both_gradients(ProductArgs f, uint32_t features, ProductArgs w)
 {
     static_assert(CfgF::kThreads == CfgW::kThreads, "one kind of workgroup");
     extern __shared__ __align__(16) char lds[];
     if (block_gate_closed(f.gate))
         return;
     if (blockIdx.x < features)
-        feature_tile<S, CfgF>(f, blockIdx.x, lds);
+        feature_tile<S, CfgF, CARRY>(f, blockIdx.x, lds);
     else
         weight_tile<S, CfgW>(w, blockIdx.x - features, lds);
 }
@@ -628,15 +611,21 @@ inline Side choose(uint32_t parts, uint64_t m, uint64_t n, uint64_t slabs, bool 
 }
 // Where k can be split: by the whole work, unless a CU would have next to none of it. Few rows take
 // narrower tiles, which read the weights at HBM's rate.
-inline Side choose_split(uint32_t parts, uint64_t m, uint64_t rows, uint64_t slabs)
+inline Side choose_split(uint32_t parts, uint64_t m, uint64_t rows, uint64_t slabs, bool carry)
 {
     if (rows <= 64)
-        return rows <= 32 ? Side::Thin : Side::Half;
+        return rows <= 32 && !(carry && parts == 3) ? Side::Thin : Side::Half;
     const SideTime l = side_time(Side::Large, parts), k = side_time(Side::Middle, parts);
     const double large = (double)tiles_of(Side::Large, parts, m, rows) / (l.per_cu * kGfx950Cus);
     const double middle = (double)tiles_of(Side::Middle, parts, m, rows) / (k.per_cu * kGfx950Cus);
     return large * l.full <= middle * k.full && large * slabs >= 4 ? Side::Large : Side::Middle;
 }
+
+// Binary32 weights that few rows read are split by the tiles' own workgroups, on their way to LDS, where a
+// copy in parts would cost more than it saves: 6 bytes a value written, and read instead of 4 (20 rows, vocabulary 51939,
+// width 896: 388 us of kernels with the copy, 283 so; 128, 121922 x 2083: 2400 and 2180). Tiles of one column each
+// (128 rows) read them once. Small weights are in the caches, and their copy's launch is needed anyway (64, 1000 x 64: 30.7 with, 32.7 so).
+constexpr uint64_t kSplitRows = 128, kSplitBytes = 8ull << 20;
 
 // How a call goes over its vocabulary and what its scratch holds.
 struct EntropyPlan {
@@ -661,8 +650,9 @@ struct EntropyPlan {
         // 390; a step of 29 rows, 34688 x 3211: three passes 324 us, the copy and three passes 248).
         const bool direct = g.width % kSlabK == 0 && g.weight_stride % 8 == 0 && ((uintptr_t)g.weights & 15) == 0 &&
                             g.weight_stride * 2 * 256 <= UINT32_MAX;
-        pack_weights = parts == 3 || (!direct && grads);
-        carry = !pack_weights && !direct;
+        const bool few = g.rows <= kSplitRows && (uint64_t)g.vocab * g.width * 4 > kSplitBytes;
+        pack_weights = parts == 3 ? !few : !direct && grads;
+        carry = parts == 3 ? few : !pack_weights && !direct;
         const uint64_t vocab_up = round_up(g.vocab, 256);
         const uint64_t row_bytes = 2ull * parts * ld;
         // G's piece is what the 256 MiB cache behind the L2s can hold; packed weights are kept
@@ -679,8 +669,8 @@ struct EntropyPlan {
             piece = piece < fit ? piece : fit < 256 ? 256 : fit;
         }
         const uint64_t within = piece < g.vocab ? piece : g.vocab, most = (within + kSlabK - 1) / kSlabK;
-        logits = g.rows <= 64 ? choose_split(parts, g.vocab, g.rows, 1) : choose(parts, g.vocab, g.rows, ld / kSlabK, true);
-        features = choose_split(parts, g.width, g.rows, most);
+        logits = g.rows <= 64 ? choose_split(parts, g.vocab, g.rows, 1, carry) : choose(parts, g.vocab, g.rows, ld / kSlabK, !(carry && parts == 3));
+        features = choose_split(parts, g.width, g.rows, most, carry);
         weights = choose(parts, g.width, within, (g.rows + kSlabK - 1) / kSlabK, false);
         const uint64_t tiles = tiles_of(features, parts, g.width, g.rows);
         const uint64_t per = side_time(features, parts).per_cu, want = tiles ? per * kGfx950Cus / tiles : 1;
@@ -728,7 +718,7 @@ template <typename S, class Cfg, bool GRAD, bool CARRY> hipError_t run_logits(hi
 }
 template <typename S, class Cfg, bool GRAD> hipError_t logits_of(bool carry, hipStream_t s, const LogitArgs &a, uint64_t vocab_rows, uint64_t rows)
 {
-    if constexpr (sizeof(S) == 2 && !GRAD)
+    if constexpr (sizeof(S) == 4 || !GRAD)
         if (carry)
             return run_logits<S, Cfg, GRAD, true>(s, a, vocab_rows, rows);
     return run_logits<S, Cfg, GRAD, false>(s, a, vocab_rows, rows);
@@ -743,15 +733,22 @@ template <typename S, bool GRAD> hipError_t logits_by(Side side, bool carry, hip
     }
 }
 
-template <typename S, class Cfg> hipError_t run_features(hipStream_t s, ProductArgs a, uint64_t width, uint64_t rows)
+template <typename S, class Cfg, bool CARRY> hipError_t launch_features(hipStream_t s, const ProductArgs &a)
+{
+    hipError_t e = with_lds(k_feature_gradient<S, Cfg, CARRY>, Cfg::kLds);
+    if (e)
+        return e;
+    hipLaunchKernelGGL((k_feature_gradient<S, Cfg, CARRY>), dim3(a.tiles_m * a.tiles_n * a.splits), dim3(Cfg::kThreads), Cfg::kLds, s, a);
+    return hipGetLastError();
+}
+template <typename S, class Cfg> hipError_t run_features(bool carry, hipStream_t s, ProductArgs a, uint64_t width, uint64_t rows)
 {
     a.tiles_m = (uint32_t)((width + Cfg::BM - 1) / Cfg::BM);
     a.tiles_n = (uint32_t)((rows + Cfg::BN - 1) / Cfg::BN);
-    hipError_t e = with_lds(k_feature_gradient<S, Cfg>, Cfg::kLds);
-    if (e)
-        return e;
-    hipLaunchKernelGGL((k_feature_gradient<S, Cfg>), dim3(a.tiles_m * a.tiles_n * a.splits), dim3(Cfg::kThreads), Cfg::kLds, s, a);
-    return hipGetLastError();
+    if constexpr (sizeof(S) == 4)
+        if (carry)
+            return launch_features<S, Cfg, true>(s, a);
+    return launch_features<S, Cfg, false>(s, a);
 }
 template <typename S, class Cfg> hipError_t run_weights(hipStream_t s, ProductArgs a, uint64_t width, uint64_t vocab_rows)
 {
@@ -774,22 +771,30 @@ inline unsigned pack_blocks(uint64_t rows, uint64_t ld)
 }
 
 // Features' and weights' gradients of a piece in one launch, the weights' by 128 x 128 tiles.
+template <typename S, class Cfg, bool CARRY> hipError_t launch_both(hipStream_t s, const ProductArgs &f, const ProductArgs &w)
+{
+    using Middle = typename Tiles<S>::Middle;
+    constexpr uint32_t lds = Cfg::kLds > Middle::kLds ? Cfg::kLds : Middle::kLds;
+    hipError_t e = with_lds(k_both_gradients<S, Cfg, Middle, CARRY>, lds);
+    if (e)
+        return e;
+    const uint32_t features = f.tiles_m * f.tiles_n * f.splits;
+    hipLaunchKernelGGL((k_both_gradients<S, Cfg, Middle, CARRY>), dim3(features + w.tiles_m * w.tiles_n), dim3(Cfg::kThreads), lds, s, f,
+                       features, w);
+    return hipGetLastError();
+}
 template <typename S, class Cfg>
-hipError_t run_both(hipStream_t s, ProductArgs f, ProductArgs w, uint64_t width, uint64_t rows, uint64_t vocab_rows)
+hipError_t run_both(bool carry, hipStream_t s, ProductArgs f, ProductArgs w, uint64_t width, uint64_t rows, uint64_t vocab_rows)
 {
     using Middle = typename Tiles<S>::Middle;
     f.tiles_m = (uint32_t)((width + Cfg::BM - 1) / Cfg::BM);
     f.tiles_n = (uint32_t)((rows + Cfg::BN - 1) / Cfg::BN);
     w.tiles_m = (uint32_t)((width + Middle::BM - 1) / Middle::BM);
     w.tiles_n = (uint32_t)((vocab_rows + Middle::BN - 1) / Middle::BN);
-    constexpr uint32_t lds = Cfg::kLds > Middle::kLds ? Cfg::kLds : Middle::kLds;
-    hipError_t e = with_lds(k_both_gradients<S, Cfg, Middle>, lds);
-    if (e)
-        return e;
-    const uint32_t features = f.tiles_m * f.tiles_n * f.splits;
-    hipLaunchKernelGGL((k_both_gradients<S, Cfg, Middle>), dim3(features + w.tiles_m * w.tiles_n), dim3(Cfg::kThreads), lds, s, f,
-                       features, w);
-    return hipGetLastError();
+    if constexpr (sizeof(S) == 4)
+        if (carry)
+            return launch_both<S, Cfg, true>(s, f, w);
+    return launch_both<S, Cfg, false>(s, f, w);
 }
 
 template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyArgs &g, void *scratch, ProgramClose close, bool *closed)
@@ -849,7 +854,7 @@ template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyAr
     // The weights of vocabulary [v, v + n), packed here where they are not kept.
     auto weights = [&](uint64_t v, uint64_t n, EntropyOperand *o) {
         if (!p.pack_weights) {
-            *o = EntropyOperand{static_cast<const uint16_t *>(g.weights) + v * g.weight_stride, 0, (uint32_t)g.weight_stride,
+            *o = EntropyOperand{reinterpret_cast<const uint16_t *>(static_cast<const S *>(g.weights) + v * g.weight_stride), 0, (uint32_t)g.weight_stride,
                                 (uint32_t)n, g.width};
             return hipSuccess;
         }
@@ -938,20 +943,20 @@ template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyAr
         if (g.feature_gradient && g.weight_gradient && p.weights == Side::Middle &&
             (p.features == Side::Middle || p.features == Side::Half || (kThinToo && p.features == Side::Thin))) {
             if (p.features == Side::Middle)
-                e = run_both<S, typename Tiles<S>::Middle>(s, f, d, g.width, g.rows, n);
+                e = run_both<S, typename Tiles<S>::Middle>(p.carry, s, f, d, g.width, g.rows, n);
             else if (p.features == Side::Half)
-                e = run_both<S, typename Tiles<S>::Half>(s, f, d, g.width, g.rows, n);
+                e = run_both<S, typename Tiles<S>::Half>(p.carry, s, f, d, g.width, g.rows, n);
             else if constexpr (kThinToo)
-                e = run_both<S, typename Tiles<S>::Thin>(s, f, d, g.width, g.rows, n);
+                e = run_both<S, typename Tiles<S>::Thin>(p.carry, s, f, d, g.width, g.rows, n);
             if (e)
                 return e;
             continue;
         }
         if (g.feature_gradient) {
-            e = p.features == Side::Large    ? run_features<S, typename Tiles<S>::Large>(s, f, g.width, g.rows)
-                : p.features == Side::Middle ? run_features<S, typename Tiles<S>::Middle>(s, f, g.width, g.rows)
-                : p.features == Side::Half   ? run_features<S, typename Tiles<S>::Half>(s, f, g.width, g.rows)
-                                             : run_features<S, typename Tiles<S>::Thin>(s, f, g.width, g.rows);
+            e = p.features == Side::Large    ? run_features<S, typename Tiles<S>::Large>(p.carry, s, f, g.width, g.rows)
+                : p.features == Side::Middle ? run_features<S, typename Tiles<S>::Middle>(p.carry, s, f, g.width, g.rows)
+                : p.features == Side::Half   ? run_features<S, typename Tiles<S>::Half>(p.carry, s, f, g.width, g.rows)
+                                             : run_features<S, typename Tiles<S>::Thin>(p.carry, s, f, g.width, g.rows);
             if (e)
                 return e;
         }

@@ -44,6 +44,56 @@ constexpr int kSlabK = 64; // operands are padded to whole slabs of the longer k
 constexpr int kPartPairs = 6;
 __device__ constexpr int kPartA[kPartPairs] = {2, 0, 1, 1, 0, 0}, kPartB[kPartPairs] = {0, 2, 1, 0, 1, 0};
 
+// The first 8 bits of a value, as a bfloat16; v becomes the rest. Three of them are the whole value;
+// what is not finite is its first part alone.
+__device__ __forceinline__ uint32_t first_part(float &v)
+{
+    const uint32_t b = __float_as_uint(v);
+    if ((b & 0x7f800000u) == 0x7f800000u) {
+        v = 0.0f;
+        return (b >> 16) | ((b & 0x7fffffu) ? 0x40u : 0u);
+    }
+    v -= __uint_as_float(b & 0xffff0000u); // exact
+    return b >> 16;
+}
+
+// The parts of 8 values.
+__device__ __forceinline__ void split8(const float (&v)[8], u32x4 (&raw)[3])
+{
+    uint32_t most = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
+    if (most < 0x7f800000u) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            x[e] = v[e];
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const uint32_t lo = __float_as_uint(x[e]), hi = __float_as_uint(x[e + 1]);
+                raw[k][e / 2] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+                if (k < 2) { // exact
+                    x[e] -= __uint_as_float(lo & 0xffff0000u);
+                    x[e + 1] -= __uint_as_float(hi & 0xffff0000u);
+                }
+            }
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < 3; k++)
+        raw[k] = u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        float x = v[e];
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+            raw[k][e / 2] |= first_part(x) << (16 * (e & 1));
+    }
+}
+
 // WM x WN waves, each with SM x SN subtiles of 16 x 16; slabs of K, STAGES of them in LDS, of PARTS parts.
 template <int WM_, int WN_, int SM_, int SN_, int K_, int STAGES, int PARTS> struct EntropyCfg {
     static constexpr int WM = WM_, WN = WN_, SM = SM_, SN = SN_, K = K_, kStages = STAGES, kParts = PARTS;
@@ -74,6 +124,10 @@ struct EntropyOperand {
 __device__ __forceinline__ uint32_t k_major_swap(uint32_t k) { return 2 * ((k & 3) | (k >> 1 & 4)); }
 
 __device__ __forceinline__ uint32_t k_contiguous_swap(uint32_t row, int k) { return k == 64 ? row / 2 & 7 : row / 4 & 3; }
+
+// What operands that go through registers are made of.
+template <int PARTS> struct SourceOf { typedef uint16_t T; };
+template <> struct SourceOf<3> { typedef uint32_t T; };
 
 template <class Cfg, int ROWS, bool T> struct SlabLoader {
     static constexpr int K = Cfg::K, IPW = ROWS * K / 512 / Cfg::kWaves; // 1 KiB loads a wave and part
@@ -117,10 +171,13 @@ template <class Cfg, int ROWS, bool T> struct SlabLoader {
     }
 };
 
-// The same through registers, for rows at any alignment of their type and of any length.
+// The same through registers, for rows at any alignment of their type and of any length. Where tiles take
+// three parts, the rows are binary32 values (`p` points to those) and are split here.
 template <class Cfg, int ROWS, bool T> struct SlabCarrier {
     static constexpr int K = Cfg::K, IPW = ROWS * K / 512 / Cfg::kWaves, kPieces = (T ? ROWS : K) / 8;
-    u32x4 held[IPW];
+    static constexpr int kHeld = Cfg::kParts == 3 ? 2 : 1; // 16-byte vectors of 8 values
+    typedef typename SourceOf<Cfg::kParts>::T Source;
+    u32x4 held[IPW][kHeld];
     __device__ __forceinline__ void fetch(const EntropyOperand &o, uint32_t at, uint32_t k0, int wave)
     {
         const uint32_t lane = threadIdx.x & 63;
@@ -130,24 +187,46 @@ template <class Cfg, int ROWS, bool T> struct SlabCarrier {
             const uint32_t r = ((wave * IPW + q) * 64 + lane) / kPieces, piece = lane % kPieces;
             const uint32_t row = min((T ? k0 : at) + r, o.rows - 1);
             const uint32_t c = (T ? at : k0) + (T ? piece ^ k_major_swap(r) : piece ^ k_contiguous_swap(r, K)) * 8;
-            const uint16_t *from = o.p + (uint64_t)row * o.ld + c;
+            const Source *from = reinterpret_cast<const Source *>(o.p) + (uint64_t)row * o.ld + c;
             if (!ragged || c + 8 <= o.cols) {
-                held[q] = *reinterpret_cast<const u32x4_any *>(from);
+#pragma unroll
+                for (int h = 0; h < kHeld; h++)
+                    held[q][h] = *reinterpret_cast<const u32x4_any *>(from + h * (8 / kHeld));
             } else {
-                u32x4 raw = {0, 0, 0, 0};
+                u32x4 raw[kHeld] = {};
 #pragma unroll
                 for (uint32_t e = 0; e < 8; e++)
-                    if (c + e < o.cols)
-                        raw[e / 2] |= (uint32_t)from[e] << (16 * (e & 1));
-                held[q] = raw;
+                    if (c + e < o.cols) {
+                        if constexpr (kHeld == 2)
+                            raw[e / 4][e % 4] = from[e];
+                        else
+                            raw[0][e / 2] |= (uint32_t)from[e] << (16 * (e & 1));
+                    }
+#pragma unroll
+                for (int h = 0; h < kHeld; h++)
+                    held[q][h] = raw[h];
             }
         }
     }
     __device__ __forceinline__ void stash(char *slab, int wave) const
     {
 #pragma unroll
-        for (int q = 0; q < IPW; q++)
-            *reinterpret_cast<u32x4 *>(slab + (wave * IPW + q) * 1024 + (threadIdx.x & 63) * 16) = held[q];
+        for (int q = 0; q < IPW; q++) {
+            char *to = slab + (wave * IPW + q) * 1024 + (threadIdx.x & 63) * 16;
+            if constexpr (kHeld == 2) {
+                float v[8];
+                u32x4 raw[3];
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    v[e] = __uint_as_float(held[q][e / 4][e % 4]);
+                split8(v, raw);
+#pragma unroll
+                for (int part = 0; part < 3; part++)
+                    *reinterpret_cast<u32x4 *>(to + part * ROWS * K * 2) = raw[part];
+            } else {
+                *reinterpret_cast<u32x4 *>(to) = held[q][0];
+            }
+        }
     }
 };
 
@@ -206,14 +285,13 @@ __device__ __forceinline__ EntropyTile entropy_tile(uint32_t bid, uint32_t tiles
 }
 
 // acc = the tile of A B over slabs [k_lo, k_hi). a, b: the operands; m0, n0: the tile's first row and
-// column; lds: Cfg::kTile bytes. CARRY: A goes through registers (one part alone). No LDS is read after
+// column; lds: Cfg::kTile bytes. CARRY: A goes through registers. No LDS is read after
 // the last barrier.
 template <typename E, class Cfg, bool TA, bool TB, bool CARRY>
 __device__ __forceinline__ void entropy_product(const EntropyOperand &a, const EntropyOperand &b, uint32_t m0, uint32_t n0, uint32_t k_lo,
                                                 uint32_t k_hi, char *lds, f32x4 (&acc)[Cfg::SM][Cfg::SN])
 {
     constexpr int SM = Cfg::SM, SN = Cfg::SN, K = Cfg::K;
-    static_assert(!CARRY || Cfg::kParts == 1, "parts are packed");
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     SlabLoader<Cfg, Cfg::BM, TA> la;
     SlabCarrier<Cfg, Cfg::BM, TA> ca;
