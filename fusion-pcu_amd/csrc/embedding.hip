@@ -105,6 +105,9 @@ template <typename S> hipError_t launch_embed_t(hipStream_t s, const EmbedArgs &
 // equal digits find each other by one ballot for each bit.
 constexpr int kSortTile = 2048, kSortThreads = 512, kSortRounds = kSortTile / kSortThreads;
 constexpr int kSortWaves = kSortThreads / 64;
+// The most that one workgroup sorts alone, of 1024 threads (4096 tokens, 1000 x 64 in binary32: a call that sorts by
+// tiles in 4 launches 37 us, 33 so; all tokens the same 57 and 43).
+constexpr int kSortAlone = 8192;
 
 __device__ __forceinline__ uint32_t token_key(const int32_t *tokens, uint64_t i, uint32_t vocab)
 {
@@ -158,18 +161,18 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_count(EmbedBackArgs g, co
 
 // Ranks of a tile's keys among the tile's equal digits, wave by wave: rank[r] within the wave, and
 // wave_count[wave][digit], the wave's number of each digit.
-template <typename Key>
+template <int THREADS, int ROUNDS, typename Key>
 __device__ __forceinline__ void rank_tile(Key key_at, uint64_t n, uint64_t tile0, int shift, int bits,
-                                          uint32_t (&k)[kSortRounds], uint32_t (&rank)[kSortRounds], uint32_t *wave_count)
+                                          uint32_t (&k)[ROUNDS], uint32_t (&rank)[ROUNDS], uint32_t *wave_count)
 {
     const uint32_t bins = 1u << bits, wave = threadIdx.x / 64, lane = threadIdx.x & 63;
     uint32_t *mine = wave_count + wave * bins;
-    for (uint32_t b = threadIdx.x; b < bins * kSortWaves; b += kSortThreads)
+    for (uint32_t b = threadIdx.x; b < bins * THREADS / 64; b += THREADS)
         wave_count[b] = 0;
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kSortRounds; r++) {
-        const uint64_t i = tile0 + wave * (kSortTile / kSortWaves) + r * 64 + lane;
+    for (int r = 0; r < ROUNDS; r++) {
+        const uint64_t i = tile0 + wave * (ROUNDS * 64) + r * 64 + lane;
         const bool on = i < n;
         k[r] = on ? key_at(i) : ~0u;
         const uint32_t d = (k[r] >> shift) & (bins - 1);
@@ -186,9 +189,9 @@ __device__ __forceinline__ void rank_tile(Key key_at, uint64_t n, uint64_t tile0
 }
 
 // Exclusive prefix over a tile's or launch's bins, in place: v[b] becomes the sum before bin b.
-__device__ __forceinline__ void scan_bins(uint32_t *v, uint32_t bins, uint32_t *part)
+template <int THREADS> __device__ __forceinline__ void scan_bins(uint32_t *v, uint32_t bins, uint32_t *part)
 {
-    const uint32_t each = (bins + kSortThreads - 1) / kSortThreads, b0 = threadIdx.x * each;
+    const uint32_t each = (bins + THREADS - 1) / THREADS, b0 = threadIdx.x * each;
     uint32_t sum = 0;
     for (uint32_t b = b0; b < b0 + each && b < bins; b++)
         sum += v[b];
@@ -249,7 +252,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_move(EmbedBackArgs g, con
     const uint32_t bins = 1u << bits, wave = threadIdx.x / 64;
     uint32_t *first = lds, *wave_count = lds + bins, *part = wave_count + bins * kSortWaves;
     uint32_t k[kSortRounds], rank[kSortRounds];
-    rank_tile([&](uint64_t i) { return keys ? keys[i] : token_key(g.tokens, i, g.vocab); }, g.rows,
+    rank_tile<kSortThreads, kSortRounds>([&](uint64_t i) { return keys ? keys[i] : token_key(g.tokens, i, g.vocab); }, g.rows,
               (uint64_t)blockIdx.x * kSortTile, shift, bits, k, rank, wave_count);
     // A digit's count in all tiles; without totals (few tiles) the tiles' counts are added up here.
     for (uint32_t b = threadIdx.x; b < bins; b += kSortThreads) {
@@ -259,7 +262,7 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_move(EmbedBackArgs g, con
         first[b] = all;
     }
     __syncthreads();
-    scan_bins(first, bins, part);
+    scan_bins<kSortThreads>(first, bins, part);
     for (uint32_t b = threadIdx.x; b < bins; b += kSortThreads) {
         uint32_t at = first[b] + (totals ? counts[(uint64_t)blockIdx.x * bins + b] : 0);
         for (uint32_t t = 0; !totals && t < blockIdx.x; t++)
@@ -282,52 +285,52 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_move(EmbedBackArgs g, con
     }
 }
 
-// One tile at most: both passes in one workgroup, through LDS.
-__global__ __launch_bounds__(kSortThreads) void k_sort_one(EmbedBackArgs g, int bits, uint32_t *keys_out, uint32_t *places_out)
+// Both passes in one workgroup, through LDS.
+template <int THREADS, int ROUNDS> __global__ __launch_bounds__(THREADS) void k_sort_one(EmbedBackArgs g, int bits, uint32_t *keys_out, uint32_t *places_out)
 {
     extern __shared__ uint32_t lds[];
     if (block_gate_closed(g.gate))
         return;
     const uint32_t bins = 1u << bits, wave = threadIdx.x / 64, lane = threadIdx.x & 63, n = (uint32_t)g.rows;
-    uint32_t *first = lds, *wave_count = lds + bins, *part = wave_count + bins * kSortWaves;
-    uint32_t *mid_key = part + kSortWaves, *mid_place = mid_key + kSortTile;
+    uint32_t *first = lds, *wave_count = lds + bins, *part = wave_count + bins * (THREADS / 64);
+    uint32_t *mid_key = part + THREADS / 64, *mid_place = mid_key + THREADS * ROUNDS;
     uint64_t key = kNoFault;
-    for (uint32_t i = threadIdx.x; i < n; i += kSortThreads) {
+    for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
         const int32_t t = g.tokens[i];
         if (t >= 0 && (uint32_t)t >= g.vocab && key == kNoFault)
             key = pack_fault(i, kInvalid);
     }
     wave_record_fault(key, g.fault, g.gate);
     for (int pass = 0; pass < 2; pass++) {
-        uint32_t k[kSortRounds], rank[kSortRounds];
-        rank_tile([&](uint64_t i) { return pass ? mid_key[i] : token_key(g.tokens, i, g.vocab); }, n, 0, pass * bits, bits,
+        uint32_t k[ROUNDS], rank[ROUNDS];
+        rank_tile<THREADS, ROUNDS>([&](uint64_t i) { return pass ? mid_key[i] : token_key(g.tokens, i, g.vocab); }, n, 0, pass * bits, bits,
                   k, rank, wave_count);
-        for (uint32_t b = threadIdx.x; b < bins; b += kSortThreads) {
+        for (uint32_t b = threadIdx.x; b < bins; b += THREADS) {
             uint32_t all = 0;
-            for (int w = 0; w < kSortWaves; w++)
+            for (int w = 0; w < THREADS / 64; w++)
                 all += wave_count[w * bins + b];
             first[b] = all;
         }
         __syncthreads();
-        scan_bins(first, bins, part);
-        for (uint32_t b = threadIdx.x; b < bins; b += kSortThreads) {
+        scan_bins<THREADS>(first, bins, part);
+        for (uint32_t b = threadIdx.x; b < bins; b += THREADS) {
             uint32_t at = first[b];
-            for (int w = 0; w < kSortWaves; w++) {
+            for (int w = 0; w < THREADS / 64; w++) {
                 const uint32_t c = wave_count[w * bins + b];
                 wave_count[w * bins + b] = at;
                 at += c;
             }
         }
-        uint32_t place[kSortRounds];
+        uint32_t place[ROUNDS];
 #pragma unroll
-        for (int r = 0; r < kSortRounds; r++) {
-            const uint32_t i = wave * (kSortTile / kSortWaves) + r * 64 + lane;
+        for (int r = 0; r < ROUNDS; r++) {
+            const uint32_t i = wave * (ROUNDS * 64) + r * 64 + lane;
             place[r] = pass && i < n ? mid_place[i] : i;
         }
         __syncthreads();
 #pragma unroll
-        for (int r = 0; r < kSortRounds; r++) {
-            const uint32_t i = wave * (kSortTile / kSortWaves) + r * 64 + lane;
+        for (int r = 0; r < ROUNDS; r++) {
+            const uint32_t i = wave * (ROUNDS * 64) + r * 64 + lane;
             if (i < n) {
                 const uint32_t to = wave_count[wave * bins + ((k[r] >> (pass * bits)) & (bins - 1))] + rank[r];
                 (pass ? keys_out : mid_key)[to] = k[r];
@@ -778,7 +781,7 @@ struct EmbedPlan {
         const uint64_t bins = 1ull << bits;
         tiles = (uint32_t)((g.rows + kSortTile - 1) / kSortTile);
         lds = (uint32_t)((bins * (1 + kSortWaves) + kSortWaves) * 4);
-        one = tiles <= 1 && bits <= 11; // its keys and places fit beside the counts in 160 KiB
+        one = g.rows <= kSortTile ? bits <= 11 : g.rows <= kSortAlone && bits <= 10; // keys and places fit beside the counts in 160 KiB
         const int size = logit_size_of(g.dtype);
         const uint64_t vecs = ((uint64_t)g.width * size + 15) / 16, stat = size == 8 ? 8 : 4;
         auto take = [&](uint64_t n) {
@@ -801,6 +804,17 @@ template <typename K> hipError_t allow_lds(K *kernel, uint32_t bytes)
 {
     return bytes > 65536 ? hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes)
                          : hipSuccess;
+}
+
+template <int THREADS, int ROUNDS> hipError_t sort_alone(hipStream_t s, const EmbedBackArgs &g, int bits, uint32_t *keys, uint32_t *places)
+{
+    constexpr uint32_t W = THREADS / 64;
+    const uint32_t bins = 1u << bits, lds = (bins * (1 + W) + W + 2 * THREADS * ROUNDS) * 4;
+    const hipError_t e = allow_lds(k_sort_one<THREADS, ROUNDS>, lds);
+    if (e)
+        return e;
+    hipLaunchKernelGGL((k_sort_one<THREADS, ROUNDS>), dim3(1), dim3(THREADS), lds, s, g, bits, keys, places);
+    return hipGetLastError();
 }
 
 template <typename S> hipError_t launch_embed_back_t(hipStream_t s, EmbedBackArgs g, void *scratch, ProgramClose close, bool *closed)
@@ -831,10 +845,9 @@ template <typename S> hipError_t launch_embed_back_t(hipStream_t s, EmbedBackArg
     uint32_t *counts = reinterpret_cast<uint32_t *>(sc + p.counts), *totals = reinterpret_cast<uint32_t *>(sc + p.totals);
     hipError_t e;
     if (p.one) {
-        const uint32_t lds = p.lds + 2 * kSortTile * 4;
-        if ((e = allow_lds(k_sort_one, lds)))
+        if ((e = g.rows <= kSortTile ? sort_alone<kSortThreads, kSortRounds>(s, g, p.bits, keys, places)
+                                     : sort_alone<1024, kSortAlone / 1024>(s, g, p.bits, keys, places)))
             return e;
-        hipLaunchKernelGGL(k_sort_one, dim3(1), dim3(kSortThreads), lds, s, g, p.bits, keys, places);
     } else {
         if ((e = allow_lds(k_sort_move, p.lds)))
             return e;

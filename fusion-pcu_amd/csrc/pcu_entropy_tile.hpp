@@ -177,11 +177,14 @@ template <class Cfg, int ROWS, bool T> struct SlabCarrier {
     static constexpr int K = Cfg::K, IPW = ROWS * K / 512 / Cfg::kWaves, kPieces = (T ? ROWS : K) / 8;
     static constexpr int kHeld = Cfg::kParts == 3 ? 2 : 1; // 16-byte vectors of 8 values
     typedef typename SourceOf<Cfg::kParts>::T Source;
+    static constexpr int kLoads = IPW * kHeld;
     u32x4 held[IPW][kHeld];
+    // Takes kLoads loads, or more where this is true.
+    static __device__ __forceinline__ bool is_ragged(const EntropyOperand &o, uint32_t at, uint32_t k0) { return (T ? at + ROWS : k0 + K) > o.cols; }
     __device__ __forceinline__ void fetch(const EntropyOperand &o, uint32_t at, uint32_t k0, int wave)
     {
         const uint32_t lane = threadIdx.x & 63;
-        const bool ragged = (T ? at + ROWS : k0 + K) > o.cols;
+        const bool ragged = is_ragged(o, at, k0);
 #pragma unroll
         for (int q = 0; q < IPW; q++) {
             const uint32_t r = ((wave * IPW + q) * 64 + lane) / kPieces, piece = lane % kPieces;
@@ -344,7 +347,50 @@ __device__ __forceinline__ void entropy_product(const EntropyOperand &a, const E
                         acc[i][j] = mfma16<E>(fa[kPartA[pair]][i], fb[kPartB[pair]][j], acc[i][j]);
         }
     };
-    if constexpr (Cfg::kStages == 2 || CARRY) {
+    if constexpr (CARRY && Cfg::kParts == 3) {
+        // A's slabs two ahead: one in registers while the next one's loads are under way, too (2 rows, vocabulary
+        // 83776, width 3648 in binary32: one ahead 396 us, 344 so; 16-bit rows, of which more workgroups share a
+        // CU, took 172 us so for 24, 97088 x 3098, 153 below).
+        SlabCarrier<Cfg, Cfg::BM, TA> cb;
+        auto fetch = [&](SlabCarrier<Cfg, Cfg::BM, TA> &c, uint32_t s) __attribute__((always_inline)) {
+            asm volatile("" ::: "memory"); // after B's loads
+            if (k_lo + s < k_hi)
+                c.fetch(a, m0, (k_lo + s) * K, wave);
+            asm volatile("" ::: "memory");
+        };
+        // Slab s + 1, fetched after B's loads of slab s, may stay under way.
+        auto arrive = [&](const SlabCarrier<Cfg, Cfg::BM, TA> &c, int stage, uint32_t s) __attribute__((always_inline)) {
+            c.stash(lds + stage * Cfg::kStage, wave);
+            if (s + 1 < steps && !c.is_ragged(a, m0, (k_lo + s + 1) * K))
+                wait_loads_but<SlabCarrier<Cfg, Cfg::BM, TA>::kLoads>();
+            else
+                wait_lds_loads();
+            __syncthreads();
+        };
+        auto load_b = [&](int stage, uint32_t s) __attribute__((always_inline)) {
+            lb.load(b, n0, (k_lo + s) * K, lds0 + stage * Cfg::kStage + Cfg::kParts * Cfg::kSlabA, wave);
+        };
+        fetch(ca, 0);
+        load_b(0, 0);
+        fetch(cb, 1);
+        arrive(ca, 0, 0);
+        for (uint32_t s = 0; s < steps; s += 2) {
+            if (s + 1 < steps)
+                load_b(1, s + 1);
+            fetch(ca, s + 2);
+            compute(0);
+            if (s + 1 < steps) {
+                arrive(cb, 1, s + 1);
+                if (s + 2 < steps)
+                    load_b(0, s + 2);
+                fetch(cb, s + 3);
+                compute(1);
+                if (s + 2 < steps)
+                    arrive(ca, 0, s + 2);
+            }
+        }
+        __syncthreads();
+    } else if constexpr (Cfg::kStages == 2 || CARRY) {
         auto arrive = [&](int stage) __attribute__((always_inline)) {
             if constexpr (CARRY)
                 ca.stash(lds + stage * Cfg::kStage, wave); // (again what was fetched last, past the last slab)
