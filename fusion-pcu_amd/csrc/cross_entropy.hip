@@ -173,16 +173,16 @@ __device__ __forceinline__ float2 join_sums(float2 a, float2 b)
     return make_float2(m, a.y * exp2_fast((a.x - from) * kLog2e) + b.y * exp2_fast((b.x - from) * kLog2e));
 }
 
-// A row's share k of 16 of its tiles' sums, in order; share 0 joined with the others, in order, is the
-// row's. Both ways that a row's sums are joined go by this.
-template <uint32_t U> __device__ __forceinline__ float2 join_share(const float2 *partial, uint32_t ld, uint32_t tiles, uint32_t n, uint32_t k)
+// A row's share k of SHARES of its tiles' sums, in order; share 0 joined with the others, in order, is the
+// row's. Both ways that a row's sums are joined go by this, with 16 shares for few tiles.
+template <uint32_t U, uint32_t SHARES = 16> __device__ __forceinline__ float2 join_share(const float2 *partial, uint32_t ld, uint32_t tiles, uint32_t n, uint32_t k)
 {
     float2 a = make_float2(-INFINITY, 0.0f);
-    for (uint32_t t = k; t < tiles; t += 16 * U) {
+    for (uint32_t t = k; t < tiles; t += SHARES * U) {
         float2 b[U];
 #pragma unroll
         for (uint32_t q = 0; q < U; q++)
-            b[q] = t + 16 * q < tiles ? partial[(uint64_t)(t + 16 * q) * ld + n] : make_float2(-INFINITY, 0.0f);
+            b[q] = t + SHARES * q < tiles ? partial[(uint64_t)(t + SHARES * q) * ld + n] : make_float2(-INFINITY, 0.0f);
 #pragma unroll
         for (uint32_t q = 0; q < U; q++)
             a = join_sums(a, b[q]);
@@ -346,20 +346,33 @@ template <typename S, class Cfg, bool GRAD, bool CARRY> __global__ __launch_boun
     }
 }
 
-// Each row's log-sum-exp from its tiles', and its loss: 16 rows a workgroup, 16 threads each.
-__global__ __launch_bounds__(256) void k_entropy_loss(const float2 *partial, uint32_t ld, uint32_t tiles, uint32_t rows, RowData row,
-                                                      float *loss, float *log_sum, NodeGate gate, ProgramClose close)
+// Each row's log-sum-exp from its tiles', and its loss: 16 rows a workgroup, SHARES threads each. Of many tiles' sums
+// 64 threads have one trip to memory each (8 rows of 1000 tiles: 11.4 us with 16, 9.5 so).
+constexpr uint32_t kManyTiles = 256;
+template <uint32_t SHARES>
+__global__ __launch_bounds__(16 * SHARES) void k_entropy_loss(const float2 *partial, uint32_t ld, uint32_t tiles, uint32_t rows, RowData row,
+                                                              float *loss, float *log_sum, NodeGate gate, ProgramClose close)
 {
-    __shared__ float2 red[16][16];
+    __shared__ float2 red[SHARES][16];
     if (block_gate_closed(gate))
         return;
     const uint32_t c = threadIdx.x & 15, k = threadIdx.x / 16, n = blockIdx.x * 16 + c;
-    red[k][c] = n < rows ? join_share<16>(partial, ld, tiles, n, k) : make_float2(0.0f, 0.0f);
+    red[k][c] = n < rows ? join_share<16, SHARES>(partial, ld, tiles, n, k) : make_float2(0.0f, 0.0f);
     __syncthreads();
+    if constexpr (SHARES > 16) {
+        // 16 runs of the shares first.
+        if (k < 16) {
+            float2 a = red[k * (SHARES / 16)][c];
+            for (uint32_t q = 1; q < SHARES / 16; q++)
+                a = join_sums(a, red[k * (SHARES / 16) + q][c]);
+            red[k * (SHARES / 16)][c] = a;
+        }
+        __syncthreads();
+    }
     if (k == 0 && n < rows) {
         float2 a = red[0][c];
-        for (int q = 1; q < 16; q++)
-            a = join_sums(a, red[q][c]);
+        for (uint32_t q = 1; q < 16; q++)
+            a = join_sums(a, red[q * (SHARES / 16)][c]);
         const float l = log_of(a);
         row.log_sum[n] = l;
         // Stored past the caches, in case the launch ends its program.
@@ -900,7 +913,11 @@ template <typename S> hipError_t launch_entropy_t(hipStream_t s, const EntropyAr
             const unsigned blocks = (unsigned)((g.rows + 15) / 16);
             const ProgramClose c = !p.grads && blocks <= kCloseMaxBlocks ? close : ProgramClose{};
             *closed = c.words != nullptr;
-            hipLaunchKernelGGL(k_entropy_loss, dim3(blocks), dim3(256), 0, s, l.partial, l.partial_ld, tiles, (uint32_t)g.rows, row,
+            if (tiles > kManyTiles)
+                hipLaunchKernelGGL(k_entropy_loss<64>, dim3(blocks), dim3(1024), 0, s, l.partial, l.partial_ld, tiles, (uint32_t)g.rows, row,
+                               g.loss, g.log_sum_out, g.gate, c);
+            else
+                hipLaunchKernelGGL(k_entropy_loss<16>, dim3(blocks), dim3(256), 0, s, l.partial, l.partial_ld, tiles, (uint32_t)g.rows, row,
                                g.loss, g.log_sum_out, g.gate, c);
             if ((e = hipGetLastError()))
                 return e;
