@@ -636,7 +636,7 @@ inline Side choose_split(uint32_t parts, uint64_t m, uint64_t rows, uint64_t sla
 
 // Binary32 weights that few rows read are split by the tiles' own workgroups, on their way to LDS, where a
 // copy in parts would cost more than it saves: 6 bytes a value written, and read instead of 4 (20 rows, vocabulary 51939,
-// width 896: 388 us of kernels with the copy, 283 so; 128, 121922 x 2083: 2400 and 2180). Tiles of one column each
+// width 896: a step of 388 us of kernels with the copy, 268 so; 128, 121922 x 2083: 2430 and 2140 a call). Tiles of one column each
 // (128 rows) read them once. Small weights are in the caches, and their copy's launch is needed anyway (64, 1000 x 64: 30.7 with, 32.7 so).
 constexpr uint64_t kSplitRows = 128, kSplitBytes = 8ull << 20;
 
