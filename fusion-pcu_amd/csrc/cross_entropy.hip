@@ -731,7 +731,7 @@ template <typename S, class Cfg, bool GRAD, bool CARRY> hipError_t run_logits(hi
 }
 template <typename S, class Cfg, bool GRAD> hipError_t logits_of(bool carry, hipStream_t s, const LogitArgs &a, uint64_t vocab_rows, uint64_t rows)
 {
-    if constexpr (sizeof(S) == 4 || !GRAD)
+    if constexpr (sizeof(S) == 4 ? Cfg::BN > 32 : !GRAD) // (no others are chosen)
         if (carry)
             return run_logits<S, Cfg, GRAD, true>(s, a, vocab_rows, rows);
     return run_logits<S, Cfg, GRAD, false>(s, a, vocab_rows, rows);
@@ -758,7 +758,7 @@ template <typename S, class Cfg> hipError_t run_features(bool carry, hipStream_t
 {
     a.tiles_m = (uint32_t)((width + Cfg::BM - 1) / Cfg::BM);
     a.tiles_n = (uint32_t)((rows + Cfg::BN - 1) / Cfg::BN);
-    if constexpr (sizeof(S) == 4)
+    if constexpr (sizeof(S) == 4 && Cfg::BN > 32)
         if (carry)
             return launch_features<S, Cfg, true>(s, a);
     return launch_features<S, Cfg, false>(s, a);

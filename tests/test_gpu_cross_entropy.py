@@ -153,7 +153,7 @@ def test_several_pieces_of_the_vocabulary(ctx, pcu_pkg, dtype):
 
 
 def test_weights_too_many_to_keep_packed(ctx, pcu_pkg):
-    """Binary32 weights whose parts take more than 512 MiB are split again for every piece."""
+    """Binary32 weights whose parts would take more than 512 MiB, for few rows and in two pieces of the vocabulary."""
     rng = np.random.default_rng(4)
     rows, vocab, width = 9, 262144, 384
     w = rng.standard_normal((vocab, width), np.float32) * np.float32(0.1)
@@ -414,3 +414,84 @@ def test_refusals(ctx, pcu_pkg):
     back = lib.pcu_native_cross_entropy_backward
     assert back(h, R(x.ptr), R(w.ptr, 30), y.ptr, None, None, out.ptr, 8, None, 0, 0, None) == A
     assert not np.any(np.isnan(ctx.native_cross_entropy_loss(ctx.upload(np.ones((4, 8), np.float32)), ctx.upload(np.ones((30, 8), np.float32)), y)[0].numpy()))
+
+
+# Binary32 weights above 8 MiB, split on the way to the tiles for at most 128 rows: every tile, odd widths, one slab and
+# many, several pieces of the vocabulary, rows that start at any binary32 value.
+@pytest.mark.parametrize("rows", [1, 32, 33, 64, 65, 128, 129])
+@pytest.mark.parametrize("vocab,width", [(30001, 131), (2111, 1023), (70001, 33)])
+@pytest.mark.parametrize("lead,more", [(0, 0), (1, 2)])
+def test_large_binary32_weights(ctx, pcu_pkg, rows, vocab, width, lead, more):
+    from fusion_pcu_amd import _abi
+    rng = np.random.default_rng(rows + vocab)
+    xa, xv, wa, wv, labels = _inputs(pcu_pkg, rng, rows, vocab, width, "f32")
+    want = Exact(xv, wv, labels, "f32")
+    x, y = ctx.upload(xa), ctx.upload(labels)
+    loss, log_sum = ctx.empty((rows,), np.float32), ctx.empty((rows,), np.float32)
+    dx, dw = ctx.empty((rows, width), np.float32), ctx.empty((vocab, width), np.float32)
+    stride = width + more
+    host = np.full(lead + vocab * stride, np.nan, np.float32)
+    host[lead:].reshape(vocab, stride)[:, :width] = wa
+    w = ctx.upload(host)
+    xr, wr = _abi.Rows(x.ptr, 0, 0, rows, width, width), _abi.Rows(w.ptr + 4 * lead, 0, 0, vocab, width, stride)
+    assert ctx._lib.pcu_native_cross_entropy_step(ctx.handle, ctypes.byref(xr), ctypes.byref(wr), y.ptr, None, loss.ptr, dx.ptr, width,
+                                                  dw.ptr, vocab, width, None) == 0
+    assert np.all(np.abs(loss.numpy() - want.loss) <= want.d_loss)
+    _near(dx.numpy().astype(np.float64), want.dx, want.d_dx, "f32", "dx")
+    _near(dw.numpy().astype(np.float64), want.dw, want.d_dw, "f32", "dw")
+    assert ctx._lib.pcu_native_cross_entropy_loss(ctx.handle, ctypes.byref(xr), ctypes.byref(wr), y.ptr, loss.ptr, log_sum.ptr, None) == 0
+    assert np.all(np.abs(loss.numpy() - want.loss) <= want.d_loss) and np.all(np.abs(log_sum.numpy() - want.log_sum) <= want.d_log_sum)
+
+
+def test_few_rows_and_several_pieces(ctx, pcu_pkg):
+    rng = np.random.default_rng(8)
+    xa, xv, wa, wv, labels = _inputs(pcu_pkg, rng, 5, 140001, 17, "f32")
+    want = Exact(xv, wv, labels, "f32")
+    loss, dx, dw = ctx.native_cross_entropy_step(ctx.upload(xa), ctx.upload(wa), ctx.upload(labels))
+    assert np.all(np.abs(loss.numpy() - want.loss) <= want.d_loss)
+    _near(dx.numpy().astype(np.float64), want.dx, want.d_dx, "f32", "dx")
+    _near(dw.numpy().astype(np.float64), want.dw, want.d_dw, "f32", "dw")
+
+
+def test_binary32_parts_beyond_what_is_kept(ctx):
+    """Weights whose parts take more than 2 GiB are split for every piece of the vocabulary. All but some of the
+    vocabulary's rows are zeros, so that the definition needs those alone and the zeros' number."""
+    rng = np.random.default_rng(6)
+    rows, vocab, width = 130, 1000003, 384
+    at = np.unique(np.concatenate([[0, 255, 256, 131071, 131072, 931839, 931840, vocab - 1], rng.integers(0, vocab, 500)]))
+    some = (0.1 * rng.standard_normal((len(at), width))).astype(np.float32)
+    weights = np.zeros((vocab, width), np.float32)
+    weights[at] = some
+    x = rng.standard_normal((rows, width)).astype(np.float32)
+    which = rng.integers(0, len(at), rows)
+    labels = at[which].astype(np.int32)
+    labels[3] = -1
+    has = labels >= 0
+    xw, sw = x.astype(np.float64), some.astype(np.float64)
+    l = xw @ sw.T
+    log_sum = np.log(np.exp(l).sum(axis=1) + (vocab - len(at)))
+    e = _sum_error("f32", width, np.abs(xw) @ np.abs(sw).T)
+    d_log_sum = e.max(axis=1) + u * (16 * np.abs(l).max(axis=1) + vocab / 16 + 128)
+    r = np.arange(rows)
+    loss = np.where(has, log_sum - l[r, which], 0)
+    d_loss = np.where(has, d_log_sum + e[r, which] + u * np.abs(loss), 0)
+    g = np.exp(l - log_sum[:, None])
+    d = g * np.expm1(e + d_log_sum[:, None] + u * (8 * np.abs(l) + 8))
+    g[r, which] -= 1
+    d = np.where(has[:, None], d + 3 * u * (np.abs(g) + d), 0)
+    g = np.where(has[:, None], g, 0)
+    zero = np.where(has, np.exp(-log_sum), 0)[:, None]
+    d_zero = zero * (np.expm1(d_log_sum[:, None] + 8 * u) + 4 * u)
+    xd, wd, yd = (ctx.upload(a) for a in (x, weights, labels))
+    got_loss, dx, dw = ctx.native_cross_entropy_step(xd, wd, yd)
+    size = np.abs(g) + d
+    assert np.all(np.abs(got_loss.numpy() - loss) <= d_loss)
+    _near(dx.numpy().astype(np.float64), g @ sw, d @ np.abs(sw) + _sum_error("f32", vocab, size @ np.abs(sw)), "f32", "dx")
+    dw = dw.numpy()
+    _near(dw[at].astype(np.float64), g.T @ xw, d.T @ np.abs(xw) + _sum_error("f32", rows, size.T @ np.abs(xw)), "f32", "dw")
+    others = np.setdiff1d(np.concatenate([np.arange(0, vocab, 997), at + 1, at - 1]), np.concatenate([at, [-1, vocab]]))
+    bound = d_zero.T @ np.abs(xw) + _sum_error("f32", rows, (zero + d_zero).T @ np.abs(xw))
+    _near(dw[others].astype(np.float64), (zero.T @ xw).repeat(len(others), axis=0), bound, "f32", "dw of zeros")
+    loss2, sums = ctx.native_cross_entropy_loss(xd, wd, yd)
+    np.testing.assert_array_equal(_bits(loss2.numpy()), _bits(got_loss.numpy()))
+    assert np.all(np.abs(sums.numpy() - log_sum) <= d_log_sum)
