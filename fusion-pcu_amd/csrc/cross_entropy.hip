@@ -329,7 +329,7 @@ template <typename S, class Cfg, bool GRAD, bool CARRY> __global__ __launch_boun
                         } else {
                             // A part, and what is left for the next ones.
                             float lo = acc[i][j][2 * h], hi = acc[i][j][2 * h + 1];
-                            two[h] = first_part(lo) | first_part(hi) << 16;
+                            two[h] = next_part(lo, part) | next_part(hi, part) << 16;
                             acc[i][j][2 * h] = lo;
                             acc[i][j][2 * h + 1] = hi;
                         }

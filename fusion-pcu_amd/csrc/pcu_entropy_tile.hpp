@@ -44,14 +44,16 @@ constexpr int kSlabK = 64; // operands are padded to whole slabs of the longer k
 constexpr int kPartPairs = 6;
 __device__ constexpr int kPartA[kPartPairs] = {2, 0, 1, 1, 0, 0}, kPartB[kPartPairs] = {0, 2, 1, 0, 1, 0};
 
-// The first 8 bits of a value, as a bfloat16; v becomes the rest. Three of them are the whole value;
-// what is not finite is its first part alone.
-__device__ __forceinline__ uint32_t first_part(float &v)
+// The first 8 bits of a value (of its rest: part 1 and 2), as a bfloat16; v becomes what is left. An infinity is
+// (1, 0, infinity), each with its sign: of the products that are kept, its last part meets the other operand's first
+// part alone, which is zero only if the value is, and its first part gives two infinities their product. (As a first
+// part it would meet the zeros that follow every value of few bits, and their product is NaN.) A NaN is its first part.
+__device__ __forceinline__ uint32_t next_part(float &v, int part)
 {
     const uint32_t b = __float_as_uint(v);
     if ((b & 0x7f800000u) == 0x7f800000u) {
-        v = 0.0f;
-        return (b >> 16) | ((b & 0x7fffffu) ? 0x40u : 0u);
+        const bool nan = b & 0x7fffffu;
+        return part == 0 ? (b >> 16 & 0x8000u) | (nan ? 0x7fc0u : 0x3f80u) : part == 2 && !nan ? b >> 16 : 0u;
     }
     v -= __uint_as_float(b & 0xffff0000u); // exact
     return b >> 16;
@@ -90,7 +92,7 @@ __device__ __forceinline__ void split8(const float (&v)[8], u32x4 (&raw)[3])
         float x = v[e];
 #pragma unroll
         for (int k = 0; k < 3; k++)
-            raw[k][e / 2] |= first_part(x) << (16 * (e & 1));
+            raw[k][e / 2] |= next_part(x, k) << (16 * (e & 1));
     }
 }
 
