@@ -166,10 +166,14 @@ struct LogitArgs {
     NodeGate gate{nullptr, 0};
 };
 
+// What exponentials are taken against, by the largest logit: that, or 0 where it is infinite (inf - inf is no number;
+// against 0 the sum is the definition's, 0 or infinity).
+__device__ __forceinline__ float exp_base(float most) { return fabsf(most) == INFINITY ? 0.0f : most; }
+
 // (maximum, sum of exponentials against it) of two sets of logits together.
 __device__ __forceinline__ float2 join_sums(float2 a, float2 b)
 {
-    const float m = fmaxf(a.x, b.x), from = m == -INFINITY ? 0.0f : m;
+    const float m = fmaxf(a.x, b.x), from = exp_base(m);
     return make_float2(m, a.y * exp2_fast((a.x - from) * kLog2e) + b.y * exp2_fast((b.x - from) * kLog2e));
 }
 
@@ -191,9 +195,8 @@ template <uint32_t U, uint32_t SHARES = 16> __device__ __forceinline__ float2 jo
 }
 __device__ __forceinline__ float log_of(float2 a)
 {
-    const float from = a.x == -INFINITY ? 0.0f : a.x;
     // A NaN among the logits is not in the maximum, but in the sum.
-    return (float)((double)from + (double)__builtin_amdgcn_logf(a.y) * kLn2);
+    return (float)((double)exp_base(a.x) + (double)__builtin_amdgcn_logf(a.y) * kLn2);
 }
 
 // Vocabulary down, rows across: a lane holds 4 SM logits of each of its SN rows.
@@ -269,7 +272,7 @@ template <typename S, class Cfg, bool GRAD, bool CARRY> __global__ __launch_boun
                     m = fmaxf(m, acc[i][j][r]);
             m = fmaxf(m, __shfl_xor(m, 16));
             m = fmaxf(m, __shfl_xor(m, 32));
-            const float from = m == -INFINITY ? 0.0f : m;
+            const float from = exp_base(m);
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < SM; i++)

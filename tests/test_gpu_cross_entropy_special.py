@@ -131,3 +131,46 @@ def test_an_infinite_scale_of_one_row(ctx, pcu_pkg, width, dtype):
                                           row_scale=ctx.upload(np.array([np.inf], np.float32)))[1:]
     want = np.where(np.arange(20)[:, None] == 4, -np.inf, np.inf) * xv
     np.testing.assert_array_equal(_values(pcu_pkg, dw.numpy()), want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,width", [(2, 8, 2), (40, 300, 100), (5, 40001, 70), (129, 1000, 200), (300, 5000, 64)])
+def test_an_infinite_logit(ctx, pcu_pkg, rows, vocab, width, dtype):
+    """An infinite weight: a logit of +inf in rows whose feature is positive, -inf in the others. The first have an
+    infinite log-sum-exp, an infinite loss (NaN if it is the label's), and reach the other tokens' weights through
+    their label alone."""
+    rng = np.random.default_rng(rows + vocab)
+    x, w = rng.normal(0, 1, (rows, width)), rng.normal(0, 1 / np.sqrt(width), (vocab, width))
+    x[:, 1] = rng.choice([1.0, -1.0, 0.3, -0.7], rows)
+    x[0, 1], x[-1, 1] = 1.0, -0.5
+    labels = rng.integers(0, vocab, rows).astype(np.int32)
+    labels[labels == 7] = 6
+    labels[rows // 2] = 7
+    (xa, xv), (_, wv) = _stored(pcu_pkg, x, dtype), _stored(pcu_pkg, w, dtype)
+    wv[7, 1] = np.inf
+    wa, _ = _stored(pcu_pkg, wv, dtype)
+    kept, at = np.arange(vocab) != 7, np.arange(rows)
+    up = xv[:, 1] > 0
+    inner = np.where(np.isinf(wv), 0, wv)
+    l = xv @ inner.T
+    e = _sum_error(dtype, width, np.abs(xv) @ np.abs(inner).T)
+    log_sum = np.where(up, np.inf, np.log(np.exp(l[:, kept]).sum(axis=1)))
+    l[:, 7] = np.where(up, np.inf, -np.inf)
+    d_log_sum = e.max(axis=1) + u * (16 * np.abs(l[:, kept]).max(axis=1) + vocab / 16 + 128)
+    with np.errstate(invalid="ignore"):
+        want = log_sum - l[at, labels]
+        d_want = d_log_sum + e[at, labels] + u * np.abs(want)
+        p = np.exp(l - log_sum[:, None])[:, kept]
+    x, w, y = ctx.upload(xa), ctx.upload(wa), ctx.upload(labels)
+    loss, sums = ctx.native_cross_entropy_loss(x, w, y)
+    _near(sums.numpy().astype(np.float64), log_sum, d_log_sum, "log_sum")
+    _near(loss.numpy().astype(np.float64), want, d_want, "loss")
+    g = p - (np.arange(vocab) == labels[:, None])[:, kept]
+    d = p * np.expm1((e + d_log_sum[:, None])[:, kept] + u * (8 * np.abs(l[:, kept]) + 8))
+    d = d + (U[dtype] + 2 * u) * (np.abs(g) + d) + (2.0 ** -39 if dtype == "f16" else 0.0)
+    dw, d_dw = g.T @ xv, d.T @ np.abs(xv) + _sum_error(dtype, rows, (np.abs(g) + d).T @ np.abs(xv))
+    for got_loss, _, got in (ctx.native_cross_entropy_step(x, w, y), (loss,) + ctx.native_cross_entropy_backward(x, w, y, sums)):
+        _near(got_loss.numpy().astype(np.float64), want, d_want, "loss")
+        got = _values(pcu_pkg, got.numpy())
+        _near(got[kept], dw, d_dw + U[dtype] * (np.abs(dw) + d_dw) + LEAST[dtype], "dw")
+        assert np.all(np.isnan(got[7]))
