@@ -311,6 +311,19 @@ template <typename S, class Cfg, bool GRAD, bool CARRY> __global__ __launch_boun
                     acc[i][j][r] = label >= 0 && !(ragged && v0 + acc_row(i, r) >= g.vocab) ? p * scale : 0.0f;
                 }
         }
+        // Values that need care in parts: any of the wave's.
+        bool special = false;
+        if constexpr (kParts<S> == 3) {
+            uint32_t most = 0;
+#pragma unroll
+            for (int j = 0; j < SN; j++)
+#pragma unroll
+                for (int i = 0; i < SM; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        most = max(most, __float_as_uint(acc[i][j][r]) & 0x7fffffffu);
+            special = __any(most >= kLeastCut);
+        }
         // Through LDS, so that a row's values are stored side by side.
         uint16_t *tile = reinterpret_cast<uint16_t *>(lds);
 #pragma unroll
@@ -332,7 +345,7 @@ template <typename S, class Cfg, bool GRAD, bool CARRY> __global__ __launch_boun
                         } else {
                             // A part, and what is left for the next ones.
                             float lo = acc[i][j][2 * h], hi = acc[i][j][2 * h + 1];
-                            two[h] = next_part(lo, part) | next_part(hi, part) << 16;
+                            two[h] = special ? next_part(lo, part) | next_part(hi, part) << 16 : next_parts(lo, hi, part);
                             acc[i][j][2 * h] = lo;
                             acc[i][j][2 * h + 1] = hi;
                         }

@@ -37,14 +37,20 @@ template <typename E> __device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, 
 
 constexpr int kSlabK = 64; // operands are padded to whole slabs of the longer kind
 
-// Binary32 operands come as three parts of 8 bits, exact together. Of the nine products of two operands'
-// parts the three smallest (below 2^-24 of the whole) are left out; small ones are added first. All
+// Binary32 operands come as three parts of 8 bits, exact together: the value rounded to 8 bits, then its rest. A rest
+// is at most half a step, so the second part is at most 2^-8 of the value and the third 2^-17. Of the nine
+// products of two operands' parts the three smallest are left out: at most 2 * 2^-25 + 2^-34 of the whole together, of
+// either sign (normal values: 0.9 * 2^-24 at most, 0 on average; parts cut off instead of rounded left out up to
+// 8 * 2^-24, always towards zero, 0.7 * 2^-24 on average). Small ones are added first. All
 // parts of a slab lie in LDS at once: 6 products for 3 + 3 parts read. (Parts pair by pair through the
 // 16-bit tiles: 1024 x 50257 x 768 1.93 ms a step, 64 x 1000 x 64 55 us; so 1.73 ms and 40.)
 constexpr int kPartPairs = 6;
 __device__ constexpr int kPartA[kPartPairs] = {2, 0, 1, 1, 0, 0}, kPartB[kPartPairs] = {0, 2, 1, 0, 1, 0};
 
-// The first 8 bits of a value (of its rest: part 1 and 2), as a bfloat16; v becomes what is left. An infinity is
+// From here on 8 bits round to infinity; such a value's first part is cut off instead.
+constexpr uint32_t kLeastCut = 0x7f7f8000u;
+
+// A value rounded to its first 8 bits (of its rest: part 1 and 2), as a bfloat16; v becomes what is left. An infinity is
 // (1, 0, infinity), each with its sign: of the products that are kept, its last part meets the other operand's first
 // part alone, which is zero only if the value is, and its first part gives two infinities their product. (As a first
 // part it would meet the zeros that follow every value of few bits, and their product is NaN.) A NaN is its first part.
@@ -55,44 +61,44 @@ __device__ __forceinline__ uint32_t next_part(float &v, int part)
         const bool nan = b & 0x7fffffu;
         return part == 0 ? (b >> 16 & 0x8000u) | (nan ? 0x7fc0u : 0x3f80u) : part == 2 && !nan ? b >> 16 : 0u;
     }
-    v -= __uint_as_float(b & 0xffff0000u); // exact
-    return b >> 16;
+    const uint32_t to = part < 2 && (b & 0x7fffffffu) < kLeastCut ? b + 0x8000u : b; // (the last rest has 8 bits)
+    v -= __uint_as_float(to & 0xffff0000u); // exact
+    return to >> 16;
+}
+
+// Part `part` of two values below kLeastCut, side by side; they become what is left.
+__device__ __forceinline__ uint32_t next_parts(float &a, float &b, int part)
+{
+    const uint32_t half = part < 2 ? 0x8000u : 0u, lo = __float_as_uint(a) + half, hi = __float_as_uint(b) + half;
+    if (part < 2) { // exact
+        a -= __uint_as_float(lo & 0xffff0000u);
+        b -= __uint_as_float(hi & 0xffff0000u);
+    }
+    return __builtin_amdgcn_perm(hi, lo, 0x07060302u);
 }
 
 // The parts of 8 values.
 __device__ __forceinline__ void split8(const float (&v)[8], u32x4 (&raw)[3])
 {
     uint32_t most = 0;
-#pragma unroll
-    for (int e = 0; e < 8; e++)
-        most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
-    if (most < 0x7f800000u) {
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-            x[e] = v[e];
-#pragma unroll
-        for (int k = 0; k < 3; k++)
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                const uint32_t lo = __float_as_uint(x[e]), hi = __float_as_uint(x[e + 1]);
-                raw[k][e / 2] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
-                if (k < 2) { // exact
-                    x[e] -= __uint_as_float(lo & 0xffff0000u);
-                    x[e + 1] -= __uint_as_float(hi & 0xffff0000u);
-                }
-            }
-        return;
-    }
-#pragma unroll
-    for (int k = 0; k < 3; k++)
-        raw[k] = u32x4{0, 0, 0, 0};
+    float x[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-        float x = v[e];
+        most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
+        x[e] = v[e];
+    }
+    if (most < kLeastCut) {
 #pragma unroll
         for (int k = 0; k < 3; k++)
-            raw[k][e / 2] |= next_part(x, k) << (16 * (e & 1));
+#pragma unroll
+            for (int e = 0; e < 8; e += 2)
+                raw[k][e / 2] = next_parts(x[e], x[e + 1], k);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2)
+                raw[k][e / 2] = next_part(x[e], k) | next_part(x[e + 1], k) << 16;
     }
 }
 
