@@ -872,14 +872,42 @@ template <typename S> hipError_t launch_embed_back_t(hipStream_t s, EmbedBackArg
     return hipGetLastError();
 }
 
+// A gradient of no values: its tokens are looked at all the same.
+__global__ __launch_bounds__(256) void k_token_check(EmbedBackArgs g, ProgramClose close)
+{
+    if (block_gate_closed(g.gate))
+        return;
+    uint64_t key = kNoFault;
+    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < g.rows; i += (uint64_t)gridDim.x * 256) {
+        const int32_t t = g.tokens[i];
+        if (t >= 0 && (uint32_t)t >= g.vocab && key == kNoFault)
+            key = pack_fault(i, kInvalid);
+    }
+    wave_record_fault(key, g.fault, g.gate);
+    program_close_block(close);
+}
+
+hipError_t launch_token_check(hipStream_t s, const EmbedBackArgs &g, ProgramClose close, bool *closed)
+{
+    if (g.rows == 0)
+        return hipSuccess;
+    const uint64_t need = (g.rows + 255) / 256;
+    const unsigned blocks = (unsigned)(need < 2048 ? need : 2048);
+    if (blocks > kCloseMaxBlocks)
+        close = ProgramClose{};
+    *closed = close.words != nullptr;
+    hipLaunchKernelGGL(k_token_check, dim3(blocks), dim3(256), 0, s, g, close);
+    return hipGetLastError();
+}
+
 } // namespace
 
 hipError_t launch_embed(hipStream_t s, const EmbedArgs &g, ProgramClose close, bool *closed)
 {
     *closed = false;
-    if (g.rows == 0 || g.width == 0)
+    if (g.rows == 0)
         return hipSuccess;
-    switch (g.dtype) {
+    switch (g.dtype) { // (rows without columns have tokens to check)
     case kLogitF32: return launch_embed_t<float>(s, g, close, closed);
     case kLogitF64: return launch_embed_t<double>(s, g, close, closed);
     case kLogitBf16: return launch_embed_t<__bf16>(s, g, close, closed);
@@ -893,7 +921,7 @@ hipError_t launch_embed_back(hipStream_t s, const EmbedBackArgs &g, void *scratc
 {
     *closed = false;
     if (g.width == 0 || g.vocab == 0)
-        return hipSuccess;
+        return launch_token_check(s, g, close, closed);
     switch (g.dtype) {
     case kLogitF32: return launch_embed_back_t<float>(s, g, scratch, close, closed);
     case kLogitF64: return launch_embed_back_t<double>(s, g, scratch, close, closed);

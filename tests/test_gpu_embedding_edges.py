@@ -1,0 +1,50 @@
+"""The embedding and its gradient at sizes of nothing, at long batches and long runs of one token, on the GPU. Values are
+whole numbers whose sums every type in question holds exactly, so results have to be equal, bit for bit."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ctx(pcu_pkg):
+    c = pcu_pkg.Context(0)
+    yield c
+    c.close()
+
+
+def _fault(pkg, call):
+    with pytest.raises(pkg.PcuExecutionError) as e:
+        call()
+    return e.value.tensor_fault.element_index
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float64, np.float16])
+@pytest.mark.parametrize("rows", [1, 70, 1500, 100000])
+def test_faults_where_there_is_nothing_to_compute(ctx, pcu_pkg, rows, dtype):
+    """A token at or past the table's rows is a fault where the table has no rows or no columns, too."""
+    tokens = np.full(rows, -1, np.int32)
+    good = ctx.upload(tokens)
+    tokens[[rows // 2, rows - 1]] = 3
+    bad = ctx.upload(tokens)
+    table, none, flat = ctx.empty((3, 0), dtype), ctx.empty((0, 5), dtype), ctx.empty((rows, 0), dtype)
+    gradient = ctx.upload(np.ones((rows, 5), dtype))
+    # No columns: forward and backward.
+    assert ctx.native_embedding(table, good).shape == (rows, 0)
+    assert _fault(pcu_pkg, lambda: ctx.native_embedding(table, bad)) == rows // 2
+    assert ctx.native_embedding_backward(flat, good, 3).shape == (3, 0)
+    assert _fault(pcu_pkg, lambda: ctx.native_embedding_backward(flat, bad, 3)) == rows // 2
+    # No rows, in the table or of its gradient.
+    assert not np.any(ctx.native_embedding(none, good).numpy())
+    assert _fault(pcu_pkg, lambda: ctx.native_embedding(none, bad)) == rows // 2
+    assert ctx.native_embedding_backward(gradient, good, 0).shape == (0, 5)
+    assert _fault(pcu_pkg, lambda: ctx.native_embedding_backward(gradient, bad, 0)) == rows // 2
+    assert ctx.native_embedding_backward(flat, good, 0).shape == (0, 0)
+    # In a program, whose later calls are then left out; and the next call is right.
+    mark = ctx.upload(np.full((3, 5), 7, dtype))
+    with pytest.raises(pcu_pkg.PcuExecutionError):
+        with ctx.program():
+            ctx.native_embedding_backward(flat, bad, 3)
+            ctx.native_embedding_backward(gradient, good, 3, out=mark)
+    assert np.all(mark.numpy() == 7)
+    assert not np.any(ctx.native_embedding_backward(gradient, good, 3, out=mark).numpy())
