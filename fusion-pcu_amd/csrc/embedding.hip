@@ -1,7 +1,7 @@
 // Embedding lookup with scaling, and the table's gradient.
 //
 //   out[i] = scale * table[t_i]                 (a negative token: zeros)
-//   grad[v] = base[v] + scale * (sum of g[i] over the i with t_i = v, i ascending)
+//   grad[v] = base[v] + scale * (sum of g[i] over the i with t_i = v, i ascending, long sums in parts)
 //
 // The gradient sorts the tokens (stable, so a row's terms are added in one order whatever the
 // launch did); then every row of the table is written once, by the lanes that own it: no atomics on
@@ -342,10 +342,9 @@ template <int THREADS, int ROUNDS> __global__ __launch_bounds__(THREADS) void k_
 }
 
 // --------------------------------------------------------------------- summing
-// First of the n sorted keys that is at least v; a wave looks at 64 of them at a time.
-__device__ __forceinline__ uint32_t lower_bound(const uint32_t *keys, uint32_t n, uint32_t v)
+// First of the sorted keys [lo, lo + len) that is at least v; a wave looks at 64 of them at a time.
+__device__ __forceinline__ uint32_t lower_bound(const uint32_t *keys, uint32_t lo, uint32_t len, uint32_t v)
 {
-    uint32_t lo = 0, len = n;
     while (len > 0) {
         const uint32_t step = (len + 63) / 64, at = (threadIdx.x & 63) * step;
         const uint32_t below = (uint32_t)__popcll(__ballot(at < len && keys[lo + min(at, len - 1)] < v));
@@ -359,8 +358,8 @@ __device__ __forceinline__ uint32_t lower_bound(const uint32_t *keys, uint32_t n
 }
 
 // A wave takes the rows whose first term is one of kStarts sorted ones. Rows of more than kLong terms
-// are added up by several waves, kLong terms each (a part, aligned in the sorted order), whose sums are
-// added in order afterwards. The other rows that begin in a wave's share end within its 64 lanes.
+// are added up by several waves, kLong terms each from the row's first on (a part; which other tokens there are makes
+// no difference to a row's sum), whose sums are added in order afterwards. The other rows that begin in a wave's share end within its 64 lanes.
 constexpr uint32_t kStarts = 16, kLong = 48;
 static_assert(kStarts - 1 + kLong < 64, "a short row's end is in sight");
 
@@ -515,8 +514,8 @@ __device__ __forceinline__ void fill_rows(const EmbedBackArgs &g, const uint32_t
         occurs[w] = 0;
     __syncthreads();
     // The rows that occur, from the sorted keys or (few tokens) from all of them.
-    const uint32_t first = keys ? lower_bound(keys, n, row0) : 0;
-    const uint32_t last = keys ? lower_bound(keys, n, min((uint32_t)((hi - 1) / vecs) + 1, g.vocab)) : n;
+    const uint32_t first = keys ? lower_bound(keys, 0, n, row0) : 0;
+    const uint32_t last = keys ? lower_bound(keys, 0, n, min((uint32_t)((hi - 1) / vecs) + 1, g.vocab)) : n;
     for (uint32_t i = first + threadIdx.x; i < last; i += 256) {
         const uint32_t t = keys ? keys[i] : (uint32_t)g.tokens[i]; // an absent one is no row's
         if (t - row0 < kFillRows)
@@ -636,11 +635,12 @@ __global__ __launch_bounds__(256) void k_embed_first(EmbedBackArgs g, uint32_t a
     program_close_block(close);
 }
 
-// A part's rows at its ends: how many of its terms are its first key's and its last key's, and how many
-// terms more those keys have right before and behind the part (64 for 64 or more).
-struct Part {
+// The rows at the ends of a window of kLong sorted terms: how many of these are its first key's and its last key's, and how
+// many terms more those keys have right before and behind the window (64 for 64 or more). At most two long rows have a part
+// that begins in a window: its first key's, unless the row ends before, and its last key's.
+struct Window {
     uint32_t lo, hi, first, last, head, tail, before, behind;
-    __device__ __forceinline__ Part(const uint32_t *keys, uint32_t n, uint32_t c)
+    __device__ __forceinline__ Window(const uint32_t *keys, uint32_t n, uint32_t c)
     {
         const uint32_t lane = threadIdx.x & 63;
         lo = c * kLong;
@@ -687,8 +687,9 @@ __device__ __forceinline__ void leave_part(const EmbedBackArgs &g, const uint32_
 }
 
 // Workgroups [0, runs): waves with the rows that begin in their terms; [runs, parts): waves that leave the
-// sums of long rows' parts, part c with its first row's sum at 2 c and its last row's at 2 c + 1; the
-// others fill the rows that do not occur. A wave takes 64 vectors of the rows, of `across`.
+// sums of the long rows' parts that begin in window c, its first row's in slot 2 c and its last row's in 2 c + 1, a
+// wave each (2560 tokens, 111 x 384: a call of 53 us with one wave for both, 44 so); the others fill the rows that do not
+// occur. A wave takes 64 vectors of the rows, of `across`.
 template <typename S, bool BASE>
 __global__ __launch_bounds__(256) void k_embed_sum(EmbedBackArgs g, const uint32_t *keys, const uint32_t *places, int lanes,
                                                    uint32_t across, uint32_t runs, uint32_t parts, uint64_t each, void *sums)
@@ -702,24 +703,33 @@ __global__ __launch_bounds__(256) void k_embed_sum(EmbedBackArgs g, const uint32
     }
     const uint32_t n = (uint32_t)g.rows, vecs = (g.width + kVec<S> - 1) / kVec<S>, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const bool of_runs = blockIdx.x < runs;
-    const uint32_t unit = (blockIdx.x - (of_runs ? 0 : runs)) * 4 + wave, c = unit / across;
+    const uint32_t unit = (blockIdx.x - (of_runs ? 0 : runs)) * 4 + wave, slot = unit / across;
     const uint32_t vec = unit % across * 64 + (threadIdx.x & (lanes - 1));
     if (of_runs) {
-        if (c * kStarts < n)
-            sum_runs<S, BASE>(g, keys, places, c, lanes, vec, vec < vecs);
+        if (slot * kStarts < n)
+            sum_runs<S, BASE>(g, keys, places, slot, lanes, vec, vec < vecs);
         return;
     }
+    const uint32_t c = slot / 2;
     if (c * kLong >= n)
         return;
-    const Part p(keys, n, c);
-    T *out = static_cast<T *>(sums) + ((uint64_t)2 * c * vecs + vec) * kVec<S>;
-    if (p.first < g.vocab && p.head_long())
-        leave_part<S>(g, places, p.lo, p.lo + p.head, lanes, vec, vec < vecs, out);
-    if (p.last != p.first && p.last < g.vocab && p.tail_long())
-        leave_part<S>(g, places, p.hi - p.tail, p.hi, lanes, vec, vec < vecs, out + (uint64_t)vecs * kVec<S>);
+    const Window p(keys, n, c);
+    uint32_t at = n, end = n;
+    if (slot & 1) {
+        if (p.last != p.first && p.last < g.vocab && p.tail_long()) {
+            at = p.hi - p.tail;
+            end = at + kLong;
+        }
+    } else if (p.first < g.vocab && p.head_long()) {
+        const uint32_t start = p.before < 64 ? p.lo - p.before : lower_bound(keys, 0, p.lo, p.first); // of the row
+        at = start + (p.lo - start + kLong - 1) / kLong * kLong;
+        end = min(at + kLong, p.lo + p.head + (p.lo + p.head == p.hi ? p.behind : 0));
+    }
+    if (at < end)
+        leave_part<S>(g, places, at, end, lanes, vec, vec < vecs, static_cast<T *>(sums) + ((uint64_t)slot * vecs + vec) * kVec<S>);
 }
 
-// The long rows, each by the part in which it begins.
+// The long rows, each by the window in which it begins.
 template <typename S>
 __global__ __launch_bounds__(256) void k_embed_join(EmbedBackArgs g, const uint32_t *keys, int lanes, uint32_t across, const void *sums)
 {
@@ -731,15 +741,15 @@ __global__ __launch_bounds__(256) void k_embed_join(EmbedBackArgs g, const uint3
     const uint32_t c = unit / across, vec = unit % across * 64 + (threadIdx.x & 63);
     if (c * kLong >= n)
         return;
-    const Part p(keys, n, c);
+    const Window p(keys, n, c);
     if (p.last >= g.vocab || !p.tail_long() || (p.tail == p.hi - p.lo && p.before > 0))
         return;
-    const uint32_t end = p.behind < 64 ? p.hi + p.behind : lower_bound(keys, n, p.last + 1);
+    const uint32_t end = p.behind < 64 ? p.hi + p.behind : lower_bound(keys, p.hi, n - p.hi, p.last + 1);
     if (vec >= vecs || (threadIdx.x & 63) >= (uint32_t)lanes)
         return;
     const T *from = static_cast<const T *>(sums) + (uint64_t)vec * V;
     const uint64_t part = (uint64_t)vecs * V;
-    const uint32_t more = (end - 1) / kLong - c; // parts after this one
+    const uint32_t more = (end - (p.hi - p.tail) - 1) / kLong; // parts after the first, one a window
     T sum[V];
 #pragma unroll
     for (int e = 0; e < V; e++)
@@ -862,13 +872,14 @@ template <typename S> hipError_t launch_embed_back_t(hipStream_t s, EmbedBackArg
         }
     }
     const uint32_t runs = (uint32_t)(((g.rows + kStarts - 1) / kStarts * across + 3) / 4);
-    const uint32_t parts = (uint32_t)(((g.rows + kLong - 1) / kLong * across + 3) / 4);
+    const uint64_t windows = (g.rows + kLong - 1) / kLong;
+    const uint32_t parts = (uint32_t)((windows * 2 * across + 3) / 4), joins = (uint32_t)((windows * across + 3) / 4);
     const dim3 grid(runs + parts + (uint32_t)fill);
     if (g.base)
         hipLaunchKernelGGL((k_embed_sum<S, true>), grid, dim3(256), 0, s, g, keys, places, lanes, across, runs, runs + parts, each, sc + p.parts);
     else
         hipLaunchKernelGGL((k_embed_sum<S, false>), grid, dim3(256), 0, s, g, keys, places, lanes, across, runs, runs + parts, each, sc + p.parts);
-    hipLaunchKernelGGL((k_embed_join<S>), dim3(parts), dim3(256), 0, s, g, keys, lanes, across, sc + p.parts);
+    hipLaunchKernelGGL((k_embed_join<S>), dim3(joins), dim3(256), 0, s, g, keys, lanes, across, sc + p.parts);
     return hipGetLastError();
 }
 

@@ -345,9 +345,10 @@ pcu_status pcu_native_sample(pcu_ctx *ctx, const pcu_logits *logits, const pcu_s
  * No counterpart in the reference: what a language model does before and behind its products.
  * Native arithmetic (non-finite results are ordinary values), each call one program node. A
  * pointer that is not aligned to its type is refused. Sums and statistics are F32, F64 for F64
- * rows, and are added in an order that the sizes alone determine; results are rounded once to
- * their type. `fault` reports a token or label that is out of its range as PCU_FAULT_INVALID with the
- * lowest such element; what the call's outputs then hold is unspecified. */
+ * rows, and are added in an order that the sizes alone determine (a row of a table's gradient: the
+ * sizes and how often its token occurs); results are rounded once to their type. `fault` reports a
+ * token or label that is out of its range as PCU_FAULT_INVALID with the lowest such element; what the
+ * call's outputs then hold is unspecified. */
 
 /* `rows` rows of `cols` values of any dtype; row r starts at element r * stride
  * (stride >= cols: the columns between belong to the caller). Any alignment of the type. */
@@ -367,8 +368,9 @@ pcu_status pcu_native_embedding(pcu_ctx *ctx, const pcu_rows *table, const int32
                                 uint64_t count, double scale, void *out, uint64_t out_stride,
                                 pcu_fault *fault);
 /* The gradient by the table: out[v] = base[v] + scale * (the sum of gradient[i] over the i with
- * tokens[i] = v, in their order) for each of table_rows rows; base may be NULL (zeros) or out itself
- * (same stride: rows whose token does not occur keep their bits and are not touched), else it overlaps nothing that is written.
+ * tokens[i] = v, in their order, a long sum in parts that are added in order) for each of table_rows
+ * rows; base may be NULL (zeros) or out itself (same stride: rows whose token does not occur keep
+ * their bits and are not touched), else it overlaps nothing that is written.
  * Negative tokens are left out; one of table_rows or more is a fault. At most 2^28 rows of 1 KiB
  * (or less) each, or as much in longer ones. */
 pcu_status pcu_native_embedding_backward(pcu_ctx *ctx, const pcu_rows *gradient,

@@ -1,5 +1,5 @@
-"""The embedding and its gradient at sizes of nothing, at long batches and long runs of one token, on the GPU. Values are
-whole numbers whose sums every type in question holds exactly, so results have to be equal, bit for bit."""
+"""The embedding and its gradient at sizes of nothing, at long batches and long runs of one token, on the GPU. Results have
+to be equal, bit for bit: values are whole numbers whose sums the type holds exactly, or two calls' sums are of the same terms."""
 import numpy as np
 import pytest
 
@@ -48,3 +48,27 @@ def test_faults_where_there_is_nothing_to_compute(ctx, pcu_pkg, rows, dtype):
             ctx.native_embedding_backward(gradient, good, 3, out=mark)
     assert np.all(mark.numpy() == 7)
     assert not np.any(ctx.native_embedding_backward(gradient, good, 3, out=mark).numpy())
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float64, np.float16])
+@pytest.mark.parametrize("width", [1, 5, 64, 300])
+@pytest.mark.parametrize("times", [3, 48, 49, 95, 96, 97, 145, 1000])
+def test_a_tokens_sum_does_not_depend_on_the_other_tokens(ctx, times, width, dtype):
+    """Its terms in their order, wherever other tokens push them in the sorted order, and whatever these are."""
+    rng = np.random.default_rng(times + width)
+    rows, vocab, token = 2500, 400, 200
+    terms = rng.normal(0, 1, (times, width)).astype(dtype)
+    first = None
+    for less in (0, 1, 7, 47, 48, 50, 333, 1499):
+        others = np.concatenate([rng.choice([3, token - 1], less), rng.integers(token + 1, vocab, rows - times - less)]).astype(np.int32)
+        tokens, gradient = np.empty(rows, np.int32), rng.normal(0, 1, (rows, width)).astype(dtype)
+        place = np.sort(rng.permutation(rows)[:times])
+        rest = np.setdiff1d(np.arange(rows), place)
+        tokens[place], tokens[rest], gradient[place] = token, rng.permutation(others), terms
+        got = ctx.native_embedding_backward(ctx.upload(gradient), ctx.upload(tokens), vocab).numpy()[token]
+        first = got if first is None else first
+        np.testing.assert_array_equal(got, first)
+    u, size = {2: 2.0 ** -11, 4: 2.0 ** -24, 8: 2.0 ** -53}[first.itemsize], np.abs(terms.astype(np.float64)).sum(axis=0)
+    acc = 2.0 ** -53 if dtype == np.float64 else 2.0 ** -24
+    exact = terms.astype(np.longdouble).sum(axis=0)
+    assert np.all(np.abs(first - exact) <= acc * times * size + u * (np.abs(exact) + acc * times * size))
