@@ -72,3 +72,23 @@ def test_a_tokens_sum_does_not_depend_on_the_other_tokens(ctx, times, width, dty
     acc = 2.0 ** -53 if dtype == np.float64 else 2.0 ** -24
     exact = terms.astype(np.longdouble).sum(axis=0)
     assert np.all(np.abs(first - exact) <= acc * times * size + u * (np.abs(exact) + acc * times * size))
+
+
+@pytest.mark.parametrize("vocab", [5, 3000, 1 << 17, 1 << 22])
+@pytest.mark.parametrize("rows", [65536, 65537, 70001, 512 * 2048, 512 * 2048 + 1, 1100003])
+@pytest.mark.parametrize("width,base", [(1, False), (3, True)])
+def test_long_batches(ctx, rows, vocab, width, base):
+    """More than 32 tiles of 2048 tokens, whose counts are summed by launches of their own, and more than 512 tiles, which
+    one workgroup's pass over them does not reach."""
+    rng = np.random.default_rng(rows + vocab + width)
+    tokens = (vocab * rng.random(rows) ** 3).astype(np.int32)  # some far more often than others
+    tokens[rng.random(rows) < 0.1] = -1
+    tokens[[0, rows - 1]] = vocab - 1
+    gradient = rng.integers(-3, 4, (rows, width)).astype(np.float32)
+    start = rng.integers(-9, 9, (vocab, width)).astype(np.float32)
+    want = start.astype(np.float64) if base else np.zeros((vocab, width))
+    for c in range(width):
+        real = tokens >= 0
+        want[:, c] += np.bincount(tokens[real], weights=gradient[real, c], minlength=vocab)
+    got = ctx.native_embedding_backward(ctx.upload(gradient), ctx.upload(tokens), vocab, base=ctx.upload(start) if base else None)
+    np.testing.assert_array_equal(got.numpy(), want)
