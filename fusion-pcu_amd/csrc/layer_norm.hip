@@ -372,7 +372,7 @@ __global__ __launch_bounds__(NT) void k_norm_back(NormBackArgs g, void *parts)
     }
 }
 
-// Rows too long to hold: the two sums of each row first (one workgroup a row), then dx and the
+// Rows too long to hold: for dx the two sums of each row first (one workgroup a row), then dx and (SUMS) the
 // columns' sums by pieces of 1024 vectors and runs of rows.
 template <typename S, typename W> __global__ __launch_bounds__(1024) void k_norm_back_sums(NormBackArgs g, void *sums)
 {
@@ -412,7 +412,7 @@ template <typename S, typename W> __global__ __launch_bounds__(1024) void k_norm
     }
 }
 
-template <typename S, typename W>
+template <typename S, typename W, bool SUMS>
 __global__ __launch_bounds__(1024) void k_norm_back_wide(NormBackArgs g, const void *sums, void *parts)
 {
     using T = typename StatOf<S>::T;
@@ -431,22 +431,26 @@ __global__ __launch_bounds__(1024) void k_norm_back_wide(NormBackArgs g, const v
         T x[V], d[V];
         unpack<S>(load_piece(static_cast<const S *>(g.x) + r * g.stride, i, n), x);
         unpack<S>(load_piece(static_cast<const S *>(g.gradient) + r * g.gradient_stride, i, n), d);
-        const T c0 = static_cast<const T *>(sums)[2 * r], c1 = static_cast<const T *>(sums)[2 * r + 1];
+        const T c0 = g.x_gradient ? static_cast<const T *>(sums)[2 * r] : (T)0, c1 = g.x_gradient ? static_cast<const T *>(sums)[2 * r + 1] : (T)0;
 #pragma unroll
         for (int e = 0; e < V; e++) {
             const T near = (x[e] - mean) * rstd;
-            dw[e] += d[e] * near;
-            db[e] += d[e];
+            if constexpr (SUMS) {
+                dw[e] += d[e] * near;
+                db[e] += d[e];
+            }
             x[e] = rstd * ((w ? d[e] * ws[e] : d[e]) - c0 - near * c1);
         }
         if (g.x_gradient)
             store_vec(static_cast<S *>(g.x_gradient) + r * g.x_gradient_stride, i, n, x, false);
     }
-    T *part = static_cast<T *>(parts) + (uint64_t)blockIdx.x * 2 * vecs * V + i * V;
+    if constexpr (SUMS) {
+        T *part = static_cast<T *>(parts) + (uint64_t)blockIdx.x * 2 * vecs * V + i * V;
 #pragma unroll
-    for (int e = 0; e < V; e++) {
-        part[e] = dw[e];
-        part[vecs * V + e] = db[e];
+        for (int e = 0; e < V; e++) {
+            part[e] = dw[e];
+            part[vecs * V + e] = db[e];
+        }
     }
 }
 
@@ -518,8 +522,8 @@ struct NormBackPlan {
         const uint64_t groups = lanes ? threads / lanes : 1, most = threads == 256 ? 512 : kGfx950Cus;
         const uint64_t need = (g.rows + groups - 1) / groups;
         grid = (uint32_t)(need < most ? need : most);
-        parts = lanes ? 0 : (g.rows * 2 * stat + 255) / 256 * 256;
-        bytes = parts + (want || !lanes ? (uint64_t)grid * 2 * vecs * v * stat : 0);
+        parts = lanes || !g.x_gradient ? 0 : (g.rows * 2 * stat + 255) / 256 * 256;
+        bytes = parts + (want ? (uint64_t)grid * 2 * vecs * v * stat : 0);
     }
 };
 
@@ -557,10 +561,17 @@ hipError_t launch_norm_back_t(hipStream_t s, const NormBackArgs &g, void *scratc
     char *sc = static_cast<char *>(scratch);
     const bool want = g.weight_gradient || g.bias_gradient;
     const uint32_t vecs = (g.width + kVec<S> - 1) / kVec<S>;
+    if (!want && !g.x_gradient)
+        return hipSuccess;
     if (p.grid) {
         if (p.lanes == 0) {
-            hipLaunchKernelGGL((k_norm_back_sums<S, W>), row_grid(g.rows), dim3(1024), 0, s, g, sc + p.sums);
-            hipLaunchKernelGGL((k_norm_back_wide<S, W>), dim3(p.grid, (vecs + 1023) / 1024), dim3(1024), 0, s, g, sc + p.sums, sc + p.parts);
+            const dim3 grid(p.grid, (vecs + 1023) / 1024);
+            if (g.x_gradient)
+                hipLaunchKernelGGL((k_norm_back_sums<S, W>), row_grid(g.rows), dim3(1024), 0, s, g, sc + p.sums);
+            if (want)
+                hipLaunchKernelGGL((k_norm_back_wide<S, W, true>), grid, dim3(1024), 0, s, g, sc + p.sums, sc + p.parts);
+            else
+                hipLaunchKernelGGL((k_norm_back_wide<S, W, false>), grid, dim3(1024), 0, s, g, sc + p.sums, nullptr);
         } else if (p.threads == 256) {
             launch_norm_narrow<S, W, 256>(s, g, p, sc, want);
         } else if (p.lanes <= 256) {
