@@ -1,5 +1,5 @@
 """Layer norm's gradients of rows too long to hold in registers, each of them alone, on the GPU: the bits of the call that
-computes all, and no more scratch than they need."""
+computes all, and no more scratch than they need. And the statistics of rows without columns."""
 import ctypes
 
 import numpy as np
@@ -53,3 +53,12 @@ def test_the_rows_gradient_alone_takes_no_columns_sums(pcu_pkg):
         assert _pool_bytes() - before < 1 << 20
         c.native_layer_norm_backward(x, stats, dy, x_gradient=dx, weight_gradient=c.empty((width,), np.float64))
         assert _pool_bytes() - before >= 512 << 20
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float64, np.float16])
+@pytest.mark.parametrize("rows", [1, 3000])
+def test_statistics_of_no_columns(ctx, rows, dtype):
+    """The mean of nothing is 0 / 0."""
+    stats = ctx.upload(np.full((rows, 2), 3, np.float64 if dtype == np.float64 else np.float32))
+    out, _ = ctx.native_layer_norm(ctx.empty((rows, 0), dtype), stats=stats)
+    assert out.shape == (rows, 0) and np.all(np.isnan(stats.numpy()))
