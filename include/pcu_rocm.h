@@ -405,8 +405,10 @@ pcu_status pcu_native_layer_norm_backward(pcu_ctx *ctx, const pcu_rows *x, const
  *   feature_gradient = G * weights, weight_gradient = G^T * features
  * A row with a negative label has loss 0 and reaches no gradient, whatever its features hold; one of
  * weights.rows or more is a fault (element_index: the row). loss, log_sum and row_scale (NULL: 1)
- * are F32. Sums are F32; F32 operands enter with 24 bits; G is rounded to the operands' precision, which
- * for F16 holds what is above 2^-38 of the largest row_scale. */
+ * are F32. Sums are F32; F32 operands enter with 24 bits, of which what is below 2^-133 is dropped; G is
+ * rounded to the operands' precision, which for F16 holds what is above 2^-38 of the largest row_scale.
+ * Infinite operands give the products and sums that they have in the formulas: a weight of -inf against a
+ * positive feature masks its token (and 0 * inf makes that weight's column of feature_gradient NaN). */
 #define PCU_ENTROPY_MAX_ROWS (1u << 22) /* and the product of any two of the three sizes at most 2^37 */
 #define PCU_ENTROPY_MAX_WIDTH (1u << 16) /* and at least 1 */
 /* log_sum may be NULL. */
